@@ -1,0 +1,507 @@
+// RMS norms of the queries and keys of each head with the position rotation,
+// and their gradients (the norm weights' per sample).
+//
+// One row is a head's D entries at one token, x; w the side's weight, p the
+// token's position, f_i the rotation's inverse frequencies (i < R/2, R <= D):
+//
+//   r = (mean(x^2) + eps)^(-1/2),  y = x r w
+//   z_a = s (y_a cos(p f_i) - y_b sin(p f_i)),  z_b = s (y_b cos(p f_i) + y_a sin(p f_i))
+//   z = y past R
+//
+// for the pairs (a, b) = (i, i + R/2), or (2i, 2i+1) interleaved.  Backward,
+// with dz given: dy = the pairs turned back (times s), g = dy w,
+//
+//   dx = r (g - x r^2 mean(g x)),  dw[b] = sum over tokens and heads of dy x r.
+//
+// The angle is position times frequency in fp64, reduced to its fraction of a
+// turn there (a position of 10^6 leaves 10^-10 of a turn), and only then fp32:
+// fp32 products would lose the angles of far positions.
+//
+// A row's pairs lie in slots of V; a group of kL lanes owns a head, lane l its
+// slots l, l + kL, ..., and a wave 64 / kL heads of one token at a time, so that
+// one token's angles serve all the heads its wave visits.  Both members of a
+// pair are in one lane: the rotation needs no exchange, and a row's two sums
+// (x^2; and g x in the backward pass) are one butterfly over the kL lanes.
+#include "common.h"
+
+namespace da {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kWaves = kThreads / kWave;
+constexpr int64_t kMaxD = 1024;
+
+struct Rows {  // one side's rows; strides in bytes
+  const char* x;
+  const char* gz;
+  char* out;
+  const void* w;
+  float* wgrad;    // (batch, D), NULL: not wanted
+  float* partial;  // (batch, chunks, D)
+  int64_t heads;
+  int64_t x_b, x_t, x_h, g_b, g_t, g_h, o_b, o_t, o_h;
+};
+
+struct QkArgs {
+  Rows side[2];
+  int64_t batch, tokens;
+  int d, rot, w_dtype;
+  const float* inv_freq;
+  const void* pos;  // NULL: the token's index
+  int pos_bytes;
+  int64_t pos_b, pos_t;  // elements
+  const uint8_t* mask;   // NULL: every token lives
+  int64_t mask_b, mask_t;
+  float scaling, eps;
+  int parts;            // forward: waves that share a token's heads
+  int64_t chunk;        // backward: tokens of a workgroup
+  int64_t chunks;       // backward: workgroups of a sample
+};
+
+__device__ __forceinline__ float load_any(const void* p, int dt, int64_t i) {
+  if (dt == DA_F32) return ((const float*)p)[i];
+  const uint32_t h = ((const uint16_t*)p)[i];
+  return dt == DA_BF16 ? bf16_bits_to_f32(h) : f16_bits_to_f32(h);
+}
+
+// Where a slot's two runs of V entries start, and what of them exists.
+template <int V, bool kInter>
+struct Slot {
+  int a, b;       // first entry of each run; interleaved: the runs follow one another
+  bool in, turn;  // the slot holds entries; they rotate
+  bool has_b;     // V == 1 only: the second entry exists (odd remainders)
+  __device__ void at(int s, int d, int rot) {
+    if constexpr (kInter) {
+      a = 2 * s * V;
+      b = a + V;
+      turn = a < rot;
+    } else {
+      const int half = rot / 2, p = s * V;
+      turn = p < half;
+      const int rest = (d - rot + 1) / 2, q = p - half;
+      a = turn ? p : (q < rest ? rot + q : d);
+      b = turn ? half + p : rot + rest + q;
+    }
+    in = a < d;
+    has_b = b < d;
+  }
+};
+
+template <int DT, int V>
+struct Run {  // V entries as they lie in memory
+  uint32_t bits[V];
+  __device__ void load(const char* p, bool in) {
+    static_assert(V == 1);
+    if constexpr (DT == DA_F32) bits[0] = in ? *(const uint32_t*)p : 0u;
+    else bits[0] = in ? *(const uint16_t*)p : 0u;
+  }
+  __device__ float get(int i) const { return Elem<DT>::from_bits(bits[i]); }
+  __device__ static void store(char* p, const float* v, bool in) {
+    static_assert(V == 1);
+    if (in) Elem<DT>::store(p, 0, v[0]);
+  }
+};
+
+// The lane's pairs of one row: fp32 values, first and second members.  Run
+// order to pair order: interleaved runs hold both members alternately.
+template <int DT, int V, int S, bool kInter>
+struct Row {
+  float a[S][V], b[S][V];
+  __device__ void load(const char* p, const Slot<V, kInter>* slots, bool live) {
+    constexpr int ES = Elem<DT>::kBytes;
+#pragma unroll
+    for (int i = 0; i < S; ++i) {
+      Run<DT, V> u, v;
+      u.load(p + (int64_t)slots[i].a * ES, live && slots[i].in);
+      v.load(p + (int64_t)slots[i].b * ES, live && slots[i].in && slots[i].has_b);
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const int ea = kInter ? 2 * e : e, eb = kInter ? 2 * e + 1 : V + e;
+        a[i][e] = ea < V ? u.get(ea) : v.get(ea - V);
+        b[i][e] = eb < V ? u.get(eb) : v.get(eb - V);
+      }
+    }
+  }
+  __device__ void store(char* p, const Slot<V, kInter>* slots, bool live) const {
+    constexpr int ES = Elem<DT>::kBytes;
+#pragma unroll
+    for (int i = 0; i < S; ++i) {
+      float u[V], v[V];
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const int ea = kInter ? 2 * e : e, eb = kInter ? 2 * e + 1 : V + e;
+        (ea < V ? u[ea < V ? ea : 0] : v[ea >= V ? ea - V : 0]) = a[i][e];
+        (eb < V ? u[eb < V ? eb : 0] : v[eb >= V ? eb - V : 0]) = b[i][e];
+      }
+      Run<DT, V>::store(p + (int64_t)slots[i].a * ES, u, live && slots[i].in);
+      Run<DT, V>::store(p + (int64_t)slots[i].b * ES, v, live && slots[i].in && slots[i].has_b);
+    }
+  }
+};
+
+__device__ __forceinline__ void turn_of(const QkArgs& a, double pos, int pair, float* c, float* s) {
+  const double turns = pos * ((double)a.inv_freq[pair] * 0.15915494309189535);  // 1 / (2 pi)
+  const float part = (float)(2.0 * (turns - rint(turns)));                      // half turns, [-1, 1]
+  float sn, cs;
+  sincospif(part, &sn, &cs);
+  *c = cs * a.scaling;
+  *s = sn * a.scaling;
+}
+
+template <int V, int S, bool kInter>
+__device__ __forceinline__ void angles(const QkArgs& a, int64_t b, int64_t t, const Slot<V, kInter>* slots,
+                                       int first_slot, int step, float (&c)[S][V], float (&s)[S][V]) {
+  double pos = (double)t;
+  if (a.pos) {
+    const int64_t at = b * a.pos_b + t * a.pos_t;
+    pos = a.pos_bytes == 8 ? (double)((const int64_t*)a.pos)[at] : (double)((const int32_t*)a.pos)[at];
+  }
+#pragma unroll
+  for (int i = 0; i < S; ++i)
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      c[i][e] = 1.f;
+      s[i][e] = 0.f;
+      if (slots[i].in && slots[i].turn) turn_of(a, pos, (first_slot + i * step) * V + e, &c[i][e], &s[i][e]);
+    }
+}
+
+template <int V, int S, bool kInter>
+__device__ __forceinline__ void weights(const void* w, int dt, const Slot<V, kInter>* slots, float (&wa)[S][V],
+                                        float (&wb)[S][V]) {
+#pragma unroll
+  for (int i = 0; i < S; ++i)
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      const int ia = kInter ? slots[i].a + 2 * e : slots[i].a + e;
+      const int ib = kInter ? slots[i].a + 2 * e + 1 : slots[i].b + e;
+      wa[i][e] = slots[i].in ? load_any(w, dt, ia) : 0.f;
+      wb[i][e] = slots[i].in && slots[i].has_b ? load_any(w, dt, ib) : 0.f;
+    }
+}
+
+template <int kL>
+__device__ __forceinline__ float lanes_sum(float v) {
+#pragma unroll
+  for (int off = kL / 2; off > 0; off >>= 1) v += __shfl_xor(v, off, kWave);
+  return v;
+}
+
+template <int DT, int V, int kL, int S, bool kInter>
+__global__ __launch_bounds__(kThreads) void qk_rope_forward(QkArgs a) {
+  constexpr int kHeads = kWave / kL;  // heads of a wave's step
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int l = lane % kL, sub = lane / kL;
+  const int64_t unit = (int64_t)blockIdx.x * kWaves + wave;
+  if (unit >= a.batch * a.tokens * a.parts) return;
+  const int64_t token = unit / a.parts;
+  const int part = (int)(unit - token * a.parts);
+  const int64_t b = token / a.tokens, t = token - b * a.tokens;
+  Slot<V, kInter> slots[S];
+#pragma unroll
+  for (int i = 0; i < S; ++i) slots[i].at(l + i * kL, a.d, a.rot);
+  const bool live = !a.mask || a.mask[b * a.mask_b + t * a.mask_t];
+  float c[S][V], s[S][V];
+  angles<V, S, kInter>(a, b, t, slots, l, kL, c, s);
+  const float inv_d = 1.f / (float)a.d;
+  int64_t g = part, base = 0;
+#pragma unroll
+  for (int side = 0; side < 2; ++side) {
+    const Rows& r = a.side[side];
+    const int64_t groups = (r.heads + kHeads - 1) / kHeads;
+    float wa[S][V], wb[S][V];
+    if (g < base + groups) weights<V, S, kInter>(r.w, a.w_dtype, slots, wa, wb);
+    for (; g < base + groups; g += a.parts) {
+      const int64_t head = (g - base) * kHeads + sub;
+      const bool in = head < r.heads;
+      Row<DT, V, S, kInter> x;
+      x.load(r.x + b * r.x_b + t * r.x_t + head * r.x_h, slots, in && live);
+      float sq = 0.f;
+#pragma unroll
+      for (int i = 0; i < S; ++i)
+#pragma unroll
+        for (int e = 0; e < V; ++e) sq += x.a[i][e] * x.a[i][e] + x.b[i][e] * x.b[i][e];
+      const float rms = rsqrtf(lanes_sum<kL>(sq) * inv_d + a.eps);
+      Row<DT, V, S, kInter> z;
+#pragma unroll
+      for (int i = 0; i < S; ++i)
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          const float ya = x.a[i][e] * rms * wa[i][e], yb = x.b[i][e] * rms * wb[i][e];
+          z.a[i][e] = live ? ya * c[i][e] - yb * s[i][e] : 0.f;
+          z.b[i][e] = live ? yb * c[i][e] + ya * s[i][e] : 0.f;
+        }
+      z.store(r.out + b * r.o_b + t * r.o_t + head * r.o_h, slots, in);
+    }
+    base += groups;
+  }
+}
+
+// A workgroup owns one side's rows of `chunk` tokens of a sample; its waves
+// take (token, group of heads) steps in turn and add their lanes' dw up, the
+// waves' sums meet in LDS and go to the chunk's place of the partials in fp32.
+template <int DT, int V, int kL, int S, bool kInter>
+__global__ __launch_bounds__(kThreads) void qk_rope_backward(QkArgs a, int64_t q_blocks) {
+  constexpr int kHeads = kWave / kL;
+  __shared__ float sums[kWaves][2 * S * V * kL];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int l = lane % kL, sub = lane / kL;
+  const int which = (int64_t)blockIdx.x >= q_blocks;
+  const Rows& r = a.side[which];
+  const int64_t block = (int64_t)blockIdx.x - (which ? q_blocks : 0);
+  const int64_t b = block / a.chunks, chunk = block - b * a.chunks;
+  Slot<V, kInter> slots[S];
+#pragma unroll
+  for (int i = 0; i < S; ++i) slots[i].at(l + i * kL, a.d, a.rot);
+  const float inv_d = 1.f / (float)a.d;
+  float wa[S][V], wb[S][V], da_[S][V], db_[S][V];
+  const int64_t groups = (r.heads + kHeads - 1) / kHeads;
+  if (groups) weights<V, S, kInter>(r.w, a.w_dtype, slots, wa, wb);  // an absent side has no weight to read
+#pragma unroll
+  for (int i = 0; i < S; ++i)
+#pragma unroll
+    for (int e = 0; e < V; ++e) da_[i][e] = db_[i][e] = 0.f;
+  const int64_t t0 = chunk * a.chunk, t1 = min(t0 + a.chunk, a.tokens);
+  int64_t t = groups ? t0 + wave / groups : t1, g = groups ? wave % groups : 0, last = -1;
+  float c[S][V], s[S][V];
+  bool live = true;
+  while (t < t1) {
+    if (t != last) {
+      angles<V, S, kInter>(a, b, t, slots, l, kL, c, s);
+      live = !a.mask || a.mask[b * a.mask_b + t * a.mask_t];
+      last = t;
+    }
+    const int64_t head = g * kHeads + sub;
+    const bool in = head < r.heads;
+    Row<DT, V, S, kInter> x, z;
+    x.load(r.x + b * r.x_b + t * r.x_t + head * r.x_h, slots, in && live);
+    z.load(r.gz + b * r.g_b + t * r.g_t + head * r.g_h, slots, in && live);
+    float sq = 0.f, along = 0.f;
+#pragma unroll
+    for (int i = 0; i < S; ++i)
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const float ya = z.a[i][e] * c[i][e] + z.b[i][e] * s[i][e];
+        const float yb = z.b[i][e] * c[i][e] - z.a[i][e] * s[i][e];
+        z.a[i][e] = ya;
+        z.b[i][e] = yb;
+        sq += x.a[i][e] * x.a[i][e] + x.b[i][e] * x.b[i][e];
+        along += ya * wa[i][e] * x.a[i][e] + yb * wb[i][e] * x.b[i][e];
+      }
+    const float rms = rsqrtf(lanes_sum<kL>(sq) * inv_d + a.eps);
+    const float back = lanes_sum<kL>(along) * inv_d * rms * rms;
+    const bool adds = in && live;
+#pragma unroll
+    for (int i = 0; i < S; ++i)
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        // A head or token that is not there has an infinite 1/rms where eps
+        // is 0: selected out, not multiplied by zero.
+        da_[i][e] += adds ? z.a[i][e] * (x.a[i][e] * rms) : 0.f;
+        db_[i][e] += adds ? z.b[i][e] * (x.b[i][e] * rms) : 0.f;
+        z.a[i][e] = live ? rms * (z.a[i][e] * wa[i][e] - x.a[i][e] * back) : 0.f;
+        z.b[i][e] = live ? rms * (z.b[i][e] * wb[i][e] - x.b[i][e] * back) : 0.f;
+      }
+    z.store(r.out + b * r.o_b + t * r.o_t + head * r.o_h, slots, in);
+    for (g += kWaves; g >= groups; g -= groups) ++t;
+  }
+  if (!r.partial) return;
+#pragma unroll
+  for (int i = 0; i < S; ++i)
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      float u = da_[i][e], v = db_[i][e];
+#pragma unroll
+      for (int off = kL; off < kWave; off <<= 1) {
+        u += __shfl_xor(u, off, kWave);
+        v += __shfl_xor(v, off, kWave);
+      }
+      if (sub == 0) {
+        sums[wave][((2 * i) * V + e) * kL + l] = u;
+        sums[wave][((2 * i + 1) * V + e) * kL + l] = v;
+      }
+    }
+  __syncthreads();
+  if (wave == 0 && sub == 0) {
+    float* out = r.partial + (b * a.chunks + chunk) * a.d;
+#pragma unroll
+    for (int i = 0; i < S; ++i)
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        float u = 0.f, v = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+          u += sums[w][((2 * i) * V + e) * kL + l];
+          v += sums[w][((2 * i + 1) * V + e) * kL + l];
+        }
+        const int ia = kInter ? slots[i].a + 2 * e : slots[i].a + e;
+        const int ib = kInter ? slots[i].a + 2 * e + 1 : slots[i].b + e;
+        if (slots[i].in) out[ia] = u;
+        if (slots[i].in && slots[i].has_b) out[ib] = v;
+      }
+  }
+}
+
+// dw of a sample: its chunks' partials in ascending order.
+__global__ __launch_bounds__(kThreads) void qk_rope_join(QkArgs a) {
+  const int64_t n = a.batch * a.d;
+  const int64_t at = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+  if (at >= n) return;
+  const Rows& r = a.side[blockIdx.y];
+  if (!r.wgrad) return;
+  const int64_t b = at / a.d, i = at - b * a.d;
+  float v = 0.f;
+  for (int64_t c = 0; c < a.chunks; ++c) v += r.partial[(b * a.chunks + c) * a.d + i];
+  r.wgrad[at] = v;
+}
+
+int check_args(const char* what, const da_qk_side* sides, int dtype, int weight_dtype, int64_t batch, int64_t tokens,
+               int64_t d, int64_t rot, const float* inv_freq, const void* positions, int position_bytes) {
+  if (!valid_dtype(dtype) || !valid_dtype(weight_dtype))
+    return set_error(DA_ERR_INVALID, "%s: bad dtype %d / %d", what, dtype, weight_dtype);
+  if (!sides) return set_error(DA_ERR_INVALID, "%s: NULL sides", what);
+  if (batch < 0 || tokens < 0 || sides[0].heads < 0 || sides[1].heads < 0)
+    return set_error(DA_ERR_INVALID, "%s: negative size", what);
+  if (d < 1 || d > kMaxD) return set_error(DA_ERR_UNSUPPORTED, "%s: head width %lld outside 1..1024", what, (long long)d);
+  if (rot < 0 || rot % 2 || rot > d)
+    return set_error(DA_ERR_INVALID, "%s: rotated width %lld must be even and at most the head width %lld", what,
+                     (long long)rot, (long long)d);
+  if (rot && !inv_freq) return set_error(DA_ERR_INVALID, "%s: NULL inv_freq", what);
+  if (positions && position_bytes != 4 && position_bytes != 8)
+    return set_error(DA_ERR_INVALID, "%s: positions must have 4 or 8 bytes", what);
+  return DA_OK;
+}
+
+void fill_side(Rows& r, const da_qk_side& s, int es) {
+  r = Rows{};
+  r.x = (const char*)s.x;
+  r.gz = (const char*)s.gz;
+  r.out = (char*)s.out;
+  r.w = s.weight;
+  r.wgrad = s.weight_grad;
+  r.heads = s.heads;
+  r.x_b = s.x_bstride * es, r.x_t = s.x_tstride * es, r.x_h = s.x_hstride * es;
+  r.g_b = s.gz_bstride * es, r.g_t = s.gz_tstride * es, r.g_h = s.gz_hstride * es;
+  r.o_b = s.out_bstride * es, r.o_t = s.out_tstride * es, r.o_h = s.out_hstride * es;
+}
+
+void chunking(int64_t batch, int64_t tokens, int64_t* chunk, int64_t* chunks) {
+  *chunk = 16;
+  *chunks = (tokens + 15) / 16;
+  (void)batch;
+}
+
+}  // namespace
+}  // namespace da
+
+using namespace da;
+
+#define DA_QK_SLOTS(CALL, DT, IL)        \
+  if (pairs <= 64) {                     \
+    CALL(DT, 1, 64, 1, IL)               \
+  } else if (pairs <= 128) {             \
+    CALL(DT, 1, 64, 2, IL)               \
+  } else if (pairs <= 256) {             \
+    CALL(DT, 1, 64, 4, IL)               \
+  } else {                               \
+    CALL(DT, 1, 64, 8, IL)               \
+  }
+#define DA_QK_DISPATCH(CALL)                                                    \
+  if (dtype == DA_BF16) {                                                       \
+    if (interleaved) { DA_QK_SLOTS(CALL, DA_BF16, true) }                       \
+    else { DA_QK_SLOTS(CALL, DA_BF16, false) }                                  \
+  } else if (dtype == DA_F16) {                                                 \
+    if (interleaved) { DA_QK_SLOTS(CALL, DA_F16, true) }                        \
+    else { DA_QK_SLOTS(CALL, DA_F16, false) }                                   \
+  } else {                                                                      \
+    if (interleaved) { DA_QK_SLOTS(CALL, DA_F32, true) }                        \
+    else { DA_QK_SLOTS(CALL, DA_F32, false) }                                   \
+  }
+
+extern "C" {
+
+int da_qk_norm_rope(const da_qk_side* sides, int dtype, int weight_dtype, int64_t batch, int64_t tokens, int64_t d,
+                    int64_t rot, const float* inv_freq, const void* positions, int position_bytes,
+                    int64_t pos_bstride, int64_t pos_tstride, const uint8_t* mask, int64_t mask_bstride,
+                    int64_t mask_tstride, int interleaved, float scaling, float eps, void* stream) {
+  if (int rc = check_args("da_qk_norm_rope", sides, dtype, weight_dtype, batch, tokens, d, rot, inv_freq, positions,
+                          position_bytes))
+    return rc;
+  QkArgs a{};
+  const int es = (int)elem_bytes(dtype);
+  for (int i = 0; i < 2; ++i) {
+    if (batch && tokens && sides[i].heads && (!sides[i].x || !sides[i].out || !sides[i].weight))
+      return set_error(DA_ERR_INVALID, "da_qk_norm_rope: NULL pointer of side %d", i);
+    fill_side(a.side[i], sides[i], es);
+  }
+  if (!batch || !tokens || !(sides[0].heads + sides[1].heads)) return DA_OK;
+  a.batch = batch, a.tokens = tokens, a.d = (int)d, a.rot = (int)rot, a.w_dtype = weight_dtype;
+  a.inv_freq = inv_freq, a.pos = positions, a.pos_bytes = position_bytes, a.pos_b = pos_bstride, a.pos_t = pos_tstride;
+  a.mask = mask, a.mask_b = mask_bstride, a.mask_t = mask_tstride, a.scaling = scaling, a.eps = eps;
+  hipStream_t st = (hipStream_t)stream;
+  const int64_t pairs = rot / 2 + (d - rot + 1) / 2;
+  a.parts = 1;
+  const int64_t blocks = (batch * tokens * a.parts + kWaves - 1) / kWaves;
+  if (blocks > 0x7fffffff) return set_error(DA_ERR_UNSUPPORTED, "da_qk_norm_rope: too many tokens");
+#define DA_QK_FWD(DT, V, L, S, IL) qk_rope_forward<DT, V, L, S, IL><<<(unsigned)blocks, kThreads, 0, st>>>(a);
+  DA_QK_DISPATCH(DA_QK_FWD)
+#undef DA_QK_FWD
+  return check_launch("da_qk_norm_rope");
+}
+
+int da_qk_norm_rope_grad_workspace(int64_t batch, int64_t tokens, int64_t d, size_t* bytes) {
+  if (!bytes || batch < 0 || tokens < 0 || d < 0)
+    return set_error(DA_ERR_INVALID, "da_qk_norm_rope_grad_workspace: bad argument");
+  int64_t chunk, chunks;
+  chunking(batch, tokens, &chunk, &chunks);
+  *bytes = (size_t)(2 * batch * chunks * d) * sizeof(float);
+  return DA_OK;
+}
+
+int da_qk_norm_rope_grad(const da_qk_side* sides, int dtype, int weight_dtype, int64_t batch, int64_t tokens,
+                         int64_t d, int64_t rot, const float* inv_freq, const void* positions, int position_bytes,
+                         int64_t pos_bstride, int64_t pos_tstride, const uint8_t* mask, int64_t mask_bstride,
+                         int64_t mask_tstride, int interleaved, float scaling, float eps, void* workspace,
+                         size_t workspace_bytes, void* stream) {
+  if (int rc = check_args("da_qk_norm_rope_grad", sides, dtype, weight_dtype, batch, tokens, d, rot, inv_freq,
+                          positions, position_bytes))
+    return rc;
+  QkArgs a{};
+  const int es = (int)elem_bytes(dtype);
+  bool wanted = false;
+  for (int i = 0; i < 2; ++i) {
+    if (batch && tokens && sides[i].heads && (!sides[i].x || !sides[i].gz || !sides[i].out || !sides[i].weight))
+      return set_error(DA_ERR_INVALID, "da_qk_norm_rope_grad: NULL pointer of side %d", i);
+    fill_side(a.side[i], sides[i], es);
+    wanted |= sides[i].weight_grad != nullptr;
+  }
+  if (!batch) return DA_OK;
+  hipStream_t st = (hipStream_t)stream;
+  chunking(batch, tokens, &a.chunk, &a.chunks);
+  const size_t need = (size_t)(2 * batch * a.chunks * d) * sizeof(float);
+  if (wanted && need && (!workspace || workspace_bytes < need))
+    return set_error(DA_ERR_WORKSPACE, "da_qk_norm_rope_grad: workspace of %zu bytes, %zu needed", workspace_bytes, need);
+  for (int i = 0; i < 2; ++i)
+    a.side[i].partial = a.side[i].wgrad ? (float*)workspace + (int64_t)i * batch * a.chunks * d : nullptr;
+  a.batch = batch, a.tokens = tokens, a.d = (int)d, a.rot = (int)rot, a.w_dtype = weight_dtype;
+  a.inv_freq = inv_freq, a.pos = positions, a.pos_bytes = position_bytes, a.pos_b = pos_bstride, a.pos_t = pos_tstride;
+  a.mask = mask, a.mask_b = mask_bstride, a.mask_t = mask_tstride, a.scaling = scaling, a.eps = eps;
+  const int64_t pairs = rot / 2 + (d - rot + 1) / 2;
+  const int64_t per_side = batch * a.chunks;
+  if (2 * per_side > 0x7fffffff) return set_error(DA_ERR_UNSUPPORTED, "da_qk_norm_rope_grad: too many tokens");
+  if (per_side) {
+    const int64_t blocks = 2 * per_side;
+#define DA_QK_BWD(DT, V, L, S, IL) \
+  qk_rope_backward<DT, V, L, S, IL><<<(unsigned)blocks, kThreads, 0, st>>>(a, per_side);
+    DA_QK_DISPATCH(DA_QK_BWD)
+#undef DA_QK_BWD
+    if (int rc = check_launch("da_qk_norm_rope_grad")) return rc;
+  }
+  if (wanted) {
+    qk_rope_join<<<dim3((unsigned)((batch * d + kThreads - 1) / kThreads), 2), kThreads, 0, st>>>(a);
+    return check_launch("da_qk_norm_rope_grad (join)");
+  }
+  return DA_OK;
+}
+
+}  // extern "C"

@@ -16,7 +16,7 @@ import torch
 
 LIB_NAME = "libdattri_amd.so"
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), LIB_NAME)
-ABI_VERSION = 16
+ABI_VERSION = 17
 
 DA_F32, DA_F16, DA_BF16 = 0, 1, 2
 DA_OK, DA_ERR_INVALID, DA_ERR_UNSUPPORTED, DA_ERR_HIP, DA_ERR_WORKSPACE = 0, 1, 2, 3, 4
@@ -196,6 +196,39 @@ SIGNATURES.update(
         "da_moe_route": (_I32, [_P, _I64, _I32, _I32, _I64, _I64, _P, _P, _P, _P, _P]),
     "da_counting_sort": (_I32, [_P, _P, _I64, _I64, _I64, _I32, _I64, _I32, _P, _P, _P]),
         "da_compact_rows": (_I32, [_P, _I64, _I64, _P, _P, _P]),
+    }
+)
+
+
+class QkSide(ctypes.Structure):
+    """Mirror of ``da_qk_side`` (include/dattri_amd.h)."""
+
+    _fields_ = [
+        *((f, ctypes.c_void_p) for f in ("x", "gz", "out", "weight", "weight_grad")),
+        *((f, ctypes.c_int64) for f in ("heads", "x_bstride", "x_tstride", "x_hstride", "gz_bstride", "gz_tstride",
+                                        "gz_hstride", "out_bstride", "out_tstride", "out_hstride")),
+    ]
+
+
+_QK = [ctypes.POINTER(QkSide), _I32, _I32, _I64, _I64, _I64, _I64, _P, _P, _I32, _I64, _I64, _P, _I64, _I64, _I32,
+       ctypes.c_float, ctypes.c_float]
+_EDGES = ctypes.POINTER(ctypes.c_int32)
+SIGNATURES.update(
+    {
+        "da_qk_norm_rope": (_I32, [*_QK, _P]),
+        "da_qk_norm_rope_grad_workspace": (_I32, [_I64, _I64, _I64, ctypes.POINTER(_SZ)]),
+        "da_qk_norm_rope_grad": (_I32, [*_QK, _P, _SZ, _P]),
+        "da_relative_bias": (
+            _I32, [_P, _I32, _I64, _I64, _I64, _I64, _I64, _I64, _EDGES, _I32, _I32, _I32, _P, _P]),
+        "da_relative_bias_grad_workspace": (_I32, [_I64, _I64, _I64, _I64, _I32, ctypes.POINTER(_SZ)]),
+        "da_relative_bias_grad": (
+            _I32, [_P, _I32, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _EDGES, _I32, _I32, _I32, _P, _I64, _I64,
+                   _P, _P, _SZ, _P]),
+        "da_balance_loss_workspace": (_I32, [_I64, _I64, _I32, ctypes.POINTER(_SZ)]),
+        "da_balance_loss": (
+            _I32, [_P, _I32, _I64, _I64, _I32, _I64, _P, _I32, _P, _I64, _I64, _P, _P, _P, _P, _P, _SZ, _P]),
+        "da_balance_loss_grad": (
+            _I32, [_P, _P, _P, _I32, _I64, _I64, _I32, _I64, _P, _P, _P, _I64, _I64, _P, _I64, _P]),
     }
 )
 

@@ -9,6 +9,7 @@ manager belong to the capture's control plane and are not part of this package.
 from dattri_llm_amd.gradient import ops
 from dattri_llm_amd.gradient.capture import FusedCapture
 from dattri_llm_amd.gradient.gradient import Factorized, Gradient, GradientRecord
+from dattri_llm_amd.gradient.layers import QKNormRope, RelativeBias
 from dattri_llm_amd.gradient.ops import (
     FisherAccumulator,
     KroneckerAccumulator,
@@ -36,6 +37,8 @@ __all__ = [
     "KroneckerAccumulator",
     "LayerFisherAccumulator",
     "LayerKroneckerAccumulator",
+    "QKNormRope",
+    "RelativeBias",
     "RowLayout",
     "canonical_class_name",
     "dot",

@@ -1,4 +1,5 @@
-"""Gradient capture fused into autograd for ``nn.Linear`` layers.
+"""Gradient capture fused into autograd for ``nn.Linear`` layers, and for the
+attention parameters of :mod:`dattri_llm_amd.gradient.layers`.
 
 The reference captures a linear layer's factors with a forward hook (stashing
 the input activation on a per-device stack) and a backward hook that pops it,
@@ -20,6 +21,11 @@ and runs the capture on ``(input, grad_output)`` on the same stream:
 * unprojected: the raw factors, or the dense ``(B, d_out * (d_in + 1))``
   gradient from the dW kernel.
 
+A :class:`QKNormRope` or :class:`RelativeBias` module is captured by its own
+backward kernel, which gives the per-sample weight gradients: materialized
+layers, ``<name>.q_weight`` and ``<name>.k_weight`` of type ``nn.RMSNorm``, and
+``<name>`` of type ``nn.Embedding``, in fp32.
+
 No weight or bias gradient is produced for a captured layer, as with the
 reference's invasive capture: use it for attribution, not for training.  The
 representation of a layer is fixed by its first micro-batch of a step, and
@@ -34,6 +40,7 @@ import torch
 from torch import nn
 
 from dattri_llm_amd.gradient.gradient import Factorized, Gradient
+from dattri_llm_amd.gradient.layers import QKNormRope, RelativeBias
 from dattri_llm_amd.gradient.ops import materialize_factors, project_layer, should_materialize
 from dattri_llm_amd.gradient.ops.projection import DattriProjector
 
@@ -110,10 +117,33 @@ class _LayerSlot:
             self.factorized = None
 
 
-class FusedCapture:
-    """Capture per-sample gradients of ``nn.Linear`` layers inside autograd.
+class _WeightSlot:
+    """A captured parameter whose backward pass forms its per-sample gradient."""
 
-    ``layers``: names of the ``nn.Linear`` modules to capture (default: all).
+    def __init__(self) -> None:
+        self.parts: list = []
+        self.lock = threading.Lock()
+
+    def put(self, per_sample: torch.Tensor) -> None:
+        with self.lock:
+            self.parts.append(per_sample)
+
+    def collect(self):
+        with self.lock:
+            parts = list(self.parts)
+        return ("materialized", torch.cat(parts, dim=0)) if parts else None
+
+    def clear(self) -> None:
+        with self.lock:
+            self.parts.clear()
+
+
+class FusedCapture:
+    """Capture per-sample gradients of ``nn.Linear``, :class:`QKNormRope` and
+    :class:`RelativeBias` layers inside autograd.
+
+    ``layers``: names of the modules to capture (default: all of these types).
+    A captured ``RelativeBias`` has to be called with ``batch``.
     ``proj_dim``: LoGRA projection width (``None``: unprojected capture), with
     ``proj_seed`` / ``projector`` as in ``project_factors`` (seed for the
     gradient side, seed + 1 for the activation side).  ``capture_style``:
@@ -132,29 +162,66 @@ class FusedCapture:
             raise ValueError(f"capture_style must be 'factorized', 'materialized' or 'auto', got {capture_style!r}.")
         root = getattr(model, "module", model)
         wanted = None if layers is None else set(layers)
-        self.slots: dict[str, _LayerSlot] = {}
+        self.slots: dict[str, _LayerSlot | _WeightSlot] = {}
+        self.types: dict[str, str] = {}
+        self._modules: list = []  # (module, the forward that captures it)
+        seen = set()
         for name, module in root.named_modules():
             if wanted is not None and name not in wanted:
                 continue
-            if type(module) is not nn.Linear:
-                if wanted is not None:
-                    raise ValueError(f"layer {name!r} is a {type(module).__name__}, not a plain nn.Linear")
-                continue
-            self.slots[name] = _LayerSlot(name, module, self)
-        if wanted is not None and wanted - set(self.slots):
-            raise ValueError(f"no such layers: {sorted(wanted - set(self.slots))}")
+            if type(module) is nn.Linear:
+                self._add_linear(name, module)
+            elif type(module) is QKNormRope:
+                self._add_qk(name, module)
+            elif type(module) is RelativeBias:
+                self._add_bias(name, module)
+            elif wanted is not None:
+                raise ValueError(f"layer {name!r} is a {type(module).__name__}, not a plain nn.Linear, QKNormRope or "
+                                 "RelativeBias")
+            seen.add(name)
+        if wanted is not None and wanted - seen:
+            raise ValueError(f"no such layers: {sorted(wanted - seen)}")
         self.proj_dim, self.proj_seed = proj_dim, proj_seed
         self.projector = DattriProjector.coerce(projector)
         self.capture_style, self.batch_first, self.include_bias = capture_style, batch_first, include_bias
         self._reverts: list = []
 
+    def _add_linear(self, name: str, module: nn.Linear) -> None:
+        slot = self.slots[name] = _LayerSlot(name, module, self)
+        self.types[name] = "nn.Linear"
+        self._modules.append((module, lambda x: _CaptureLinear.apply(x, module.weight, module.bias, slot)))
+
+    def _add_qk(self, name: str, module: QKNormRope) -> None:
+        slots = []
+        for part in ("q_weight", "k_weight"):
+            at = f"{name}.{part}" if name else part
+            self.slots[at] = _WeightSlot()
+            self.types[at] = "nn.RMSNorm"
+            slots.append(self.slots[at])
+
+        def forward(q, k, positions=None, mask=None):
+            self._check_batch_first(name)
+            return QKNormRope.forward(module, q, k, positions, mask, _slots=tuple(slots))
+
+        self._modules.append((module, forward))
+
+    def _add_bias(self, name: str, module: RelativeBias) -> None:
+        slot = self.slots[name] = _WeightSlot()
+        self.types[name] = "nn.Embedding"
+
+        def forward(q_len, k_len, *, batch=None, q_start=0, mask=None):
+            if batch is None:
+                raise ValueError(f"layer {name!r}: a captured RelativeBias needs batch, the samples apart")
+            return RelativeBias.forward(module, q_len, k_len, batch=batch, q_start=q_start, mask=mask, _slot=slot)
+
+        self._modules.append((module, forward))
+
+    def _check_batch_first(self, name: str) -> None:
+        if not self.batch_first:
+            raise ValueError(f"layer {name!r}: QKNormRope is captured batch first only")
+
     def __enter__(self) -> FusedCapture:
-        for slot in self.slots.values():
-            m = slot.module
-
-            def forward(x, _m=m, _slot=slot):
-                return _CaptureLinear.apply(x, _m.weight, _m.bias, _slot)
-
+        for m, forward in self._modules:
             had = "forward" in m.__dict__
             old = m.__dict__.get("forward")
             m.forward = forward
@@ -177,7 +244,7 @@ class FusedCapture:
             if got is None:
                 continue
             rep[name], data[name] = got
-            types[name] = "nn.Linear"
+            types[name] = self.types[name]
         if not data:
             raise RuntimeError("FusedCapture: no layer has been captured since the last clear()")
         return Gradient(rep, data, types)

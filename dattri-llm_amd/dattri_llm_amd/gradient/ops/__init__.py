@@ -7,6 +7,12 @@ tensors, the unsuffixed ones take :class:`Factorized` (or dense tensors).
 """
 
 from dattri_llm_amd.gradient.ops import cost, dtypes, kronecker, moe
+from dattri_llm_amd.gradient.ops.attention import (
+    qk_norm_rope,
+    qk_norm_rope_grad,
+    relative_bias,
+    relative_bias_grad,
+)
 from dattri_llm_amd.gradient.ops.cost import CostModel, calibrate, get_routing_policy, set_routing_policy
 from dattri_llm_amd.gradient.ops.dot import (
     block_grad_norm_sq,
@@ -133,6 +139,7 @@ __all__ = [
     "maybe_use_materialized_norm", "moe", "pairwise_dot", "pairwise_dot_factors", "preprocess_factorized",
     "preprocess_factors", "project_activation", "project_factorized", "project_factors",
     "project_gradient", "project_layer", "project_materialized", "project_materialized_factors",
-    "project_outer_factors", "route_flops", "set_compute_dtype",
+    "project_outer_factors", "qk_norm_rope", "qk_norm_rope_grad", "relative_bias", "relative_bias_grad",
+    "route_flops", "set_compute_dtype",
     "set_routing_policy", "should_materialize", "to_3d",
 ]

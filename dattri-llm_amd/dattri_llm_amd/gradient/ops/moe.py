@@ -19,6 +19,8 @@ over experts accumulates into one fp32 matrix.
 
 from __future__ import annotations
 
+from typing import NamedTuple
+
 import torch
 
 from dattri_llm_amd import kernels
@@ -31,6 +33,70 @@ def router_topk(logits: torch.Tensor, k: int) -> tuple[torch.Tensor, torch.Tenso
     """``(weights, indices)`` of the top-k router; indices int64 (N, k)."""
     logits = logits.reshape(-1, logits.shape[-1])
     return kernels.moe_topk(logits, k)
+
+
+class BalanceLoss(NamedTuple):
+    """:func:`balance_loss`'s result: the two losses of each sample, the live
+    choices of each expert and the live tokens."""
+
+    loss: torch.Tensor  # (B,)
+    z_loss: torch.Tensor  # (B,)
+    counts: torch.Tensor  # (B, E) int32
+    live: torch.Tensor  # (B,) int32
+
+
+class _BalanceLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, index, batch, mask):
+        loss, z_loss, counts, live = kernels.balance_loss(logits, index, batch=batch, mask=mask)
+        ctx.save_for_backward(logits, counts, live, mask)
+        ctx.mark_non_differentiable(counts, live)
+        return loss, z_loss, counts, live
+
+    @staticmethod
+    def backward(ctx, up, up_z, _counts, _live):
+        logits, counts, live, mask = ctx.saved_tensors
+        return kernels.balance_loss_grad(up, up_z, logits, counts, live, mask=mask), None, None, None
+
+
+def balance_loss(logits: torch.Tensor, top_idx: torch.Tensor, *, batch: int | None = None,
+                 mask: torch.Tensor | None = None) -> BalanceLoss:
+    """Load-balance and z losses of a router, per sample, differentiable in the
+    logits.
+
+    ``logits`` (B, T, E), or (N, E) with ``batch`` samples of equal length
+    (default 1: one loss over all tokens); ``top_idx`` the chosen experts
+    (``router_topk``'s), int64, ``k`` for each token.  Over a sample's ``n`` live
+    tokens (``mask`` (B, T) non-zero, or all), with ``p = softmax(logits)``::
+
+        counts[e] = choices of e,   loss = E * sum_e (counts[e] / n) * mean(p[e])
+        z_loss = mean(logsumexp(logits) ** 2)
+
+    so that an even load gives ``loss = k``.  Masked tokens take no part,
+    whatever their logits hold; a sample without live tokens has zeros.  An
+    index outside the experts (a dropped choice) counts for none."""
+    if logits.dim() not in (2, 3) or top_idx.dim() not in (2, 3):
+        raise ValueError("balance_loss expects (B, T, E) or (N, E) logits and expert indices alike")
+    if logits.dim() == 3:
+        if batch not in (None, logits.shape[0]):
+            raise ValueError(f"balance_loss: batch {batch} for logits of {logits.shape[0]} samples")
+        batch = logits.shape[0]
+    logits, top_idx = logits.flatten(0, -2), top_idx.flatten(0, -2)
+    batch = 1 if batch is None else batch
+    if torch.is_grad_enabled() and logits.requires_grad:
+        return BalanceLoss(*_BalanceLoss.apply(logits, top_idx, batch, mask))
+    return BalanceLoss(*kernels.balance_loss(logits, top_idx, batch=batch, mask=mask))
+
+
+def balance_loss_grad(up: torch.Tensor | None, up_z: torch.Tensor | None, logits: torch.Tensor, counts: torch.Tensor,
+                      live: torch.Tensor, *, mask: torch.Tensor | None = None) -> torch.Tensor:
+    """The backward pass of :func:`balance_loss` as a plain call: the logits'
+    gradient, in their shape and dtype, for the losses' gradients ``up`` and
+    ``up_z`` (B,; None: zero); ``counts`` and ``live`` are its results."""
+    if logits.dim() not in (2, 3):
+        raise ValueError("balance_loss_grad expects (B, T, E) or (N, E) logits")
+    grad = kernels.balance_loss_grad(up, up_z, logits.flatten(0, -2), counts, live, mask=mask)
+    return grad.view(logits.shape)
 
 
 def expert_segments(top_idx: torch.Tensor, n_experts: int) -> tuple[torch.Tensor, torch.Tensor]:

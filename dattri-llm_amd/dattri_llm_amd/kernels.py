@@ -12,6 +12,7 @@ from __future__ import annotations
 import array
 import contextlib
 import ctypes
+import functools
 import math
 
 import numpy as np
@@ -1471,3 +1472,270 @@ def ghost_gram_segmented(a1, g1, seg1, idx1, tokens1, a2, g2, seg2, idx2, tokens
          s1, s2, k, d, code, out.data_ptr(), out.stride(0), int(accumulate), ws.data_ptr(), ws.numel(),
          nat.stream_ptr(dev))
     return out
+
+
+def _run_on(dev: torch.device, what: str, fn, *args) -> None:
+    """:func:`_run` with ``dev`` made the current device where it is not."""
+    if dev.index is None or dev.index == torch.cuda.current_device():
+        _run(dev, what, fn, *args)
+        return
+    with torch.cuda.device(dev):
+        _run(dev, what, fn, *args)
+
+
+def _token_mask(what: str, mask: torch.Tensor | None, batch: int, tokens: int):
+    """``(tensor, pointer, batch stride, token stride)`` of a (batch, tokens)
+    byte mask; other integer masks are compared with zero first."""
+    if mask is None:
+        return None, None, 0, 0
+    if tuple(mask.shape) != (batch, tokens):
+        raise ValueError(f"{what}: mask must have shape ({batch}, {tokens}), got {tuple(mask.shape)}")
+    if mask.dtype not in (torch.bool, torch.uint8):
+        mask = mask != 0
+    return mask, mask.data_ptr(), mask.stride(0), mask.stride(1)
+
+
+def _unit_rows(x: torch.Tensor) -> torch.Tensor:
+    return x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
+
+
+def _qk_sides(xs, ws, gzs, grads: bool):
+    """The two ``da_qk_side`` records; returns them with the outputs and every
+    tensor the launch reads."""
+    sides = (nat.QkSide * 2)()
+    outs, wgrads, keep = [], [], []
+    b, t, d = xs[0].shape[0], xs[0].shape[1], xs[0].shape[3]
+    for side, x, w, gz in zip(sides, xs, ws, gzs):
+        if x is None:
+            side.heads = 0
+            outs.append(None)
+            wgrads.append(None)
+            continue
+        x, w = _unit_rows(x), w.contiguous()
+        out = torch.empty_like(x)
+        side.x, side.out, side.weight, side.heads = x.data_ptr(), out.data_ptr(), w.data_ptr(), x.shape[2]
+        side.x_bstride, side.x_tstride, side.x_hstride = x.stride()[:3]
+        side.out_bstride, side.out_tstride, side.out_hstride = out.stride()[:3]
+        wgrad = None
+        if gz is not None:
+            gz = _unit_rows(gz)
+            side.gz = gz.data_ptr()
+            side.gz_bstride, side.gz_tstride, side.gz_hstride = gz.stride()[:3]
+            if grads:
+                wgrad = torch.empty(b, d, dtype=torch.float32, device=x.device)
+                side.weight_grad = wgrad.data_ptr()
+        outs.append(out)
+        wgrads.append(wgrad)
+        keep += (x, w, gz)
+    return sides, outs, wgrads, keep, b, t, d
+
+
+def _qk_rope(what, q, k, q_weight, k_weight, inv_freq, positions, mask, gq, gk, interleaved, scaling, eps, grads=True):
+    if q.dim() != 4 or (k is not None and k.dim() != 4):
+        raise ValueError(f"{what} expects (B, T, heads, D) queries and keys")
+    if k is not None and (k.shape[:2] != q.shape[:2] or k.shape[3] != q.shape[3]):
+        raise ValueError(f"{what}: queries {tuple(q.shape)} and keys {tuple(k.shape)} disagree on B, T or D")
+    b, t, _, d = q.shape
+    for x, w, gz in ((q, q_weight, gq), (k, k_weight, gk)):
+        if x is None:
+            continue
+        if w is None or tuple(w.shape) != (d,):
+            raise ValueError(f"{what}: a norm weight must have shape ({d},)")
+        if x.dtype != q.dtype or (gz is not None and gz.dtype != q.dtype) or w.dtype != q_weight.dtype:
+            raise ValueError(f"{what}: queries, keys and their gradients must share one dtype, and so the weights")
+        if gz is not None and gz.shape != x.shape:
+            raise ValueError(f"{what}: a gradient of shape {tuple(gz.shape)} for rows of {tuple(x.shape)}")
+    if inv_freq.dim() != 1 or inv_freq.dtype != torch.float32:
+        raise ValueError(f"{what}: inv_freq must be a 1-D float32 tensor")
+    rot = 2 * inv_freq.shape[0]
+    if rot > d:
+        raise ValueError(f"{what}: {inv_freq.shape[0]} frequencies rotate {rot} entries, the heads have {d}")
+    codes = nat.dtype_code(q.dtype), nat.dtype_code(q_weight.dtype)
+    inv_freq = inv_freq.contiguous()
+    pos_ptr, pos_bytes, pos_b, pos_t = None, 0, 0, 0
+    if positions is not None:
+        if positions.dtype not in (torch.int32, torch.int64):
+            raise ValueError(f"{what}: positions must be int32 or int64")
+        if tuple(positions.shape) not in ((t,), (1, t), (b, t)):
+            raise ValueError(f"{what}: positions must have shape ({t},) or ({b}, {t}), got {tuple(positions.shape)}")
+        pos_ptr, pos_bytes, pos_t = positions.data_ptr(), positions.element_size(), positions.stride(-1)
+        pos_b = positions.stride(0) if positions.dim() == 2 and positions.shape[0] == b else 0
+    mask, mask_ptr, mask_b, mask_t = _token_mask(what, mask, b, t)
+    dev = nat.require_device(q, k, q_weight, k_weight, inv_freq, positions, mask, gq, gk)
+    sides, outs, wgrads, keep, b, t, d = _qk_sides( (q, k), (q_weight, k_weight), (gq, gk), grads)
+    args = (sides, *codes, b, t, d, rot, inv_freq.data_ptr(), pos_ptr,
+            pos_bytes, pos_b, pos_t, mask_ptr, mask_b, mask_t, int(bool(interleaved)), float(scaling), float(eps))
+    lib = nat.load()
+    if gq is None:
+        _run_on(dev, what, lib.da_qk_norm_rope, *args, nat.stream_ptr(dev))
+        return outs
+    nbytes = ctypes.c_size_t(0)
+    nat.check(lib.da_qk_norm_rope_grad_workspace(b, t, d, ctypes.byref(nbytes)), what)
+    ws = nat.workspace(nbytes.value if grads else 0, dev)
+    _run_on(dev, what, lib.da_qk_norm_rope_grad, *args, ws.data_ptr(), ws.numel(), nat.stream_ptr(dev))
+    del keep
+    return (*outs, *wgrads)
+
+
+def qk_norm_rope(q, k, q_weight, k_weight, inv_freq, positions=None, *, eps: float, interleaved: bool = False,
+                 scaling: float = 1.0, mask=None):
+    """RMS norm of each head's queries and keys with the position rotation
+    (``da_qk_norm_rope``): ``(q_out, k_out)`` like ``q`` and ``k``.
+
+    ``q`` (B, T, Hq, D) and ``k`` (B, T, Hk, D, or None) may have any strides
+    (a copy is made where entries are not contiguous); weights ``(D,)``,
+    ``inv_freq`` float32 ``(R/2,)``, ``positions`` int32/int64 ``(T,)`` or
+    ``(B, T)`` (default: the token's index), ``mask`` (B, T), zero for tokens
+    whose output is zero."""
+    return tuple(_qk_rope("qk_norm_rope", q, k, q_weight, k_weight, inv_freq, positions, mask, None, None, interleaved,
+                          scaling, eps))
+
+
+def qk_norm_rope_grad(gq, gk, q, k, q_weight, k_weight, inv_freq, positions=None, *, eps: float,
+                      interleaved: bool = False, scaling: float = 1.0, mask=None, weight_grads: bool = True):
+    """Gradients of :func:`qk_norm_rope` for its outputs' gradients ``gq`` and
+    ``gk``: ``(dq, dk, dq_weight, dk_weight)``, the weights' per sample, fp32
+    ``(B, D)`` (None without ``weight_grads``)."""
+    if gq is None or (k is None) != (gk is None):
+        raise ValueError("qk_norm_rope_grad: one output gradient for each side given")
+    return _qk_rope("qk_norm_rope_grad", q, k, q_weight, k_weight, inv_freq, positions, mask, gq, gk, interleaved,
+                    scaling, eps, weight_grads)
+
+
+@functools.lru_cache(maxsize=64)
+def _bucket_edges(num_buckets: int, max_distance: int, bidirectional: bool):
+    """The least distance of each bucket of one side, as a ctypes array.
+
+    Of a side's ``n`` buckets the first ``m = n // 2`` hold one distance each;
+    bucket ``m + j`` starts at the least ``r`` with ``(r / m)^(n - m) >=
+    (max_distance / m)^j``, worked out in integers."""
+    if num_buckets < 2 or num_buckets > 256 or (bidirectional and (num_buckets % 2 or num_buckets < 4)):
+        raise ValueError(f"relative bias: num_buckets must be 2 to 256 (bidirectional: even, from 4), got {num_buckets}")
+    n = num_buckets // 2 if bidirectional else num_buckets
+    m = n // 2
+    if not m < max_distance <= 1 << 30:
+        raise ValueError(f"relative bias: max_distance must be above {m} and at most 2^30, got {max_distance}")
+    edges = list(range(m + 1))
+    for j in range(1, n - m):
+        lo, hi = edges[-1], max_distance
+        bound = max_distance ** j * m ** (n - m - j)  # r^(n-m) has to reach it
+        while lo < hi:
+            mid = (lo + hi) // 2
+            if mid ** (n - m) >= bound:
+                hi = mid
+            else:
+                lo = mid + 1
+        edges.append(lo)
+    return (ctypes.c_int32 * n)(*edges)
+
+
+def relative_bias(table: torch.Tensor, q_len: int, k_len: int, *, q_start: int = 0, bidirectional: bool = True,
+                  max_distance: int = 128, causal: bool = False) -> torch.Tensor:
+    """``(H, q_len, k_len)`` attention bias from a ``(num_buckets, H)`` table in
+    its dtype (``da_relative_bias``); query ``i`` is at position ``i + q_start``."""
+    if table.dim() != 2:
+        raise ValueError("relative_bias expects a (num_buckets, heads) table")
+    if q_len < 0 or k_len < 0:
+        raise ValueError("relative_bias: negative length")
+    edges = _bucket_edges(int(table.shape[0]), int(max_distance), bool(bidirectional))
+    code = nat.dtype_code(table.dtype)
+    dev = nat.require_device(table)
+    out = torch.empty(table.shape[1], q_len, k_len, dtype=table.dtype, device=dev)
+    _run_on(dev, "relative_bias", nat.load().da_relative_bias,
+            table.data_ptr(), code, table.stride(0), table.stride(1), table.shape[1], q_len,
+            k_len, int(q_start), edges, len(edges), int(bool(bidirectional)), int(bool(causal)), out.data_ptr(),
+            nat.stream_ptr(dev))
+    return out
+
+
+def relative_bias_grad(g: torch.Tensor, num_buckets: int, *, q_start: int = 0, bidirectional: bool = True,
+                       max_distance: int = 128, causal: bool = False, mask=None) -> torch.Tensor:
+    """Per-sample table gradient ``(B, num_buckets, H)``, fp32, of the gradient
+    ``g (B, H, q_len, k_len)`` of the scores the bias was added to
+    (``da_relative_bias_grad``).  ``causal``: entries after their query are not
+    read; ``mask`` (B, k_len): entries of a dead query (position ``i +
+    q_start``) or key add nothing."""
+    if g.dim() != 4:
+        raise ValueError("relative_bias_grad expects a (B, heads, q_len, k_len) gradient")
+    b, h, tq, tk = g.shape
+    edges = _bucket_edges(int(num_buckets), int(max_distance), bool(bidirectional))
+    code = nat.dtype_code(g.dtype)
+    mask, mask_ptr, mask_b, mask_k = _token_mask("relative_bias_grad", mask, b, tk)
+    if mask is not None and not 0 <= q_start <= tk - tq:
+        raise ValueError(f"relative_bias_grad: a mask over {tk} positions has to hold the queries', {q_start} to "
+                         f"{q_start + tq - 1}")
+    dev = nat.require_device(g, mask)
+    g = _unit_rows(g)
+    out = torch.empty(b, num_buckets, h, dtype=torch.float32, device=dev)
+    lib = nat.load()
+    nbytes = ctypes.c_size_t(0)
+    nat.check(lib.da_relative_bias_grad_workspace(b, h, tq, tk, num_buckets, ctypes.byref(nbytes)), "relative_bias_grad")
+    ws = nat.workspace(nbytes.value, dev)
+    sb, sh, si, _ = g.stride()
+    _run_on(dev, "relative_bias_grad", lib.da_relative_bias_grad,
+            g.data_ptr(), code, b, h, tq, tk, sb, sh, si, int(q_start), edges, len(edges),
+            int(bool(bidirectional)), int(bool(causal)), mask_ptr, mask_b, mask_k, out.data_ptr(), ws.data_ptr(),
+            ws.numel(), nat.stream_ptr(dev))
+    return out
+
+
+def balance_loss(logits: torch.Tensor, index: torch.Tensor, *, batch: int = 1, mask=None):
+    """Router losses of ``batch`` samples of equally many tokens
+    (``da_balance_loss``): ``(loss (B,), z_loss (B,), counts (B, E) int32, live
+    (B,) int32)`` of ``(N, E)`` logits and the ``(N, k)`` int64 choices."""
+    if logits.dim() != 2 or index.dim() != 2 or index.shape[0] != logits.shape[0]:
+        raise ValueError("balance_loss expects (N, E) logits and (N, k) expert indices")
+    if index.dtype != torch.int64:
+        raise ValueError("balance_loss: expert indices must be int64")
+    n, e = logits.shape
+    if batch < 1 or n % batch:
+        raise ValueError(f"balance_loss: {n} tokens are not {batch} samples of one length")
+    code = nat.dtype_code(logits.dtype)
+    mask, mask_ptr, mask_b, mask_t = _token_mask("balance_loss", mask, batch, n // batch)
+    dev = nat.require_device(logits, index, mask)
+    logits, index = _unit_rows(logits), index.contiguous()
+    loss = torch.empty(2, batch, dtype=torch.float32, device=dev)
+    counts = torch.empty(batch, e, dtype=torch.int32, device=dev)
+    live = torch.empty(batch, dtype=torch.int32, device=dev)
+    lib = nat.load()
+    nbytes = ctypes.c_size_t(0)
+    nat.check(lib.da_balance_loss_workspace(batch, n // batch, e, ctypes.byref(nbytes)), "balance_loss")
+    ws = nat.workspace(nbytes.value, dev)
+    _run_on(dev, "balance_loss", lib.da_balance_loss,
+            logits.data_ptr(), code, batch, n // batch, e, logits.stride(0), index.data_ptr(),
+            index.shape[1], mask_ptr, mask_b, mask_t, loss.data_ptr(), loss.data_ptr() + 4 * batch, counts.data_ptr(),
+            live.data_ptr(), ws.data_ptr(), ws.numel(), nat.stream_ptr(dev))
+    return loss[0], loss[1], counts, live
+
+
+def _per_sample(what: str, v: torch.Tensor | None, batch: int):
+    if v is None:
+        return None
+    if tuple(v.shape) != (batch,):
+        raise ValueError(f"{what}: a loss gradient must have shape ({batch},), got {tuple(v.shape)}")
+    return v.to(torch.float32).contiguous()
+
+
+def balance_loss_grad(up, up_z, logits: torch.Tensor, counts: torch.Tensor, live: torch.Tensor, *,
+                      mask=None) -> torch.Tensor:
+    """Gradient of ``(N, E)`` logits for the gradients ``up`` and ``up_z`` (B,;
+    None: zero) of :func:`balance_loss`'s two losses, in the logits' dtype."""
+    if logits.dim() != 2 or counts.dim() != 2 or counts.shape[1] != logits.shape[1]:
+        raise ValueError("balance_loss_grad expects (N, E) logits and (B, E) counts")
+    n, e = logits.shape
+    batch = counts.shape[0]
+    if batch < 1 or n % batch or tuple(live.shape) != (batch,):
+        raise ValueError(f"balance_loss_grad: {n} tokens are not {batch} samples of one length")
+    if counts.dtype != torch.int32 or live.dtype != torch.int32:
+        raise ValueError("balance_loss_grad: counts and live must be int32, as balance_loss returns them")
+    up, up_z = _per_sample("balance_loss_grad", up, batch), _per_sample("balance_loss_grad", up_z, batch)
+    code = nat.dtype_code(logits.dtype)
+    mask, mask_ptr, mask_b, mask_t = _token_mask("balance_loss_grad", mask, batch, n // batch)
+    dev = nat.require_device(logits, counts, live, mask, up, up_z)
+    logits, counts, live = _unit_rows(logits), counts.contiguous(), live.contiguous()
+    grad = torch.empty(n, e, dtype=logits.dtype, device=dev)
+    _run_on(dev, "balance_loss_grad", nat.load().da_balance_loss_grad,
+            None if up is None else up.data_ptr(), None if up_z is None else up_z.data_ptr(), logits.data_ptr(),
+            code, batch, n // batch, e, logits.stride(0), counts.data_ptr(), live.data_ptr(),
+            mask_ptr, mask_b, mask_t, grad.data_ptr(), e, nat.stream_ptr(dev))
+    return grad

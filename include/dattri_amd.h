@@ -723,6 +723,114 @@ int da_match_rows(const void* src, int64_t n_src, int64_t src_rstride, const voi
                   void* stream);
 
 /*
+ * RMS norms of the queries and keys of each head with the position rotation.
+ *
+ * One side: rows x (batch, tokens, heads, d), entries contiguous, any other
+ * strides (elements); weight (d); out like x.  gz (the gradient of out) and
+ * weight_grad (batch, d) fp32 are the backward call's; weight_grad NULL leaves
+ * that sum out.  Per row, with r = (mean(x^2) + eps)^(-1/2):
+ *
+ *   y = x r weight;  for each pair (m, n) = (i, i + rot/2), interleaved
+ *   (2i, 2i+1), i < rot/2, at the angle position * inv_freq[i]:
+ *   out_m = scaling (y_m cos - y_n sin),  out_n = scaling (y_n cos + y_m sin);
+ *   entries from rot on: out = y.
+ *
+ * sides[0] are the queries, sides[1] the keys (their heads may differ; 0 heads:
+ * the side is absent).  positions: int32 or int64 (position_bytes 4 or 8) with
+ * strides in elements (0 broadcasts), NULL: the token's index.  mask: bytes,
+ * 0 marks a token whose rows of x and gz are not used, whose out is zero and
+ * which adds nothing to weight_grad; NULL: none.  d <= 1024, rot even, <= d.
+ * The angles are formed in fp64, everything else in fp32, rounded once.
+ *
+ * The backward call writes the gradient of x to out, and each sample's weight
+ * gradient sum over tokens and heads of dy x r (dy the gradient of y), the sum
+ * that da_norm_weight_grad forms for a norm whose output gradient is at hand;
+ * it takes a workspace from da_qk_norm_rope_grad_workspace.
+ */
+typedef struct da_qk_side {
+  const void* x;
+  const void* gz;
+  void* out;
+  const void* weight;
+  float* weight_grad;
+  int64_t heads;
+  int64_t x_bstride, x_tstride, x_hstride;
+  int64_t gz_bstride, gz_tstride, gz_hstride;
+  int64_t out_bstride, out_tstride, out_hstride;
+} da_qk_side;
+
+int da_qk_norm_rope(const da_qk_side* sides, int dtype, int weight_dtype, int64_t batch, int64_t tokens, int64_t d,
+                    int64_t rot, const float* inv_freq, const void* positions, int position_bytes,
+                    int64_t pos_bstride, int64_t pos_tstride, const uint8_t* mask, int64_t mask_bstride,
+                    int64_t mask_tstride, int interleaved, float scaling, float eps, void* stream);
+int da_qk_norm_rope_grad_workspace(int64_t batch, int64_t tokens, int64_t d, size_t* bytes);
+int da_qk_norm_rope_grad(const da_qk_side* sides, int dtype, int weight_dtype, int64_t batch, int64_t tokens,
+                         int64_t d, int64_t rot, const float* inv_freq, const void* positions, int position_bytes,
+                         int64_t pos_bstride, int64_t pos_tstride, const uint8_t* mask, int64_t mask_bstride,
+                         int64_t mask_tstride, int interleaved, float scaling, float eps, void* workspace,
+                         size_t workspace_bytes, void* stream);
+
+/*
+ * Relative position bias by buckets: out (heads, q_len, k_len), contiguous, in
+ * the table's dtype,
+ *
+ *   out[h,i,j] = table[bucket(j - i - q_start), h]
+ *
+ * with table (buckets, heads) at table_bstride / table_hstride (elements).  With
+ * distance r = |o| (bidirectional) or max(-o, 0) of the offset o, the bucket is
+ * the last x < side_buckets with edges[x] <= r (host array, edges[0] = 0,
+ * ascending), plus side_buckets where bidirectional and o > 0; at most 256 in
+ * all.  causal: -inf where o > 0.
+ *
+ * da_relative_bias_grad: the per-sample gradient (batch, buckets, heads), fp32,
+ *
+ *   out[b,v,h] = sum of g[b,h,i,j] over bucket(j - i - q_start) = v
+ *
+ * of g (batch, heads, q_len, k_len) with contiguous rows and any other strides
+ * (0 broadcasts).  causal: entries with j > i + q_start are not read.  mask
+ * (bytes, batch x k_len; query i is position i + q_start of it, which has to lie
+ * inside): entries of a dead query or key add nothing, whatever they hold.
+ * NULL: none.  The sums run in a fixed order.
+ */
+int da_relative_bias(const void* table, int dtype, int64_t table_bstride, int64_t table_hstride, int64_t heads,
+                     int64_t q_len, int64_t k_len, int64_t q_start, const int32_t* edges, int side_buckets,
+                     int bidirectional, int causal, void* out, void* stream);
+int da_relative_bias_grad_workspace(int64_t batch, int64_t heads, int64_t q_len, int64_t k_len, int buckets,
+                                    size_t* bytes);
+int da_relative_bias_grad(const void* g, int dtype, int64_t batch, int64_t heads, int64_t q_len, int64_t k_len,
+                          int64_t g_bstride, int64_t g_hstride, int64_t g_istride, int64_t q_start,
+                          const int32_t* edges, int side_buckets, int bidirectional, int causal, const uint8_t* mask,
+                          int64_t mask_bstride, int64_t mask_kstride, float* out, void* workspace,
+                          size_t workspace_bytes, void* stream);
+
+/*
+ * Router losses of each sample and their gradient.  logits (batch * tokens,
+ * experts) with row_stride; index (batch * tokens, top) int64, contiguous: the
+ * chosen experts (da_moe_topk's, say; an entry outside the experts counts for
+ * none, one that a row holds twice counts twice); mask bytes (batch, tokens),
+ * 0 a token that takes no part, NULL: none.  With n live tokens in sample b and
+ * p = softmax(logits):
+ *
+ *   counts[b,e] = live choices of e,   live[b] = n
+ *   loss[b] = experts * sum_e (counts[b,e] / n) mean(p_e)
+ *   z_loss[b] = mean(logsumexp(logits)^2)                        (0 where n = 0)
+ *
+ * The backward call writes the logits' gradient for the losses' gradients up
+ * and up_z (each (batch), NULL: zero); dead tokens' rows become zero.  The
+ * counts carry no gradient.  experts <= 1024.  Counts and sums do not depend on
+ * the order in which workgroups run.
+ */
+int da_balance_loss_workspace(int64_t batch, int64_t tokens, int experts, size_t* bytes);
+int da_balance_loss(const void* logits, int dtype, int64_t batch, int64_t tokens, int experts, int64_t row_stride,
+                    const int64_t* index, int top, const uint8_t* mask, int64_t mask_bstride, int64_t mask_tstride,
+                    float* loss, float* z_loss, int32_t* counts, int32_t* live, void* workspace,
+                    size_t workspace_bytes, void* stream);
+int da_balance_loss_grad(const float* up, const float* up_z, const void* logits, int dtype, int64_t batch,
+                         int64_t tokens, int experts, int64_t row_stride, const int32_t* counts, const int32_t* live,
+                         const uint8_t* mask, int64_t mask_bstride, int64_t mask_tstride, void* grad,
+                         int64_t grad_row_stride, void* stream);
+
+/*
  * Lane-layout self test of the MFMA conventions every kernel relies on.
  * shape 32: a and b are (32 x k) row-major with k = 16 (bf16/f16) or 8 (f32),
  *           one 16-byte chunk per lane half; out receives 64 lanes x 16

@@ -1,0 +1,283 @@
+"""CPU tests of the attention and router operators' host side: bucket borders,
+refused arguments (Python and C ABI), the capture's layer selection."""
+
+from __future__ import annotations
+
+import ctypes
+import math
+
+import pytest
+import torch
+from torch import nn
+
+from dattri_llm_amd import _native as nat
+from dattri_llm_amd import kernels
+from dattri_llm_amd.gradient import FusedCapture, QKNormRope, RelativeBias, ops
+
+
+def bucket(r: int, n: int, far: int) -> int:
+    """The definition, by whole numbers: distance r on one side of n buckets."""
+    m = n // 2
+    if r < m:
+        return r
+    j = 0
+    while j + 1 < n - m and r ** (n - m) * m ** (j + 1) >= far ** (j + 1) * m ** (n - m):
+        j += 1
+    return m + j
+
+
+@pytest.mark.parametrize("buckets,far,both", [(32, 128, True), (32, 128, False), (2, 5, False), (4, 3, True),
+                                              (256, 128, True), (256, 4096, False), (7, 100, False), (16, 9, False)])
+def test_bucket_edges_follow_the_definition(buckets, far, both):
+    edges = list(kernels._bucket_edges(buckets, far, both))
+    n = buckets // 2 if both else buckets
+    assert len(edges) == n and edges[0] == 0
+    for r in range(2 * far + 2):
+        assert max(x for x in range(n) if edges[x] <= r) == bucket(r, n, far), r
+
+
+def test_bucket_edges_match_the_logarithm_off_the_borders():
+    n, m, far = 16, 8, 128
+    edges = list(kernels._bucket_edges(2 * n, far, True))
+    for r in range(m, 4 * far):
+        x = math.log(r / m) / math.log(far / m) * (n - m)
+        if abs(x - round(x)) > 1e-9:
+            want = min(n - 1, m + math.floor(x))
+            assert max(i for i in range(n) if edges[i] <= r) == want, r
+
+
+@pytest.mark.parametrize("args", [(1, 128, False), (2, 128, True), (33, 128, True), (257, 128, False), (32, 8, True),
+                                  (32, 16, False), (32, (1 << 30) + 1, True)])
+def test_bucket_edges_refuse(args):
+    with pytest.raises(ValueError, match="relative bias"):
+        kernels._bucket_edges(*args)
+
+
+def qk_args(**change):
+    a = dict(q=torch.zeros(2, 3, 4, 8), k=torch.zeros(2, 3, 2, 8), q_weight=torch.ones(8), k_weight=torch.ones(8),
+             inv_freq=torch.ones(4), positions=None)
+    opts = {k: change.pop(k) for k in ("mask",) if k in change}
+    a.update(change)
+    return a, opts
+
+
+@pytest.mark.parametrize("change,words", [
+    (dict(q=torch.zeros(2, 3, 8)), "B, T, heads, D"),
+    (dict(k=torch.zeros(2, 4, 2, 8)), "disagree"),
+    (dict(k=torch.zeros(2, 3, 2, 16)), "disagree"),
+    (dict(q_weight=torch.ones(4)), "norm weight"),
+    (dict(k_weight=None), "norm weight"),
+    (dict(k=torch.zeros(2, 3, 2, 8).half()), "dtype"),
+    (dict(k_weight=torch.ones(8).half()), "dtype"),
+    (dict(inv_freq=torch.ones(5)), "rotate 10"),
+    (dict(inv_freq=torch.ones(4).double()), "float32"),
+    (dict(positions=torch.zeros(2, 3)), "int32 or int64"),
+    (dict(positions=torch.zeros(4, dtype=torch.int64)), "positions must have shape"),
+    (dict(mask=torch.ones(2, 4, dtype=torch.bool)), "mask must have shape"),
+])
+def test_qk_norm_rope_refuses(change, words):
+    a, opts = qk_args(**change)
+    with pytest.raises(ValueError, match=words):
+        ops.qk_norm_rope(**a, **opts)
+    with pytest.raises(ValueError, match=words):
+        ops.qk_norm_rope_grad(a["q"], a["k"], **a, **opts)
+
+
+def test_qk_norm_rope_refuses_types_gradients_and_the_cpu():
+    a, _ = qk_args()
+    with pytest.raises(NotImplementedError, match="float64"):
+        ops.qk_norm_rope(**{k: v.double() if k in "qk" else v for k, v in a.items()})
+    with pytest.raises(ValueError, match="one output gradient"):
+        ops.qk_norm_rope_grad(a["q"], None, **a)
+    with pytest.raises(ValueError, match="gradient of shape"):
+        ops.qk_norm_rope_grad(a["k"], a["k"], **a)
+    with pytest.raises(nat.NativeLibraryError, match="ROCm GPU"):
+        ops.qk_norm_rope(**a)
+
+
+def test_relative_bias_refuses():
+    table, g = torch.zeros(32, 4), torch.zeros(2, 4, 5, 9)
+    with pytest.raises(ValueError, match="table"):
+        ops.relative_bias(table[0], 5, 5)
+    with pytest.raises(ValueError, match="negative"):
+        ops.relative_bias(table, -1, 5)
+    with pytest.raises(ValueError, match="need batch"):
+        ops.relative_bias(table, 5, 5, mask=torch.ones(2, 5))
+    with pytest.raises(NotImplementedError):
+        ops.relative_bias(table.double(), 5, 5)
+    with pytest.raises(ValueError, match="gradient"):
+        ops.relative_bias_grad(g[0], 32)
+    with pytest.raises(ValueError, match="mask must have shape"):
+        ops.relative_bias_grad(g, 32, mask=torch.ones(2, 5))
+    for start in (-1, 5):
+        with pytest.raises(ValueError, match="hold the queries"):
+            ops.relative_bias_grad(g, 32, q_start=start, mask=torch.ones(2, 9))
+    for call in (lambda: ops.relative_bias(table, 5, 5), lambda: ops.relative_bias_grad(g, 32)):
+        with pytest.raises(nat.NativeLibraryError, match="ROCm GPU"):
+            call()
+
+
+def test_balance_loss_refuses():
+    x, i = torch.zeros(6, 4), torch.zeros(6, 2, dtype=torch.int64)
+    counts, live = torch.zeros(2, 4, dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
+    for bad, words in ((lambda: ops.moe.balance_loss(x, i[:5]), "expert indices"),
+                       (lambda: ops.moe.balance_loss(x[0], i), "expects"),
+                       (lambda: ops.moe.balance_loss_grad(None, None, x[0], counts, live), "expects"),
+                       (lambda: ops.moe.balance_loss(x, i.int()), "int64"),
+                       (lambda: ops.moe.balance_loss(x, i, batch=4), "samples of one length"),
+                       (lambda: ops.moe.balance_loss(x, i, batch=0), "samples of one length"),
+                       (lambda: ops.moe.balance_loss(x.view(2, 3, 4), i, batch=3), "batch 3"),
+                       (lambda: ops.moe.balance_loss(x, i, batch=2, mask=torch.ones(3, 2)), "mask must have shape"),
+                       (lambda: ops.moe.balance_loss_grad(None, None, x, counts[:, :3], live), "counts"),
+                       (lambda: ops.moe.balance_loss_grad(None, None, x, counts, live[:1]), "samples of one length"),
+                       (lambda: ops.moe.balance_loss_grad(None, None, x, counts.long(), live), "int32"),
+                       (lambda: ops.moe.balance_loss_grad(torch.ones(3), None, x, counts, live), "loss gradient")):
+        with pytest.raises(ValueError, match=words):
+            bad()
+    with pytest.raises(NotImplementedError):
+        ops.moe.balance_loss(x.double(), i)
+    with pytest.raises(nat.NativeLibraryError, match="ROCm GPU"):
+        ops.moe.balance_loss(x, i)
+
+
+X, OUT = 0x10000, 0x20000  # aligned placeholders, never dereferenced
+
+
+def refused(status, code, *words):
+    msg = nat.load().da_last_error().decode()
+    assert status == code and all(w in msg for w in words), (status, msg)
+
+
+def test_c_abi_qk_norm_rope_checks():
+    lib = nat.load()
+    sides = (nat.QkSide * 2)()
+    for s in sides:
+        s.x = s.gz = s.out = s.weight = X
+        s.weight_grad = X
+        s.heads = 2
+
+    def call(sides=sides, dt=2, wdt=0, b=2, t=3, d=8, rot=8, freq=X, pos=None, pos_bytes=0):
+        return lib.da_qk_norm_rope(sides, dt, wdt, b, t, d, rot, freq, pos, pos_bytes, 0, 1, None, 0, 0, 0, 1.0, 1e-6,
+                                   None)
+
+    refused(call(dt=9), nat.DA_ERR_INVALID, "dtype")
+    refused(call(sides=None), nat.DA_ERR_INVALID, "NULL sides")
+    refused(call(b=-1), nat.DA_ERR_INVALID, "negative")
+    refused(call(d=0, rot=0), nat.DA_ERR_UNSUPPORTED, "head width")
+    refused(call(d=1025), nat.DA_ERR_UNSUPPORTED, "head width")
+    refused(call(rot=3), nat.DA_ERR_INVALID, "even")
+    refused(call(rot=10), nat.DA_ERR_INVALID, "at most")
+    refused(call(freq=None), nat.DA_ERR_INVALID, "inv_freq")
+    refused(call(pos=X, pos_bytes=2), nat.DA_ERR_INVALID, "4 or 8")
+    assert call(b=0) == nat.DA_OK and call(t=0) == nat.DA_OK
+    sides[1].x = None
+    refused(call(), nat.DA_ERR_INVALID, "NULL pointer of side 1")
+    sides[1].x = X
+
+    def back(ws=None, n=0):
+        return lib.da_qk_norm_rope_grad(sides, 2, 0, 2, 3, 8, 8, X, None, 0, 0, 1, None, 0, 0, 0, 1.0, 1e-6, ws, n,
+                                        None)
+
+    refused(back(), nat.DA_ERR_WORKSPACE, "needed")
+    refused(back(X, 16), nat.DA_ERR_WORKSPACE, "needed")
+    sides[0].gz = None
+    refused(back(X, 1 << 20), nat.DA_ERR_INVALID, "NULL pointer of side 0")
+    refused(lib.da_qk_norm_rope_grad_workspace(1, 1, 8, None), nat.DA_ERR_INVALID, "argument")
+
+
+def test_c_abi_relative_bias_checks():
+    lib = nat.load()
+    edges = (ctypes.c_int32 * 4)(0, 1, 2, 9)
+    down = (ctypes.c_int32 * 4)(0, 2, 1, 9)
+    late = (ctypes.c_int32 * 4)(1, 2, 3, 9)
+
+    def fwd(dt=2, h=2, tq=3, tk=3, start=0, e=edges, n=4, table=X):
+        return lib.da_relative_bias(table, dt, 2, 1, h, tq, tk, start, e, n, 0, 0, OUT, None)
+
+    refused(fwd(dt=7), nat.DA_ERR_INVALID, "dtype")
+    refused(fwd(tq=-1), nat.DA_ERR_INVALID, "negative")
+    refused(fwd(start=1 << 31), nat.DA_ERR_UNSUPPORTED, "lengths")
+    refused(fwd(h=70000), nat.DA_ERR_UNSUPPORTED, "heads")
+    refused(fwd(n=0), nat.DA_ERR_UNSUPPORTED, "buckets")
+    refused(fwd(n=257), nat.DA_ERR_UNSUPPORTED, "buckets")
+    refused(fwd(e=None), nat.DA_ERR_UNSUPPORTED, "buckets")
+    refused(fwd(e=down), nat.DA_ERR_INVALID, "ascend")
+    refused(fwd(e=late), nat.DA_ERR_INVALID, "must be 0")
+    refused(fwd(table=None), nat.DA_ERR_INVALID, "NULL")
+    assert fwd(tq=0) == nat.DA_OK
+
+    def bwd(g=X, mask=None, start=0, out=OUT, ws=None, n=0, b=2):
+        return lib.da_relative_bias_grad(g, 2, b, 2, 3, 3, 18, 9, 3, start, edges, 4, 0, 0, mask, 3, 1, out, ws, n,
+                                         None)
+
+    refused(bwd(), nat.DA_ERR_WORKSPACE, "needed")
+    refused(bwd(g=None), nat.DA_ERR_INVALID, "NULL g")
+    refused(bwd(out=None), nat.DA_ERR_INVALID, "NULL out")
+    refused(bwd(mask=X, start=1), nat.DA_ERR_INVALID, "among them")
+    assert bwd(b=0) == nat.DA_OK
+
+
+def test_c_abi_balance_loss_checks():
+    lib = nat.load()
+
+    def fwd(dt=0, b=2, t=3, e=4, logits=X, index=X, top=2, loss=OUT, ws=None, n=0):
+        return lib.da_balance_loss(logits, dt, b, t, e, 4, index, top, None, 0, 0, loss, OUT, OUT, OUT, ws, n, None)
+
+    refused(fwd(dt=5), nat.DA_ERR_INVALID, "dtype")
+    refused(fwd(b=-1), nat.DA_ERR_INVALID, "negative")
+    refused(fwd(e=0), nat.DA_ERR_UNSUPPORTED, "experts")
+    refused(fwd(e=1025), nat.DA_ERR_UNSUPPORTED, "experts")
+    refused(fwd(top=-1), nat.DA_ERR_INVALID, "negative")
+    refused(fwd(logits=None), nat.DA_ERR_INVALID, "NULL")
+    refused(fwd(index=None), nat.DA_ERR_INVALID, "NULL")
+    refused(fwd(loss=None), nat.DA_ERR_INVALID, "NULL")
+    refused(fwd(t=100_000), nat.DA_ERR_WORKSPACE, "needed")
+    assert fwd(b=0) == nat.DA_OK
+
+    def bwd(counts=X, t=3):
+        return lib.da_balance_loss_grad(X, X, X, 0, 2, t, 4, 4, counts, X, None, 0, 0, OUT, 4, None)
+
+    refused(bwd(counts=None), nat.DA_ERR_INVALID, "NULL")
+    assert bwd(t=0) == nat.DA_OK
+
+
+class Block(nn.Module):
+    def __init__(self):
+        super().__init__()
+        self.rope = QKNormRope(8)
+        self.bias = RelativeBias(8, 2)
+        self.out = nn.Linear(8, 8)
+        self.act = nn.ReLU()
+
+
+def test_capture_selects_the_modules_by_type_and_name():
+    m = Block()
+    cap = FusedCapture(m)
+    assert cap.types == {"rope.q_weight": "nn.RMSNorm", "rope.k_weight": "nn.RMSNorm", "bias": "nn.Embedding",
+                         "out": "nn.Linear"}
+    assert list(FusedCapture(m, ["rope"]).slots) == ["rope.q_weight", "rope.k_weight"]
+    assert list(FusedCapture(m, ["bias", "out"]).slots) == ["bias", "out"]
+    with pytest.raises(ValueError, match="ReLU"):
+        FusedCapture(m, ["act"])
+    with pytest.raises(ValueError, match="no such layers"):
+        FusedCapture(m, ["rope", "gone"])
+    with pytest.raises(RuntimeError, match="no layer"):
+        cap.gradient()
+    with cap:
+        with pytest.raises(ValueError, match="needs batch"):
+            m.bias(4, 4)
+    assert "forward" not in m.bias.__dict__ and "forward" not in m.rope.__dict__
+    with FusedCapture(m, batch_first=False):
+        with pytest.raises(ValueError, match="batch first"):
+            m.rope(torch.zeros(1, 2, 1, 8), None)
+
+
+def test_modules_keep_their_frequencies_in_fp32():
+    m = QKNormRope(16, rotary_dim=8, base=100.0)
+    want = torch.tensor([100.0 ** (-i / 8) for i in range(0, 8, 2)])
+    assert torch.equal(m.inv_freq, want)
+    m.to(torch.bfloat16)
+    assert m.inv_freq.dtype == torch.float32 and torch.equal(m.inv_freq, want) and m.q_weight.dtype == torch.bfloat16
+    for bad in (3, 18, -2):
+        with pytest.raises(ValueError, match="rotary_dim"):
+            QKNormRope(16, rotary_dim=bad)
