@@ -220,7 +220,8 @@ SIGNATURES.update(
         "da_qk_norm_rope_grad": (_I32, [*_QK, _P, _SZ, _P]),
         "da_relative_bias": (
             _I32, [_P, _I32, _I64, _I64, _I64, _I64, _I64, _I64, _EDGES, _I32, _I32, _I32, _P, _P]),
-        "da_relative_bias_grad_workspace": (_I32, [_I64, _I64, _I64, _I64, _I32, ctypes.POINTER(_SZ)]),
+        "da_relative_bias_grad_workspace": (
+            _I32, [_I32, _I64, _I64, _I64, _I64, _I64, _I32, _I32, ctypes.POINTER(_SZ)]),
         "da_relative_bias_grad": (
             _I32, [_P, _I32, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _EDGES, _I32, _I32, _I32, _P, _I64, _I64,
                    _P, _P, _SZ, _P]),

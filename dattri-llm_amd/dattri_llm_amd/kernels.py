@@ -1669,7 +1669,8 @@ def relative_bias_grad(g: torch.Tensor, num_buckets: int, *, q_start: int = 0, b
     out = torch.empty(b, num_buckets, h, dtype=torch.float32, device=dev)
     lib = nat.load()
     nbytes = ctypes.c_size_t(0)
-    nat.check(lib.da_relative_bias_grad_workspace(b, h, tq, tk, num_buckets, ctypes.byref(nbytes)), "relative_bias_grad")
+    nat.check(lib.da_relative_bias_grad_workspace(code, b, h, tq, tk, int(q_start), num_buckets, int(bool(causal)),
+                                                  ctypes.byref(nbytes)), "relative_bias_grad")
     ws = nat.workspace(nbytes.value, dev)
     sb, sh, si, _ = g.stride()
     _run_on(dev, "relative_bias_grad", lib.da_relative_bias_grad,

@@ -206,13 +206,14 @@ def test_c_abi_relative_bias_checks():
     refused(fwd(table=None), nat.DA_ERR_INVALID, "NULL")
     assert fwd(tq=0) == nat.DA_OK
 
-    def bwd(g=X, mask=None, start=0, out=OUT, ws=None, n=0, b=2):
-        return lib.da_relative_bias_grad(g, 2, b, 2, 3, 3, 18, 9, 3, start, edges, 4, 0, 0, mask, 3, 1, out, ws, n,
-                                         None)
+    def bwd(g=X, mask=None, start=0, out=OUT, ws=None, n=0, b=2, stride=999):
+        return lib.da_relative_bias_grad(g, 2, b, 2, 999, 999, 2 * 999 * 999, stride * 999, stride, start, edges, 4, 0, 0,
+                                         mask, 999, 1, out, ws, n, None)
 
     refused(bwd(), nat.DA_ERR_WORKSPACE, "needed")
     refused(bwd(g=None), nat.DA_ERR_INVALID, "NULL g")
     refused(bwd(out=None), nat.DA_ERR_INVALID, "NULL out")
+    refused(bwd(stride=-8), nat.DA_ERR_INVALID, "negative stride")
     refused(bwd(mask=X, start=1), nat.DA_ERR_INVALID, "among them")
     assert bwd(b=0) == nat.DA_OK
 
