@@ -56,6 +56,21 @@ struct Walk {
   static constexpr int kLine = (kWave + 2) * V;  // offsets of a wave's 64 diagonal blocks
   __host__ __device__ static constexpr int shift(int e) { return e * R % V; }
   __host__ __device__ static constexpr int at(int e, int x) { return x - e - shift(e) + 2 * (V - 1); }
+  __host__ __device__ static constexpr int end(bool last) {
+    int t = last ? 0 : 3 * V;
+    for (int e = 0; e < V; ++e) {
+      const int u = at(e, last ? V - 1 : 0);
+      if (last ? u > t : u < t) t = u;
+    }
+    return t;
+  }
+  static constexpr int kFirst = end(false), kLast = end(true);  // the places in use
+  // Bit x: a run may reach column first - (V - 1) + x (first: of an unshifted run).
+  __host__ __device__ static constexpr int columns() {
+    int bits = 0;
+    for (int e = 0; e < V; ++e) bits |= ((1 << V) - 1) << (V - 1 - shift(e));
+    return bits;
+  }
 };
 
 // Offsets o that belong to a bucket: one range each.
@@ -164,134 +179,215 @@ struct GradArgs {
   int64_t mask_b, mask_k;
   int64_t blocks;  // workgroups of a plane
   int buckets, start, causal;
-  int row_blocks, first_block, last_block;
-  int windows, splits, steps;
+  int row_blocks, last_block;  // row blocks; the last diagonal block that counts
+  int windows, steps;          // groups of column blocks; row blocks of a group
 };
 
-constexpr int kMaxSteps = 512;  // row blocks of a workgroup at most: its mask bits lie in LDS
+// Row blocks of a group of lanes at most (even): its sums lie in LDS.
+__host__ __device__ constexpr int max_steps(int group) { return group == 64 ? 64 : 16; }
 
-// A workgroup sums 64 diagonal blocks of one plane over a part of its rows; its
-// waves take row blocks in turn.  Their 3V - 2 sums a lane meet in LDS, lane by
-// lane in three steps (a lane's offsets overlap its neighbours'), and each
-// bucket's range of offsets is then summed by one wave.
-template <int DT, int R>
+__device__ const u32x4 kZeros = {0, 0, 0, 0};
+
+// Whole-wave (kG 64) or row-of-16 shift by one lane: lane l takes lane l - 1's
+// value, the first lane of a group zero.
+template <int kG>
+__device__ __forceinline__ float from_left(float v) {
+  constexpr int kCtrl = kG == 64 ? 0x138 : 0x111;  // wave_shr:1, row_shr:1
+  return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), kCtrl, 0xf, 0xf, false));
+}
+
+// A group of kG lanes owns kG column blocks and walks down `steps` row blocks of
+// one plane.  A lane's column stays while its diagonal moves one block left with
+// each row block, so its sums move one lane right: every load of the walk is
+// whole lines, all lanes work, and all groups alike.  The sums of the diagonal
+// block that leaves at the last lane go to its slot in LDS, at the end those of
+// all lanes.  An offset lies in up to three slots of each group; their sums form the
+// workgroup's line, and sixteen lanes sum a bucket's range of it.
+template <int DT, int R, int kG>
 __global__ __launch_bounds__(kThreads) void bias_backward(GradArgs a, Edges e) {
-  constexpr int V = Elem<DT>::kVec, ES = Elem<DT>::kBytes;
+  constexpr int V = Elem<DT>::kVec, ES = Elem<DT>::kBytes, kGroups = kThreads / kG;
   using W = Walk<V, R>;
-  __shared__ float line[kWaves][W::kLine];
-  __shared__ uint8_t live_cols[kMaxSteps + kWave + 1], live_rows[kMaxSteps];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  constexpr int kSums = W::kLast - W::kFirst + 1, kSlot = (kSums + 3) / 4 * 4;
+  extern __shared__ __attribute__((aligned(16))) float slots[];  // [kGroups][steps + kG][kSlot]
+  __shared__ int ranges[kMaxBuckets][2];
+  __shared__ uint8_t live_rows[kGroups * max_steps(kG)];
+  const int tid = threadIdx.x, l = tid % kG, group = tid / kG;
   const int window = blockIdx.x % a.windows, split = blockIdx.x / a.windows;
   const int64_t h = blockIdx.y, b = blockIdx.z;
   const char* plane = a.g + (b * a.g_b + h * a.g_h) * ES;
   const int mis = (int)((uintptr_t)plane / ES % V);
-  const int k0 = a.first_block + window * kWave, k = k0 + lane;
   const int k_len = (int)a.k_len, q_len = (int)a.q_len;
-  // Row blocks where some lane's column block holds an entry of a row.
-  const int r0 = max(split * a.steps, 1 - kWave - k0);
-  const int r1 = min(min((split + 1) * a.steps, a.row_blocks), (k_len + mis + 2 * V - 2) / V - k0);
+  const int c = window * kG + l;  // column block
+  const int first = c * V - mis;  // column of its unshifted run
+  const int begin = split * kGroups * a.steps;
+  const int r0 = begin + group * a.steps, r1 = min(r0 + a.steps, a.row_blocks);
+  float* mine = slots + group * (a.steps + kG) * kSlot;
+  for (int p = l; p < a.steps * kSlot; p += kG) mine[p] = 0.f;
+  if (tid < a.buckets) {
+    bucket_range(e, tid, &ranges[tid][0], &ranges[tid][1]);
+    if (a.causal) ranges[tid][1] = min(ranges[tid][1], 0);
+  }
+  // Bit x: column first - (V - 1) + x is there and live.
+  constexpr int kAll = W::columns(), kRows = (1 << V) - 1;
+  const int lo = min(max(V - 1 - first, 0), 2 * V - 1), hi = min(max(k_len - first + V - 1, 0), 2 * V - 1);
+  int cols = ((1 << hi) - 1) & ~((1 << lo) - 1);
+  bool dead_row = false;
   if (a.mask) {
     const uint8_t* m = a.mask + b * a.mask_b;
-    for (int n = tid; n < r1 - r0 + kWave; n += kThreads) {  // column blocks r0 + k0 - 1 ...
-      const int64_t j0 = (int64_t)(r0 + k0 - 1 + n) * V - mis;
-      int bits = 0;
-      for (int x = 0; x < V; ++x)
-        if (j0 + x >= 0 && j0 + x < k_len && m[(j0 + x) * a.mask_k]) bits |= 1 << x;
-      live_cols[n] = (uint8_t)bits;
-    }
-    for (int n = tid; n < r1 - r0; n += kThreads) {
-      int bits = 0;
-      for (int x = 0; x < V; ++x) {
-        const int64_t i = (int64_t)(r0 + n) * V + x;
-        if (i < q_len && m[(i + a.start) * a.mask_k]) bits |= 1 << x;
-      }
+    int bits = 0;
+#pragma unroll
+    for (int x = 0; x < 2 * V - 1; ++x)  // places past the ends read an end: cols has no bit there
+      bits |= (m[min(max(first - (V - 1) + x, 0), k_len - 1) * a.mask_k] != 0) << x;
+    cols &= bits;
+    for (int n = tid; n < kGroups * a.steps; n += kThreads) {
+      bits = 0;
+#pragma unroll
+      for (int x = 0; x < V; ++x) bits |= (m[(min((begin + n) * V + x, q_len - 1) + a.start) * a.mask_k] != 0) << x;
       live_rows[n] = (uint8_t)bits;
+      dead_row |= bits != kRows;
     }
-    __syncthreads();
   }
-  float sum[3 * V - 2];
-#pragma unroll
-  for (int t = 0; t < 3 * V - 2; ++t) sum[t] = 0.f;
+  dead_row = __syncthreads_or(dead_row);
   const int64_t plane_end = (int64_t)(q_len - 1) * a.g_i + k_len;
-  for (int r = r0 + wave; r < r1; r += kWaves) {
-    const int first = (r + k) * V - mis;
-    int rows = q_len - r * V >= V ? (1 << V) - 1 : (1 << (q_len - r * V)) - 1;
-    // Bit x of cols: column first - (V - 1) + x is there (and live).
-    constexpr int kAll = (1 << (2 * V - 1)) - 1;
-    int cols = 0;
-    if (k <= a.last_block) {
-      const int lo = min(max(V - 1 - first, 0), 2 * V - 1), hi = min(max(k_len - first + V - 1, 0), 2 * V - 1);
-      cols = ((1 << hi) - 1) & ~((1 << lo) - 1);
-      if (a.mask) cols &= (live_cols[r - r0 + lane] | live_cols[r - r0 + lane + 1] << V) >> 1;
-    }
-    if (a.mask) rows = __builtin_amdgcn_readfirstlane(live_rows[r - r0]);
-    if (!__any(cols) || !rows) continue;
-    u32x4 v[V];
+
+  float sum[kSlot];
+#pragma unroll
+  for (int t = 0; t < kSlot; ++t) sum[t] = 0.f;
+
+  // The lane's runs of row block r: every entry there, live and counted.
+  auto load_whole = [&](u32x4 (&v)[V], int r) {
+    const char* at = plane + ((int64_t)(r * V) * a.g_i + first) * ES;
+#pragma unroll
+    for (int x = 0; x < V; ++x)
+      v[x] = __builtin_nontemporal_load((const u32x4*)(at + (x * a.g_i - W::shift(x)) * ES));
+  };
+  auto add_whole = [&](const u32x4 (&v)[V]) {
 #pragma unroll
     for (int x = 0; x < V; ++x) {
-      v[x] = u32x4{0, 0, 0, 0};
-      if (!(rows >> x & 1)) continue;
-      const int64_t at = (int64_t)(r * V + x) * a.g_i + first - W::shift(x);
-      const int here = cols >> (V - 1 - W::shift(x)) & ((1 << V) - 1);  // the run's live entries
-      if (here) {
-        if (at >= 0 && at + V <= plane_end) v[x] = ld16(plane + at * ES);
-        else {  // the plane's first or last run sticks out of it
+      float f[V];
+      unpack16<DT>(v[x], f);
 #pragma unroll
-          for (int q = 0; q < V; ++q)
-            if (here >> q & 1) v[x][q * ES / 4] |= load_bits<ES>(plane, at + q) << (ES == 2 ? q % 2 * 16 : 0);
-        }
-      }
+      for (int q = 0; q < V; ++q) sum[W::at(x, q) - W::kFirst] += f[q];
     }
-    if (__all(cols == kAll)) {
-#pragma unroll
-      for (int x = 0; x < V; ++x) {
-        float f[V];
-        unpack16<DT>(v[x], f);
-#pragma unroll
-        for (int q = 0; q < V; ++q) sum[W::at(x, q)] += f[q];
-      }
-    } else {
-#pragma unroll
-      for (int x = 0; x < V; ++x) {
-        float f[V];
-        unpack16<DT>(v[x], f);
-#pragma unroll
-        for (int q = 0; q < V; ++q) sum[W::at(x, q)] += cols >> (V - 1 - W::shift(x) + q) & 1 ? f[q] : 0.f;
-      }
-    }
-  }
-  float* mine = line[wave];
-#pragma unroll
-  for (int step = 0; step < 3; ++step) {
+  };
+  // Any row block: a run without a live entry, or one that sticks out of the
+  // plane (its entries are added one by one), reads zeros instead.
+  auto rows_of = [&](int r) {
+    int rows = r >= r1 || c - r > a.last_block ? 0 : q_len - r * V >= V ? kRows : (1 << (q_len - r * V)) - 1;
+    if (a.mask && r < r1) rows &= live_rows[r - begin];
+    return rows;
+  };
+  auto load_some = [&](u32x4 (&v)[V], int r) {
+    const int rows = rows_of(r);
+    const int64_t at0 = (int64_t)(r * V) * a.g_i + first;
 #pragma unroll
     for (int x = 0; x < V; ++x) {
-      const int t = step * V + x;
-      const float u = t < 3 * V - 2 ? sum[t < 3 * V - 2 ? t : 0] : 0.f;
-      const int p = (lane + step) * V + x;
-      // The last `step` blocks of the line are met for the first time.
-      mine[p] = step == 0 || lane == kWave - 1 ? u : mine[p] + u;
+      const int64_t at = at0 + x * a.g_i - W::shift(x);
+      const bool ok = rows >> x & 1 && (cols >> (V - 1 - W::shift(x)) & kRows) && at >= 0 && at + V <= plane_end;
+      v[x] = *(ok ? (const u32x4*)(plane + at * ES) : &kZeros);
     }
-    __syncthreads();
-  }
-  for (int p = tid; p < W::kLine; p += kThreads) {
-    float u = line[0][p];
+  };
+  auto add_some = [&](u32x4 (&v)[V], int r) {
+    int keep_cols = cols;
+    asm volatile("" : "+v"(keep_cols));  // its masks are made here, not held through the loop
 #pragma unroll
-    for (int w = 1; w < kWaves; ++w) u += line[w][p];
-    line[0][p] = u;
+    for (int x = 0; x < V; ++x)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {  // entries that are not there, or dead, to zero bits
+        const int at = V - 1 - W::shift(x) + q * 4 / ES;
+        uint32_t keep = keep_cols >> at & 1 ? ~0u : 0u;
+        if constexpr (ES == 2) keep = (keep & 0xffffu) | (keep_cols >> (at + 1) & 1 ? 0xffff0000u : 0u);
+        v[x][q] &= keep;
+      }
+    add_whole(v);
+    // Only a plane's first and last row block, or rows closer than two runs, reach out of it.
+    if (r > 0 && r < a.row_blocks - 1 && a.g_i >= 2 * V) return;
+    const int rows = rows_of(r);
+#pragma unroll
+    for (int x = 0; x < V; ++x) {
+      const int64_t at = ((int64_t)(r * V) + x) * a.g_i + first - W::shift(x);
+      if (rows >> x & 1 && (at < 0 || at + V > plane_end)) {
+#pragma unroll
+        for (int q = 0; q < V; ++q)
+          if (cols >> (V - 1 - W::shift(x) + q) & 1) sum[W::at(x, q) - W::kFirst] += Elem<DT>::load(plane, at + q);
+      }
+    }
+  };
+  // On to row block r0 + step + 1.  Diagonal block c - r lies in slot l + steps - 1 - step.
+  auto next = [&](int step) {
+    if (l == kG - 1) {
+      f32x4* out = (f32x4*)(mine + (a.steps - 1 - step + l) * kSlot);
+#pragma unroll
+      for (int t = 0; t < kSlot; t += 4) out[t / 4] = f32x4{sum[t], sum[t + 1], sum[t + 2], sum[t + 3]};
+    }
+#pragma unroll
+    for (int t = 0; t < kSums; ++t) sum[t] = from_left<kG>(sum[t]);
+  };
+
+  // Row blocks whose diagonal blocks are all past the last are left out.
+  const int count = (max(r1 - r0, 0) + 1) & ~1;
+  int step = min(max(window * kG - a.last_block - r0, 0) & ~1, count);
+  const bool whole = !dead_row && __all((cols & kAll) == kAll && r1 * V <= q_len && count == r1 - r0 &&
+                                        c - (r0 + step) <= a.last_block);
+  for (int s = 0; s < step; ++s)  // slots that no row block reaches
+    if (l == kG - 1)
+#pragma unroll
+      for (int t = 0; t < kSlot; ++t) mine[(a.steps - 1 - s + l) * kSlot + t] = 0.f;
+  u32x4 v0[V], v1[V];
+  if (whole) {
+    if (step < count) load_whole(v0, r0 + step);
+    for (; step < count; step += 2) {
+      load_whole(v1, r0 + step + 1);
+      add_whole(v0);
+      next(step);
+      if (step + 2 < count) load_whole(v0, r0 + step + 2);
+      add_whole(v1);
+      next(step + 1);
+    }
+  } else {
+    load_some(v0, r0 + step);
+    for (; step < count; step += 2) {
+      load_some(v1, r0 + step + 1);
+      add_some(v0, r0 + step);
+      next(step);
+      load_some(v0, r0 + step + 2);
+      add_some(v1, r0 + step + 1);
+      next(step + 1);
+    }
+  }
+  // Before row block r0 + count the lanes from 1 on hold diagonal blocks.
+  if (l > 0 || count < a.steps) {
+    float* out = mine + (a.steps - 1 - count + l) * kSlot;
+#pragma unroll
+    for (int t = 0; t < kSlot; ++t) out[t] = sum[t];
   }
   __syncthreads();
-  const int o0 = k0 * V - 2 * (V - 1) - mis - a.start;  // the line's first offset
-  for (int x = wave; x < a.buckets; x += kWaves) {
-    int lo, hi;
-    bucket_range(e, x, &lo, &hi);
-    if (a.causal) hi = min(hi, 0);
-    lo = max(lo - o0, 0);
-    hi = min(hi - o0, W::kLine - 1);
+
+  // The workgroup's line of offsets: block 0 is the last group's first slot.
+  float* line = slots + kGroups * (a.steps + kG) * kSlot;
+  const int used = a.steps + kG - 1, blocks = (kGroups - 1) * a.steps + used, length = (blocks - 1) * V + kSums;
+  for (int p = tid; p < length; p += kThreads) {
+    const int k = p / V, t = p % V;
     float u = 0.f;
-    if (lo <= hi) {
-      for (int p = lo + lane; p <= hi; p += kWave) u += line[0][p];
-      u = wave_sum(u);
+#pragma unroll
+    for (int back = 0; back < 3; ++back) {
+      if (t + back * V >= kSums) continue;
+      int at = k - back - (kGroups - 1) * a.steps;
+#pragma unroll 4
+      for (int g = 0; g < kGroups; ++g, at += a.steps)
+        if (at >= 0 && at < used) u += slots[(g * (a.steps + kG) + at) * kSlot + t + back * V];
     }
+    line[p] = u;
+  }
+  __syncthreads();
+  const int lane = tid & 15;
+  const int o0 = (window * kG - (begin + kGroups * a.steps - 1)) * V + W::kFirst - 2 * (V - 1) - mis - a.start;
+  for (int x = tid >> 4; x < a.buckets; x += kThreads / 16) {
+    const int from = max(ranges[x][0] - o0, 0), to = min(ranges[x][1] - o0, length - 1);
+    float u = 0.f;
+    for (int p = from + lane; p <= to; p += 16) u += line[p];
+#pragma unroll
+    for (int off = 8; off > 0; off >>= 1) u += __shfl_xor(u, off, 16);
     if (lane == 0) {
       if (a.blocks == 1) a.out[(b * a.buckets + x) * a.heads + h] = u;
       else a.partial[((b * a.heads + h) * a.blocks + blockIdx.x) * a.buckets + x] = u;
@@ -340,28 +436,51 @@ constexpr int64_t kMaxLen = (int64_t)1 << 26;
 constexpr int64_t kWantBlocks = 1024;  // four workgroups for each CU
 
 struct Plan {
-  int row_blocks, first_block, last_block, windows, splits, steps;
+  int row_blocks, first_block, windows, splits, steps;
 };
 
-// Diagonal blocks run from the first column block against the last row block to
-// the last column block against the first (with `causal` to the last that holds
-// an offset up to 0), whatever the plane's misalignment.  The rows are split
-// until `planes` of them fill the card with `want` workgroups, each of at least
-// four row blocks a wave.
-Plan make_plan(int v, bool aligned, int64_t planes, int64_t q_len, int64_t k_len, int64_t start, bool causal) {
+// The forward pass: diagonal blocks run from the first column block against the
+// last row block to the last column block against the first; planes whose rows
+// are not all aligned reach further.  The rows are split until the planes fill the
+// card with kWantBlocks workgroups, each of at least four row blocks a wave.
+Plan make_plan(int v, bool aligned, int64_t planes, int64_t q_len, int64_t k_len) {
   Plan p;
   p.row_blocks = (int)((q_len + v - 1) / v);
   p.first_block = 1 - p.row_blocks;
   const int64_t slack = aligned ? 0 : v - 1;  // most that mis, and that a row's shift, can be
-  int64_t last = (k_len - 1 + 2 * slack) / v;
-  if (causal) last = std::min(last, std::max<int64_t>((start + v - 1 + 2 * slack) / v, p.first_block));
-  p.last_block = (int)last;
+  const int64_t last = (k_len - 1 + 2 * slack) / v;
   p.windows = (int)((last - p.first_block + kWave) / kWave);
   int64_t splits = (kWantBlocks + planes * p.windows - 1) / (planes * p.windows);
   splits = std::min<int64_t>(splits, (p.row_blocks + 4 * kWaves - 1) / (4 * kWaves));
-  splits = std::max<int64_t>(splits, (p.row_blocks + kMaxSteps - 1) / kMaxSteps);
   p.steps = (int)((p.row_blocks + splits - 1) / splits);
   p.splits = (p.row_blocks + p.steps - 1) / p.steps;
+  return p;
+}
+
+struct GradPlan {
+  int group, row_blocks, last_block, windows, splits, steps;
+};
+
+// Column blocks go to groups of lanes, row blocks to the groups of a workgroup
+// and, where the planes are few, to several workgroups.
+GradPlan grad_plan(int v, bool aligned, int64_t planes, int64_t q_len, int64_t k_len, int64_t start, bool causal) {
+  GradPlan p;
+  p.row_blocks = (int)((q_len + v - 1) / v);
+  const int64_t slack = aligned ? 0 : v - 1;
+  int64_t last = kMaxLen, columns = (k_len - 1 + 2 * slack) / v + 1;
+  if (causal) {
+    last = std::max<int64_t>((start + v - 1 + 2 * slack) / v, -p.row_blocks);
+    columns = std::max<int64_t>(std::min(columns, last + p.row_blocks), 1);
+  }
+  p.last_block = (int)last;
+  p.group = columns <= 16 ? 16 : 64;
+  const int groups = kThreads / p.group;
+  p.windows = (int)((columns + p.group - 1) / p.group);
+  int64_t steps = p.row_blocks * planes * p.windows / (kWantBlocks * groups);
+  steps = std::min<int64_t>(std::max<int64_t>(steps, 8), max_steps(p.group));
+  steps = std::min<int64_t>(steps, (p.row_blocks + groups - 1) / groups);
+  p.steps = (int)(steps + 1) & ~1;
+  p.splits = (p.row_blocks + groups * p.steps - 1) / (groups * p.steps);
   return p;
 }
 
@@ -390,9 +509,8 @@ int da_relative_bias(const void* table, int dtype, int64_t table_bstride, int64_
   if (!heads || !q_len || !k_len) return DA_OK;
   if (!table || !out) return set_error(DA_ERR_INVALID, "%s: NULL pointer", what);
   const int es = (int)elem_bytes(dtype), v = 16 / es;
-  // Every column block of a row is written: no diagonal block is left out.
   const bool aligned = (uintptr_t)out % 16 == 0 && k_len % v == 0;
-  const Plan p = make_plan(v, aligned, heads, q_len, k_len, q_start, false);
+  const Plan p = make_plan(v, aligned, heads, q_len, k_len);
   BiasArgs a{};
   a.table = (const char*)table, a.out = (char*)out, a.q_len = q_len, a.k_len = k_len, a.t_b = table_bstride;
   a.t_h = table_hstride, a.start = (int)q_start, a.causal = causal, a.row_blocks = p.row_blocks;
@@ -422,7 +540,7 @@ int da_relative_bias_grad_workspace(int dtype, int64_t batch, int64_t heads, int
   *bytes = 0;
   if (!batch || !heads || !q_len || !k_len) return DA_OK;
   for (int aligned = 0; aligned < 2; ++aligned) {
-    const Plan p = make_plan(dtype == DA_F32 ? 4 : 8, aligned, batch * heads, q_len, k_len, q_start, causal);
+    const GradPlan p = grad_plan(dtype == DA_F32 ? 4 : 8, aligned, batch * heads, q_len, k_len, q_start, causal);
     const int64_t blocks = (int64_t)p.windows * p.splits;
     if (blocks > 1) *bytes = std::max(*bytes, (size_t)(blocks * batch * heads * buckets) * sizeof(float));
   }
@@ -452,20 +570,25 @@ int da_relative_bias_grad(const void* g, int dtype, int64_t batch, int64_t heads
   const int v = dtype == DA_F32 ? 4 : 8;
   const bool aligned = (uintptr_t)g % 16 == 0 && g_istride % v == 0 && (heads == 1 || g_hstride % v == 0) &&
                        (batch == 1 || g_bstride % v == 0);
-  const Plan p = make_plan(v, aligned, batch * heads, q_len, k_len, q_start, causal);
+  const GradPlan p = grad_plan(v, aligned, batch * heads, q_len, k_len, q_start, causal);
   GradArgs a{};
   a.g = (const char*)g, a.mask = mask, a.out = out, a.heads = heads, a.q_len = q_len, a.k_len = k_len;
   a.start = (int)q_start, a.g_b = g_bstride, a.g_h = g_hstride, a.g_i = g_istride, a.mask_b = mask_bstride;
   a.mask_k = mask_kstride, a.buckets = buckets, a.causal = causal, a.row_blocks = p.row_blocks;
-  a.first_block = p.first_block, a.last_block = p.last_block, a.windows = p.windows, a.splits = p.splits;
-  a.steps = p.steps, a.blocks = (int64_t)p.windows * p.splits;
+  a.last_block = p.last_block, a.windows = p.windows, a.steps = p.steps;
+  a.blocks = (int64_t)p.windows * p.splits;
   const size_t need = a.blocks > 1 ? (size_t)(a.blocks * batch * heads * buckets) * sizeof(float) : 0;
   if (need && (!workspace || workspace_bytes < need))
     return set_error(DA_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", what, workspace_bytes, need);
   a.partial = (float*)workspace;
   const dim3 grid((unsigned)a.blocks, (unsigned)heads, (unsigned)batch);
-#define DA_BWD(DT, R) \
-  case R: bias_backward<DT, R><<<grid, kThreads, 0, st>>>(a, e); break;
+  const int groups = kThreads / p.group;
+  const size_t lds = (size_t)(groups * (p.steps + p.group) * 3 + groups * p.steps + p.group + 1) * v * sizeof(float);
+#define DA_BWD(DT, R)                                                                 \
+  case R:                                                                             \
+    if (p.group == 16) bias_backward<DT, R, 16><<<grid, kThreads, lds, st>>>(a, e);   \
+    else bias_backward<DT, R, 64><<<grid, kThreads, lds, st>>>(a, e);                 \
+    break;
 #define DA_BWD8(DT)                                                                                    \
   switch (g_istride % 8) {                                                                             \
     DA_BWD(DT, 0) DA_BWD(DT, 1) DA_BWD(DT, 2) DA_BWD(DT, 3) DA_BWD(DT, 4) DA_BWD(DT, 5) DA_BWD(DT, 6) \
