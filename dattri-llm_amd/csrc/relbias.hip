@@ -221,6 +221,14 @@ __global__ __launch_bounds__(kThreads) void bias_backward(GradArgs a, Edges e) {
   const int first = c * V - mis;  // column of its unshifted run
   const int begin = split * kGroups * a.steps;
   const int r0 = begin + group * a.steps, r1 = min(r0 + a.steps, a.row_blocks);
+  auto store = [&](int x, float u) {
+    if (a.blocks == 1) a.out[(b * a.buckets + x) * a.heads + h] = u;
+    else a.partial[((b * a.heads + h) * a.blocks + blockIdx.x) * a.buckets + x] = u;
+  };
+  if (window * kG - a.last_block >= begin + kGroups * a.steps) {  // causal: all keys follow the queries
+    if (tid < a.buckets) store(tid, 0.f);
+    return;
+  }
   float* mine = slots + group * (a.steps + kG) * kSlot;
   for (int p = l; p < a.steps * kSlot; p += kG) mine[p] = 0.f;
   if (tid < a.buckets) {
@@ -234,18 +242,20 @@ __global__ __launch_bounds__(kThreads) void bias_backward(GradArgs a, Edges e) {
   bool dead_row = false;
   if (a.mask) {
     const uint8_t* m = a.mask + b * a.mask_b;
-    int bits = 0;
+    uint8_t col[2 * V - 1];  // places past the ends read an end: cols has no bit there
 #pragma unroll
-    for (int x = 0; x < 2 * V - 1; ++x)  // places past the ends read an end: cols has no bit there
-      bits |= (m[min(max(first - (V - 1) + x, 0), k_len - 1) * a.mask_k] != 0) << x;
-    cols &= bits;
+    for (int x = 0; x < 2 * V - 1; ++x) col[x] = m[min(max(first - (V - 1) + x, 0), k_len - 1) * a.mask_k];
     for (int n = tid; n < kGroups * a.steps; n += kThreads) {
-      bits = 0;
+      int bits = 0;
 #pragma unroll
       for (int x = 0; x < V; ++x) bits |= (m[(min((begin + n) * V + x, q_len - 1) + a.start) * a.mask_k] != 0) << x;
       live_rows[n] = (uint8_t)bits;
       dead_row |= bits != kRows;
     }
+    int bits = 0;
+#pragma unroll
+    for (int x = 0; x < 2 * V - 1; ++x) bits |= (col[x] != 0) << x;
+    cols &= bits;
   }
   dead_row = __syncthreads_or(dead_row);
   const int64_t plane_end = (int64_t)(q_len - 1) * a.g_i + k_len;
@@ -388,10 +398,7 @@ __global__ __launch_bounds__(kThreads) void bias_backward(GradArgs a, Edges e) {
     for (int p = from + lane; p <= to; p += 16) u += line[p];
 #pragma unroll
     for (int off = 8; off > 0; off >>= 1) u += __shfl_xor(u, off, 16);
-    if (lane == 0) {
-      if (a.blocks == 1) a.out[(b * a.buckets + x) * a.heads + h] = u;
-      else a.partial[((b * a.heads + h) * a.blocks + blockIdx.x) * a.buckets + x] = u;
-    }
+    if (lane == 0) store(x, u);
   }
 }
 
