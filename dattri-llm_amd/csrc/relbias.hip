@@ -17,7 +17,6 @@ namespace da {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kWaves = kThreads / kWave;
 constexpr int kMaxBuckets = 256;
 
 struct Edges {
@@ -26,34 +25,29 @@ struct Edges {
   int32_t least[kMaxBuckets];
 };
 
-__device__ __forceinline__ int bucket_of(const Edges& e, int64_t o) {
-  const int64_t away = e.both ? (o < 0 ? -o : o) : (o < 0 ? -o : 0);
-  const int32_t r = (int32_t)min(away, (int64_t)0x7fffffff);
-  int lo = 0, hi = e.n;  // least[lo] <= r < least[hi]
+__device__ __forceinline__ int bucket_of(const int* least, int n, int both, int o) {
+  const int r = o < 0 ? -o : both ? o : 0;
+  int lo = 0, hi = n;  // least[lo] <= r < least[hi]
   while (hi - lo > 1) {
     const int mid = (lo + hi) / 2;
-    if (e.least[mid] <= r) lo = mid;
+    if (least[mid] <= r) lo = mid;
     else hi = mid;
   }
-  return lo + (e.both && o > 0 ? e.n : 0);
+  return lo + (both && o > 0 ? n : 0);
 }
 
-// A square of scores is walked along its diagonals.  With V entries in 16 bytes,
-// a lane owns diagonal block k: in row block r (rows rV .. rV + V - 1) its
-// columns are those of column block r + k, so that from one row block to the
-// next it meets the same 2V - 1 offsets j - i again: they stay in registers for
-// the whole walk -- as sums in the backward pass, as packed 16-byte values in the
-// forward pass -- while every access is one aligned 16 bytes and the lanes of a
-// wave are neighbours in the row.
+// With V entries in 16 bytes, rows and columns are taken in blocks of V: the square
+// of row block r and column block c holds the offsets of diagonal block k = c - r,
+// whatever r.  All accesses are aligned runs of 16 bytes.
 //
 // Rows need not be aligned: entry j of row i is at address mis + i stride + j
 // (modulo V; mis that of the plane's first entry), so with R = stride mod V the
-// aligned run of row rV + e starts at column (r + k) V - mis - shift(e), shift(e)
-// = e R mod V.  R is a template argument, all indices into the registers are
-// constants, and 3V - 2 offsets cover every R.
+// aligned run of row rV + e in column block c starts at column c V - mis -
+// shift(e), shift(e) = e R mod V, and 3V - 2 offsets k V - mis + [-2 (V - 1), V - 1]
+// cover a diagonal block for every R.  In the backward pass R is a template
+// argument: all indices into a lane's sums are constants.
 template <int V, int R>
 struct Walk {
-  static constexpr int kLine = (kWave + 2) * V;  // offsets of a wave's 64 diagonal blocks
   __host__ __device__ static constexpr int shift(int e) { return e * R % V; }
   __host__ __device__ static constexpr int at(int e, int x) { return x - e - shift(e) + 2 * (V - 1); }
   __host__ __device__ static constexpr int end(bool last) {
@@ -92,8 +86,7 @@ struct BiasArgs {
   int64_t q_len, k_len;
   int64_t t_b, t_h;  // table strides in elements
   int start, causal;
-  int row_blocks, first_block;  // row blocks; the least diagonal block
-  int windows, splits, steps;   // waves of diagonal blocks; parts of the rows, row blocks of each
+  int columns, windows, steps;  // column blocks, windows of kWave of them; row blocks of a workgroup
   uint32_t closed;              // bits of -inf
 };
 
@@ -108,64 +101,62 @@ __device__ __forceinline__ void store_bits(char* p, int64_t i, uint32_t v) {
   else ((uint16_t*)p)[i] = (uint16_t)v;
 }
 
-// A workgroup writes one head's entries of 64 diagonal blocks in a part of the
-// rows: the offsets' values go to LDS once, each lane packs the V runs of its
-// block and then only stores.  Runs that a row's end cuts are left to the
-// workgroup of the first window, entry by entry.
-template <int ES, int R>
+// A workgroup writes one head's entries of up to 64 column blocks and `steps` row
+// blocks.  The run of row rV + e in column block c depends on e and on c - r alone:
+// the runs of all diagonal blocks lie ready in LDS, one array for each e, and a
+// store is one 16-byte LDS read (neighbouring lanes read neighbours) and one
+// aligned 16-byte write, a row's whole lines by one wave.  Runs that a row's end
+// cuts are written entry by entry at the end.
+template <int ES>
 __global__ __launch_bounds__(kThreads) void bias_forward(BiasArgs a, Edges e) {
   constexpr int V = 16 / ES;
-  using W = Walk<V, R>;
-  __shared__ uint32_t line[W::kLine];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int window = blockIdx.x % a.windows, split = blockIdx.x / a.windows;
+  extern __shared__ u32x4 runs[];  // [V][blocks], then the line of single values
+  __shared__ int least[kMaxBuckets];
+  __shared__ uint32_t column[kMaxBuckets];
+  const int tid = threadIdx.x;
+  const int window = blockIdx.x % a.windows, r0 = blockIdx.x / a.windows * a.steps;
   const int64_t h = blockIdx.y;
   char* plane = a.out + h * a.q_len * a.k_len * ES;
   const int mis = (int)((uintptr_t)plane / ES % V);
-  const int k0 = a.first_block + window * kWave, k = k0 + lane;
-  const char* column = a.table + h * a.t_h * ES;
-  for (int p = tid; p < W::kLine; p += kThreads) {
+  const int k_len = (int)a.k_len, i0 = r0 * V, rows = (int)min((int64_t)a.steps * V, a.q_len - i0);
+  const int c0 = window * kWave, width = min(kWave, a.columns - c0);
+  const int blocks = width + a.steps - 1, k0 = c0 - (r0 + a.steps - 1);  // diagonal blocks, the first of them
+  uint32_t* line = (uint32_t*)(runs + V * blocks);
+  if (tid < e.n) least[tid] = e.least[tid];
+  if (tid < (e.both ? 2 : 1) * e.n) column[tid] = load_bits<ES>(a.table, tid * a.t_b + h * a.t_h);
+  __syncthreads();
+  for (int p = tid; p < (blocks + 2) * V; p += kThreads) {
     const int o = k0 * V + p - 2 * (V - 1) - mis - a.start;
-    line[p] = a.causal && o > 0 ? a.closed : load_bits<ES>(column, bucket_of(e, o) * a.t_b);
+    line[p] = a.causal && o > 0 ? a.closed : column[bucket_of(least, e.n, e.both, o)];
   }
   __syncthreads();
-  u32x4 run[V];
+  const int stride = k_len % V;
+  for (int n = tid; n < min(rows, V) * blocks; n += kThreads) {
+    const int r = n / blocks, k = n - r * blocks;
+    const uint32_t* at = line + k * V + 2 * (V - 1) - r - r * stride % V;
+    u32x4 run;
 #pragma unroll
-  for (int r = 0; r < V; ++r)
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      if constexpr (ES == 4) run[r][q] = line[lane * V + W::at(r, q)];
-      else run[r][q] = line[lane * V + W::at(r, 2 * q)] | line[lane * V + W::at(r, 2 * q + 1)] << 16;
-    }
-  const int r0 = split * a.steps, r1 = min(r0 + a.steps, a.row_blocks);
-  const int k_len = (int)a.k_len, q_len = (int)a.q_len;
-  const int last = min(r1, (k_len + mis + 2 * V - 2) / V - k0);
-  for (int r = max(r0, 1 - kWave - k0) + wave; r < last; r += kWaves) {
-    const int first = (r + k) * V - mis;  // column of an unshifted run
-#pragma unroll
-    for (int x = 0; x < V; ++x) {
-      const int i = r * V + x, j = first - W::shift(x);
-      if (i < q_len && j >= 0 && j + V <= k_len) st16(plane + ((int64_t)i * k_len + j) * ES, run[x]);
-    }
+    for (int q = 0; q < 4; ++q) run[q] = ES == 4 ? at[q] : at[2 * q] | at[2 * q + 1] << 16;
+    runs[n] = run;
   }
-  if (window == 0 && (R != 0 || mis != 0 || k_len % V != 0)) {
-    const int rows = min(r1 * V, q_len) - r0 * V;
-    for (int n = tid; n < rows * 2 * V; n += kThreads) {
-      const int i = r0 * V + n / (2 * V), x = n % (2 * V);
-      const int lead = (int)((V - (mis + (int64_t)i * k_len) % V) % V);  // entries before the first whole run
-      const int tail = k_len < lead ? 0 : (k_len - lead) % V;
-      int j;
-      if (x < V) {
-        if (x >= min(lead, k_len)) continue;
-        j = x;
-      } else {
-        if (x - V >= tail) continue;
-        j = k_len - tail + x - V;
-      }
-      const int o = j - i - a.start;
-      store_bits<ES>(plane, (int64_t)i * k_len + j,
-                     a.causal && o > 0 ? a.closed : load_bits<ES>(column, bucket_of(e, o) * a.t_b));
+  __syncthreads();
+  const int together = kThreads / width;  // rows that the workgroup writes at once
+  const int c = tid % width;
+  if (tid < together * width)
+    for (int i = tid / width; i < rows; i += together) {
+      const int r = i % V, j = (c0 + c) * V - mis - r * stride % V;
+      if (j >= 0 && j + V <= k_len)
+        st16(plane + ((int64_t)(i0 + i) * k_len + j) * ES, runs[r * blocks + c + a.steps - 1 - i / V]);
     }
+  if (stride == 0 && mis == 0) return;
+  for (int n = tid; n < rows * 2 * V; n += kThreads) {  // the first and the last run of each row
+    const int i = n / (2 * V), x = n % V, r = i % V, shift = mis + r * stride % V;
+    const int at = n % (2 * V) < V ? shift / V : (k_len - 1 + shift) / V;  // column block
+    const int first = at * V - shift, j = first + x;
+    if (first >= 0 && first + V <= k_len) continue;  // a whole run
+    if (n % (2 * V) >= V && at == shift / V) continue;  // one run is both
+    if (j >= 0 && j < k_len && at >= c0 && at < c0 + width)
+      store_bits<ES>(plane, (int64_t)(i0 + i) * k_len + j, line[(at - c0 + a.steps - 1 - i / V) * V + 2 * (V - 1) - r - r * stride % V + x]);
   }
 }
 
@@ -442,28 +433,6 @@ constexpr int64_t kMaxLen = (int64_t)1 << 26;
 
 constexpr int64_t kWantBlocks = 1024;  // four workgroups for each CU
 
-struct Plan {
-  int row_blocks, first_block, windows, splits, steps;
-};
-
-// The forward pass: diagonal blocks run from the first column block against the
-// last row block to the last column block against the first; planes whose rows
-// are not all aligned reach further.  The rows are split until the planes fill the
-// card with kWantBlocks workgroups, each of at least four row blocks a wave.
-Plan make_plan(int v, bool aligned, int64_t planes, int64_t q_len, int64_t k_len) {
-  Plan p;
-  p.row_blocks = (int)((q_len + v - 1) / v);
-  p.first_block = 1 - p.row_blocks;
-  const int64_t slack = aligned ? 0 : v - 1;  // most that mis, and that a row's shift, can be
-  const int64_t last = (k_len - 1 + 2 * slack) / v;
-  p.windows = (int)((last - p.first_block + kWave) / kWave);
-  int64_t splits = (kWantBlocks + planes * p.windows - 1) / (planes * p.windows);
-  splits = std::min<int64_t>(splits, (p.row_blocks + 4 * kWaves - 1) / (4 * kWaves));
-  p.steps = (int)((p.row_blocks + splits - 1) / splits);
-  p.splits = (p.row_blocks + p.steps - 1) / p.steps;
-  return p;
-}
-
 struct GradPlan {
   int group, row_blocks, last_block, windows, splits, steps;
 };
@@ -517,24 +486,25 @@ int da_relative_bias(const void* table, int dtype, int64_t table_bstride, int64_
   if (!table || !out) return set_error(DA_ERR_INVALID, "%s: NULL pointer", what);
   const int es = (int)elem_bytes(dtype), v = 16 / es;
   const bool aligned = (uintptr_t)out % 16 == 0 && k_len % v == 0;
-  const Plan p = make_plan(v, aligned, heads, q_len, k_len);
+  const int64_t row_blocks = (q_len + v - 1) / v;
   BiasArgs a{};
   a.table = (const char*)table, a.out = (char*)out, a.q_len = q_len, a.k_len = k_len, a.t_b = table_bstride;
-  a.t_h = table_hstride, a.start = (int)q_start, a.causal = causal, a.row_blocks = p.row_blocks;
-  a.first_block = p.first_block, a.windows = p.windows, a.splits = p.splits, a.steps = p.steps;
+  a.t_h = table_hstride, a.start = (int)q_start, a.causal = causal;
+  // A row's first run may start up to 2 (v - 1) entries before it.
+  a.columns = (int)((k_len - 1 + (aligned ? 0 : 2 * (v - 1))) / v + 1);
+  a.windows = (a.columns + kWave - 1) / kWave;
+  // Row blocks of a workgroup: 4 to 32, so that there are kWantBlocks workgroups.
+  a.steps = (int)std::min<int64_t>(std::max<int64_t>(row_blocks * a.windows * heads / kWantBlocks, 4), 32);
+  a.steps = (int)std::min<int64_t>(a.steps, row_blocks);
   a.closed = dtype == DA_F32 ? 0xff800000u : dtype == DA_BF16 ? 0xff80u : 0xfc00u;
   hipStream_t st = (hipStream_t)stream;
-  const dim3 grid((unsigned)(p.windows * p.splits), (unsigned)heads);
-#define DA_FWD(ES, R) \
-  case R: bias_forward<ES, R><<<grid, kThreads, 0, st>>>(a, e); break;
-  if (es == 2) {
-    switch (k_len % 8) {
-      DA_FWD(2, 0) DA_FWD(2, 1) DA_FWD(2, 2) DA_FWD(2, 3) DA_FWD(2, 4) DA_FWD(2, 5) DA_FWD(2, 6) DA_FWD(2, 7)
-    }
-  } else {
-    switch (k_len % 4) { DA_FWD(4, 0) DA_FWD(4, 1) DA_FWD(4, 2) DA_FWD(4, 3) }
-  }
-#undef DA_FWD
+  const int64_t grid_x = a.windows * ((row_blocks + a.steps - 1) / a.steps);
+  if (grid_x > 0x7fffffff) return set_error(DA_ERR_UNSUPPORTED, "%s: too many entries", what);
+  const dim3 grid((unsigned)grid_x, (unsigned)heads);
+  const int blocks = std::min<int>(kWave, a.columns) + a.steps - 1;
+  const size_t lds = (size_t)v * blocks * 16 + (size_t)(blocks + 2) * v * 4;
+  if (es == 2) bias_forward<2><<<grid, kThreads, lds, st>>>(a, e);
+  else bias_forward<4><<<grid, kThreads, lds, st>>>(a, e);
   return check_launch(what);
 }
 
