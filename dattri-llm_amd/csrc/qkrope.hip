@@ -87,18 +87,46 @@ struct Slot {
   }
 };
 
-template <int DT, int V>
-struct Run {  // V entries as they lie in memory
-  uint32_t bits[V];
-  __device__ void load(const char* p, bool in) {
-    static_assert(V == 1);
-    if constexpr (DT == DA_F32) bits[0] = in ? *(const uint32_t*)p : 0u;
-    else bits[0] = in ? *(const uint16_t*)p : 0u;
+// Two fp32 values rounded to 16 bits each (to nearest even), packed.
+template <int DT>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  if constexpr (DT == DA_BF16) {
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, bf16x2));
+  } else {
+    typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, f16x2));
   }
-  __device__ float get(int i) const { return Elem<DT>::from_bits(bits[i]); }
+}
+
+template <int DT, int V>
+struct Run {  // V entries as they lie in memory, in one access
+  static constexpr int kBytes = V * Elem<DT>::kBytes, kWords = kBytes < 4 ? 1 : kBytes / 4;
+  typedef uint32_t Words __attribute__((ext_vector_type(kWords)));
+  Words w;
+  __device__ void load(const char* p, bool in) {
+    w = Words(0);
+    if (!in) return;
+    if constexpr (kBytes == 2) w[0] = *(const uint16_t*)p;
+    else w = *(const Words*)p;
+  }
+  __device__ float get(int i) const {
+    if constexpr (DT == DA_F32) return __uint_as_float(w[i]);
+    else return Elem<DT>::from_bits(i & 1 ? w[i >> 1] >> 16 : w[i >> 1] & 0xffffu);
+  }
   __device__ static void store(char* p, const float* v, bool in) {
-    static_assert(V == 1);
-    if (in) Elem<DT>::store(p, 0, v[0]);
+    if (!in) return;
+    if constexpr (V == 1) Elem<DT>::store(p, 0, v[0]);
+    else {
+      Words w;
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) {
+        if constexpr (DT == DA_F32) w[i] = __float_as_uint(v[i]);
+        else w[i] = pack2<DT>(v[2 * i], v[2 * i + 1]);
+      }
+      *(Words*)p = w;
+    }
   }
 };
 
@@ -396,26 +424,69 @@ void chunking(int64_t batch, int64_t tokens, int64_t* chunk, int64_t* chunks) {
 
 using namespace da;
 
-#define DA_QK_SLOTS(CALL, DT, IL)        \
-  if (pairs <= 64) {                     \
-    CALL(DT, 1, 64, 1, IL)               \
-  } else if (pairs <= 128) {             \
-    CALL(DT, 1, 64, 2, IL)               \
-  } else if (pairs <= 256) {             \
-    CALL(DT, 1, 64, 4, IL)               \
-  } else {                               \
-    CALL(DT, 1, 64, 8, IL)               \
+// Entries of a lane's run: what every slot and every row's alignment allow, up to
+// 16 bytes; then the lanes of a head, or its slots a lane.
+namespace {
+int run_entries(const QkArgs& a, int es, bool grad) {
+  const int64_t d = a.d, rot = a.rot;
+  for (int v = 16 / es; v > 1; v = v == 8 ? 4 : 1) {
+    bool fits = rot / 2 % v == 0 && (d - rot) % (2 * v) == 0;
+    for (int i = 0; i < 2 && fits; ++i) {
+      const Rows& s = a.side[i];
+      if (!s.heads) continue;
+      int64_t all = (int64_t)s.x | (int64_t)s.out;
+      if (grad) all |= (int64_t)s.gz;
+      // the stride of an axis of one entry says nothing
+      if (a.batch > 1) all |= s.x_b | s.o_b | (grad ? s.g_b : 0);
+      if (a.tokens > 1) all |= s.x_t | s.o_t | (grad ? s.g_t : 0);
+      if (s.heads > 1) all |= s.x_h | s.o_h | (grad ? s.g_h : 0);
+      fits = (uint64_t)all % (uint64_t)(v * es) == 0;
+    }
+    if (fits) return v;
   }
-#define DA_QK_DISPATCH(CALL)                                                    \
-  if (dtype == DA_BF16) {                                                       \
-    if (interleaved) { DA_QK_SLOTS(CALL, DA_BF16, true) }                       \
-    else { DA_QK_SLOTS(CALL, DA_BF16, false) }                                  \
-  } else if (dtype == DA_F16) {                                                 \
-    if (interleaved) { DA_QK_SLOTS(CALL, DA_F16, true) }                        \
-    else { DA_QK_SLOTS(CALL, DA_F16, false) }                                   \
-  } else {                                                                      \
-    if (interleaved) { DA_QK_SLOTS(CALL, DA_F32, true) }                        \
-    else { DA_QK_SLOTS(CALL, DA_F32, false) }                                   \
+  return 1;
+}
+}  // namespace
+
+#define DA_QK_LANES(CALL, DT, V, IL)      \
+  if (slots <= 4) {                       \
+    CALL(DT, V, 4, 1, IL)                 \
+  } else if (slots <= 8) {                \
+    CALL(DT, V, 8, 1, IL)                 \
+  } else if (slots <= 16) {               \
+    CALL(DT, V, 16, 1, IL)                \
+  } else if (slots <= 32) {               \
+    CALL(DT, V, 32, 1, IL)                \
+  } else if (slots <= 64) {               \
+    CALL(DT, V, 64, 1, IL)                \
+  } else {                                \
+    CALL(DT, V, 64, 2, IL)                \
+  }
+#define DA_QK_SINGLE(CALL, DT, IL)        \
+  if (pairs <= 64) {                      \
+    CALL(DT, 1, 64, 1, IL)                \
+  } else if (pairs <= 128) {              \
+    CALL(DT, 1, 64, 2, IL)                \
+  } else if (pairs <= 256) {              \
+    CALL(DT, 1, 64, 4, IL)                \
+  } else {                                \
+    CALL(DT, 1, 64, 8, IL)                \
+  }
+#define DA_QK_RUNS(CALL, DT, IL)                                              \
+  if (DT != DA_F32 && v == 8) { DA_QK_LANES(CALL, DT, (DT == DA_F32 ? 4 : 8), IL) }                   \
+  else if (v == 4) { DA_QK_LANES(CALL, DT, 4, IL) }                           \
+  else { DA_QK_SINGLE(CALL, DT, IL) }
+#define DA_QK_DISPATCH(CALL)                                        \
+  const int64_t slots = pairs / v;                                  \
+  if (dtype == DA_BF16) {                                           \
+    if (interleaved) { DA_QK_RUNS(CALL, DA_BF16, true) }            \
+    else { DA_QK_RUNS(CALL, DA_BF16, false) }                       \
+  } else if (dtype == DA_F16) {                                     \
+    if (interleaved) { DA_QK_RUNS(CALL, DA_F16, true) }             \
+    else { DA_QK_RUNS(CALL, DA_F16, false) }                        \
+  } else {                                                          \
+    if (interleaved) { DA_QK_RUNS(CALL, DA_F32, true) }             \
+    else { DA_QK_RUNS(CALL, DA_F32, false) }                        \
   }
 
 extern "C" {
@@ -440,6 +511,7 @@ int da_qk_norm_rope(const da_qk_side* sides, int dtype, int weight_dtype, int64_
   a.mask = mask, a.mask_b = mask_bstride, a.mask_t = mask_tstride, a.scaling = scaling, a.eps = eps;
   hipStream_t st = (hipStream_t)stream;
   const int64_t pairs = rot / 2 + (d - rot + 1) / 2;
+  const int v = run_entries(a, es, false);
   a.parts = 1;
   const int64_t blocks = (batch * tokens * a.parts + kWaves - 1) / kWaves;
   if (blocks > 0x7fffffff) return set_error(DA_ERR_UNSUPPORTED, "da_qk_norm_rope: too many tokens");
@@ -487,6 +559,7 @@ int da_qk_norm_rope_grad(const da_qk_side* sides, int dtype, int weight_dtype, i
   a.inv_freq = inv_freq, a.pos = positions, a.pos_bytes = position_bytes, a.pos_b = pos_bstride, a.pos_t = pos_tstride;
   a.mask = mask, a.mask_b = mask_bstride, a.mask_t = mask_tstride, a.scaling = scaling, a.eps = eps;
   const int64_t pairs = rot / 2 + (d - rot + 1) / 2;
+  const int v = run_entries(a, es, true);
   const int64_t per_side = batch * a.chunks;
   if (2 * per_side > 0x7fffffff) return set_error(DA_ERR_UNSUPPORTED, "da_qk_norm_rope_grad: too many tokens");
   if (per_side) {
