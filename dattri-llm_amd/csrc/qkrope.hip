@@ -64,6 +64,14 @@ __device__ __forceinline__ float load_any(const void* p, int dt, int64_t i) {
   return dt == DA_BF16 ? bf16_bits_to_f32(h) : f16_bits_to_f32(h);
 }
 
+// LDS written by a wave's lanes is read by its other lanes: the hardware keeps a
+// wave's LDS accesses in order, this keeps the compiler to it.
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // Where a slot's two runs of V entries start, and what of them exists.
 template <int V, bool kInter>
 struct Slot {
@@ -130,23 +138,35 @@ struct Run {  // V entries as they lie in memory, in one access
   }
 };
 
-// The lane's pairs of one row: fp32 values, first and second members.  Run
-// order to pair order: interleaved runs hold both members alternately.
+// The lane's runs of one row as they lie in memory.
 template <int DT, int V, int S, bool kInter>
-struct Row {
-  float a[S][V], b[S][V];
+struct RawRow {
+  Run<DT, V> u[S], v[S];
   __device__ void load(const char* p, const Slot<V, kInter>* slots, bool live) {
     constexpr int ES = Elem<DT>::kBytes;
 #pragma unroll
     for (int i = 0; i < S; ++i) {
-      Run<DT, V> u, v;
-      u.load(p + (int64_t)slots[i].a * ES, live && slots[i].in);
-      v.load(p + (int64_t)slots[i].b * ES, live && slots[i].in && slots[i].has_b);
+      u[i].load(p + (int64_t)slots[i].a * ES, live && slots[i].in);
+      v[i].load(p + (int64_t)slots[i].b * ES, live && slots[i].in && slots[i].has_b);
+    }
+  }
+};
+
+// Its pairs: fp32 values, first and second members.  Interleaved runs hold both
+// members alternately.
+template <int DT, int V, int S, bool kInter>
+struct Row {
+  float a[S][V], b[S][V];
+  __device__ void unpack(const RawRow<DT, V, S, kInter>& raw) {
+#pragma unroll
+    for (int i = 0; i < S; ++i) {
+      float t[2 * V];
+#pragma unroll
+      for (int e = 0; e < V; ++e) t[e] = raw.u[i].get(e), t[V + e] = raw.v[i].get(e);
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        const int ea = kInter ? 2 * e : e, eb = kInter ? 2 * e + 1 : V + e;
-        a[i][e] = ea < V ? u.get(ea) : v.get(ea - V);
-        b[i][e] = eb < V ? u.get(eb) : v.get(eb - V);
+        a[i][e] = t[kInter ? 2 * e : e];
+        b[i][e] = t[kInter ? 2 * e + 1 : V + e];
       }
     }
   }
@@ -154,43 +174,48 @@ struct Row {
     constexpr int ES = Elem<DT>::kBytes;
 #pragma unroll
     for (int i = 0; i < S; ++i) {
-      float u[V], v[V];
+      float t[2 * V];
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        const int ea = kInter ? 2 * e : e, eb = kInter ? 2 * e + 1 : V + e;
-        (ea < V ? u[ea < V ? ea : 0] : v[ea >= V ? ea - V : 0]) = a[i][e];
-        (eb < V ? u[eb < V ? eb : 0] : v[eb >= V ? eb - V : 0]) = b[i][e];
+        t[kInter ? 2 * e : e] = a[i][e];
+        t[kInter ? 2 * e + 1 : V + e] = b[i][e];
       }
-      Run<DT, V>::store(p + (int64_t)slots[i].a * ES, u, live && slots[i].in);
-      Run<DT, V>::store(p + (int64_t)slots[i].b * ES, v, live && slots[i].in && slots[i].has_b);
+      Run<DT, V>::store(p + (int64_t)slots[i].a * ES, t, live && slots[i].in);
+      Run<DT, V>::store(p + (int64_t)slots[i].b * ES, t + V, live && slots[i].in && slots[i].has_b);
     }
   }
 };
 
-__device__ __forceinline__ void turn_of(const QkArgs& a, double pos, int pair, float* c, float* s) {
-  const double turns = pos * ((double)a.inv_freq[pair] * 0.15915494309189535);  // 1 / (2 pi)
-  const float part = (float)(2.0 * (turns - rint(turns)));                      // half turns, [-1, 1]
-  float sn, cs;
-  sincospif(part, &sn, &cs);
-  *c = cs * a.scaling;
-  *s = sn * a.scaling;
-}
-
-template <int V, int S, bool kInter>
-__device__ __forceinline__ void angles(const QkArgs& a, int64_t b, int64_t t, const Slot<V, kInter>* slots,
-                                       int first_slot, int step, float (&c)[S][V], float (&s)[S][V]) {
+// Cosine and sine of a token's pairs, one pair a lane: a wave's heads share them
+// through its own part of the LDS (`table`: kL S V pairs).  Pairs past the
+// rotated ones stay as they are.
+template <int V, int kL, int S>
+__device__ __forceinline__ void angles(const QkArgs& a, int64_t b, int64_t t, float2* table, int lane, int l,
+                                       float (&c)[S][V], float (&s)[S][V]) {
   double pos = (double)t;
   if (a.pos) {
     const int64_t at = b * a.pos_b + t * a.pos_t;
     pos = a.pos_bytes == 8 ? (double)((const int64_t*)a.pos)[at] : (double)((const int32_t*)a.pos)[at];
   }
+  wave_sync();  // the last token's are read
+  for (int pair = lane; pair < kL * S * V; pair += kWave) {
+    float sn = 0.f, cs = 1.f;
+    if (pair < a.rot / 2) {
+      const double turns = pos * ((double)a.inv_freq[pair] * 0.15915494309189535);  // 1 / (2 pi)
+      sincospif((float)(2.0 * (turns - rint(turns))), &sn, &cs);                    // half turns, [-1, 1]
+      sn *= a.scaling;
+      cs *= a.scaling;
+    }
+    table[pair] = make_float2(cs, sn);
+  }
+  wave_sync();
 #pragma unroll
   for (int i = 0; i < S; ++i)
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-      c[i][e] = 1.f;
-      s[i][e] = 0.f;
-      if (slots[i].in && slots[i].turn) turn_of(a, pos, (first_slot + i * step) * V + e, &c[i][e], &s[i][e]);
+      const float2 cs = table[(l + i * kL) * V + e];
+      c[i][e] = cs.x;
+      s[i][e] = cs.y;
     }
 }
 
@@ -218,6 +243,7 @@ __device__ __forceinline__ float lanes_sum(float v) {
 template <int DT, int V, int kL, int S, bool kInter>
 __global__ __launch_bounds__(kThreads) void qk_rope_forward(QkArgs a) {
   constexpr int kHeads = kWave / kL;  // heads of a wave's step
+  __shared__ float2 tables[kWaves][kL * S * V];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int l = lane % kL, sub = lane / kL;
   const int64_t unit = (int64_t)blockIdx.x * kWaves + wave;
@@ -230,36 +256,43 @@ __global__ __launch_bounds__(kThreads) void qk_rope_forward(QkArgs a) {
   for (int i = 0; i < S; ++i) slots[i].at(l + i * kL, a.d, a.rot);
   const bool live = !a.mask || a.mask[b * a.mask_b + t * a.mask_t];
   float c[S][V], s[S][V];
-  angles<V, S, kInter>(a, b, t, slots, l, kL, c, s);
+  angles<V, kL, S>(a, b, t, tables[wave], lane, l, c, s);
   const float inv_d = 1.f / (float)a.d;
   int64_t g = part, base = 0;
 #pragma unroll
   for (int side = 0; side < 2; ++side) {
     const Rows& r = a.side[side];
     const int64_t groups = (r.heads + kHeads - 1) / kHeads;
-    float wa[S][V], wb[S][V];
-    if (g < base + groups) weights<V, S, kInter>(r.w, a.w_dtype, slots, wa, wb);
-    for (; g < base + groups; g += a.parts) {
-      const int64_t head = (g - base) * kHeads + sub;
-      const bool in = head < r.heads;
-      Row<DT, V, S, kInter> x;
-      x.load(r.x + b * r.x_b + t * r.x_t + head * r.x_h, slots, in && live);
-      float sq = 0.f;
+    const char* x_token = r.x + b * r.x_b + t * r.x_t;
+    char* out_token = r.out + b * r.o_b + t * r.o_t;
+    if (g < base + groups) {
+      float wa[S][V], wb[S][V];
+      RawRow<DT, V, S, kInter> raw;
+      int64_t head = (g - base) * kHeads + sub;
+      raw.load(x_token + head * r.x_h, slots, head < r.heads && live);
+      weights<V, S, kInter>(r.w, a.w_dtype, slots, wa, wb);
+      for (; g < base + groups; g += a.parts) {
+        Row<DT, V, S, kInter> x, z;
+        x.unpack(raw);
+        const int64_t now = head;
+        head += (int64_t)a.parts * kHeads;
+        if (g + a.parts < base + groups) raw.load(x_token + head * r.x_h, slots, head < r.heads && live);
+        float sq = 0.f;
 #pragma unroll
-      for (int i = 0; i < S; ++i)
+        for (int i = 0; i < S; ++i)
 #pragma unroll
-        for (int e = 0; e < V; ++e) sq += x.a[i][e] * x.a[i][e] + x.b[i][e] * x.b[i][e];
-      const float rms = rsqrtf(lanes_sum<kL>(sq) * inv_d + a.eps);
-      Row<DT, V, S, kInter> z;
+          for (int e = 0; e < V; ++e) sq += x.a[i][e] * x.a[i][e] + x.b[i][e] * x.b[i][e];
+        const float rms = rsqrtf(lanes_sum<kL>(sq) * inv_d + a.eps);
 #pragma unroll
-      for (int i = 0; i < S; ++i)
+        for (int i = 0; i < S; ++i)
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-          const float ya = x.a[i][e] * rms * wa[i][e], yb = x.b[i][e] * rms * wb[i][e];
-          z.a[i][e] = live ? ya * c[i][e] - yb * s[i][e] : 0.f;
-          z.b[i][e] = live ? yb * c[i][e] + ya * s[i][e] : 0.f;
-        }
-      z.store(r.out + b * r.o_b + t * r.o_t + head * r.o_h, slots, in);
+          for (int e = 0; e < V; ++e) {
+            const float ya = x.a[i][e] * rms * wa[i][e], yb = x.b[i][e] * rms * wb[i][e];
+            z.a[i][e] = live ? ya * c[i][e] - yb * s[i][e] : 0.f;
+            z.b[i][e] = live ? yb * c[i][e] + ya * s[i][e] : 0.f;
+          }
+        z.store(out_token + now * r.o_h, slots, now < r.heads);
+      }
     }
     base += groups;
   }
@@ -271,6 +304,7 @@ __global__ __launch_bounds__(kThreads) void qk_rope_forward(QkArgs a) {
 template <int DT, int V, int kL, int S, bool kInter>
 __global__ __launch_bounds__(kThreads) void qk_rope_backward(QkArgs a, int64_t q_blocks) {
   constexpr int kHeads = kWave / kL;
+  __shared__ float2 tables[kWaves][kL * S * V];
   __shared__ float sums[kWaves][2 * S * V * kL];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int l = lane % kL, sub = lane / kL;
@@ -295,15 +329,18 @@ __global__ __launch_bounds__(kThreads) void qk_rope_backward(QkArgs a, int64_t q
   bool live = true;
   while (t < t1) {
     if (t != last) {
-      angles<V, S, kInter>(a, b, t, slots, l, kL, c, s);
+      angles<V, kL, S>(a, b, t, tables[wave], lane, l, c, s);
       live = !a.mask || a.mask[b * a.mask_b + t * a.mask_t];
       last = t;
     }
     const int64_t head = g * kHeads + sub;
     const bool in = head < r.heads;
+    RawRow<DT, V, S, kInter> raw_x, raw_z;
+    raw_x.load(r.x + b * r.x_b + t * r.x_t + head * r.x_h, slots, in && live);
+    raw_z.load(r.gz + b * r.g_b + t * r.g_t + head * r.g_h, slots, in && live);
     Row<DT, V, S, kInter> x, z;
-    x.load(r.x + b * r.x_b + t * r.x_t + head * r.x_h, slots, in && live);
-    z.load(r.gz + b * r.g_b + t * r.g_t + head * r.g_h, slots, in && live);
+    x.unpack(raw_x);
+    z.unpack(raw_z);
     float sq = 0.f, along = 0.f;
 #pragma unroll
     for (int i = 0; i < S; ++i)
