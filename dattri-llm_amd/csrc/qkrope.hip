@@ -22,6 +22,8 @@
 // one token's angles serve all the heads its wave visits.  Both members of a
 // pair are in one lane: the rotation needs no exchange, and a row's two sums
 // (x^2; and g x in the backward pass) are one butterfly over the kL lanes.
+#include <algorithm>
+
 #include "common.h"
 
 namespace da {
@@ -30,6 +32,8 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / kWave;
 constexpr int64_t kMaxD = 1024;
+constexpr int64_t kWantWaves = 4096;  // a token's heads are spread over waves while there are fewer
+constexpr int64_t kMostBlocks = 2048;
 
 struct Rows {  // one side's rows; strides in bytes
   const char* x;
@@ -160,13 +164,16 @@ struct Row {
   __device__ void unpack(const RawRow<DT, V, S, kInter>& raw) {
 #pragma unroll
     for (int i = 0; i < S; ++i) {
-      float t[2 * V];
-#pragma unroll
-      for (int e = 0; e < V; ++e) t[e] = raw.u[i].get(e), t[V + e] = raw.v[i].get(e);
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        a[i][e] = t[kInter ? 2 * e : e];
-        b[i][e] = t[kInter ? 2 * e + 1 : V + e];
+        if constexpr (kInter && V > 1) {
+          const Run<DT, V>& from = 2 * e < V ? raw.u[i] : raw.v[i];
+          a[i][e] = from.get(2 * e % V);
+          b[i][e] = from.get(2 * e % V + 1);
+        } else {
+          a[i][e] = raw.u[i].get(e);
+          b[i][e] = raw.v[i].get(e);
+        }
       }
     }
   }
@@ -174,14 +181,19 @@ struct Row {
     constexpr int ES = Elem<DT>::kBytes;
 #pragma unroll
     for (int i = 0; i < S; ++i) {
-      float t[2 * V];
+      float u[V], v[V];
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        t[kInter ? 2 * e : e] = a[i][e];
-        t[kInter ? 2 * e + 1 : V + e] = b[i][e];
+        if constexpr (kInter && V > 1) {
+          u[e] = e % 2 ? b[i][e / 2] : a[i][e / 2];
+          v[e] = e % 2 ? b[i][(V + e) / 2] : a[i][(V + e) / 2];
+        } else {
+          u[e] = a[i][e];
+          v[e] = b[i][e];
+        }
       }
-      Run<DT, V>::store(p + (int64_t)slots[i].a * ES, t, live && slots[i].in);
-      Run<DT, V>::store(p + (int64_t)slots[i].b * ES, t + V, live && slots[i].in && slots[i].has_b);
+      Run<DT, V>::store(p + (int64_t)slots[i].a * ES, u, live && slots[i].in);
+      Run<DT, V>::store(p + (int64_t)slots[i].b * ES, v, live && slots[i].in && slots[i].has_b);
     }
   }
 };
@@ -219,17 +231,25 @@ __device__ __forceinline__ void angles(const QkArgs& a, int64_t b, int64_t t, fl
     }
 }
 
-template <int V, int S, bool kInter>
-__device__ __forceinline__ void weights(const void* w, int dt, const Slot<V, kInter>* slots, float (&wa)[S][V],
-                                        float (&wb)[S][V]) {
+// The weight in the order of the pairs, in LDS: first members, then second.
+template <bool kInter>
+__device__ __forceinline__ void weights(const QkArgs& a, const void* w, float* to, int pairs) {
+  const int half = a.rot / 2, rest = (a.d - a.rot + 1) / 2;
+  for (int n = threadIdx.x; n < 2 * pairs; n += kThreads) {
+    const int p = n < pairs ? n : n - pairs, second = n >= pairs;
+    int at = kInter ? 2 * p + second : p < half ? p + second * half : a.rot + p - half + second * rest;
+    if (!kInter && p >= half + rest) at = a.d;
+    to[n] = at < a.d ? load_any(w, a.w_dtype, at) : 0.f;
+  }
+}
+template <int V, int kL, int S>
+__device__ __forceinline__ void lane_weights(const float* from, int l, float (&wa)[S][V], float (&wb)[S][V]) {
 #pragma unroll
   for (int i = 0; i < S; ++i)
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-      const int ia = kInter ? slots[i].a + 2 * e : slots[i].a + e;
-      const int ib = kInter ? slots[i].a + 2 * e + 1 : slots[i].b + e;
-      wa[i][e] = slots[i].in ? load_any(w, dt, ia) : 0.f;
-      wb[i][e] = slots[i].in && slots[i].has_b ? load_any(w, dt, ib) : 0.f;
+      wa[i][e] = from[(l + i * kL) * V + e];
+      wb[i][e] = from[(kL * S + l + i * kL) * V + e];
     }
 }
 
@@ -240,61 +260,74 @@ __device__ __forceinline__ float lanes_sum(float v) {
   return v;
 }
 
+// A wave takes units in turn: a token's heads, or every `parts`-th group of them
+// where the tokens are few.
 template <int DT, int V, int kL, int S, bool kInter>
 __global__ __launch_bounds__(kThreads) void qk_rope_forward(QkArgs a) {
-  constexpr int kHeads = kWave / kL;  // heads of a wave's step
-  __shared__ float2 tables[kWaves][kL * S * V];
+  constexpr int kHeads = kWave / kL, kPairs = kL * S * V;  // heads of a wave's step, pairs of a head
+  __shared__ float2 tables[kWaves][kPairs];
+  __shared__ float w[2][2 * kPairs];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int l = lane % kL, sub = lane / kL;
-  const int64_t unit = (int64_t)blockIdx.x * kWaves + wave;
-  if (unit >= a.batch * a.tokens * a.parts) return;
-  const int64_t token = unit / a.parts;
-  const int part = (int)(unit - token * a.parts);
-  const int64_t b = token / a.tokens, t = token - b * a.tokens;
   Slot<V, kInter> slots[S];
 #pragma unroll
   for (int i = 0; i < S; ++i) slots[i].at(l + i * kL, a.d, a.rot);
-  const bool live = !a.mask || a.mask[b * a.mask_b + t * a.mask_t];
-  float c[S][V], s[S][V];
-  angles<V, kL, S>(a, b, t, tables[wave], lane, l, c, s);
+#pragma unroll
+  for (int side = 0; side < 2; ++side)
+    if (a.side[side].heads) weights<kInter>(a, a.side[side].w, w[side], kPairs);
+  __syncthreads();
   const float inv_d = 1.f / (float)a.d;
-  int64_t g = part, base = 0;
+  const uint32_t units = (uint32_t)(a.batch * a.tokens) * (uint32_t)a.parts;
+  for (uint32_t unit = blockIdx.x * kWaves + wave; unit < units; unit += gridDim.x * kWaves) {
+    const uint32_t token = unit / (uint32_t)a.parts, part = unit - token * (uint32_t)a.parts;
+    const int64_t b = token / (uint32_t)a.tokens, t = token - (uint32_t)b * (uint32_t)a.tokens;
+    const bool live = !a.mask || a.mask[b * a.mask_b + t * a.mask_t];
+    float c[S][V], s[S][V];
+    bool turned = false;
+    int g = part, base = 0;
 #pragma unroll
-  for (int side = 0; side < 2; ++side) {
-    const Rows& r = a.side[side];
-    const int64_t groups = (r.heads + kHeads - 1) / kHeads;
-    const char* x_token = r.x + b * r.x_b + t * r.x_t;
-    char* out_token = r.out + b * r.o_b + t * r.o_t;
-    if (g < base + groups) {
-      float wa[S][V], wb[S][V];
-      RawRow<DT, V, S, kInter> raw;
-      int64_t head = (g - base) * kHeads + sub;
-      raw.load(x_token + head * r.x_h, slots, head < r.heads && live);
-      weights<V, S, kInter>(r.w, a.w_dtype, slots, wa, wb);
-      for (; g < base + groups; g += a.parts) {
-        Row<DT, V, S, kInter> x, z;
-        x.unpack(raw);
-        const int64_t now = head;
-        head += (int64_t)a.parts * kHeads;
-        if (g + a.parts < base + groups) raw.load(x_token + head * r.x_h, slots, head < r.heads && live);
-        float sq = 0.f;
+    for (int side = 0; side < 2; ++side) {
+      const Rows& r = a.side[side];
+      const int heads = (int)r.heads, groups = (heads + kHeads - 1) / kHeads, end = base + groups;
+      if (g < end) {
+        int head = (g - base) * kHeads + sub;
+        const char* x_row = r.x + b * r.x_b + t * r.x_t + head * r.x_h;
+        char* out_row = r.out + b * r.o_b + t * r.o_t + head * r.o_h;
+        const int64_t x_step = r.x_h * kHeads * a.parts, out_step = r.o_h * kHeads * a.parts;
+        RawRow<DT, V, S, kInter> raw;
+        raw.load(x_row, slots, head < heads && live);
+        if (!turned) angles<V, kL, S>(a, b, t, tables[wave], lane, l, c, s);
+        turned = true;
+        float wa[S][V], wb[S][V];
+        lane_weights<V, kL, S>(w[side], l, wa, wb);
+        for (; g < end; g += a.parts) {
+          Row<DT, V, S, kInter> x;
+          x.unpack(raw);
+          const bool in = head < heads;
+          head += kHeads * a.parts;
+          x_row += x_step;
+          if (g + a.parts < end) raw.load(x_row, slots, head < heads && live);
+          float sq = 0.f;
 #pragma unroll
-        for (int i = 0; i < S; ++i)
+          for (int i = 0; i < S; ++i)
 #pragma unroll
-          for (int e = 0; e < V; ++e) sq += x.a[i][e] * x.a[i][e] + x.b[i][e] * x.b[i][e];
-        const float rms = rsqrtf(lanes_sum<kL>(sq) * inv_d + a.eps);
+            for (int e = 0; e < V; ++e) sq += x.a[i][e] * x.a[i][e] + x.b[i][e] * x.b[i][e];
+          // A dead token's rows are zero, and stay zero without an eps.
+          const float rms = live ? rsqrtf(lanes_sum<kL>(sq) * inv_d + a.eps) : 0.f;
 #pragma unroll
-        for (int i = 0; i < S; ++i)
+          for (int i = 0; i < S; ++i)
 #pragma unroll
-          for (int e = 0; e < V; ++e) {
-            const float ya = x.a[i][e] * rms * wa[i][e], yb = x.b[i][e] * rms * wb[i][e];
-            z.a[i][e] = live ? ya * c[i][e] - yb * s[i][e] : 0.f;
-            z.b[i][e] = live ? yb * c[i][e] + ya * s[i][e] : 0.f;
-          }
-        z.store(out_token + now * r.o_h, slots, now < r.heads);
+            for (int e = 0; e < V; ++e) {
+              const float ya = x.a[i][e] * rms * wa[i][e], yb = x.b[i][e] * rms * wb[i][e];
+              x.a[i][e] = ya * c[i][e] - yb * s[i][e];
+              x.b[i][e] = yb * c[i][e] + ya * s[i][e];
+            }
+          x.store(out_row, slots, in);
+          out_row += out_step;
+        }
       }
+      base = end;
     }
-    base += groups;
   }
 }
 
@@ -304,8 +337,10 @@ __global__ __launch_bounds__(kThreads) void qk_rope_forward(QkArgs a) {
 template <int DT, int V, int kL, int S, bool kInter>
 __global__ __launch_bounds__(kThreads) void qk_rope_backward(QkArgs a, int64_t q_blocks) {
   constexpr int kHeads = kWave / kL;
-  __shared__ float2 tables[kWaves][kL * S * V];
-  __shared__ float sums[kWaves][2 * S * V * kL];
+  constexpr int kPairs = kL * S * V;
+  __shared__ float2 tables[kWaves][kPairs];
+  __shared__ float w[2 * kPairs];
+  __shared__ float sums[kWaves][2 * kPairs];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int l = lane % kL, sub = lane / kL;
   const int which = (int64_t)blockIdx.x >= q_blocks;
@@ -317,30 +352,41 @@ __global__ __launch_bounds__(kThreads) void qk_rope_backward(QkArgs a, int64_t q
   for (int i = 0; i < S; ++i) slots[i].at(l + i * kL, a.d, a.rot);
   const float inv_d = 1.f / (float)a.d;
   float wa[S][V], wb[S][V], da_[S][V], db_[S][V];
-  const int64_t groups = (r.heads + kHeads - 1) / kHeads;
-  if (groups) weights<V, S, kInter>(r.w, a.w_dtype, slots, wa, wb);  // an absent side has no weight to read
+  const int groups = ((int)r.heads + kHeads - 1) / kHeads;
+  if (groups) weights<kInter>(a, r.w, w, kPairs);  // an absent side has no weight to read
+  __syncthreads();
+  lane_weights<V, kL, S>(w, l, wa, wb);
 #pragma unroll
   for (int i = 0; i < S; ++i)
 #pragma unroll
     for (int e = 0; e < V; ++e) da_[i][e] = db_[i][e] = 0.f;
   const int64_t t0 = chunk * a.chunk, t1 = min(t0 + a.chunk, a.tokens);
-  int64_t t = groups ? t0 + wave / groups : t1, g = groups ? wave % groups : 0, last = -1;
-  float c[S][V], s[S][V];
+  // Steps of (token, group of heads), the waves in turn; the next step's rows are loaded ahead.
+  int64_t t = groups ? t0 + wave / groups : t1, last = -1;
+  int g = groups ? wave % groups : 0;
+  RawRow<DT, V, S, kInter> raw_x, raw_z;
   bool live = true;
+  auto load = [&]() {
+    live = !a.mask || a.mask[b * a.mask_b + t * a.mask_t];
+    const int64_t head = g * kHeads + sub;
+    raw_x.load(r.x + b * r.x_b + t * r.x_t + head * r.x_h, slots, head < r.heads && live);
+    raw_z.load(r.gz + b * r.g_b + t * r.g_t + head * r.g_h, slots, head < r.heads && live);
+  };
+  if (t < t1) load();
+  float c[S][V], s[S][V];
   while (t < t1) {
     if (t != last) {
       angles<V, kL, S>(a, b, t, tables[wave], lane, l, c, s);
-      live = !a.mask || a.mask[b * a.mask_b + t * a.mask_t];
       last = t;
     }
     const int64_t head = g * kHeads + sub;
-    const bool in = head < r.heads;
-    RawRow<DT, V, S, kInter> raw_x, raw_z;
-    raw_x.load(r.x + b * r.x_b + t * r.x_t + head * r.x_h, slots, in && live);
-    raw_z.load(r.gz + b * r.g_b + t * r.g_t + head * r.g_h, slots, in && live);
+    const bool in = head < r.heads, lives = live;
+    char* out = r.out + b * r.o_b + t * r.o_t + head * r.o_h;
     Row<DT, V, S, kInter> x, z;
     x.unpack(raw_x);
     z.unpack(raw_z);
+    for (g += kWaves; g >= groups; g -= groups) ++t;
+    if (t < t1) load();
     float sq = 0.f, along = 0.f;
 #pragma unroll
     for (int i = 0; i < S; ++i)
@@ -355,7 +401,7 @@ __global__ __launch_bounds__(kThreads) void qk_rope_backward(QkArgs a, int64_t q
       }
     const float rms = rsqrtf(lanes_sum<kL>(sq) * inv_d + a.eps);
     const float back = lanes_sum<kL>(along) * inv_d * rms * rms;
-    const bool adds = in && live;
+    const bool adds = in && lives;
 #pragma unroll
     for (int i = 0; i < S; ++i)
 #pragma unroll
@@ -364,11 +410,10 @@ __global__ __launch_bounds__(kThreads) void qk_rope_backward(QkArgs a, int64_t q
         // is 0: selected out, not multiplied by zero.
         da_[i][e] += adds ? z.a[i][e] * (x.a[i][e] * rms) : 0.f;
         db_[i][e] += adds ? z.b[i][e] * (x.b[i][e] * rms) : 0.f;
-        z.a[i][e] = live ? rms * (z.a[i][e] * wa[i][e] - x.a[i][e] * back) : 0.f;
-        z.b[i][e] = live ? rms * (z.b[i][e] * wb[i][e] - x.b[i][e] * back) : 0.f;
+        z.a[i][e] = lives ? rms * (z.a[i][e] * wa[i][e] - x.a[i][e] * back) : 0.f;
+        z.b[i][e] = lives ? rms * (z.b[i][e] * wb[i][e] - x.b[i][e] * back) : 0.f;
       }
-    z.store(r.out + b * r.o_b + t * r.o_t + head * r.o_h, slots, in);
-    for (g += kWaves; g >= groups; g -= groups) ++t;
+    z.store(out, slots, in);
   }
   if (!r.partial) return;
 #pragma unroll
@@ -514,7 +559,6 @@ int run_entries(const QkArgs& a, int es, bool grad) {
   else if (v == 4) { DA_QK_LANES(CALL, DT, 4, IL) }                           \
   else { DA_QK_SINGLE(CALL, DT, IL) }
 #define DA_QK_DISPATCH(CALL)                                        \
-  const int64_t slots = pairs / v;                                  \
   if (dtype == DA_BF16) {                                           \
     if (interleaved) { DA_QK_RUNS(CALL, DA_BF16, true) }            \
     else { DA_QK_RUNS(CALL, DA_BF16, false) }                       \
@@ -549,9 +593,15 @@ int da_qk_norm_rope(const da_qk_side* sides, int dtype, int weight_dtype, int64_
   hipStream_t st = (hipStream_t)stream;
   const int64_t pairs = rot / 2 + (d - rot + 1) / 2;
   const int v = run_entries(a, es, false);
-  a.parts = 1;
-  const int64_t blocks = (batch * tokens * a.parts + kWaves - 1) / kWaves;
-  if (blocks > 0x7fffffff) return set_error(DA_ERR_UNSUPPORTED, "da_qk_norm_rope: too many tokens");
+  const int64_t slots = pairs / v;
+  int lanes = 4;
+  while (lanes < 64 && lanes < slots) lanes *= 2;
+  const int64_t per_step = kWave / lanes;  // heads
+  const int64_t groups = (sides[0].heads + per_step - 1) / per_step + (sides[1].heads + per_step - 1) / per_step;
+  a.parts = (int)std::min<int64_t>(groups, std::max<int64_t>(1, kWantWaves / (batch * tokens)));
+  if (batch * tokens * a.parts > 0x7fffffff || sides[0].heads > 65535 || sides[1].heads > 65535)
+    return set_error(DA_ERR_UNSUPPORTED, "da_qk_norm_rope: up to 2^31 tokens and 65535 heads");
+  const int64_t blocks = std::min<int64_t>((batch * tokens * a.parts + kWaves - 1) / kWaves, kMostBlocks);
 #define DA_QK_FWD(DT, V, L, S, IL) qk_rope_forward<DT, V, L, S, IL><<<(unsigned)blocks, kThreads, 0, st>>>(a);
   DA_QK_DISPATCH(DA_QK_FWD)
 #undef DA_QK_FWD
@@ -597,6 +647,7 @@ int da_qk_norm_rope_grad(const da_qk_side* sides, int dtype, int weight_dtype, i
   a.mask = mask, a.mask_b = mask_bstride, a.mask_t = mask_tstride, a.scaling = scaling, a.eps = eps;
   const int64_t pairs = rot / 2 + (d - rot + 1) / 2;
   const int v = run_entries(a, es, true);
+  const int64_t slots = pairs / v;
   const int64_t per_side = batch * a.chunks;
   if (2 * per_side > 0x7fffffff) return set_error(DA_ERR_UNSUPPORTED, "da_qk_norm_rope_grad: too many tokens");
   if (per_side) {
