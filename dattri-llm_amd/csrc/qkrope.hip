@@ -34,6 +34,8 @@ constexpr int kWaves = kThreads / kWave;
 constexpr int64_t kMaxD = 1024;
 constexpr int64_t kWantWaves = 4096;  // a token's heads are spread over waves while there are fewer
 constexpr int64_t kMostBlocks = 2048;
+constexpr int64_t kRows = 512;
+constexpr int64_t kWantBlocks = 512;
 
 struct Rows {  // one side's rows; strides in bytes
   const char* x;
@@ -43,6 +45,7 @@ struct Rows {  // one side's rows; strides in bytes
   float* wgrad;    // (batch, D), NULL: not wanted
   float* partial;  // (batch, chunks, D)
   int64_t heads;
+  int64_t chunk, chunks;  // backward: tokens of a workgroup, workgroups of a sample
   int64_t x_b, x_t, x_h, g_b, g_t, g_h, o_b, o_t, o_h;
 };
 
@@ -57,9 +60,7 @@ struct QkArgs {
   const uint8_t* mask;   // NULL: every token lives
   int64_t mask_b, mask_t;
   float scaling, eps;
-  int parts;            // forward: waves that share a token's heads
-  int64_t chunk;        // backward: tokens of a workgroup
-  int64_t chunks;       // backward: workgroups of a sample
+  int parts;  // forward: waves that share a token's heads
 };
 
 __device__ __forceinline__ float load_any(const void* p, int dt, int64_t i) {
@@ -253,10 +254,20 @@ __device__ __forceinline__ void lane_weights(const float* from, int l, float (&w
     }
 }
 
+// Sum over a group of kL lanes, in all of them: within sixteen lanes by DPP
+// (neighbours, pairs, then mirrored halves, whose lanes agree by then).
+template <int kCtrl>
+__device__ __forceinline__ float add_dpp(float v) {
+  return v + __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), kCtrl, 0xf, 0xf, true));
+}
 template <int kL>
 __device__ __forceinline__ float lanes_sum(float v) {
-#pragma unroll
-  for (int off = kL / 2; off > 0; off >>= 1) v += __shfl_xor(v, off, kWave);
+  v = add_dpp<0xb1>(v);                         // quad_perm [1, 0, 3, 2]
+  v = add_dpp<0x4e>(v);                         // quad_perm [2, 3, 0, 1]
+  if constexpr (kL >= 8) v = add_dpp<0x141>(v);   // row_half_mirror
+  if constexpr (kL >= 16) v = add_dpp<0x140>(v);  // row_mirror
+  if constexpr (kL >= 32) v += __shfl_xor(v, 16, kWave);
+  if constexpr (kL >= 64) v += __shfl_xor(v, 32, kWave);
   return v;
 }
 
@@ -346,7 +357,7 @@ __global__ __launch_bounds__(kThreads) void qk_rope_backward(QkArgs a, int64_t q
   const int which = (int64_t)blockIdx.x >= q_blocks;
   const Rows& r = a.side[which];
   const int64_t block = (int64_t)blockIdx.x - (which ? q_blocks : 0);
-  const int64_t b = block / a.chunks, chunk = block - b * a.chunks;
+  const int64_t b = block / r.chunks, chunk = block - b * r.chunks;
   Slot<V, kInter> slots[S];
 #pragma unroll
   for (int i = 0; i < S; ++i) slots[i].at(l + i * kL, a.d, a.rot);
@@ -360,7 +371,7 @@ __global__ __launch_bounds__(kThreads) void qk_rope_backward(QkArgs a, int64_t q
   for (int i = 0; i < S; ++i)
 #pragma unroll
     for (int e = 0; e < V; ++e) da_[i][e] = db_[i][e] = 0.f;
-  const int64_t t0 = chunk * a.chunk, t1 = min(t0 + a.chunk, a.tokens);
+  const int64_t t0 = chunk * r.chunk, t1 = min(t0 + r.chunk, a.tokens);
   // Steps of (token, group of heads), the waves in turn; the next step's rows are loaded ahead.
   int64_t t = groups ? t0 + wave / groups : t1, last = -1;
   int g = groups ? wave % groups : 0;
@@ -399,19 +410,17 @@ __global__ __launch_bounds__(kThreads) void qk_rope_backward(QkArgs a, int64_t q
         sq += x.a[i][e] * x.a[i][e] + x.b[i][e] * x.b[i][e];
         along += ya * wa[i][e] * x.a[i][e] + yb * wb[i][e] * x.b[i][e];
       }
-    const float rms = rsqrtf(lanes_sum<kL>(sq) * inv_d + a.eps);
+    // Rows that are not there, or a dead token's, are zero, and stay zero without an eps.
+    const float rms = in && lives ? rsqrtf(lanes_sum<kL>(sq) * inv_d + a.eps) : 0.f;
     const float back = lanes_sum<kL>(along) * inv_d * rms * rms;
-    const bool adds = in && lives;
 #pragma unroll
     for (int i = 0; i < S; ++i)
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        // A head or token that is not there has an infinite 1/rms where eps
-        // is 0: selected out, not multiplied by zero.
-        da_[i][e] += adds ? z.a[i][e] * (x.a[i][e] * rms) : 0.f;
-        db_[i][e] += adds ? z.b[i][e] * (x.b[i][e] * rms) : 0.f;
-        z.a[i][e] = lives ? rms * (z.a[i][e] * wa[i][e] - x.a[i][e] * back) : 0.f;
-        z.b[i][e] = lives ? rms * (z.b[i][e] * wb[i][e] - x.b[i][e] * back) : 0.f;
+        da_[i][e] += z.a[i][e] * (x.a[i][e] * rms);
+        db_[i][e] += z.b[i][e] * (x.b[i][e] * rms);
+        z.a[i][e] = rms * (z.a[i][e] * wa[i][e] - x.a[i][e] * back);
+        z.b[i][e] = rms * (z.b[i][e] * wb[i][e] - x.b[i][e] * back);
       }
     z.store(out, slots, in);
   }
@@ -433,7 +442,7 @@ __global__ __launch_bounds__(kThreads) void qk_rope_backward(QkArgs a, int64_t q
     }
   __syncthreads();
   if (wave == 0 && sub == 0) {
-    float* out = r.partial + (b * a.chunks + chunk) * a.d;
+    float* out = r.partial + (b * r.chunks + chunk) * a.d;
 #pragma unroll
     for (int i = 0; i < S; ++i)
 #pragma unroll
@@ -452,17 +461,27 @@ __global__ __launch_bounds__(kThreads) void qk_rope_backward(QkArgs a, int64_t q
   }
 }
 
-// dw of a sample: its chunks' partials in ascending order.
+// dw of a sample: eight threads an entry take its chunks in turn and are added in
+// order.
 __global__ __launch_bounds__(kThreads) void qk_rope_join(QkArgs a) {
-  const int64_t n = a.batch * a.d;
-  const int64_t at = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  if (at >= n) return;
-  const Rows& r = a.side[blockIdx.y];
+  __shared__ float sums[8][32];
+  const Rows& r = a.side[blockIdx.z];
   if (!r.wgrad) return;
-  const int64_t b = at / a.d, i = at - b * a.d;
+  const int64_t b = blockIdx.y;
+  const int x = threadIdx.x % 32, y = threadIdx.x / 32, i = blockIdx.x * 32 + x;
   float v = 0.f;
-  for (int64_t c = 0; c < a.chunks; ++c) v += r.partial[(b * a.chunks + c) * a.d + i];
-  r.wgrad[at] = v;
+  if (i < a.d) {
+    const float* p = r.partial + b * r.chunks * a.d + i;
+#pragma unroll 4
+    for (int64_t c = y; c < r.chunks; c += 8) v += p[c * a.d];
+  }
+  sums[y][x] = v;
+  __syncthreads();
+  if (y == 0 && i < a.d) {
+#pragma unroll
+    for (int k = 1; k < 8; ++k) v += sums[k][x];
+    r.wgrad[b * a.d + i] = v;
+  }
 }
 
 int check_args(const char* what, const da_qk_side* sides, int dtype, int weight_dtype, int64_t batch, int64_t tokens,
@@ -495,10 +514,11 @@ void fill_side(Rows& r, const da_qk_side& s, int es) {
   r.o_b = s.out_bstride * es, r.o_t = s.out_tstride * es, r.o_h = s.out_hstride * es;
 }
 
-void chunking(int64_t batch, int64_t tokens, int64_t* chunk, int64_t* chunks) {
-  *chunk = 16;
-  *chunks = (tokens + 15) / 16;
-  (void)batch;
+// Backward: tokens of a workgroup of one side, about kRows rows, fewer where that
+// leaves less than kWantBlocks workgroups.
+int64_t chunk_tokens(int64_t batch, int64_t tokens, int64_t heads) {
+  const int64_t most = std::max<int64_t>(1, kRows / std::max<int64_t>(heads, 1));
+  return std::max<int64_t>(1, std::min(most, batch * tokens / kWantBlocks));
 }
 
 }  // namespace
@@ -608,12 +628,15 @@ int da_qk_norm_rope(const da_qk_side* sides, int dtype, int weight_dtype, int64_
   return check_launch("da_qk_norm_rope");
 }
 
-int da_qk_norm_rope_grad_workspace(int64_t batch, int64_t tokens, int64_t d, size_t* bytes) {
-  if (!bytes || batch < 0 || tokens < 0 || d < 0)
+int da_qk_norm_rope_grad_workspace(int64_t batch, int64_t tokens, int64_t q_heads, int64_t k_heads, int64_t d,
+                                   size_t* bytes) {
+  if (!bytes || batch < 0 || tokens < 0 || q_heads < 0 || k_heads < 0 || d < 0)
     return set_error(DA_ERR_INVALID, "da_qk_norm_rope_grad_workspace: bad argument");
-  int64_t chunk, chunks;
-  chunking(batch, tokens, &chunk, &chunks);
-  *bytes = (size_t)(2 * batch * chunks * d) * sizeof(float);
+  *bytes = 0;
+  for (int64_t heads : {q_heads, k_heads}) {
+    const int64_t chunk = chunk_tokens(batch, tokens, heads);
+    *bytes += (size_t)(batch * ((tokens + chunk - 1) / chunk) * d) * sizeof(float);
+  }
   return DA_OK;
 }
 
@@ -636,30 +659,35 @@ int da_qk_norm_rope_grad(const da_qk_side* sides, int dtype, int weight_dtype, i
   }
   if (!batch) return DA_OK;
   hipStream_t st = (hipStream_t)stream;
-  chunking(batch, tokens, &a.chunk, &a.chunks);
-  const size_t need = (size_t)(2 * batch * a.chunks * d) * sizeof(float);
-  if (wanted && need && (!workspace || workspace_bytes < need))
+  size_t need = 0;
+  for (int i = 0; i < 2; ++i) {
+    Rows& r = a.side[i];
+    r.chunk = chunk_tokens(batch, tokens, r.heads);
+    r.chunks = (tokens + r.chunk - 1) / r.chunk;
+    if (!r.wgrad) continue;
+    r.partial = (float*)((char*)workspace + need);
+    need += (size_t)(batch * r.chunks * d) * sizeof(float);
+  }
+  if (need && (!workspace || workspace_bytes < need))
     return set_error(DA_ERR_WORKSPACE, "da_qk_norm_rope_grad: workspace of %zu bytes, %zu needed", workspace_bytes, need);
-  for (int i = 0; i < 2; ++i)
-    a.side[i].partial = a.side[i].wgrad ? (float*)workspace + (int64_t)i * batch * a.chunks * d : nullptr;
   a.batch = batch, a.tokens = tokens, a.d = (int)d, a.rot = (int)rot, a.w_dtype = weight_dtype;
   a.inv_freq = inv_freq, a.pos = positions, a.pos_bytes = position_bytes, a.pos_b = pos_bstride, a.pos_t = pos_tstride;
   a.mask = mask, a.mask_b = mask_bstride, a.mask_t = mask_tstride, a.scaling = scaling, a.eps = eps;
   const int64_t pairs = rot / 2 + (d - rot + 1) / 2;
   const int v = run_entries(a, es, true);
   const int64_t slots = pairs / v;
-  const int64_t per_side = batch * a.chunks;
-  if (2 * per_side > 0x7fffffff) return set_error(DA_ERR_UNSUPPORTED, "da_qk_norm_rope_grad: too many tokens");
-  if (per_side) {
-    const int64_t blocks = 2 * per_side;
+  const int64_t q_blocks = batch * a.side[0].chunks, blocks = q_blocks + batch * a.side[1].chunks;
+  if (blocks > 0x7fffffff || batch > 65535 || sides[0].heads > 65535 || sides[1].heads > 65535)
+    return set_error(DA_ERR_UNSUPPORTED, "da_qk_norm_rope_grad: up to 2^31 tokens, 65535 samples and heads");
+  if (blocks) {
 #define DA_QK_BWD(DT, V, L, S, IL) \
-  qk_rope_backward<DT, V, L, S, IL><<<(unsigned)blocks, kThreads, 0, st>>>(a, per_side);
+  qk_rope_backward<DT, V, L, S, IL><<<(unsigned)blocks, kThreads, 0, st>>>(a, q_blocks);
     DA_QK_DISPATCH(DA_QK_BWD)
 #undef DA_QK_BWD
     if (int rc = check_launch("da_qk_norm_rope_grad")) return rc;
   }
   if (wanted) {
-    qk_rope_join<<<dim3((unsigned)((batch * d + kThreads - 1) / kThreads), 2), kThreads, 0, st>>>(a);
+    qk_rope_join<<<dim3((unsigned)((d + 31) / 32), (unsigned)batch, 2), kThreads, 0, st>>>(a);
     return check_launch("da_qk_norm_rope_grad (join)");
   }
   return DA_OK;

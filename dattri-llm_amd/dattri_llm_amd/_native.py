@@ -216,7 +216,7 @@ _EDGES = ctypes.POINTER(ctypes.c_int32)
 SIGNATURES.update(
     {
         "da_qk_norm_rope": (_I32, [*_QK, _P]),
-        "da_qk_norm_rope_grad_workspace": (_I32, [_I64, _I64, _I64, ctypes.POINTER(_SZ)]),
+        "da_qk_norm_rope_grad_workspace": (_I32, [_I64, _I64, _I64, _I64, _I64, ctypes.POINTER(_SZ)]),
         "da_qk_norm_rope_grad": (_I32, [*_QK, _P, _SZ, _P]),
         "da_relative_bias": (
             _I32, [_P, _I32, _I64, _I64, _I64, _I64, _I64, _I64, _EDGES, _I32, _I32, _I32, _P, _P]),

@@ -1570,7 +1570,8 @@ def _qk_rope(what, q, k, q_weight, k_weight, inv_freq, positions, mask, gq, gk, 
         _run_on(dev, what, lib.da_qk_norm_rope, *args, nat.stream_ptr(dev))
         return outs
     nbytes = ctypes.c_size_t(0)
-    nat.check(lib.da_qk_norm_rope_grad_workspace(b, t, d, ctypes.byref(nbytes)), what)
+    nat.check(lib.da_qk_norm_rope_grad_workspace(b, t, sides[0].heads, sides[1].heads, d, ctypes.byref(nbytes)),
+              what)
     ws = nat.workspace(nbytes.value if grads else 0, dev)
     _run_on(dev, what, lib.da_qk_norm_rope_grad, *args, ws.data_ptr(), ws.numel(), nat.stream_ptr(dev))
     del keep

@@ -763,7 +763,8 @@ int da_qk_norm_rope(const da_qk_side* sides, int dtype, int weight_dtype, int64_
                     int64_t rot, const float* inv_freq, const void* positions, int position_bytes,
                     int64_t pos_bstride, int64_t pos_tstride, const uint8_t* mask, int64_t mask_bstride,
                     int64_t mask_tstride, int interleaved, float scaling, float eps, void* stream);
-int da_qk_norm_rope_grad_workspace(int64_t batch, int64_t tokens, int64_t d, size_t* bytes);
+int da_qk_norm_rope_grad_workspace(int64_t batch, int64_t tokens, int64_t q_heads, int64_t k_heads, int64_t d,
+                                   size_t* bytes);
 int da_qk_norm_rope_grad(const da_qk_side* sides, int dtype, int weight_dtype, int64_t batch, int64_t tokens,
                          int64_t d, int64_t rot, const float* inv_freq, const void* positions, int position_bytes,
                          int64_t pos_bstride, int64_t pos_tstride, const uint8_t* mask, int64_t mask_bstride,

@@ -182,7 +182,7 @@ def test_c_abi_qk_norm_rope_checks():
     refused(back(X, 16), nat.DA_ERR_WORKSPACE, "needed")
     sides[0].gz = None
     refused(back(X, 1 << 20), nat.DA_ERR_INVALID, "NULL pointer of side 0")
-    refused(lib.da_qk_norm_rope_grad_workspace(1, 1, 8, None), nat.DA_ERR_INVALID, "argument")
+    refused(lib.da_qk_norm_rope_grad_workspace(1, 1, 1, 1, 8, None), nat.DA_ERR_INVALID, "argument")
 
 
 def test_c_abi_relative_bias_checks():
