@@ -34,7 +34,12 @@ constexpr int kWaves = kThreads / kWave;
 constexpr int64_t kMaxD = 1024;
 constexpr int64_t kWantWaves = 4096;  // a token's heads are spread over waves while there are fewer
 constexpr int64_t kMostBlocks = 2048;
-constexpr int64_t kRows = 512;
+// Rows of this many bytes in all are read past the caches.  Fewer may lie in the
+// last-level cache (256 MB) from the kernel that wrote them: at 84 MB of rows
+// (4 x 2048 tokens, 32 + 8 heads of 128, bf16) both take 34 us forward, at 168 MB
+// 70 us with cached loads, 58 us with streamed ones; 21 MB: 10.9 and 12.7 us.
+constexpr int64_t kStreamBytes = 128 << 20;
+constexpr int64_t kRows = 1024;
 constexpr int64_t kWantBlocks = 512;
 
 struct Rows {  // one side's rows; strides in bytes
@@ -118,28 +123,34 @@ struct Run {  // V entries as they lie in memory, in one access
   static constexpr int kBytes = V * Elem<DT>::kBytes, kWords = kBytes < 4 ? 1 : kBytes / 4;
   typedef uint32_t Words __attribute__((ext_vector_type(kWords)));
   Words w;
+  template <bool kStream>
   __device__ void load(const char* p, bool in) {
     w = Words(0);
     if (!in) return;
     if constexpr (kBytes == 2) w[0] = *(const uint16_t*)p;
+    else if constexpr (kStream) w = __builtin_nontemporal_load((const Words*)p);
     else w = *(const Words*)p;
   }
   __device__ float get(int i) const {
     if constexpr (DT == DA_F32) return __uint_as_float(w[i]);
     else return Elem<DT>::from_bits(i & 1 ? w[i >> 1] >> 16 : w[i >> 1] & 0xffffu);
   }
-  __device__ static void store(char* p, const float* v, bool in) {
-    if (!in) return;
-    if constexpr (V == 1) Elem<DT>::store(p, 0, v[0]);
-    else {
-      Words w;
+  template <class Vec>
+  __device__ void pack(const Vec& v) {
+    if constexpr (DT == DA_F32) {
 #pragma unroll
-      for (int i = 0; i < kWords; ++i) {
-        if constexpr (DT == DA_F32) w[i] = __float_as_uint(v[i]);
-        else w[i] = pack2<DT>(v[2 * i], v[2 * i + 1]);
-      }
-      *(Words*)p = w;
+      for (int i = 0; i < V; ++i) w[i] = __float_as_uint(v[i]);
+    } else if constexpr (V == 1) {
+      w[0] = DT == DA_BF16 ? f32_to_bf16_bits(v[0]) : f32_to_f16_bits(v[0]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < V / 2; ++i) w[i] = pack2<DT>(v[2 * i], v[2 * i + 1]);
     }
+  }
+  __device__ void store(char* p, bool in) const {
+    if (!in) return;
+    if constexpr (kBytes == 2) *(uint16_t*)p = (uint16_t)w[0];
+    else *(Words*)p = w;
   }
 };
 
@@ -147,12 +158,13 @@ struct Run {  // V entries as they lie in memory, in one access
 template <int DT, int V, int S, bool kInter>
 struct RawRow {
   Run<DT, V> u[S], v[S];
+  template <bool kStream>
   __device__ void load(const char* p, const Slot<V, kInter>* slots, bool live) {
     constexpr int ES = Elem<DT>::kBytes;
 #pragma unroll
     for (int i = 0; i < S; ++i) {
-      u[i].load(p + (int64_t)slots[i].a * ES, live && slots[i].in);
-      v[i].load(p + (int64_t)slots[i].b * ES, live && slots[i].in && slots[i].has_b);
+      u[i].template load<kStream>(p + (int64_t)slots[i].a * ES, live && slots[i].in);
+      v[i].template load<kStream>(p + (int64_t)slots[i].b * ES, live && slots[i].in && slots[i].has_b);
     }
   }
 };
@@ -161,16 +173,22 @@ struct RawRow {
 // members alternately.
 template <int DT, int V, int S, bool kInter>
 struct Row {
-  float a[S][V], b[S][V];
+  typedef float Vec __attribute__((ext_vector_type(V)));
+  Vec a[S], b[S];
   __device__ void unpack(const RawRow<DT, V, S, kInter>& raw) {
 #pragma unroll
     for (int i = 0; i < S; ++i) {
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         if constexpr (kInter && V > 1) {
-          const Run<DT, V>& from = 2 * e < V ? raw.u[i] : raw.v[i];
-          a[i][e] = from.get(2 * e % V);
-          b[i][e] = from.get(2 * e % V + 1);
+          if constexpr (DT == DA_F32) {
+            a[i][e] = __uint_as_float(e < V / 2 ? raw.u[i].w[2 * e % V] : raw.v[i].w[2 * e % V]);
+            b[i][e] = __uint_as_float(e < V / 2 ? raw.u[i].w[2 * e % V + 1] : raw.v[i].w[2 * e % V + 1]);
+          } else {  // a pair is a word
+            const uint32_t pair = e < V / 2 ? raw.u[i].w[e % (V / 2)] : raw.v[i].w[e % (V / 2)];
+            a[i][e] = Elem<DT>::from_bits(pair & 0xffffu);
+            b[i][e] = Elem<DT>::from_bits(pair >> 16);
+          }
         } else {
           a[i][e] = raw.u[i].get(e);
           b[i][e] = raw.v[i].get(e);
@@ -182,19 +200,29 @@ struct Row {
     constexpr int ES = Elem<DT>::kBytes;
 #pragma unroll
     for (int i = 0; i < S; ++i) {
-      float u[V], v[V];
+      if constexpr (kInter && V > 1) {
+        Run<DT, V> u, v;
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        if constexpr (kInter && V > 1) {
-          u[e] = e % 2 ? b[i][e / 2] : a[i][e / 2];
-          v[e] = e % 2 ? b[i][(V + e) / 2] : a[i][(V + e) / 2];
-        } else {
-          u[e] = a[i][e];
-          v[e] = b[i][e];
+        for (int e = 0; e < V / 2; ++e) {
+          if constexpr (DT == DA_F32) {
+            u.w[2 * e] = __float_as_uint(a[i][e]);
+            u.w[2 * e + 1] = __float_as_uint(b[i][e]);
+            v.w[2 * e] = __float_as_uint(a[i][V / 2 + e]);
+            v.w[2 * e + 1] = __float_as_uint(b[i][V / 2 + e]);
+          } else {
+            u.w[e] = pack2<DT>(a[i][e], b[i][e]);
+            v.w[e] = pack2<DT>(a[i][V / 2 + e], b[i][V / 2 + e]);
+          }
         }
+        u.store(p + (int64_t)slots[i].a * ES, live && slots[i].in);
+        v.store(p + (int64_t)slots[i].b * ES, live && slots[i].in);
+        continue;
       }
-      Run<DT, V>::store(p + (int64_t)slots[i].a * ES, u, live && slots[i].in);
-      Run<DT, V>::store(p + (int64_t)slots[i].b * ES, v, live && slots[i].in && slots[i].has_b);
+      Run<DT, V> u, v;
+      u.pack(a[i]);
+      v.pack(b[i]);
+      u.store(p + (int64_t)slots[i].a * ES, live && slots[i].in);
+      v.store(p + (int64_t)slots[i].b * ES, live && slots[i].in && slots[i].has_b);
     }
   }
 };
@@ -273,7 +301,7 @@ __device__ __forceinline__ float lanes_sum(float v) {
 
 // A wave takes units in turn: a token's heads, or every `parts`-th group of them
 // where the tokens are few.
-template <int DT, int V, int kL, int S, bool kInter>
+template <int DT, int V, int kL, int S, bool kInter, bool kStream>
 __global__ __launch_bounds__(kThreads) void qk_rope_forward(QkArgs a) {
   constexpr int kHeads = kWave / kL, kPairs = kL * S * V;  // heads of a wave's step, pairs of a head
   __shared__ float2 tables[kWaves][kPairs];
@@ -306,7 +334,7 @@ __global__ __launch_bounds__(kThreads) void qk_rope_forward(QkArgs a) {
         char* out_row = r.out + b * r.o_b + t * r.o_t + head * r.o_h;
         const int64_t x_step = r.x_h * kHeads * a.parts, out_step = r.o_h * kHeads * a.parts;
         RawRow<DT, V, S, kInter> raw;
-        raw.load(x_row, slots, head < heads && live);
+        raw.template load<kStream>(x_row, slots, head < heads && live);
         if (!turned) angles<V, kL, S>(a, b, t, tables[wave], lane, l, c, s);
         turned = true;
         float wa[S][V], wb[S][V];
@@ -317,7 +345,7 @@ __global__ __launch_bounds__(kThreads) void qk_rope_forward(QkArgs a) {
           const bool in = head < heads;
           head += kHeads * a.parts;
           x_row += x_step;
-          if (g + a.parts < end) raw.load(x_row, slots, head < heads && live);
+          if (g + a.parts < end) raw.template load<kStream>(x_row, slots, head < heads && live);
           float sq = 0.f;
 #pragma unroll
           for (int i = 0; i < S; ++i)
@@ -345,7 +373,7 @@ __global__ __launch_bounds__(kThreads) void qk_rope_forward(QkArgs a) {
 // A workgroup owns one side's rows of `chunk` tokens of a sample; its waves
 // take (token, group of heads) steps in turn and add their lanes' dw up, the
 // waves' sums meet in LDS and go to the chunk's place of the partials in fp32.
-template <int DT, int V, int kL, int S, bool kInter>
+template <int DT, int V, int kL, int S, bool kInter, bool kStream>
 __global__ __launch_bounds__(kThreads) void qk_rope_backward(QkArgs a, int64_t q_blocks) {
   constexpr int kHeads = kWave / kL;
   constexpr int kPairs = kL * S * V;
@@ -366,7 +394,6 @@ __global__ __launch_bounds__(kThreads) void qk_rope_backward(QkArgs a, int64_t q
   const int groups = ((int)r.heads + kHeads - 1) / kHeads;
   if (groups) weights<kInter>(a, r.w, w, kPairs);  // an absent side has no weight to read
   __syncthreads();
-  lane_weights<V, kL, S>(w, l, wa, wb);
 #pragma unroll
   for (int i = 0; i < S; ++i)
 #pragma unroll
@@ -380,8 +407,8 @@ __global__ __launch_bounds__(kThreads) void qk_rope_backward(QkArgs a, int64_t q
   auto load = [&]() {
     live = !a.mask || a.mask[b * a.mask_b + t * a.mask_t];
     const int64_t head = g * kHeads + sub;
-    raw_x.load(r.x + b * r.x_b + t * r.x_t + head * r.x_h, slots, head < r.heads && live);
-    raw_z.load(r.gz + b * r.g_b + t * r.g_t + head * r.g_h, slots, head < r.heads && live);
+    raw_x.template load<kStream>(r.x + b * r.x_b + t * r.x_t + head * r.x_h, slots, head < r.heads && live);
+    raw_z.template load<kStream>(r.gz + b * r.g_b + t * r.g_t + head * r.g_h, slots, head < r.heads && live);
   };
   if (t < t1) load();
   float c[S][V], s[S][V];
@@ -398,6 +425,8 @@ __global__ __launch_bounds__(kThreads) void qk_rope_backward(QkArgs a, int64_t q
     z.unpack(raw_z);
     for (g += kWaves; g >= groups; g -= groups) ++t;
     if (t < t1) load();
+    asm volatile("" ::: "memory");  // the weights stay in LDS: registers bound the waves of a SIMD
+    lane_weights<V, kL, S>(w, l, wa, wb);
     float sq = 0.f, along = 0.f;
 #pragma unroll
     for (int i = 0; i < S; ++i)
@@ -550,45 +579,55 @@ int run_entries(const QkArgs& a, int es, bool grad) {
 }
 }  // namespace
 
-#define DA_QK_LANES(CALL, DT, V, IL)      \
-  if (slots <= 4) {                       \
-    CALL(DT, V, 4, 1, IL)                 \
-  } else if (slots <= 8) {                \
-    CALL(DT, V, 8, 1, IL)                 \
-  } else if (slots <= 16) {               \
-    CALL(DT, V, 16, 1, IL)                \
-  } else if (slots <= 32) {               \
-    CALL(DT, V, 32, 1, IL)                \
-  } else if (slots <= 64) {               \
-    CALL(DT, V, 64, 1, IL)                \
-  } else {                                \
-    CALL(DT, V, 64, 2, IL)                \
+namespace {
+
+// Launches the forward or the backward kernel for the operands' type, the entries
+// of a run, the lanes of a head (one slot each, or several slots of 64 lanes) and
+// the order of the pairs.
+struct Launch {
+  const QkArgs& a;
+  bool grad;
+  int64_t blocks, q_blocks;
+  hipStream_t stream;
+
+  template <int DT, int V, int kL, int S, bool kInter, bool kStream>
+  void kernel() const {
+    if (grad) qk_rope_backward<DT, V, kL, S, kInter, kStream><<<(unsigned)blocks, kThreads, 0, stream>>>(a, q_blocks);
+    else qk_rope_forward<DT, V, kL, S, kInter, kStream><<<(unsigned)blocks, kThreads, 0, stream>>>(a);
   }
-#define DA_QK_SINGLE(CALL, DT, IL)        \
-  if (pairs <= 64) {                      \
-    CALL(DT, 1, 64, 1, IL)                \
-  } else if (pairs <= 128) {              \
-    CALL(DT, 1, 64, 2, IL)                \
-  } else if (pairs <= 256) {              \
-    CALL(DT, 1, 64, 4, IL)                \
-  } else {                                \
-    CALL(DT, 1, 64, 8, IL)                \
+  template <int DT, int V, bool kInter, bool kStream>
+  void lanes(int64_t slots) const {
+    if (slots <= 4) kernel<DT, V, 4, 1, kInter, kStream>();
+    else if (slots <= 8) kernel<DT, V, 8, 1, kInter, kStream>();
+    else if (slots <= 16) kernel<DT, V, 16, 1, kInter, kStream>();
+    else if (slots <= 32) kernel<DT, V, 32, 1, kInter, kStream>();
+    else if (V == 8 || slots <= 64) kernel<DT, V, 64, 1, kInter, kStream>();
+    else if constexpr (V == 4) kernel<DT, V, 64, 2, kInter, kStream>();
   }
-#define DA_QK_RUNS(CALL, DT, IL)                                              \
-  if (DT != DA_F32 && v == 8) { DA_QK_LANES(CALL, DT, (DT == DA_F32 ? 4 : 8), IL) }                   \
-  else if (v == 4) { DA_QK_LANES(CALL, DT, 4, IL) }                           \
-  else { DA_QK_SINGLE(CALL, DT, IL) }
-#define DA_QK_DISPATCH(CALL)                                        \
-  if (dtype == DA_BF16) {                                           \
-    if (interleaved) { DA_QK_RUNS(CALL, DA_BF16, true) }            \
-    else { DA_QK_RUNS(CALL, DA_BF16, false) }                       \
-  } else if (dtype == DA_F16) {                                     \
-    if (interleaved) { DA_QK_RUNS(CALL, DA_F16, true) }             \
-    else { DA_QK_RUNS(CALL, DA_F16, false) }                        \
-  } else {                                                          \
-    if (interleaved) { DA_QK_RUNS(CALL, DA_F32, true) }             \
-    else { DA_QK_RUNS(CALL, DA_F32, false) }                        \
+  template <int DT, bool kInter>
+  void runs(int v, int64_t pairs, bool streamed) const {
+    constexpr int kFull = 16 / Elem<DT>::kBytes;
+    if (v == kFull && streamed) lanes<DT, kFull, kInter, true>(pairs / v);
+    else if (v == kFull) lanes<DT, kFull, kInter, false>(pairs / v);
+    else if (v == 4) lanes<DT, 4, kInter, false>(pairs / v);
+    else if (pairs <= 64) kernel<DT, 1, 64, 1, kInter, false>();
+    else if (pairs <= 128) kernel<DT, 1, 64, 2, kInter, false>();
+    else if (pairs <= 256) kernel<DT, 1, 64, 4, kInter, false>();
+    else kernel<DT, 1, 64, 8, kInter, false>();
   }
+  void operator()(int dtype, bool interleaved, int v, int64_t pairs) const {
+    const bool streamed = rows_bytes() >= kStreamBytes;
+    if (dtype == DA_BF16) interleaved ? runs<DA_BF16, true>(v, pairs, streamed) : runs<DA_BF16, false>(v, pairs, streamed);
+    else if (dtype == DA_F16) interleaved ? runs<DA_F16, true>(v, pairs, streamed) : runs<DA_F16, false>(v, pairs, streamed);
+    else interleaved ? runs<DA_F32, true>(v, pairs, streamed) : runs<DA_F32, false>(v, pairs, streamed);
+  }
+  int64_t rows_bytes() const {
+    return a.batch * a.tokens * (a.side[0].heads + a.side[1].heads) * a.d * bytes * (grad ? 2 : 1);
+  }
+  int bytes;  // of an entry
+};
+
+}  // namespace
 
 extern "C" {
 
@@ -622,9 +661,7 @@ int da_qk_norm_rope(const da_qk_side* sides, int dtype, int weight_dtype, int64_
   if (batch * tokens * a.parts > 0x7fffffff || sides[0].heads > 65535 || sides[1].heads > 65535)
     return set_error(DA_ERR_UNSUPPORTED, "da_qk_norm_rope: up to 2^31 tokens and 65535 heads");
   const int64_t blocks = std::min<int64_t>((batch * tokens * a.parts + kWaves - 1) / kWaves, kMostBlocks);
-#define DA_QK_FWD(DT, V, L, S, IL) qk_rope_forward<DT, V, L, S, IL><<<(unsigned)blocks, kThreads, 0, st>>>(a);
-  DA_QK_DISPATCH(DA_QK_FWD)
-#undef DA_QK_FWD
+  Launch{a, false, blocks, 0, st, es}(dtype, interleaved, v, pairs);
   return check_launch("da_qk_norm_rope");
 }
 
@@ -675,15 +712,11 @@ int da_qk_norm_rope_grad(const da_qk_side* sides, int dtype, int weight_dtype, i
   a.mask = mask, a.mask_b = mask_bstride, a.mask_t = mask_tstride, a.scaling = scaling, a.eps = eps;
   const int64_t pairs = rot / 2 + (d - rot + 1) / 2;
   const int v = run_entries(a, es, true);
-  const int64_t slots = pairs / v;
   const int64_t q_blocks = batch * a.side[0].chunks, blocks = q_blocks + batch * a.side[1].chunks;
   if (blocks > 0x7fffffff || batch > 65535 || sides[0].heads > 65535 || sides[1].heads > 65535)
     return set_error(DA_ERR_UNSUPPORTED, "da_qk_norm_rope_grad: up to 2^31 tokens, 65535 samples and heads");
   if (blocks) {
-#define DA_QK_BWD(DT, V, L, S, IL) \
-  qk_rope_backward<DT, V, L, S, IL><<<(unsigned)blocks, kThreads, 0, st>>>(a, q_blocks);
-    DA_QK_DISPATCH(DA_QK_BWD)
-#undef DA_QK_BWD
+    Launch{a, true, blocks, q_blocks, st, es}(dtype, interleaved, v, pairs);
     if (int rc = check_launch("da_qk_norm_rope_grad")) return rc;
   }
   if (wanted) {
