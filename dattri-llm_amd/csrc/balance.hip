@@ -8,6 +8,15 @@
 //
 // (n = 0: zeros).  The counts carry no gradient.  A choice outside the experts
 // (a dropped one) counts for none.
+//
+// kL lanes share a token, each with S runs of V experts (16 bytes where the rows
+// allow it), and a wave takes 64 / kL tokens at once: the softmax is two butterflies
+// over kL lanes, a lane adds its experts' probabilities up in registers, and no
+// probability goes to memory.  A workgroup sums a chunk of one sample's tokens; a
+// sample of one chunk is finished there, else a second launch joins its chunks in
+// order.  Counts are whole numbers: their LDS atomics have no order to keep.
+#include <algorithm>
+
 #include "common.h"
 
 namespace da {
@@ -15,6 +24,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / kWave;
+constexpr int kJoinThreads = 512;
 constexpr int kMaxExperts = 1024;
 
 struct BalArgs {
@@ -24,11 +34,13 @@ struct BalArgs {
   int64_t tokens, batch;
   int64_t row, mask_b, mask_t;  // elements
   int experts, top;
-  float* partial;      // (batch, chunks, experts + 1): sums of p, sum of logsumexp^2
-  int32_t* part_live;  // (batch, chunks, experts + 1): counts, live tokens
+  float* p;        // (batch, chunks, experts): sums of the probabilities
+  int32_t* seen;   // (batch, chunks, experts): choices
+  float* z;        // (batch, chunks): sums of logsumexp^2
+  int32_t* n;      // (batch, chunks): live tokens
   int64_t chunk, chunks;
   float* loss;
-  float* z;
+  float* z_loss;
   int32_t* counts;
   int32_t* live;
   const float* up;
@@ -37,138 +49,306 @@ struct BalArgs {
   int64_t grad_row;
 };
 
-// One token's logits in a wave: lane l holds experts l, l + 64, ...
-template <int DT, int S>
+// ---------------------------------------------------------------------------
+// Reductions over a token's lanes.
+// ---------------------------------------------------------------------------
+template <int kCtrl>
+__device__ __forceinline__ float dpp(float v) {
+  return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), kCtrl, 0xf, 0xf, true));
+}
+// quad_perm [1, 0, 3, 2] and [2, 3, 0, 1], row_half_mirror, row_mirror: each pairs
+// lanes whose values already agree within the halves that it joins.
+template <int kL, class Op>
+__device__ __forceinline__ float over_lanes(float v, Op op) {
+  if constexpr (kL >= 2) v = op(v, dpp<0xb1>(v));
+  if constexpr (kL >= 4) v = op(v, dpp<0x4e>(v));
+  if constexpr (kL >= 8) v = op(v, dpp<0x141>(v));
+  if constexpr (kL >= 16) v = op(v, dpp<0x140>(v));
+  if constexpr (kL >= 32) v = op(v, __shfl_xor(v, 16, kWave));
+  if constexpr (kL >= 64) v = op(v, __shfl_xor(v, 32, kWave));
+  return v;
+}
+struct Sum {
+  __device__ float operator()(float a, float b) const { return a + b; }
+};
+struct Max {
+  __device__ float operator()(float a, float b) const { return fmaxf(a, b); }
+};
+
+// ---------------------------------------------------------------------------
+// One token's logits: lane l of its kL holds runs l, l + kL, ... of V experts.
+// ---------------------------------------------------------------------------
+template <int DT, int V, int kL, int S>
 struct Token {
-  float p[S];
-  float lse;
-  __device__ void load(const char* row, int experts, int lane) {
+  static constexpr int ES = Elem<DT>::kBytes;
+  u32x4 raw[V == 1 ? (S + 3) / 4 : S];  // V == 1: one value a word
+
+  __device__ void load(const char* row, int experts, int l, bool live) {
+#pragma unroll
+    for (int i = 0; i < S; ++i) {
+      const int e = (l + i * kL) * V;
+      const bool in = live && e < experts;
+      if constexpr (V == 1) {
+        uint32_t w = 0;
+        if (in) w = ES == 4 ? *(const uint32_t*)(row + e * ES) : *(const uint16_t*)(row + e * ES);
+        raw[i / 4][i % 4] = w;
+      } else {
+        raw[i] = u32x4{0, 0, 0, 0};
+        if (in) raw[i] = ld16(row + e * ES);
+      }
+    }
+  }
+  // p = softmax of the logits, 0 past the experts; returns their logsumexp.
+  __device__ float softmax(int experts, int l, float (&p)[S][V]) const {
     float top = -__builtin_inff();
 #pragma unroll
     for (int i = 0; i < S; ++i) {
-      const int e = lane + i * kWave;
-      p[i] = e < experts ? Elem<DT>::load(row, e) : -__builtin_inff();
-      top = fmaxf(top, p[i]);
-    }
+      const bool in = (l + i * kL) * V < experts;
+      float x[V];
+      if constexpr (V == 1) x[0] = Elem<DT>::from_bits(raw[i / 4][i % 4]);
+      else unpack16<DT>(raw[i], x);
 #pragma unroll
-    for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, kWave));
+      for (int e = 0; e < V; ++e) {
+        p[i][e] = in ? x[e] : -__builtin_inff();
+        top = fmaxf(top, p[i][e]);
+      }
+    }
+    top = over_lanes<kL>(top, Max());
     float sum = 0.f;
 #pragma unroll
     for (int i = 0; i < S; ++i) {
-      const int e = lane + i * kWave;
-      p[i] = e < experts ? expf(p[i] - top) : 0.f;
-      sum += p[i];
+      const bool in = (l + i * kL) * V < experts;
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        // The difference is exact or rounded once; its product with log2(e) is off
+        // by at most 2^-24 of itself, which a probability below e^-16 alone notices.
+        const float x = __builtin_amdgcn_exp2f((p[i][e] - top) * 1.44269504088896341f);
+        p[i][e] = in ? x : 0.f;  // all -inf: -inf - -inf is NaN, as in a softmax
+        sum += p[i][e];
+      }
     }
-    sum = wave_sum(sum);
+    sum = over_lanes<kL>(sum, Sum());
     const float inv = 1.f / sum;
 #pragma unroll
-    for (int i = 0; i < S; ++i) p[i] *= inv;
-    lse = top + logf(sum);
+    for (int i = 0; i < S; ++i)
+#pragma unroll
+      for (int e = 0; e < V; ++e) p[i][e] *= inv;
+    return top + logf(sum);
   }
 };
 
-template <int DT, int S>
-__global__ __launch_bounds__(kThreads) void balance_partials(BalArgs a) {
-  extern __shared__ char lds[];
-  const int w = a.experts + 1;
-  float* sums = (float*)lds;                // [kWaves][w]
-  int32_t* seen = (int32_t*)(sums + kWaves * w);  // [w]
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int64_t b = blockIdx.x / a.chunks, chunk = blockIdx.x - b * a.chunks;
-  for (int e = tid; e < w; e += kThreads) seen[e] = 0;
-  __syncthreads();
-  const int64_t t0 = chunk * a.chunk, t1 = min(t0 + a.chunk, a.tokens);
-  float p[S], z = 0.f;
-#pragma unroll
-  for (int i = 0; i < S; ++i) p[i] = 0.f;
-  for (int64_t t = t0 + wave; t < t1; t += kWaves) {
-    if (a.mask && !a.mask[b * a.mask_b + t * a.mask_t]) continue;
-    Token<DT, S> x;
-    x.load(a.logits + (b * a.tokens + t) * a.row * Elem<DT>::kBytes, a.experts, lane);
-#pragma unroll
-    for (int i = 0; i < S; ++i) p[i] += x.p[i];
-    z += x.lse * x.lse;
-    for (int k = lane; k < a.top; k += kWave) {
-      const int64_t e = a.index[(b * a.tokens + t) * a.top + k];
-      if (e >= 0 && e < a.experts) atomicAdd(&seen[e], 1);
-    }
-    if (lane == 0) atomicAdd(&seen[a.experts], 1);
-  }
-#pragma unroll
-  for (int i = 0; i < S; ++i)
-    if (lane + i * kWave < a.experts) sums[wave * w + lane + i * kWave] = p[i];
-  if (lane == 0) sums[wave * w + a.experts] = z;
-  __syncthreads();
-  for (int e = tid; e < w; e += kThreads) {
-    float v = 0.f;
-    for (int k = 0; k < kWaves; ++k) v += sums[k * w + e];
-    a.partial[(int64_t)blockIdx.x * w + e] = v;
-    a.part_live[(int64_t)blockIdx.x * w + e] = seen[e];
-  }
-}
-
-__global__ __launch_bounds__(kThreads) void balance_join(BalArgs a) {
-  __shared__ float terms[kThreads];
-  const int w = a.experts + 1, tid = threadIdx.x;
-  const int64_t b = blockIdx.x;
-  int n = 0;
-  for (int64_t c = 0; c < a.chunks; ++c) n += a.part_live[(b * a.chunks + c) * w + a.experts];
+// A sample's losses from its sums in LDS; every thread of the workgroup calls.
+template <int kN>
+__device__ void finish(const BalArgs& a, int64_t b, const float* p, const int32_t* seen, float z, int n) {
+  __shared__ float terms[kN / kWave];
   const float inv = n ? 1.f / (float)n : 0.f;
   float term = 0.f;
-  for (int e = tid; e < w; e += kThreads) {
-    float v = 0.f;
-    int32_t k = 0;
-    for (int64_t c = 0; c < a.chunks; ++c) {
-      v += a.partial[(b * a.chunks + c) * w + e];
-      k += a.part_live[(b * a.chunks + c) * w + e];
-    }
-    if (e < a.experts) {
-      a.counts[b * a.experts + e] = k;
-      term += ((float)k * inv) * (v * inv);
-    } else {
-      a.z[b] = v * inv;
-      a.live[b] = k;
-    }
+  for (int e = threadIdx.x; e < a.experts; e += kN) {
+    a.counts[b * a.experts + e] = seen[e];
+    term += ((float)seen[e] * inv) * (p[e] * inv);
   }
-  terms[tid] = term;
+  term = wave_sum(term);
+  if (threadIdx.x % kWave == 0) terms[threadIdx.x / kWave] = term;
   __syncthreads();
-  for (int off = kThreads / 2; off > 0; off >>= 1) {
-    if (tid < off) terms[tid] += terms[tid + off];
-    __syncthreads();
+  if (threadIdx.x == 0) {
+    float sum = 0.f;
+    for (int w = 0; w < kN / kWave; ++w) sum += terms[w];
+    a.loss[b] = (float)a.experts * sum;
+    a.z_loss[b] = z * inv;
+    a.live[b] = n;
   }
-  if (tid == 0) a.loss[b] = (float)a.experts * terms[0];
 }
 
-template <int DT, int S>
-__global__ __launch_bounds__(kThreads) void balance_backward(BalArgs a) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t token = (int64_t)blockIdx.x * kWaves + wave;
-  if (token >= a.batch * a.tokens) return;
-  const int64_t b = token / a.tokens, t = token - b * a.tokens;
-  const int n = a.live[b];
-  const bool live = n > 0 && (!a.mask || a.mask[b * a.mask_b + t * a.mask_t]);
-  char* out = a.grad + token * a.grad_row * Elem<DT>::kBytes;
-  if (!live) {
-#pragma unroll
-    for (int i = 0; i < S; ++i)
-      if (lane + i * kWave < a.experts) Elem<DT>::store(out, lane + i * kWave, 0.f);
-    return;
-  }
-  const float inv = 1.f / (float)n;
-  Token<DT, S> x;
-  x.load(a.logits + token * a.row * Elem<DT>::kBytes, a.experts, lane);
-  float f[S], dot = 0.f;
-#pragma unroll
-  for (int i = 0; i < S; ++i) {
-    const int e = lane + i * kWave;
-    f[i] = e < a.experts ? (float)a.counts[b * a.experts + e] * inv : 0.f;
-    dot += f[i] * x.p[i];
-  }
-  dot = wave_sum(dot);
-  const float up = (a.up ? a.up[b] : 0.f) * (float)a.experts * inv, up_z = (a.up_z ? a.up_z[b] : 0.f) * 2.f * inv * x.lse;
+template <int DT, int V, int kL, int S>
+__global__ __launch_bounds__(kThreads) void balance_forward(BalArgs a) {
+  constexpr int kTokens = kWave / kL, kStep = kWaves * kTokens;  // tokens of a wave, of a workgroup's step
+  extern __shared__ char lds[];
+  float* sums = (float*)lds;                            // [kWaves][experts]
+  int32_t* seen = (int32_t*)(sums + kWaves * a.experts);  // [experts]
+  __shared__ float z_sums[kWaves];
+  __shared__ int n_sums[kWaves];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l = lane % kL, sub = lane / kL;
+  const int64_t b = blockIdx.x / a.chunks, chunk = blockIdx.x - b * a.chunks;
+  for (int e = tid; e < a.experts; e += kThreads) seen[e] = 0;
+  __syncthreads();
+  const int64_t t0 = chunk * a.chunk, t1 = min(t0 + a.chunk, a.tokens);
+  const uint8_t* mask = a.mask ? a.mask + b * a.mask_b : nullptr;
+  float p[S][V], z = 0.f;
+  int n = 0;
 #pragma unroll
   for (int i = 0; i < S; ++i)
-    if (lane + i * kWave < a.experts) Elem<DT>::store(out, lane + i * kWave, x.p[i] * (up * (f[i] - dot) + up_z));
+#pragma unroll
+    for (int e = 0; e < V; ++e) p[i][e] = 0.f;
+  int64_t t = t0 + wave * kTokens + sub;
+  const char* row = a.logits + (b * a.tokens + t) * a.row * Elem<DT>::kBytes;
+  Token<DT, V, kL, S> x;
+  bool live = t < t1 && (!mask || mask[t * a.mask_t]);
+  x.load(row, a.experts, l, live);
+  // The choices meanwhile: one entry a thread.
+  const int64_t* index = a.index + (b * a.tokens + t0) * a.top;
+  const int entries = (int)(t1 - t0) * a.top;
+  for (int at = tid; at < entries; at += kThreads) {
+    const int64_t e = index[at];
+    if (e >= 0 && e < a.experts && (!mask || mask[(t0 + at / a.top) * a.mask_t])) atomicAdd(&seen[e], 1);
+  }
+  for (int64_t first = t0; first < t1; first += kStep) {
+    const Token<DT, V, kL, S> now = x;
+    const bool counts = live;
+    t += kStep;
+    row += kStep * a.row * Elem<DT>::kBytes;
+    live = t < t1 && (!mask || mask[t * a.mask_t]);
+    x.load(row, a.experts, l, live);
+    float q[S][V];
+    const float lse = now.softmax(a.experts, l, q);
+    if (counts) {
+#pragma unroll
+      for (int i = 0; i < S; ++i)
+#pragma unroll
+        for (int e = 0; e < V; ++e) p[i][e] += q[i][e];
+      z += lse * lse;
+      ++n;
+    }
+  }
+  // The wave's tokens, then the waves.
+#pragma unroll
+  for (int i = 0; i < S; ++i)
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+#pragma unroll
+      for (int off = kL; off < kWave; off <<= 1) p[i][e] += __shfl_xor(p[i][e], off, kWave);
+      const int at = (l + i * kL) * V + e;
+      if (sub == 0 && at < a.experts) sums[wave * a.experts + at] = p[i][e];
+    }
+#pragma unroll
+  for (int off = kL; off < kWave; off <<= 1) {
+    z += __shfl_xor(z, off, kWave);
+    n += __shfl_xor(n, off, kWave);
+  }
+  if (lane == 0) z_sums[wave] = z, n_sums[wave] = n;
+  __syncthreads();
+  z = 0.f, n = 0;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) z += z_sums[w], n += n_sums[w];
+  const bool alone = a.chunks == 1;
+  for (int e = tid; e < a.experts; e += kThreads) {
+    float v = sums[e];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) v += sums[w * a.experts + e];
+    if (alone) sums[e] = v;
+    else {
+      a.p[(int64_t)blockIdx.x * a.experts + e] = v;
+      a.seen[(int64_t)blockIdx.x * a.experts + e] = seen[e];
+    }
+  }
+  if (alone) finish<kThreads>(a, b, sums, seen, z, n);  // each thread reads the entries it wrote
+  else if (tid == 0) {
+    a.z[blockIdx.x] = z;
+    a.n[blockIdx.x] = n;
+  }
+}
+
+// A sample's chunks in order: groups of threads stride over them, then the groups.
+__global__ __launch_bounds__(kJoinThreads) void balance_join(BalArgs a) {
+  __shared__ float p[kMaxExperts], parts[kJoinThreads];
+  __shared__ int32_t seen[kMaxExperts], seen_parts[kJoinThreads];
+  const int tid = threadIdx.x;
+  const int64_t b = blockIdx.x, first = b * a.chunks;
+  int width = 1;
+  while (width < a.experts && width < kJoinThreads) width *= 2;
+  const int groups = kJoinThreads / width, x = tid % width;
+  for (int e0 = 0; e0 < a.experts; e0 += width) {
+    float v = 0.f;
+    int32_t k = 0;
+    if (e0 + x < a.experts)
+#pragma unroll 4
+      for (int64_t c = tid / width; c < a.chunks; c += groups) {
+        v += a.p[(first + c) * a.experts + e0 + x];
+        k += a.seen[(first + c) * a.experts + e0 + x];
+      }
+    __syncthreads();
+    parts[tid] = v;
+    seen_parts[tid] = k;
+    __syncthreads();
+    if (tid < width && e0 + tid < a.experts) {
+      for (int g = 1; g < groups; ++g) v += parts[g * width + tid], k += seen_parts[g * width + tid];
+      p[e0 + tid] = v;
+      seen[e0 + tid] = k;
+    }
+  }
+  float z = 0.f;
+  int n = 0;
+  for (int64_t c = tid; c < a.chunks; c += kJoinThreads) z += a.z[first + c], n += a.n[first + c];
+  __syncthreads();
+  parts[tid] = z;
+  seen_parts[tid] = n;
+  for (int off = kJoinThreads / 2; off > 0; off >>= 1) {
+    __syncthreads();
+    if (tid < off) parts[tid] += parts[tid + off], seen_parts[tid] += seen_parts[tid + off];
+  }
+  __syncthreads();
+  finish<kJoinThreads>(a, b, p, seen, parts[0], seen_parts[0]);
+}
+
+template <int DT, int V, int kL, int S>
+__global__ __launch_bounds__(kThreads) void balance_backward(BalArgs a) {
+  constexpr int ES = Elem<DT>::kBytes, kTokens = kWave / kL, kStep = kWaves * kTokens;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l = lane % kL, sub = lane / kL;
+  const int64_t b = blockIdx.x / a.chunks, chunk = blockIdx.x - b * a.chunks;
+  const int64_t t0 = chunk * a.chunk, t1 = min(t0 + a.chunk, a.tokens);
+  const uint8_t* mask = a.mask ? a.mask + b * a.mask_b : nullptr;
+  int64_t t = t0 + wave * kTokens + sub;
+  const char* row = a.logits + (b * a.tokens + t) * a.row * ES;
+  char* out = a.grad + (b * a.tokens + t) * a.grad_row * ES;
+  const int n = a.live[b];
+  Token<DT, V, kL, S> x;
+  bool live = t < t1 && n > 0 && (!mask || mask[t * a.mask_t]);
+  x.load(row, a.experts, l, live);
+  const float inv = n ? 1.f / (float)n : 0.f;
+  const float up = (a.up ? a.up[b] : 0.f) * (float)a.experts * inv, up_z = (a.up_z ? a.up_z[b] : 0.f) * 2.f * inv;
+  float f[S][V];
+#pragma unroll
+  for (int i = 0; i < S; ++i)
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      const int at = (l + i * kL) * V + e;
+      f[i][e] = at < a.experts ? (float)a.counts[b * a.experts + at] * inv : 0.f;
+    }
+  for (int64_t first = t0; first < t1; first += kStep) {
+    const Token<DT, V, kL, S> now = x;
+    const bool there = t < t1, lives = live;
+    char* to = out;
+    t += kStep;
+    row += kStep * a.row * ES;
+    out += kStep * a.grad_row * ES;
+    live = t < t1 && n > 0 && (!mask || mask[t * a.mask_t]);
+    x.load(row, a.experts, l, live);
+    float q[S][V], dot = 0.f;
+    const float lse = now.softmax(a.experts, l, q);
+#pragma unroll
+    for (int i = 0; i < S; ++i)
+#pragma unroll
+      for (int e = 0; e < V; ++e) dot += f[i][e] * q[i][e];
+    dot = over_lanes<kL>(dot, Sum());
+    const float with_z = up_z * lse;
+#pragma unroll
+    for (int i = 0; i < S; ++i) {
+      const int e0 = (l + i * kL) * V;
+      float g[V];
+#pragma unroll
+      for (int e = 0; e < V; ++e) g[e] = lives ? q[i][e] * (up * (f[i][e] - dot) + with_z) : 0.f;
+      if (!there || e0 >= a.experts) continue;
+      if constexpr (V == 1) Elem<DT>::store(to, e0, g[0]);
+      else {
+        u32x4 w;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          if constexpr (DT == DA_F32) w[k] = __float_as_uint(g[k]);
+          else w[k] = pack2<DT>(g[2 * k], g[2 * k + 1]);
+        }
+        st16(to + e0 * ES, w);
+      }
+    }
+  }
 }
 
 int check_args(const char* what, int dtype, int64_t batch, int64_t tokens, int experts) {
@@ -179,35 +359,94 @@ int check_args(const char* what, int dtype, int64_t batch, int64_t tokens, int e
   return DA_OK;
 }
 
-void chunking(BalArgs& a) {
-  a.chunk = 64;
-  a.chunks = (a.tokens + a.chunk - 1) / a.chunk;
+// Experts of a run, lanes of a token, runs of a lane.
+struct Shape {
+  int v, lanes, runs;
+};
+Shape shape_of(int dtype, int experts, bool aligned) {
+  Shape s;
+  s.v = dtype == DA_F32 ? 4 : 8;
+  if (!aligned || experts % s.v) s.v = 1;
+  const int slots = (experts + s.v - 1) / s.v;
+  s.lanes = 1;
+  while (s.lanes < slots && s.lanes < 64) s.lanes *= 2;
+  s.runs = (slots + s.lanes - 1) / s.lanes;
+  return s;
 }
+
+constexpr int64_t kWantBlocks = 1024;
+
+// Tokens of a workgroup: at least `least` of its steps, and a sample of up to twice
+// that stays whole (the forward pass then needs no second launch).
+void chunking(BalArgs& a, const Shape& s, int64_t least) {
+  const int64_t step = kWaves * kWave / s.lanes;
+  const int64_t steps = std::max<int64_t>(least, a.batch * a.tokens / (step * kWantBlocks));
+  a.chunk = step * steps;
+  if (a.tokens <= 2 * a.chunk) a.chunk = std::max<int64_t>(a.tokens, 1);
+  a.chunks = std::max<int64_t>((a.tokens + a.chunk - 1) / a.chunk, 1);
+}
+
+size_t partial_bytes(const BalArgs& a) {
+  return a.chunks > 1 ? (size_t)(a.batch * a.chunks * (a.experts + 1)) * 8 : 0;
+}
+
+// Launches the forward or the backward kernel for a type and a shape.
+struct Launch {
+  const BalArgs& a;
+  bool grad;
+  hipStream_t stream;
+
+  template <int DT, int V, int kL, int S>
+  void kernel() const {
+    const unsigned blocks = (unsigned)(a.batch * a.chunks);
+    if (grad) balance_backward<DT, V, kL, S><<<blocks, kThreads, 0, stream>>>(a);
+    else balance_forward<DT, V, kL, S><<<blocks, kThreads, (size_t)a.experts * (kWaves + 1) * 4, stream>>>(a);
+  }
+  template <int DT, int V>
+  void lanes(const Shape& s) const {
+    if (s.lanes == 1) kernel<DT, V, 1, 1>();
+    else if (s.lanes == 2) kernel<DT, V, 2, 1>();
+    else if (s.lanes == 4) kernel<DT, V, 4, 1>();
+    else if (s.lanes == 8) kernel<DT, V, 8, 1>();
+    else if (s.lanes == 16) kernel<DT, V, 16, 1>();
+    else if (s.lanes == 32) kernel<DT, V, 32, 1>();
+    else if (s.runs == 1) kernel<DT, V, 64, 1>();
+    else if (s.runs == 2) kernel<DT, V, 64, 2>();
+    else if (V < 8 && s.runs <= 4) kernel<DT, V, V < 8 ? 64 : 1, V < 8 ? 4 : 1>();
+    else if (V == 1) kernel<DT, V, V == 1 ? 64 : 1, V == 1 ? 16 : 1>();
+  }
+  template <int DT>
+  void runs(const Shape& s) const {
+    if (s.v == 1) lanes<DT, 1>(s);
+    else lanes<DT, 16 / Elem<DT>::kBytes>(s);
+  }
+  void operator()(int dtype, const Shape& s) const {
+    if (dtype == DA_BF16) runs<DA_BF16>(s);
+    else if (dtype == DA_F16) runs<DA_F16>(s);
+    else runs<DA_F32>(s);
+  }
+};
+
+constexpr int64_t kForwardSteps = 4, kBackwardSteps = 1;
 
 }  // namespace
 }  // namespace da
 
 using namespace da;
 
-#define DA_BAL_SLOTS(CALL, DT)                       \
-  if (experts <= 64) { CALL(DT, 1) }                 \
-  else if (experts <= 128) { CALL(DT, 2) }           \
-  else if (experts <= 256) { CALL(DT, 4) }           \
-  else { CALL(DT, 16) }
-#define DA_BAL_DISPATCH(CALL)                              \
-  if (dtype == DA_BF16) { DA_BAL_SLOTS(CALL, DA_BF16) }    \
-  else if (dtype == DA_F16) { DA_BAL_SLOTS(CALL, DA_F16) } \
-  else { DA_BAL_SLOTS(CALL, DA_F32) }
-
 extern "C" {
 
-int da_balance_loss_workspace(int64_t batch, int64_t tokens, int experts, size_t* bytes) {
-  if (!bytes) return set_error(DA_ERR_INVALID, "da_balance_loss_workspace: NULL bytes");
-  if (int rc = check_args("da_balance_loss_workspace", DA_F32, batch, tokens, experts)) return rc;
-  BalArgs a{};
-  a.batch = batch, a.tokens = tokens;
-  chunking(a);
-  *bytes = (size_t)(batch * a.chunks * (experts + 1)) * 8;
+int da_balance_loss_workspace(int dtype, int64_t batch, int64_t tokens, int experts, size_t* bytes) {
+  const char* what = "da_balance_loss_workspace";
+  if (!bytes) return set_error(DA_ERR_INVALID, "%s: NULL bytes", what);
+  if (int rc = check_args(what, dtype, batch, tokens, experts)) return rc;
+  *bytes = 0;
+  for (int aligned = 0; aligned < 2; ++aligned) {
+    BalArgs a{};
+    a.batch = batch, a.tokens = tokens, a.experts = experts;
+    chunking(a, shape_of(dtype, experts, aligned), kForwardSteps);
+    *bytes = std::max(*bytes, partial_bytes(a));
+  }
   return DA_OK;
 }
 
@@ -221,27 +460,28 @@ int da_balance_loss(const void* logits, int dtype, int64_t batch, int64_t tokens
   if (!batch) return DA_OK;
   if (!loss || !z_loss || !counts || !live || (tokens && (!logits || (top && !index))))
     return set_error(DA_ERR_INVALID, "%s: NULL pointer", what);
+  const int es = (int)elem_bytes(dtype);
   BalArgs a{};
   a.logits = (const char*)logits, a.index = index, a.mask = mask, a.tokens = tokens, a.batch = batch;
   a.row = row_stride, a.mask_b = mask_bstride, a.mask_t = mask_tstride, a.experts = experts, a.top = top;
-  a.loss = loss, a.z = z_loss, a.counts = counts, a.live = live;
-  chunking(a);
-  const int64_t entries = batch * a.chunks * (experts + 1);
-  if (entries && (!workspace || workspace_bytes < (size_t)entries * 8))
-    return set_error(DA_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", what, workspace_bytes, (size_t)entries * 8);
-  if (batch * a.chunks > 0x7fffffff || batch > 0x7fffffff) return set_error(DA_ERR_UNSUPPORTED, "%s: too many tokens", what);
-  a.partial = (float*)workspace;
-  a.part_live = (int32_t*)(a.partial + entries);
+  a.loss = loss, a.z_loss = z_loss, a.counts = counts, a.live = live;
+  const Shape shape = shape_of(dtype, experts, (uintptr_t)logits % 16 == 0 && row_stride * es % 16 == 0);
+  chunking(a, shape, kForwardSteps);
+  const size_t need = partial_bytes(a);
+  if (need && (!workspace || workspace_bytes < need))
+    return set_error(DA_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", what, workspace_bytes, need);
+  if (batch * a.chunks > 0x7fffffff || a.chunk * top > 0x7fffffff)
+    return set_error(DA_ERR_UNSUPPORTED, "%s: too many tokens", what);
+  const int64_t parts = batch * a.chunks;
+  a.p = (float*)workspace;
+  a.seen = (int32_t*)(a.p + parts * experts);
+  a.z = (float*)(a.seen + parts * experts);
+  a.n = (int32_t*)(a.z + parts);
   hipStream_t st = (hipStream_t)stream;
-  if (entries) {
-    const unsigned blocks = (unsigned)(batch * a.chunks);
-    const size_t lds = (size_t)(experts + 1) * (kWaves + 1) * 4;
-#define DA_BAL_FWD(DT, S) balance_partials<DT, S><<<blocks, kThreads, lds, st>>>(a);
-    DA_BAL_DISPATCH(DA_BAL_FWD)
-#undef DA_BAL_FWD
-    if (int rc = check_launch(what)) return rc;
-  }
-  balance_join<<<(unsigned)batch, kThreads, 0, st>>>(a);
+  Launch{a, false, st}(dtype, shape);
+  if (int rc = check_launch(what)) return rc;
+  if (a.chunks == 1) return DA_OK;
+  balance_join<<<(unsigned)batch, kJoinThreads, 0, st>>>(a);
   return check_launch(what);
 }
 
@@ -253,16 +493,16 @@ int da_balance_loss_grad(const float* up, const float* up_z, const void* logits,
   if (int rc = check_args(what, dtype, batch, tokens, experts)) return rc;
   if (!batch || !tokens) return DA_OK;
   if (!logits || !counts || !live || !grad) return set_error(DA_ERR_INVALID, "%s: NULL pointer", what);
+  const int es = (int)elem_bytes(dtype);
   BalArgs a{};
   a.up = up, a.up_z = up_z, a.logits = (const char*)logits, a.mask = mask, a.tokens = tokens, a.batch = batch;
   a.row = row_stride, a.mask_b = mask_bstride, a.mask_t = mask_tstride, a.experts = experts;
   a.counts = (int32_t*)counts, a.live = (int32_t*)live, a.grad = (char*)grad, a.grad_row = grad_row_stride;
-  const int64_t blocks = (batch * tokens + kWaves - 1) / kWaves;
-  if (blocks > 0x7fffffff) return set_error(DA_ERR_UNSUPPORTED, "%s: too many tokens", what);
-  hipStream_t st = (hipStream_t)stream;
-#define DA_BAL_BWD(DT, S) balance_backward<DT, S><<<(unsigned)blocks, kThreads, 0, st>>>(a);
-  DA_BAL_DISPATCH(DA_BAL_BWD)
-#undef DA_BAL_BWD
+  const bool aligned = ((uintptr_t)logits | (uintptr_t)grad) % 16 == 0 && (row_stride | grad_row_stride) * es % 16 == 0;
+  const Shape shape = shape_of(dtype, experts, aligned);
+  chunking(a, shape, kBackwardSteps);
+  if (batch * a.chunks > 0x7fffffff) return set_error(DA_ERR_UNSUPPORTED, "%s: too many tokens", what);
+  Launch{a, true, (hipStream_t)stream}(dtype, shape);
   return check_launch(what);
 }
 

@@ -105,19 +105,6 @@ struct Slot {
   }
 };
 
-// Two fp32 values rounded to 16 bits each (to nearest even), packed.
-template <int DT>
-__device__ __forceinline__ uint32_t pack2(float a, float b) {
-  typedef float f32x2 __attribute__((ext_vector_type(2)));
-  if constexpr (DT == DA_BF16) {
-    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, bf16x2));
-  } else {
-    typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, f16x2));
-  }
-}
-
 template <int DT, int V>
 struct Run {  // V entries as they lie in memory, in one access
   static constexpr int kBytes = V * Elem<DT>::kBytes, kWords = kBytes < 4 ? 1 : kBytes / 4;

@@ -225,7 +225,7 @@ SIGNATURES.update(
         "da_relative_bias_grad": (
             _I32, [_P, _I32, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _EDGES, _I32, _I32, _I32, _P, _I64, _I64,
                    _P, _P, _SZ, _P]),
-        "da_balance_loss_workspace": (_I32, [_I64, _I64, _I32, ctypes.POINTER(_SZ)]),
+        "da_balance_loss_workspace": (_I32, [_I32, _I64, _I64, _I32, ctypes.POINTER(_SZ)]),
         "da_balance_loss": (
             _I32, [_P, _I32, _I64, _I64, _I32, _I64, _P, _I32, _P, _I64, _I64, _P, _P, _P, _P, _P, _SZ, _P]),
         "da_balance_loss_grad": (

@@ -1701,7 +1701,7 @@ def balance_loss(logits: torch.Tensor, index: torch.Tensor, *, batch: int = 1, m
     live = torch.empty(batch, dtype=torch.int32, device=dev)
     lib = nat.load()
     nbytes = ctypes.c_size_t(0)
-    nat.check(lib.da_balance_loss_workspace(batch, n // batch, e, ctypes.byref(nbytes)), "balance_loss")
+    nat.check(lib.da_balance_loss_workspace(code, batch, n // batch, e, ctypes.byref(nbytes)), "balance_loss")
     ws = nat.workspace(nbytes.value, dev)
     _run_on(dev, "balance_loss", lib.da_balance_loss,
             logits.data_ptr(), code, batch, n // batch, e, logits.stride(0), index.data_ptr(),

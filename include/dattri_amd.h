@@ -822,7 +822,7 @@ int da_relative_bias_grad(const void* g, int dtype, int64_t batch, int64_t heads
  * counts carry no gradient.  experts <= 1024.  Counts and sums do not depend on
  * the order in which workgroups run.
  */
-int da_balance_loss_workspace(int64_t batch, int64_t tokens, int experts, size_t* bytes);
+int da_balance_loss_workspace(int dtype, int64_t batch, int64_t tokens, int experts, size_t* bytes);
 int da_balance_loss(const void* logits, int dtype, int64_t batch, int64_t tokens, int experts, int64_t row_stride,
                     const int64_t* index, int top, const uint8_t* mask, int64_t mask_bstride, int64_t mask_tstride,
                     float* loss, float* z_loss, int32_t* counts, int32_t* live, void* workspace,
