@@ -210,7 +210,8 @@ class QkSide(ctypes.Structure):
     ]
 
 
-_QK = [ctypes.POINTER(QkSide), _I32, _I32, _I64, _I64, _I64, _I64, _P, _P, _I32, _I64, _I64, _P, _I64, _I64, _I32,
+# The records of one call are passed as an array of 64-bit words (QkSide's fields in order).
+_QK = [_P, _I32, _I32, _I64, _I64, _I64, _I64, _P, _P, _I32, _I64, _I64, _P, _I64, _I64, _I32,
        ctypes.c_float, ctypes.c_float]
 _EDGES = ctypes.POINTER(ctypes.c_int32)
 SIGNATURES.update(
@@ -301,8 +302,25 @@ def require_device(*tensors: torch.Tensor) -> torch.device:
     return dev
 
 
+# The handle of a device's current stream and the current device's index, without
+# the objects that the public calls build around them (1 us each) where torch has them.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
 def stream_ptr(device: torch.device) -> int:
+    if _raw_stream is not None and device.index is not None:
+        return _raw_stream(device.index)
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def same_device(first: torch.Tensor, *others) -> torch.device:
+    """:func:`require_device` of tensors or None, quick where all is well."""
+    index = first.get_device()
+    for t in others:
+        if t is not None and t.get_device() != index:
+            return require_device(first, *others)
+    return first.device if index >= 0 else require_device(first)
 
 
 def dtype_code(dtype: torch.dtype) -> int:

@@ -81,7 +81,10 @@ def balance_loss(logits: torch.Tensor, top_idx: torch.Tensor, *, batch: int | No
         if batch not in (None, logits.shape[0]):
             raise ValueError(f"balance_loss: batch {batch} for logits of {logits.shape[0]} samples")
         batch = logits.shape[0]
-    logits, top_idx = logits.flatten(0, -2), top_idx.flatten(0, -2)
+    if logits.dim() == 3:
+        logits = logits.flatten(0, 1)
+    if top_idx.dim() == 3:
+        top_idx = top_idx.flatten(0, 1)
     batch = 1 if batch is None else batch
     if torch.is_grad_enabled() and logits.requires_grad:
         return BalanceLoss(*_BalanceLoss.apply(logits, top_idx, batch, mask))
@@ -95,8 +98,9 @@ def balance_loss_grad(up: torch.Tensor | None, up_z: torch.Tensor | None, logits
     ``up_z`` (B,; None: zero); ``counts`` and ``live`` are its results."""
     if logits.dim() not in (2, 3):
         raise ValueError("balance_loss_grad expects (B, T, E) or (N, E) logits")
-    grad = kernels.balance_loss_grad(up, up_z, logits.flatten(0, -2), counts, live, mask=mask)
-    return grad.view(logits.shape)
+    if logits.dim() == 2:
+        return kernels.balance_loss_grad(up, up_z, logits, counts, live, mask=mask)
+    return kernels.balance_loss_grad(up, up_z, logits.flatten(0, 1), counts, live, mask=mask).view(logits.shape)
 
 
 def expert_segments(top_idx: torch.Tensor, n_experts: int) -> tuple[torch.Tensor, torch.Tensor]:

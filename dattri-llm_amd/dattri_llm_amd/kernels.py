@@ -1476,7 +1476,7 @@ def ghost_gram_segmented(a1, g1, seg1, idx1, tokens1, a2, g2, seg2, idx2, tokens
 
 def _run_on(dev: torch.device, what: str, fn, *args) -> None:
     """:func:`_run` with ``dev`` made the current device where it is not."""
-    if dev.index is None or dev.index == torch.cuda.current_device():
+    if dev.index == nat.current_device():
         _run(dev, what, fn, *args)
         return
     with torch.cuda.device(dev):
@@ -1485,97 +1485,94 @@ def _run_on(dev: torch.device, what: str, fn, *args) -> None:
 
 def _token_mask(what: str, mask: torch.Tensor | None, batch: int, tokens: int):
     """``(tensor, pointer, batch stride, token stride)`` of a (batch, tokens)
-    byte mask; other integer masks are compared with zero first."""
+    byte mask; other types are compared with zero first."""
     if mask is None:
         return None, None, 0, 0
-    if tuple(mask.shape) != (batch, tokens):
+    if mask.shape != (batch, tokens):
         raise ValueError(f"{what}: mask must have shape ({batch}, {tokens}), got {tuple(mask.shape)}")
     if mask.dtype not in (torch.bool, torch.uint8):
         mask = mask != 0
-    return mask, mask.data_ptr(), mask.stride(0), mask.stride(1)
+    return mask, mask.data_ptr(), *mask.stride()
 
 
 def _unit_rows(x: torch.Tensor) -> torch.Tensor:
     return x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
 
 
-def _qk_sides(xs, ws, gzs, grads: bool):
-    """The two ``da_qk_side`` records; returns them with the outputs and every
-    tensor the launch reads."""
-    sides = (nat.QkSide * 2)()
-    outs, wgrads, keep = [], [], []
-    b, t, d = xs[0].shape[0], xs[0].shape[1], xs[0].shape[3]
-    for side, x, w, gz in zip(sides, xs, ws, gzs):
-        if x is None:
-            side.heads = 0
-            outs.append(None)
-            wgrads.append(None)
-            continue
-        x, w = _unit_rows(x), w.contiguous()
-        out = torch.empty_like(x)
-        side.x, side.out, side.weight, side.heads = x.data_ptr(), out.data_ptr(), w.data_ptr(), x.shape[2]
-        side.x_bstride, side.x_tstride, side.x_hstride = x.stride()[:3]
-        side.out_bstride, side.out_tstride, side.out_hstride = out.stride()[:3]
-        wgrad = None
-        if gz is not None:
-            gz = _unit_rows(gz)
-            side.gz = gz.data_ptr()
-            side.gz_bstride, side.gz_tstride, side.gz_hstride = gz.stride()[:3]
-            if grads:
-                wgrad = torch.empty(b, d, dtype=torch.float32, device=x.device)
-                side.weight_grad = wgrad.data_ptr()
-        outs.append(out)
-        wgrads.append(wgrad)
-        keep += (x, w, gz)
-    return sides, outs, wgrads, keep, b, t, d
+_NO_SIDE = (0,) * 15  # a da_qk_side without heads
+
+
+def _qk_side(what: str, x, w, gz, wgrad):
+    """One ``da_qk_side`` as words, with the output and the tensors it points to."""
+    if w is None or w.shape != x.shape[3:]:
+        raise ValueError(f"{what}: a norm weight must have shape ({x.shape[3]},)")
+    x, w = _unit_rows(x), w.contiguous()
+    out = torch.empty_like(x)
+    xb, xt, xh, _ = x.stride()
+    ob, ot, oh, _ = out.stride()
+    if gz is None:
+        return (x.data_ptr(), 0, out.data_ptr(), w.data_ptr(), 0, x.shape[2], xb, xt, xh, 0, 0, 0, ob, ot, oh), out, x, w
+    gz = _unit_rows(gz)
+    gb, gt, gh, _ = gz.stride()
+    return ((x.data_ptr(), gz.data_ptr(), out.data_ptr(), w.data_ptr(), 0 if wgrad is None else wgrad.data_ptr(),
+             x.shape[2], xb, xt, xh, gb, gt, gh, ob, ot, oh), out, x, w, gz)
 
 
 def _qk_rope(what, q, k, q_weight, k_weight, inv_freq, positions, mask, gq, gk, interleaved, scaling, eps, grads=True):
     if q.dim() != 4 or (k is not None and k.dim() != 4):
         raise ValueError(f"{what} expects (B, T, heads, D) queries and keys")
-    if k is not None and (k.shape[:2] != q.shape[:2] or k.shape[3] != q.shape[3]):
+    b, t, hq, d = q.shape
+    dt = q.dtype
+    if k is not None and k.shape != (b, t, k.shape[2], d):
         raise ValueError(f"{what}: queries {tuple(q.shape)} and keys {tuple(k.shape)} disagree on B, T or D")
-    b, t, _, d = q.shape
-    for x, w, gz in ((q, q_weight, gq), (k, k_weight, gk)):
-        if x is None:
-            continue
-        if w is None or tuple(w.shape) != (d,):
-            raise ValueError(f"{what}: a norm weight must have shape ({d},)")
-        if x.dtype != q.dtype or (gz is not None and gz.dtype != q.dtype) or w.dtype != q_weight.dtype:
-            raise ValueError(f"{what}: queries, keys and their gradients must share one dtype, and so the weights")
-        if gz is not None and gz.shape != x.shape:
-            raise ValueError(f"{what}: a gradient of shape {tuple(gz.shape)} for rows of {tuple(x.shape)}")
+    if q_weight is None or (k is not None and k_weight is None):
+        raise ValueError(f"{what}: a norm weight must have shape ({d},)")
+    if k is not None and (k.dtype != dt or k_weight.dtype != q_weight.dtype) or gq is not None and (
+            gq.dtype != dt or (gk is not None and gk.dtype != dt)):
+        raise ValueError(f"{what}: queries, keys and their gradients must share one dtype, and so the weights")
+    if gq is not None:
+        for x, g in ((q, gq), (k, gk)):
+            if x is not None and g.shape != x.shape:
+                raise ValueError(f"{what}: a gradient of shape {tuple(g.shape)} for rows of {tuple(x.shape)}")
     if inv_freq.dim() != 1 or inv_freq.dtype != torch.float32:
         raise ValueError(f"{what}: inv_freq must be a 1-D float32 tensor")
     rot = 2 * inv_freq.shape[0]
     if rot > d:
         raise ValueError(f"{what}: {inv_freq.shape[0]} frequencies rotate {rot} entries, the heads have {d}")
-    codes = nat.dtype_code(q.dtype), nat.dtype_code(q_weight.dtype)
-    inv_freq = inv_freq.contiguous()
     pos_ptr, pos_bytes, pos_b, pos_t = None, 0, 0, 0
     if positions is not None:
         if positions.dtype not in (torch.int32, torch.int64):
             raise ValueError(f"{what}: positions must be int32 or int64")
-        if tuple(positions.shape) not in ((t,), (1, t), (b, t)):
-            raise ValueError(f"{what}: positions must have shape ({t},) or ({b}, {t}), got {tuple(positions.shape)}")
+        shape = positions.shape
+        if shape != (b, t) and shape != (t,) and shape != (1, t):
+            raise ValueError(f"{what}: positions must have shape ({t},) or ({b}, {t}), got {tuple(shape)}")
         pos_ptr, pos_bytes, pos_t = positions.data_ptr(), positions.element_size(), positions.stride(-1)
-        pos_b = positions.stride(0) if positions.dim() == 2 and positions.shape[0] == b else 0
+        pos_b = positions.stride(0) if shape == (b, t) else 0
     mask, mask_ptr, mask_b, mask_t = _token_mask(what, mask, b, t)
-    dev = nat.require_device(q, k, q_weight, k_weight, inv_freq, positions, mask, gq, gk)
-    sides, outs, wgrads, keep, b, t, d = _qk_sides( (q, k), (q_weight, k_weight), (gq, gk), grads)
-    args = (sides, *codes, b, t, d, rot, inv_freq.data_ptr(), pos_ptr,
-            pos_bytes, pos_b, pos_t, mask_ptr, mask_b, mask_t, int(bool(interleaved)), float(scaling), float(eps))
+    code, w_code = nat.dtype_code(dt), nat.dtype_code(q_weight.dtype)
+    wq = wk = None
+    if grads and gq is not None and gq.is_cuda:
+        wq = torch.empty((b, d), dtype=torch.float32, device=q.device)
+        wk = None if k is None else torch.empty((b, d), dtype=torch.float32, device=q.device)
+    words_q, q_out, *keep = _qk_side(what, q, q_weight, gq, wq)
+    words_k, k_out, *keep_k = (_NO_SIDE, None) if k is None else _qk_side(what, k, k_weight, gk, wk)
+    dev = nat.same_device(q, k, q_weight, k_weight if k is not None else None, inv_freq, positions, mask, gq, gk)
+    inv_freq = inv_freq.contiguous()
+    sides = array.array("q", words_q + words_k)
+    args = (sides.buffer_info()[0], code, w_code, b, t, d, rot, inv_freq.data_ptr(), pos_ptr, pos_bytes, pos_b, pos_t,
+            mask_ptr, mask_b, mask_t, int(interleaved), scaling, eps)
     lib = nat.load()
     if gq is None:
         _run_on(dev, what, lib.da_qk_norm_rope, *args, nat.stream_ptr(dev))
-        return outs
-    nbytes = ctypes.c_size_t(0)
-    nat.check(lib.da_qk_norm_rope_grad_workspace(b, t, sides[0].heads, sides[1].heads, d, ctypes.byref(nbytes)),
-              what)
-    ws = nat.workspace(nbytes.value if grads else 0, dev)
-    _run_on(dev, what, lib.da_qk_norm_rope_grad, *args, ws.data_ptr(), ws.numel(), nat.stream_ptr(dev))
-    del keep
-    return (*outs, *wgrads)
+        return q_out, k_out
+    ws_ptr, nbytes = None, ctypes.c_size_t(0)
+    if grads:
+        nat.check(lib.da_qk_norm_rope_grad_workspace(b, t, hq, words_k[5], d, ctypes.byref(nbytes)), what)
+        ws = nat.workspace(nbytes.value, dev)
+        ws_ptr = ws.data_ptr()
+    _run_on(dev, what, lib.da_qk_norm_rope_grad, *args, ws_ptr, nbytes.value, nat.stream_ptr(dev))
+    del keep, keep_k
+    return q_out, k_out, wq, wk
 
 
 def qk_norm_rope(q, k, q_weight, k_weight, inv_freq, positions=None, *, eps: float, interleaved: bool = False,
@@ -1588,8 +1585,8 @@ def qk_norm_rope(q, k, q_weight, k_weight, inv_freq, positions=None, *, eps: flo
     ``inv_freq`` float32 ``(R/2,)``, ``positions`` int32/int64 ``(T,)`` or
     ``(B, T)`` (default: the token's index), ``mask`` (B, T), zero for tokens
     whose output is zero."""
-    return tuple(_qk_rope("qk_norm_rope", q, k, q_weight, k_weight, inv_freq, positions, mask, None, None, interleaved,
-                          scaling, eps))
+    return _qk_rope("qk_norm_rope", q, k, q_weight, k_weight, inv_freq, positions, mask, None, None, interleaved,
+                    scaling, eps)
 
 
 def qk_norm_rope_grad(gq, gk, q, k, q_weight, k_weight, inv_freq, positions=None, *, eps: float,
@@ -1640,12 +1637,12 @@ def relative_bias(table: torch.Tensor, q_len: int, k_len: int, *, q_start: int =
         raise ValueError("relative_bias: negative length")
     edges = _bucket_edges(int(table.shape[0]), int(max_distance), bool(bidirectional))
     code = nat.dtype_code(table.dtype)
-    dev = nat.require_device(table)
-    out = torch.empty(table.shape[1], q_len, k_len, dtype=table.dtype, device=dev)
+    dev = nat.same_device(table)
+    heads = table.shape[1]
+    out = torch.empty((heads, q_len, k_len), dtype=table.dtype, device=dev)
     _run_on(dev, "relative_bias", nat.load().da_relative_bias,
-            table.data_ptr(), code, table.stride(0), table.stride(1), table.shape[1], q_len,
-            k_len, int(q_start), edges, len(edges), int(bool(bidirectional)), int(bool(causal)), out.data_ptr(),
-            nat.stream_ptr(dev))
+            table.data_ptr(), code, *table.stride(), heads, q_len, k_len, int(q_start), edges, len(edges),
+            int(bidirectional), int(causal), out.data_ptr(), nat.stream_ptr(dev))
     return out
 
 
@@ -1665,18 +1662,18 @@ def relative_bias_grad(g: torch.Tensor, num_buckets: int, *, q_start: int = 0, b
     if mask is not None and not 0 <= q_start <= tk - tq:
         raise ValueError(f"relative_bias_grad: a mask over {tk} positions has to hold the queries', {q_start} to "
                          f"{q_start + tq - 1}")
-    dev = nat.require_device(g, mask)
+    dev = nat.same_device(g, mask)
     g = _unit_rows(g)
-    out = torch.empty(b, num_buckets, h, dtype=torch.float32, device=dev)
+    out = torch.empty((b, num_buckets, h), dtype=torch.float32, device=dev)
     lib = nat.load()
     nbytes = ctypes.c_size_t(0)
-    nat.check(lib.da_relative_bias_grad_workspace(code, b, h, tq, tk, int(q_start), num_buckets, int(bool(causal)),
+    nat.check(lib.da_relative_bias_grad_workspace(code, b, h, tq, tk, int(q_start), num_buckets, int(causal),
                                                   ctypes.byref(nbytes)), "relative_bias_grad")
     ws = nat.workspace(nbytes.value, dev)
     sb, sh, si, _ = g.stride()
     _run_on(dev, "relative_bias_grad", lib.da_relative_bias_grad,
             g.data_ptr(), code, b, h, tq, tk, sb, sh, si, int(q_start), edges, len(edges),
-            int(bool(bidirectional)), int(bool(causal)), mask_ptr, mask_b, mask_k, out.data_ptr(), ws.data_ptr(),
+            int(bidirectional), int(causal), mask_ptr, mask_b, mask_k, out.data_ptr(), ws.data_ptr(),
             ws.numel(), nat.stream_ptr(dev))
     return out
 
@@ -1694,28 +1691,31 @@ def balance_loss(logits: torch.Tensor, index: torch.Tensor, *, batch: int = 1, m
         raise ValueError(f"balance_loss: {n} tokens are not {batch} samples of one length")
     code = nat.dtype_code(logits.dtype)
     mask, mask_ptr, mask_b, mask_t = _token_mask("balance_loss", mask, batch, n // batch)
-    dev = nat.require_device(logits, index, mask)
+    dev = nat.same_device(logits, index, mask)
     logits, index = _unit_rows(logits), index.contiguous()
-    loss = torch.empty(2, batch, dtype=torch.float32, device=dev)
-    counts = torch.empty(batch, e, dtype=torch.int32, device=dev)
-    live = torch.empty(batch, dtype=torch.int32, device=dev)
+    loss = torch.empty((batch,), dtype=torch.float32, device=dev)
+    z_loss = torch.empty((batch,), dtype=torch.float32, device=dev)
+    counts = torch.empty((batch, e), dtype=torch.int32, device=dev)
+    live = torch.empty((batch,), dtype=torch.int32, device=dev)
     lib = nat.load()
-    nbytes = ctypes.c_size_t(0)
+    ws_ptr, nbytes = None, ctypes.c_size_t(0)
     nat.check(lib.da_balance_loss_workspace(code, batch, n // batch, e, ctypes.byref(nbytes)), "balance_loss")
-    ws = nat.workspace(nbytes.value, dev)
+    if nbytes.value:
+        ws = nat.workspace(nbytes.value, dev)
+        ws_ptr = ws.data_ptr()
     _run_on(dev, "balance_loss", lib.da_balance_loss,
             logits.data_ptr(), code, batch, n // batch, e, logits.stride(0), index.data_ptr(),
-            index.shape[1], mask_ptr, mask_b, mask_t, loss.data_ptr(), loss.data_ptr() + 4 * batch, counts.data_ptr(),
-            live.data_ptr(), ws.data_ptr(), ws.numel(), nat.stream_ptr(dev))
-    return loss[0], loss[1], counts, live
+            index.shape[1], mask_ptr, mask_b, mask_t, loss.data_ptr(), z_loss.data_ptr(), counts.data_ptr(),
+            live.data_ptr(), ws_ptr, nbytes.value, nat.stream_ptr(dev))
+    return loss, z_loss, counts, live
 
 
 def _per_sample(what: str, v: torch.Tensor | None, batch: int):
     if v is None:
         return None
-    if tuple(v.shape) != (batch,):
+    if v.shape != (batch,):
         raise ValueError(f"{what}: a loss gradient must have shape ({batch},), got {tuple(v.shape)}")
-    return v.to(torch.float32).contiguous()
+    return v if v.dtype == torch.float32 and v.is_contiguous() else v.to(torch.float32).contiguous()
 
 
 def balance_loss_grad(up, up_z, logits: torch.Tensor, counts: torch.Tensor, live: torch.Tensor, *,
@@ -1726,16 +1726,16 @@ def balance_loss_grad(up, up_z, logits: torch.Tensor, counts: torch.Tensor, live
         raise ValueError("balance_loss_grad expects (N, E) logits and (B, E) counts")
     n, e = logits.shape
     batch = counts.shape[0]
-    if batch < 1 or n % batch or tuple(live.shape) != (batch,):
+    if batch < 1 or n % batch or live.shape != (batch,):
         raise ValueError(f"balance_loss_grad: {n} tokens are not {batch} samples of one length")
     if counts.dtype != torch.int32 or live.dtype != torch.int32:
         raise ValueError("balance_loss_grad: counts and live must be int32, as balance_loss returns them")
     up, up_z = _per_sample("balance_loss_grad", up, batch), _per_sample("balance_loss_grad", up_z, batch)
     code = nat.dtype_code(logits.dtype)
     mask, mask_ptr, mask_b, mask_t = _token_mask("balance_loss_grad", mask, batch, n // batch)
-    dev = nat.require_device(logits, counts, live, mask, up, up_z)
+    dev = nat.same_device(logits, counts, live, mask, up, up_z)
     logits, counts, live = _unit_rows(logits), counts.contiguous(), live.contiguous()
-    grad = torch.empty(n, e, dtype=logits.dtype, device=dev)
+    grad = torch.empty((n, e), dtype=logits.dtype, device=dev)
     _run_on(dev, "balance_loss_grad", nat.load().da_balance_loss_grad,
             None if up is None else up.data_ptr(), None if up_z is None else up_z.data_ptr(), logits.data_ptr(),
             code, batch, n // batch, e, logits.stride(0), counts.data_ptr(), live.data_ptr(),
