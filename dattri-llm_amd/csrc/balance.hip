@@ -26,6 +26,7 @@ constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / kWave;
 constexpr int kJoinThreads = 512;
 constexpr int kMaxExperts = 1024;
+constexpr float kLog2e = 1.44269504088896341f;
 
 struct BalArgs {
   const char* logits;
@@ -41,8 +42,8 @@ struct BalArgs {
   int64_t chunk, chunks;
   float* loss;
   float* z_loss;
-  int32_t* counts;
-  int32_t* live;
+  int64_t* counts;
+  int64_t* live;
   const float* up;
   const float* up_z;
   char* grad;
@@ -98,42 +99,37 @@ struct Token {
       }
     }
   }
-  // p = softmax of the logits, 0 past the experts; returns their logsumexp.
-  __device__ float softmax(int experts, int l, float (&p)[S][V]) const {
+  // p = exp(logit - c) for a c next to the largest logit, 0 past the experts; inv =
+  // 1 / their sum; returns the logits' logsumexp.  c is the largest logit times
+  // log2(e) as fp32 rounds it: that rounding is common to all experts, the sum
+  // takes it back out, and each exponent is one fma, rounded once.
+  __device__ float softmax(int experts, int l, float (&p)[S][V], float& inv) const {
     float top = -__builtin_inff();
 #pragma unroll
     for (int i = 0; i < S; ++i) {
       const bool in = (l + i * kL) * V < experts;
-      float x[V];
-      if constexpr (V == 1) x[0] = Elem<DT>::from_bits(raw[i / 4][i % 4]);
-      else unpack16<DT>(raw[i], x);
+      if constexpr (V == 1) p[i][0] = Elem<DT>::from_bits(raw[i / 4][i % 4]);
+      else unpack16<DT>(raw[i], p[i]);
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        p[i][e] = in ? x[e] : -__builtin_inff();
-        top = fmaxf(top, p[i][e]);
-      }
+      for (int e = 0; e < V; ++e) top = fmaxf(top, in ? p[i][e] : -__builtin_inff());
     }
     top = over_lanes<kL>(top, Max());
+    const float c = top * kLog2e;
     float sum = 0.f;
 #pragma unroll
     for (int i = 0; i < S; ++i) {
       const bool in = (l + i * kL) * V < experts;
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        // The difference is exact or rounded once; its product with log2(e) is off
-        // by at most 2^-24 of itself, which a probability below e^-16 alone notices.
-        const float x = __builtin_amdgcn_exp2f((p[i][e] - top) * 1.44269504088896341f);
-        p[i][e] = in ? x : 0.f;  // all -inf: -inf - -inf is NaN, as in a softmax
+        // All -inf: inf - inf is NaN here, as in a softmax.
+        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(p[i][e], kLog2e, -c));
+        p[i][e] = in ? x : 0.f;
         sum += p[i][e];
       }
     }
     sum = over_lanes<kL>(sum, Sum());
-    const float inv = 1.f / sum;
-#pragma unroll
-    for (int i = 0; i < S; ++i)
-#pragma unroll
-      for (int e = 0; e < V; ++e) p[i][e] *= inv;
-    return top + logf(sum);
+    inv = __builtin_amdgcn_rcpf(sum);
+    return (c + __builtin_amdgcn_logf(sum)) * 0.69314718055994531f;  // base 2 to natural
   }
 };
 
@@ -187,9 +183,16 @@ __global__ __launch_bounds__(kThreads) void balance_forward(BalArgs a) {
   // The choices meanwhile: one entry a thread.
   const int64_t* index = a.index + (b * a.tokens + t0) * a.top;
   const int entries = (int)(t1 - t0) * a.top;
-  for (int at = tid; at < entries; at += kThreads) {
-    const int64_t e = index[at];
-    if (e >= 0 && e < a.experts && (!mask || mask[(t0 + at / a.top) * a.mask_t])) atomicAdd(&seen[e], 1);
+  for (int at0 = tid; at0 < entries; at0 += 4 * kThreads) {
+    int64_t e[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) e[k] = index[min(at0 + k * kThreads, entries - 1)];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int at = at0 + k * kThreads;
+      if (at < entries && e[k] >= 0 && e[k] < a.experts && (!mask || mask[(t0 + at / a.top) * a.mask_t]))
+        atomicAdd(&seen[e[k]], 1);
+    }
   }
   for (int64_t first = t0; first < t1; first += kStep) {
     const Token<DT, V, kL, S> now = x;
@@ -198,16 +201,15 @@ __global__ __launch_bounds__(kThreads) void balance_forward(BalArgs a) {
     row += kStep * a.row * Elem<DT>::kBytes;
     live = t < t1 && (!mask || mask[t * a.mask_t]);
     x.load(row, a.experts, l, live);
-    float q[S][V];
-    const float lse = now.softmax(a.experts, l, q);
-    if (counts) {
+    float q[S][V], inv;
+    const float lse = now.softmax(a.experts, l, q, inv);
+    inv = counts ? inv : 0.f;  // a token without a part reads zeros: finite
 #pragma unroll
-      for (int i = 0; i < S; ++i)
+    for (int i = 0; i < S; ++i)
 #pragma unroll
-        for (int e = 0; e < V; ++e) p[i][e] += q[i][e];
-      z += lse * lse;
-      ++n;
-    }
+      for (int e = 0; e < V; ++e) p[i][e] += q[i][e] * inv;
+    z += counts ? lse * lse : 0.f;
+    n += counts;
   }
   // The wave's tokens, then the waves.
 #pragma unroll
@@ -299,19 +301,19 @@ __global__ __launch_bounds__(kThreads) void balance_backward(BalArgs a) {
   int64_t t = t0 + wave * kTokens + sub;
   const char* row = a.logits + (b * a.tokens + t) * a.row * ES;
   char* out = a.grad + (b * a.tokens + t) * a.grad_row * ES;
-  const int n = a.live[b];
+  const int n = (int)a.live[b];
   Token<DT, V, kL, S> x;
-  bool live = t < t1 && n > 0 && (!mask || mask[t * a.mask_t]);
+  bool live = t < t1 && (!mask || mask[t * a.mask_t]);
   x.load(row, a.experts, l, live);
   const float inv = n ? 1.f / (float)n : 0.f;
   const float up = (a.up ? a.up[b] : 0.f) * (float)a.experts * inv, up_z = (a.up_z ? a.up_z[b] : 0.f) * 2.f * inv;
-  float f[S][V];
+  float f[S][V];  // up f
 #pragma unroll
   for (int i = 0; i < S; ++i)
 #pragma unroll
     for (int e = 0; e < V; ++e) {
       const int at = (l + i * kL) * V + e;
-      f[i][e] = at < a.experts ? (float)a.counts[b * a.experts + at] * inv : 0.f;
+      f[i][e] = at < a.experts ? up * ((float)a.counts[b * a.experts + at] * inv) : 0.f;
     }
   for (int64_t first = t0; first < t1; first += kStep) {
     const Token<DT, V, kL, S> now = x;
@@ -320,22 +322,21 @@ __global__ __launch_bounds__(kThreads) void balance_backward(BalArgs a) {
     t += kStep;
     row += kStep * a.row * ES;
     out += kStep * a.grad_row * ES;
-    live = t < t1 && n > 0 && (!mask || mask[t * a.mask_t]);
+    live = t < t1 && (!mask || mask[t * a.mask_t]);
     x.load(row, a.experts, l, live);
-    float q[S][V], dot = 0.f;
-    const float lse = now.softmax(a.experts, l, q);
+    float q[S][V], by, dot = 0.f;
+    const float lse = now.softmax(a.experts, l, q, by);
 #pragma unroll
     for (int i = 0; i < S; ++i)
 #pragma unroll
       for (int e = 0; e < V; ++e) dot += f[i][e] * q[i][e];
-    dot = over_lanes<kL>(dot, Sum());
-    const float with_z = up_z * lse;
+    const float rest = up_z * lse - over_lanes<kL>(dot, Sum()) * by;
 #pragma unroll
     for (int i = 0; i < S; ++i) {
       const int e0 = (l + i * kL) * V;
       float g[V];
 #pragma unroll
-      for (int e = 0; e < V; ++e) g[e] = lives ? q[i][e] * (up * (f[i][e] - dot) + with_z) : 0.f;
+      for (int e = 0; e < V; ++e) g[e] = lives ? q[i][e] * by * (f[i][e] + rest) : 0.f;
       if (!there || e0 >= a.experts) continue;
       if constexpr (V == 1) Elem<DT>::store(to, e0, g[0]);
       else {
@@ -374,13 +375,12 @@ Shape shape_of(int dtype, int experts, bool aligned) {
   return s;
 }
 
-constexpr int64_t kWantBlocks = 1024;
-
-// Tokens of a workgroup: at least `least` of its steps, and a sample of up to twice
+// Tokens of a workgroup: `least` of its steps, more where the tokens fill `most`
+// workgroups; a sample of up to twice
 // that stays whole (the forward pass then needs no second launch).
-void chunking(BalArgs& a, const Shape& s, int64_t least) {
+void chunking(BalArgs& a, const Shape& s, int64_t least, int64_t most) {
   const int64_t step = kWaves * kWave / s.lanes;
-  const int64_t steps = std::max<int64_t>(least, a.batch * a.tokens / (step * kWantBlocks));
+  const int64_t steps = std::max<int64_t>(least, a.batch * a.tokens / (step * most));
   a.chunk = step * steps;
   if (a.tokens <= 2 * a.chunk) a.chunk = std::max<int64_t>(a.tokens, 1);
   a.chunks = std::max<int64_t>((a.tokens + a.chunk - 1) / a.chunk, 1);
@@ -427,7 +427,7 @@ struct Launch {
   }
 };
 
-constexpr int64_t kForwardSteps = 4, kBackwardSteps = 1;
+constexpr int64_t kForwardSteps = 4, kForwardBlocks = 2048, kBackwardSteps = 1, kBackwardBlocks = 2048;
 
 }  // namespace
 }  // namespace da
@@ -444,7 +444,7 @@ int da_balance_loss_workspace(int dtype, int64_t batch, int64_t tokens, int expe
   for (int aligned = 0; aligned < 2; ++aligned) {
     BalArgs a{};
     a.batch = batch, a.tokens = tokens, a.experts = experts;
-    chunking(a, shape_of(dtype, experts, aligned), kForwardSteps);
+    chunking(a, shape_of(dtype, experts, aligned), kForwardSteps, kForwardBlocks);
     *bytes = std::max(*bytes, partial_bytes(a));
   }
   return DA_OK;
@@ -452,7 +452,7 @@ int da_balance_loss_workspace(int dtype, int64_t batch, int64_t tokens, int expe
 
 int da_balance_loss(const void* logits, int dtype, int64_t batch, int64_t tokens, int experts, int64_t row_stride,
                     const int64_t* index, int top, const uint8_t* mask, int64_t mask_bstride, int64_t mask_tstride,
-                    float* loss, float* z_loss, int32_t* counts, int32_t* live, void* workspace,
+                    float* loss, float* z_loss, int64_t* counts, int64_t* live, void* workspace,
                     size_t workspace_bytes, void* stream) {
   const char* what = "da_balance_loss";
   if (int rc = check_args(what, dtype, batch, tokens, experts)) return rc;
@@ -466,7 +466,7 @@ int da_balance_loss(const void* logits, int dtype, int64_t batch, int64_t tokens
   a.row = row_stride, a.mask_b = mask_bstride, a.mask_t = mask_tstride, a.experts = experts, a.top = top;
   a.loss = loss, a.z_loss = z_loss, a.counts = counts, a.live = live;
   const Shape shape = shape_of(dtype, experts, (uintptr_t)logits % 16 == 0 && row_stride * es % 16 == 0);
-  chunking(a, shape, kForwardSteps);
+  chunking(a, shape, kForwardSteps, kForwardBlocks);
   const size_t need = partial_bytes(a);
   if (need && (!workspace || workspace_bytes < need))
     return set_error(DA_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", what, workspace_bytes, need);
@@ -486,7 +486,7 @@ int da_balance_loss(const void* logits, int dtype, int64_t batch, int64_t tokens
 }
 
 int da_balance_loss_grad(const float* up, const float* up_z, const void* logits, int dtype, int64_t batch,
-                         int64_t tokens, int experts, int64_t row_stride, const int32_t* counts, const int32_t* live,
+                         int64_t tokens, int experts, int64_t row_stride, const int64_t* counts, const int64_t* live,
                          const uint8_t* mask, int64_t mask_bstride, int64_t mask_tstride, void* grad,
                          int64_t grad_row_stride, void* stream) {
   const char* what = "da_balance_loss_grad";
@@ -497,10 +497,10 @@ int da_balance_loss_grad(const float* up, const float* up_z, const void* logits,
   BalArgs a{};
   a.up = up, a.up_z = up_z, a.logits = (const char*)logits, a.mask = mask, a.tokens = tokens, a.batch = batch;
   a.row = row_stride, a.mask_b = mask_bstride, a.mask_t = mask_tstride, a.experts = experts;
-  a.counts = (int32_t*)counts, a.live = (int32_t*)live, a.grad = (char*)grad, a.grad_row = grad_row_stride;
+  a.counts = (int64_t*)counts, a.live = (int64_t*)live, a.grad = (char*)grad, a.grad_row = grad_row_stride;
   const bool aligned = ((uintptr_t)logits | (uintptr_t)grad) % 16 == 0 && (row_stride | grad_row_stride) * es % 16 == 0;
   const Shape shape = shape_of(dtype, experts, aligned);
-  chunking(a, shape, kBackwardSteps);
+  chunking(a, shape, kBackwardSteps, kBackwardBlocks);
   if (batch * a.chunks > 0x7fffffff) return set_error(DA_ERR_UNSUPPORTED, "%s: too many tokens", what);
   Launch{a, true, (hipStream_t)stream}(dtype, shape);
   return check_launch(what);

@@ -69,7 +69,8 @@ def qk_norm_rope(q, k, q_weight, k_weight, inv_freq, positions=None, *, eps: flo
     ``slots``: a ``(q, k)`` pair that takes the weights' per-sample gradients in
     the backward pass, in place of their summed ones (``FusedCapture``)."""
     cfg = {"eps": eps, "interleaved": interleaved, "scaling": scaling}
-    if torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in (q, k, q_weight, k_weight)):
+    if torch.is_grad_enabled() and (q.requires_grad or q_weight.requires_grad or (
+            k is not None and k_weight is not None and (k.requires_grad or k_weight.requires_grad))):
         return _QkNormRope.apply(q, k, q_weight, k_weight, inv_freq, positions, mask, cfg, slots)
     return kernels.qk_norm_rope(q, k, q_weight, k_weight, inv_freq, positions, mask=mask, **cfg)
 

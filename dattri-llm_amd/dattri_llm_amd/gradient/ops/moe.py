@@ -41,8 +41,8 @@ class BalanceLoss(NamedTuple):
 
     loss: torch.Tensor  # (B,)
     z_loss: torch.Tensor  # (B,)
-    counts: torch.Tensor  # (B, E) int32
-    live: torch.Tensor  # (B,) int32
+    counts: torch.Tensor  # (B, E) int64
+    live: torch.Tensor  # (B,) int64
 
 
 class _BalanceLoss(torch.autograd.Function):

@@ -1680,8 +1680,8 @@ def relative_bias_grad(g: torch.Tensor, num_buckets: int, *, q_start: int = 0, b
 
 def balance_loss(logits: torch.Tensor, index: torch.Tensor, *, batch: int = 1, mask=None):
     """Router losses of ``batch`` samples of equally many tokens
-    (``da_balance_loss``): ``(loss (B,), z_loss (B,), counts (B, E) int32, live
-    (B,) int32)`` of ``(N, E)`` logits and the ``(N, k)`` int64 choices."""
+    (``da_balance_loss``): ``(loss (B,), z_loss (B,), counts (B, E) int64, live
+    (B,) int64)`` of ``(N, E)`` logits and the ``(N, k)`` int64 choices."""
     if logits.dim() != 2 or index.dim() != 2 or index.shape[0] != logits.shape[0]:
         raise ValueError("balance_loss expects (N, E) logits and (N, k) expert indices")
     if index.dtype != torch.int64:
@@ -1695,8 +1695,8 @@ def balance_loss(logits: torch.Tensor, index: torch.Tensor, *, batch: int = 1, m
     logits, index = _unit_rows(logits), index.contiguous()
     loss = torch.empty((batch,), dtype=torch.float32, device=dev)
     z_loss = torch.empty((batch,), dtype=torch.float32, device=dev)
-    counts = torch.empty((batch, e), dtype=torch.int32, device=dev)
-    live = torch.empty((batch,), dtype=torch.int32, device=dev)
+    counts = torch.empty((batch, e), dtype=torch.int64, device=dev)
+    live = torch.empty((batch,), dtype=torch.int64, device=dev)
     lib = nat.load()
     ws_ptr, nbytes = None, ctypes.c_size_t(0)
     nat.check(lib.da_balance_loss_workspace(code, batch, n // batch, e, ctypes.byref(nbytes)), "balance_loss")
@@ -1728,8 +1728,8 @@ def balance_loss_grad(up, up_z, logits: torch.Tensor, counts: torch.Tensor, live
     batch = counts.shape[0]
     if batch < 1 or n % batch or live.shape != (batch,):
         raise ValueError(f"balance_loss_grad: {n} tokens are not {batch} samples of one length")
-    if counts.dtype != torch.int32 or live.dtype != torch.int32:
-        raise ValueError("balance_loss_grad: counts and live must be int32, as balance_loss returns them")
+    if counts.dtype != torch.int64 or live.dtype != torch.int64:
+        raise ValueError("balance_loss_grad: counts and live must be int64, as balance_loss returns them")
     up, up_z = _per_sample("balance_loss_grad", up, batch), _per_sample("balance_loss_grad", up_z, batch)
     code = nat.dtype_code(logits.dtype)
     mask, mask_ptr, mask_b, mask_t = _token_mask("balance_loss_grad", mask, batch, n // batch)

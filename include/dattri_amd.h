@@ -825,10 +825,10 @@ int da_relative_bias_grad(const void* g, int dtype, int64_t batch, int64_t heads
 int da_balance_loss_workspace(int dtype, int64_t batch, int64_t tokens, int experts, size_t* bytes);
 int da_balance_loss(const void* logits, int dtype, int64_t batch, int64_t tokens, int experts, int64_t row_stride,
                     const int64_t* index, int top, const uint8_t* mask, int64_t mask_bstride, int64_t mask_tstride,
-                    float* loss, float* z_loss, int32_t* counts, int32_t* live, void* workspace,
+                    float* loss, float* z_loss, int64_t* counts, int64_t* live, void* workspace,
                     size_t workspace_bytes, void* stream);
 int da_balance_loss_grad(const float* up, const float* up_z, const void* logits, int dtype, int64_t batch,
-                         int64_t tokens, int experts, int64_t row_stride, const int32_t* counts, const int32_t* live,
+                         int64_t tokens, int experts, int64_t row_stride, const int64_t* counts, const int64_t* live,
                          const uint8_t* mask, int64_t mask_bstride, int64_t mask_tstride, void* grad,
                          int64_t grad_row_stride, void* stream);
 

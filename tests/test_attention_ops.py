@@ -119,7 +119,7 @@ def test_relative_bias_refuses():
 
 def test_balance_loss_refuses():
     x, i = torch.zeros(6, 4), torch.zeros(6, 2, dtype=torch.int64)
-    counts, live = torch.zeros(2, 4, dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
+    counts, live = torch.zeros(2, 4, dtype=torch.int64), torch.zeros(2, dtype=torch.int64)
     for bad, words in ((lambda: ops.moe.balance_loss(x, i[:5]), "expert indices"),
                        (lambda: ops.moe.balance_loss(x[0], i), "expects"),
                        (lambda: ops.moe.balance_loss_grad(None, None, x[0], counts, live), "expects"),
@@ -130,7 +130,7 @@ def test_balance_loss_refuses():
                        (lambda: ops.moe.balance_loss(x, i, batch=2, mask=torch.ones(3, 2)), "mask must have shape"),
                        (lambda: ops.moe.balance_loss_grad(None, None, x, counts[:, :3], live), "counts"),
                        (lambda: ops.moe.balance_loss_grad(None, None, x, counts, live[:1]), "samples of one length"),
-                       (lambda: ops.moe.balance_loss_grad(None, None, x, counts.long(), live), "int32"),
+                       (lambda: ops.moe.balance_loss_grad(None, None, x, counts.int(), live), "int64"),
                        (lambda: ops.moe.balance_loss_grad(torch.ones(3), None, x, counts, live), "loss gradient")):
         with pytest.raises(ValueError, match=words):
             bad()
