@@ -21,6 +21,7 @@ bits or more (no compute-dtype policy applies).
 from __future__ import annotations
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from dattri_llm_amd import kernels
 
@@ -33,6 +34,7 @@ class _QkNormRope(torch.autograd.Function):
         return kernels.qk_norm_rope(q, k, q_weight, k_weight, inv_freq, positions, mask=mask, **cfg)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, gq, gk):
         q, k, q_weight, k_weight, inv_freq, positions, mask = ctx.saved_tensors
         # None: no gradient reached that output.
@@ -93,6 +95,7 @@ class _RelativeBias(torch.autograd.Function):
         return bias if batch is None else bias.expand(batch, -1, -1, -1)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, g):
         (mask,) = ctx.saved_tensors
         buckets, dtype = ctx.table

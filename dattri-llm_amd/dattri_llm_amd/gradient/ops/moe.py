@@ -22,6 +22,7 @@ from __future__ import annotations
 from typing import NamedTuple
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from dattri_llm_amd import kernels
 from dattri_llm_amd.gradient.ops import dtypes
@@ -54,6 +55,7 @@ class _BalanceLoss(torch.autograd.Function):
         return loss, z_loss, counts, live
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, up, up_z, _counts, _live):
         logits, counts, live, mask = ctx.saved_tensors
         return kernels.balance_loss_grad(up, up_z, logits, counts, live, mask=mask), None, None, None

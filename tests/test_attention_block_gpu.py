@@ -123,3 +123,18 @@ def test_without_the_session_parameters_get_summed_gradients(device):
     cap.clear()
     with pytest.raises(RuntimeError, match="no layer"):
         cap.gradient()
+
+
+def test_no_second_derivatives(device):
+    """A gradient of a gradient is refused, not taken for zero."""
+    q, w = torch.randn(1, 3, 2, 16, device=device, requires_grad=True), torch.ones(16, device=device)
+    freq = torch.ones(8, device=device)
+    table = torch.randn(16, 2, device=device, requires_grad=True)
+    logits = torch.randn(6, 4, device=device, requires_grad=True)
+    index = torch.zeros(6, 1, dtype=torch.int64, device=device)
+    for leaf, loss in ((q, ops.qk_norm_rope(q, None, w, None, freq)[0].square().sum()),
+                       (table, ops.relative_bias(table, 5, 5).square().sum()),
+                       (logits, ops.moe.balance_loss(logits, index).z_loss.square().sum())):
+        (grad,) = torch.autograd.grad(loss, leaf, create_graph=True)
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            grad.sum().backward()
