@@ -177,6 +177,8 @@ struct GradArgs {
 // Row blocks of a group of lanes at most (even): its sums lie in LDS.
 __host__ __device__ constexpr int max_steps(int group) { return group == 64 ? 64 : 16; }
 
+constexpr int kGroups = 4;  // of a team
+
 __device__ const u32x4 kZeros = {0, 0, 0, 0};
 
 // Whole-wave (kG 64) or row-of-16 shift by one lane: lane l takes lane l - 1's
@@ -192,19 +194,26 @@ __device__ __forceinline__ float from_left(float v) {
 // each row block, so its sums move one lane right: every load of the walk is
 // whole lines, all lanes work, and all groups alike.  The sums of the diagonal
 // block that leaves at the last lane go to its slot in LDS, at the end those of
-// all lanes.  An offset lies in up to three slots of each group; their sums form the
-// workgroup's line, and sixteen lanes sum a bucket's range of it.
+// all lanes.  An offset lies in up to three slots of each group; their sums form a
+// line, and sixteen lanes sum a bucket's range of it.  Four groups are a team: with
+// groups of 16 (narrow planes) a wave is a team, and four heads share a workgroup.
 template <int DT, int R, int kG>
 __global__ __launch_bounds__(kThreads) void bias_backward(GradArgs a, Edges e) {
-  constexpr int V = Elem<DT>::kVec, ES = Elem<DT>::kBytes, kGroups = kThreads / kG;
+  constexpr int V = Elem<DT>::kVec, ES = Elem<DT>::kBytes;
+  constexpr int kTeam = kGroups * kG, kTeams = kThreads / kTeam;
   using W = Walk<V, R>;
   constexpr int kSums = W::kLast - W::kFirst + 1, kSlot = (kSums + 3) / 4 * 4;
-  extern __shared__ __attribute__((aligned(16))) float slots[];  // [kGroups][steps + kG][kSlot]
+  extern __shared__ __attribute__((aligned(16))) float shared[];
   __shared__ int ranges[kMaxBuckets][2];
   __shared__ uint8_t live_rows[kGroups * max_steps(kG)];
-  const int tid = threadIdx.x, l = tid % kG, group = tid / kG;
+  const int tid = threadIdx.x, team = tid / kTeam, u = tid % kTeam, l = u % kG;
+  const int group = kG == 64 ? __builtin_amdgcn_readfirstlane(u / kG) : u / kG;
   const int window = blockIdx.x % a.windows, split = blockIdx.x / a.windows;
-  const int64_t h = blockIdx.y, b = blockIdx.z;
+  const int64_t own = (int64_t)blockIdx.y * kTeams + team, b = blockIdx.z;
+  const int64_t h = min(own, a.heads - 1);  // a team past the heads only keeps step
+  // A team's LDS: slots [kGroups][steps + kG][kSlot], then its line of offsets.
+  const int line_at = kGroups * (a.steps + kG) * kSlot;
+  float* slots = shared + team * (line_at + (kGroups * a.steps + kG + 1) * V);
   const char* plane = a.g + (b * a.g_b + h * a.g_h) * ES;
   const int mis = (int)((uintptr_t)plane / ES % V);
   const int k_len = (int)a.k_len, q_len = (int)a.q_len;
@@ -213,11 +222,12 @@ __global__ __launch_bounds__(kThreads) void bias_backward(GradArgs a, Edges e) {
   const int begin = split * kGroups * a.steps;
   const int r0 = begin + group * a.steps, r1 = min(r0 + a.steps, a.row_blocks);
   auto store = [&](int x, float u) {
+    if (own >= a.heads) return;
     if (a.blocks == 1) a.out[(b * a.buckets + x) * a.heads + h] = u;
     else a.partial[((b * a.heads + h) * a.blocks + blockIdx.x) * a.buckets + x] = u;
   };
   if (window * kG - a.last_block >= begin + kGroups * a.steps) {  // causal: all keys follow the queries
-    if (tid < a.buckets) store(tid, 0.f);
+    for (int x = u; x < a.buckets; x += kTeam) store(x, 0.f);
     return;
   }
   float* mine = slots + group * (a.steps + kG) * kSlot;
@@ -271,22 +281,33 @@ __global__ __launch_bounds__(kThreads) void bias_backward(GradArgs a, Edges e) {
       for (int q = 0; q < V; ++q) sum[W::at(x, q) - W::kFirst] += f[q];
     }
   };
-  // Any row block: a run without a live entry, or one that sticks out of the
-  // plane (its entries are added one by one), reads zeros instead.
+  int runs = 0;  // bit x: the run of row x has a live entry
+#pragma unroll
+  for (int x = 0; x < V; ++x) runs |= ((cols >> (V - 1 - W::shift(x)) & kRows) != 0) << x;
+  // Only a plane's first and last row block, or rows closer than two runs, have
+  // runs that stick out of the plane (bit x): their entries are added one by one.
+  auto torn_of = [&](int r) {
+    int torn = 0;
+    if (r > 0 && r < a.row_blocks - 1 && a.g_i >= 2 * V) return torn;
+#pragma unroll
+    for (int x = 0; x < V; ++x) {
+      const int64_t at = ((int64_t)(r * V) + x) * a.g_i + first - W::shift(x);
+      torn |= (at < 0 || at + V > plane_end) << x;
+    }
+    return torn;
+  };
+  // Any row block: a run without a live entry, or a torn one, reads zeros instead.
   auto rows_of = [&](int r) {
     int rows = r >= r1 || c - r > a.last_block ? 0 : q_len - r * V >= V ? kRows : (1 << (q_len - r * V)) - 1;
     if (a.mask && r < r1) rows &= live_rows[r - begin];
     return rows;
   };
   auto load_some = [&](u32x4 (&v)[V], int r) {
-    const int rows = rows_of(r);
-    const int64_t at0 = (int64_t)(r * V) * a.g_i + first;
+    const int need = rows_of(r) & runs & ~torn_of(r);
+    const char* at = plane + ((int64_t)(r * V) * a.g_i + first) * ES;
 #pragma unroll
-    for (int x = 0; x < V; ++x) {
-      const int64_t at = at0 + x * a.g_i - W::shift(x);
-      const bool ok = rows >> x & 1 && (cols >> (V - 1 - W::shift(x)) & kRows) && at >= 0 && at + V <= plane_end;
-      v[x] = *(ok ? (const u32x4*)(plane + at * ES) : &kZeros);
-    }
+    for (int x = 0; x < V; ++x)
+      v[x] = *(need >> x & 1 ? (const u32x4*)(at + (x * a.g_i - W::shift(x)) * ES) : &kZeros);
   };
   auto add_some = [&](u32x4 (&v)[V], int r) {
     int keep_cols = cols;
@@ -296,22 +317,21 @@ __global__ __launch_bounds__(kThreads) void bias_backward(GradArgs a, Edges e) {
 #pragma unroll
       for (int q = 0; q < 4; ++q) {  // entries that are not there, or dead, to zero bits
         const int at = V - 1 - W::shift(x) + q * 4 / ES;
-        uint32_t keep = keep_cols >> at & 1 ? ~0u : 0u;
-        if constexpr (ES == 2) keep = (keep & 0xffffu) | (keep_cols >> (at + 1) & 1 ? 0xffff0000u : 0u);
+        uint32_t keep = (uint32_t)__builtin_amdgcn_sbfe(keep_cols, at, 1);
+        if constexpr (ES == 2)
+          keep = (keep & 0xffffu) | ((uint32_t)__builtin_amdgcn_sbfe(keep_cols, at + 1, 1) & 0xffff0000u);
         v[x][q] &= keep;
       }
     add_whole(v);
-    // Only a plane's first and last row block, or rows closer than two runs, reach out of it.
-    if (r > 0 && r < a.row_blocks - 1 && a.g_i >= 2 * V) return;
-    const int rows = rows_of(r);
+    const int torn = torn_of(r) & rows_of(r);
+    if (!__any(torn)) return;
 #pragma unroll
     for (int x = 0; x < V; ++x) {
       const int64_t at = ((int64_t)(r * V) + x) * a.g_i + first - W::shift(x);
-      if (rows >> x & 1 && (at < 0 || at + V > plane_end)) {
 #pragma unroll
-        for (int q = 0; q < V; ++q)
-          if (cols >> (V - 1 - W::shift(x) + q) & 1) sum[W::at(x, q) - W::kFirst] += Elem<DT>::load(plane, at + q);
-      }
+      for (int q = 0; q < V; ++q)
+        if (torn >> x & 1 && cols >> (V - 1 - W::shift(x) + q) & 1)
+          sum[W::at(x, q) - W::kFirst] += Elem<DT>::load(plane, at + q);
     }
   };
   // On to row block r0 + step + 1.  Diagonal block c - r lies in slot l + steps - 1 - step.
@@ -364,32 +384,32 @@ __global__ __launch_bounds__(kThreads) void bias_backward(GradArgs a, Edges e) {
   }
   __syncthreads();
 
-  // The workgroup's line of offsets: block 0 is the last group's first slot.
-  float* line = slots + kGroups * (a.steps + kG) * kSlot;
+  // The team's line of offsets: block 0 is the last group's first slot.
+  float* line = slots + line_at;
   const int used = a.steps + kG - 1, blocks = (kGroups - 1) * a.steps + used, length = (blocks - 1) * V + kSums;
-  for (int p = tid; p < length; p += kThreads) {
+  for (int p = u; p < length; p += kTeam) {
     const int k = p / V, t = p % V;
-    float u = 0.f;
+    float sum_p = 0.f;
 #pragma unroll
     for (int back = 0; back < 3; ++back) {
       if (t + back * V >= kSums) continue;
       int at = k - back - (kGroups - 1) * a.steps;
-#pragma unroll 4
+#pragma unroll
       for (int g = 0; g < kGroups; ++g, at += a.steps)
-        if (at >= 0 && at < used) u += slots[(g * (a.steps + kG) + at) * kSlot + t + back * V];
+        if (at >= 0 && at < used) sum_p += slots[(g * (a.steps + kG) + at) * kSlot + t + back * V];
     }
-    line[p] = u;
+    line[p] = sum_p;
   }
   __syncthreads();
-  const int lane = tid & 15;
+  const int lane = u & 15;
   const int o0 = (window * kG - (begin + kGroups * a.steps - 1)) * V + W::kFirst - 2 * (V - 1) - mis - a.start;
-  for (int x = tid >> 4; x < a.buckets; x += kThreads / 16) {
+  for (int x = u >> 4; x < a.buckets; x += kTeam / 16) {
     const int from = max(ranges[x][0] - o0, 0), to = min(ranges[x][1] - o0, length - 1);
-    float u = 0.f;
-    for (int p = from + lane; p <= to; p += 16) u += line[p];
+    float sum_x = 0.f;
+    for (int p = from + lane; p <= to; p += 16) sum_x += line[p];
 #pragma unroll
-    for (int off = 8; off > 0; off >>= 1) u += __shfl_xor(u, off, 16);
-    if (lane == 0) store(x, u);
+    for (int off = 8; off > 0; off >>= 1) sum_x += __shfl_xor(sum_x, off, 16);
+    if (lane == 0) store(x, sum_x);
   }
 }
 
@@ -449,15 +469,26 @@ GradPlan grad_plan(int v, bool aligned, int64_t planes, int64_t q_len, int64_t k
     columns = std::max<int64_t>(std::min(columns, last + p.row_blocks), 1);
   }
   p.last_block = (int)last;
-  p.group = columns <= 16 ? 16 : 64;
-  const int groups = kThreads / p.group;
+  // Groups of 16 where those of 64 would leave a quarter more of their lanes idle.
+  const int64_t by16 = (columns + 15) / 16 * 16, by64 = (columns + 63) / 64 * 64;
+  p.group = by16 * 5 <= by64 * 4 ? 16 : 64;
   p.windows = (int)((columns + p.group - 1) / p.group);
-  int64_t steps = p.row_blocks * planes * p.windows / (kWantBlocks * groups);
+  const int teams = kThreads / (kGroups * p.group);
+  int64_t steps = p.row_blocks * planes * p.windows / (kWantBlocks * kGroups * teams);
   steps = std::min<int64_t>(std::max<int64_t>(steps, 8), max_steps(p.group));
-  steps = std::min<int64_t>(steps, (p.row_blocks + groups - 1) / groups);
+  steps = std::min<int64_t>(steps, (p.row_blocks + kGroups - 1) / kGroups);
   p.steps = (int)(steps + 1) & ~1;
-  p.splits = (p.row_blocks + groups * p.steps - 1) / (groups * p.steps);
+  p.splits = (p.row_blocks + kGroups * p.steps - 1) / (kGroups * p.steps);
   return p;
+}
+
+// Bytes of LDS of a team.
+template <int DT, int R>
+size_t team_lds(const GradPlan& p) {
+  constexpr int V = 16 / (DT == DA_F32 ? 4 : 2);
+  using W = Walk<V, R>;
+  constexpr int kSlot = (W::kLast - W::kFirst + 1 + 3) / 4 * 4;
+  return (size_t)(kGroups * (p.steps + p.group) * kSlot + (kGroups * p.steps + p.group + 1) * V) * sizeof(float);
 }
 
 int check_sizes(const char* what, int64_t batch, int64_t heads, int64_t q_len, int64_t k_len, int64_t start) {
@@ -558,13 +589,13 @@ int da_relative_bias_grad(const void* g, int dtype, int64_t batch, int64_t heads
   if (need && (!workspace || workspace_bytes < need))
     return set_error(DA_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", what, workspace_bytes, need);
   a.partial = (float*)workspace;
-  const dim3 grid((unsigned)a.blocks, (unsigned)heads, (unsigned)batch);
-  const int groups = kThreads / p.group;
-  const size_t lds = (size_t)(groups * (p.steps + p.group) * 3 + groups * p.steps + p.group + 1) * v * sizeof(float);
+  const int teams = kThreads / (kGroups * p.group);
+  const dim3 grid((unsigned)a.blocks, (unsigned)((heads + teams - 1) / teams), (unsigned)batch);
 #define DA_BWD(DT, R)                                                                 \
   case R:                                                                             \
-    if (p.group == 16) bias_backward<DT, R, 16><<<grid, kThreads, lds, st>>>(a, e);   \
-    else bias_backward<DT, R, 64><<<grid, kThreads, lds, st>>>(a, e);                 \
+    if (p.group == 16)                                                                \
+      bias_backward<DT, R, 16><<<grid, kThreads, team_lds<DT, R>(p) * teams, st>>>(a, e); \
+    else bias_backward<DT, R, 64><<<grid, kThreads, team_lds<DT, R>(p), st>>>(a, e);  \
     break;
 #define DA_BWD8(DT)                                                                                    \
   switch (g_istride % 8) {                                                                             \
