@@ -87,6 +87,7 @@ struct BiasArgs {
   int64_t t_b, t_h;  // table strides in elements
   int start, causal;
   int columns, windows, steps;  // column blocks, windows of kWave of them; row blocks of a workgroup
+  int spread;                   // runs that a row may be ahead of its line: 7, or 0 where all rows start one
   uint32_t closed;              // bits of -inf
 };
 
@@ -105,8 +106,15 @@ __device__ __forceinline__ void store_bits(char* p, int64_t i, uint32_t v) {
 // blocks.  The run of row rV + e in column block c depends on e and on c - r alone:
 // the runs of all diagonal blocks lie ready in LDS, one array for each e, and a
 // store is one 16-byte LDS read (neighbouring lanes read neighbours) and one
-// aligned 16-byte write, a row's whole lines by one wave.  Runs that a row's end
+// aligned 16-byte write.  Each row's columns are shifted so that a wave's 64 runs
+// are whole 128-byte lines: a line that two workgroups write in parts goes to memory
+// twice (32 x 2047 x 2047 bf16: 84 us unshifted, 72 us so).  Runs that a row's end
 // cuts are written entry by entry at the end.
+//
+// Bound by the writes: 32 x 2048 x 2048 bf16 takes 48 us into one buffer, 55 us into
+// alternating ones (5.6 and 4.9 TB/s; a kernel that only fills memory 5.3 to 5.6).
+// With the runs in the lanes' registers, lanes on fixed diagonals, it took 86 us: a
+// wave's columns then start at any run, and every line is written in parts.
 template <int ES>
 __global__ __launch_bounds__(kThreads) void bias_forward(BiasArgs a, Edges e) {
   constexpr int V = 16 / ES;
@@ -119,8 +127,9 @@ __global__ __launch_bounds__(kThreads) void bias_forward(BiasArgs a, Edges e) {
   char* plane = a.out + h * a.q_len * a.k_len * ES;
   const int mis = (int)((uintptr_t)plane / ES % V);
   const int k_len = (int)a.k_len, i0 = r0 * V, rows = (int)min((int64_t)a.steps * V, a.q_len - i0);
-  const int c0 = window * kWave, width = min(kWave, a.columns - c0);
-  const int blocks = width + a.steps - 1, k0 = c0 - (r0 + a.steps - 1);  // diagonal blocks, the first of them
+  const int c0 = window * kWave, width = min(kWave, a.columns + a.spread - c0);
+  // Diagonal blocks, the first of them: a row's column blocks start up to `spread` before c0.
+  const int blocks = width + a.steps - 1 + a.spread, k0 = c0 - a.spread - (r0 + a.steps - 1);
   uint32_t* line = (uint32_t*)(runs + V * blocks);
   if (tid < e.n) least[tid] = e.least[tid];
   if (tid < (e.both ? 2 : 1) * e.n) column[tid] = load_bits<ES>(a.table, tid * a.t_b + h * a.t_h);
@@ -131,6 +140,12 @@ __global__ __launch_bounds__(kThreads) void bias_forward(BiasArgs a, Edges e) {
   }
   __syncthreads();
   const int stride = k_len % V;
+  // Runs from a line's start to column block 0 of row i (whole lines are a power of
+  // two long: the product may wrap).
+  const uint32_t base = (uint32_t)((uintptr_t)plane / 16);
+  auto ahead = [&](int i, int shift) {
+    return (int)((base + ((uint32_t)(i0 + i) * (uint32_t)k_len - (uint32_t)shift) / V) & (uint32_t)a.spread);
+  };
   for (int n = tid; n < min(rows, V) * blocks; n += kThreads) {
     const int r = n / blocks, k = n - r * blocks;
     const uint32_t* at = line + k * V + 2 * (V - 1) - r - r * stride % V;
@@ -144,19 +159,22 @@ __global__ __launch_bounds__(kThreads) void bias_forward(BiasArgs a, Edges e) {
   const int c = tid % width;
   if (tid < together * width)
     for (int i = tid / width; i < rows; i += together) {
-      const int r = i % V, j = (c0 + c) * V - mis - r * stride % V;
+      const int r = i % V, shift = r * stride % V, at = c - ahead(i, shift), j = (c0 + at) * V - mis - shift;
       if (j >= 0 && j + V <= k_len)
-        st16(plane + ((int64_t)(i0 + i) * k_len + j) * ES, runs[r * blocks + c + a.steps - 1 - i / V]);
+        st16(plane + ((int64_t)(i0 + i) * k_len + j) * ES, runs[r * blocks + at + a.spread + a.steps - 1 - i / V]);
     }
   if (stride == 0 && mis == 0) return;
   for (int n = tid; n < rows * 2 * V; n += kThreads) {  // the first and the last run of each row
-    const int i = n / (2 * V), x = n % V, r = i % V, shift = mis + r * stride % V;
-    const int at = n % (2 * V) < V ? shift / V : (k_len - 1 + shift) / V;  // column block
-    const int first = at * V - shift, j = first + x;
+    const int i = n / (2 * V), x = n % V, r = i % V, shift = r * stride % V;
+    const int head = (mis + shift) / V, tail = (k_len - 1 + mis + shift) / V;  // their column blocks
+    const bool second = n % (2 * V) >= V;
+    if (second && tail == head) continue;  // one run is both
+    const int at = (second ? tail : head) - c0, first = (c0 + at) * V - mis - shift, j = first + x;
     if (first >= 0 && first + V <= k_len) continue;  // a whole run
-    if (n % (2 * V) >= V && at == shift / V) continue;  // one run is both
-    if (j >= 0 && j < k_len && at >= c0 && at < c0 + width)
-      store_bits<ES>(plane, (int64_t)(i0 + i) * k_len + j, line[(at - c0 + a.steps - 1 - i / V) * V + 2 * (V - 1) - r - r * stride % V + x]);
+    const int c = at + ahead(i, shift);
+    if (j >= 0 && j < k_len && c >= 0 && c < width)
+      store_bits<ES>(plane, (int64_t)(i0 + i) * k_len + j,
+                     line[(at + a.spread + a.steps - 1 - i / V) * V + 2 * (V - 1) - r - shift + x]);
   }
 }
 
@@ -523,7 +541,8 @@ int da_relative_bias(const void* table, int dtype, int64_t table_bstride, int64_
   a.t_h = table_hstride, a.start = (int)q_start, a.causal = causal;
   // A row's first run may start up to 2 (v - 1) entries before it.
   a.columns = (int)((k_len - 1 + (aligned ? 0 : 2 * (v - 1))) / v + 1);
-  a.windows = (a.columns + kWave - 1) / kWave;
+  a.spread = (uintptr_t)out % 128 == 0 && k_len * es % 128 == 0 ? 0 : 7;
+  a.windows = (a.columns + a.spread + kWave - 1) / kWave;
   // Row blocks of a workgroup: 4 to 32, so that there are kWantBlocks workgroups.
   a.steps = (int)std::min<int64_t>(std::max<int64_t>(row_blocks * a.windows * heads / kWantBlocks, 4), 32);
   a.steps = (int)std::min<int64_t>(a.steps, row_blocks);
@@ -532,7 +551,7 @@ int da_relative_bias(const void* table, int dtype, int64_t table_bstride, int64_
   const int64_t grid_x = a.windows * ((row_blocks + a.steps - 1) / a.steps);
   if (grid_x > 0x7fffffff) return set_error(DA_ERR_UNSUPPORTED, "%s: too many entries", what);
   const dim3 grid((unsigned)grid_x, (unsigned)heads);
-  const int blocks = std::min<int>(kWave, a.columns) + a.steps - 1;
+  const int blocks = std::min<int>(kWave, a.columns + a.spread) + a.steps - 1 + a.spread;
   const size_t lds = (size_t)v * blocks * 16 + (size_t)(blocks + 2) * v * 4;
   if (es == 2) bias_forward<2><<<grid, kThreads, lds, st>>>(a, e);
   else bias_forward<4><<<grid, kThreads, lds, st>>>(a, e);
