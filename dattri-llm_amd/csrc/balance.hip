@@ -51,32 +51,6 @@ struct BalArgs {
 };
 
 // ---------------------------------------------------------------------------
-// Reductions over a token's lanes.
-// ---------------------------------------------------------------------------
-template <int kCtrl>
-__device__ __forceinline__ float dpp(float v) {
-  return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), kCtrl, 0xf, 0xf, true));
-}
-// quad_perm [1, 0, 3, 2] and [2, 3, 0, 1], row_half_mirror, row_mirror: each pairs
-// lanes whose values already agree within the halves that it joins.
-template <int kL, class Op>
-__device__ __forceinline__ float over_lanes(float v, Op op) {
-  if constexpr (kL >= 2) v = op(v, dpp<0xb1>(v));
-  if constexpr (kL >= 4) v = op(v, dpp<0x4e>(v));
-  if constexpr (kL >= 8) v = op(v, dpp<0x141>(v));
-  if constexpr (kL >= 16) v = op(v, dpp<0x140>(v));
-  if constexpr (kL >= 32) v = op(v, __shfl_xor(v, 16, kWave));
-  if constexpr (kL >= 64) v = op(v, __shfl_xor(v, 32, kWave));
-  return v;
-}
-struct Sum {
-  __device__ float operator()(float a, float b) const { return a + b; }
-};
-struct Max {
-  __device__ float operator()(float a, float b) const { return fmaxf(a, b); }
-};
-
-// ---------------------------------------------------------------------------
 // One token's logits: lane l of its kL holds runs l, l + kL, ... of V experts.
 // ---------------------------------------------------------------------------
 template <int DT, int V, int kL, int S>
@@ -113,7 +87,7 @@ struct Token {
 #pragma unroll
       for (int e = 0; e < V; ++e) top = fmaxf(top, in ? p[i][e] : -__builtin_inff());
     }
-    top = over_lanes<kL>(top, Max());
+    top = lanes_max<kL>(top);
     const float c = top * kLog2e;
     float sum = 0.f;
 #pragma unroll
@@ -127,7 +101,7 @@ struct Token {
         sum += p[i][e];
       }
     }
-    sum = over_lanes<kL>(sum, Sum());
+    sum = lanes_sum<kL>(sum);
     inv = __builtin_amdgcn_rcpf(sum);
     return (c + __builtin_amdgcn_logf(sum)) * 0.69314718055994531f;  // base 2 to natural
   }
@@ -330,7 +304,7 @@ __global__ __launch_bounds__(kThreads) void balance_backward(BalArgs a) {
     for (int i = 0; i < S; ++i)
 #pragma unroll
       for (int e = 0; e < V; ++e) dot += f[i][e] * q[i][e];
-    const float rest = up_z * lse - over_lanes<kL>(dot, Sum()) * by;
+    const float rest = up_z * lse - lanes_sum<kL>(dot) * by;
 #pragma unroll
     for (int i = 0; i < S; ++i) {
       const int e0 = (l + i * kL) * V;

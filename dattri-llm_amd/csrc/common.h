@@ -188,6 +188,32 @@ __device__ __forceinline__ float wave_sum(float v) {
   return v;
 }
 
+// Over groups of kL lanes (a power of two), the result in all of them: within
+// sixteen lanes by DPP -- quad_perm [1, 0, 3, 2] and [2, 3, 0, 1], row_half_mirror,
+// row_mirror, each of which pairs lanes that agree within the halves it joins.
+template <int kCtrl>
+__device__ __forceinline__ float lane_dpp(float v) {
+  return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), kCtrl, 0xf, 0xf, true));
+}
+template <int kL, class Op>
+__device__ __forceinline__ float over_lanes(float v, Op op) {
+  if constexpr (kL >= 2) v = op(v, lane_dpp<0xb1>(v));
+  if constexpr (kL >= 4) v = op(v, lane_dpp<0x4e>(v));
+  if constexpr (kL >= 8) v = op(v, lane_dpp<0x141>(v));
+  if constexpr (kL >= 16) v = op(v, lane_dpp<0x140>(v));
+  if constexpr (kL >= 32) v = op(v, __shfl_xor(v, 16, kWave));
+  if constexpr (kL >= 64) v = op(v, __shfl_xor(v, 32, kWave));
+  return v;
+}
+template <int kL>
+__device__ __forceinline__ float lanes_sum(float v) {
+  return over_lanes<kL>(v, [](float a, float b) { return a + b; });
+}
+template <int kL>
+__device__ __forceinline__ float lanes_max(float v) {
+  return over_lanes<kL>(v, [](float a, float b) { return fmaxf(a, b); });
+}
+
 // ---------------------------------------------------------------------------
 // Grid helpers.
 // ---------------------------------------------------------------------------

@@ -269,23 +269,6 @@ __device__ __forceinline__ void lane_weights(const float* from, int l, float (&w
     }
 }
 
-// Sum over a group of kL lanes, in all of them: within sixteen lanes by DPP
-// (neighbours, pairs, then mirrored halves, whose lanes agree by then).
-template <int kCtrl>
-__device__ __forceinline__ float add_dpp(float v) {
-  return v + __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), kCtrl, 0xf, 0xf, true));
-}
-template <int kL>
-__device__ __forceinline__ float lanes_sum(float v) {
-  v = add_dpp<0xb1>(v);                         // quad_perm [1, 0, 3, 2]
-  v = add_dpp<0x4e>(v);                         // quad_perm [2, 3, 0, 1]
-  if constexpr (kL >= 8) v = add_dpp<0x141>(v);   // row_half_mirror
-  if constexpr (kL >= 16) v = add_dpp<0x140>(v);  // row_mirror
-  if constexpr (kL >= 32) v += __shfl_xor(v, 16, kWave);
-  if constexpr (kL >= 64) v += __shfl_xor(v, 32, kWave);
-  return v;
-}
-
 // A wave takes units in turn: a token's heads, or every `parts`-th group of them
 // where the tokens are few.
 template <int DT, int V, int kL, int S, bool kInter, bool kStream>
