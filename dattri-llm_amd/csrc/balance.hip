@@ -15,6 +15,12 @@
 // probability goes to memory.  A workgroup sums a chunk of one sample's tokens; a
 // sample of one chunk is finished there, else a second launch joins its chunks in
 // order.  Counts are whole numbers: their LDS atomics have no order to keep.
+//
+// 32 x 4096 tokens, 128 experts, top-8, bf16 (42 MB read forward, 67 MB read and
+// written backward): 13.7 + 4.6 us forward, 17.7 us backward; one wave a token, from
+// memory to the losses, 132 us for both.  The exponentials and butterflies take about
+// half of that, HBM the rest.  Small layers are bound by their launches: 16 x 256
+// tokens of 8 experts 5.8 and 3.6 us.
 #include <algorithm>
 
 #include "common.h"
@@ -401,6 +407,8 @@ struct Launch {
   }
 };
 
+// 32 x 4096 tokens of 128 experts: backward 22 us at 4096 workgroups, 17.7 at 2048,
+// 19.8 at 512; forward 17.4 at 512, 14.5 at 1024, 13.7 at 2048.
 constexpr int64_t kForwardSteps = 4, kForwardBlocks = 2048, kBackwardSteps = 1, kBackwardBlocks = 2048;
 
 }  // namespace

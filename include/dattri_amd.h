@@ -789,10 +789,10 @@ int da_qk_norm_rope_grad(const da_qk_side* sides, int dtype, int weight_dtype, i
  *
  * of g (batch, heads, q_len, k_len) with contiguous rows and any other strides
  * (0 broadcasts).  causal: entries with j > i + q_start add nothing, whatever
- * they hold.  mask
- * (bytes, batch x k_len; query i is position i + q_start of it, which has to lie
- * inside): entries of a dead query or key add nothing, whatever they hold.
- * NULL: none.  The sums run in a fixed order.  Lengths and q_start up to 2^26.
+ * they hold.  mask (bytes, batch x k_len; query i is position i + q_start of it,
+ * which has to lie inside): entries of a dead query or key add nothing, whatever
+ * they hold; NULL: none.  The sums run in a fixed order.  Lengths and q_start up
+ * to 2^26, batch and heads up to 65535.
  */
 int da_relative_bias(const void* table, int dtype, int64_t table_bstride, int64_t table_hstride, int64_t heads,
                      int64_t q_len, int64_t k_len, int64_t q_start, const int32_t* edges, int side_buckets,
