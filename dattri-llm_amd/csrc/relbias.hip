@@ -619,6 +619,7 @@ int da_relative_bias_grad(const void* g, int dtype, int64_t batch, int64_t heads
   const size_t need = a.blocks > 1 ? (size_t)(a.blocks * batch * heads * buckets) * sizeof(float) : 0;
   if (need && (!workspace || workspace_bytes < need))
     return set_error(DA_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", what, workspace_bytes, need);
+  if (a.blocks > 0x7fffffff) return set_error(DA_ERR_UNSUPPORTED, "%s: too many entries", what);
   a.partial = (float*)workspace;
   const int teams = kThreads / (kGroups * p.group);
   const dim3 grid((unsigned)a.blocks, (unsigned)((heads + teams - 1) / teams), (unsigned)batch);

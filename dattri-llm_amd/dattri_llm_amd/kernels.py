@@ -1560,7 +1560,7 @@ def _qk_rope(what, q, k, q_weight, k_weight, inv_freq, positions, mask, gq, gk, 
     inv_freq = inv_freq.contiguous()
     sides = array.array("q", words_q + words_k)
     args = (sides.buffer_info()[0], code, w_code, b, t, d, rot, inv_freq.data_ptr(), pos_ptr, pos_bytes, pos_b, pos_t,
-            mask_ptr, mask_b, mask_t, int(interleaved), scaling, eps)
+            mask_ptr, mask_b, mask_t, int(interleaved), float(scaling), float(eps))
     lib = nat.load()
     if gq is None:
         _run_on(dev, what, lib.da_qk_norm_rope, *args, nat.stream_ptr(dev))

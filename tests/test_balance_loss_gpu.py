@@ -234,3 +234,28 @@ def test_two_streams_and_a_graph(device):
         torch.cuda.synchronize()
         want = call()
         assert all(torch.equal(a, b) for a, b in zip(out, want)), i
+
+
+def test_transposed_logits_and_offsets_past_32_bits(device):
+    x, index = make(1, 3, 16, 2, torch.bfloat16)
+    want = ops.moe.balance_loss(x.to(device), index.to(device))
+    across = x[0].t().contiguous().to(device).t()  # experts first in memory
+    got = ops.moe.balance_loss(across, index[0].to(device))
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+    far = torch.empty((1 << 33) + 64, dtype=torch.bfloat16, device=device)
+    rows = far.as_strided((3, 16), (1 << 32, 1))
+    rows.copy_(x[0])
+    got = ops.moe.balance_loss(rows, index[0].to(device))
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+    up = torch.ones(1, device=device)
+    assert torch.equal(ops.moe.balance_loss_grad(up, up, rows, got.counts, got.live),
+                       ops.moe.balance_loss_grad(up, up, x[0].to(device), got.counts, got.live))
+
+
+def test_expanded_loss_gradients(device):
+    x, index = make(5, 12, 8, 2, torch.float32)
+    got = ops.moe.balance_loss(x.to(device), index.to(device))
+    one = torch.ones(1, device=device)
+    a = ops.moe.balance_loss_grad(one.expand(5), one.double().expand(5), x.to(device), got.counts, got.live)
+    b = ops.moe.balance_loss_grad(one.repeat(5), one.repeat(5), x.to(device), got.counts, got.live)
+    assert torch.equal(a, b)

@@ -329,3 +329,39 @@ def test_captured_and_replayed(device):
         want = call()
         assert all(torch.equal(a, b) for a, b in zip(out, want)), i
         assert math.isfinite(float(out[0].float().sum()))
+
+
+@pytest.mark.parametrize("w_dt", DTYPES, ids=NAME.get)
+@pytest.mark.parametrize("dt", DTYPES, ids=NAME.get)
+def test_weights_of_another_type(dt, w_dt, device):
+    q, k, gq, gk, wq, wk, freq, p = inputs(2, 9, 6, 2, 64, 32, dt)
+    wq, wk = wq.to(w_dt), wk.to(w_dt)
+    zq, zk = ops.qk_norm_rope(q, k, wq, wk, freq, eps=torch.tensor(1e-6))
+    dq, dk, dwq, dwk = ops.qk_norm_rope_grad(gq, gk, q, k, wq, wk, freq)
+    check_side(zq, dq, dwq, q, gq, wq, freq, p, 1e-6, False, 1.0, None)
+    check_side(zk, dk, dwk, k, gk, wk, freq, p, 1e-6, False, 1.0, None)
+
+
+def test_offsets_past_32_bits(device):
+    """Samples 2^32 entries apart, in every operand."""
+    q, k, gq, gk, wq, wk, freq, p = inputs(2, 5, 3, 1, 128, 128, torch.bfloat16)
+    far = torch.empty((1 << 32) + 4096, dtype=torch.bfloat16, device=device)
+
+    def apart(x, at):
+        view = far.as_strided(x.shape, (1 << 32, *x.stride()[1:]), at)
+        view.copy_(x)
+        return view
+
+    q2, gq2 = apart(q, 0), apart(gq, 2048)
+    want = (*ops.qk_norm_rope(q, k, wq, wk, freq), *ops.qk_norm_rope_grad(gq, gk, q, k, wq, wk, freq))
+    got = (*ops.qk_norm_rope(q2, k, wq, wk, freq), *ops.qk_norm_rope_grad(gq2, gk, q2, k, wq, wk, freq))
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+def test_many_tokens_and_many_samples(device):
+    """More tokens than one pass of the waves, more samples than workgroups of one."""
+    for b, t in ((1, 20000), (3000, 2)):
+        q, k, gq, gk, wq, wk, freq, p = inputs(b, t, 2, 1, 16, 16, torch.float32)
+        zq, _ = ops.qk_norm_rope(q, k, wq, wk, freq)
+        dq, _, dwq, _ = ops.qk_norm_rope_grad(gq, gk, q, k, wq, wk, freq)
+        check_side(zq, dq, dwq, q, gq, wq, freq, p, 1e-6, False, 1.0, None)

@@ -231,3 +231,27 @@ def test_two_streams_and_a_graph(device):
         torch.cuda.synchronize()
         want = call()
         assert all(torch.equal(a, b) for a, b in zip(out, want)), i
+
+
+def test_offsets_past_32_bits(device):
+    """Samples 2^32 entries apart; a plane of 70000 x 40000; an output of as many."""
+    g = torch.randn(2, 2, 33, 40, device=device).bfloat16()
+    far = torch.zeros((1 << 32) + 8192, dtype=torch.bfloat16, device=device)
+    view = far.as_strided(g.shape, (1 << 32, *g.stride()[1:]))
+    view.copy_(g)
+    assert torch.equal(ops.relative_bias_grad(view, 32), ops.relative_bias_grad(g, 32))
+    del view
+    plane = far[: 70000 * 40000].view(1, 1, 70000, 40000).zero_()
+    entries = [(0, 0), (69999, 39999), (69999, 0), (0, 39999), (50000, 39990), (40010, 39999), (54000, 123)]
+    want = torch.zeros(32)
+    for n, (i, j) in enumerate(entries):
+        plane[0, 0, i, j] = 2.0 ** n
+        _, ids = ids_of(1, 1, i - j, 32, 128, True)
+        want[ids[0, 0]] += 2.0 ** n
+    assert torch.equal(ops.relative_bias_grad(plane, 32)[0, :, 0].cpu(), want)
+    del plane, far
+    table = torch.randn(32, 2, device=device).bfloat16()
+    out = ops.relative_bias(table, 50000, 50001)
+    for h, i, j in ((1, 49999, 50000), (1, 49999, 0), (0, 49999, 49990), (1, 0, 50000), (1, 43000, 43002)):
+        _, ids = ids_of(1, 1, i - j, 32, 128, True)
+        assert out[h, i, j] == table[ids[0, 0], h]
