@@ -17,10 +17,10 @@
 // order.  Counts are whole numbers: their LDS atomics have no order to keep.
 //
 // 32 x 4096 tokens, 128 experts, top-8, bf16 (42 MB read forward, 67 MB read and
-// written backward): 13.7 + 4.6 us forward, 17.7 us backward; one wave a token, from
+// written backward): 13.0 + 4.7 us forward, 17.1 us backward; one wave a token, from
 // memory to the losses, 132 us for both.  The exponentials and butterflies take about
 // half of that, HBM the rest.  Small layers are bound by their launches: 16 x 256
-// tokens of 8 experts 5.8 and 3.6 us.
+// tokens of 8 experts 5.6 and 3.6 us.
 #include <algorithm>
 
 #include "common.h"
@@ -64,49 +64,47 @@ struct Token {
   static constexpr int ES = Elem<DT>::kBytes;
   u32x4 raw[V == 1 ? (S + 3) / 4 : S];  // V == 1: one value a word
 
+  // Runs past the experts hold -inf: no weight in the largest logit or the sum.  A
+  // token without a part holds zeros: its softmax is finite, and not used.
   __device__ void load(const char* row, int experts, int l, bool live) {
 #pragma unroll
     for (int i = 0; i < S; ++i) {
       const int e = (l + i * kL) * V;
-      const bool in = live && e < experts;
+      const uint32_t none = e < experts ? 0u : DT == DA_F32 ? 0xff800000u : DT == DA_BF16 ? 0xff80ff80u : 0xfc00fc00u;
       if constexpr (V == 1) {
-        uint32_t w = 0;
-        if (in) w = ES == 4 ? *(const uint32_t*)(row + e * ES) : *(const uint16_t*)(row + e * ES);
+        uint32_t w = ES == 4 ? none : none & 0xffffu;
+        if (live && e < experts) w = ES == 4 ? *(const uint32_t*)(row + e * ES) : *(const uint16_t*)(row + e * ES);
         raw[i / 4][i % 4] = w;
       } else {
-        raw[i] = u32x4{0, 0, 0, 0};
-        if (in) raw[i] = ld16(row + e * ES);
+        raw[i] = u32x4{none, none, none, none};
+        if (live && e < experts) raw[i] = ld16(row + e * ES);
       }
     }
   }
-  // p = exp(logit - c) for a c next to the largest logit, 0 past the experts; inv =
-  // 1 / their sum; returns the logits' logsumexp.  c is the largest logit times
-  // log2(e) as fp32 rounds it: that rounding is common to all experts, the sum
-  // takes it back out, and each exponent is one fma, rounded once.
-  __device__ float softmax(int experts, int l, float (&p)[S][V], float& inv) const {
+  // p = exp(logit - c) for a c next to the largest logit; inv = 1 / their sum;
+  // returns the logits' logsumexp.  c is the largest logit times log2(e) as fp32
+  // rounds it: that rounding is common to all experts, the sum takes it back out,
+  // and each exponent is one fma, rounded once.
+  __device__ float softmax(float (&p)[S][V], float& inv) const {
     float top = -__builtin_inff();
 #pragma unroll
     for (int i = 0; i < S; ++i) {
-      const bool in = (l + i * kL) * V < experts;
       if constexpr (V == 1) p[i][0] = Elem<DT>::from_bits(raw[i / 4][i % 4]);
       else unpack16<DT>(raw[i], p[i]);
 #pragma unroll
-      for (int e = 0; e < V; ++e) top = fmaxf(top, in ? p[i][e] : -__builtin_inff());
+      for (int e = 0; e < V; ++e) top = fmaxf(top, p[i][e]);
     }
     top = lanes_max<kL>(top);
     const float c = top * kLog2e;
     float sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < S; ++i) {
-      const bool in = (l + i * kL) * V < experts;
+    for (int i = 0; i < S; ++i)
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         // All -inf: inf - inf is NaN here, as in a softmax.
-        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(p[i][e], kLog2e, -c));
-        p[i][e] = in ? x : 0.f;
+        p[i][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[i][e], kLog2e, -c));
         sum += p[i][e];
       }
-    }
     sum = lanes_sum<kL>(sum);
     inv = __builtin_amdgcn_rcpf(sum);
     return (c + __builtin_amdgcn_logf(sum)) * 0.69314718055994531f;  // base 2 to natural
@@ -182,7 +180,7 @@ __global__ __launch_bounds__(kThreads) void balance_forward(BalArgs a) {
     live = t < t1 && (!mask || mask[t * a.mask_t]);
     x.load(row, a.experts, l, live);
     float q[S][V], inv;
-    const float lse = now.softmax(a.experts, l, q, inv);
+    const float lse = now.softmax(q, inv);
     inv = counts ? inv : 0.f;  // a token without a part reads zeros: finite
 #pragma unroll
     for (int i = 0; i < S; ++i)
@@ -305,7 +303,7 @@ __global__ __launch_bounds__(kThreads) void balance_backward(BalArgs a) {
     live = t < t1 && (!mask || mask[t * a.mask_t]);
     x.load(row, a.experts, l, live);
     float q[S][V], by, dot = 0.f;
-    const float lse = now.softmax(a.experts, l, q, by);
+    const float lse = now.softmax(q, by);
 #pragma unroll
     for (int i = 0; i < S; ++i)
 #pragma unroll
@@ -392,8 +390,10 @@ struct Launch {
     else if (s.lanes == 32) kernel<DT, V, 32, 1>();
     else if (s.runs == 1) kernel<DT, V, 64, 1>();
     else if (s.runs == 2) kernel<DT, V, 64, 2>();
-    else if (V < 8 && s.runs <= 4) kernel<DT, V, V < 8 ? 64 : 1, V < 8 ? 4 : 1>();
-    else if (V == 1) kernel<DT, V, V == 1 ? 64 : 1, V == 1 ? 16 : 1>();
+    else if constexpr (V < 8) {
+      if (s.runs <= 4) kernel<DT, V, 64, 4>();
+      else if constexpr (V == 1) kernel<DT, V, 64, 16>();
+    }
   }
   template <int DT>
   void runs(const Shape& s) const {
