@@ -8,7 +8,8 @@
 // is at most r, plus n (the buckets of one side) where bidirectional and o > 0.
 // The edges are integers worked out by the caller, so that no logarithm decides
 // which side of a border a distance falls on.  With `causal`, keys after their
-// query are no part of the attention: the bias is -inf there and g is not read.
+// query are no part of the attention: the bias is -inf there, and whatever g holds
+// there adds nothing.
 #include <algorithm>
 
 #include "common.h"
@@ -293,7 +294,9 @@ __global__ __launch_bounds__(kThreads) void bias_backward(GradArgs a, Edges e) {
 #pragma unroll
   for (int t = 0; t < kSlot; ++t) sum[t] = 0.f;
 
-  // The lane's runs of row block r: every entry there, live and counted.
+  // The lane's runs of row block r: every entry there, live and counted. Read
+  // once, and past the caches: 537 MB of scores take 91 us so and 102 us cached, 33
+  // MB 15.7 and 14.8.
   auto load_whole = [&](u32x4 (&v)[V], int r) {
     const char* at = plane + ((int64_t)(r * V) * a.g_i + first) * ES;
 #pragma unroll
