@@ -224,7 +224,7 @@ __device__ __forceinline__ float from_left(float v) {
 // for 537 MB (6.2 TB/s; a kernel that only reads reaches 6.3, streamed 6.9) and 4 us
 // to join.  A thread a diagonal took 4075 us; lanes on fixed diagonals 125, a third of
 // them past the planes' corners.  Rows of any other length than a multiple of V need
-// their ends masked: 1023 x 1023 134 us.  Small planes are bound by what a team does
+// their ends masked: 1023 x 1023 122 us.  Small planes are bound by what a team does
 // once (10 us: edges, slots, line, buckets): 512 of 128 x 128 take 11 us.
 template <int DT, int R, int kG>
 __global__ __launch_bounds__(kThreads) void bias_backward(GradArgs a, Edges e) {
@@ -500,11 +500,12 @@ GradPlan grad_plan(int v, bool aligned, int64_t planes, int64_t q_len, int64_t k
     columns = std::max<int64_t>(std::min(columns, last + p.row_blocks), 1);
   }
   p.last_block = (int)last;
-  // Groups of 16 where those of 64 would leave a quarter more of their lanes idle
-  // (512 planes of 513 x 513: 87 us in groups of 16, 149 in groups of 64; where both
-  // fit, groups of 64 are 10% faster: 1024 x 1024).
+  // Groups of 16 where those of 64 would have half as many lanes again, idle ones: 512
+  // planes of 513 x 513 take 94 us in groups of 16, 128 in groups of 64.  With fewer
+  // idle lanes the longer lines of 64 count for more: 300 x 300 48 us against 67,
+  // 1023 x 1023 122 against 133.
   const int64_t by16 = (columns + 15) / 16 * 16, by64 = (columns + 63) / 64 * 64;
-  p.group = by16 * 5 <= by64 * 4 ? 16 : 64;
+  p.group = by16 * 3 <= by64 * 2 ? 16 : 64;
   p.windows = (int)((columns + p.group - 1) / p.group);
   const int teams = kThreads / (kGroups * p.group);
   int64_t steps = p.row_blocks * planes * p.windows / (kWantBlocks * kGroups * teams);
