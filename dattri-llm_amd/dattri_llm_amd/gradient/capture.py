@@ -143,7 +143,9 @@ class FusedCapture:
     :class:`RelativeBias` layers inside autograd.
 
     ``layers``: names of the modules to capture (default: all of these types).
-    A captured ``RelativeBias`` has to be called with ``batch``.
+    A captured ``RelativeBias`` has to be called with ``batch``; the gradients of
+    these two are small and kept whole, whatever ``proj_dim`` and
+    ``capture_style`` are.
     ``proj_dim``: LoGRA projection width (``None``: unprojected capture), with
     ``proj_seed`` / ``projector`` as in ``project_factors`` (seed for the
     gradient side, seed + 1 for the activation side).  ``capture_style``:

@@ -138,3 +138,22 @@ def test_no_second_derivatives(device):
         (grad,) = torch.autograd.grad(loss, leaf, create_graph=True)
         with pytest.raises(RuntimeError, match="once_differentiable"):
             grad.sum().backward()
+
+
+@pytest.mark.parametrize("style", ["factorized", "materialized"])
+def test_a_projected_session_keeps_these_gradients_whole(device, style):
+    torch.manual_seed(3)
+    model = Block().to(device)
+    x = torch.randn(3, 11, WIDTH, device=device)
+    mask = torch.ones(3, 11, dtype=torch.bool, device=device)
+    whole, projected = FusedCapture(model), FusedCapture(model, proj_dim=8, capture_style=style)
+    for cap in (whole, projected):
+        with cap:
+            sample_losses(model, x, x.flip(1), mask).sum().backward()
+    a, b = whole.gradient(), projected.gradient()
+    assert set(a.layer_names) == set(b.layer_names)
+    for n in ("rope.q_weight", "rope.k_weight", "bias"):
+        assert torch.equal(a.data[n], b.data[n])
+    scores = ops.layerwise_cross_dot(b, b)
+    want = sum((v := b.materialize().data[n].double().flatten(1)) @ v.T for n in b.layer_names)
+    assert_parity(scores if torch.is_tensor(scores) else sum(scores.values()), want, "float32", tight=6e-5)
