@@ -81,10 +81,9 @@ struct Token {
       }
     }
   }
-  // p = exp(logit - c) for a c next to the largest logit; inv = 1 / their sum;
-  // returns the logits' logsumexp.  c is the largest logit times log2(e) as fp32
-  // rounds it: that rounding is common to all experts, the sum takes it back out,
-  // and each exponent is one fma, rounded once.
+  // p = exp(logit - largest); inv = 1 / their sum; returns the logits' logsumexp.
+  // The difference is taken first: equal logits of any size, a type's lowest value
+  // among them, leave zeros.
   __device__ float softmax(float (&p)[S][V], float& inv) const {
     float top = -__builtin_inff();
 #pragma unroll
@@ -95,19 +94,18 @@ struct Token {
       for (int e = 0; e < V; ++e) top = fmaxf(top, p[i][e]);
     }
     top = lanes_max<kL>(top);
-    const float c = top * kLog2e;
     float sum = 0.f;
 #pragma unroll
     for (int i = 0; i < S; ++i)
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         // All -inf: inf - inf is NaN here, as in a softmax.
-        p[i][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[i][e], kLog2e, -c));
+        p[i][e] = __builtin_amdgcn_exp2f((p[i][e] - top) * kLog2e);
         sum += p[i][e];
       }
     sum = lanes_sum<kL>(sum);
     inv = __builtin_amdgcn_rcpf(sum);
-    return (c + __builtin_amdgcn_logf(sum)) * 0.69314718055994531f;  // base 2 to natural
+    return top + __builtin_amdgcn_logf(sum) * 0.69314718055994531f;  // base 2 to natural
   }
 };
 

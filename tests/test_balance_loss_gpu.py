@@ -123,6 +123,38 @@ def test_closed_experts_and_extreme_logits(device):
     assert bool(torch.isnan(got.loss[1])) and bool(torch.isfinite(got.loss[0]))
 
 
+@pytest.mark.parametrize("dt", DTYPES, ids=NAME.get)
+@pytest.mark.parametrize("experts", [8, 33])
+def test_tokens_whose_logits_are_all_filled(dt, experts, device):
+    """A token all of whose experts hold one large fill value, the type's lowest
+    among them, is spread evenly; beside an ordinary logit a fill has no weight."""
+    big = float(torch.finfo(dt).max)
+    fills = [-big, big, -min(1e30, big / 2), min(1e12, big / 4), -min(1e9, big / 8)]
+    for fill in fills:
+        x, index = make(2, 12, experts, 2, dt)
+        x[:, 3:6] = fill
+        if fill < 0:
+            x[0, 7, 1:] = fill
+            x[1, 8, :-1] = fill
+        dev_x, dev_index = x.to(device), index.to(device)
+        got = ops.moe.balance_loss(dev_x, dev_index)
+        up = torch.tensor([1.0, -0.5])
+        grad = ops.moe.balance_loss_grad(up.to(device), None, dev_x, got.counts, got.live)
+        xd = x.double().requires_grad_()
+        loss, z, counts, n = plain(xd, index, torch.ones(2, 12, dtype=torch.bool))
+        (loss * up.double()).sum().backward()
+        assert torch.equal(got.counts.cpu(), counts) and torch.equal(got.live.cpu().double(), n)
+        assert bool(((got.loss.cpu().double() - loss).abs() <= TIGHT_FP32 * loss).all()), fill
+        square = (xd.detach().abs().amax(-1) ** 2).amax()
+        if square < 3e38:  # else fp32 holds no such square
+            assert bool(((got.z_loss.cpu().double() - z).abs() <= TIGHT_FP32 * z).all()), fill
+        else:
+            assert bool(torch.isinf(got.z_loss).all()), fill
+        # terms up (E/n) p f: p <= 1, f <= 1
+        tol = TIGHT_FP32 * experts / 12 + HALF_ULP.get(NAME[dt], 0.0) * xd.grad.abs() + 2.0 ** -25
+        assert bool(((grad.cpu().double() - xd.grad).abs() <= tol).all()), fill
+
+
 def test_dropped_and_repeated_choices(device):
     x, index = make(2, 40, 8, 3, torch.float32)
     index[0, :10, 0] = -1  # dropped
