@@ -66,7 +66,8 @@ def qk_norm_rope(q, k, q_weight, k_weight, inv_freq, positions=None, *, eps: flo
     ``(B, T)``, by default the token's index; ``inv_freq`` float32.  ``mask`` (B,
     T): a token with a zero gets zero rows, whatever its input holds, and takes
     no part in any gradient.  ``k`` may be None.  Inputs of any strides; outputs
-    keep their layout.  A single new token is ``T = 1`` with its position.
+    keep their layout (contiguous where rows overlap in memory).  A single new
+    token is ``T = 1`` with its position.
 
     ``slots``: a ``(q, k)`` pair that takes the weights' per-sample gradients in
     the backward pass, in place of their summed ones (``FusedCapture``)."""

@@ -1508,6 +1508,8 @@ def _qk_side(what: str, x, w, gz, wgrad):
         raise ValueError(f"{what}: a norm weight must have shape ({x.shape[3]},)")
     x, w = _unit_rows(x), w.contiguous()
     out = torch.empty_like(x)
+    if out.stride(3) != 1:  # the kernels write whole rows; rows that overlap may give another order of the axes
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     xb, xt, xh, _ = x.stride()
     ob, ot, oh, _ = out.stride()
     if gz is None:
@@ -1578,7 +1580,8 @@ def _qk_rope(what, q, k, q_weight, k_weight, inv_freq, positions, mask, gq, gk, 
 def qk_norm_rope(q, k, q_weight, k_weight, inv_freq, positions=None, *, eps: float, interleaved: bool = False,
                  scaling: float = 1.0, mask=None):
     """RMS norm of each head's queries and keys with the position rotation
-    (``da_qk_norm_rope``): ``(q_out, k_out)`` like ``q`` and ``k``.
+    (``da_qk_norm_rope``): ``(q_out, k_out)`` like ``q`` and ``k``, contiguous
+    where their rows overlap in memory.
 
     ``q`` (B, T, Hq, D) and ``k`` (B, T, Hk, D, or None) may have any strides
     (a copy is made where entries are not contiguous); weights ``(D,)``,

@@ -95,6 +95,34 @@ def test_qk_norm_rope_refuses_types_gradients_and_the_cpu():
         ops.qk_norm_rope(**a)
 
 
+OVERLAPPING = {  # rows of 16 that share entries, as sliding windows do: their strides leave the axes' order open
+    "windows": lambda x: x.view(-1)[:48].view(2, 24).unfold(1, 16, 1).unsqueeze(2),
+    "windows of heads": lambda x: x.view(-1)[:240].view(2, 5, 24).unfold(2, 16, 1),
+    "one entry apart": lambda x: x.view(-1).as_strided((2, 5, 3, 16), (100, 1, 40, 1)),
+    "one head": lambda x: x.view(-1).as_strided((2, 1, 3, 16), (0, 1, 0, 1)),
+}
+
+
+@pytest.mark.parametrize("how", [*OVERLAPPING, "expanded", "fused", "one entry"])
+def test_rows_are_written_where_no_other_row_lies(how):
+    """What the kernels are told of the output: entries in a row, and each row's
+    place its own."""
+    x = torch.zeros(4, 6, 8, 16)
+    x = {**OVERLAPPING, "expanded": lambda x: x[:1, :, :1].expand(4, 6, 8, 16), "fused": lambda x: x[:, :, 2:5],
+         "one entry": lambda x: x[..., 3:4]}[how](x)
+    words, out, *_ = kernels._qk_side("test", x, torch.ones(x.shape[3]), None, None)
+    told = dict(zip([f[0] for f in nat.QkSide._fields_], words))
+    at = sum(torch.arange(n).view([-1 if i == axis else 1 for i in range(3)]) * told[f"out_{name}stride"]
+             for axis, (n, name) in enumerate(zip(x.shape[:3], "bth")))
+    at = at[..., None] + torch.arange(x.shape[3])
+    assert told["out"] == out.data_ptr() and out.shape == x.shape
+    assert at.unique().numel() == x.numel() and int(at.max()) < out.untyped_storage().nbytes() // 4
+    # and the output's own strides say the same
+    mine = sum(torch.arange(n).view([-1 if i == axis else 1 for i in range(4)]) * out.stride(axis)
+               for axis, n in enumerate(x.shape))
+    assert torch.equal(at, mine)
+
+
 def test_relative_bias_refuses():
     table, g = torch.zeros(32, 4), torch.zeros(2, 4, 5, 9)
     with pytest.raises(ValueError, match="table"):

@@ -365,3 +365,20 @@ def test_many_tokens_and_many_samples(device):
         zq, _ = ops.qk_norm_rope(q, k, wq, wk, freq)
         dq, _, dwq, _ = ops.qk_norm_rope_grad(gq, gk, q, k, wq, wk, freq)
         check_side(zq, dq, dwq, q, gq, wq, freq, p, 1e-6, False, 1.0, None)
+
+
+@pytest.mark.parametrize("dt", DTYPES, ids=NAME.get)
+@pytest.mark.parametrize("inter", [False, True])
+@pytest.mark.parametrize("t,shift", [(9, 1), (13, 4), (40, 8), (1, 3)])
+def test_rows_that_overlap_in_memory(t, shift, inter, dt, device):
+    """Sliding windows over one line a sample, queries, keys and gradients alike:
+    each output row has a place of its own."""
+    b, d = 2, 16
+    _, _, _, _, wq, wk, freq, p = inputs(b, t, 1, 1, d, d, dt)
+    gen = torch.Generator().manual_seed(t)
+    q, k, gq, gk = (torch.randn(b, d + shift * (t - 1), generator=gen).to(dt).to(device).unfold(1, d, shift).unsqueeze(2)
+                    for _ in range(4))
+    zq, zk = ops.qk_norm_rope(q, k, wq, wk, freq, interleaved=inter)
+    dq, dk, dwq, dwk = ops.qk_norm_rope_grad(gq, gk, q, k, wq, wk, freq, interleaved=inter)
+    check_side(zq, dq, dwq, q, gq, wq, freq, p, 1e-6, inter, 1.0, None)
+    check_side(zk, dk, dwk, k, gk, wk, freq, p, 1e-6, inter, 1.0, None)
