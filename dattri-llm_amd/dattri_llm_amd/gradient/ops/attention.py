@@ -124,10 +124,13 @@ def relative_bias(table, q_len: int, k_len: int, *, batch: int | None = None, q_
     it; its gradient then arrives with the samples apart, which a per-sample
     gradient needs.  ``mask`` (batch, k_len) names the live positions of each
     sample: gradients of the others' scores are not counted.  ``slot`` takes the
-    per-sample gradient in place of the summed one (``FusedCapture``)."""
+    per-sample gradient in place of the summed one, a frozen table's too
+    (``FusedCapture``)."""
     if batch is None and (mask is not None or slot is not None):
         raise ValueError("relative_bias: mask and slot need batch, the samples apart")
     cfg = {"q_start": q_start, "bidirectional": bidirectional, "max_distance": max_distance, "causal": causal}
+    if slot is not None and torch.is_grad_enabled() and not table.requires_grad:
+        table = table.detach().requires_grad_()  # a frozen table has no input to carry the gradient to its slot
     if torch.is_grad_enabled() and table.requires_grad:
         return _RelativeBias.apply(table, q_len, k_len, batch, mask, cfg, slot)
     bias = kernels.relative_bias(table, q_len, k_len, **cfg)

@@ -157,3 +157,21 @@ def test_a_projected_session_keeps_these_gradients_whole(device, style):
     scores = ops.layerwise_cross_dot(b, b)
     want = sum((v := b.materialize().data[n].double().flatten(1)) @ v.T for n in b.layer_names)
     assert_parity(scores if torch.is_tensor(scores) else sum(scores.values()), want, "float32", tight=6e-5)
+
+
+def test_a_frozen_block_is_captured_through_its_input(device):
+    torch.manual_seed(4)
+    model = Block().to(device)
+    x = torch.randn(3, 11, WIDTH, device=device)
+    mask = torch.ones(3, 11, dtype=torch.bool, device=device)
+    got = []
+    for frozen in (False, True):
+        model.requires_grad_(not frozen)
+        cap = FusedCapture(model)
+        with cap:
+            sample_losses(model, x.clone().requires_grad_(), x.flip(1), mask).sum().backward()
+        got.append(cap.gradient().materialize())
+    assert set(got[0].layer_names) == set(got[1].layer_names) and "bias" in got[1].layer_names
+    for n in got[0].layer_names:
+        assert_parity(got[1].data[n], got[0].data[n], "float32", label=n)
+    assert all(p.grad is None for p in model.parameters())

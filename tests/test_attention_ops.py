@@ -310,3 +310,26 @@ def test_modules_keep_their_frequencies_in_fp32():
     for bad in (3, 18, -2):
         with pytest.raises(ValueError, match="rotary_dim"):
             QKNormRope(16, rotary_dim=bad)
+
+
+@pytest.fixture
+def plain_bias(monkeypatch):
+    """Stand-ins for the bias kernels on the CPU: a bias that ignores the offsets,
+    and a gradient of ones a sample."""
+    monkeypatch.setattr(kernels, "relative_bias", lambda table, tq, tk, **kw: table[0][:, None, None].expand(-1, tq, tk).clone())
+    monkeypatch.setattr(kernels, "relative_bias_grad", lambda g, n, **kw: torch.ones(g.shape[0], n, g.shape[1]))
+
+
+@pytest.mark.parametrize("frozen", [False, True])
+def test_a_captured_bias_is_captured_with_its_weight_frozen_too(plain_bias, frozen):
+    m = Block()
+    m.bias.weight.requires_grad_(not frozen)
+    cap = FusedCapture(m, ["bias"])
+    with cap:
+        m.bias(4, 5, batch=3).sum().backward()
+        with torch.no_grad():
+            assert not m.bias(4, 5, batch=3).requires_grad
+    got = cap.gradient()
+    assert got.data["bias"].shape == (3, 16) and m.bias.weight.grad is None
+    assert m.bias.weight.requires_grad != frozen
+    assert m.bias(4, 5, batch=3).requires_grad != frozen  # outside the session
