@@ -128,6 +128,10 @@ def relative_bias(table, q_len: int, k_len: int, *, batch: int | None = None, q_
     (``FusedCapture``)."""
     if batch is None and (mask is not None or slot is not None):
         raise ValueError("relative_bias: mask and slot need batch, the samples apart")
+    if mask is not None:  # read by the backward pass alone, checked here
+        kernels.check_bias_mask("relative_bias", mask, batch, q_len, k_len, q_start)
+        if mask.device != table.device:
+            raise ValueError(f"relative_bias: tensors on different devices: {table.device} and {mask.device}")
     cfg = {"q_start": q_start, "bidirectional": bidirectional, "max_distance": max_distance, "causal": causal}
     if slot is not None and torch.is_grad_enabled() and not table.requires_grad:
         table = table.detach().requires_grad_()  # a frozen table has no input to carry the gradient to its slot

@@ -1649,6 +1649,17 @@ def relative_bias(table: torch.Tensor, q_len: int, k_len: int, *, q_start: int =
     return out
 
 
+def check_bias_mask(what: str, mask: torch.Tensor | None, batch: int, q_len: int, k_len: int, q_start: int) -> None:
+    """A (batch, k_len) mask of positions, the queries' from ``q_start`` on among them."""
+    if mask is None:
+        return
+    if mask.shape != (batch, k_len):
+        raise ValueError(f"{what}: mask must have shape ({batch}, {k_len}), got {tuple(mask.shape)}")
+    if not 0 <= q_start <= k_len - q_len:
+        raise ValueError(f"{what}: a mask over {k_len} positions has to hold the queries', {q_start} to "
+                         f"{q_start + q_len - 1}")
+
+
 def relative_bias_grad(g: torch.Tensor, num_buckets: int, *, q_start: int = 0, bidirectional: bool = True,
                        max_distance: int = 128, causal: bool = False, mask=None) -> torch.Tensor:
     """Per-sample table gradient ``(B, num_buckets, H)``, fp32, of the gradient
@@ -1661,10 +1672,8 @@ def relative_bias_grad(g: torch.Tensor, num_buckets: int, *, q_start: int = 0, b
     b, h, tq, tk = g.shape
     edges = _bucket_edges(int(num_buckets), int(max_distance), bool(bidirectional))
     code = nat.dtype_code(g.dtype)
+    check_bias_mask("relative_bias_grad", mask, b, tq, tk, q_start)
     mask, mask_ptr, mask_b, mask_k = _token_mask("relative_bias_grad", mask, b, tk)
-    if mask is not None and not 0 <= q_start <= tk - tq:
-        raise ValueError(f"relative_bias_grad: a mask over {tk} positions has to hold the queries', {q_start} to "
-                         f"{q_start + tq - 1}")
     dev = nat.same_device(g, mask)
     g = _unit_rows(g)
     out = torch.empty((b, num_buckets, h), dtype=torch.float32, device=dev)

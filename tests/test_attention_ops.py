@@ -333,3 +333,17 @@ def test_a_captured_bias_is_captured_with_its_weight_frozen_too(plain_bias, froz
     assert got.data["bias"].shape == (3, 16) and m.bias.weight.grad is None
     assert m.bias.weight.requires_grad != frozen
     assert m.bias(4, 5, batch=3).requires_grad != frozen  # outside the session
+
+
+def test_relative_bias_refuses_a_mask_in_the_forward_call(plain_bias):
+    for table in (torch.zeros(8, 2), torch.zeros(8, 2, requires_grad=True)):
+        for mask, start, words in ((torch.ones(2, 5), 0, "mask must have shape"),
+                                   (torch.ones(3, 4), 0, "mask must have shape"),
+                                   (torch.ones(3, 5), -1, "hold the queries"),
+                                   (torch.ones(3, 5), 2, "hold the queries")):
+            with pytest.raises(ValueError, match=words):
+                ops.relative_bias(table, 4, 5, batch=3, q_start=start, mask=mask)
+        with pytest.raises(ValueError, match="different devices"):
+            ops.relative_bias(table, 4, 5, batch=3, mask=torch.ones(3, 5, device="meta"))
+        for start in (0, 1):
+            assert ops.relative_bias(table, 4, 5, batch=3, q_start=start, mask=torch.ones(3, 5)).shape == (3, 2, 4, 5)
