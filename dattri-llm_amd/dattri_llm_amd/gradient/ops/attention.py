@@ -14,6 +14,7 @@ gives the per-sample gradient itself:
 
 The unsuffixed functions are differentiable; the ``_grad`` functions are the
 same backward passes as plain calls, which can be captured into a HIP graph.
+Second and forward-mode derivatives are refused.
 Both work in the dtypes they are given and hold sums, norms and angles in 32
 bits or more (no compute-dtype policy applies).
 """
@@ -71,6 +72,7 @@ def qk_norm_rope(q, k, q_weight, k_weight, inv_freq, positions=None, *, eps: flo
 
     ``slots``: a ``(q, k)`` pair that takes the weights' per-sample gradients in
     the backward pass, in place of their summed ones (``FusedCapture``)."""
+    kernels.refuse_tangents("qk_norm_rope", q, k, q_weight, k_weight, inv_freq)
     cfg = {"eps": eps, "interleaved": interleaved, "scaling": scaling}
     if torch.is_grad_enabled() and (q.requires_grad or q_weight.requires_grad or (
             k is not None and k_weight is not None and (k.requires_grad or k_weight.requires_grad))):
@@ -126,6 +128,7 @@ def relative_bias(table, q_len: int, k_len: int, *, batch: int | None = None, q_
     sample: gradients of the others' scores are not counted.  ``slot`` takes the
     per-sample gradient in place of the summed one, a frozen table's too
     (``FusedCapture``)."""
+    kernels.refuse_tangents("relative_bias", table)
     if batch is None and (mask is not None or slot is not None):
         raise ValueError("relative_bias: mask and slot need batch, the samples apart")
     if mask is not None:  # read by the backward pass alone, checked here

@@ -17,6 +17,7 @@ import math
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 
 from dattri_llm_amd import _native as nat
 
@@ -1481,6 +1482,16 @@ def _run_on(dev: torch.device, what: str, fn, *args) -> None:
         return
     with torch.cuda.device(dev):
         _run(dev, what, fn, *args)
+
+
+def refuse_tangents(what: str, *tensors) -> None:
+    """Forward-mode operands are refused: a result without a tangent would pass
+    for one whose derivative is zero."""
+    if getattr(forward_ad, "_current_level", 0) < 0:  # outside every level, the rule: 0.1 us
+        return
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f"{what}: forward-mode derivatives are not supported")
 
 
 def _token_mask(what: str, mask: torch.Tensor | None, batch: int, tokens: int):

@@ -347,3 +347,30 @@ def test_relative_bias_refuses_a_mask_in_the_forward_call(plain_bias):
             ops.relative_bias(table, 4, 5, batch=3, mask=torch.ones(3, 5, device="meta"))
         for start in (0, 1):
             assert ops.relative_bias(table, 4, 5, batch=3, q_start=start, mask=torch.ones(3, 5)).shape == (3, 2, 4, 5)
+
+
+def test_forward_mode_derivatives_are_refused():
+    """Refused, not taken for zero: with and without a graph, under functional
+    transforms, for each operand that a tangent can come from."""
+    from torch.autograd import forward_ad
+
+    a, _ = qk_args()
+    floats = ("q", "k", "q_weight", "k_weight", "inv_freq")
+    index = torch.zeros(6, 2, dtype=torch.int64)
+    calls = [(lambda v, n=n: ops.qk_norm_rope(**{**a, n: v}), a[n]) for n in floats]
+    calls += [(lambda v: ops.relative_bias(v, 4, 5), torch.zeros(8, 2)),
+              (lambda v: ops.relative_bias(v, 4, 5, batch=2), torch.zeros(8, 2)),
+              (lambda v: ops.moe.balance_loss(v, index), torch.zeros(6, 4)),
+              (lambda v: ops.moe.balance_loss(v, index.view(2, 3, 2)), torch.zeros(2, 3, 4))]
+    for call, v in calls:
+        for leaf in (v, v.clone().requires_grad_()):
+            with forward_ad.dual_level():
+                dual = forward_ad.make_dual(leaf, torch.ones_like(v))
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    call(dual)
+                with torch.no_grad(), pytest.raises(NotImplementedError, match="forward-mode"):
+                    call(dual)
+                with pytest.raises(nat.NativeLibraryError, match="ROCm GPU"):  # a level without a tangent changes nothing
+                    call(leaf)
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            torch.func.jvp(call, (v,), (torch.ones_like(v),))
