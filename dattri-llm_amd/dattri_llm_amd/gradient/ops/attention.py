@@ -64,15 +64,17 @@ def qk_norm_rope(q, k, q_weight, k_weight, inv_freq, positions=None, *, eps: flo
 
     Pairs are ``(i, i + R/2)``, or ``(2i, 2i+1)`` with ``interleaved``; cosine and
     sine are multiplied by ``scaling``.  ``positions``: int32/int64 ``(T,)`` or
-    ``(B, T)``, by default the token's index; ``inv_freq`` float32.  ``mask`` (B,
-    T): a token with a zero gets zero rows, whatever its input holds, and takes
-    no part in any gradient.  ``k`` may be None.  Inputs of any strides; outputs
-    keep their layout (contiguous where rows overlap in memory).  A single new
-    token is ``T = 1`` with its position.
+    ``(B, T)``, by default the token's index; ``inv_freq`` float32, without a
+    gradient.  ``mask`` (B, T): a token with a zero gets zero rows, whatever its
+    input holds, and takes no part in any gradient.  ``k`` may be None.  Inputs of
+    any strides; outputs keep their layout (contiguous where rows overlap in
+    memory).  A single new token is ``T = 1`` with its position.
 
     ``slots``: a ``(q, k)`` pair that takes the weights' per-sample gradients in
     the backward pass, in place of their summed ones (``FusedCapture``)."""
     kernels.refuse_tangents("qk_norm_rope", q, k, q_weight, k_weight, inv_freq)
+    if inv_freq.requires_grad and torch.is_grad_enabled():
+        raise NotImplementedError("qk_norm_rope: inv_freq takes no gradient; pass it detached")
     cfg = {"eps": eps, "interleaved": interleaved, "scaling": scaling}
     if torch.is_grad_enabled() and (q.requires_grad or q_weight.requires_grad or (
             k is not None and k_weight is not None and (k.requires_grad or k_weight.requires_grad))):

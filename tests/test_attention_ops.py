@@ -370,7 +370,17 @@ def test_forward_mode_derivatives_are_refused():
                     call(dual)
                 with torch.no_grad(), pytest.raises(NotImplementedError, match="forward-mode"):
                     call(dual)
-                with pytest.raises(nat.NativeLibraryError, match="ROCm GPU"):  # a level without a tangent changes nothing
+                with torch.no_grad(), pytest.raises(nat.NativeLibraryError, match="ROCm GPU"):  # no tangent: as ever
                     call(leaf)
         with pytest.raises(NotImplementedError, match="forward-mode"):
             torch.func.jvp(call, (v,), (torch.ones_like(v),))
+
+
+def test_frequencies_that_want_a_gradient_are_refused():
+    """The rotation's frequencies take no gradient: refused, not left out."""
+    a, _ = qk_args(inv_freq=torch.ones(4, requires_grad=True))
+    for q in (a["q"], a["q"].clone().requires_grad_()):
+        with pytest.raises(NotImplementedError, match="inv_freq"):
+            ops.qk_norm_rope(**{**a, "q": q})
+        with torch.no_grad(), pytest.raises(nat.NativeLibraryError, match="ROCm GPU"):
+            ops.qk_norm_rope(**{**a, "q": q})
