@@ -38,9 +38,7 @@ class _QkNormRope(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, gq, gk):
         q, k, q_weight, k_weight, inv_freq, positions, mask = ctx.saved_tensors
-        # None: no gradient reached that output.
-        gq = torch.zeros_like(q) if gq is None else gq
-        gk = torch.zeros_like(k) if gk is None and k is not None else gk
+        # An output that no gradient reached has zeros; gk is None where k is.
         wanted = ctx.slots is not None or ctx.needs_input_grad[2] or ctx.needs_input_grad[3]
         dq, dk, wq, wk = kernels.qk_norm_rope_grad(gq, gk, q, k, q_weight, k_weight, inv_freq, positions, mask=mask,
                                                    weight_grads=wanted, **ctx.cfg)

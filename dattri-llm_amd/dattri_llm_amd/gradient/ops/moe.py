@@ -52,6 +52,7 @@ class _BalanceLoss(torch.autograd.Function):
         loss, z_loss, counts, live = kernels.balance_loss(logits, index, batch=batch, mask=mask)
         ctx.save_for_backward(logits, counts, live, mask)
         ctx.mark_non_differentiable(counts, live)
+        ctx.set_materialize_grads(False)  # an unused loss has None, not zeros
         return loss, z_loss, counts, live
 
     @staticmethod

@@ -384,3 +384,22 @@ def test_frequencies_that_want_a_gradient_are_refused():
             ops.qk_norm_rope(**{**a, "q": q})
         with torch.no_grad(), pytest.raises(nat.NativeLibraryError, match="ROCm GPU"):
             ops.qk_norm_rope(**{**a, "q": q})
+
+
+@pytest.mark.parametrize("used", ["loss", "z_loss", "both"])
+def test_a_loss_without_a_gradient_reaches_the_backward_call_as_none(monkeypatch, used):
+    """Nothing is made for an unused loss or for the counts."""
+    got = []
+
+    def backward(up, up_z, logits, counts, live, *, mask=None):
+        got.append((up, up_z))
+        return torch.zeros_like(logits)
+
+    monkeypatch.setattr(kernels, "balance_loss", lambda x, i, **kw: (
+        torch.zeros(2), torch.zeros(2), torch.zeros(2, 4, dtype=torch.int64), torch.zeros(2, dtype=torch.int64)))
+    monkeypatch.setattr(kernels, "balance_loss_grad", backward)
+    x = torch.zeros(2, 3, 4, requires_grad=True)
+    res = ops.moe.balance_loss(x, torch.zeros(2, 3, 2, dtype=torch.int64))
+    (res.loss.sum() if used == "loss" else res.z_loss.sum() if used == "z_loss" else res.loss.sum() + res.z_loss.sum()).backward()
+    (up, up_z), = got
+    assert (up is None) == (used == "z_loss") and (up_z is None) == (used == "loss") and x.grad.shape == x.shape
