@@ -77,7 +77,7 @@ __device__ __forceinline__ void bucket_range(const Edges& e, int x, int* lo, int
     *hi = next - 1;
   } else {
     *lo = 1 - next;
-    *hi = !e.both && first == 0 ? 0x3fffffff : -first;
+    *hi = !e.both && first == 0 && next > 0 ? 0x3fffffff : -first;  // later offsets: the last bucket from 0 on
   }
 }
 

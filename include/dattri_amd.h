@@ -780,8 +780,8 @@ int da_qk_norm_rope_grad(const da_qk_side* sides, int dtype, int weight_dtype, i
  * with table (buckets, heads) at table_bstride / table_hstride (elements).  With
  * distance r = |o| (bidirectional) or max(-o, 0) of the offset o, the bucket is
  * the last x < side_buckets with edges[x] <= r (host array, edges[0] = 0,
- * ascending), plus side_buckets where bidirectional and o > 0; at most 256 in
- * all.  causal: -inf where o > 0.
+ * ascending; of equal ones the last counts), plus side_buckets where bidirectional
+ * and o > 0; at most 256 in all.  causal: -inf where o > 0.
  *
  * da_relative_bias_grad: the per-sample gradient (batch, buckets, heads), fp32,
  *

@@ -8,9 +8,12 @@ q_len entries, then the offsets of a bucket in steps of at most 512).
 
 from __future__ import annotations
 
+import ctypes
+
 import pytest
 import torch
 
+from dattri_llm_amd import _native as nat
 from dattri_llm_amd.gradient import ops
 from test_attention_ops import bucket
 
@@ -255,3 +258,36 @@ def test_offsets_past_32_bits(device):
     for h, i, j in ((1, 49999, 50000), (1, 49999, 0), (0, 49999, 49990), (1, 0, 50000), (1, 43000, 43002)):
         _, ids = ids_of(1, 1, i - j, 32, 128, True)
         assert out[h, i, j] == table[ids[0, 0], h]
+
+
+@pytest.mark.parametrize("both", [False, True])
+@pytest.mark.parametrize("edges", [(0, 0, 3), (0, 0, 0, 2, 2, 5), (0, 0), (0, 4, 4, 9), (0,)], ids=str)
+def test_c_abi_edges_that_repeat(edges, both, device):
+    """An offset belongs to the last bucket whose edge is at most its distance, to
+    no other: whole numbers, forward and backward, past and future offsets."""
+    h, tq, tk, start = 2, 37, 41, 9
+    n = len(edges)
+    lib, c_edges = nat.load(), (ctypes.c_int32 * n)(*edges)
+    rel = torch.arange(tk)[None] - torch.arange(tq)[:, None] - start
+    r = rel.abs() if both else (-rel).clamp(min=0)
+    ids = (r[..., None] >= torch.tensor(edges)).sum(-1) - 1 + n * (both & (rel > 0))
+    buckets = n * (1 + both)
+    table = torch.arange(buckets * h, dtype=torch.float32, device=device).view(buckets, h)
+    out = torch.empty(h, tq, tk, device=device)
+    stream = torch.cuda.current_stream().cuda_stream
+    nat.check(lib.da_relative_bias(table.data_ptr(), 0, h, 1, h, tq, tk, start, c_edges, n, int(both), 0,
+                                   out.data_ptr(), stream), "forward")
+    assert torch.equal(out.cpu(), table.cpu()[ids].permute(2, 0, 1))
+    g = torch.randint(-8, 9, (3, h, tq, tk), generator=torch.Generator().manual_seed(n)).float()
+    dev_g = g.to(device)
+    for causal in (0, 1):
+        size = ctypes.c_size_t(0)
+        nat.check(lib.da_relative_bias_grad_workspace(0, 3, h, tq, tk, start, buckets, causal, ctypes.byref(size)), "size")
+        ws = torch.empty(max(size.value, 16), dtype=torch.uint8, device=device)
+        got = torch.empty(3, buckets, h, device=device)
+        nat.check(lib.da_relative_bias_grad(dev_g.data_ptr(), 0, 3, h, tq, tk, h * tq * tk, tq * tk, tk, start, c_edges, n,
+                                            int(both), causal, None, 0, 0, got.data_ptr(), ws.data_ptr(), ws.numel(),
+                                            stream), "backward")
+        live = torch.where(rel <= 0, g, 0.0) if causal else g
+        want = live.flatten(2) @ torch.nn.functional.one_hot(ids.flatten(), buckets).float()
+        assert torch.equal(got.cpu(), want.transpose(1, 2)), causal
