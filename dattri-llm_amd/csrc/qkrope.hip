@@ -229,7 +229,8 @@ struct Row {
 
 // Cosine and sine of a token's pairs, one pair a lane: a wave's heads share them
 // through its own part of the LDS (`table`: kL S V pairs).  Pairs past the
-// rotated ones stay as they are.
+// rotated ones get (1, 0) and are not turned by it: 0 times a partner that is not
+// finite is no zero.  (A selection a value: no difference in time.)
 template <int V, int kL, int S>
 __device__ __forceinline__ void angles(const QkArgs& a, int64_t b, int64_t t, float2* table, int lane, int l,
                                        float (&c)[S][V], float (&s)[S][V]) {
@@ -341,8 +342,8 @@ __global__ __launch_bounds__(kThreads) void qk_rope_forward(QkArgs a) {
 #pragma unroll
             for (int e = 0; e < V; ++e) {
               const float ya = x.a[i][e] * rms * wa[i][e], yb = x.b[i][e] * rms * wb[i][e];
-              x.a[i][e] = ya * c[i][e] - yb * s[i][e];
-              x.b[i][e] = yb * c[i][e] + ya * s[i][e];
+              x.a[i][e] = slots[i].turn ? ya * c[i][e] - yb * s[i][e] : ya;
+              x.b[i][e] = slots[i].turn ? yb * c[i][e] + ya * s[i][e] : yb;
             }
           x.store(out_row, slots, in);
           out_row += out_step;
@@ -416,8 +417,8 @@ __global__ __launch_bounds__(kThreads) void qk_rope_backward(QkArgs a, int64_t q
     for (int i = 0; i < S; ++i)
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        const float ya = z.a[i][e] * c[i][e] + z.b[i][e] * s[i][e];
-        const float yb = z.b[i][e] * c[i][e] - z.a[i][e] * s[i][e];
+        const float ya = slots[i].turn ? z.a[i][e] * c[i][e] + z.b[i][e] * s[i][e] : z.a[i][e];
+        const float yb = slots[i].turn ? z.b[i][e] * c[i][e] - z.a[i][e] * s[i][e] : z.b[i][e];
         z.a[i][e] = ya;
         z.b[i][e] = yb;
         sq += x.a[i][e] * x.a[i][e] + x.b[i][e] * x.b[i][e];

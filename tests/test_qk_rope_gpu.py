@@ -382,3 +382,24 @@ def test_rows_that_overlap_in_memory(t, shift, inter, dt, device):
     dq, dk, dwq, dwk = ops.qk_norm_rope_grad(gq, gk, q, k, wq, wk, freq, interleaved=inter)
     check_side(zq, dq, dwq, q, gq, wq, freq, p, 1e-6, inter, 1.0, None)
     check_side(zk, dk, dwk, k, gk, wk, freq, p, 1e-6, inter, 1.0, None)
+
+
+@pytest.mark.parametrize("inter,d,rot", [(False, 128, 64), (True, 128, 64), (False, 7, 4), (True, 23, 8), (False, 80, 32),
+                                         (False, 300, 4)])
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+def test_entries_that_do_not_rotate_stay_apart(bad, inter, d, rot, device):
+    """A weight, or a gradient, that is not finite at one entry past the rotated ones."""
+    at = rot + (d - rot) // 3
+    q, k, gq, gk, wq, wk, freq, p = inputs(2, 9, 3, 2, d, rot, torch.float32, pos="any")
+    clean, _ = ops.qk_norm_rope(q, k, wq, wk, freq, p, interleaved=inter)
+    w = wq.clone()
+    w[at] = bad
+    z, _ = ops.qk_norm_rope(q, k, w, wk, freq, p, interleaved=inter)
+    others = torch.arange(d, device=device) != at
+    assert torch.equal(z[..., others], clean[..., others]) and not bool(torch.isfinite(z[..., at]).any())
+    dw = ops.qk_norm_rope_grad(gq, gk, q, k, wq, wk, freq, p, interleaved=inter)[2]
+    g = gq.clone()
+    g[1, 4, 1, at] = bad
+    got = ops.qk_norm_rope_grad(g, gk, q, k, wq, wk, freq, p, interleaved=inter)[2]
+    assert torch.equal(got[:, others], dw[:, others]) and torch.equal(got[0], dw[0])
+    assert not bool(torch.isfinite(got[1, at]))
