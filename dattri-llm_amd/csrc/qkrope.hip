@@ -330,21 +330,22 @@ __global__ __launch_bounds__(kThreads) void qk_rope_forward(QkArgs a) {
           head += kHeads * a.parts;
           x_row += x_step;
           if (g + a.parts < end) raw.template load<kStream>(x_row, slots, head < heads && live);
-          float sq = 0.f;
+          if (live) {  // a dead token's rows hold zeros, and stay so whatever weights and angles are
+            float sq = 0.f;
 #pragma unroll
-          for (int i = 0; i < S; ++i)
+            for (int i = 0; i < S; ++i)
 #pragma unroll
-            for (int e = 0; e < V; ++e) sq += x.a[i][e] * x.a[i][e] + x.b[i][e] * x.b[i][e];
-          // A dead token's rows are zero, and stay zero without an eps.
-          const float rms = live ? rsqrtf(lanes_sum<kL>(sq) * inv_d + a.eps) : 0.f;
+              for (int e = 0; e < V; ++e) sq += x.a[i][e] * x.a[i][e] + x.b[i][e] * x.b[i][e];
+            const float rms = rsqrtf(lanes_sum<kL>(sq) * inv_d + a.eps);
 #pragma unroll
-          for (int i = 0; i < S; ++i)
+            for (int i = 0; i < S; ++i)
 #pragma unroll
-            for (int e = 0; e < V; ++e) {
-              const float ya = x.a[i][e] * rms * wa[i][e], yb = x.b[i][e] * rms * wb[i][e];
-              x.a[i][e] = slots[i].turn ? ya * c[i][e] - yb * s[i][e] : ya;
-              x.b[i][e] = slots[i].turn ? yb * c[i][e] + ya * s[i][e] : yb;
-            }
+              for (int e = 0; e < V; ++e) {
+                const float ya = x.a[i][e] * rms * wa[i][e], yb = x.b[i][e] * rms * wb[i][e];
+                x.a[i][e] = slots[i].turn ? ya * c[i][e] - yb * s[i][e] : ya;
+                x.b[i][e] = slots[i].turn ? yb * c[i][e] + ya * s[i][e] : yb;
+              }
+          }
           x.store(out_row, slots, in);
           out_row += out_step;
         }
@@ -412,30 +413,32 @@ __global__ __launch_bounds__(kThreads) void qk_rope_backward(QkArgs a, int64_t q
     if (t < t1) load();
     asm volatile("" ::: "memory");  // the weights stay in LDS: registers bound the waves of a SIMD
     lane_weights<V, kL, S>(w, l, wa, wb);
-    float sq = 0.f, along = 0.f;
+    if (lives) {  // as in the forward pass: nothing into dw, dx as loaded, zero
+      float sq = 0.f, along = 0.f;
 #pragma unroll
-    for (int i = 0; i < S; ++i)
+      for (int i = 0; i < S; ++i)
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const float ya = slots[i].turn ? z.a[i][e] * c[i][e] + z.b[i][e] * s[i][e] : z.a[i][e];
-        const float yb = slots[i].turn ? z.b[i][e] * c[i][e] - z.a[i][e] * s[i][e] : z.b[i][e];
-        z.a[i][e] = ya;
-        z.b[i][e] = yb;
-        sq += x.a[i][e] * x.a[i][e] + x.b[i][e] * x.b[i][e];
-        along += ya * wa[i][e] * x.a[i][e] + yb * wb[i][e] * x.b[i][e];
-      }
-    // Rows that are not there, or a dead token's, are zero, and stay zero without an eps.
-    const float rms = in && lives ? rsqrtf(lanes_sum<kL>(sq) * inv_d + a.eps) : 0.f;
-    const float back = lanes_sum<kL>(along) * inv_d * rms * rms;
+        for (int e = 0; e < V; ++e) {
+          const float ya = slots[i].turn ? z.a[i][e] * c[i][e] + z.b[i][e] * s[i][e] : z.a[i][e];
+          const float yb = slots[i].turn ? z.b[i][e] * c[i][e] - z.a[i][e] * s[i][e] : z.b[i][e];
+          z.a[i][e] = ya;
+          z.b[i][e] = yb;
+          sq += x.a[i][e] * x.a[i][e] + x.b[i][e] * x.b[i][e];
+          along += ya * wa[i][e] * x.a[i][e] + yb * wb[i][e] * x.b[i][e];
+        }
+      // Rows that are not there are zero, and stay zero without an eps.
+      const float rms = in ? rsqrtf(lanes_sum<kL>(sq) * inv_d + a.eps) : 0.f;
+      const float back = lanes_sum<kL>(along) * inv_d * rms * rms;
 #pragma unroll
-    for (int i = 0; i < S; ++i)
+      for (int i = 0; i < S; ++i)
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        da_[i][e] += z.a[i][e] * (x.a[i][e] * rms);
-        db_[i][e] += z.b[i][e] * (x.b[i][e] * rms);
-        z.a[i][e] = rms * (z.a[i][e] * wa[i][e] - x.a[i][e] * back);
-        z.b[i][e] = rms * (z.b[i][e] * wb[i][e] - x.b[i][e] * back);
-      }
+        for (int e = 0; e < V; ++e) {
+          da_[i][e] += z.a[i][e] * (x.a[i][e] * rms);
+          db_[i][e] += z.b[i][e] * (x.b[i][e] * rms);
+          z.a[i][e] = rms * (z.a[i][e] * wa[i][e] - x.a[i][e] * back);
+          z.b[i][e] = rms * (z.b[i][e] * wb[i][e] - x.b[i][e] * back);
+        }
+    }
     z.store(out, slots, in);
   }
   if (!r.partial) return;

@@ -403,3 +403,22 @@ def test_entries_that_do_not_rotate_stay_apart(bad, inter, d, rot, device):
     got = ops.qk_norm_rope_grad(g, gk, q, k, wq, wk, freq, p, interleaved=inter)[2]
     assert torch.equal(got[:, others], dw[:, others]) and torch.equal(got[0], dw[0])
     assert not bool(torch.isfinite(got[1, at]))
+
+
+@pytest.mark.parametrize("inter,d,rot", [(False, 128, 128), (True, 80, 32), (False, 7, 4)])
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+def test_masked_rows_are_zero_whatever_the_weights_hold(bad, inter, d, rot, device):
+    """Weights and frequencies that are not finite reach the live rows alone."""
+    q, k, gq, gk, wq, wk, freq, p = inputs(2, 9, 3, 2, d, rot, torch.float32, pos="any")
+    mask = torch.ones(2, 9, dtype=torch.bool, device=device)
+    mask[0, 3:7] = mask[1] = False
+    for at in ("weight", "frequency"):
+        w, f = wq.clone(), freq.clone()
+        if at == "weight":
+            w[0] = bad
+        else:
+            f[0] = bad
+        z, _ = ops.qk_norm_rope(q, k, w, wk, f, p, interleaved=inter, mask=mask)
+        dq, _, dw, _ = ops.qk_norm_rope_grad(gq, gk, q, k, w, wk, f, p, interleaved=inter, mask=mask)
+        assert not z[~mask].any() and not dq[~mask].any() and not dw[1].any()
+        assert not bool(torch.isfinite(z[mask]).all()) and not bool(torch.isfinite(dq[mask]).all())
