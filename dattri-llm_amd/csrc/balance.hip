@@ -450,7 +450,8 @@ int da_balance_loss(const void* logits, int dtype, int64_t batch, int64_t tokens
   const size_t need = partial_bytes(a);
   if (need && (!workspace || workspace_bytes < need))
     return set_error(DA_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", what, workspace_bytes, need);
-  if (batch * a.chunks > 0x7fffffff || a.chunk * top > 0x7fffffff)
+  // The choices' 32-bit index runs up to four strides past the last of them.
+  if (batch * a.chunks > 0x7fffffff || a.chunk * top > 0x7fffffff - 4 * kThreads)
     return set_error(DA_ERR_UNSUPPORTED, "%s: too many tokens", what);
   const int64_t parts = batch * a.chunks;
   a.p = (float*)workspace;

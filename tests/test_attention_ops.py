@@ -403,3 +403,15 @@ def test_a_loss_without_a_gradient_reaches_the_backward_call_as_none(monkeypatch
     (res.loss.sum() if used == "loss" else res.z_loss.sum() if used == "z_loss" else res.loss.sum() + res.z_loss.sum()).backward()
     (up, up_z), = got
     assert (up is None) == (used == "z_loss") and (up_z is None) == (used == "loss") and x.grad.shape == x.shape
+
+
+def test_c_abi_balance_loss_refuses_choices_past_32_bits():
+    """A workgroup's choices are counted in 32 bits, four strides of its threads
+    ahead of the last one."""
+    lib = nat.load()
+
+    def fwd(t, top):
+        return lib.da_balance_loss(X, 0, 1, t, 4, 4, X, top, None, 0, 0, OUT, OUT, OUT, OUT, X, 1 << 40, None)
+
+    for t, top in ((1, 0x7fffffff), (1, 0x7fffffff - 1023), (2, 0x3fffffff), (64, 33554430)):
+        refused(fwd(t, top), nat.DA_ERR_UNSUPPORTED, "too many")
