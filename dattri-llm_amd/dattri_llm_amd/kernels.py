@@ -1641,6 +1641,13 @@ def _bucket_edges(num_buckets: int, max_distance: int, bidirectional: bool):
     return (ctypes.c_int32 * n)(*edges)
 
 
+def _bias_start(what: str, q_start: int) -> int:
+    """The C ABI's range, checked before ctypes cuts a wider integer."""
+    if not -(1 << 26) <= q_start <= 1 << 26:
+        raise NotImplementedError(f"{what}: q_start up to 2^26 either way, got {q_start}")
+    return int(q_start)
+
+
 def relative_bias(table: torch.Tensor, q_len: int, k_len: int, *, q_start: int = 0, bidirectional: bool = True,
                   max_distance: int = 128, causal: bool = False) -> torch.Tensor:
     """``(H, q_len, k_len)`` attention bias from a ``(num_buckets, H)`` table in
@@ -1650,12 +1657,13 @@ def relative_bias(table: torch.Tensor, q_len: int, k_len: int, *, q_start: int =
     if q_len < 0 or k_len < 0:
         raise ValueError("relative_bias: negative length")
     edges = _bucket_edges(int(table.shape[0]), int(max_distance), bool(bidirectional))
+    q_start = _bias_start("relative_bias", q_start)
     code = nat.dtype_code(table.dtype)
     dev = nat.same_device(table)
     heads = table.shape[1]
     out = torch.empty((heads, q_len, k_len), dtype=table.dtype, device=dev)
     _run_on(dev, "relative_bias", nat.load().da_relative_bias,
-            table.data_ptr(), code, *table.stride(), heads, q_len, k_len, int(q_start), edges, len(edges),
+            table.data_ptr(), code, *table.stride(), heads, q_len, k_len, q_start, edges, len(edges),
             int(bidirectional), int(causal), out.data_ptr(), nat.stream_ptr(dev))
     return out
 
@@ -1682,6 +1690,7 @@ def relative_bias_grad(g: torch.Tensor, num_buckets: int, *, q_start: int = 0, b
         raise ValueError("relative_bias_grad expects a (B, heads, q_len, k_len) gradient")
     b, h, tq, tk = g.shape
     edges = _bucket_edges(int(num_buckets), int(max_distance), bool(bidirectional))
+    q_start = _bias_start("relative_bias_grad", q_start)
     code = nat.dtype_code(g.dtype)
     check_bias_mask("relative_bias_grad", mask, b, tq, tk, q_start)
     mask, mask_ptr, mask_b, mask_k = _token_mask("relative_bias_grad", mask, b, tk)
@@ -1690,15 +1699,21 @@ def relative_bias_grad(g: torch.Tensor, num_buckets: int, *, q_start: int = 0, b
     out = torch.empty((b, num_buckets, h), dtype=torch.float32, device=dev)
     lib = nat.load()
     nbytes = ctypes.c_size_t(0)
-    nat.check(lib.da_relative_bias_grad_workspace(code, b, h, tq, tk, int(q_start), num_buckets, int(causal),
+    nat.check(lib.da_relative_bias_grad_workspace(code, b, h, tq, tk, q_start, num_buckets, int(causal),
                                                   ctypes.byref(nbytes)), "relative_bias_grad")
     ws = nat.workspace(nbytes.value, dev)
     sb, sh, si, _ = g.stride()
     _run_on(dev, "relative_bias_grad", lib.da_relative_bias_grad,
-            g.data_ptr(), code, b, h, tq, tk, sb, sh, si, int(q_start), edges, len(edges),
+            g.data_ptr(), code, b, h, tq, tk, sb, sh, si, q_start, edges, len(edges),
             int(bidirectional), int(causal), mask_ptr, mask_b, mask_k, out.data_ptr(), ws.data_ptr(),
             ws.numel(), nat.stream_ptr(dev))
     return out
+
+
+def _fits_32_bits(what: str, *sizes: int) -> None:
+    """Sizes that the C ABI takes as 32-bit integers (ctypes would cut them)."""
+    if max(sizes) > 0x7FFFFFFF:
+        raise NotImplementedError(f"{what}: {max(sizes)} experts or choices do not fit 32 bits")
 
 
 def balance_loss(logits: torch.Tensor, index: torch.Tensor, *, batch: int = 1, mask=None):
@@ -1710,6 +1725,7 @@ def balance_loss(logits: torch.Tensor, index: torch.Tensor, *, batch: int = 1, m
     if index.dtype != torch.int64:
         raise ValueError("balance_loss: expert indices must be int64")
     n, e = logits.shape
+    _fits_32_bits("balance_loss", e, index.shape[1])
     if batch < 1 or n % batch:
         raise ValueError(f"balance_loss: {n} tokens are not {batch} samples of one length")
     code = nat.dtype_code(logits.dtype)
@@ -1748,6 +1764,7 @@ def balance_loss_grad(up, up_z, logits: torch.Tensor, counts: torch.Tensor, live
     if logits.dim() != 2 or counts.dim() != 2 or counts.shape[1] != logits.shape[1]:
         raise ValueError("balance_loss_grad expects (N, E) logits and (B, E) counts")
     n, e = logits.shape
+    _fits_32_bits("balance_loss_grad", e)
     batch = counts.shape[0]
     if batch < 1 or n % batch or live.shape != (batch,):
         raise ValueError(f"balance_loss_grad: {n} tokens are not {batch} samples of one length")

@@ -415,3 +415,20 @@ def test_c_abi_balance_loss_refuses_choices_past_32_bits():
 
     for t, top in ((1, 0x7fffffff), (1, 0x7fffffff - 1023), (2, 0x3fffffff), (64, 33554430)):
         refused(fwd(t, top), nat.DA_ERR_UNSUPPORTED, "too many")
+
+
+def test_sizes_past_the_c_types_are_refused():
+    """Not cut to their low 32 or 64 bits: the tensors here are one entry, expanded."""
+    x, index = torch.zeros(1, 4), torch.zeros(1, 2, dtype=torch.int64)
+    wide, many = torch.zeros(1).expand(1, (1 << 32) + 4), torch.zeros(1, dtype=torch.int64).expand(1, (1 << 32) + 2)
+    counts = torch.zeros(1, dtype=torch.int64).expand(1, (1 << 32) + 4)
+    for bad in (lambda: ops.moe.balance_loss(wide, index), lambda: ops.moe.balance_loss(x, many),
+                lambda: ops.moe.balance_loss_grad(None, None, wide, counts, torch.zeros(1, dtype=torch.int64))):
+        with pytest.raises(NotImplementedError, match="32 bits"):
+            bad()
+    table, g = torch.zeros(8, 2), torch.zeros(2, 4, 5, 9)
+    for start in (1 << 64, -(1 << 64), (1 << 26) + 1):
+        for bad in (lambda: ops.relative_bias(table, 4, 4, q_start=start),
+                    lambda: ops.relative_bias_grad(g, 8, q_start=start)):
+            with pytest.raises(NotImplementedError, match="q_start"):
+                bad()
