@@ -451,7 +451,7 @@ int da_balance_loss(const void* logits, int dtype, int64_t batch, int64_t tokens
   if (need && (!workspace || workspace_bytes < need))
     return set_error(DA_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", what, workspace_bytes, need);
   // The choices' 32-bit index runs up to four strides past the last of them.
-  if (batch * a.chunks > 0x7fffffff || a.chunk * top > 0x7fffffff - 4 * kThreads)
+  if (batch * a.chunks > kMaxBlocks || a.chunk * top > 0x7fffffff - 4 * kThreads)
     return set_error(DA_ERR_UNSUPPORTED, "%s: too many tokens", what);
   const int64_t parts = batch * a.chunks;
   a.p = (float*)workspace;
@@ -482,7 +482,7 @@ int da_balance_loss_grad(const float* up, const float* up_z, const void* logits,
   const bool aligned = ((uintptr_t)logits | (uintptr_t)grad) % 16 == 0 && (row_stride | grad_row_stride) * es % 16 == 0;
   const Shape shape = shape_of(dtype, experts, aligned);
   chunking(a, shape, kBackwardSteps, kBackwardBlocks);
-  if (batch * a.chunks > 0x7fffffff) return set_error(DA_ERR_UNSUPPORTED, "%s: too many tokens", what);
+  if (batch * a.chunks > kMaxBlocks) return set_error(DA_ERR_UNSUPPORTED, "%s: too many tokens", what);
   Launch{a, true, (hipStream_t)stream}(dtype, shape);
   return check_launch(what);
 }

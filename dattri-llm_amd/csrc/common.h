@@ -217,6 +217,9 @@ __device__ __forceinline__ float lanes_max(float v) {
 // ---------------------------------------------------------------------------
 // Grid helpers.
 // ---------------------------------------------------------------------------
+// Workgroups of 256 threads of a grid's axis: HIP counts its threads in 32 bits.
+constexpr int64_t kMaxBlocks = 0xffffffffLL / 256;
+
 // The dispatcher places workgroup w on XCD (w % 8).  Remap so each XCD owns a
 // contiguous range of logical tile ids (so neighbouring tiles, which share
 // operand rows, hit the same L2).  Bijective for any n.

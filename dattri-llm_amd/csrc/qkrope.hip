@@ -702,8 +702,8 @@ int da_qk_norm_rope_grad(const da_qk_side* sides, int dtype, int weight_dtype, i
   const int64_t pairs = rot / 2 + (d - rot + 1) / 2;
   const int v = run_entries(a, es, true);
   const int64_t q_blocks = batch * a.side[0].chunks, blocks = q_blocks + batch * a.side[1].chunks;
-  if (blocks > 0x7fffffff || batch > 65535 || sides[0].heads > 65535 || sides[1].heads > 65535)
-    return set_error(DA_ERR_UNSUPPORTED, "da_qk_norm_rope_grad: up to 2^31 tokens, 65535 samples and heads");
+  if (blocks > kMaxBlocks || batch > 65535 || sides[0].heads > 65535 || sides[1].heads > 65535)
+    return set_error(DA_ERR_UNSUPPORTED, "da_qk_norm_rope_grad: too many tokens; up to 65535 samples and heads");
   if (blocks) {
     Launch{a, true, blocks, q_blocks, st, es}(dtype, interleaved, v, pairs);
     if (int rc = check_launch("da_qk_norm_rope_grad")) return rc;

@@ -432,3 +432,19 @@ def test_sizes_past_the_c_types_are_refused():
                     lambda: ops.relative_bias_grad(g, 8, q_start=start)):
             with pytest.raises(NotImplementedError, match="q_start"):
                 bad()
+
+
+def test_c_abi_refuses_launches_past_32_bits_of_threads():
+    """A grid's threads, 256 a workgroup, are counted in 32 bits by the launch."""
+    lib = nat.load()
+    b = 1 << 24
+    refused(lib.da_balance_loss(X, 0, b, 1, 4, 4, X, 2, None, 0, 0, OUT, OUT, OUT, OUT, X, 1 << 40, None),
+            nat.DA_ERR_UNSUPPORTED, "too many")
+    refused(lib.da_balance_loss_grad(X, X, X, 0, b, 1, 4, 4, X, X, None, 0, 0, OUT, 4, None), nat.DA_ERR_UNSUPPORTED,
+            "too many")
+    sides = (nat.QkSide * 2)()
+    for side in sides:
+        side.x = side.gz = side.out = side.weight = side.weight_grad = X
+        side.heads = 1024
+    refused(lib.da_qk_norm_rope_grad(sides, 2, 0, 8, 1 << 20, 8, 8, X, None, 0, 0, 1, None, 0, 0, 0, 1.0, 1e-6, X, 1 << 40,
+                                     None), nat.DA_ERR_UNSUPPORTED, "up to")
