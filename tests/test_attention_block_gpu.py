@@ -11,6 +11,7 @@ from torch import nn
 
 from conftest import assert_parity
 from dattri_llm_amd.gradient import FusedCapture, QKNormRope, RelativeBias, ops
+from test_relative_bias_gpu import ids_of
 
 pytestmark = pytest.mark.gpu
 WIDTH, HEADS, KEYS, D, EXPERTS, TOP = 64, 4, 2, 16, 6, 2
@@ -175,3 +176,32 @@ def test_a_frozen_block_is_captured_through_its_input(device):
     for n in got[0].layer_names:
         assert_parity(got[1].data[n], got[0].data[n], "float32", label=n)
     assert all(p.grad is None for p in model.parameters())
+
+
+@pytest.mark.parametrize("autocast", [False, True])
+def test_captured_in_bf16(device, autocast):
+    """Rotated norms and the bias in a bf16 model, and in an fp32 one under autocast.
+    Whole numbers: rows and gradients of -1 and 1 at angle 0 and without an eps, so
+    that the sums are exact but for the root of 1 (a step of 2^-23 of sums below
+    160), and score gradients from -8 to 8, whose sums are exact."""
+    torch.manual_seed(5)
+    b, t, buckets = 3, 40, 8
+    dt = torch.float32 if autocast else torch.bfloat16
+    rope = QKNormRope(D, eps=0.0).to(device, dt)
+    bias = RelativeBias(buckets, HEADS, max_distance=20).to(device, dt)
+    q, k, gq, gk = (torch.randint(0, 2, (b, t, h, D), device=device).mul_(2).sub_(1).bfloat16()
+                    for h in (HEADS, KEYS, HEADS, KEYS))
+    gs = torch.randint(-8, 9, (b, HEADS, t, t), device=device).to(dt)
+    cap = FusedCapture(nn.ModuleDict({"rope": rope, "bias": bias}))
+    with cap, torch.autocast("cuda", torch.bfloat16, enabled=autocast):
+        zq, zk = rope(q, k, torch.zeros(t, dtype=torch.int64, device=device))
+        s = bias(t, t, batch=b)
+        assert zq.dtype == zk.dtype == torch.bfloat16 and s.dtype == dt
+        torch.autograd.backward([zq, zk, s], [gq, gk, gs])
+    got = cap.gradient().data
+    for name, x, g in (("rope.q_weight", q, gq), ("rope.k_weight", k, gk)):
+        want = (x.float() * g.float()).sum((1, 2))
+        assert got[name].dtype == torch.float32 and bool(((got[name] - want).abs() < 0.01).all())
+    _, ids = ids_of(t, t, 0, buckets, 20, True)
+    pick = nn.functional.one_hot(ids.flatten(), buckets).float().to(device)
+    assert torch.equal(got["bias"].view(b, buckets, HEADS), (gs.float().flatten(2) @ pick).transpose(1, 2))

@@ -422,3 +422,86 @@ def test_masked_rows_are_zero_whatever_the_weights_hold(bad, inter, d, rot, devi
         dq, _, dw, _ = ops.qk_norm_rope_grad(gq, gk, q, k, w, wk, f, p, interleaved=inter, mask=mask)
         assert not z[~mask].any() and not dq[~mask].any() and not dw[1].any()
         assert not bool(torch.isfinite(z[mask]).all()) and not bool(torch.isfinite(dq[mask]).all())
+
+
+def dw_roundings(b, t, heads):
+    """Roundings behind an entry of a weight gradient, at most: its term (12), a
+    wave's quarter of the chunk's rows, the lanes (6), the waves (4), the chunks that
+    one of eight threads adds, the eight."""
+    chunk = max(1, min(1024 // heads, b * t // 512))
+    chunks = -(-t // chunk)
+    return 12 + chunk * heads // 4 + 1 + 6 + 4 + -(-chunks // 8) + 8
+
+
+STREAMED = [
+    # dt, b, t, hq, hk, d, rot, interleaved, layout: lanes of a head 8, 4, 16, 16, 32, 64 (two runs each), 64
+    (torch.bfloat16, 4, 5251, 20, 5, 128, 128, False, "fused"),
+    (torch.bfloat16, 13, 4051, 16, 4, 64, 64, True, "heads"),
+    (torch.float32, 5, 3511, 18, 6, 80, 32, True, "heads"),
+    (torch.float16, 7, 2689, 11, 3, 256, 128, False, "plain"),
+    (torch.bfloat16, 3, 8741, 4, 1, 512, 512, True, "fused"),
+    (torch.float32, 2, 3299, 4, 1, 1024, 1024, False, "heads"),
+    (torch.float16, 1, 13127, 4, 1, 1024, 512, True, "plain"),
+]
+
+
+@pytest.mark.parametrize("case", STREAMED, ids=lambda c: f"{NAME[c[0]]}-{c[5]}-{c[6]}-{c[7]}-{c[8]}")
+def test_rows_of_128_mib_and_more(case, device):
+    """Read past the caches, by instances of their own: every row against fp64 (on
+    the GPU, elementwise), padded sequences, NaN in the padding."""
+    dt, b, t, hq, hk, d, rot, inter, how = case
+    assert b * t * (hq + hk) * d * dt.itemsize >= 128 << 20
+    gen = torch.Generator(device=device).manual_seed(d)
+    mask = torch.arange(t, device=device)[None] < t - torch.randint(0, t // 4, (b, 1), generator=gen, device=device)
+    freq = torch.tensor([10000.0 ** (-i / rot) for i in range(0, rot, 2)], device=device)
+    p = torch.arange(t, device=device) + torch.randint(0, 100_000, (b, 1), generator=gen, device=device)
+    x, g, w = [], [], []
+    for h in (hq, hk):
+        for side in (x, g):
+            v = torch.randn(b, t, h, d, generator=gen, device=device, dtype=dt)
+            v[~mask] = float("nan")
+            side.append(layout(v, how))
+        w.append((1 + 0.2 * torch.randn(d, generator=gen, device=device)).to(dt))
+    z = ops.qk_norm_rope(*x, *w, freq, p, interleaved=inter, mask=mask)
+    got = ops.qk_norm_rope_grad(*g, *x, *w, freq, p, interleaved=inter, mask=mask)
+    half = HALF_ULP.get(NAME[dt], 0.0)
+    least = 2.0 ** -25 if dt == torch.float16 else 0.0  # half a step below fp16's least normal value
+    for i, h in enumerate((hq, hk)):
+        xd = torch.where(mask[:, :, None, None], x[i].double(), 0.0).requires_grad_()
+        wd = w[i].double().expand(b, -1).clone().requires_grad_()
+        want = plain(xd, wd[:, None, None, :], freq, p, 1e-6, inter, 1.0, mask)
+        live = torch.where(mask[:, :, None, None], g[i].double(), 0.0)
+        want.backward(live)
+        want, dx, dw = want.detach(), xd.grad, wd.grad
+        off = (z[i].double() - want).abs()
+        assert bool((off <= TIGHT_FP32 * want.abs().amax(-1, keepdim=True) + half * want.abs() + least).all())
+        rms = (xd.detach().square().mean(-1, keepdim=True) + 1e-6).rsqrt()
+        size = rms * live.abs().amax(-1, keepdim=True) * w[i].double().abs().max() + dx.abs()
+        off = (got[i].double() - dx).abs()
+        assert bool((off <= 4 * TIGHT_FP32 * size + half * dx.abs() + least).all())
+        assert not z[i][~mask].any() and not got[i][~mask].any()
+        terms = plain_back_abs(live, freq, p, inter, 1.0) * (xd.detach() * rms).abs()
+        bound = dw_roundings(b, t, h) * 2.0 ** -24 * terms.sum((1, 2))
+        assert bool(((got[2 + i].double() - dw).abs() <= bound).all())
+        del want, off, dx, live, terms, xd
+
+
+@pytest.mark.parametrize("b,t,hq,hk", [(1, 20000, 2, 1), (3000, 2, 2, 1), (3, 4001, 5, 1), (700, 7, 3, 3), (2, 1, 64, 8)])
+@pytest.mark.parametrize("dt", DTYPES, ids=NAME.get)
+def test_no_row_is_lost_from_the_weight_gradients(dt, b, t, hq, hk, device):
+    """Rows and gradients of -1 and 1 at angle 0: a weight gradient is a whole number
+    that each of its rows changes by 1, and rounding leaves it by less than a half."""
+    d = 16
+    gen = torch.Generator().manual_seed(t)
+    q, k, gq, gk = (torch.randint(0, 2, (b, t, h, d), generator=gen).mul_(2).sub_(1).to(dt) for h in (hq, hk, hq, hk))
+    w, freq, p = torch.ones(d, dtype=dt), torch.ones(d // 2), torch.zeros(t, dtype=torch.int64)
+    got = ops.qk_norm_rope_grad(*(v.to(device) for v in (gq, gk, q, k, w, w, freq, p)), eps=0.0)
+    for x, g, dx, dw in ((q, gq, got[0], got[2]), (k, gk, got[1], got[3])):
+        heads = x.shape[2]
+        assert dw_roundings(b, t, heads) * 2.0 ** -24 * t * heads < 0.5
+        x, g = x.double(), g.double()
+        assert torch.equal(dw.cpu().double().round(), (x * g).sum((1, 2)))
+        want = g - x * (g * x).mean(-1, keepdim=True)
+        # a root of 1 off by a step, three products of sums that are exact
+        off = (dx.cpu().double() - want).abs()
+        assert bool((off <= 12 * 2.0 ** -24 * 2 + HALF_ULP.get(NAME[dt], 0.0) * want.abs()).all())
