@@ -22,6 +22,7 @@ bits or more (no compute-dtype policy applies).
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from dattri_llm_amd import kernels
@@ -70,7 +71,8 @@ def qk_norm_rope(q, k, q_weight, k_weight, inv_freq, positions=None, *, eps: flo
 
     ``slots``: a ``(q, k)`` pair that takes the weights' per-sample gradients in
     the backward pass, in place of their summed ones (``FusedCapture``)."""
-    kernels.refuse_tangents("qk_norm_rope", q, k, q_weight, k_weight, inv_freq)
+    if getattr(forward_ad, "_current_level", 0) >= 0:
+        kernels.refuse_tangents("qk_norm_rope", q, k, q_weight, k_weight, inv_freq)
     if inv_freq.requires_grad and torch.is_grad_enabled():
         raise NotImplementedError("qk_norm_rope: inv_freq takes no gradient; pass it detached")
     cfg = {"eps": eps, "interleaved": interleaved, "scaling": scaling}
@@ -128,7 +130,8 @@ def relative_bias(table, q_len: int, k_len: int, *, batch: int | None = None, q_
     sample: gradients of the others' scores are not counted.  ``slot`` takes the
     per-sample gradient in place of the summed one, a frozen table's too
     (``FusedCapture``)."""
-    kernels.refuse_tangents("relative_bias", table)
+    if getattr(forward_ad, "_current_level", 0) >= 0:
+        kernels.refuse_tangents("relative_bias", table)
     if batch is None and (mask is not None or slot is not None):
         raise ValueError("relative_bias: mask and slot need batch, the samples apart")
     if mask is not None:  # read by the backward pass alone, checked here

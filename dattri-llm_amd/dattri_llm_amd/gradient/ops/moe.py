@@ -22,6 +22,7 @@ from __future__ import annotations
 from typing import NamedTuple
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from dattri_llm_amd import kernels
@@ -78,7 +79,8 @@ def balance_loss(logits: torch.Tensor, top_idx: torch.Tensor, *, batch: int | No
     so that an even load gives ``loss = k``.  Masked tokens take no part,
     whatever their logits hold; a sample without live tokens has zeros.  An
     index outside the experts (a dropped choice) counts for none."""
-    kernels.refuse_tangents("balance_loss", logits)
+    if getattr(forward_ad, "_current_level", 0) >= 0:
+        kernels.refuse_tangents("balance_loss", logits)
     if logits.dim() not in (2, 3) or top_idx.dim() not in (2, 3):
         raise ValueError("balance_loss expects (B, T, E) or (N, E) logits and expert indices alike")
     if logits.dim() == 3:

@@ -1486,9 +1486,9 @@ def _run_on(dev: torch.device, what: str, fn, *args) -> None:
 
 def refuse_tangents(what: str, *tensors) -> None:
     """Forward-mode operands are refused: a result without a tangent would pass
-    for one whose derivative is zero."""
-    if getattr(forward_ad, "_current_level", 0) < 0:  # outside every level, the rule: 0.1 us
-        return
+    for one whose derivative is zero.  Called inside a dual level alone
+    (``forward_ad._current_level``, -1 outside): calls elsewhere are bound by such
+    host steps."""
     for t in tensors:
         if t is not None and forward_ad.unpack_dual(t).tangent is not None:
             raise NotImplementedError(f"{what}: forward-mode derivatives are not supported")
@@ -1519,10 +1519,11 @@ def _qk_side(what: str, x, w, gz, wgrad):
         raise ValueError(f"{what}: a norm weight must have shape ({x.shape[3]},)")
     x, w = _unit_rows(x), w.contiguous()
     out = torch.empty_like(x)
-    if out.stride(3) != 1:  # the kernels write whole rows; rows that overlap may give another order of the axes
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     xb, xt, xh, _ = x.stride()
-    ob, ot, oh, _ = out.stride()
+    ob, ot, oh, oe = out.stride()
+    if oe != 1:  # the kernels write whole rows; rows that overlap may give another order of the axes
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        ob, ot, oh, _ = out.stride()
     if gz is None:
         return (x.data_ptr(), 0, out.data_ptr(), w.data_ptr(), 0, x.shape[2], xb, xt, xh, 0, 0, 0, ob, ot, oh), out, x, w
     gz = _unit_rows(gz)
@@ -1641,11 +1642,11 @@ def _bucket_edges(num_buckets: int, max_distance: int, bidirectional: bool):
     return (ctypes.c_int32 * n)(*edges)
 
 
-def _bias_start(what: str, q_start: int) -> int:
-    """The C ABI's range, checked before ctypes cuts a wider integer."""
-    if not -(1 << 26) <= q_start <= 1 << 26:
-        raise NotImplementedError(f"{what}: q_start up to 2^26 either way, got {q_start}")
-    return int(q_start)
+_MOST_START = 1 << 26  # the C ABI's range, checked before ctypes cuts a wider integer
+
+
+def _too_far(what: str, q_start: int) -> None:
+    raise NotImplementedError(f"{what}: q_start up to 2^26 either way, got {q_start}")
 
 
 def relative_bias(table: torch.Tensor, q_len: int, k_len: int, *, q_start: int = 0, bidirectional: bool = True,
@@ -1657,7 +1658,9 @@ def relative_bias(table: torch.Tensor, q_len: int, k_len: int, *, q_start: int =
     if q_len < 0 or k_len < 0:
         raise ValueError("relative_bias: negative length")
     edges = _bucket_edges(int(table.shape[0]), int(max_distance), bool(bidirectional))
-    q_start = _bias_start("relative_bias", q_start)
+    q_start = int(q_start)
+    if not -_MOST_START <= q_start <= _MOST_START:
+        _too_far("relative_bias", q_start)
     code = nat.dtype_code(table.dtype)
     dev = nat.same_device(table)
     heads = table.shape[1]
@@ -1690,7 +1693,9 @@ def relative_bias_grad(g: torch.Tensor, num_buckets: int, *, q_start: int = 0, b
         raise ValueError("relative_bias_grad expects a (B, heads, q_len, k_len) gradient")
     b, h, tq, tk = g.shape
     edges = _bucket_edges(int(num_buckets), int(max_distance), bool(bidirectional))
-    q_start = _bias_start("relative_bias_grad", q_start)
+    q_start = int(q_start)
+    if not -_MOST_START <= q_start <= _MOST_START:
+        _too_far("relative_bias_grad", q_start)
     code = nat.dtype_code(g.dtype)
     check_bias_mask("relative_bias_grad", mask, b, tq, tk, q_start)
     mask, mask_ptr, mask_b, mask_k = _token_mask("relative_bias_grad", mask, b, tk)
@@ -1710,10 +1715,11 @@ def relative_bias_grad(g: torch.Tensor, num_buckets: int, *, q_start: int = 0, b
     return out
 
 
-def _fits_32_bits(what: str, *sizes: int) -> None:
-    """Sizes that the C ABI takes as 32-bit integers (ctypes would cut them)."""
-    if max(sizes) > 0x7FFFFFFF:
-        raise NotImplementedError(f"{what}: {max(sizes)} experts or choices do not fit 32 bits")
+_MOST = 0x7FFFFFFF  # the C ABI's integers of experts and choices; ctypes would cut a wider one
+
+
+def _too_wide(what: str, size: int) -> None:
+    raise NotImplementedError(f"{what}: {size} experts or choices do not fit 32 bits")
 
 
 def balance_loss(logits: torch.Tensor, index: torch.Tensor, *, batch: int = 1, mask=None):
@@ -1725,7 +1731,9 @@ def balance_loss(logits: torch.Tensor, index: torch.Tensor, *, batch: int = 1, m
     if index.dtype != torch.int64:
         raise ValueError("balance_loss: expert indices must be int64")
     n, e = logits.shape
-    _fits_32_bits("balance_loss", e, index.shape[1])
+    top = index.shape[1]
+    if e > _MOST or top > _MOST:
+        _too_wide("balance_loss", max(e, top))
     if batch < 1 or n % batch:
         raise ValueError(f"balance_loss: {n} tokens are not {batch} samples of one length")
     code = nat.dtype_code(logits.dtype)
@@ -1744,7 +1752,7 @@ def balance_loss(logits: torch.Tensor, index: torch.Tensor, *, batch: int = 1, m
         ws_ptr = ws.data_ptr()
     _run_on(dev, "balance_loss", lib.da_balance_loss,
             logits.data_ptr(), code, batch, n // batch, e, logits.stride(0), index.data_ptr(),
-            index.shape[1], mask_ptr, mask_b, mask_t, loss.data_ptr(), z_loss.data_ptr(), counts.data_ptr(),
+            top, mask_ptr, mask_b, mask_t, loss.data_ptr(), z_loss.data_ptr(), counts.data_ptr(),
             live.data_ptr(), ws_ptr, nbytes.value, nat.stream_ptr(dev))
     return loss, z_loss, counts, live
 
@@ -1764,7 +1772,8 @@ def balance_loss_grad(up, up_z, logits: torch.Tensor, counts: torch.Tensor, live
     if logits.dim() != 2 or counts.dim() != 2 or counts.shape[1] != logits.shape[1]:
         raise ValueError("balance_loss_grad expects (N, E) logits and (B, E) counts")
     n, e = logits.shape
-    _fits_32_bits("balance_loss_grad", e)
+    if e > _MOST:
+        _too_wide("balance_loss_grad", e)
     batch = counts.shape[0]
     if batch < 1 or n % batch or live.shape != (batch,):
         raise ValueError(f"balance_loss_grad: {n} tokens are not {batch} samples of one length")
