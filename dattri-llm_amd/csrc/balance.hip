@@ -18,9 +18,10 @@
 //
 // 32 x 4096 tokens, 128 experts, top-8, bf16 (42 MB read forward, 67 MB read and
 // written backward): 13.0 + 4.7 us forward, 17.1 us backward; one wave a token, from
-// memory to the losses, 132 us for both.  The exponentials and butterflies take about
-// half of that, HBM the rest.  Small layers are bound by their launches: 16 x 256
-// tokens of 8 experts 5.6 and 3.6 us.
+// memory to the losses, 132 us for both.  By counters the vector ALU is active for 8.3
+// and 10.5 us of that (exponentials, butterflies), and waves wait for 47% and 58% of
+// their time: a token's mask is read before its logits, one step ahead.  Small layers
+// are bound by their launches: 16 x 256 tokens of 8 experts 5.6 and 3.6 us.
 #include <algorithm>
 
 #include "common.h"

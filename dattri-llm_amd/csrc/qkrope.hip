@@ -358,7 +358,8 @@ __global__ __launch_bounds__(kThreads) void qk_rope_forward(QkArgs a) {
 // A workgroup owns one side's rows of `chunk` tokens of a sample; its waves
 // take (token, group of heads) steps in turn and add their lanes' dw up, the
 // waves' sums meet in LDS and go to the chunk's place of the partials in fp32.
-// Three waves a SIMD fit its registers; held to four, it spills (241 us).
+// Three waves a SIMD fit its registers (130 for 8 lanes of bf16 runs, half-split); held
+// to four at 139, it spilled (241 us).
 template <int DT, int V, int kL, int S, bool kInter, bool kStream>
 __global__ __launch_bounds__(kThreads) void qk_rope_backward(QkArgs a, int64_t q_blocks) {
   constexpr int kHeads = kWave / kL;
