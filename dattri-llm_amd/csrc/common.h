@@ -233,6 +233,21 @@ __device__ __forceinline__ int64_t xcd_remap(int64_t w, int64_t n) {
 __device__ __forceinline__ u32x4 ld16(const void* p) { return *(const u32x4*)p; }
 __device__ __forceinline__ void st16(void* p, u32x4 v) { *(u32x4*)p = v; }
 
+// 16 bytes at an address that only elements of ES bytes are aligned to (gfx950 reads and
+// writes them in one instruction too).
+typedef uint32_t u32x4_at2 __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t u32x4_at4 __attribute__((ext_vector_type(4), aligned(4)));
+template <int ES>
+__device__ __forceinline__ u32x4 ld16_any(const void* p) {
+  if constexpr (ES == 4) return *(const u32x4_at4*)p;
+  else return *(const u32x4_at2*)p;
+}
+template <int ES>
+__device__ __forceinline__ void st16_any(void* p, u32x4 v) {
+  if constexpr (ES == 4) *(u32x4_at4*)p = v;
+  else *(u32x4_at2*)p = v;
+}
+
 // ---------------------------------------------------------------------------
 // Buffer loads straight into LDS (gfx950: 16 bytes per lane).
 // ---------------------------------------------------------------------------

@@ -1,0 +1,591 @@
+// Log probabilities of given tokens with the entropy and the most likely
+// alternatives, and the logits' gradient.
+//
+// Per live token, z = logits / temperature, m its largest, d_v = z_v - m:
+//
+//   lse = m + log sum e^d,   logprob = z_target - lse,
+//   entropy = log sum e^d - (sum d e^d) / (sum e^d)
+//   dlogits_v = (up [v = target] + p_v (up_lse - up - up_h (log p_v + entropy))) / temperature
+//
+// (a masked token: zeros; a target outside the vocabulary: none, logprob 0.)  One pass
+// over the row: each thread keeps the running maximum, sum and weighted sum of its runs of
+// 16 bytes, with one rescaling a batch of runs.  A row is one workgroup's,
+// or with few rows cut into parts that a second launch joins.
+//
+// The alternatives need no second pass over the row.  Every thread knows its own largest
+// entry, so the k-th largest of 64 groups' maxima is a bound that at least k entries
+// reach; only the threads whose maximum reaches it read their runs again and put what
+// reaches it into LDS.  Entries are ordered by (value, lower index first), as one 64-bit
+// key each, so that no two are alike and their ranks are their places.
+#include <algorithm>
+#include <type_traits>
+
+#include "common.h"
+
+namespace da {
+namespace {
+
+constexpr int kMaxTop = 32;
+constexpr int kGroups = 64;       // groups whose maxima bound the alternatives: kMaxTop and more
+constexpr int kCandidates = 2048; // entries that reach the bound, at most: past it the row is searched
+constexpr int kBatch = 4;         // runs of 16 bytes a thread has under way
+constexpr float kLog2e = 1.44269504088896341f;
+constexpr float kLn2 = 0.69314718055994531f;
+constexpr float kFloor = -3.4028234663852886e38f;  // the maximum where there is none or -inf: the lowest value
+
+struct LpArgs {
+  const char* logits;
+  const int64_t* targets;
+  const uint8_t* mask;
+  int64_t tokens, rows, vocab;
+  int64_t l_b, l_t, t_b, t_t, m_b, m_t;  // elements
+  float inv_temperature;
+  int top;
+  int64_t part, parts;  // entries of a part (whole runs), parts of a row
+  float* logprob;
+  float* entropy;
+  float* lse;
+  float* top_logprob;
+  int64_t* top_index;
+  float4* stats;    // (rows, parts): maximum, sum, weighted sum
+  uint64_t* keys;   // (rows, parts, top)
+  // backward
+  const float* up;
+  const float* up_h;
+  const float* up_lse;
+  const float* entropy_in;
+  const float* lse_in;
+  int64_t u_b, u_t, h_b, h_t, ul_b, ul_t;
+  char* grad;
+};
+
+// a b, 0 where either is 0 whatever the other one is.
+extern "C" __device__ float da_mul_or_zero(float a, float b) __asm("llvm.amdgcn.fmul.legacy");
+
+template <int DT>
+__device__ __forceinline__ uint32_t none() {  // -inf in every place of a word
+  return DT == DA_F32 ? 0xff800000u : DT == DA_BF16 ? 0xff80ff80u : 0xfc00fc00u;
+}
+
+// The run at v0 of a row; entries from end on are -inf and not read.
+template <int DT>
+__device__ __forceinline__ u32x4 load_run(const char* row, int64_t v0, int64_t end) {
+  constexpr int ES = Elem<DT>::kBytes, V = Elem<DT>::kVec;
+  if (v0 + V <= end) return ld16_any<ES>(row + v0 * ES);
+  u32x4 w = {none<DT>(), none<DT>(), none<DT>(), none<DT>()};
+  if (v0 >= end) return w;
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+    if (v0 + e >= end) continue;
+    if constexpr (ES == 4) {
+      w[e] = *(const uint32_t*)(row + (v0 + e) * 4);
+    } else {
+      const uint32_t bits = *(const uint16_t*)(row + (v0 + e) * 2);
+      w[e / 2] = e % 2 ? (w[e / 2] & 0xffffu) | bits << 16 : (w[e / 2] & 0xffff0000u) | bits;
+    }
+  }
+  return w;
+}
+
+// The order of two entries as whole numbers: by value, then by the lower index.  -0 is +0.
+__device__ __forceinline__ uint64_t key_of(float x, int64_t v) {
+  const uint32_t u = __float_as_uint(x + 0.f);
+  const uint32_t up = u & 0x80000000u ? ~u : u | 0x80000000u;
+  return (uint64_t)up << 32 | (0xffffffffu - (uint32_t)v);
+}
+__device__ __forceinline__ float key_value(uint64_t key) {
+  const uint32_t up = (uint32_t)(key >> 32);
+  return __uint_as_float(up & 0x80000000u ? up & 0x7fffffffu : ~up);
+}
+__device__ __forceinline__ int64_t key_index(uint64_t key) { return 0xffffffffu - (uint32_t)key; }
+
+// Sums of 2^d and of d 2^d, d = (logit - m) c, relative to the largest logit m.  The
+// difference comes first: logits of a type's lowest value do not overflow.
+struct Stats {
+  float m, s, e;
+  __device__ void join(float m2, float s2, float e2, float c) {
+    const float top = fmaxf(m, m2), d1 = (m - top) * c, d2 = (m2 - top) * c;
+    const float f1 = __builtin_amdgcn_exp2f(d1), f2 = __builtin_amdgcn_exp2f(d2);
+    // s = 0 where nothing was seen: its distance does not count.
+    e = f1 * (e + da_mul_or_zero(s, d1)) + f2 * (e2 + da_mul_or_zero(s2, d2));
+    s = s * f1 + s2 * f2;
+    m = top;
+  }
+};
+
+// A row's outputs from its sums.
+__device__ void finish(const LpArgs& a, int64_t row, int64_t b, int64_t t, const char* logits, int dt, float c,
+                       const Stats& x) {
+  const int64_t target = a.targets[b * a.t_b + t * a.t_t];
+  const float bits = log2f(x.s);
+  float logprob = 0.f;
+  if (target >= 0 && target < a.vocab) {
+    const float v = dt == DA_F32 ? Elem<DA_F32>::load(logits, target)
+                    : dt == DA_BF16 ? Elem<DA_BF16>::load(logits, target) : Elem<DA_F16>::load(logits, target);
+    logprob = ((v - x.m) * c - bits) * kLn2;
+  }
+  a.logprob[row] = logprob;
+  a.entropy[row] = (bits - x.e / x.s) * kLn2;
+  a.lse[row] = fmaf(x.m, a.inv_temperature, bits * kLn2);
+}
+
+// The largest of a wave's keys.
+__device__ __forceinline__ uint64_t wave_max_key(uint64_t k) {
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) {
+    const uint64_t o = (uint64_t)__shfl_xor((unsigned long long)k, off, kWave);
+    k = o > k ? o : k;
+  }
+  return k;
+}
+
+// The top-th largest of 64 keys, one a lane (0: none).
+__device__ __forceinline__ uint64_t bound_of(uint64_t k, int top) {
+  int above = 0;
+  for (int l = 0; l < kWave; ++l) above += (uint64_t)__shfl((unsigned long long)k, l, kWave) > k;
+  const uint64_t at = __ballot(k != 0 && above == top - 1);
+  return at ? (uint64_t)__shfl((unsigned long long)k, __ffsll((unsigned long long)at) - 1, kWave) : 0;
+}
+
+// The top largest of n different keys in LDS, in order, to f(place, key).
+template <int NT, class F>
+__device__ __forceinline__ void place(const uint64_t* keys, int n, int top, F f) {
+  for (int i = threadIdx.x; i < n; i += NT) {
+    const uint64_t k = keys[i];
+    int above = 0;
+    for (int j = 0; j < n; ++j) above += keys[j] > k;
+    if (above < top) f(above, k);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Forward: workgroup (row, part).
+// ---------------------------------------------------------------------------
+template <int DT, int NT, bool kTop>
+__global__ __launch_bounds__(NT) void logprobs_forward(LpArgs a) {
+  constexpr int ES = Elem<DT>::kBytes, V = Elem<DT>::kVec, kWaves = NT / kWave;
+  __shared__ float stat[3][kWaves];
+  __shared__ uint64_t maxima[kTop ? kGroups : 1];
+  __shared__ uint64_t found[kTop ? kCandidates : 1];
+  __shared__ uint64_t bound_at;
+  __shared__ int count;
+  const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
+  const int64_t row = blockIdx.x / a.parts, part = blockIdx.x - row * a.parts;
+  const int64_t b = row / a.tokens, t = row - b * a.tokens;
+  if (a.mask && !a.mask[b * a.m_b + t * a.m_t]) {
+    if (part) return;
+    if (tid == 0) a.logprob[row] = a.entropy[row] = a.lse[row] = 0.f;
+    if (kTop && tid < a.top) {
+      a.top_logprob[row * a.top + tid] = 0.f;
+      a.top_index[row * a.top + tid] = -1;
+    }
+    return;
+  }
+  const char* logits = a.logits + (b * a.l_b + t * a.l_t) * ES;
+  const int64_t v0 = part * a.part, end = min(v0 + a.part, a.vocab);
+  const float c = a.inv_temperature * kLog2e;
+  Stats x = {kFloor, 0.f, 0.f};
+  float most = -__builtin_inff();  // the thread's largest logit, and the batch that has it first
+  int64_t most_at = v0 + (int64_t)tid * V;
+  for (int64_t v = v0 + (int64_t)tid * V; v < end; v += (int64_t)NT * V * kBatch) {
+    u32x4 raw[kBatch];
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) raw[i] = load_run<DT>(logits, v + (int64_t)i * NT * V, end);
+    float f[kBatch][V], top = -__builtin_inff();
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      unpack16<DT>(raw[i], f[i]);
+#pragma unroll
+      for (int e = 0; e < V; ++e) top = fmaxf(top, f[i][e]);
+    }
+    if (kTop && top > most) most = top, most_at = v;
+    if (__any(top > x.m)) {
+      const float m = fmaxf(x.m, top), by = (x.m - m) * c, scale = __builtin_amdgcn_exp2f(by);
+      x.e = scale * (x.e + da_mul_or_zero(x.s, by));
+      x.s *= scale;
+      x.m = m;
+    }
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i)
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const float d = (f[i][e] - x.m) * c, p = __builtin_amdgcn_exp2f(d);
+        x.s += p;
+        x.e += da_mul_or_zero(p, d);  // 0 where p is: a logit of -inf
+      }
+  }
+  Stats sum = x;
+#pragma unroll
+  for (int off = 1; off < kWave; off <<= 1)
+    sum.join(__shfl_xor(sum.m, off, kWave), __shfl_xor(sum.s, off, kWave), __shfl_xor(sum.e, off, kWave), c);
+  if (lane == 0) stat[0][wave] = sum.m, stat[1][wave] = sum.s, stat[2][wave] = sum.e;
+  uint64_t mine = 0;
+  if constexpr (kTop) {
+    if (most_at < end) {  // the first entry of the batch that has the thread's largest
+      int64_t first = most_at;
+      bool seen = false;
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const int64_t at = most_at + (int64_t)i * NT * V;
+        float f[V];
+        unpack16<DT>(load_run<DT>(logits, at, end), f);
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+          if (!seen && f[e] == most && at + e < end) first = at + e, seen = true;
+      }
+      mine = key_of(most, first);
+    }
+    uint64_t k = mine;
+    constexpr int kEach = NT / kGroups;  // threads of a group
+#pragma unroll
+    for (int off = 1; off < kEach; off <<= 1) {
+      const uint64_t o = (uint64_t)__shfl_xor((unsigned long long)k, off, kWave);
+      k = o > k ? o : k;
+    }
+    if (tid % kEach == 0) maxima[tid / kEach] = k;
+    if (tid == 0) count = 0;
+  }
+  __syncthreads();
+  if (wave == 0) {
+    Stats all = {stat[0][0], stat[1][0], stat[2][0]};
+    for (int w = 1; w < kWaves; ++w) all.join(stat[0][w], stat[1][w], stat[2][w], c);
+    if (a.parts == 1) {
+      stat[0][0] = all.m, stat[1][0] = all.s;
+      if (lane == 0) finish(a, row, b, t, logits, DT, c, all);
+    } else if (lane == 0) {
+      a.stats[blockIdx.x] = float4{all.m, all.s, all.e, 0.f};
+    }
+    if constexpr (kTop) {
+      const uint64_t bound = bound_of(maxima[lane], a.top);
+      if (lane == 0) bound_at = bound;
+    }
+  }
+  if constexpr (!kTop) return;
+  __syncthreads();
+  const uint64_t bound = bound_at;
+  if (mine != 0 && mine >= bound) {
+    for (int64_t v = v0 + (int64_t)tid * V; v < end; v += (int64_t)NT * V) {
+      float f[V];
+      unpack16<DT>(load_run<DT>(logits, v, end), f);
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        if (v + e >= end) continue;
+        const uint64_t k = key_of(f[e], v + e);
+        if (k < bound) continue;
+        const int at = atomicAdd(&count, 1);  // places do not matter: keys are ranked
+        if (at < kCandidates) found[at] = k;
+      }
+    }
+  }
+  __syncthreads();
+  int n = count;
+  const float m = stat[0][0], bits = a.parts == 1 ? log2f(stat[1][0]) : 0.f;
+  auto put = [&](int at, uint64_t key) {
+    if (a.parts > 1) {
+      a.keys[(int64_t)blockIdx.x * a.top + at] = key;
+    } else {
+      a.top_logprob[row * a.top + at] = ((key_value(key) - m) * c - bits) * kLn2;
+      a.top_index[row * a.top + at] = key_index(key);
+    }
+  };
+  if (n <= kCandidates) {
+    place<NT>(found, n, a.top, put);
+    if (tid >= n && tid < a.top) {  // a part of fewer entries; a row with NaN
+      if (a.parts > 1) {
+        a.keys[(int64_t)blockIdx.x * a.top + tid] = 0;
+      } else {
+        a.top_logprob[row * a.top + tid] = __builtin_nanf("");
+        a.top_index[row * a.top + tid] = -1;
+      }
+    }
+    return;
+  }
+  // More entries reach the bound than LDS holds (sorted logits, say): the largest one below
+  // the last, `top` times over.
+  uint64_t last = ~0ull;
+  for (int at = 0; at < a.top; ++at) {
+    uint64_t k = 0;
+    for (int64_t v = v0 + (int64_t)tid * V; v < end; v += (int64_t)NT * V) {
+      float f[V];
+      unpack16<DT>(load_run<DT>(logits, v, end), f);
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const uint64_t o = v + e < end ? key_of(f[e], v + e) : 0;
+        if (o < last && o > k) k = o;
+      }
+    }
+    k = wave_max_key(k);
+    __syncthreads();
+    if (lane == 0) found[wave] = k;
+    __syncthreads();
+    for (int w = 0; w < kWaves; ++w) k = found[w] > k ? found[w] : k;
+    if (tid == 0) put(at, k);
+    last = k;
+  }
+}
+
+// The parts of a row: their sums in order, and the largest of their alternatives.
+constexpr int kJoin = 256, kMaxParts = 64;
+template <bool kTop>
+__global__ __launch_bounds__(kJoin) void logprobs_join(LpArgs a, int dt) {
+  __shared__ uint64_t keys[kTop ? kMaxParts * kMaxTop : 1];
+  __shared__ uint64_t kept[kTop ? kMaxParts * kMaxTop : 1];
+  __shared__ float stat[2];
+  __shared__ uint64_t bound_at;
+  __shared__ int count;
+  const int tid = threadIdx.x;
+  const int64_t row = blockIdx.x, b = row / a.tokens, t = row - b * a.tokens;
+  if (a.mask && !a.mask[b * a.m_b + t * a.m_t]) return;  // written by the first launch
+  const float c = a.inv_temperature * kLog2e;
+  const int parts = (int)a.parts, n = kTop ? parts * a.top : 0;
+  if (tid < kWave) {
+    Stats x = {kFloor, 0.f, 0.f};
+    if (tid < parts) {
+      const float4 v = a.stats[row * parts + tid];
+      x = Stats{v.x, v.y, v.z};
+    }
+#pragma unroll
+    for (int off = 1; off < kWave; off <<= 1)
+      x.join(__shfl_xor(x.m, off, kWave), __shfl_xor(x.s, off, kWave), __shfl_xor(x.e, off, kWave), c);
+    if (tid == 0) {
+      const int es = dt == DA_F32 ? 4 : 2;
+      finish(a, row, b, t, a.logits + (b * a.l_b + t * a.l_t) * es, dt, c, x);
+      stat[0] = x.m, stat[1] = x.s;
+      count = 0;
+    }
+  }
+  if constexpr (!kTop) return;
+  for (int i = tid; i < n; i += kJoin) keys[i] = a.keys[row * n + i];
+  __syncthreads();
+  if (tid < kWave) {
+    uint64_t k = 0;
+    for (int i = tid; i < n; i += kWave) k = keys[i] > k ? keys[i] : k;
+    const uint64_t bound = bound_of(k, a.top);
+    if (tid == 0) bound_at = bound;
+  }
+  __syncthreads();
+  const uint64_t bound = bound_at;
+  for (int i = tid; i < n; i += kJoin)
+    if (keys[i] && keys[i] >= bound) kept[atomicAdd(&count, 1)] = keys[i];
+  __syncthreads();
+  const float m = stat[0], bits = log2f(stat[1]);
+  if (tid >= count && tid < a.top) {
+    a.top_logprob[row * a.top + tid] = __builtin_nanf("");
+    a.top_index[row * a.top + tid] = -1;
+  }
+  place<kJoin>(kept, count, a.top, [&](int at, uint64_t key) {
+    a.top_logprob[row * a.top + at] = ((key_value(key) - m) * c - bits) * kLn2;
+    a.top_index[row * a.top + at] = key_index(key);
+  });
+}
+
+// ---------------------------------------------------------------------------
+// Backward: workgroup (row, part), a run of 16 bytes a thread and step.
+// ---------------------------------------------------------------------------
+template <int DT, int NT>
+__global__ __launch_bounds__(NT) void logprobs_backward(LpArgs a) {
+  constexpr int ES = Elem<DT>::kBytes, V = Elem<DT>::kVec;
+  const int64_t row = blockIdx.x / a.parts, part = blockIdx.x - row * a.parts;
+  const int64_t b = row / a.tokens, t = row - b * a.tokens;
+  const bool live = !a.mask || a.mask[b * a.m_b + t * a.m_t];
+  const char* logits = a.logits + (b * a.l_b + t * a.l_t) * ES;
+  char* grad = a.grad + row * a.vocab * ES;
+  const int64_t v0 = part * a.part, end = min(v0 + a.part, a.vocab);
+  int64_t target = a.targets[b * a.t_b + t * a.t_t];
+  const bool named = live && target >= 0 && target < a.vocab;
+  target = named ? target : -1;
+  const float up = named && a.up ? a.up[b * a.u_b + t * a.u_t] * a.inv_temperature : 0.f;
+  const float up_h = live && a.up_h ? a.up_h[b * a.h_b + t * a.h_t] * a.inv_temperature : 0.f;
+  const float up_lse = live && a.up_lse ? a.up_lse[b * a.ul_b + t * a.ul_t] * a.inv_temperature : 0.f;
+  const float lse = live ? a.lse_in[row] : 0.f;
+  const float whole = up_lse - up - (a.up_h && live ? up_h * a.entropy_in[row] : 0.f), slope = -up_h;
+  for (int64_t v = v0 + (int64_t)threadIdx.x * V; v < end; v += (int64_t)NT * V * kBatch) {
+    u32x4 raw[kBatch];
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      raw[i] = u32x4{0, 0, 0, 0};
+      if (live) raw[i] = load_run<DT>(logits, v + (int64_t)i * NT * V, end);
+    }
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const int64_t at = v + (int64_t)i * NT * V;
+      float f[V];
+      unpack16<DT>(raw[i], f);
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const float d = fmaf(f[e], a.inv_temperature, -lse), p = __builtin_amdgcn_exp2f(d * kLog2e);
+        f[e] = live ? da_mul_or_zero(p, fmaf(d, slope, whole)) : 0.f;
+      }
+      if (target >= at && target < at + V) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) f[e] += at + e == target ? up : 0.f;
+      }
+      u32x4 w;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if constexpr (DT == DA_F32) w[k] = __float_as_uint(f[k]);
+        else w[k] = pack2<DT>(f[2 * k], f[2 * k + 1]);
+      }
+      if (at + V <= end) {
+        st16_any<ES>(grad + at * ES, w);
+      } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          if (at + e >= end) continue;
+          if constexpr (ES == 4) *(uint32_t*)(grad + (at + e) * 4) = w[e];
+          else *(uint16_t*)(grad + (at + e) * 2) = (uint16_t)(w[e / 2] >> (16 * (e % 2)));
+        }
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Launches.
+// ---------------------------------------------------------------------------
+int check_rows(const char* what, int dtype, int64_t batch, int64_t tokens, int64_t vocab, float temperature) {
+  if (!valid_dtype(dtype)) return set_error(DA_ERR_INVALID, "%s: bad dtype %d", what, dtype);
+  if (batch < 0 || tokens < 0) return set_error(DA_ERR_INVALID, "%s: negative size", what);
+  if (vocab < 1 || vocab > INT32_MAX) return set_error(DA_ERR_UNSUPPORTED, "%s: vocabularies of 1 to 2^31 - 1 tokens", what);
+  if (!(temperature > 0.f) || !(1.f / temperature < 1e30f))
+    return set_error(DA_ERR_INVALID, "%s: the temperature must be positive", what);
+  if (tokens && batch > kMaxBlocks / 4 / tokens) return set_error(DA_ERR_UNSUPPORTED, "%s: too many rows", what);
+  return DA_OK;
+}
+
+// Threads of a row's workgroup: one wave where a row is a few kilobytes.
+int threads_of(int64_t vocab, int dtype) { return vocab * (int64_t)elem_bytes(dtype) <= 8192 ? 64 : 512; }
+
+// Parts of a row: enough workgroups for every CU, no part under two runs a thread.
+int parts_of(int64_t rows, int64_t vocab, int dtype, int64_t* part, int64_t* parts) {
+  int64_t cus;
+  const int rc = device_cu_count(&cus);
+  if (rc) return rc;
+  const int64_t vec = dtype == DA_F32 ? 4 : 8, least = 2 * threads_of(vocab, dtype) * vec;
+  int64_t n = rows >= cus ? 1 : std::min<int64_t>(kMaxParts, 2 * cus / std::max<int64_t>(rows, 1));
+  n = std::max<int64_t>(1, std::min(n, vocab / least));
+  *part = ((vocab + n - 1) / n + vec - 1) / vec * vec;
+  *parts = (vocab + *part - 1) / *part;
+  return DA_OK;
+}
+
+size_t workspace_of(int64_t rows, int64_t parts, int top) {
+  return parts > 1 ? (size_t)(rows * parts) * (sizeof(float4) + (size_t)top * sizeof(uint64_t)) : 0;
+}
+
+template <class F>
+int by_type(int dtype, int threads, F f) {
+#define DA_LP(DT)                                                                                 \
+  return threads == 64 ? f(std::integral_constant<int, DT>{}, std::integral_constant<int, 64>{}) \
+                       : f(std::integral_constant<int, DT>{}, std::integral_constant<int, 512>{});
+  if (dtype == DA_F32) DA_LP(DA_F32)
+  if (dtype == DA_BF16) DA_LP(DA_BF16)
+  DA_LP(DA_F16)
+#undef DA_LP
+}
+
+}  // namespace
+}  // namespace da
+
+extern "C" {
+
+int da_token_logprobs_workspace(int dtype, int64_t batch, int64_t tokens, int64_t vocab, int top, size_t* bytes) {
+  using namespace da;
+  if (!bytes) return set_error(DA_ERR_INVALID, "da_token_logprobs_workspace: NULL pointer");
+  *bytes = 0;
+  int rc = check_rows("da_token_logprobs_workspace", dtype, batch, tokens, vocab, 1.f);
+  if (rc) return rc;
+  if (top < 0 || top > kMaxTop || top > vocab)
+    return set_error(DA_ERR_UNSUPPORTED, "da_token_logprobs_workspace: 0 to %d alternatives, no more than tokens", kMaxTop);
+  int64_t part, parts;
+  rc = parts_of(batch * tokens, vocab, dtype, &part, &parts);
+  if (rc == DA_OK) *bytes = workspace_of(batch * tokens, parts, top);
+  return rc;
+}
+
+int da_token_logprobs(const void* logits, int dtype, int64_t batch, int64_t tokens, int64_t vocab, int64_t l_bstride,
+                      int64_t l_tstride, const int64_t* targets, int64_t t_bstride, int64_t t_tstride,
+                      const uint8_t* mask, int64_t mask_bstride, int64_t mask_tstride, float temperature, int top,
+                      float* logprob, float* entropy, float* lse, float* top_logprob, int64_t* top_index,
+                      void* workspace, size_t workspace_bytes, void* stream) {
+  using namespace da;
+  int rc = check_rows("da_token_logprobs", dtype, batch, tokens, vocab, temperature);
+  if (rc) return rc;
+  if (top < 0 || top > kMaxTop || top > vocab)
+    return set_error(DA_ERR_UNSUPPORTED, "da_token_logprobs: 0 to %d alternatives, no more than tokens", kMaxTop);
+  if (batch == 0 || tokens == 0) return DA_OK;
+  if (!logits || !targets || !logprob || !entropy || !lse || (top && (!top_logprob || !top_index)))
+    return set_error(DA_ERR_INVALID, "da_token_logprobs: NULL pointer");
+  LpArgs a = {};
+  rc = parts_of(batch * tokens, vocab, dtype, &a.part, &a.parts);
+  if (rc) return rc;
+  a.rows = batch * tokens;
+  const size_t need = workspace_of(a.rows, a.parts, top);
+  if (need && (!workspace || workspace_bytes < need))
+    return set_error(DA_ERR_WORKSPACE, "da_token_logprobs: workspace of %zu bytes needed", need);
+  if ((uintptr_t)workspace % 16) return set_error(DA_ERR_INVALID, "da_token_logprobs: workspace must be 16-byte aligned");
+  a.logits = (const char*)logits;
+  a.targets = targets;
+  a.mask = mask;
+  a.tokens = tokens, a.vocab = vocab;
+  a.l_b = l_bstride, a.l_t = l_tstride, a.t_b = t_bstride, a.t_t = t_tstride, a.m_b = mask_bstride, a.m_t = mask_tstride;
+  a.inv_temperature = 1.f / temperature;
+  a.top = top;
+  a.logprob = logprob, a.entropy = entropy, a.lse = lse, a.top_logprob = top_logprob, a.top_index = top_index;
+  a.stats = (float4*)workspace;
+  a.keys = need ? (uint64_t*)((float4*)workspace + a.rows * a.parts) : nullptr;
+  const hipStream_t st = (hipStream_t)stream;
+  rc = by_type(dtype, threads_of(vocab, dtype), [&](auto dt, auto nt) {
+    constexpr int DT = decltype(dt)::value, NT = decltype(nt)::value;
+    const unsigned grid = (unsigned)(a.rows * a.parts);
+    if (top) logprobs_forward<DT, NT, true><<<grid, NT, 0, st>>>(a);
+    else logprobs_forward<DT, NT, false><<<grid, NT, 0, st>>>(a);
+    return check_launch("da_token_logprobs");
+  });
+  if (rc || a.parts == 1) return rc;
+  if (top) logprobs_join<true><<<(unsigned)a.rows, kJoin, 0, st>>>(a, dtype);
+  else logprobs_join<false><<<(unsigned)a.rows, kJoin, 0, st>>>(a, dtype);
+  return check_launch("da_token_logprobs");
+}
+
+int da_token_logprobs_grad(const float* up, int64_t up_bstride, int64_t up_tstride, const float* up_entropy,
+                           int64_t uh_bstride, int64_t uh_tstride, const float* up_lse, int64_t ul_bstride,
+                           int64_t ul_tstride, const void* logits, int dtype, int64_t batch, int64_t tokens,
+                           int64_t vocab, int64_t l_bstride, int64_t l_tstride, const int64_t* targets,
+                           int64_t t_bstride, int64_t t_tstride, const float* lse, const float* entropy,
+                           const uint8_t* mask, int64_t mask_bstride, int64_t mask_tstride, float temperature,
+                           void* grad, void* stream) {
+  using namespace da;
+  const int rc = check_rows("da_token_logprobs_grad", dtype, batch, tokens, vocab, temperature);
+  if (rc) return rc;
+  if (batch == 0 || tokens == 0) return DA_OK;
+  if (!logits || !targets || !lse || !grad || (up_entropy && !entropy))
+    return set_error(DA_ERR_INVALID, "da_token_logprobs_grad: NULL pointer");
+  LpArgs a = {};
+  a.rows = batch * tokens;
+  const int64_t vec = dtype == DA_F32 ? 4 : 8;
+  const int nt = threads_of(vocab, dtype) == 64 ? 64 : 512;
+  // Parts of two batches a thread: nothing is joined.
+  a.part = 2 * (int64_t)kBatch * nt * vec;
+  a.parts = (vocab + a.part - 1) / a.part;
+  if (a.rows > kMaxBlocks / 4 / a.parts) return set_error(DA_ERR_UNSUPPORTED, "da_token_logprobs_grad: too many rows");
+  a.up = up, a.u_b = up_bstride, a.u_t = up_tstride;
+  a.up_h = up_entropy, a.h_b = uh_bstride, a.h_t = uh_tstride;
+  a.up_lse = up_lse, a.ul_b = ul_bstride, a.ul_t = ul_tstride;
+  a.logits = (const char*)logits;
+  a.targets = targets;
+  a.mask = mask;
+  a.tokens = tokens, a.vocab = vocab;
+  a.l_b = l_bstride, a.l_t = l_tstride, a.t_b = t_bstride, a.t_t = t_tstride, a.m_b = mask_bstride, a.m_t = mask_tstride;
+  a.inv_temperature = 1.f / temperature;
+  a.lse_in = lse, a.entropy_in = entropy;
+  a.grad = (char*)grad;
+  const hipStream_t st = (hipStream_t)stream;
+  return by_type(dtype, nt, [&](auto dt, auto n) {
+    constexpr int NT = decltype(n)::value;
+    logprobs_backward<decltype(dt)::value, NT><<<(unsigned)(a.rows * a.parts), NT, 0, st>>>(a);
+    return check_launch("da_token_logprobs_grad");
+  });
+}
+
+}  // extern "C"

@@ -16,7 +16,7 @@ import torch
 
 LIB_NAME = "libdattri_amd.so"
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), LIB_NAME)
-ABI_VERSION = 17
+ABI_VERSION = 18
 
 DA_F32, DA_F16, DA_BF16 = 0, 1, 2
 DA_OK, DA_ERR_INVALID, DA_ERR_UNSUPPORTED, DA_ERR_HIP, DA_ERR_WORKSPACE = 0, 1, 2, 3, 4
@@ -231,6 +231,47 @@ SIGNATURES.update(
             _I32, [_P, _I32, _I64, _I64, _I32, _I64, _P, _I32, _P, _I64, _I64, _P, _P, _P, _P, _P, _SZ, _P]),
         "da_balance_loss_grad": (
             _I32, [_P, _P, _P, _I32, _I64, _I64, _I32, _I64, _P, _P, _P, _I64, _I64, _P, _I64, _P]),
+    }
+)
+
+
+
+class DiffInputs(ctypes.Structure):
+    """Mirror of ``da_diff_inputs`` (include/dattri_amd.h)."""
+
+    _fields_ = [
+        *((f, ctypes.c_void_p) for f in ("q", "k", "v", "lam")),
+        *((f, ctypes.c_int64) for f in ("lam_dtype", "lam_stride", "q_bstride", "q_tstride", "q_hstride", "k_bstride",
+                                        "k_tstride", "k_hstride", "v_bstride", "v_tstride", "v_hstride")),
+        ("mask", ctypes.c_void_p),
+        *((f, ctypes.c_int64) for f in ("mask_bstride", "mask_kstride")),
+        ("q_mask", ctypes.c_void_p),
+        *((f, ctypes.c_int64) for f in ("q_mask_bstride", "q_mask_tstride")),
+    ]
+
+
+# The record of one call is passed as an array of 64-bit words (DiffInputs' fields in order).
+_F32 = ctypes.c_float
+_DIFF = [_I32, *[_I64] * 7, _F32, _I32, _I64]  # dtype, sizes, scale, causal, q_start
+_SIZES = [_I32, *[_I64] * 7, ctypes.POINTER(_SZ)]
+SIGNATURES.update(
+    {
+        "da_add_rms_norm": (
+            _I32, [_P, _P, _P, _I32, _I32, *[_I64] * 7, _P, _I64, _I64, _F32, _I32, _P, _P, _P, _P]),
+        "da_add_rms_norm_grad_workspace": (_I32, [_I32, _I64, _I64, _I64, ctypes.POINTER(_SZ)]),
+        "da_add_rms_norm_grad": (
+            _I32, [_P, _P, _P, _P, _I32, _I32, *[_I64] * 9, _P, _I64, _I64, _F32, _P, _P, _P, _SZ, _P]),
+        "da_diff_attention_workspace": (_I32, _SIZES),
+        "da_diff_attention": (_I32, [_P, *_DIFF, _P, _P, _P, _P, _SZ, _P]),
+        "da_diff_attention_grad_workspace": (_I32, _SIZES),
+        "da_diff_attention_grad": (
+            _I32, [_P, _P, _I64, _I64, _I64, _P, _P, _P, *_DIFF, _P, _P, _P, _P, _P, _SZ, _P]),
+        "da_token_logprobs_workspace": (_I32, [_I32, _I64, _I64, _I64, _I32, ctypes.POINTER(_SZ)]),
+        "da_token_logprobs": (
+            _I32, [_P, _I32, *[_I64] * 5, _P, _I64, _I64, _P, _I64, _I64, _F32, _I32, *[_P] * 6, _SZ, _P]),
+        "da_token_logprobs_grad": (
+            _I32, [*[_P, _I64, _I64] * 3, _P, _I32, *[_I64] * 5, _P, _I64, _I64, _P, _P, _P, _I64, _I64, _F32, _P,
+                   _P]),
     }
 )
 

@@ -8,6 +8,9 @@ tensors, the unsuffixed ones take :class:`Factorized` (or dense tensors).
 
 from dattri_llm_amd.gradient.ops import cost, dtypes, kronecker, moe
 from dattri_llm_amd.gradient.ops.attention import (
+    DiffAttentionState,
+    diff_attention,
+    diff_attention_grad,
     qk_norm_rope,
     qk_norm_rope_grad,
     relative_bias,
@@ -56,12 +59,14 @@ from dattri_llm_amd.gradient.ops.kronecker import (
     kfac_precondition_materialized,
     sym_inverse,
 )
+from dattri_llm_amd.gradient.ops.loss import TokenLogprobs, token_logprobs, token_logprobs_grad
 from dattri_llm_amd.gradient.ops.materialize import (
     materialize,
     materialize_blocked,
     materialize_factors,
     materialize_group,
 )
+from dattri_llm_amd.gradient.ops.norm import AddNorm, add_rms_norm, add_rms_norm_grad
 from dattri_llm_amd.gradient.ops.preprocess import (
     extract_module_kwargs,
     preprocess_factorized,
@@ -142,4 +147,6 @@ __all__ = [
     "project_outer_factors", "qk_norm_rope", "qk_norm_rope_grad", "relative_bias", "relative_bias_grad",
     "route_flops", "set_compute_dtype",
     "set_routing_policy", "should_materialize", "to_3d",
+    "AddNorm", "DiffAttentionState", "TokenLogprobs", "add_rms_norm", "add_rms_norm_grad", "diff_attention",
+    "diff_attention_grad", "token_logprobs", "token_logprobs_grad",
 ]

@@ -1,25 +1,29 @@
 """The learned parts of attention beside its linear layers: the norms of queries
-and keys with the position rotation, and the relative position bias.
+and keys with the position rotation, the relative position bias, and attention
+by the difference of two softmax maps.
 
-Both hold parameters whose per-sample gradient cannot be formed from the
+They hold parameters whose per-sample gradient cannot be formed from the
 layer's own input and output, as the reference does for its norm and embedding
 layers (``dattri_llm/gradient/ops/materialize.py:22-48``, ``:96-98``): the
 norms' output gradient is known only behind the rotation, and a bias table is
 looked up once for the whole batch, so that the gradient which reaches it is
-already summed over the samples.  Here the backward pass of each operator
+already summed over the samples, as is that of the factor between two maps.  Here the backward pass of each operator
 gives the per-sample gradient itself:
 
 * :func:`qk_norm_rope` / :func:`qk_norm_rope_grad` (``da_qk_norm_rope``);
-* :func:`relative_bias` / :func:`relative_bias_grad` (``da_relative_bias``).
+* :func:`relative_bias` / :func:`relative_bias_grad` (``da_relative_bias``);
+* :func:`diff_attention` / :func:`diff_attention_grad` (``da_diff_attention``).
 
 The unsuffixed functions are differentiable; the ``_grad`` functions are the
 same backward passes as plain calls, which can be captured into a HIP graph.
 Second and forward-mode derivatives are refused.
-Both work in the dtypes they are given and hold sums, norms and angles in 32
+They work in the dtypes they are given and hold sums, norms and angles in 32
 bits or more (no compute-dtype policy applies).
 """
 
 from __future__ import annotations
+
+from typing import NamedTuple
 
 import torch
 from torch.autograd import forward_ad
@@ -156,4 +160,82 @@ def relative_bias_grad(g, num_buckets: int, *, q_start: int = 0, bidirectional: 
                                       max_distance=max_distance, causal=causal, mask=mask)
 
 
-__all__ = ["qk_norm_rope", "qk_norm_rope_grad", "relative_bias", "relative_bias_grad"]
+class DiffAttentionState(NamedTuple):
+    """What :func:`diff_attention_grad` needs of the forward call beside its output."""
+
+    second: torch.Tensor
+    lse: torch.Tensor
+
+
+class _DiffAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, lam, mask, q_mask, cfg, slot):
+        out, second, lse = kernels.diff_attention(q, k, v, lam, mask=mask, q_mask=q_mask, state=True, **cfg)
+        ctx.save_for_backward(q, k, v, lam, mask, q_mask, out, second, lse)
+        ctx.cfg, ctx.slot = cfg, slot
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        q, k, v, lam, mask, q_mask, out, second, lse = ctx.saved_tensors
+        dq, dk, dv, per_sample = kernels.diff_attention_grad(g, q, k, v, lam, out, second, lse, mask=mask,
+                                                             q_mask=q_mask, **ctx.cfg)
+        need = ctx.needs_input_grad
+        dlam = None
+        if ctx.slot is not None:
+            ctx.slot.put(per_sample)
+        elif need[3]:
+            dlam = per_sample.sum(0) if lam.numel() > 1 else per_sample.sum()
+            dlam = dlam.reshape(lam.shape).to(lam.dtype)
+        return (dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, dlam,
+                None, None, None, None)
+
+
+def diff_attention(q, k, v, lam, *, scale: float | None = None, causal: bool = False, q_start: int | None = None,
+                   mask=None, q_mask=None, return_state: bool = False, slot=None):
+    """Attention by the difference of two softmax maps, differentiable:
+    ``out_h = softmax(scale q_2h k^T) v - lam_h softmax(scale q_2h+1 k^T) v``.
+
+    ``q (B, T, 2 H, D)`` holds head ``h``'s two query maps at ``2h`` and ``2h +
+    1``, ``k (B, S, 2 Hk, D)`` a key head's two key maps likewise, ``v (B, S, Hk,
+    Dv)``; head ``h`` reads key head ``h // (H // Hk)``.  ``out (B, T, H, Dv)``,
+    contiguous.  ``lam``: ``(H,)``, or one entry for all heads.  ``D`` up to 128,
+    ``Dv`` up to 256; ``scale`` is ``D ** -0.5`` by default.  Inputs of any
+    strides (a copy is made where entries are not contiguous).
+
+    ``causal``: query ``i`` sees the keys up to ``i + q_start``, by default ``S -
+    T`` (the queries are the last positions; one new token against a cache is
+    ``T = 1``).  ``mask`` (B, S): a zero hides the key from every query;
+    ``q_mask`` (B, T): a zero takes the query out.  Both may hold anything there.
+    A query that sees no key has a zero row and no gradient.
+
+    ``return_state``: ``(out, state)`` for :func:`diff_attention_grad`; not
+    differentiable.  ``slot`` takes ``lam``'s per-sample gradient ``(B, H)`` in the
+    backward pass, in place of its summed one (``FusedCapture``).  In 16 bits that
+    gradient carries the rounding of the maps' values."""
+    if getattr(forward_ad, "_current_level", 0) >= 0:
+        kernels.refuse_tangents("diff_attention", q, k, v, lam)
+    cfg = {"scale": scale, "causal": causal, "q_start": q_start}
+    if torch.is_grad_enabled() and (slot is not None or q.requires_grad or k.requires_grad or v.requires_grad or
+                                    lam.requires_grad):
+        if return_state:
+            raise ValueError("diff_attention: return_state is for plain calls; call it under no_grad")
+        if slot is not None and not lam.requires_grad:
+            lam = lam.detach().requires_grad_()  # a frozen factor is captured too
+        return _DiffAttention.apply(q, k, v, lam, mask, q_mask, cfg, slot)
+    out, second, lse = kernels.diff_attention(q, k, v, lam, mask=mask, q_mask=q_mask, state=return_state, **cfg)
+    return (out, DiffAttentionState(second, lse)) if return_state else out
+
+
+def diff_attention_grad(g, q, k, v, lam, out, state: DiffAttentionState, *, scale: float | None = None,
+                        causal: bool = False, q_start: int | None = None, mask=None, q_mask=None):
+    """The backward pass of :func:`diff_attention` for the gradient ``g`` of
+    ``out``, with what it returned under ``return_state`` and the same settings:
+    ``(dq, dk, dv, dlam)``, ``dlam`` per sample, fp32 ``(B, H)``."""
+    return kernels.diff_attention_grad(g, q, k, v, lam, out, state.second, state.lse, scale=scale, causal=causal,
+                                       q_start=q_start, mask=mask, q_mask=q_mask)
+
+
+__all__ = ["DiffAttentionState", "diff_attention", "diff_attention_grad", "qk_norm_rope", "qk_norm_rope_grad",
+           "relative_bias", "relative_bias_grad"]

@@ -1790,3 +1790,272 @@ def balance_loss_grad(up, up_z, logits: torch.Tensor, counts: torch.Tensor, live
             code, batch, n // batch, e, logits.stride(0), counts.data_ptr(), live.data_ptr(),
             mask_ptr, mask_b, mask_t, grad.data_ptr(), e, nat.stream_ptr(dev))
     return grad
+
+
+# ---------------------------------------------------------------------------
+# The residual's addition with the RMS norm that follows it.
+# ---------------------------------------------------------------------------
+_QUANTIZE = {None: 0, "row": 1, "block": 2}
+
+
+def _norm_rows(what: str, weight, x: torch.Tensor, *others):
+    """Rows (B, T, d) of one shape and dtype with entries contiguous, and the
+    weight in their dtype or fp32."""
+    if x.dim() != 3:
+        raise ValueError(f"{what} expects (B, T, d) rows, got {tuple(x.shape)}")
+    for o in others:
+        if o is not None and (o.shape != x.shape or o.dtype != x.dtype):
+            raise ValueError(f"{what}: rows of one shape and dtype are expected, got {tuple(x.shape)} {x.dtype} and "
+                             f"{tuple(o.shape)} {o.dtype}")
+    if weight.shape != x.shape[2:]:
+        raise ValueError(f"{what}: the weight must have shape ({x.shape[2]},), got {tuple(weight.shape)}")
+    nat.dtype_code(x.dtype)
+    nat.dtype_code(weight.dtype)
+    if weight.dtype not in (x.dtype, torch.float32):
+        weight = weight.to(torch.float32)
+    return weight.contiguous(), _unit_rows(x), *(None if o is None else _unit_rows(o) for o in others)
+
+
+def add_rms_norm(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Tensor, *, eps: float, mask=None,
+                 quantize: str | None = None):
+    """``(out, total, scales)`` of ``da_add_rms_norm``: ``total = x + residual``
+    (None without a residual), ``out`` its RMS norm times the weight, contiguous;
+    with ``quantize`` in 8 bits with fp32 ``scales`` (B, T) or (B, T, runs)."""
+    if quantize not in _QUANTIZE:
+        raise ValueError(f"add_rms_norm: quantize is None, 'row' or 'block', got {quantize!r}")
+    weight, x, residual = _norm_rows("add_rms_norm", weight, x, residual)
+    b, t, d = x.shape
+    mask, mask_ptr, mask_b, mask_t = _token_mask("add_rms_norm", mask, b, t)
+    dev = nat.same_device(x, residual, weight, mask)
+    scales = total = None
+    if quantize is not None:
+        shape = (b, t) if quantize == "row" else (b, t, -(-d // 128))
+        scales = torch.empty(shape, dtype=torch.float32, device=dev)
+    out = torch.empty((b, t, d), dtype=x.dtype if quantize is None else torch.float8_e4m3fn, device=dev)
+    r_ptr, r_b, r_t, total_ptr = None, 0, 0, None
+    if residual is not None:
+        total = torch.empty((b, t, d), dtype=x.dtype, device=dev)
+        r_ptr, r_b, r_t, total_ptr = residual.data_ptr(), residual.stride(0), residual.stride(1), total.data_ptr()
+    _run_on(dev, "add_rms_norm", nat.load().da_add_rms_norm,
+            x.data_ptr(), r_ptr, weight.data_ptr(), nat.DTYPE_CODE[x.dtype], nat.DTYPE_CODE[weight.dtype], b, t, d,
+            x.stride(0), x.stride(1), r_b, r_t, mask_ptr, mask_b, mask_t, float(eps), _QUANTIZE[quantize],
+            out.data_ptr(), total_ptr, None if scales is None else scales.data_ptr(), nat.stream_ptr(dev))
+    return out, total, scales
+
+
+def add_rms_norm_grad(g: torch.Tensor, g_total: torch.Tensor | None, total: torch.Tensor, weight: torch.Tensor, *,
+                      eps: float, mask=None, weight_grads: bool = True):
+    """``(dx, dweight)`` of ``da_add_rms_norm_grad``: the gradient of ``x`` and of
+    ``residual``, and the weight's per sample, fp32 (B, d) (None without
+    ``weight_grads``)."""
+    weight, total, g, g_total = _norm_rows("add_rms_norm_grad", weight, total, g, g_total)
+    if g is None:
+        raise ValueError("add_rms_norm_grad: the output's gradient is missing")
+    b, t, d = total.shape
+    mask, mask_ptr, mask_b, mask_t = _token_mask("add_rms_norm_grad", mask, b, t)
+    dev = nat.same_device(total, g, g_total, weight, mask)
+    dx = torch.empty((b, t, d), dtype=total.dtype, device=dev)
+    lib = nat.load()
+    code = nat.DTYPE_CODE[total.dtype]
+    dw, ws_ptr, nbytes = None, None, ctypes.c_size_t(0)
+    if weight_grads:
+        dw = torch.empty((b, d), dtype=torch.float32, device=dev)
+    with _on(dev):
+        if weight_grads:
+            nat.check(lib.da_add_rms_norm_grad_workspace(code, b, t, d, ctypes.byref(nbytes)), "add_rms_norm_grad")
+            if nbytes.value:
+                ws = nat.workspace(nbytes.value, dev)
+                ws_ptr = ws.data_ptr()
+        gt_ptr, gt_b, gt_t = (None, 0, 0) if g_total is None else (g_total.data_ptr(), *g_total.stride()[:2])
+        _run(dev, "add_rms_norm_grad", lib.da_add_rms_norm_grad,
+             g.data_ptr(), gt_ptr, total.data_ptr(), weight.data_ptr(), code, nat.DTYPE_CODE[weight.dtype], b, t, d,
+             g.stride(0), g.stride(1), gt_b, gt_t, total.stride(0), total.stride(1), mask_ptr, mask_b, mask_t,
+             float(eps), dx.data_ptr(), None if dw is None else dw.data_ptr(), ws_ptr, nbytes.value,
+             nat.stream_ptr(dev))
+    return dx, dw
+
+
+_HERE = contextlib.nullcontext()
+
+
+def _on(dev: torch.device):
+    """``dev`` as the current device: workspaces are sized for the current device's CUs."""
+    return _HERE if dev.index == nat.current_device() else torch.cuda.device(dev)
+
+
+# ---------------------------------------------------------------------------
+# Attention by the difference of two softmax maps.
+# ---------------------------------------------------------------------------
+def _diff_sizes(what: str, q, k, v, lam):
+    if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
+        raise ValueError(f"{what} expects (B, T, 2 H, D) queries, (B, S, 2 Hk, D) keys and (B, S, Hk, Dv) values")
+    b, t, h2, d = q.shape
+    s, hk, dv = v.shape[1:]
+    if k.shape != (b, s, 2 * hk, d) or v.shape[0] != b or h2 % 2 or hk < 1 or (h2 // 2) % hk or h2 < 1:
+        raise ValueError(f"{what}: queries {tuple(q.shape)}, keys {tuple(k.shape)} and values {tuple(v.shape)} do not "
+                         "belong together: two maps a head, heads a multiple of the key heads")
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError(f"{what}: queries, keys and values must share one dtype")
+    if lam.numel() != 1 and lam.shape != (h2 // 2,):
+        raise ValueError(f"{what}: lam must have shape ({h2 // 2},) or one entry, got {tuple(lam.shape)}")
+    nat.dtype_code(lam.dtype)
+    return b, t, s, h2 // 2, hk, d, dv
+
+
+def _diff_call(what, q, k, v, lam, mask, q_mask, scale, causal, q_start):
+    """Sizes, the record of the inputs as words, and the tensors it points to."""
+    sizes = _diff_sizes(what, q, k, v, lam)
+    b, t, s, h, hk, d, dv = sizes
+    code = nat.dtype_code(q.dtype)
+    mask, mask_ptr, mask_b, mask_k = _token_mask(what, mask, b, s)
+    q_mask, qm_ptr, qm_b, qm_t = _token_mask(what, q_mask, b, t)
+    dev = nat.same_device(q, k, v, lam, mask, q_mask)
+    q, k, v = _unit_rows(q), _unit_rows(k), _unit_rows(v)
+    scale = d ** -0.5 if scale is None else float(scale)
+    q_start = s - t if q_start is None else int(q_start)
+    words = array.array("q", (
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), lam.data_ptr(), nat.DTYPE_CODE[lam.dtype],
+        lam.stride(0) if lam.numel() > 1 else 0, *q.stride()[:3], *k.stride()[:3], *v.stride()[:3],
+        mask_ptr or 0, mask_b, mask_k, qm_ptr or 0, qm_b, qm_t))
+    return dev, sizes, (code, b, t, s, h, hk, d, dv), (scale, int(causal), q_start), words, (q, k, v, lam, mask, q_mask)
+
+
+def diff_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lam: torch.Tensor, *, scale: float | None = None,
+                   causal: bool = False, q_start: int | None = None, mask=None, q_mask=None, state: bool = False):
+    """``(out, second, lse)`` of ``da_diff_attention``: ``out`` (B, T, H, Dv), and
+    with ``state`` what :func:`diff_attention_grad` needs beside it (else None)."""
+    dev, (b, t, s, h, hk, d, dv), sizes, rest, words, keep = _diff_call("diff_attention", q, k, v, lam, mask, q_mask,
+                                                                        scale, causal, q_start)
+    lib = nat.load()
+    out = torch.empty((b, t, h, dv), dtype=q.dtype, device=dev)
+    second = lse = None
+    if state:
+        second = torch.empty((b, t, h, dv), dtype=q.dtype, device=dev)
+        lse = torch.empty((b, hk, 2, t * (h // hk)), dtype=torch.float32, device=dev)
+    nbytes = ctypes.c_size_t(0)
+    with _on(dev):
+        nat.check(lib.da_diff_attention_workspace(*sizes, ctypes.byref(nbytes)), "diff_attention")
+        ws_ptr = None
+        if nbytes.value:
+            ws = nat.workspace(nbytes.value, dev)
+            ws_ptr = ws.data_ptr()
+        _run(dev, "diff_attention", lib.da_diff_attention, words.buffer_info()[0], *sizes, *rest, out.data_ptr(),
+             None if second is None else second.data_ptr(), None if lse is None else lse.data_ptr(), ws_ptr,
+             nbytes.value, nat.stream_ptr(dev))
+    del keep
+    return out, second, lse
+
+
+def diff_attention_grad(g: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lam: torch.Tensor,
+                        out: torch.Tensor, second: torch.Tensor, lse: torch.Tensor, *, scale: float | None = None,
+                        causal: bool = False, q_start: int | None = None, mask=None, q_mask=None):
+    """``(dq, dk, dv, dlam)`` of ``da_diff_attention_grad`` for the gradient ``g`` of
+    ``out``, contiguous; ``dlam`` per sample, fp32 (B, H)."""
+    what = "diff_attention_grad"
+    dev, (b, t, s, h, hk, d, dv), sizes, rest, words, keep = _diff_call(what, q, k, v, lam, mask, q_mask, scale, causal,
+                                                                        q_start)
+    for name, x in (("g", g), ("out", out), ("second", second)):
+        if x.shape != (b, t, h, dv) or x.dtype != q.dtype:
+            raise ValueError(f"{what}: {name} must be {(b, t, h, dv)} {q.dtype}, got {tuple(x.shape)} {x.dtype}")
+    if lse.shape != (b, hk, 2, t * (h // hk)) or lse.dtype != torch.float32:
+        raise ValueError(f"{what}: the state does not belong to these inputs")
+    nat.same_device(q, g, out, second, lse)
+    g, out, second, lse = _unit_rows(g), out.contiguous(), second.contiguous(), lse.contiguous()
+    lib = nat.load()
+    dq = torch.empty((b, t, 2 * h, d), dtype=q.dtype, device=dev)
+    dk = torch.empty((b, s, 2 * hk, d), dtype=q.dtype, device=dev)
+    dval = torch.empty((b, s, hk, dv), dtype=q.dtype, device=dev)
+    dlam = torch.empty((b, h), dtype=torch.float32, device=dev)
+    nbytes = ctypes.c_size_t(0)
+    with _on(dev):
+        nat.check(lib.da_diff_attention_grad_workspace(*sizes, ctypes.byref(nbytes)), what)
+        ws = nat.workspace(nbytes.value, dev)
+        _run(dev, what, lib.da_diff_attention_grad, words.buffer_info()[0], g.data_ptr(), *g.stride()[:3],
+             out.data_ptr(), second.data_ptr(), lse.data_ptr(), *sizes, *rest, dq.data_ptr(), dk.data_ptr(),
+             dval.data_ptr(), dlam.data_ptr(), ws.data_ptr(), nbytes.value, nat.stream_ptr(dev))
+    del keep
+    return dq, dk, dval, dlam
+
+
+# ---------------------------------------------------------------------------
+# Log probabilities of given tokens.
+# ---------------------------------------------------------------------------
+def _token_rows(what: str, logits: torch.Tensor, targets: torch.Tensor, mask):
+    """(B, T, V) logits, their (B, T) targets and mask; (N, V) rows are one sample."""
+    if logits.dim() not in (2, 3) or targets.shape != logits.shape[:-1]:
+        raise ValueError(f"{what} expects (B, T, V) or (N, V) logits with a target each, got {tuple(logits.shape)} and "
+                         f"{tuple(targets.shape)}")
+    if targets.dtype != torch.int64:
+        raise ValueError(f"{what}: targets must be int64, got {targets.dtype}")
+    if mask is not None and mask.shape != targets.shape:
+        raise ValueError(f"{what}: mask must have shape {tuple(targets.shape)}, got {tuple(mask.shape)}")
+    if logits.dim() == 2:
+        logits, targets, mask = logits[None], targets[None], None if mask is None else mask[None]
+    return _unit_rows(logits), targets, mask
+
+
+def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, *, mask=None, temperature: float = 1.0, top: int = 0):
+    """``(logprob, entropy, lse, top_logprob, top_index)`` of ``da_token_logprobs``,
+    fp32 (int64 indices) in the targets' shape (times ``top``; None without)."""
+    what, shape = "token_logprobs", targets.shape
+    logits, targets, mask = _token_rows(what, logits, targets, mask)
+    b, t, v = logits.shape
+    if isinstance(top, bool) or not isinstance(top, int) or not 0 <= top <= min(32, v):
+        raise ValueError(f"{what}: top must be 0 to {min(32, v)}, got {top!r}")
+    code = nat.dtype_code(logits.dtype)
+    mask, mask_ptr, mask_b, mask_t = _token_mask(what, mask, b, t)
+    dev = nat.same_device(logits, targets, mask)
+    logprob, entropy, lse = (torch.empty(shape, dtype=torch.float32, device=dev) for _ in range(3))
+    top_logprob = top_index = None
+    if top:
+        top_logprob = torch.empty((*shape, top), dtype=torch.float32, device=dev)
+        top_index = torch.empty((*shape, top), dtype=torch.int64, device=dev)
+    lib = nat.load()
+    nbytes = ctypes.c_size_t(0)
+    with _on(dev):
+        nat.check(lib.da_token_logprobs_workspace(code, b, t, v, top, ctypes.byref(nbytes)), what)
+        ws_ptr = None
+        if nbytes.value:
+            ws = nat.workspace(nbytes.value, dev)
+            ws_ptr = ws.data_ptr()
+        _run(dev, what, lib.da_token_logprobs,
+             logits.data_ptr(), code, b, t, v, logits.stride(0), logits.stride(1), targets.data_ptr(),
+             targets.stride(0), targets.stride(1), mask_ptr, mask_b, mask_t, float(temperature), top,
+             logprob.data_ptr(), entropy.data_ptr(), lse.data_ptr(), top_logprob.data_ptr() if top else None,
+             top_index.data_ptr() if top else None, ws_ptr, nbytes.value, nat.stream_ptr(dev))
+    return logprob, entropy, lse, top_logprob, top_index
+
+
+def token_logprobs_grad(up, up_entropy, logits: torch.Tensor, targets: torch.Tensor, lse: torch.Tensor,
+                        entropy: torch.Tensor, *, up_lse=None, mask=None, temperature: float = 1.0) -> torch.Tensor:
+    """Gradient of the logits (``da_token_logprobs_grad``), contiguous, for the
+    gradients of :func:`token_logprobs`'s ``logprob``, ``entropy`` and ``lse``
+    (targets' shape; None: zero)."""
+    what, shape = "token_logprobs_grad", targets.shape
+    for x in (lse, entropy):
+        if x.shape != shape or x.dtype != torch.float32:
+            raise ValueError(f"{what}: lse and entropy must be fp32 of shape {tuple(shape)}, as token_logprobs returns them")
+    full = logits.shape
+    logits, targets, mask = _token_rows(what, logits, targets, mask)
+    b, t, v = logits.shape
+    code = nat.dtype_code(logits.dtype)
+    mask, mask_ptr, mask_b, mask_t = _token_mask(what, mask, b, t)
+    words, keep = [], []
+    for x in (up, up_entropy, up_lse):
+        if x is None:
+            words += (None, 0, 0)
+            continue
+        if x.shape != shape:
+            raise ValueError(f"{what}: a gradient must have shape {tuple(shape)}, got {tuple(x.shape)}")
+        x = x.to(torch.float32)
+        x = x if x.dim() == 2 else x[None]
+        keep.append(x)
+        words += (x.data_ptr(), x.stride(0), x.stride(1))
+    dev = nat.same_device(logits, targets, mask, lse, entropy, *keep)
+    lse, entropy = lse.contiguous(), entropy.contiguous()
+    grad = torch.empty(full, dtype=logits.dtype, device=dev)
+    _run_on(dev, what, nat.load().da_token_logprobs_grad,
+            *words, logits.data_ptr(), code, b, t, v, logits.stride(0), logits.stride(1), targets.data_ptr(),
+            targets.stride(0), targets.stride(1), lse.data_ptr(), entropy.data_ptr(), mask_ptr, mask_b, mask_t,
+            float(temperature), grad.data_ptr(), nat.stream_ptr(dev))
+    return grad

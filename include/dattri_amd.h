@@ -833,6 +833,116 @@ int da_balance_loss_grad(const float* up, const float* up_z, const void* logits,
                          int64_t grad_row_stride, void* stream);
 
 /*
+ * The residual's addition with the RMS norm that follows it.
+ *
+ * Rows x and residual (batch, tokens, d), entries contiguous, any other strides
+ * (elements); residual NULL: none.  Per token, with r = (mean(total^2) + eps)^(-1/2):
+ *
+ *   total = round(x + residual),   out = total r weight
+ *
+ * out and total are contiguous (total NULL: not wanted).  weight (d) in the rows'
+ * dtype or fp32.  mask: bytes, 0 marks a token whose rows are not read and whose
+ * outputs are zero; NULL: none.  quantize: 0 out in the rows' dtype; 1 out in 8
+ * bits (e4m3), to be multiplied by its row's entry of scales (batch, tokens); 2 by
+ * the scale of each 128 entries, (batch, tokens, ceil(d / 128)).  A scale is the
+ * largest |out| / 448 (1 where that is below 2^-100: such entries become zero).
+ * Rows of up to 64 KB.
+ *
+ * The backward call writes dx (contiguous; the residual's gradient is the same) for
+ * the gradients g of out and g_total of total (NULL: zero), and each sample's
+ * weight gradient, the sum over its tokens of g total r (batch, d) fp32 (NULL: not
+ * wanted); it takes a workspace from da_add_rms_norm_grad_workspace.  Sums run in a
+ * fixed order.
+ */
+int da_add_rms_norm(const void* x, const void* residual, const void* weight, int dtype, int weight_dtype,
+                    int64_t batch, int64_t tokens, int64_t d, int64_t x_bstride, int64_t x_tstride,
+                    int64_t r_bstride, int64_t r_tstride, const uint8_t* mask, int64_t mask_bstride,
+                    int64_t mask_tstride, float eps, int quantize, void* out, void* total, float* scales,
+                    void* stream);
+int da_add_rms_norm_grad_workspace(int dtype, int64_t batch, int64_t tokens, int64_t d, size_t* bytes);
+int da_add_rms_norm_grad(const void* g, const void* g_total, const void* total, const void* weight, int dtype,
+                         int weight_dtype, int64_t batch, int64_t tokens, int64_t d, int64_t g_bstride,
+                         int64_t g_tstride, int64_t gt_bstride, int64_t gt_tstride, int64_t total_bstride,
+                         int64_t total_tstride, const uint8_t* mask, int64_t mask_bstride, int64_t mask_tstride,
+                         float eps, void* dx, float* weight_grad, void* workspace, size_t workspace_bytes,
+                         void* stream);
+
+/*
+ * Attention by the difference of two softmax maps.  q (batch, q_len, 2 heads, d), k
+ * (batch, k_len, 2 k_heads, d), v (batch, k_len, k_heads, dv), entries contiguous,
+ * any other strides (elements).  Head h has the query maps 2 h and 2 h + 1, and reads
+ * key head h / (heads / k_heads), which has two key maps likewise:
+ *
+ *   out_h = softmax(scale q_2h k^T) v - lam_h softmax(scale q_2h+1 k^T) v
+ *
+ * lam (heads) at lam_stride (0 broadcasts).  causal: query i sees the keys up to
+ * i + q_start.  mask (batch, k_len) and q_mask (batch, q_len): bytes, 0 marks a key
+ * that no query sees, a query that takes no part, whatever they hold; NULL: none.  A
+ * query that sees no key has zero rows.  out (batch, q_len, heads, dv), contiguous.
+ * d <= 128, dv <= 256.
+ *
+ * second (like out: the second map's values) and lse (batch, 2 heads, q_len values)
+ * are what da_diff_attention_grad needs of the forward call; both NULL: not wanted.
+ * It writes dq, dk, dv (contiguous) and each sample's gradient of lam (batch, heads)
+ * fp32 for the gradient g of out.  All sums run in a fixed order.
+ */
+typedef struct da_diff_inputs {
+  const void *q, *k, *v, *lam;
+  int64_t lam_dtype, lam_stride;
+  int64_t q_bstride, q_tstride, q_hstride;
+  int64_t k_bstride, k_tstride, k_hstride;
+  int64_t v_bstride, v_tstride, v_hstride;
+  const uint8_t* mask;
+  int64_t mask_bstride, mask_kstride;
+  const uint8_t* q_mask;
+  int64_t q_mask_bstride, q_mask_tstride;
+} da_diff_inputs;
+
+int da_diff_attention_workspace(int dtype, int64_t batch, int64_t q_len, int64_t k_len, int64_t heads,
+                                int64_t k_heads, int64_t d, int64_t dv, size_t* bytes);
+int da_diff_attention(const da_diff_inputs* in, int dtype, int64_t batch, int64_t q_len, int64_t k_len, int64_t heads,
+                      int64_t k_heads, int64_t d, int64_t dv, float scale, int causal, int64_t q_start, void* out,
+                      void* second, float* lse, void* workspace, size_t workspace_bytes, void* stream);
+int da_diff_attention_grad_workspace(int dtype, int64_t batch, int64_t q_len, int64_t k_len, int64_t heads,
+                                     int64_t k_heads, int64_t d, int64_t dv, size_t* bytes);
+int da_diff_attention_grad(const da_diff_inputs* in, const void* g, int64_t g_bstride, int64_t g_tstride,
+                           int64_t g_hstride, const void* out, const void* second, const float* lse, int dtype,
+                           int64_t batch, int64_t q_len, int64_t k_len, int64_t heads, int64_t k_heads, int64_t d,
+                           int64_t dv, float scale, int causal, int64_t q_start, void* dq, void* dk, void* dvalue,
+                           float* dlam, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Log probabilities of given tokens.  logits (batch, tokens, vocab), entries
+ * contiguous, targets (batch, tokens) int64, any other strides (elements).  Per token,
+ * with z = logits / temperature and p = softmax(z):
+ *
+ *   lse = log sum e^z,  logprob = z_target - lse,  entropy = -sum p log p
+ *   top_logprob, top_index (batch, tokens, top): the top most likely tokens in order
+ *     (of equal logits the lower index first), and their log probabilities
+ *
+ * A target outside the vocabulary (-100, say) names none: logprob 0.  mask: bytes, 0
+ * marks a token whose logits are not read and whose outputs are zero (indices -1);
+ * NULL: none.  top <= 32; vocab < 2^31.
+ *
+ * The backward call writes the logits' gradient (contiguous) for the gradients up,
+ * up_entropy and up_lse (batch, tokens; any strides; NULL: zero) of logprob, entropy
+ * and lse; masked tokens' rows become zero.
+ */
+int da_token_logprobs_workspace(int dtype, int64_t batch, int64_t tokens, int64_t vocab, int top, size_t* bytes);
+int da_token_logprobs(const void* logits, int dtype, int64_t batch, int64_t tokens, int64_t vocab, int64_t l_bstride,
+                      int64_t l_tstride, const int64_t* targets, int64_t t_bstride, int64_t t_tstride,
+                      const uint8_t* mask, int64_t mask_bstride, int64_t mask_tstride, float temperature, int top,
+                      float* logprob, float* entropy, float* lse, float* top_logprob, int64_t* top_index,
+                      void* workspace, size_t workspace_bytes, void* stream);
+int da_token_logprobs_grad(const float* up, int64_t up_bstride, int64_t up_tstride, const float* up_entropy,
+                           int64_t uh_bstride, int64_t uh_tstride, const float* up_lse, int64_t ul_bstride,
+                           int64_t ul_tstride, const void* logits, int dtype, int64_t batch, int64_t tokens,
+                           int64_t vocab, int64_t l_bstride, int64_t l_tstride, const int64_t* targets,
+                           int64_t t_bstride, int64_t t_tstride, const float* lse, const float* entropy,
+                           const uint8_t* mask, int64_t mask_bstride, int64_t mask_tstride, float temperature,
+                           void* grad, void* stream);
+
+/*
  * Lane-layout self test of the MFMA conventions every kernel relies on.
  * shape 32: a and b are (32 x k) row-major with k = 16 (bf16/f16) or 8 (f32),
  *           one 16-byte chunk per lane half; out receives 64 lanes x 16
