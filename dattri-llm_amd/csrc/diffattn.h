@@ -28,16 +28,19 @@ struct Args {
   int causal;
   int64_t q_start;
   float scale;
+  uint32_t g_factor;  // r / G = r g_factor >> g_shift for 0 <= r < 2^31
+  int g_shift;
   char* out;      // (batch, T, Hk G, Dv)
   char* second;   // like out: the second map's values, for the backward pass; NULL: none
   float* lse;     // (batch, Hk, 2, T G): log2 of the exponentials' sums; +inf for a row that sees nothing
-  int splits, split_keys, row_blocks;
-  float* part;    // (splits, batch, Hk, T G, 2, DVP + 2): values, maximum, sum of each part
+  int blocks;     // workgroups of one (batch, key head), apart from splits
+  int splits, each;  // the other side's entries of a split (a whole number of tiles)
+  float* part;    // sums of each split, joined by a second launch
   // backward
   const char* g;
   int64_t g_b, g_t, g_h;
   float* delta;   // (batch, Hk, 2, T G): g . o_m
-  float* most;    // largest |g| of the call (16-bit floats of five exponent bits), NULL: not needed
+  float* most;    // largest |g| of the call (16-bit floats of five exponent bits)
   char *dq, *dk, *dv;
   float* lam_part;  // (batch, heads, chunks)
   int chunk, chunks;
@@ -50,45 +53,28 @@ struct Type {
   static constexpr int kChunks = kTile / kStep;   // chunks of a tile contracted over its rows
 };
 
+__device__ __forceinline__ int token_of(const Args& a, int r) {
+  return (int)((uint64_t)(uint32_t)r * a.g_factor >> a.g_shift);
+}
+
 __device__ __forceinline__ float lam_of(const Args& a, int h) {
   const int64_t at = h * a.lam_stride;
   return a.lam_dtype == DA_F32 ? Elem<DA_F32>::load(a.lam, at)
          : a.lam_dtype == DA_BF16 ? Elem<DA_BF16>::load(a.lam, at) : Elem<DA_F16>::load(a.lam, at);
 }
 
-// Entries e0 .. e0 + V of a row of d entries, from any address; zeros past its end, not read.
+// Entries e0 .. e0 + V of a row of d entries, d a multiple of V.
 template <int DT>
 __device__ __forceinline__ u32x4 load_run(const char* row, int e0, int d) {
-  constexpr int ES = Type<DT>::ES, V = Type<DT>::V;
-  if (e0 + V <= d) return ld16_any<ES>(row + e0 * ES);
-  u32x4 v = {0, 0, 0, 0};
-  if (e0 >= d) return v;
-#pragma unroll
-  for (int e = 0; e < V; ++e) {
-    if (e0 + e >= d) continue;
-    if constexpr (ES == 4) v[e] = *(const uint32_t*)(row + (e0 + e) * 4);
-    else v[e / 2] |= (uint32_t)(*(const uint16_t*)(row + (e0 + e) * 2)) << (16 * (e % 2));
-  }
-  return v;
+  return e0 < d ? ld16(row + e0 * Type<DT>::ES) : u32x4{0, 0, 0, 0};
 }
 
-// Four entries e0 .. e0 + 3 of a row of d, rounded once.
+// Four entries e0 .. e0 + 3 of a row of d, a multiple of four, rounded once.
 template <int DT>
 __device__ __forceinline__ void store4(char* row, int e0, int d, float f0, float f1, float f2, float f3) {
-  constexpr int ES = Type<DT>::ES;
   if (e0 >= d) return;
-  if (e0 + 4 <= d) {
-    if constexpr (ES == 4) {
-      st16_any<4>(row + e0 * 4, u32x4{__float_as_uint(f0), __float_as_uint(f1), __float_as_uint(f2), __float_as_uint(f3)});
-    } else {
-      typedef uint32_t u32x2_at2 __attribute__((ext_vector_type(2), aligned(2)));
-      *(u32x2_at2*)(row + e0 * 2) = u32x2_at2{pack2<DT>(f0, f1), pack2<DT>(f2, f3)};
-    }
-    return;
-  }
-  Elem<DT>::store(row, e0, f0);
-  if (e0 + 1 < d) Elem<DT>::store(row, e0 + 1, f1);
-  if (e0 + 2 < d) Elem<DT>::store(row, e0 + 2, f2);
+  if constexpr (DT == DA_F32) *(f32x4*)(row + e0 * 4) = f32x4{f0, f1, f2, f3};
+  else *(u32x2*)(row + e0 * 2) = u32x2{pack2<DT>(f0, f1), pack2<DT>(f2, f3)};
 }
 
 // Chunk (16 bytes) c of row r of a tile lies at place c ^ swizzle(r) of its row.  Read by
@@ -101,33 +87,66 @@ __device__ __forceinline__ int swizzle(int r) {
   else return r >> 2 & 3;
 }
 
-// A tile of kTile rows of W entries on its way from memory to LDS, over NT threads.
+// A tile of kTile rows of W entries, read straight into LDS by NT threads: 16 bytes a lane,
+// nothing in registers on the way.  A lane's place in LDS is fixed, so the swizzle is in what
+// it reads; a row that takes no part, and entries past d, read as zeros and touch no memory.
+constexpr uint32_t kOutside = 0x80000000u;  // past the range of any buffer here
+
 template <int DT, int W, int NT>
 struct Tile {
   static constexpr int kRow = W * Type<DT>::ES, kPer = kRow / 16, kBytes = kTile * kRow;
   static constexpr int N = kTile * kPer / NT;
   static_assert(N * NT == kTile * kPer, "whole chunks a thread");
-  u32x4 r[N];
-  // row(i): where row i starts, NULL: a row of zeros
-  template <class F>
-  __device__ __forceinline__ void fetch(F row, int d) {
+  __device__ __forceinline__ static int row(int i) { return (threadIdx.x + i * NT) / kPer; }
+  __device__ __forceinline__ static uint32_t column(int i, int d) {  // in bytes
+    const int at = threadIdx.x + i * NT, c = (at % kPer) ^ swizzle<kRow>(at / kPer);
+    return c * Type<DT>::V < d ? c * 16 : kOutside;
+  }
+  __device__ __forceinline__ static void issue(u32x4 rsrc, uint32_t lds, int i, uint32_t offset) {
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x & ~63u);
+    dma16(rsrc, lds + (wave + i * NT) * 16, offset);
+  }
+};
+
+// Tiles of consecutive rows (keys): a lane's offsets are the same in every tile.
+template <int DT, int W, int NT>
+struct Keys : Tile<DT, W, NT> {
+  using T = Tile<DT, W, NT>;
+  uint32_t at[T::N];
+  __device__ __forceinline__ Keys(int64_t stride, int d) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int at = threadIdx.x + i * NT;
-      const char* p = row(at / kPer);
-      r[i] = p ? load_run<DT>(p, at % kPer * Type<DT>::V, d) : u32x4{0, 0, 0, 0};
+    for (int i = 0; i < T::N; ++i) {
+      const uint32_t c = T::column(i, d);
+      at[i] = c == kOutside ? kOutside : (uint32_t)(T::row(i) * stride * Type<DT>::ES) + c;
     }
   }
-  // `live`: a bit a row; the others are stored as zeros, whatever was read
-  __device__ __forceinline__ void put(char* lds, uint32_t live) const {
+  // `base`: the tile's first row; `live`: a bit a row
+  __device__ __forceinline__ void fetch(const char* base, uint32_t lds, uint32_t live) const {
+    const u32x4 rsrc = make_rsrc(base, kOutside - 1);
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int at = threadIdx.x + i * NT, row = at / kPer, c = at % kPer;
-      const uint32_t keep = (live >> row & 1) ? ~0u : 0u;
-      st16(lds + row * kRow + ((c ^ swizzle<kRow>(row)) << 4), r[i] & u32x4{keep, keep, keep, keep});
+    for (int i = 0; i < T::N; ++i) T::issue(rsrc, lds, i, (live >> T::row(i) & 1) ? at[i] : kOutside);
+  }
+};
+
+// Tiles of rows r = t G + g: heads of one token are `head` apart, tokens `token` (bytes).
+template <int DT, int W, int NT>
+struct Rows : Tile<DT, W, NT> {
+  using T = Tile<DT, W, NT>;
+  // `base`: the first head of token t0 = r0 / G
+  __device__ __forceinline__ static void fetch(const Args& a, const char* base, uint32_t lds, int r0, int t0,
+                                               uint32_t token, uint32_t head, int d, uint32_t live) {
+    const u32x4 rsrc = make_rsrc(base, kOutside - 1);
+#pragma unroll
+    for (int i = 0; i < T::N; ++i) {
+      const int row = T::row(i), r = r0 + row, t = token_of(a, r);
+      const uint32_t c = T::column(i, d);
+      const uint32_t at = (uint32_t)(t - t0) * token + (uint32_t)(r - t * a.G) * head + c;
+      T::issue(rsrc, lds, i, (live >> row & 1) && c != kOutside ? at : kOutside);
     }
   }
 };
+
+__device__ __forceinline__ uint32_t lds_address(const char* p) { return (uint32_t)(uintptr_t)(const lds_char*)p; }
 
 // Operand chunk kk of a tile read by rows: lane l has row l % 32, the entries of its half.
 template <int DT, int W>
@@ -182,6 +201,17 @@ __device__ __forceinline__ u32x4 from_acc(const f32x16& x, int j) {
   return v;
 }
 
+// What rounding to operand chunk j left, rounded in turn.
+template <int DT>
+__device__ __forceinline__ u32x4 rest_of(const f32x16& x, int j, u32x4 p) {
+  u32x4 v;
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    v[k] = pack2<DT>(x[8 * j + 2 * k] - Elem<DT>::from_bits(p[k] & 0xffffu),
+                     x[8 * j + 2 * k + 1] - Elem<DT>::from_bits(p[k] >> 16));
+  return v;
+}
+
 // Row r of an accumulator's registers within its tile.
 __device__ __forceinline__ int acc_at(int r, int half) { return 8 * (r >> 2) + 4 * half + (r & 3); }
 
@@ -199,6 +229,24 @@ __device__ __forceinline__ int key_byte(const Args& a, int b, int k0, int end, i
 }
 __device__ __forceinline__ uint32_t key_word(int byte) { return (uint32_t)__ballot(byte != 0); }
 
+// Goes over the tiles that have a live key: their first key, and a bit a key (0: no more).
+struct Live {
+  int key, byte;
+  uint32_t word;
+  __device__ __forceinline__ Live(const Args& a, int b, int first, int end, int lane) {
+    key = first - kTile;
+    byte = key_byte(a, b, first, end, lane);
+    next(a, b, end, lane);
+  }
+  __device__ __forceinline__ void next(const Args& a, int b, int end, int lane) {
+    do {
+      key += kTile;
+      word = key < end ? key_word(byte) : 0;
+      byte = key_byte(a, b, key + kTile, end, lane);
+    } while (!word && key < end);
+  }
+};
+
 // The last key that row r sees (-1: none, also for a row that takes no part).
 __device__ __forceinline__ int last_key(const Args& a, int b, int t) {
   if (t >= a.T || (a.q_mask && !a.q_mask[b * a.qm_b + t * a.qm_t])) return -1;
@@ -212,8 +260,11 @@ __device__ __forceinline__ int last_key(const Args& a, int b, int t) {
 // ---------------------------------------------------------------------------
 int check_sizes(const char* what, int dtype, int64_t batch, int64_t T, int64_t S, int64_t heads, int64_t k_heads,
                 int64_t D, int64_t Dv, int64_t q_start);
-int fill_args(Args& a, const char* what, const da_diff_inputs* in, int64_t batch, int64_t T, int64_t S, int64_t heads,
+int fill_args(Args& a, const char* what, int dtype, const da_diff_inputs* in, int64_t batch, int64_t T, int64_t S, int64_t heads,
               int64_t k_heads, int64_t D, int64_t Dv, float scale, int causal, int64_t q_start);
+// Whether one operand's rows can be read as the kernels do.
+int check_side(const char* what, const char* name, const void* x, int es, int64_t width, int64_t tokens, int64_t heads,
+               int64_t bs, int64_t ts, int64_t hs);
 // Dynamic LDS past 64 KB has to be asked for.
 int allow_lds(const void* kernel, int bytes);
 // The least kernel widths that hold D and Dv: an index of by_widths.

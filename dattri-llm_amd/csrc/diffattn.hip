@@ -4,12 +4,13 @@
 //
 //   out = o_1 - lam_h o_2,   o_m = softmax(scale q_m k_m^T) v     (zero for a row without keys)
 //
-// One pass over the keys: a wave holds 32 rows, with each map's running maximum and sum.
-// It forms the transposed scores, k q^T, so that a row is a lane's (two lanes', 16 keys
-// each) and its maximum and sum stay within them; the accumulator's registers then are,
-// rounded, the second operand of o^T = v^T p^T as they stand, where v is read transposed
-// out of LDS and once for both maps.  The accumulators are rescaled only when a maximum
-// grows by more than 2^8: what is summed meanwhile is at most that much larger.
+// One pass over the keys, a wave to a map: it holds R tiles of 32 rows, with their running
+// maxima and sums.  It forms the transposed scores, k q^T, so that a row is a lane's (two
+// lanes', 16 keys each) and its maximum and sum stay within them; the accumulator's
+// registers then are, rounded, the second operand of o^T = v^T p^T as they stand, where v is
+// read transposed out of LDS.  The accumulators are rescaled only when a maximum grows by
+// more than 2^8: what is summed meanwhile is at most that much larger.  At the end the second
+// map's waves hand their values, divided and weighted, to the first's through LDS.
 #include <algorithm>
 #include <type_traits>
 
@@ -21,33 +22,43 @@ namespace {
 
 constexpr float kSlack = 8.f;  // log2 of how far exponentials may pass 1 before a rescaling
 
-template <int DT, int DP, int DVP, int NW>
+// NG groups of R tiles of rows, each with a wave for either map.
+template <int DT, int DP, int DVP, int R, int NG>
 struct Smem {
-  static constexpr int kK = Tile<DT, DP, NW * kWave>::kBytes, kV = Tile<DT, DVP, NW * kWave>::kBytes;
-  static constexpr int kStage = 2 * kK + kV;
-  static constexpr int kBytes = 2 * kStage;
+  static constexpr int NT = 2 * NG * kWave;
+  static constexpr int kK = Tile<DT, DP, NT>::kBytes, kV = Tile<DT, DVP, NT>::kBytes;
+  static constexpr int kStage = 2 * kK + kV, kHanded = NG * DVP / 32 * 4096;
+  static constexpr int kBytes = 2 * kStage > kHanded ? 2 * kStage : kHanded;
 };
 
-template <int DT, int DP, int DVP, int NW>
-__global__ __launch_bounds__(NW * kWave) void diff_forward(Args a) {
-  using L = Smem<DT, DP, DVP, NW>;
-  constexpr int NT = NW * kWave, ES = Type<DT>::ES, V = Type<DT>::V;
+// kFine: probabilities as the sum of two 16-bit values.  Where a token's few rows leave the
+// matrix units idle that costs nothing, and the values are rounded once, at the end.
+template <int DT, int DP, int DVP, int R, int NG, bool kFine>
+__global__ __launch_bounds__(2 * NG * kWave, 2) void diff_forward(Args a) {
+  using L = Smem<DT, DP, DVP, R, NG>;
+  constexpr int NT = L::NT, ES = Type<DT>::ES, V = Type<DT>::V;
   constexpr int KD = DP / Type<DT>::kStep, NB = DVP / 32, KC = Type<DT>::kChunks;
   extern __shared__ __attribute__((aligned(16))) char lds[];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
-  // Workgroups of one key head are neighbours; the rows with the most keys go first.
-  int at = blockIdx.x;
-  const int block = a.row_blocks - 1 - at % a.row_blocks;
-  at /= a.row_blocks;
+  const int lane = threadIdx.x & 63, half = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), map = wave & 1, group = wave >> 1;
+  // Workgroups of one key head are neighbours on one die; the rows with the most keys go first.
+  int at = (int)xcd_remap(blockIdx.x, gridDim.x);
+  const int block = a.blocks - 1 - at % a.blocks;
+  at /= a.blocks;
   const int split = at % a.splits;
   at /= a.splits;
   const int hk = at % a.Hk, b = at / a.Hk;
   const int rows = a.T * a.G;
-  const int r = (block * NW + wave) * kTile + (lane & 31);
-  const int t = r / a.G, h = hk * a.G + (r - t * a.G);
-  const int last = r < rows ? last_key(a, b, t) : -1;
-  // The wave's and the workgroup's ranges of keys: rows come in order, so the last one sees most.
-  int most = last, least = last;
+  int r[R], t[R], h[R], last[R], most = -1, least = a.S;
+#pragma unroll
+  for (int n = 0; n < R; ++n) {
+    r[n] = ((block * NG + group) * R + n) * kTile + (lane & 31);
+    t[n] = token_of(a, r[n]);
+    h[n] = hk * a.G + (r[n] - t[n] * a.G);
+    last[n] = r[n] < rows ? last_key(a, b, t[n]) : -1;
+    most = max(most, last[n]);
+    least = min(least, last[n]);
+  }
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) {
     most = max(most, __shfl_xor(most, off, kWave));
@@ -56,153 +67,162 @@ __global__ __launch_bounds__(NW * kWave) void diff_forward(Args a) {
   most = __builtin_amdgcn_readfirstlane(most);
   least = __builtin_amdgcn_readfirstlane(least);
   int end = a.S;
-  if (a.causal) {
-    const int64_t t_last = min((block + 1) * NW * kTile, rows) - 1;
-    end = (int)max((int64_t)0, min((int64_t)a.S, t_last / a.G + a.q_start + 1));
+  if (a.causal) {  // rows come in order: the workgroup's last one sees most
+    const int64_t t_last = (min((block + 1) * NG * R * kTile, rows) - 1) / a.G;
+    end = (int)max((int64_t)0, min((int64_t)a.S, t_last + a.q_start + 1));
   }
-  const int first = split * a.split_keys;
-  end = min(end, first + a.split_keys);
+  int key = split * a.each;
+  end = min(end, key + a.each);
 
-  u32x4 q[2][KD];
+  u32x4 q[R][KD];
 #pragma unroll
-  for (int m = 0; m < 2; ++m)
+  for (int n = 0; n < R; ++n)
 #pragma unroll
-    for (int kk = 0; kk < KD; ++kk) {
-      q[m][kk] = u32x4{0, 0, 0, 0};
-      if (last >= 0)
-        q[m][kk] = load_run<DT>(a.q + (b * a.q_b + t * a.q_t + (2 * h + m) * a.q_h) * ES, (2 * kk + half) * V, a.D);
-    }
+    for (int kk = 0; kk < KD; ++kk)
+      q[n][kk] = last[n] >= 0
+          ? load_run<DT>(a.q + (b * a.q_b + t[n] * a.q_t + (2 * h[n] + map) * a.q_h) * ES, (2 * kk + half) * V, a.D)
+          : u32x4{0, 0, 0, 0};
 
-  Tile<DT, DP, NT> k0, k1;
-  Tile<DT, DVP, NT> v;
+  const Keys<DT, DP, NT> keys(a.k_t, a.D);
+  const Keys<DT, DVP, NT> values(a.v_t, a.Dv);
   const char* kp = a.k + (b * a.k_b + 2 * hk * a.k_h) * ES;
   const char* vp = a.v + (b * a.v_b + hk * a.v_h) * ES;
-  auto fetch = [&](int key) {
-    k0.fetch([&](int i) { return key + i < end ? kp + (key + i) * a.k_t * ES : nullptr; }, a.D);
-    k1.fetch([&](int i) { return key + i < end ? kp + ((key + i) * a.k_t + a.k_h) * ES : nullptr; }, a.D);
-    v.fetch([&](int i) { return key + i < end ? vp + (key + i) * a.v_t * ES : nullptr; }, a.Dv);
+  auto fetch = [&](int to, int stage, uint32_t live) {
+    const uint32_t l = lds_address(lds) + stage * L::kStage;
+    keys.fetch(kp + to * a.k_t * ES, l, live);
+    keys.fetch(kp + (to * a.k_t + a.k_h) * ES, l + L::kK, live);
+    values.fetch(vp + to * a.v_t * ES, l + 2 * L::kK, live);
   };
 
   const float c = a.scale * kLog2e;
-  f32x16 o[2][NB];
-  float top[2] = {kLowest, kLowest}, sum[2] = {0.f, 0.f};
+  f32x16 o[R][NB];
+  float top[R], sum[R];
 #pragma unroll
-  for (int m = 0; m < 2; ++m)
+  for (int n = 0; n < R; ++n) {
+    top[n] = kLowest, sum[n] = 0.f;
 #pragma unroll
-    for (int n = 0; n < NB; ++n) o[m][n] = zeros();
+    for (int x = 0; x < NB; ++x) o[n][x] = zeros();
+  }
 
-  // Two tiles are under way: the words of live keys one ahead of their tiles, so that a
-  // tile without any is not read.
-  uint32_t word = first < end ? key_word(key_byte(a, b, first, end, lane)) : 0;
-  int byte = key_byte(a, b, first + kTile, end, lane);
-  if (word) fetch(first);
-  int stage = 0;
-  for (int key = first; key < end; key += kTile) {
-    char* lk = lds + stage * L::kStage;
-    const uint32_t live = word;
-    if (live) {
-      k0.put(lk, live);
-      k1.put(lk + L::kK, live);
-      v.put(lk + 2 * L::kK, live);
-    }
-    word = key_word(byte);
-    if (word) fetch(key + kTile);
-    byte = key_byte(a, b, key + 2 * kTile, end, lane);
-    if (!live) continue;
+  // The next tile with a live key is on its way while one is multiplied.
+  Live live(a, b, key, end, lane);
+  if (live.word) fetch(live.key, 0, live.word);
+  for (int stage = 0; live.word; stage ^= 1) {
+    key = live.key;
+    const uint32_t word = live.word;
+    live.next(a, b, end, lane);
     __syncthreads();
-    stage ^= 1;
+    if (live.word) fetch(live.key, stage ^ 1, live.word);
     if (key > most) continue;
-    const char* lv = lk + 2 * L::kK;
-    f32x16 s[2];
+    const char* lk = lds + stage * L::kStage + map * L::kK;
+    const char* lv = lds + stage * L::kStage + 2 * L::kK;
+    f32x16 s[R];
 #pragma unroll
-    for (int m = 0; m < 2; ++m) {
-      s[m] = zeros();
+    for (int n = 0; n < R; ++n) s[n] = zeros();
 #pragma unroll
-      for (int kk = 0; kk < KD; ++kk) Mfma32<DT>::mma(s[m], by_rows<DT, DP>(lk + m * L::kK, kk, lane), q[m][kk]);
+    for (int kk = 0; kk < KD; ++kk) {
+      const u32x4 x = by_rows<DT, DP>(lk, kk, lane);
+#pragma unroll
+      for (int n = 0; n < R; ++n) Mfma32<DT>::mma(s[n], x, q[n][kk]);
     }
-    if (live != ~0u || key + kTile - 1 > least) {
+    if (word != ~0u || key + kTile - 1 > least) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int x = acc_at(i, half);
-        const bool seen = key + x <= last && (live >> x & 1);
-        s[0][i] = seen ? s[0][i] : -__builtin_inff();
-        s[1][i] = seen ? s[1][i] : -__builtin_inff();
-      }
+      for (int n = 0; n < R; ++n)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int x = acc_at(i, half);
+          s[n][i] = key + x <= last[n] && (word >> x & 1) ? s[n][i] : -__builtin_inff();
+        }
     }
 #pragma unroll
-    for (int m = 0; m < 2; ++m) {
-      float x = s[m][0];
+    for (int n = 0; n < R; ++n) {
+      float x = s[n][0];
 #pragma unroll
-      for (int i = 1; i < 16; ++i) x = fmaxf(x, s[m][i]);
+      for (int i = 1; i < 16; ++i) x = fmaxf(x, s[n][i]);
       x = fmaxf(x, __shfl_xor(x, 32, kWave)) * c;
-      if (__any(x > top[m] + kSlack)) {  // kLowest + 8 is kLowest
-        const float now = fmaxf(top[m], x), by = __builtin_amdgcn_exp2f(top[m] - now);
-        top[m] = now;
-        sum[m] *= by;
+      if (__any(x > top[n] + kSlack)) {  // kLowest + 8 is kLowest
+        const float now = fmaxf(top[n], x), by = __builtin_amdgcn_exp2f(top[n] - now);
+        top[n] = now;
+        sum[n] *= by;
 #pragma unroll
-        for (int n = 0; n < NB; ++n)
+        for (int y = 0; y < NB; ++y)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) o[m][n][i] *= by;
+          for (int i = 0; i < 16; ++i) o[n][y][i] *= by;
       }
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        s[m][i] = __builtin_amdgcn_exp2f(fmaf(s[m][i], c, -top[m]));
-        sum[m] += s[m][i];
+        s[n][i] = __builtin_amdgcn_exp2f(fmaf(s[n][i], c, -top[n]));
+        sum[n] += s[n][i];
       }
     }
 #pragma unroll
     for (int j = 0; j < KC; ++j) {
-      const u32x4 p0 = from_acc<DT>(s[0], j), p1 = from_acc<DT>(s[1], j);
+      u32x4 p[R], rest[R];
 #pragma unroll
-      for (int n = 0; n < NB; ++n) {
-        const u32x4 x = by_columns<DT, DVP>(lv, n, j, lane);
-        Mfma32<DT>::mma(o[0][n], x, p0);
-        Mfma32<DT>::mma(o[1][n], x, p1);
+      for (int n = 0; n < R; ++n) {
+        p[n] = from_acc<DT>(s[n], j);
+        if constexpr (kFine) rest[n] = rest_of<DT>(s[n], j, p[n]);
+      }
+#pragma unroll
+      for (int y = 0; y < NB; ++y) {
+        const u32x4 x = by_columns<DT, DVP>(lv, y, j, lane);
+#pragma unroll
+        for (int n = 0; n < R; ++n) {
+          Mfma32<DT>::mma(o[n][y], x, p[n]);
+          if constexpr (kFine) Mfma32<DT>::mma(o[n][y], x, rest[n]);
+        }
       }
     }
   }
 
-  if (a.splits > 1) {  // this part's sums: joined by a second launch
-    if (r >= rows) return;
-    sum[0] += __shfl_xor(sum[0], 32, kWave);
-    sum[1] += __shfl_xor(sum[1], 32, kWave);
-    float* to = a.part + ((((int64_t)split * a.batch + b) * a.Hk + hk) * rows + r) * 2 * (DVP + 2);
 #pragma unroll
-    for (int m = 0; m < 2; ++m) {
+  for (int n = 0; n < R; ++n) sum[n] += __shfl_xor(sum[n], 32, kWave);
+  if (a.splits > 1) {  // this split's sums
 #pragma unroll
-      for (int n = 0; n < NB; ++n)
+    for (int n = 0; n < R; ++n) {
+      if (r[n] >= rows) continue;
+      float* to = a.part + ((((int64_t)split * a.batch + b) * a.Hk + hk) * rows + r[n]) * 2 * (DVP + 2);
+#pragma unroll
+      for (int y = 0; y < NB; ++y)
 #pragma unroll
         for (int i = 0; i < 16; i += 4)
-          *(f32x4*)(to + m * DVP + 32 * n + acc_at(i, half)) =
-              f32x4{o[m][n][i], o[m][n][i + 1], o[m][n][i + 2], o[m][n][i + 3]};
-      if (half == 0) to[2 * DVP + 2 * m] = top[m], to[2 * DVP + 2 * m + 1] = sum[m];
+          *(f32x4*)(to + map * DVP + 32 * y + acc_at(i, half)) =
+              f32x4{o[n][y][i], o[n][y][i + 1], o[n][y][i + 2], o[n][y][i + 3]};
+      if (half == 0) to[2 * DVP + 2 * map] = top[n], to[2 * DVP + 2 * map + 1] = sum[n];
     }
     return;
   }
-  sum[0] += __shfl_xor(sum[0], 32, kWave);
-  sum[1] += __shfl_xor(sum[1], 32, kWave);
-  if (r >= rows) return;
-  const float by0 = sum[0] > 0.f ? 1.f / sum[0] : 0.f, by1 = sum[1] > 0.f ? 1.f / sum[1] : 0.f;
-  const float by2 = by1 != 0.f ? lam_of(a, h) * by1 : 0.f;
-  const int64_t to = ((int64_t)b * a.T + t) * (a.Hk * a.G) + h;
+  f32x4* handed = (f32x4*)(lds + group * (L::kHanded / NG));
 #pragma unroll
-  for (int n = 0; n < NB; ++n)
+  for (int n = 0; n < R; ++n) {
+    const bool in = r[n] < rows;
+    const float by = sum[n] > 0.f ? 1.f / sum[n] : 0.f;
+    const int64_t to = (((int64_t)b * a.T + t[n]) * (a.Hk * a.G) + h[n]) * a.Dv * ES;
+    if (a.lse && half == 0 && in)
+      a.lse[(((int64_t)b * a.Hk + hk) * 2 + map) * rows + r[n]] = sum[n] > 0.f ? top[n] + log2f(sum[n]) : __builtin_inff();
+    __syncthreads();  // the tiles, and what was handed before, have been read
+    if (map) {
+      const float lam = in && by != 0.f ? lam_of(a, h[n]) : 0.f;
 #pragma unroll
-    for (int i = 0; i < 16; i += 4) {
-      const int e = 32 * n + acc_at(i, half);
-      float f[4], g[4];
+      for (int y = 0; y < NB; ++y)
 #pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        f[x] = o[0][n][i + x] * by0 - o[1][n][i + x] * by2;
-        g[x] = o[1][n][i + x] * by1;
-      }
-      store4<DT>(a.out + to * a.Dv * ES, e, a.Dv, f[0], f[1], f[2], f[3]);
-      if (a.second) store4<DT>(a.second + to * a.Dv * ES, e, a.Dv, g[0], g[1], g[2], g[3]);
+        for (int i = 0; i < 16; i += 4) {
+          const f32x4 v = f32x4{o[n][y][i], o[n][y][i + 1], o[n][y][i + 2], o[n][y][i + 3]} * by;
+          if (a.second && in) store4<DT>(a.second + to, 32 * y + acc_at(i, half), a.Dv, v[0], v[1], v[2], v[3]);
+          handed[(y * 4 + i / 4) * kWave + lane] = v * lam;
+        }
     }
-  if (a.lse && half == 0) {
-    float* lse = a.lse + ((int64_t)b * a.Hk + hk) * 2 * rows + r;
-    lse[0] = sum[0] > 0.f ? top[0] + log2f(sum[0]) : __builtin_inff();
-    lse[rows] = sum[1] > 0.f ? top[1] + log2f(sum[1]) : __builtin_inff();
+    __syncthreads();
+    if (!map && in) {
+#pragma unroll
+      for (int y = 0; y < NB; ++y)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+          const f32x4 v = handed[(y * 4 + i / 4) * kWave + lane];
+          store4<DT>(a.out + to, 32 * y + acc_at(i, half), a.Dv, o[n][y][i] * by - v[0], o[n][y][i + 1] * by - v[1],
+                     o[n][y][i + 2] * by - v[2], o[n][y][i + 3] * by - v[3]);
+        }
+    }
   }
 }
 
@@ -265,10 +285,29 @@ int check_sizes(const char* what, int dtype, int64_t batch, int64_t T, int64_t S
   return DA_OK;
 }
 
-int fill_args(Args& a, const char* what, const da_diff_inputs* in, int64_t batch, int64_t T, int64_t S, int64_t heads,
+// Rows are read in runs of 16 bytes, and a tile's by 31-bit offsets from its first row.
+int check_side(const char* what, const char* name, const void* x, int es, int64_t width, int64_t tokens,
+                      int64_t heads, int64_t bs, int64_t ts, int64_t hs) {
+  if (!x) return DA_OK;
+  const int64_t most = int64_t{1} << 31;
+  if (((uintptr_t)x | (uint64_t)(bs * es) | (uint64_t)(ts * es) | (uint64_t)(hs * es) | (uint64_t)(width * es)) & 15)
+    return set_error(DA_ERR_INVALID, "%s: rows of %s must be whole 16-byte runs at 16-byte aligned addresses", what, name);
+  if (bs < 0 || ts < 0 || hs < 0) return set_error(DA_ERR_INVALID, "%s: negative stride of %s", what, name);
+  if (ts >= most || hs >= most || (std::min<int64_t>(tokens, kTile + 1) * ts + heads * hs + width) * es >= most)
+    return set_error(DA_ERR_UNSUPPORTED, "%s: tokens of %s lie too far apart", what, name);
+  return DA_OK;
+}
+
+int fill_args(Args& a, const char* what, int dtype, const da_diff_inputs* in, int64_t batch, int64_t T, int64_t S, int64_t heads,
               int64_t k_heads, int64_t D, int64_t Dv, float scale, int causal, int64_t q_start) {
   if (!valid_dtype((int)in->lam_dtype)) return set_error(DA_ERR_INVALID, "%s: bad dtype %d", what, (int)in->lam_dtype);
   if (!(scale > 0.f) || !(scale < 1e30f)) return set_error(DA_ERR_INVALID, "%s: the scale must be positive", what);
+  const int es = (int)elem_bytes(dtype);
+  const int64_t group = heads / k_heads;
+  int rc = check_side(what, "q", in->q, es, D, T, 2 * group, in->q_bstride, in->q_tstride, in->q_hstride);
+  if (rc == DA_OK) rc = check_side(what, "k", in->k, es, D, S, 2, in->k_bstride, in->k_tstride, in->k_hstride);
+  if (rc == DA_OK) rc = check_side(what, "v", in->v, es, Dv, S, 1, in->v_bstride, in->v_tstride, in->v_hstride);
+  if (rc) return rc;
   a.q = (const char*)in->q, a.k = (const char*)in->k, a.v = (const char*)in->v;
   a.lam = in->lam, a.lam_dtype = (int)in->lam_dtype, a.lam_stride = in->lam_stride;
   a.mask = in->mask, a.q_mask = in->q_mask;
@@ -277,6 +316,10 @@ int fill_args(Args& a, const char* what, const da_diff_inputs* in, int64_t batch
   a.v_b = in->v_bstride, a.v_t = in->v_tstride, a.v_h = in->v_hstride;
   a.m_b = in->mask_bstride, a.m_k = in->mask_kstride, a.qm_b = in->q_mask_bstride, a.qm_t = in->q_mask_tstride;
   a.batch = (int)batch, a.T = (int)T, a.S = (int)S, a.Hk = (int)k_heads, a.G = (int)(heads / k_heads);
+  int bits = 0;
+  while ((1 << bits) < a.G) ++bits;
+  a.g_factor = (uint32_t)(((uint64_t{1} << (31 + bits)) + a.G - 1) / a.G);
+  a.g_shift = 31 + bits;
   a.D = (int)D, a.Dv = (int)Dv, a.causal = causal, a.q_start = q_start, a.scale = scale;
   return DA_OK;
 }
@@ -289,25 +332,31 @@ int allow_lds(const void* kernel, int bytes) {
 
 namespace {
 
-// One wave a workgroup where there are no more rows than it takes, and a tile of keys and
-// values fits its registers on the way (16 KB: 64 a lane).
-int waves_of(int64_t rows, int dtype, int w) { return rows <= kTile && dtype != DA_F32 && w < 2 ? 1 : 4; }
+// How rows are shared out: R tiles a wave and NG groups a workgroup.
+struct Shape {
+  int r, ng;
+};
 
-// Keys are split where the rows alone leave CUs without work: about eight waves' worth of
-// workgroups a CU, no part under 256 keys.
-int split_of(int dtype, int w, int64_t batch, int64_t T, int64_t S, int64_t k_heads, int64_t G, int* blocks, int* splits, int* keys) {
+// Few rows: a tile a workgroup.  Else two groups; 16-bit maps of up to 64 entries have room
+// for two tiles a wave, which halves what is read from LDS a product.
+int plan(int dtype, int w, int64_t batch, int64_t T, int64_t S, int64_t k_heads, int64_t G, Shape* shape, Args* a) {
   int64_t cus;
   const int rc = device_cu_count(&cus);
   if (rc) return rc;
-  const int64_t rows = T * G, nw = waves_of(rows, dtype, w);
-  const int64_t n = (rows + nw * kTile - 1) / (nw * kTile), groups = batch * k_heads * n;
-  int64_t want = groups >= cus ? 1 : (nw == 1 ? 8 : 2) * cus / std::max<int64_t>(groups, 1);
-  if (nw == 1 && groups >= cus) want = 8 * cus / groups;
-  want = std::max<int64_t>(1, std::min<int64_t>(want, S / 256));
-  const int64_t each = ((S + want - 1) / want + kTile - 1) / kTile * kTile;
-  *blocks = (int)n;
-  *keys = (int)std::max<int64_t>(each, kTile);
-  *splits = (int)std::max<int64_t>(1, (S + *keys - 1) / *keys);
+  const int64_t rows = T * G, heads = batch * k_heads;
+  const auto blocks_of = [&](int64_t n) { return (rows + n * kTile - 1) / (n * kTile); };
+  *shape = {1, 1};
+  if (dtype != DA_F32 && w < 2 && heads * blocks_of(4) >= 2 * cus) *shape = {2, 2};
+  else if (heads * blocks_of(2) >= 2 * cus) *shape = {1, 2};
+  const int64_t blocks = blocks_of(shape->r * shape->ng), groups = std::max<int64_t>(1, heads * blocks);
+  // Keys are split where the rows leave CUs without work: up to eight workgroups a CU, no
+  // split under 256 keys.
+  int64_t want = shape->ng == 1 ? std::max<int64_t>(1, 8 * cus / groups) : 1;
+  want = std::max<int64_t>(1, std::min(want, S / 256));
+  const int64_t each = std::max<int64_t>(kTile, ((S + want - 1) / want + kTile - 1) / kTile * kTile);
+  a->blocks = (int)blocks;
+  a->each = (int)each;
+  a->splits = (int)std::max<int64_t>(1, (S + each - 1) / each);
   return DA_OK;
 }
 
@@ -331,9 +380,10 @@ int da_diff_attention_workspace(int dtype, int64_t batch, int64_t q_len, int64_t
   *bytes = 0;
   int rc = check_sizes("da_diff_attention_workspace", dtype, batch, q_len, k_len, heads, k_heads, d, dv, 0);
   if (rc || batch == 0 || q_len == 0) return rc;
-  int blocks, splits, keys;
-  rc = split_of(dtype, widths(d, dv), batch, q_len, k_len, k_heads, heads / k_heads, &blocks, &splits, &keys);
-  if (rc == DA_OK) *bytes = workspace_of(batch, q_len * (heads / k_heads), k_heads, splits, widths(d, dv));
+  Shape shape;
+  Args a;
+  rc = plan(dtype, widths(d, dv), batch, q_len, k_len, k_heads, heads / k_heads, &shape, &a);
+  if (rc == DA_OK) *bytes = workspace_of(batch, q_len * (heads / k_heads), k_heads, a.splits, widths(d, dv));
   return rc;
 }
 
@@ -348,11 +398,12 @@ int da_diff_attention(const da_diff_inputs* in, int dtype, int64_t batch, int64_
   if (!in || !in->q || !in->lam || !out || (k_len && (!in->k || !in->v)) || !second != !lse)
     return set_error(DA_ERR_INVALID, "da_diff_attention: NULL pointer");
   Args a = {};
-  rc = fill_args(a, "da_diff_attention", in, batch, q_len, k_len, heads, k_heads, d, dv, scale, causal, q_start);
+  rc = fill_args(a, "da_diff_attention", dtype, in, batch, q_len, k_len, heads, k_heads, d, dv, scale, causal, q_start);
   if (rc) return rc;
   a.out = (char*)out, a.second = (char*)second, a.lse = lse;
   const int w = widths(d, dv);
-  rc = split_of(dtype, w, batch, q_len, k_len, k_heads, a.G, &a.row_blocks, &a.splits, &a.split_keys);
+  Shape shape;
+  rc = plan(dtype, w, batch, q_len, k_len, k_heads, a.G, &shape, &a);
   if (rc) return rc;
   const int64_t rows = q_len * a.G;
   const size_t need = workspace_of(batch, rows, k_heads, a.splits, w);
@@ -360,21 +411,29 @@ int da_diff_attention(const da_diff_inputs* in, int dtype, int64_t batch, int64_
     return set_error(DA_ERR_WORKSPACE, "da_diff_attention: workspace of %zu bytes needed", need);
   if ((uintptr_t)workspace % 16) return set_error(DA_ERR_INVALID, "da_diff_attention: workspace must be 16-byte aligned");
   a.part = (float*)workspace;
-  if (batch * k_heads > kMaxBlocks / a.splits / a.row_blocks)
+  if (batch * k_heads > kMaxBlocks / a.splits / a.blocks)
     return set_error(DA_ERR_UNSUPPORTED, "da_diff_attention: too many rows");
-  const unsigned grid = (unsigned)(batch * k_heads * a.splits * a.row_blocks);
+  const unsigned grid = (unsigned)(batch * k_heads * a.splits * a.blocks);
   const hipStream_t st = (hipStream_t)stream;
-  const bool one = waves_of(rows, dtype, w) == 1;
   return by_widths(dtype, w, [&](auto dt, auto dp, auto dvp) {
     constexpr int DT = decltype(dt)::value, DP = decltype(dp)::value, DVP = decltype(dvp)::value;
-    if constexpr (DT != DA_F32 && DP == 64) {
-      if (one) diff_forward<DT, DP, DVP, 1><<<grid, 64, Smem<DT, DP, DVP, 1>::kBytes, st>>>(a);
-    }
-    if (!one) {
-      constexpr int kBytes = Smem<DT, DP, DVP, 4>::kBytes;
-      if (const int err = allow_lds((const void*)diff_forward<DT, DP, DVP, 4>, kBytes)) return err;
-      diff_forward<DT, DP, DVP, 4><<<grid, 256, kBytes, st>>>(a);
-    }
+    const auto launch = [&](auto tiles, auto groups) {
+      constexpr int R = decltype(tiles)::value, NG = decltype(groups)::value;
+      constexpr bool kFine = DT != DA_F32 && NG == 1;
+      constexpr int kBytes = Smem<DT, DP, DVP, R, NG>::kBytes;
+      const auto kernel = diff_forward<DT, DP, DVP, R, NG, kFine>;
+      if (const int err = allow_lds((const void*)kernel, kBytes)) return err;
+      kernel<<<grid, 2 * NG * kWave, kBytes, st>>>(a);
+      return (int)DA_OK;
+    };
+    using One = std::integral_constant<int, 1>;
+    using Two = std::integral_constant<int, 2>;
+    int err = DA_OK;
+    if (shape.ng == 1) err = launch(One{}, One{});
+    else if (shape.r == 1) err = launch(One{}, Two{});
+    if constexpr (DT != DA_F32 && DP == 64)
+      if (shape.r == 2) err = launch(Two{}, Two{});
+    if (err) return err;
     if (a.splits > 1) {
       constexpr int kRows = 256 / (DVP / 4);
       const int64_t all = batch * k_heads * rows;

@@ -98,32 +98,36 @@ __device__ __forceinline__ float small_scale(const Args& a) {
 }
 
 // ---------------------------------------------------------------------------
-// dk and dv: four waves of 32 keys over all rows r = t G + g of their key head.
+// dk and dv: four waves of 32 keys over the rows r = t G + g of their key head.
 // ---------------------------------------------------------------------------
-constexpr int kKeyWaves = 4;
+constexpr int kWaves = 4, kThreads = kWaves * kWave;
 
 template <int DT, int DP, int DVP>
 struct KeySmem {
-  static constexpr int NT = kKeyWaves * kWave;
-  static constexpr int kQ = Tile<DT, DP, NT>::kBytes, kG = Tile<DT, DVP, NT>::kBytes;
-  static constexpr int kRow = 6 * kTile * 4;  // of each row: lse, delta of both maps, lam, the last key
+  static constexpr int kQ = Tile<DT, DP, kThreads>::kBytes, kG = Tile<DT, DVP, kThreads>::kBytes;
+  static constexpr int kRow = 5 * kTile * 4;  // of each row: lse and delta of both maps, the last key
   static constexpr int kStage = 2 * kQ + kG + kRow;
   static constexpr int kBytes = 2 * kStage;
 };
 
 template <int DT, int DP, int DVP>
-__global__ __launch_bounds__(kKeyWaves * kWave) void diff_grad_keys(Args a) {
+__global__ __launch_bounds__(kThreads) void diff_grad_keys(Args a) {
   using L = KeySmem<DT, DP, DVP>;
-  constexpr int NT = L::NT, ES = Type<DT>::ES, V = Type<DT>::V;
+  constexpr int ES = Type<DT>::ES, V = Type<DT>::V;
   constexpr int KD = DP / Type<DT>::kStep, KV = DVP / Type<DT>::kStep, KC = Type<DT>::kChunks;
   constexpr int ND = DP / 32, NV = DVP / 32;
   extern __shared__ __attribute__((aligned(16))) char lds[];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
-  const int blocks = (a.S + kKeyWaves * kTile - 1) / (kKeyWaves * kTile);
-  const int block = blockIdx.x % blocks, hk = blockIdx.x / blocks % a.Hk, b = blockIdx.x / blocks / a.Hk;
-  const int key0 = (block * kKeyWaves + wave) * kTile, key = key0 + (lane & 31);
+  const int lane = threadIdx.x & 63, half = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int at = (int)xcd_remap(blockIdx.x, gridDim.x);
+  const int block = at % a.blocks;  // the first keys have the most rows
+  at /= a.blocks;
+  const int split = at % a.splits;
+  at /= a.splits;
+  const int hk = at % a.Hk, b = at / a.Hk;
+  const int key0 = (block * kWaves + wave) * kTile, key = key0 + (lane & 31);
   const bool alive = key < a.S && (!a.mask || a.mask[b * a.m_b + key * a.m_k]);
-  const int rows = a.T * a.G;
+  const int rows = a.T * a.G, end = min(rows, (split + 1) * a.each);
   u32x4 k[2][KD], v[KV];
 #pragma unroll
   for (int kk = 0; kk < KD; ++kk)
@@ -136,7 +140,6 @@ __global__ __launch_bounds__(kKeyWaves * kWave) void diff_grad_keys(Args a) {
     v[kk] = alive ? load_run<DT>(a.v + (b * a.v_b + key * a.v_t + hk * a.v_h) * ES, (2 * kk + half) * V, a.Dv)
                   : u32x4{0, 0, 0, 0};
   const bool work = __any(alive);
-  const bool whole = __all(alive);
   f32x16 dk[2][ND], dv[NV];
 #pragma unroll
   for (int n = 0; n < ND; ++n) dk[0][n] = zeros(), dk[1][n] = zeros();
@@ -144,48 +147,64 @@ __global__ __launch_bounds__(kKeyWaves * kWave) void diff_grad_keys(Args a) {
   for (int n = 0; n < NV; ++n) dv[n] = zeros();
   const float c = a.scale * kLog2e, small = small_scale<DT>(a);
 
-  Tile<DT, DP, NT> q0, q1;
-  Tile<DT, DVP, NT> g;
-  float row_value = 0.f;
-  // One value of a row a thread: 32 rows of lse and delta of both maps, lam, the last key.
-  const int what = threadIdx.x / kTile, which = threadIdx.x % kTile;
-  auto fetch = [&](int r0) {
-    auto place = [&](int i, int64_t st, int64_t sh, int maps) -> int64_t {
-      const int r = r0 + i, t = r / a.G;
-      if (r >= rows || (a.q_mask && !a.q_mask[b * a.qm_b + t * a.qm_t])) return -1;
-      return b * (maps == 2 ? a.q_b : a.g_b) + t * st + (int64_t)(hk * a.G + r - t * a.G) * maps * sh;
-    };
-    q0.fetch([&](int i) { const int64_t at = place(i, a.q_t, a.q_h, 2); return at < 0 ? nullptr : a.q + at * ES; }, a.D);
-    q1.fetch([&](int i) { const int64_t at = place(i, a.q_t, a.q_h, 2); return at < 0 ? nullptr : a.q + (at + a.q_h) * ES; },
-             a.D);
-    g.fetch([&](int i) { const int64_t at = place(i, a.g_t, a.g_h, 1); return at < 0 ? nullptr : a.g + at * ES; }, a.Dv);
-    const int r = r0 + which;
-    const int64_t base = ((int64_t)b * a.Hk + hk) * 2 * rows;
-    if (what < 2) row_value = r < rows ? a.lse[base + what * rows + r] : __builtin_inff();
-    else if (what < 4) row_value = r < rows ? a.delta[base + (what - 2) * rows + r] : 0.f;
-    else if (what == 4) row_value = r < rows ? lam_of(a, hk * a.G + r % a.G) : 0.f;
-    else if (what == 5) row_value = __int_as_float(r < rows ? last_key(a, b, r / a.G) : -1);
-  };
   // The first row that sees the workgroup's first key.
-  int first = 0;
+  int first = split * a.each;
   if (a.causal) {
-    const int64_t t = (int64_t)block * kKeyWaves * kTile - a.q_start;
-    first = t <= 0 ? 0 : t >= a.T ? rows : (int)t * a.G / kTile * kTile;
+    const int64_t t = (int64_t)block * kWaves * kTile - a.q_start;
+    if (t > 0) first = max(first, t >= a.T ? end : (int)t * a.G / kTile * kTile);
   }
-  if (first < rows) fetch(first);
+  const uint32_t q_token = (uint32_t)(a.q_t * ES), q_head = (uint32_t)(2 * a.q_h * ES);
+  const uint32_t g_token = (uint32_t)(a.g_t * ES), g_head = (uint32_t)(a.g_h * ES);
+  const char* qp = a.q + (b * a.q_b + (int64_t)2 * hk * a.G * a.q_h) * ES;
+  const char* gp = a.g + (b * a.g_b + (int64_t)hk * a.G * a.g_h) * ES;
+  const float* lse = a.lse + ((int64_t)b * a.Hk + hk) * 2 * rows;
+  const float* delta = a.delta + ((int64_t)b * a.Hk + hk) * 2 * rows;
+  // A value of a row a thread: lse and delta of both maps, the last key.
+  const int what = threadIdx.x / kTile, which = threadIdx.x % kTile;
+  float value = 0.f, lam = 0.f;  // lam: every wave's lanes have the tile's 32 rows
+  int byte = 0;
+  auto row_byte = [&](int r0) {
+    const int r = r0 + (lane & 31);
+    return r < end ? (a.q_mask ? a.q_mask[b * a.qm_b + token_of(a, r) * a.qm_t] : 1) : 0;
+  };
+  auto fetch = [&](int r0, int stage, uint32_t live) {
+    const int t0 = token_of(a, r0);
+    const uint32_t l = lds_address(lds) + stage * L::kStage;
+    Rows<DT, DP, kThreads>::fetch(a, qp + t0 * a.q_t * ES, l, r0, t0, q_token, q_head, a.D, live);
+    Rows<DT, DP, kThreads>::fetch(a, qp + (t0 * a.q_t + a.q_h) * ES, l + L::kQ, r0, t0, q_token, q_head, a.D, live);
+    Rows<DT, DVP, kThreads>::fetch(a, gp + t0 * a.g_t * ES, l + 2 * L::kQ, r0, t0, g_token, g_head, a.Dv, live);
+    const int mine = r0 + (lane & 31), r = r0 + which;
+    lam = mine < end ? lam_of(a, hk * a.G + mine - token_of(a, mine) * a.G) : 0.f;
+    if (what < 2) value = r < end ? lse[what * rows + r] : __builtin_inff();
+    else if (what < 4) value = r < end ? delta[(what - 2) * rows + r] : 0.f;
+    else if (what == 4) value = __int_as_float(r < end ? last_key(a, b, token_of(a, r)) : -1);
+  };
+  if (first < end) {
+    byte = row_byte(first);
+    fetch(first, 0, key_word(byte));
+    byte = row_byte(first + kTile);
+  }
   int stage = 0;
-  for (int r0 = first; r0 < rows; r0 += kTile, stage ^= 1) {
+  for (int r0 = first; r0 < end; r0 += kTile, stage ^= 1) {
     char* l = lds + stage * L::kStage;
-    q0.put(l, ~0u);
-    q1.put(l + L::kQ, ~0u);
-    g.put(l + 2 * L::kQ, ~0u);
     float* of_rows = (float*)(l + 2 * L::kQ + L::kG);
-    if (what < 6) of_rows[what * kTile + which] = row_value;
-    if (r0 + kTile < rows) fetch(r0 + kTile);
+    // The second map's factor goes into its exponent, its sign into a bit a row.
+    const uint32_t minus = (uint32_t)__ballot(lam < 0.f);
+    const float bits = __builtin_amdgcn_logf(fabsf(lam));  // base 2; -inf for none
+    const float factor = __shfl(bits, which, kWave);
+    if (what == 1) value -= factor;
+    if (what < 5) of_rows[what * kTile + which] = value;
     __syncthreads();
+    if (r0 + kTile < end) {
+      fetch(r0 + kTile, stage ^ 1, key_word(byte));
+      byte = row_byte(r0 + 2 * kTile);
+    }
     if (!work) continue;
-    const int last_row = min(r0 + kTile, rows) - 1;
-    if (a.causal && last_row / a.G + a.q_start < key0) continue;
+    bool some = false;
+    if (a.causal) {
+      if (token_of(a, min(r0 + kTile, rows) - 1) + a.q_start < key0) continue;
+      some = token_of(a, r0) + a.q_start < key0 + kTile - 1;
+    }
     const char* lg = l + 2 * L::kQ;
     f32x16 s0 = zeros(), s1 = zeros(), dp = zeros();
 #pragma unroll
@@ -200,21 +219,28 @@ __global__ __launch_bounds__(kKeyWaves * kWave) void diff_grad_keys(Args a) {
       const int x = acc_at(i, half);
       const f32x4 lse0 = *(const f32x4*)(of_rows + x), lse1 = *(const f32x4*)(of_rows + kTile + x);
       const f32x4 de0 = *(const f32x4*)(of_rows + 2 * kTile + x), de1 = *(const f32x4*)(of_rows + 3 * kTile + x);
-      const f32x4 lam = *(const f32x4*)(of_rows + 4 * kTile + x), last = *(const f32x4*)(of_rows + 5 * kTile + x);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        float p0 = __builtin_amdgcn_exp2f(fmaf(s0[i + e], c, -lse0[e]));
-        float p1 = __builtin_amdgcn_exp2f(fmaf(s1[i + e], c, -lse1[e]));
-        const bool seen = alive && key <= __float_as_int(last[e]);
-        p0 = seen ? p0 : 0.f;
-        p1 = seen ? p1 * lam[e] : 0.f;
-        const float x0 = p0 * small, x1 = p1 * small;
+        s0[i + e] = __builtin_amdgcn_exp2f(fmaf(s0[i + e], c, -lse0[e]));
+        s1[i + e] = __builtin_amdgcn_exp2f(fmaf(s1[i + e], c, -lse1[e]));
+      }
+      if (minus)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s1[i + e] = minus >> (x + e) & 1 ? -s1[i + e] : s1[i + e];
+      if (some) {
+        const f32x4 last = *(const f32x4*)(of_rows + 4 * kTile + x);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (key > __float_as_int(last[e])) s0[i + e] = s1[i + e] = 0.f;
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float p0 = s0[i + e], p1 = s1[i + e], x0 = DT == DA_F16 ? p0 * small : p0, x1 = DT == DA_F16 ? p1 * small : p1;
         s0[i + e] = x0 * (dp[i + e] - de0[e]);
         s1[i + e] = x1 * (de1[e] - dp[i + e]);
         dp[i + e] = p0 - p1;
       }
     }
-    (void)whole;
 #pragma unroll
     for (int j = 0; j < KC; ++j) {
       const u32x4 x = from_acc<DT>(dp, j), y0 = from_acc<DT>(s0, j), y1 = from_acc<DT>(s1, j);
@@ -229,47 +255,60 @@ __global__ __launch_bounds__(kKeyWaves * kWave) void diff_grad_keys(Args a) {
   }
   if (key >= a.S) return;
   const float by = a.scale / small;
-  const int64_t at = ((int64_t)b * a.S + key) * a.Hk + hk;
+  const int64_t n_keys = (int64_t)a.batch * a.S * a.Hk;
+  const int64_t to = ((int64_t)b * a.S + key) * a.Hk + hk;
+  // A key that takes no part was a column of its own: whatever it holds is dropped here.
+  auto put = [&](char* whole, int64_t skip, int64_t row, int d, int e, f32x4 x) {
+    if (!alive) x = f32x4{0, 0, 0, 0};
+    if (a.splits > 1) {
+      if (e < d) *(f32x4*)(a.part + split * n_keys * (2 * a.D + a.Dv) + skip + row * d + e) = x;
+    } else {
+      store4<DT>(whole + row * d * ES, e, d, x[0], x[1], x[2], x[3]);
+    }
+  };
 #pragma unroll
   for (int m = 0; m < 2; ++m)
 #pragma unroll
     for (int n = 0; n < ND; ++n)
 #pragma unroll
       for (int i = 0; i < 16; i += 4)
-        store4<DT>(a.dk + (2 * at + m) * a.D * ES, 32 * n + acc_at(i, half), a.D, dk[m][n][i] * by, dk[m][n][i + 1] * by,
-                   dk[m][n][i + 2] * by, dk[m][n][i + 3] * by);
+        put(a.dk, 0, 2 * to + m, a.D, 32 * n + acc_at(i, half),
+            f32x4{dk[m][n][i], dk[m][n][i + 1], dk[m][n][i + 2], dk[m][n][i + 3]} * by);
 #pragma unroll
   for (int n = 0; n < NV; ++n)
 #pragma unroll
     for (int i = 0; i < 16; i += 4)
-      store4<DT>(a.dv + at * a.Dv * ES, 32 * n + acc_at(i, half), a.Dv, dv[n][i], dv[n][i + 1], dv[n][i + 2], dv[n][i + 3]);
+      put(a.dv, n_keys * 2 * a.D, to, a.Dv, 32 * n + acc_at(i, half),
+          f32x4{dv[n][i], dv[n][i + 1], dv[n][i + 2], dv[n][i + 3]});
 }
 
 // ---------------------------------------------------------------------------
 // dq: four waves of 32 rows over their keys.
 // ---------------------------------------------------------------------------
-constexpr int kRowWaves = 4;
-
 template <int DT, int DP, int DVP>
 struct RowSmem {
-  static constexpr int NT = kRowWaves * kWave;
-  static constexpr int kK = Tile<DT, DP, NT>::kBytes, kV = Tile<DT, DVP, NT>::kBytes;
+  static constexpr int kK = Tile<DT, DP, kThreads>::kBytes, kV = Tile<DT, DVP, kThreads>::kBytes;
   static constexpr int kStage = 2 * kK + kV;
   static constexpr int kBytes = 2 * kStage;
 };
 
 template <int DT, int DP, int DVP>
-__global__ __launch_bounds__(kRowWaves * kWave) void diff_grad_rows(Args a) {
+__global__ __launch_bounds__(kThreads, DT != DA_F32 && DVP <= 128 ? 2 : 1) void diff_grad_rows(Args a) {
   using L = RowSmem<DT, DP, DVP>;
-  constexpr int NT = L::NT, ES = Type<DT>::ES, V = Type<DT>::V;
+  constexpr int ES = Type<DT>::ES, V = Type<DT>::V;
   constexpr int KD = DP / Type<DT>::kStep, KV = DVP / Type<DT>::kStep, KC = Type<DT>::kChunks, ND = DP / 32;
   extern __shared__ __attribute__((aligned(16))) char lds[];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
-  const int block = a.row_blocks - 1 - blockIdx.x % a.row_blocks;  // the rows with the most keys first
-  const int hk = blockIdx.x / a.row_blocks % a.Hk, b = blockIdx.x / a.row_blocks / a.Hk;
+  const int lane = threadIdx.x & 63, half = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int at = (int)xcd_remap(blockIdx.x, gridDim.x);
+  const int block = a.blocks - 1 - at % a.blocks;  // the rows with the most keys first
+  at /= a.blocks;
+  const int split = at % a.splits;
+  at /= a.splits;
+  const int hk = at % a.Hk, b = at / a.Hk;
   const int rows = a.T * a.G;
-  const int r = (block * kRowWaves + wave) * kTile + (lane & 31);
-  const int t = r / a.G, h = hk * a.G + (r - t * a.G);
+  const int r = (block * kWaves + wave) * kTile + (lane & 31);
+  const int t = token_of(a, r), h = hk * a.G + (r - t * a.G);
   const int last = r < rows ? last_key(a, b, t) : -1;
   int most = last, least = last;
 #pragma unroll
@@ -281,58 +320,52 @@ __global__ __launch_bounds__(kRowWaves * kWave) void diff_grad_rows(Args a) {
   least = __builtin_amdgcn_readfirstlane(least);
   int end = a.S;
   if (a.causal) {
-    const int64_t t_last = min((block + 1) * kRowWaves * kTile, rows) - 1;
-    end = (int)max((int64_t)0, min((int64_t)a.S, t_last / a.G + a.q_start + 1));
+    const int64_t t_last = token_of(a, min((block + 1) * kWaves * kTile, rows) - 1);
+    end = (int)max((int64_t)0, min((int64_t)a.S, t_last + a.q_start + 1));
   }
+  int key = split * a.each;
+  end = min(end, key + a.each);
+  const bool in = last >= 0;
   u32x4 q[2][KD], g[KV];
 #pragma unroll
   for (int m = 0; m < 2; ++m)
 #pragma unroll
     for (int kk = 0; kk < KD; ++kk)
-      q[m][kk] = last >= 0 ? load_run<DT>(a.q + (b * a.q_b + t * a.q_t + (2 * h + m) * a.q_h) * ES, (2 * kk + half) * V, a.D)
-                           : u32x4{0, 0, 0, 0};
+      q[m][kk] = in ? load_run<DT>(a.q + (b * a.q_b + t * a.q_t + (2 * h + m) * a.q_h) * ES, (2 * kk + half) * V, a.D)
+                    : u32x4{0, 0, 0, 0};
 #pragma unroll
   for (int kk = 0; kk < KV; ++kk)
-    g[kk] = last >= 0 ? load_run<DT>(a.g + (b * a.g_b + t * a.g_t + h * a.g_h) * ES, (2 * kk + half) * V, a.Dv)
-                      : u32x4{0, 0, 0, 0};
+    g[kk] = in ? load_run<DT>(a.g + (b * a.g_b + t * a.g_t + h * a.g_h) * ES, (2 * kk + half) * V, a.Dv)
+               : u32x4{0, 0, 0, 0};
   const int64_t base = ((int64_t)b * a.Hk + hk) * 2 * rows + r;
-  const bool in = last >= 0;
   const float lse0 = in ? a.lse[base] : __builtin_inff(), lse1 = in ? a.lse[base + rows] : __builtin_inff();
   const float de0 = in ? a.delta[base] : 0.f, de1 = in ? a.delta[base + rows] : 0.f;
   const float c = a.scale * kLog2e, small = small_scale<DT>(a);
   const float lam = in ? lam_of(a, h) * small : 0.f;
 
-  Tile<DT, DP, NT> k0, k1;
-  Tile<DT, DVP, NT> v;
+  const Keys<DT, DP, kThreads> keys(a.k_t, a.D);
+  const Keys<DT, DVP, kThreads> values(a.v_t, a.Dv);
   const char* kp = a.k + (b * a.k_b + 2 * hk * a.k_h) * ES;
   const char* vp = a.v + (b * a.v_b + hk * a.v_h) * ES;
-  auto fetch = [&](int key) {
-    k0.fetch([&](int i) { return key + i < end ? kp + (key + i) * a.k_t * ES : nullptr; }, a.D);
-    k1.fetch([&](int i) { return key + i < end ? kp + ((key + i) * a.k_t + a.k_h) * ES : nullptr; }, a.D);
-    v.fetch([&](int i) { return key + i < end ? vp + (key + i) * a.v_t * ES : nullptr; }, a.Dv);
+  auto fetch = [&](int to, int stage, uint32_t live) {
+    const uint32_t l = lds_address(lds) + stage * L::kStage;
+    keys.fetch(kp + to * a.k_t * ES, l, live);
+    keys.fetch(kp + (to * a.k_t + a.k_h) * ES, l + L::kK, live);
+    values.fetch(vp + to * a.v_t * ES, l + 2 * L::kK, live);
   };
   f32x16 dq[2][ND];
 #pragma unroll
   for (int n = 0; n < ND; ++n) dq[0][n] = zeros(), dq[1][n] = zeros();
-  uint32_t word = end > 0 ? key_word(key_byte(a, b, 0, end, lane)) : 0;
-  int byte = key_byte(a, b, kTile, end, lane);
-  if (word) fetch(0);
-  int stage = 0;
-  for (int key = 0; key < end; key += kTile) {
-    char* l = lds + stage * L::kStage;
-    const uint32_t live = word;
-    if (live) {
-      k0.put(l, live);
-      k1.put(l + L::kK, live);
-      v.put(l + 2 * L::kK, live);
-    }
-    word = key_word(byte);
-    if (word) fetch(key + kTile);
-    byte = key_byte(a, b, key + 2 * kTile, end, lane);
-    if (!live) continue;
+  Live live(a, b, key, end, lane);
+  if (live.word) fetch(live.key, 0, live.word);
+  for (int stage = 0; live.word; stage ^= 1) {
+    key = live.key;
+    const uint32_t word = live.word;
+    live.next(a, b, end, lane);
     __syncthreads();
-    stage ^= 1;
+    if (live.word) fetch(live.key, stage ^ 1, live.word);
     if (key > most) continue;
+    const char* l = lds + stage * L::kStage;
     f32x16 s0 = zeros(), s1 = zeros(), dp = zeros();
 #pragma unroll
     for (int kk = 0; kk < KD; ++kk) {
@@ -341,14 +374,15 @@ __global__ __launch_bounds__(kRowWaves * kWave) void diff_grad_rows(Args a) {
     }
 #pragma unroll
     for (int kk = 0; kk < KV; ++kk) Mfma32<DT>::mma(dp, by_rows<DT, DVP>(l + 2 * L::kK, kk, lane), g[kk]);
-    const bool some = live != ~0u || key + kTile - 1 > least;
+    const bool some = word != ~0u || key + kTile - 1 > least;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      float p0 = __builtin_amdgcn_exp2f(fmaf(s0[i], c, -lse0)) * small;
+      float p0 = __builtin_amdgcn_exp2f(fmaf(s0[i], c, -lse0));
       float p1 = __builtin_amdgcn_exp2f(fmaf(s1[i], c, -lse1)) * lam;
+      if constexpr (DT == DA_F16) p0 *= small;
       if (some) {
         const int x = acc_at(i, half);
-        const bool seen = key + x <= last && (live >> x & 1);
+        const bool seen = key + x <= last && (word >> x & 1);
         p0 = seen ? p0 : 0.f;
         p1 = seen ? p1 : 0.f;
       }
@@ -367,15 +401,32 @@ __global__ __launch_bounds__(kRowWaves * kWave) void diff_grad_rows(Args a) {
   }
   if (r >= rows) return;
   const float by = a.scale / small;
-  const int64_t at = ((int64_t)b * a.T + t) * (a.Hk * a.G) + h;
+  const int64_t to = ((int64_t)b * a.T + t) * (a.Hk * a.G) + h;
 #pragma unroll
   for (int m = 0; m < 2; ++m)
 #pragma unroll
     for (int n = 0; n < ND; ++n)
 #pragma unroll
-      for (int i = 0; i < 16; i += 4)
-        store4<DT>(a.dq + (2 * at + m) * a.D * ES, 32 * n + acc_at(i, half), a.D, dq[m][n][i] * by, dq[m][n][i + 1] * by,
-                   dq[m][n][i + 2] * by, dq[m][n][i + 3] * by);
+      for (int i = 0; i < 16; i += 4) {
+        const int e = 32 * n + acc_at(i, half);
+        const f32x4 x = f32x4{dq[m][n][i], dq[m][n][i + 1], dq[m][n][i + 2], dq[m][n][i + 3]} * by;
+        if (a.splits == 1)
+          store4<DT>(a.dq + (2 * to + m) * a.D * ES, e, a.D, x[0], x[1], x[2], x[3]);
+        else if (e < a.D)
+          *(f32x4*)(a.part + (split * (int64_t)a.batch * rows * a.Hk + to) * 2 * a.D + m * a.D + e) = x;
+      }
+}
+
+// Sums of splits, in order, four entries a thread: to `first` up to n_first, then to `second`.
+template <int DT>
+__global__ __launch_bounds__(256) void diff_grad_join(const float* part, int splits, int64_t n, char* first,
+                                                      int64_t n_first, char* second) {
+  const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (at >= n) return;
+  f32x4 v = *(const f32x4*)(part + at);
+  for (int p = 1; p < splits; ++p) v += *(const f32x4*)(part + p * n + at);
+  char* to = at < n_first ? first + at * Type<DT>::ES : second + (at - n_first) * Type<DT>::ES;
+  store4<DT>(to, 0, 4, v[0], v[1], v[2], v[3]);
 }
 
 // Tokens of a chunk of delta: about four workgroups a CU, no fewer than 16 tokens.
@@ -386,11 +437,48 @@ void chunks_of(int64_t groups, int64_t T, int64_t cus, int* chunk, int* chunks) 
   *chunks = (int)std::max<int64_t>(1, (T + each - 1) / each);
 }
 
-// The workspace: delta, the parts of dlam, the largest |g|.
-size_t workspace_of(int64_t batch, int64_t heads, int64_t T, int chunks, int64_t* parts_at, int64_t* most_at) {
-  *parts_at = batch * heads * T * 2;
-  *most_at = *parts_at + batch * heads * chunks;
-  return (size_t)(*most_at + 1) * sizeof(float);
+// Blocks of one side's entries, and splits of the other's: so many that every CU has two
+// workgroups, none under 256 entries.
+void share(int64_t mine, int64_t others, int64_t groups, int64_t cus, int* blocks, int* splits, int* each) {
+  const int64_t n = std::max<int64_t>(1, (mine + kWaves * kTile - 1) / (kWaves * kTile));
+  int64_t want = std::max<int64_t>(1, 2 * cus / std::max<int64_t>(1, groups * n));
+  want = std::max<int64_t>(1, std::min(want, others / 256));
+  const int64_t e = std::max<int64_t>(kTile, ((others + want - 1) / want + kTile - 1) / kTile * kTile);
+  *blocks = (int)n, *each = (int)e;
+  *splits = (int)std::max<int64_t>(1, (others + e - 1) / e);
+}
+
+// How the two passes are shared out, and the workspace: delta, the parts of dlam, the largest
+// |g|, and the sums of the splits (of one pass after the other).
+struct Plan {
+  Args keys, rows;  // blocks, splits, each
+  int64_t parts_at, most_at, sums_at;
+  size_t bytes;
+};
+
+int plan(int64_t batch, int64_t heads, int64_t k_heads, int64_t T, int64_t S, int64_t D, int64_t Dv, Args* a, Plan* p) {
+  int64_t cus;
+  const int rc = device_cu_count(&cus);
+  if (rc) return rc;
+  const int64_t rows = T * (heads / k_heads);
+  chunks_of(batch * heads, T, cus, &a->chunk, &a->chunks);
+  share(S, rows, batch * k_heads, cus, &p->keys.blocks, &p->keys.splits, &p->keys.each);
+  share(rows, S, batch * k_heads, cus, &p->rows.blocks, &p->rows.splits, &p->rows.each);
+  p->parts_at = batch * heads * T * 2;
+  p->most_at = p->parts_at + batch * heads * a->chunks;
+  p->sums_at = (p->most_at + 4) / 4 * 4;
+  const int64_t of_keys = p->keys.splits > 1 ? p->keys.splits * batch * S * k_heads * (2 * D + Dv) : 0;
+  const int64_t of_rows = p->rows.splits > 1 ? p->rows.splits * batch * T * heads * 2 * D : 0;
+  p->bytes = (size_t)(p->sums_at + std::max(of_keys, of_rows)) * sizeof(float);
+  return DA_OK;
+}
+
+template <int DT>
+int join(const float* part, int splits, int64_t n, void* first, int64_t n_first, void* second, hipStream_t st) {
+  const int64_t blocks = (n / 4 + 255) / 256;
+  if (blocks > kMaxBlocks) return set_error(DA_ERR_UNSUPPORTED, "da_diff_attention_grad: too many rows");
+  diff_grad_join<DT><<<(unsigned)blocks, 256, 0, st>>>(part, splits, n, (char*)first, n_first, (char*)second);
+  return DA_OK;
 }
 
 }  // namespace
@@ -407,13 +495,11 @@ int da_diff_attention_grad_workspace(int dtype, int64_t batch, int64_t q_len, in
   *bytes = 0;
   int rc = check_sizes("da_diff_attention_grad_workspace", dtype, batch, q_len, k_len, heads, k_heads, d, dv, 0);
   if (rc || batch == 0) return rc;
-  int64_t cus, parts, most;
-  rc = device_cu_count(&cus);
-  if (rc) return rc;
-  int chunk, chunks;
-  chunks_of(batch * heads, q_len, cus, &chunk, &chunks);
-  *bytes = workspace_of(batch, heads, q_len, chunks, &parts, &most);
-  return DA_OK;
+  Args a;
+  Plan p;
+  rc = plan(batch, heads, k_heads, q_len, k_len, d, dv, &a, &p);
+  if (rc == DA_OK) *bytes = p.bytes;
+  return rc;
 }
 
 int da_diff_attention_grad(const da_diff_inputs* in, const void* g, int64_t g_bstride, int64_t g_tstride,
@@ -431,30 +517,28 @@ int da_diff_attention_grad(const da_diff_inputs* in, const void* g, int64_t g_bs
       (k_len && (!in->k || !in->v || !dk || !dvalue)))
     return set_error(DA_ERR_INVALID, "%s: NULL pointer", what);
   Args a = {};
-  rc = fill_args(a, what, in, batch, q_len, k_len, heads, k_heads, d, dv, scale, causal, q_start);
+  rc = fill_args(a, what, dtype, in, batch, q_len, k_len, heads, k_heads, d, dv, scale, causal, q_start);
+  if (rc == DA_OK)
+    rc = check_side(what, "g", g, (int)elem_bytes(dtype), dv, q_len, a.G, g_bstride, g_tstride, g_hstride);
   if (rc) return rc;
-  int64_t cus, parts_at, most_at;
-  rc = device_cu_count(&cus);
+  Plan p;
+  rc = plan(batch, heads, k_heads, q_len, k_len, d, dv, &a, &p);
   if (rc) return rc;
-  chunks_of(batch * heads, q_len, cus, &a.chunk, &a.chunks);
-  const size_t need = workspace_of(batch, heads, q_len, a.chunks, &parts_at, &most_at);
-  if (!workspace || workspace_bytes < need)
-    return set_error(DA_ERR_WORKSPACE, "%s: workspace of %zu bytes needed", what, need);
+  if (!workspace || workspace_bytes < p.bytes)
+    return set_error(DA_ERR_WORKSPACE, "%s: workspace of %zu bytes needed", what, p.bytes);
   if ((uintptr_t)workspace % 16) return set_error(DA_ERR_INVALID, "%s: workspace must be 16-byte aligned", what);
-  const int64_t rows = q_len * a.G;
-  const int64_t row_blocks = (rows + kRowWaves * kTile - 1) / (kRowWaves * kTile);
-  const int64_t key_blocks = (k_len + kKeyWaves * kTile - 1) / (kKeyWaves * kTile);
-  if (batch * heads > kMaxBlocks / a.chunks || batch * k_heads > kMaxBlocks / std::max<int64_t>(1, row_blocks) ||
-      batch * k_heads > kMaxBlocks / std::max<int64_t>(1, key_blocks))
+  const int64_t rows = q_len * a.G, pairs = batch * k_heads;
+  if (batch * heads > kMaxBlocks / a.chunks || pairs > kMaxBlocks / p.rows.blocks / p.rows.splits ||
+      pairs > kMaxBlocks / p.keys.blocks / p.keys.splits)
     return set_error(DA_ERR_UNSUPPORTED, "%s: too many rows", what);
   a.g = (const char*)g, a.g_b = g_bstride, a.g_t = g_tstride, a.g_h = g_hstride;
   a.out = (char*)const_cast<void*>(out), a.second = (char*)const_cast<void*>(second);
   a.lse = const_cast<float*>(lse);
   a.delta = (float*)workspace;
-  a.lam_part = a.delta + parts_at;
-  a.most = a.delta + most_at;
+  a.lam_part = a.delta + p.parts_at;
+  a.most = a.delta + p.most_at;
+  a.part = a.delta + p.sums_at;
   a.dq = (char*)dq, a.dk = (char*)dk, a.dv = (char*)dvalue;
-  a.row_blocks = (int)row_blocks;
   const hipStream_t st = (hipStream_t)stream;
   if (dtype == DA_F16 && (rc = zero_f32_2d(a.most, 1, 1, 1, st))) return rc;
   const unsigned delta_grid = (unsigned)(batch * heads * a.chunks);
@@ -467,14 +551,20 @@ int da_diff_attention_grad(const da_diff_inputs* in, const void* g, int64_t g_bs
     if (k_len) {
       constexpr int kBytes = KeySmem<DT, DP, DVP>::kBytes;
       if (const int err = allow_lds((const void*)diff_grad_keys<DT, DP, DVP>, kBytes)) return err;
-      diff_grad_keys<DT, DP, DVP>
-          <<<(unsigned)(batch * k_heads * key_blocks), kKeyWaves * kWave, kBytes, st>>>(a);
+      a.blocks = p.keys.blocks, a.splits = p.keys.splits, a.each = p.keys.each;
+      diff_grad_keys<DT, DP, DVP><<<(unsigned)(pairs * a.blocks * a.splits), kThreads, kBytes, st>>>(a);
+      const int64_t n_first = pairs * k_len * 2 * d, n = n_first + pairs * k_len * dv;
+      if (a.splits > 1)
+        if (const int err = join<DT>(a.part, a.splits, n, dk, n_first, dvalue, st)) return err;
     }
     if (rows) {
       constexpr int kBytes = RowSmem<DT, DP, DVP>::kBytes;
       if (const int err = allow_lds((const void*)diff_grad_rows<DT, DP, DVP>, kBytes)) return err;
-      diff_grad_rows<DT, DP, DVP>
-          <<<(unsigned)(batch * k_heads * row_blocks), kRowWaves * kWave, kBytes, st>>>(a);
+      a.blocks = p.rows.blocks, a.splits = p.rows.splits, a.each = p.rows.each;
+      diff_grad_rows<DT, DP, DVP><<<(unsigned)(pairs * a.blocks * a.splits), kThreads, kBytes, st>>>(a);
+      const int64_t n = batch * q_len * heads * 2 * d;
+      if (a.splits > 1)
+        if (const int err = join<DT>(a.part, a.splits, n, dq, n, nullptr, st)) return err;
     }
     return check_launch("da_diff_attention_grad");
   });

@@ -1902,6 +1902,19 @@ def _diff_sizes(what: str, q, k, v, lam):
     return b, t, s, h2 // 2, hk, d, dv
 
 
+def _head_rows(x: torch.Tensor) -> torch.Tensor:
+    """(B, T, heads, width) rows as the kernels read them (:func:`prepare_rows`):
+    whole 16-byte runs, padded with zeros, tokens within 31 bits of each other."""
+    x = prepare_rows(x)
+    es = x.element_size()
+    far = (min(x.shape[1], 33) * x.stride(1) + x.shape[2] * x.stride(2) + x.shape[3]) * es
+    return x if far < 1 << 31 else x.contiguous()
+
+
+def _unpadded(x: torch.Tensor, width: int) -> torch.Tensor:
+    return x if x.shape[-1] == width else x[..., :width].contiguous()
+
+
 def _diff_call(what, q, k, v, lam, mask, q_mask, scale, causal, q_start):
     """Sizes, the record of the inputs as words, and the tensors it points to."""
     sizes = _diff_sizes(what, q, k, v, lam)
@@ -1910,14 +1923,15 @@ def _diff_call(what, q, k, v, lam, mask, q_mask, scale, causal, q_start):
     mask, mask_ptr, mask_b, mask_k = _token_mask(what, mask, b, s)
     q_mask, qm_ptr, qm_b, qm_t = _token_mask(what, q_mask, b, t)
     dev = nat.same_device(q, k, v, lam, mask, q_mask)
-    q, k, v = _unit_rows(q), _unit_rows(k), _unit_rows(v)
+    q, k, v = _head_rows(q), _head_rows(k), _head_rows(v)
+    sizes = (b, t, s, h, hk, q.shape[3], v.shape[3])
     scale = d ** -0.5 if scale is None else float(scale)
     q_start = s - t if q_start is None else int(q_start)
     words = array.array("q", (
         q.data_ptr(), k.data_ptr(), v.data_ptr(), lam.data_ptr(), nat.DTYPE_CODE[lam.dtype],
         lam.stride(0) if lam.numel() > 1 else 0, *q.stride()[:3], *k.stride()[:3], *v.stride()[:3],
         mask_ptr or 0, mask_b, mask_k, qm_ptr or 0, qm_b, qm_t))
-    return dev, sizes, (code, b, t, s, h, hk, d, dv), (scale, int(causal), q_start), words, (q, k, v, lam, mask, q_mask)
+    return dev, (b, t, s, h, hk, d, dv), (code, *sizes), (scale, int(causal), q_start), words, (q, k, v, lam, mask, q_mask)
 
 
 def diff_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lam: torch.Tensor, *, scale: float | None = None,
@@ -1927,10 +1941,11 @@ def diff_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lam: torch
     dev, (b, t, s, h, hk, d, dv), sizes, rest, words, keep = _diff_call("diff_attention", q, k, v, lam, mask, q_mask,
                                                                         scale, causal, q_start)
     lib = nat.load()
-    out = torch.empty((b, t, h, dv), dtype=q.dtype, device=dev)
+    wide = sizes[-1]  # the values' width, padded
+    out = torch.empty((b, t, h, wide), dtype=q.dtype, device=dev)
     second = lse = None
     if state:
-        second = torch.empty((b, t, h, dv), dtype=q.dtype, device=dev)
+        second = torch.empty((b, t, h, wide), dtype=q.dtype, device=dev)
         lse = torch.empty((b, hk, 2, t * (h // hk)), dtype=torch.float32, device=dev)
     nbytes = ctypes.c_size_t(0)
     with _on(dev):
@@ -1943,7 +1958,7 @@ def diff_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lam: torch
              None if second is None else second.data_ptr(), None if lse is None else lse.data_ptr(), ws_ptr,
              nbytes.value, nat.stream_ptr(dev))
     del keep
-    return out, second, lse
+    return _unpadded(out, dv), second, lse
 
 
 def diff_attention_grad(g: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lam: torch.Tensor,
@@ -1954,17 +1969,18 @@ def diff_attention_grad(g: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: to
     what = "diff_attention_grad"
     dev, (b, t, s, h, hk, d, dv), sizes, rest, words, keep = _diff_call(what, q, k, v, lam, mask, q_mask, scale, causal,
                                                                         q_start)
-    for name, x in (("g", g), ("out", out), ("second", second)):
-        if x.shape != (b, t, h, dv) or x.dtype != q.dtype:
-            raise ValueError(f"{what}: {name} must be {(b, t, h, dv)} {q.dtype}, got {tuple(x.shape)} {x.dtype}")
+    pad_d, pad_dv = sizes[-2:]
+    for name, x, w in (("g", g, dv), ("out", out, dv), ("second", second, pad_dv)):
+        if x.shape != (b, t, h, w) or x.dtype != q.dtype:
+            raise ValueError(f"{what}: {name} must be {(b, t, h, w)} {q.dtype}, got {tuple(x.shape)} {x.dtype}")
     if lse.shape != (b, hk, 2, t * (h // hk)) or lse.dtype != torch.float32:
         raise ValueError(f"{what}: the state does not belong to these inputs")
     nat.same_device(q, g, out, second, lse)
-    g, out, second, lse = _unit_rows(g), out.contiguous(), second.contiguous(), lse.contiguous()
+    g, out, second, lse = _head_rows(g), prepare_rows(out.contiguous()), second.contiguous(), lse.contiguous()
     lib = nat.load()
-    dq = torch.empty((b, t, 2 * h, d), dtype=q.dtype, device=dev)
-    dk = torch.empty((b, s, 2 * hk, d), dtype=q.dtype, device=dev)
-    dval = torch.empty((b, s, hk, dv), dtype=q.dtype, device=dev)
+    dq = torch.empty((b, t, 2 * h, pad_d), dtype=q.dtype, device=dev)
+    dk = torch.empty((b, s, 2 * hk, pad_d), dtype=q.dtype, device=dev)
+    dval = torch.empty((b, s, hk, pad_dv), dtype=q.dtype, device=dev)
     dlam = torch.empty((b, h), dtype=torch.float32, device=dev)
     nbytes = ctypes.c_size_t(0)
     with _on(dev):
@@ -1974,7 +1990,7 @@ def diff_attention_grad(g: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: to
              out.data_ptr(), second.data_ptr(), lse.data_ptr(), *sizes, *rest, dq.data_ptr(), dk.data_ptr(),
              dval.data_ptr(), dlam.data_ptr(), ws.data_ptr(), nbytes.value, nat.stream_ptr(dev))
     del keep
-    return dq, dk, dval, dlam
+    return _unpadded(dq, d), _unpadded(dk, d), _unpadded(dval, dv), dlam
 
 
 # ---------------------------------------------------------------------------
