@@ -40,6 +40,7 @@ struct Args {
   const char* g;
   int64_t g_b, g_t, g_h;
   float* delta;   // (batch, Hk, 2, T G): g . o_m
+  char* records;  // (batch, Hk, T G): lse and delta of both maps as diff_grad_keys reads them
   float* most;    // largest |g| of the call (16-bit floats of five exponent bits)
   char *dq, *dk, *dv;
   float* lam_part;  // (batch, heads, chunks)
@@ -52,6 +53,21 @@ struct Type {
   static constexpr int kStep = 2 * V;             // contracted entries of one pair of chunks
   static constexpr int kChunks = kTile / kStep;   // chunks of a tile contracted over its rows
 };
+
+// Which of n groups (batch, key head, split) and of their `blocks` a workgroup takes: block 0
+// has the most work.  A group's workgroups run on one die where the groups can be dealt out
+// evenly, the heaviest blocks of all its groups first, every other round of a die's 32 CUs
+// backwards: two workgroups that share a CU then have a heavy block and a light one.
+__device__ __forceinline__ void deal(int n, int blocks, int* group, int* block) {
+  const bool even = n % kXcds == 0;
+  const int id = blockIdx.x, die = even ? id % kXcds : 0, per = even ? n / kXcds : n;
+  const int slots = even ? 32 : 256, all = per * blocks;
+  int i = even ? id / kXcds : id;
+  const int round = i / slots;
+  if (round & 1) i = round * slots + min((round + 1) * slots, all) - 1 - i;
+  *block = i / per;
+  *group = die * per + (i - *block * per);
+}
 
 __device__ __forceinline__ int token_of(const Args& a, int r) {
   return (int)((uint64_t)(uint32_t)r * a.g_factor >> a.g_shift);
@@ -122,72 +138,107 @@ struct Keys : Tile<DT, W, NT> {
   }
   // `base`: the tile's first row; `live`: a bit a row
   __device__ __forceinline__ void fetch(const char* base, uint32_t lds, uint32_t live) const {
-    const u32x4 rsrc = make_rsrc(base, kOutside - 1);
+    const u32x4 rsrc = uniform4(make_rsrc(base, kOutside - 1));
 #pragma unroll
-    for (int i = 0; i < T::N; ++i) T::issue(rsrc, lds, i, (live >> T::row(i) & 1) ? at[i] : kOutside);
+    for (int i = 0; i < T::N; ++i)
+      T::issue(rsrc, lds, i, (live >> T::row(i) & 1) ? at[i] : kOutside);
   }
 };
 
 // Tiles of rows r = t G + g: heads of one token are `head` apart, tokens `token` (bytes).
+// Where G divides a tile, a lane's offsets from the tile's first token are the same in every
+// tile that starts at a whole one.
 template <int DT, int W, int NT>
 struct Rows : Tile<DT, W, NT> {
   using T = Tile<DT, W, NT>;
-  // `base`: the first head of token t0 = r0 / G
-  __device__ __forceinline__ static void fetch(const Args& a, const char* base, uint32_t lds, int r0, int t0,
-                                               uint32_t token, uint32_t head, int d, uint32_t live) {
-    const u32x4 rsrc = make_rsrc(base, kOutside - 1);
+  __device__ __forceinline__ static void place(const Args& a, int r0, uint32_t token, uint32_t head, int d,
+                                               uint32_t* at) {
+    const int t0 = token_of(a, r0);
 #pragma unroll
     for (int i = 0; i < T::N; ++i) {
-      const int row = T::row(i), r = r0 + row, t = token_of(a, r);
+      const int r = r0 + T::row(i), t = token_of(a, r);
       const uint32_t c = T::column(i, d);
-      const uint32_t at = (uint32_t)(t - t0) * token + (uint32_t)(r - t * a.G) * head + c;
-      T::issue(rsrc, lds, i, (live >> row & 1) && c != kOutside ? at : kOutside);
+      at[i] = c == kOutside ? kOutside : (uint32_t)(t - t0) * token + (uint32_t)(r - t * a.G) * head + c;
     }
+  }
+  // `base`: the first head of the tile's first token; `thread`: the thread's number
+  __device__ __forceinline__ static void fetch(const char* base, uint32_t lds, const uint32_t* at, uint32_t live,
+                                               int thread) {
+    const u32x4 rsrc = uniform4(make_rsrc(base, kOutside - 1));
+#pragma unroll
+    for (int i = 0; i < T::N; ++i)
+      T::issue(rsrc, lds, i, live >> ((thread + i * NT) / T::kPer) & 1 ? at[i] : kOutside);
   }
 };
 
-__device__ __forceinline__ uint32_t lds_address(const char* p) { return (uint32_t)(uintptr_t)(const lds_char*)p; }
 
-// Operand chunk kk of a tile read by rows: lane l has row l % 32, the entries of its half.
-template <int DT, int W>
-__device__ __forceinline__ u32x4 by_rows(const char* lds, int kk, int lane) {
-  constexpr int kRow = W * Type<DT>::ES;
-  const int row = lane & 31, c = 2 * kk + (lane >> 5);
-  return ld16(lds + row * kRow + ((c ^ swizzle<kRow>(row)) << 4));
+__device__ __forceinline__ uint32_t lds_address(const char* p) { return (uint32_t)(uintptr_t)(const lds_char*)p; }
+__device__ __forceinline__ u32x4 lds16(uint32_t at) {
+  return *(const __attribute__((address_space(3))) u32x4*)(uintptr_t)at;
 }
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
-// Operand chunk j of a tile read transposed: lane l has column 32 block + l % 32, at the
-// rows that registers of an accumulator hold in the same half: those of chunk j.
+// Where a lane reads tiles of W entries.  A chunk's place is its number xor the row's
+// swizzle, so that of all chunks which one lane reads differ from one register by a constant:
+// xor in the bits that are swizzled (16 .. 240 bytes), else added.
 template <int DT, int W>
-__device__ __forceinline__ u32x4 by_columns(const char* lds, int block, int j, int lane) {
-  constexpr int kRow = W * Type<DT>::ES;
-  const int half = lane >> 5;
-  if constexpr (DT == DA_F32) {
-    const int col = 32 * block + (lane & 31), c = col >> 2;
-    u32x4 v;
-#pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      const int row = 8 * j + 4 * half + s;
-      v[s] = *(const uint32_t*)(lds + row * kRow + ((c ^ swizzle<kRow>(row)) << 4) + (col & 3) * 4);
+struct Reader {
+  static constexpr int kRow = W * Type<DT>::ES;
+  uint32_t of_rows, of_columns;
+  __device__ __forceinline__ Reader(const char* lds, int lane) {
+    const uint32_t base = lds_address(lds), half = lane >> 5;
+    const int row = lane & 31;
+    of_rows = base + row * kRow + ((half ^ swizzle<kRow>(row)) << 4);
+    if constexpr (DT == DA_F32) {
+      const int col = lane & 31;
+      of_columns = base + 4 * half * kRow + (((col >> 2) ^ half) << 4) + (col & 3) * 4;
+    } else {
+      const int i = lane & 15, r = 4 * half + i / 4, c = (lane >> 4 & 1) * 2 + (i & 3) / 2;
+      of_columns = base + r * kRow + ((c ^ swizzle<kRow>(r)) << 4) + (i & 1) * 8;
     }
-    return v;
-  } else {
-    // ds_read_b64_tr_b16: of 16 lanes, lane i addresses four columns (i % 4) of row i / 4
-    // and receives four rows of column i.
-    const int i = lane & 15, c = 4 * block + (lane >> 4 & 1) * 2 + (i & 3) / 2;
-    u32x2 part[2];
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      const int row = 16 * j + 8 * s + 4 * half + i / 4;
-      const char* p = lds + row * kRow + ((c ^ swizzle<kRow>(row)) << 4) + (i & 1) * 8;
-      part[s] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-          (__attribute__((address_space(3))) s16x4*)(const lds_char*)p));
-    }
-    return u32x4{part[0][0], part[0][1], part[1][0], part[1][1]};
   }
-}
+  // The registers as they stand in the tile of `key`: else sums with every constant are kept
+  // over the loop instead, and fill the registers.
+  __device__ __forceinline__ Reader fresh(int key) const {
+    Reader r = *this;
+    asm("" : "+v"(r.of_rows) : "s"(key));
+    asm("" : "+v"(r.of_columns) : "s"(key));
+    return r;
+  }
+  // Operand chunk kk of the tile `skip` bytes on, by rows: lane l has row l % 32, the entries of
+  // its half.
+  __device__ __forceinline__ u32x4 rows(int skip, int kk) const {
+    const uint32_t c = kk << 5;
+    return lds16((of_rows ^ (c & 0xf0)) + (c & ~0xf0u) + skip);
+  }
+  // Operand chunk j transposed: lane l has column 32 n + l % 32, at the rows that registers of
+  // an accumulator hold in the same half, those of chunk j.
+  __device__ __forceinline__ u32x4 columns(int skip, int n, int j) const {
+    if constexpr (DT == DA_F32) {
+      u32x4 v;
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        const uint32_t c = n << 7 ^ s << 6 ^ (j & 1) << 5;
+        v[s] = *(const __attribute__((address_space(3))) uint32_t*)(uintptr_t)(
+            (of_columns ^ (c & 0xf0)) + (c & ~0xf0u) + skip + (8 * j + s) * kRow);
+      }
+      return v;
+    } else {
+      // ds_read_b64_tr_b16: of 16 lanes, lane i addresses four columns (i % 4) of row i / 4
+      // and receives four rows of column i.
+      u32x2 part[2];
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const uint32_t c = n << 6 ^ s << 5;
+        part[s] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (__attribute__((address_space(3))) s16x4*)(uintptr_t)(
+                (of_columns ^ (c & 0xf0)) + (c & ~0xf0u) + skip + (16 * j + 8 * s) * kRow)));
+      }
+      return u32x4{part[0][0], part[0][1], part[1][0], part[1][1]};
+    }
+  }
+};
 
 // Operand chunk j from an accumulator's registers: the other operand of by_columns.
 template <int DT>
@@ -228,6 +279,14 @@ __device__ __forceinline__ int key_byte(const Args& a, int b, int k0, int end, i
   return key < end ? (a.mask ? a.mask[b * a.m_b + key * a.m_k] : 1) : 0;
 }
 __device__ __forceinline__ uint32_t key_word(int byte) { return (uint32_t)__ballot(byte != 0); }
+
+// Of a tile's live keys, a bit each, those up to `last`: shifted so that the lane's half has
+// its row x at bit acc_at(x, 0).
+__device__ __forceinline__ uint32_t seen_of(uint32_t word, int key, int last, int half) {
+  const int n = last - key;  // the last one seen
+  const uint32_t upto = n >= 31 ? ~0u : n < 0 ? 0u : (2u << n) - 1u;
+  return (word & upto) >> (4 * half);
+}
 
 // Goes over the tiles that have a live key: their first key, and a bit a key (0: no more).
 struct Live {

@@ -104,35 +104,37 @@ __global__ __launch_bounds__(2 * NG * kWave, 2) void diff_forward(Args a) {
     for (int x = 0; x < NB; ++x) o[n][x] = zeros();
   }
 
+  const Reader<DT, DP> key_reader(lds + map * L::kK, lane);
+  const Reader<DT, DVP> value_reader(lds + 2 * L::kK, lane);
   // The next tile with a live key is on its way while one is multiplied.
   Live live(a, b, key, end, lane);
   if (live.word) fetch(live.key, 0, live.word);
-  for (int stage = 0; live.word; stage ^= 1) {
+  const auto step = [&](auto of) __attribute__((always_inline)) {
+    constexpr int stage = decltype(of)::value;
     key = live.key;
     const uint32_t word = live.word;
     live.next(a, b, end, lane);
     __syncthreads();
     if (live.word) fetch(live.key, stage ^ 1, live.word);
-    if (key > most) continue;
-    const char* lk = lds + stage * L::kStage + map * L::kK;
-    const char* lv = lds + stage * L::kStage + 2 * L::kK;
+    if (key > most) return;
+    const auto lk = key_reader.fresh(key);
+    const auto lv = value_reader.fresh(key);
     f32x16 s[R];
 #pragma unroll
     for (int n = 0; n < R; ++n) s[n] = zeros();
 #pragma unroll
     for (int kk = 0; kk < KD; ++kk) {
-      const u32x4 x = by_rows<DT, DP>(lk, kk, lane);
+      const u32x4 x = lk.rows(stage * L::kStage, kk);
 #pragma unroll
       for (int n = 0; n < R; ++n) Mfma32<DT>::mma(s[n], x, q[n][kk]);
     }
     if (word != ~0u || key + kTile - 1 > least) {
 #pragma unroll
-      for (int n = 0; n < R; ++n)
+      for (int n = 0; n < R; ++n) {
+        const uint32_t seen = seen_of(word, key, last[n], half);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int x = acc_at(i, half);
-          s[n][i] = key + x <= last[n] && (word >> x & 1) ? s[n][i] : -__builtin_inff();
-        }
+        for (int i = 0; i < 16; ++i) s[n][i] = seen & 1u << acc_at(i, 0) ? s[n][i] : -__builtin_inff();
+      }
     }
 #pragma unroll
     for (int n = 0; n < R; ++n) {
@@ -165,7 +167,7 @@ __global__ __launch_bounds__(2 * NG * kWave, 2) void diff_forward(Args a) {
       }
 #pragma unroll
       for (int y = 0; y < NB; ++y) {
-        const u32x4 x = by_columns<DT, DVP>(lv, y, j, lane);
+        const u32x4 x = lv.columns(stage * L::kStage, y, j);
 #pragma unroll
         for (int n = 0; n < R; ++n) {
           Mfma32<DT>::mma(o[n][y], x, p[n]);
@@ -173,6 +175,10 @@ __global__ __launch_bounds__(2 * NG * kWave, 2) void diff_forward(Args a) {
         }
       }
     }
+  };
+  while (live.word) {
+    step(std::integral_constant<int, 0>{});
+    if (live.word) step(std::integral_constant<int, 1>{});
   }
 
 #pragma unroll

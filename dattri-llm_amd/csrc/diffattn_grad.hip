@@ -17,6 +17,7 @@
 // 16-bit floats of five exponent bits lose small values of ds: there ds is scaled by the
 // power of two that brings the largest |g| near one, and its products back.
 #include <algorithm>
+#include <type_traits>
 
 #include "diffattn.h"
 
@@ -25,9 +26,45 @@ namespace diff {
 namespace {
 
 // ---------------------------------------------------------------------------
-// delta, parts of dlam, largest |g|.  Workgroup (b, h, chunk of tokens), 16 lanes a token.
+// delta, its records, parts of dlam, largest |g|.  Workgroup (b, h, chunk of tokens), 16 lanes
+// a token.
+//
+// Where keys are columns, a row's lse and delta are needed in every lane, by register.  In
+// bf16 they come with the products instead: one more step of contraction over their parts
+// (three bf16 values hold 24 bits) against ones makes the scores' accumulators z - lse / c and
+// g v^T - delta, from two reads of LDS in place of sixteen.  A record then is the parts of
+// [-lse_1 / c | -delta_1 | -lse_2' / c | delta_1 - delta_2], eight entries each; else it is the
+// four values in fp32.  lse_2' = lse_2 - log2 |lam|: the factor comes with the exponential.
+// A row without keys has an exponential of nothing, by a finite number: no product is NaN.
 // ---------------------------------------------------------------------------
 constexpr int kLanes = 16;
+constexpr float kNothing = -1e30f;
+
+template <int DT>
+struct Record {
+  static constexpr bool kParts = DT == DA_BF16;
+  static constexpr int kBytes = kParts ? 64 : 16;
+};
+
+__device__ __forceinline__ u32x4 three_parts(float x) {
+  const uint32_t hi = f32_to_bf16_bits(x);
+  const float r1 = x - bf16_bits_to_f32(hi);
+  const uint32_t mid = f32_to_bf16_bits(r1);
+  const uint32_t lo = f32_to_bf16_bits(r1 - bf16_bits_to_f32(mid));
+  return u32x4{hi | mid << 16, lo, 0, 0};
+}
+
+template <int DT>
+__device__ __forceinline__ void put_record(char* to, float c, float lse0, float lse1, float de0, float de1) {
+  if constexpr (Record<DT>::kParts) {
+    st16(to, three_parts(lse0 == __builtin_inff() ? kNothing : -lse0 / c));
+    st16(to + 16, three_parts(-de0));
+    st16(to + 32, three_parts(lse1 == __builtin_inff() ? kNothing : -lse1 / c));
+    st16(to + 48, three_parts(de0 - de1));
+  } else {
+    *(f32x4*)to = f32x4{lse0, lse1, de0, de1};
+  }
+}
 
 template <int DT>
 __global__ __launch_bounds__(256) void diff_delta(Args a) {
@@ -62,9 +99,15 @@ __global__ __launch_bounds__(256) void diff_delta(Args a) {
     d0 = lanes_sum<kLanes>(d0);
     d1 = lanes_sum<kLanes>(d1);
     if (l == 0) {
-      float* to = a.delta + ((int64_t)b * a.Hk + hk) * 2 * rows + t * a.G + (h - hk * a.G);
-      to[0] = d0 + lam * d1;  // o_1 = out + lam o_2
+      const int64_t of = (int64_t)b * a.Hk + hk;
+      const int r = t * a.G + (h - hk * a.G);
+      float* to = a.delta + of * 2 * rows + r;
+      d0 += lam * d1;  // o_1 = out + lam o_2
+      to[0] = d0;
       to[rows] = d1;
+      const float* lse = a.lse + of * 2 * rows + r;
+      put_record<DT>(a.records + (of * rows + r) * Record<DT>::kBytes, a.scale * kLog2e, lse[0],
+                     lse[rows] - log2f(fabsf(lam)), d0, d1);
     }
     all += d1;
   }
@@ -102,43 +145,60 @@ __device__ __forceinline__ float small_scale(const Args& a) {
 // ---------------------------------------------------------------------------
 constexpr int kWaves = 4, kThreads = kWaves * kWave;
 
+// In 16 bits the values of a wave's keys lie in LDS, read again for every tile of rows: with
+// them in registers there is room for one wave a SIMD only.
 template <int DT, int DP, int DVP>
 struct KeySmem {
   static constexpr int kQ = Tile<DT, DP, kThreads>::kBytes, kG = Tile<DT, DVP, kThreads>::kBytes;
-  static constexpr int kRow = 5 * kTile * 4;  // of each row: lse and delta of both maps, the last key
-  static constexpr int kStage = 2 * kQ + kG + kRow;
-  static constexpr int kBytes = 2 * kStage;
+  static constexpr int kR = Record<DT>::kParts ? kTile * 64 : 1024;  // one load a wave writes 1 KB
+  static constexpr int kStage = 2 * kQ + kG + kR;
+  static constexpr bool kValues = DT != DA_F32;
+  static constexpr int kOf = kValues ? kG : 0;  // a wave's values
+  // A thread's offsets of rows.  They lie in LDS too: kept in registers they would be spilled,
+  // and a load of a spilled one waits for the tiles under way.
+  static constexpr int kOffsets = (Tile<DT, DP, kThreads>::N + Tile<DT, DVP, kThreads>::N + 3) / 4;
+  static constexpr int kOffsetsAt = 2 * kStage + kWaves * kOf;
+  static constexpr int kBytes = kOffsetsAt + kOffsets * kThreads * 16;
 };
 
 template <int DT, int DP, int DVP>
-__global__ __launch_bounds__(kThreads) void diff_grad_keys(Args a) {
+__global__ __launch_bounds__(kThreads, DT != DA_F32 && DP == 64 ? 2 : 1) void diff_grad_keys(Args a) {
   using L = KeySmem<DT, DP, DVP>;
+  using Rec = Record<DT>;
   constexpr int ES = Type<DT>::ES, V = Type<DT>::V;
   constexpr int KD = DP / Type<DT>::kStep, KV = DVP / Type<DT>::kStep, KC = Type<DT>::kChunks;
   constexpr int ND = DP / 32, NV = DVP / 32;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int lane = threadIdx.x & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  int at = (int)xcd_remap(blockIdx.x, gridDim.x);
-  const int block = at % a.blocks;  // the first keys have the most rows
-  at /= a.blocks;
+  int at, block;
+  deal(a.batch * a.Hk * a.splits, a.blocks, &at, &block);  // the first keys have the most rows
   const int split = at % a.splits;
   at /= a.splits;
   const int hk = at % a.Hk, b = at / a.Hk;
   const int key0 = (block * kWaves + wave) * kTile, key = key0 + (lane & 31);
   const bool alive = key < a.S && (!a.mask || a.mask[b * a.m_b + key * a.m_k]);
   const int rows = a.T * a.G, end = min(rows, (split + 1) * a.each);
-  u32x4 k[2][KD], v[KV];
+  u32x4 k[2][KD], v[L::kValues ? 1 : KV];
 #pragma unroll
   for (int kk = 0; kk < KD; ++kk)
 #pragma unroll
     for (int m = 0; m < 2; ++m)
       k[m][kk] = alive ? load_run<DT>(a.k + (b * a.k_b + key * a.k_t + (2 * hk + m) * a.k_h) * ES,
                                       (2 * kk + half) * V, a.D) : u32x4{0, 0, 0, 0};
+  char* lv = lds + 2 * L::kStage + wave * L::kOf;
 #pragma unroll
-  for (int kk = 0; kk < KV; ++kk)
-    v[kk] = alive ? load_run<DT>(a.v + (b * a.v_b + key * a.v_t + hk * a.v_h) * ES, (2 * kk + half) * V, a.Dv)
-                  : u32x4{0, 0, 0, 0};
+  for (int kk = 0; kk < KV; ++kk) {
+    const u32x4 x = alive ? load_run<DT>(a.v + (b * a.v_b + key * a.v_t + hk * a.v_h) * ES, (2 * kk + half) * V, a.Dv)
+                          : u32x4{0, 0, 0, 0};
+    if constexpr (L::kValues) {
+      constexpr int kRow = DVP * ES;
+      const int row = lane & 31;
+      st16(lv + row * kRow + (((2 * kk + half) ^ swizzle<kRow>(row)) << 4), x);
+    } else {
+      v[kk] = x;
+    }
+  }
   const bool work = __any(alive);
   f32x16 dk[2][ND], dv[NV];
 #pragma unroll
@@ -146,112 +206,168 @@ __global__ __launch_bounds__(kThreads) void diff_grad_keys(Args a) {
 #pragma unroll
   for (int n = 0; n < NV; ++n) dv[n] = zeros();
   const float c = a.scale * kLog2e, small = small_scale<DT>(a);
+  // Ones against the parts of one half's records.
+  constexpr uint32_t kOnes = 0x3f803f80u, kOne = 0x3f80u;
+  const uint32_t in_low = half ? 0u : ~0u;
 
-  // The first row that sees the workgroup's first key.
-  int first = split * a.each;
-  if (a.causal) {
-    const int64_t t = (int64_t)block * kWaves * kTile - a.q_start;
-    if (t > 0) first = max(first, t >= a.T ? end : (int)t * a.G / kTile * kTile);
-  }
+  // The rows that see the lane's key are those from `from` on; the wave's keys, all or some.
+  const auto first_row = [&](int to) {
+    const int64_t t = to - a.q_start;
+    return !a.causal || t <= 0 ? 0 : t >= a.T ? rows : (int)t * a.G;
+  };
+  const int from_some = first_row(key0), from_all = first_row(key0 + kTile - 1);
+  const int first = max(split * a.each, first_row(block * kWaves * kTile) / kTile * kTile);
   const uint32_t q_token = (uint32_t)(a.q_t * ES), q_head = (uint32_t)(2 * a.q_h * ES);
   const uint32_t g_token = (uint32_t)(a.g_t * ES), g_head = (uint32_t)(a.g_h * ES);
   const char* qp = a.q + (b * a.q_b + (int64_t)2 * hk * a.G * a.q_h) * ES;
   const char* gp = a.g + (b * a.g_b + (int64_t)hk * a.G * a.g_h) * ES;
-  const float* lse = a.lse + ((int64_t)b * a.Hk + hk) * 2 * rows;
-  const float* delta = a.delta + ((int64_t)b * a.Hk + hk) * 2 * rows;
-  // A value of a row a thread: lse and delta of both maps, the last key.
-  const int what = threadIdx.x / kTile, which = threadIdx.x % kTile;
-  float value = 0.f, lam = 0.f;  // lam: every wave's lanes have the tile's 32 rows
-  int byte = 0;
+  const char* records = a.records + ((int64_t)b * a.Hk + hk) * rows * Rec::kBytes;
+  const bool steady = kTile % a.G == 0;
+  using Q = Rows<DT, DP, kThreads>;
+  using G = Rows<DT, DVP, kThreads>;
+  const auto place = [&](int r0, uint32_t* at) __attribute__((always_inline)) {
+    Q::place(a, r0, q_token, q_head, a.D, at);
+    G::place(a, r0, g_token, g_head, a.Dv, at + Q::N);
+  };
+  {
+    uint32_t at[4 * L::kOffsets] = {};
+    place(first, at);
+#pragma unroll
+    for (int i = 0; i < L::kOffsets; ++i)
+      st16(lds + L::kOffsetsAt + (i * kThreads + threadIdx.x) * 16,
+           u32x4{at[4 * i], at[4 * i + 1], at[4 * i + 2], at[4 * i + 3]});
+  }
+  // Negative factors: their sign is not in the exponential.
+  bool any_minus = false;
+  for (int i = lane; i < a.G; i += kWave) any_minus |= lam_of(a, hk * a.G + i) < 0.f;
+  any_minus = __any(any_minus);
   auto row_byte = [&](int r0) {
     const int r = r0 + (lane & 31);
     return r < end ? (a.q_mask ? a.q_mask[b * a.qm_b + token_of(a, r) * a.qm_t] : 1) : 0;
   };
   auto fetch = [&](int r0, int stage, uint32_t live) {
-    const int t0 = token_of(a, r0);
+    const int64_t t0 = token_of(a, r0);
     const uint32_t l = lds_address(lds) + stage * L::kStage;
-    Rows<DT, DP, kThreads>::fetch(a, qp + t0 * a.q_t * ES, l, r0, t0, q_token, q_head, a.D, live);
-    Rows<DT, DP, kThreads>::fetch(a, qp + (t0 * a.q_t + a.q_h) * ES, l + L::kQ, r0, t0, q_token, q_head, a.D, live);
-    Rows<DT, DVP, kThreads>::fetch(a, gp + t0 * a.g_t * ES, l + 2 * L::kQ, r0, t0, g_token, g_head, a.Dv, live);
-    const int mine = r0 + (lane & 31), r = r0 + which;
-    lam = mine < end ? lam_of(a, hk * a.G + mine - token_of(a, mine) * a.G) : 0.f;
-    if (what < 2) value = r < end ? lse[what * rows + r] : __builtin_inff();
-    else if (what < 4) value = r < end ? delta[(what - 2) * rows + r] : 0.f;
-    else if (what == 4) value = __int_as_float(r < end ? last_key(a, b, token_of(a, r)) : -1);
+    int thread = threadIdx.x;
+    asm("" : "+v"(thread) : "s"(r0));  // what follows from it is formed anew in each tile
+    uint32_t at[4 * L::kOffsets];
+    if (steady) {
+#pragma unroll
+      for (int i = 0; i < L::kOffsets; ++i) {
+        const u32x4 x = lds16(lds_address(lds) + L::kOffsetsAt + (i * kThreads + thread) * 16);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) at[4 * i + e] = x[e];
+      }
+    } else {
+      place(r0, at);
+    }
+    Q::fetch(qp + t0 * a.q_t * ES, l, at, live, thread);
+    Q::fetch(qp + (t0 * a.q_t + a.q_h) * ES, l + L::kQ, at, live, thread);
+    G::fetch(gp + t0 * a.g_t * ES, l + 2 * L::kQ, at + Q::N, live, thread);
+    if (wave * 1024 < kTile * Rec::kBytes) {  // rows past the end have records of zeros
+      const int row = thread / (Rec::kBytes / 16);
+      int column = thread % (Rec::kBytes / 16);
+      if constexpr (Rec::kParts) column ^= swizzle<64>(row);
+      dma16(uniform4(make_rsrc(records + (int64_t)r0 * Rec::kBytes, kOutside - 1)), l + 2 * L::kQ + L::kG + wave * 1024,
+            row < kTile && r0 + row < end ? row * Rec::kBytes + column * 16 : kOutside);
+    }
   };
+  int byte = 0;
   if (first < end) {
-    byte = row_byte(first);
-    fetch(first, 0, key_word(byte));
+    fetch(first, 0, key_word(row_byte(first)));
     byte = row_byte(first + kTile);
   }
-  int stage = 0;
-  for (int r0 = first; r0 < end; r0 += kTile, stage ^= 1) {
-    char* l = lds + stage * L::kStage;
-    float* of_rows = (float*)(l + 2 * L::kQ + L::kG);
-    // The second map's factor goes into its exponent, its sign into a bit a row.
-    const uint32_t minus = (uint32_t)__ballot(lam < 0.f);
-    const float bits = __builtin_amdgcn_logf(fabsf(lam));  // base 2; -inf for none
-    const float factor = __shfl(bits, which, kWave);
-    if (what == 1) value -= factor;
-    if (what < 5) of_rows[what * kTile + which] = value;
+  const Reader<DT, DP> q_reader(lds, lane);
+  const Reader<DT, DVP> g_reader(lds + 2 * L::kQ, lane);
+  const int to_values = 2 * L::kStage + wave * L::kOf - 2 * L::kQ;  // of the wave's keys, from g's tile
+  const Reader<DT, 32> record_reader(lds + 2 * L::kQ + L::kG, lane);
+  const auto step = [&](int r0, auto of) __attribute__((always_inline)) {
+    constexpr int stage = decltype(of)::value;
+    constexpr int skip = stage * L::kStage;
     __syncthreads();
     if (r0 + kTile < end) {
       fetch(r0 + kTile, stage ^ 1, key_word(byte));
       byte = row_byte(r0 + 2 * kTile);
     }
-    if (!work) continue;
-    bool some = false;
-    if (a.causal) {
-      if (token_of(a, min(r0 + kTile, rows) - 1) + a.q_start < key0) continue;
-      some = token_of(a, r0) + a.q_start < key0 + kTile - 1;
-    }
-    const char* lg = l + 2 * L::kQ;
-    f32x16 s0 = zeros(), s1 = zeros(), dp = zeros();
+    if (!work || r0 + kTile <= from_some) return;
+    const auto lq = q_reader.fresh(r0);
+    const auto lg = g_reader.fresh(r0);
+    f32x16 s0 = zeros(), s1 = zeros(), dp = zeros(), dp1;
 #pragma unroll
     for (int kk = 0; kk < KD; ++kk) {
-      Mfma32<DT>::mma(s0, by_rows<DT, DP>(l, kk, lane), k[0][kk]);
-      Mfma32<DT>::mma(s1, by_rows<DT, DP>(l + L::kQ, kk, lane), k[1][kk]);
+      Mfma32<DT>::mma(s0, lq.rows(skip, kk), k[0][kk]);
+      Mfma32<DT>::mma(s1, lq.rows(skip + L::kQ, kk), k[1][kk]);
     }
 #pragma unroll
-    for (int kk = 0; kk < KV; ++kk) Mfma32<DT>::mma(dp, by_rows<DT, DVP>(lg, kk, lane), v[kk]);
+    for (int kk = 0; kk < KV; ++kk) {
+      if constexpr (L::kValues) Mfma32<DT>::mma(dp, lg.rows(skip, kk), lg.rows(to_values, kk));
+      else Mfma32<DT>::mma(dp, lg.rows(skip, kk), v[kk]);
+    }
+    if constexpr (Rec::kParts) {
+      const auto lr = record_reader.fresh(r0);
+      const u32x4 r1 = lr.rows(skip, 0), r2 = lr.rows(skip, 1);
+      uint32_t low = in_low;
+      asm("" : "+v"(low) : "s"(r0));  // two instructions a tile instead of eight registers
+      const u32x4 of_low = {kOnes & low, kOne & low, 0, 0}, of_high = {kOnes & ~low, kOne & ~low, 0, 0};
+      Mfma32<DT>::mma(s0, r1, of_low);
+      Mfma32<DT>::mma(s1, r2, of_low);
+      Mfma32<DT>::mma(dp, r1, of_high);
+      dp1 = dp;
+      Mfma32<DT>::mma(dp1, r2, of_high);
+    } else {
+      dp1 = dp;
 #pragma unroll
-    for (int i = 0; i < 16; i += 4) {
-      const int x = acc_at(i, half);
-      const f32x4 lse0 = *(const f32x4*)(of_rows + x), lse1 = *(const f32x4*)(of_rows + kTile + x);
-      const f32x4 de0 = *(const f32x4*)(of_rows + 2 * kTile + x), de1 = *(const f32x4*)(of_rows + 3 * kTile + x);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        s0[i + e] = __builtin_amdgcn_exp2f(fmaf(s0[i + e], c, -lse0[e]));
-        s1[i + e] = __builtin_amdgcn_exp2f(fmaf(s1[i + e], c, -lse1[e]));
+      for (int i = 0; i < 16; ++i) {
+        const f32x4 x = *(const f32x4*)(lds + skip + 2 * L::kQ + L::kG + acc_at(i, half) * 16);
+        s0[i] = fmaf(s0[i], c, -x[0]);
+        s1[i] = fmaf(s1[i], c, -x[1]);
+        dp[i] -= x[2];
+        dp1[i] -= x[3];
       }
-      if (minus)
+    }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s1[i + e] = minus >> (x + e) & 1 ? -s1[i + e] : s1[i + e];
-      if (some) {
-        const f32x4 last = *(const f32x4*)(of_rows + 4 * kTile + x);
+    for (int i = 0; i < 16; ++i) {
+      s0[i] = __builtin_amdgcn_exp2f(Rec::kParts ? s0[i] * c : s0[i]);
+      s1[i] = __builtin_amdgcn_exp2f(Rec::kParts ? s1[i] * c : s1[i]);
+    }
+    if (any_minus) {
+      const int r = r0 + (lane & 31);
+      const uint32_t minus =
+          (uint32_t)__ballot(r < rows && lam_of(a, hk * a.G + r - token_of(a, r) * a.G) < 0.f) >> (4 * half);
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (key > __float_as_int(last[e])) s0[i + e] = s1[i + e] = 0.f;
+      for (int i = 0; i < 16; ++i) s1[i] = minus & 1u << acc_at(i, 0) ? -s1[i] : s1[i];
+    }
+    if (r0 < from_all) {
+      const int n = first_row(key0 + (lane & 31)) - r0;
+      const uint32_t seen = (n <= 0 ? ~0u : n >= kTile ? 0u : ~0u << n) >> (4 * half);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        s0[i] = seen & 1u << acc_at(i, 0) ? s0[i] : 0.f;
+        s1[i] = seen & 1u << acc_at(i, 0) ? s1[i] : 0.f;
       }
+    }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float p0 = s0[i + e], p1 = s1[i + e], x0 = DT == DA_F16 ? p0 * small : p0, x1 = DT == DA_F16 ? p1 * small : p1;
-        s0[i + e] = x0 * (dp[i + e] - de0[e]);
-        s1[i + e] = x1 * (de1[e] - dp[i + e]);
-        dp[i + e] = p0 - p1;
-      }
+    for (int i = 0; i < 16; ++i) {
+      const float p0 = s0[i], p1 = s1[i];
+      s0[i] = (DT == DA_F16 ? p0 * small : p0) * dp[i];
+      s1[i] = (DT == DA_F16 ? p1 * small : p1) * -dp1[i];
+      dp[i] = p0 - p1;
     }
 #pragma unroll
     for (int j = 0; j < KC; ++j) {
       const u32x4 x = from_acc<DT>(dp, j), y0 = from_acc<DT>(s0, j), y1 = from_acc<DT>(s1, j);
 #pragma unroll
-      for (int n = 0; n < NV; ++n) Mfma32<DT>::mma(dv[n], by_columns<DT, DVP>(lg, n, j, lane), x);
+      for (int n = 0; n < NV; ++n) Mfma32<DT>::mma(dv[n], lg.columns(skip, n, j), x);
 #pragma unroll
       for (int n = 0; n < ND; ++n) {
-        Mfma32<DT>::mma(dk[0][n], by_columns<DT, DP>(l, n, j, lane), y0);
-        Mfma32<DT>::mma(dk[1][n], by_columns<DT, DP>(l + L::kQ, n, j, lane), y1);
+        Mfma32<DT>::mma(dk[0][n], lq.columns(skip, n, j), y0);
+        Mfma32<DT>::mma(dk[1][n], lq.columns(skip + L::kQ, n, j), y1);
       }
     }
+  };
+  for (int r0 = first; r0 < end; r0 += 2 * kTile) {
+    step(r0, std::integral_constant<int, 0>{});
+    if (r0 + kTile < end) step(r0 + kTile, std::integral_constant<int, 1>{});
   }
   if (key >= a.S) return;
   const float by = a.scale / small;
@@ -338,10 +454,12 @@ __global__ __launch_bounds__(kThreads, DT != DA_F32 && DVP <= 128 ? 2 : 1) void 
     g[kk] = in ? load_run<DT>(a.g + (b * a.g_b + t * a.g_t + h * a.g_h) * ES, (2 * kk + half) * V, a.Dv)
                : u32x4{0, 0, 0, 0};
   const int64_t base = ((int64_t)b * a.Hk + hk) * 2 * rows + r;
-  const float lse0 = in ? a.lse[base] : __builtin_inff(), lse1 = in ? a.lse[base + rows] : __builtin_inff();
-  const float de0 = in ? a.delta[base] : 0.f, de1 = in ? a.delta[base + rows] : 0.f;
+  // The second map's factor comes with its exponential, the sign with its values' gradient.
+  const float lam = in ? lam_of(a, h) : 0.f, sign = lam < 0.f ? 1.f : -1.f;
+  const float lse0 = in ? a.lse[base] : __builtin_inff();
+  const float lse1 = in ? a.lse[base + rows] - log2f(fabsf(lam)) : __builtin_inff();
+  const float de0 = in ? a.delta[base] : 0.f, de1 = in ? -sign * a.delta[base + rows] : 0.f;
   const float c = a.scale * kLog2e, small = small_scale<DT>(a);
-  const float lam = in ? lam_of(a, h) * small : 0.f;
 
   const Keys<DT, DP, kThreads> keys(a.k_t, a.D);
   const Keys<DT, DVP, kThreads> values(a.v_t, a.Dv);
@@ -358,46 +476,54 @@ __global__ __launch_bounds__(kThreads, DT != DA_F32 && DVP <= 128 ? 2 : 1) void 
   for (int n = 0; n < ND; ++n) dq[0][n] = zeros(), dq[1][n] = zeros();
   Live live(a, b, key, end, lane);
   if (live.word) fetch(live.key, 0, live.word);
-  for (int stage = 0; live.word; stage ^= 1) {
+  const Reader<DT, DP> key_reader(lds, lane);
+  const Reader<DT, DVP> value_reader(lds + 2 * L::kK, lane);
+  const auto step = [&](auto of) __attribute__((always_inline)) {
+    constexpr int stage = decltype(of)::value;
     key = live.key;
     const uint32_t word = live.word;
     live.next(a, b, end, lane);
     __syncthreads();
     if (live.word) fetch(live.key, stage ^ 1, live.word);
-    if (key > most) continue;
-    const char* l = lds + stage * L::kStage;
+    if (key > most) return;
+    constexpr int skip = stage * L::kStage;
+    const auto lk = key_reader.fresh(key);
+    const auto lv = value_reader.fresh(key);
     f32x16 s0 = zeros(), s1 = zeros(), dp = zeros();
 #pragma unroll
     for (int kk = 0; kk < KD; ++kk) {
-      Mfma32<DT>::mma(s0, by_rows<DT, DP>(l, kk, lane), q[0][kk]);
-      Mfma32<DT>::mma(s1, by_rows<DT, DP>(l + L::kK, kk, lane), q[1][kk]);
+      Mfma32<DT>::mma(s0, lk.rows(skip, kk), q[0][kk]);
+      Mfma32<DT>::mma(s1, lk.rows(skip + L::kK, kk), q[1][kk]);
     }
 #pragma unroll
-    for (int kk = 0; kk < KV; ++kk) Mfma32<DT>::mma(dp, by_rows<DT, DVP>(l + 2 * L::kK, kk, lane), g[kk]);
+    for (int kk = 0; kk < KV; ++kk) Mfma32<DT>::mma(dp, lv.rows(skip, kk), g[kk]);
     const bool some = word != ~0u || key + kTile - 1 > least;
+    const uint32_t seen = some ? seen_of(word, key, last, half) : ~0u;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       float p0 = __builtin_amdgcn_exp2f(fmaf(s0[i], c, -lse0));
-      float p1 = __builtin_amdgcn_exp2f(fmaf(s1[i], c, -lse1)) * lam;
-      if constexpr (DT == DA_F16) p0 *= small;
+      float p1 = __builtin_amdgcn_exp2f(fmaf(s1[i], c, -lse1));
+      if constexpr (DT == DA_F16) p0 *= small, p1 *= small;
       if (some) {
-        const int x = acc_at(i, half);
-        const bool seen = key + x <= last && (word >> x & 1);
-        p0 = seen ? p0 : 0.f;
-        p1 = seen ? p1 : 0.f;
+        p0 = seen & 1u << acc_at(i, 0) ? p0 : 0.f;
+        p1 = seen & 1u << acc_at(i, 0) ? p1 : 0.f;
       }
       s0[i] = p0 * (dp[i] - de0);
-      s1[i] = p1 * (de1 - dp[i]);
+      s1[i] = p1 * fmaf(dp[i], sign, de1);
     }
 #pragma unroll
     for (int j = 0; j < KC; ++j) {
       const u32x4 y0 = from_acc<DT>(s0, j), y1 = from_acc<DT>(s1, j);
 #pragma unroll
       for (int n = 0; n < ND; ++n) {
-        Mfma32<DT>::mma(dq[0][n], by_columns<DT, DP>(l, n, j, lane), y0);
-        Mfma32<DT>::mma(dq[1][n], by_columns<DT, DP>(l + L::kK, n, j, lane), y1);
+        Mfma32<DT>::mma(dq[0][n], lk.columns(skip, n, j), y0);
+        Mfma32<DT>::mma(dq[1][n], lk.columns(skip + L::kK, n, j), y1);
       }
     }
+  };
+  while (live.word) {
+    step(std::integral_constant<int, 0>{});
+    if (live.word) step(std::integral_constant<int, 1>{});
   }
   if (r >= rows) return;
   const float by = a.scale / small;
@@ -449,14 +575,14 @@ void share(int64_t mine, int64_t others, int64_t groups, int64_t cus, int* block
 }
 
 // How the two passes are shared out, and the workspace: delta, the parts of dlam, the largest
-// |g|, and the sums of the splits (of one pass after the other).
+// |g|, the records, and the sums of the splits (of one pass after the other).
 struct Plan {
   Args keys, rows;  // blocks, splits, each
-  int64_t parts_at, most_at, sums_at;
+  int64_t records_at, parts_at, most_at, sums_at;  // in floats
   size_t bytes;
 };
 
-int plan(int64_t batch, int64_t heads, int64_t k_heads, int64_t T, int64_t S, int64_t D, int64_t Dv, Args* a, Plan* p) {
+int plan(int dtype, int64_t batch, int64_t heads, int64_t k_heads, int64_t T, int64_t S, int64_t D, int64_t Dv, Args* a, Plan* p) {
   int64_t cus;
   const int rc = device_cu_count(&cus);
   if (rc) return rc;
@@ -464,7 +590,8 @@ int plan(int64_t batch, int64_t heads, int64_t k_heads, int64_t T, int64_t S, in
   chunks_of(batch * heads, T, cus, &a->chunk, &a->chunks);
   share(S, rows, batch * k_heads, cus, &p->keys.blocks, &p->keys.splits, &p->keys.each);
   share(rows, S, batch * k_heads, cus, &p->rows.blocks, &p->rows.splits, &p->rows.each);
-  p->parts_at = batch * heads * T * 2;
+  p->records_at = (batch * heads * T * 2 + 3) / 4 * 4;
+  p->parts_at = p->records_at + batch * heads * T * (dtype == DA_BF16 ? Record<DA_BF16>::kBytes : Record<DA_F32>::kBytes) / 4;
   p->most_at = p->parts_at + batch * heads * a->chunks;
   p->sums_at = (p->most_at + 4) / 4 * 4;
   const int64_t of_keys = p->keys.splits > 1 ? p->keys.splits * batch * S * k_heads * (2 * D + Dv) : 0;
@@ -497,7 +624,7 @@ int da_diff_attention_grad_workspace(int dtype, int64_t batch, int64_t q_len, in
   if (rc || batch == 0) return rc;
   Args a;
   Plan p;
-  rc = plan(batch, heads, k_heads, q_len, k_len, d, dv, &a, &p);
+  rc = plan(dtype, batch, heads, k_heads, q_len, k_len, d, dv, &a, &p);
   if (rc == DA_OK) *bytes = p.bytes;
   return rc;
 }
@@ -522,7 +649,7 @@ int da_diff_attention_grad(const da_diff_inputs* in, const void* g, int64_t g_bs
     rc = check_side(what, "g", g, (int)elem_bytes(dtype), dv, q_len, a.G, g_bstride, g_tstride, g_hstride);
   if (rc) return rc;
   Plan p;
-  rc = plan(batch, heads, k_heads, q_len, k_len, d, dv, &a, &p);
+  rc = plan(dtype, batch, heads, k_heads, q_len, k_len, d, dv, &a, &p);
   if (rc) return rc;
   if (!workspace || workspace_bytes < p.bytes)
     return set_error(DA_ERR_WORKSPACE, "%s: workspace of %zu bytes needed", what, p.bytes);
@@ -535,6 +662,7 @@ int da_diff_attention_grad(const da_diff_inputs* in, const void* g, int64_t g_bs
   a.out = (char*)const_cast<void*>(out), a.second = (char*)const_cast<void*>(second);
   a.lse = const_cast<float*>(lse);
   a.delta = (float*)workspace;
+  a.records = (char*)(a.delta + p.records_at);
   a.lam_part = a.delta + p.parts_at;
   a.most = a.delta + p.most_at;
   a.part = a.delta + p.sums_at;
