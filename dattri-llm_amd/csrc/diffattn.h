@@ -263,6 +263,25 @@ __device__ __forceinline__ u32x4 rest_of(const f32x16& x, int j, u32x4 p) {
   return v;
 }
 
+// The other half's value: lane l's of lane l ^ 32.
+__device__ __forceinline__ float other_half(float v) {
+  const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(__lane_id() < 32 ? x[1] : x[0]);
+}
+
+// Over an accumulator's registers, in a tree.
+template <class Op>
+__device__ __forceinline__ float over_acc(const f32x16& x, Op op) {
+  float v[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = op(x[i], x[i + 8]);
+#pragma unroll
+  for (int n = 4; n > 0; n /= 2)
+#pragma unroll
+    for (int i = 0; i < n; ++i) v[i] = op(v[i], v[i + n]);
+  return v[0];
+}
+
 // Row r of an accumulator's registers within its tile.
 __device__ __forceinline__ int acc_at(int r, int half) { return 8 * (r >> 2) + 4 * half + (r & 3); }
 

@@ -138,10 +138,8 @@ __global__ __launch_bounds__(2 * NG * kWave, 2) void diff_forward(Args a) {
     }
 #pragma unroll
     for (int n = 0; n < R; ++n) {
-      float x = s[n][0];
-#pragma unroll
-      for (int i = 1; i < 16; ++i) x = fmaxf(x, s[n][i]);
-      x = fmaxf(x, __shfl_xor(x, 32, kWave)) * c;
+      float x = over_acc(s[n], [](float u, float v) { return fmaxf(u, v); });
+      x = fmaxf(x, other_half(x)) * c;
       if (__any(x > top[n] + kSlack)) {  // kLowest + 8 is kLowest
         const float now = fmaxf(top[n], x), by = __builtin_amdgcn_exp2f(top[n] - now);
         top[n] = now;
@@ -152,10 +150,8 @@ __global__ __launch_bounds__(2 * NG * kWave, 2) void diff_forward(Args a) {
           for (int i = 0; i < 16; ++i) o[n][y][i] *= by;
       }
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        s[n][i] = __builtin_amdgcn_exp2f(fmaf(s[n][i], c, -top[n]));
-        sum[n] += s[n][i];
-      }
+      for (int i = 0; i < 16; ++i) s[n][i] = __builtin_amdgcn_exp2f(fmaf(s[n][i], c, -top[n]));
+      sum[n] += over_acc(s[n], [](float u, float v) { return u + v; });
     }
 #pragma unroll
     for (int j = 0; j < KC; ++j) {
@@ -182,7 +178,7 @@ __global__ __launch_bounds__(2 * NG * kWave, 2) void diff_forward(Args a) {
   }
 
 #pragma unroll
-  for (int n = 0; n < R; ++n) sum[n] += __shfl_xor(sum[n], 32, kWave);
+  for (int n = 0; n < R; ++n) sum[n] += other_half(sum[n]);
   if (a.splits > 1) {  // this split's sums
 #pragma unroll
     for (int n = 0; n < R; ++n) {
@@ -354,6 +350,9 @@ int plan(int dtype, int w, int64_t batch, int64_t T, int64_t S, int64_t k_heads,
   *shape = {1, 1};
   if (dtype != DA_F32 && w < 2 && heads * blocks_of(4) >= 2 * cus) *shape = {2, 2};
   else if (heads * blocks_of(2) >= 2 * cus) *shape = {1, 2};
+#ifdef DIFF_R
+  if (shape->ng == 2) *shape = {DIFF_R, 2};
+#endif
   const int64_t blocks = blocks_of(shape->r * shape->ng), groups = std::max<int64_t>(1, heads * blocks);
   // Keys are split where the rows leave CUs without work: up to eight workgroups a CU, no
   // split under 256 keys.

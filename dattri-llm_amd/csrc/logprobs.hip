@@ -12,11 +12,12 @@
 // 16 bytes, with one rescaling a batch of runs.  A row is one workgroup's,
 // or with few rows cut into parts that a second launch joins.
 //
-// The alternatives need no second pass over the row.  Every thread knows its own largest
-// entry, so the k-th largest of 64 groups' maxima is a bound that at least k entries
-// reach; only the threads whose maximum reaches it read their runs again and put what
-// reaches it into LDS.  Entries are ordered by (value, lower index first), as one 64-bit
-// key each, so that no two are alike and their ranks are their places.
+// The alternatives need no second pass over the row.  Every thread knows its largest
+// value and the batch of runs that has it first, so the k-th largest of 64 groups' maxima is
+// a bound that at least k entries reach; the runs of the threads whose maximum may reach
+// it, few of them, are read again by all threads, and what reaches it goes to LDS.  Entries
+// are ordered by (value, lower index first), as one 64-bit key each, so that no two are
+// alike and their ranks are their places.
 #include <algorithm>
 #include <type_traits>
 
@@ -113,18 +114,10 @@ struct Stats {
   }
 };
 
-// A row's outputs from its sums.
-__device__ void finish(const LpArgs& a, int64_t row, int64_t b, int64_t t, const char* logits, int dt, float c,
-                       const Stats& x) {
-  const int64_t target = a.targets[b * a.t_b + t * a.t_t];
+// A row's outputs from its sums and its target's logit.
+__device__ void finish(const LpArgs& a, int64_t row, bool named, float logit, float c, const Stats& x) {
   const float bits = log2f(x.s);
-  float logprob = 0.f;
-  if (target >= 0 && target < a.vocab) {
-    const float v = dt == DA_F32 ? Elem<DA_F32>::load(logits, target)
-                    : dt == DA_BF16 ? Elem<DA_BF16>::load(logits, target) : Elem<DA_F16>::load(logits, target);
-    logprob = ((v - x.m) * c - bits) * kLn2;
-  }
-  a.logprob[row] = logprob;
+  a.logprob[row] = named ? ((logit - x.m) * c - bits) * kLn2 : 0.f;
   a.entropy[row] = (bits - x.e / x.s) * kLn2;
   a.lse[row] = fmaf(x.m, a.inv_temperature, bits * kLn2);
 }
@@ -141,10 +134,15 @@ __device__ __forceinline__ uint64_t wave_max_key(uint64_t k) {
 
 // The top-th largest of 64 keys, one a lane (0: none).
 __device__ __forceinline__ uint64_t bound_of(uint64_t k, int top) {
+  const int hi = (int)(k >> 32), lo = (int)(uint32_t)k;
+  const auto of = [&](int l) {
+    return (uint64_t)(uint32_t)__builtin_amdgcn_readlane(hi, l) << 32 | (uint32_t)__builtin_amdgcn_readlane(lo, l);
+  };
   int above = 0;
-  for (int l = 0; l < kWave; ++l) above += (uint64_t)__shfl((unsigned long long)k, l, kWave) > k;
+#pragma unroll 8
+  for (int l = 0; l < kWave; ++l) above += of(l) > k;
   const uint64_t at = __ballot(k != 0 && above == top - 1);
-  return at ? (uint64_t)__shfl((unsigned long long)k, __ffsll((unsigned long long)at) - 1, kWave) : 0;
+  return at ? of(__ffsll((unsigned long long)at) - 1) : 0;
 }
 
 // The top largest of n different keys in LDS, in order, to f(place, key).
@@ -167,8 +165,9 @@ __global__ __launch_bounds__(NT) void logprobs_forward(LpArgs a) {
   __shared__ float stat[3][kWaves];
   __shared__ uint64_t maxima[kTop ? kGroups : 1];
   __shared__ uint64_t found[kTop ? kCandidates : 1];
+  __shared__ uint16_t winner[kTop ? NT : 1];
   __shared__ uint64_t bound_at;
-  __shared__ int count;
+  __shared__ int count, winners;
   const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
   const int64_t row = blockIdx.x / a.parts, part = blockIdx.x - row * a.parts;
   const int64_t b = row / a.tokens, t = row - b * a.tokens;
@@ -184,13 +183,21 @@ __global__ __launch_bounds__(NT) void logprobs_forward(LpArgs a) {
   const char* logits = a.logits + (b * a.l_b + t * a.l_t) * ES;
   const int64_t v0 = part * a.part, end = min(v0 + a.part, a.vocab);
   const float c = a.inv_temperature * kLog2e;
+  // The target's logit comes with the first runs.
+  const int64_t target = a.targets[b * a.t_b + t * a.t_t];
+  const bool named = target >= 0 && target < a.vocab;
+  const float logit = named && a.parts == 1 ? Elem<DT>::load(logits, target) : 0.f;
+  constexpr int64_t kStride = (int64_t)NT * V * kBatch;
   Stats x = {kFloor, 0.f, 0.f};
   float most = -__builtin_inff();  // the thread's largest logit, and the batch that has it first
   int64_t most_at = v0 + (int64_t)tid * V;
-  for (int64_t v = v0 + (int64_t)tid * V; v < end; v += (int64_t)NT * V * kBatch) {
-    u32x4 raw[kBatch];
+  u32x4 raw[kBatch];
+  const auto fetch = [&](int64_t v) {
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) raw[i] = load_run<DT>(logits, v + (int64_t)i * NT * V, end);
+  };
+  fetch(most_at);
+  for (int64_t v = most_at; v < end; v += kStride) {
     float f[kBatch][V], top = -__builtin_inff();
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
@@ -198,6 +205,7 @@ __global__ __launch_bounds__(NT) void logprobs_forward(LpArgs a) {
 #pragma unroll
       for (int e = 0; e < V; ++e) top = fmaxf(top, f[i][e]);
     }
+    fetch(v + kStride);
     if (kTop && top > most) most = top, most_at = v;
     if (__any(top > x.m)) {
       const float m = fmaxf(x.m, top), by = (x.m - m) * c, scale = __builtin_amdgcn_exp2f(by);
@@ -214,28 +222,16 @@ __global__ __launch_bounds__(NT) void logprobs_forward(LpArgs a) {
         x.e += da_mul_or_zero(p, d);  // 0 where p is: a logit of -inf
       }
   }
-  Stats sum = x;
-#pragma unroll
-  for (int off = 1; off < kWave; off <<= 1)
-    sum.join(__shfl_xor(sum.m, off, kWave), __shfl_xor(sum.s, off, kWave), __shfl_xor(sum.e, off, kWave), c);
-  if (lane == 0) stat[0][wave] = sum.m, stat[1][wave] = sum.s, stat[2][wave] = sum.e;
-  uint64_t mine = 0;
+  {  // the wave's, relative to its maximum
+    const float m = lanes_max<kWave>(x.m), by = (x.m - m) * c, scale = __builtin_amdgcn_exp2f(by);
+    const float s = lanes_sum<kWave>(x.s * scale);
+    const float e = lanes_sum<kWave>(scale * (x.e + da_mul_or_zero(x.s, by)));
+    if (lane == 0) stat[0][wave] = m, stat[1][wave] = s, stat[2][wave] = e;
+  }
+  const bool mine = kTop && v0 + (int64_t)tid * V < end;
   if constexpr (kTop) {
-    if (most_at < end) {  // the first entry of the batch that has the thread's largest
-      int64_t first = most_at;
-      bool seen = false;
-#pragma unroll
-      for (int i = 0; i < kBatch; ++i) {
-        const int64_t at = most_at + (int64_t)i * NT * V;
-        float f[V];
-        unpack16<DT>(load_run<DT>(logits, at, end), f);
-#pragma unroll
-        for (int e = 0; e < V; ++e)
-          if (!seen && f[e] == most && at + e < end) first = at + e, seen = true;
-      }
-      mine = key_of(most, first);
-    }
-    uint64_t k = mine;
+    // At least as good as this is one entry of the thread: the last place of that batch.
+    uint64_t k = mine ? key_of(most, most_at + (kBatch - 1) * (int64_t)NT * V + V - 1) : 0;
     constexpr int kEach = NT / kGroups;  // threads of a group
 #pragma unroll
     for (int off = 1; off < kEach; off <<= 1) {
@@ -243,7 +239,7 @@ __global__ __launch_bounds__(NT) void logprobs_forward(LpArgs a) {
       k = o > k ? o : k;
     }
     if (tid % kEach == 0) maxima[tid / kEach] = k;
-    if (tid == 0) count = 0;
+    if (tid == 0) count = winners = 0;
   }
   __syncthreads();
   if (wave == 0) {
@@ -251,7 +247,7 @@ __global__ __launch_bounds__(NT) void logprobs_forward(LpArgs a) {
     for (int w = 1; w < kWaves; ++w) all.join(stat[0][w], stat[1][w], stat[2][w], c);
     if (a.parts == 1) {
       stat[0][0] = all.m, stat[1][0] = all.s;
-      if (lane == 0) finish(a, row, b, t, logits, DT, c, all);
+      if (lane == 0) finish(a, row, named, logit, c, all);
     } else if (lane == 0) {
       a.stats[blockIdx.x] = float4{all.m, all.s, all.e, 0.f};
     }
@@ -263,18 +259,24 @@ __global__ __launch_bounds__(NT) void logprobs_forward(LpArgs a) {
   if constexpr (!kTop) return;
   __syncthreads();
   const uint64_t bound = bound_at;
-  if (mine != 0 && mine >= bound) {
-    for (int64_t v = v0 + (int64_t)tid * V; v < end; v += (int64_t)NT * V) {
-      float f[V];
-      unpack16<DT>(load_run<DT>(logits, v, end), f);
+  // At best the thread's largest is the first place of its batch.
+  if (mine && key_of(most, most_at) >= bound) winner[atomicAdd(&winners, 1)] = (uint16_t)tid;
+  __syncthreads();
+  // Runs of a thread, the same for all (those past the end hold nothing).
+  const int each = (int)((end - v0 + (int64_t)NT * V - 1) / ((int64_t)NT * V)), again = winners * each;
+#pragma unroll 2
+  for (int i = tid; i < again; i += NT) {
+    const int w = i / each;
+    const int64_t v = v0 + ((int64_t)winner[w] + (int64_t)(i - w * each) * NT) * V;
+    float f[V];
+    unpack16<DT>(load_run<DT>(logits, v, end), f);
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        if (v + e >= end) continue;
-        const uint64_t k = key_of(f[e], v + e);
-        if (k < bound) continue;
-        const int at = atomicAdd(&count, 1);  // places do not matter: keys are ranked
-        if (at < kCandidates) found[at] = k;
-      }
+    for (int e = 0; e < V; ++e) {
+      if (v + e >= end) continue;
+      const uint64_t k = key_of(f[e], v + e);
+      if (k < bound) continue;
+      const int at = atomicAdd(&count, 1);  // places do not matter: keys are ranked
+      if (at < kCandidates) found[at] = k;
     }
   }
   __syncthreads();
@@ -338,6 +340,11 @@ __global__ __launch_bounds__(kJoin) void logprobs_join(LpArgs a, int dt) {
   if (a.mask && !a.mask[b * a.m_b + t * a.m_t]) return;  // written by the first launch
   const float c = a.inv_temperature * kLog2e;
   const int parts = (int)a.parts, n = kTop ? parts * a.top : 0;
+  const int64_t target = a.targets[b * a.t_b + t * a.t_t];
+  const bool named = target >= 0 && target < a.vocab;
+  const char* logits = a.logits + (b * a.l_b + t * a.l_t) * (dt == DA_F32 ? 4 : 2);
+  const float logit = !named ? 0.f : dt == DA_F32 ? Elem<DA_F32>::load(logits, target)
+                      : dt == DA_BF16 ? Elem<DA_BF16>::load(logits, target) : Elem<DA_F16>::load(logits, target);
   if (tid < kWave) {
     Stats x = {kFloor, 0.f, 0.f};
     if (tid < parts) {
@@ -348,8 +355,7 @@ __global__ __launch_bounds__(kJoin) void logprobs_join(LpArgs a, int dt) {
     for (int off = 1; off < kWave; off <<= 1)
       x.join(__shfl_xor(x.m, off, kWave), __shfl_xor(x.s, off, kWave), __shfl_xor(x.e, off, kWave), c);
     if (tid == 0) {
-      const int es = dt == DA_F32 ? 4 : 2;
-      finish(a, row, b, t, a.logits + (b * a.l_b + t * a.l_t) * es, dt, c, x);
+      finish(a, row, named, logit, c, x);
       stat[0] = x.m, stat[1] = x.s;
       count = 0;
     }
