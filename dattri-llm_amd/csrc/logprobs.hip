@@ -68,23 +68,13 @@ __device__ __forceinline__ uint32_t none() {  // -inf in every place of a word
   return DT == DA_F32 ? 0xff800000u : DT == DA_BF16 ? 0xff80ff80u : 0xfc00fc00u;
 }
 
-// The run at v0 of a row; entries from end on are -inf and not read.
+// The run at v0 of a row where all of it lies before `end`, else -inf and nothing is read.
+// (No other case: a row's last entries that are no whole run are read one a thread, so that
+// no load has a branch behind it that would have to wait for the others.)
 template <int DT>
 __device__ __forceinline__ u32x4 load_run(const char* row, int64_t v0, int64_t end) {
-  constexpr int ES = Elem<DT>::kBytes, V = Elem<DT>::kVec;
-  if (v0 + V <= end) return ld16_any<ES>(row + v0 * ES);
   u32x4 w = {none<DT>(), none<DT>(), none<DT>(), none<DT>()};
-  if (v0 >= end) return w;
-#pragma unroll
-  for (int e = 0; e < V; ++e) {
-    if (v0 + e >= end) continue;
-    if constexpr (ES == 4) {
-      w[e] = *(const uint32_t*)(row + (v0 + e) * 4);
-    } else {
-      const uint32_t bits = *(const uint16_t*)(row + (v0 + e) * 2);
-      w[e / 2] = e % 2 ? (w[e / 2] & 0xffffu) | bits << 16 : (w[e / 2] & 0xffff0000u) | bits;
-    }
-  }
+  if (v0 + Elem<DT>::kVec <= end) w = ld16_any<Elem<DT>::kBytes>(row + v0 * Elem<DT>::kBytes);
   return w;
 }
 
@@ -188,16 +178,11 @@ __global__ __launch_bounds__(NT) void logprobs_forward(LpArgs a) {
   const bool named = target >= 0 && target < a.vocab;
   const float logit = named && a.parts == 1 ? Elem<DT>::load(logits, target) : 0.f;
   constexpr int64_t kStride = (int64_t)NT * V * kBatch;
+  const int64_t whole = end - (end - v0) % V;  // where the whole runs end
   Stats x = {kFloor, 0.f, 0.f};
   float most = -__builtin_inff();  // the thread's largest logit, and the batch that has it first
   int64_t most_at = v0 + (int64_t)tid * V;
-  u32x4 raw[kBatch];
-  const auto fetch = [&](int64_t v) {
-#pragma unroll
-    for (int i = 0; i < kBatch; ++i) raw[i] = load_run<DT>(logits, v + (int64_t)i * NT * V, end);
-  };
-  fetch(most_at);
-  for (int64_t v = most_at; v < end; v += kStride) {
+  const auto add = [&](const u32x4 (&raw)[kBatch], int64_t v) __attribute__((always_inline)) {
     float f[kBatch][V], top = -__builtin_inff();
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
@@ -205,7 +190,6 @@ __global__ __launch_bounds__(NT) void logprobs_forward(LpArgs a) {
 #pragma unroll
       for (int e = 0; e < V; ++e) top = fmaxf(top, f[i][e]);
     }
-    fetch(v + kStride);
     if (kTop && top > most) most = top, most_at = v;
     if (__any(top > x.m)) {
       const float m = fmaxf(x.m, top), by = (x.m - m) * c, scale = __builtin_amdgcn_exp2f(by);
@@ -221,6 +205,39 @@ __global__ __launch_bounds__(NT) void logprobs_forward(LpArgs a) {
         x.s += p;
         x.e += da_mul_or_zero(p, d);  // 0 where p is: a logit of -inf
       }
+  };
+  // Batches that are whole for every thread, the next one on its way (the last again in its
+  // place: no load has a condition); then one that is not.
+  const int64_t full = (whole - v0) / kStride;
+  int64_t v = v0 + (int64_t)tid * V;
+  u32x4 raw[kBatch];
+  if (full) {
+    const char* at = logits + v * ES;
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) raw[i] = ld16_any<ES>(at + i * (NT * 16));
+    for (int64_t n = full; n > 0; --n, v += kStride) {
+      u32x4 now[kBatch];
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) now[i] = raw[i];
+      at += n > 1 ? kStride * ES : 0;
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) raw[i] = ld16_any<ES>(at + i * (NT * 16));
+      add(now, v);
+    }
+  }
+  const bool left = v0 + full * kStride < end;
+  float rest = -__builtin_inff();  // one of the last entries, no whole run
+  const bool has_rest = tid < end - whole;
+  if (left) {
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) raw[i] = load_run<DT>(logits, v + (int64_t)i * NT * V, whole);
+    if (has_rest) rest = Elem<DT>::load(logits, whole + tid);
+    add(raw, v);
+    const float m = fmaxf(x.m, rest), by = (x.m - m) * c, scale = __builtin_amdgcn_exp2f(by);
+    const float d = (rest - m) * c, p = __builtin_amdgcn_exp2f(d);
+    x.e = scale * (x.e + da_mul_or_zero(x.s, by)) + da_mul_or_zero(p, d);
+    x.s = x.s * scale + p;
+    x.m = m;
   }
   {  // the wave's, relative to its maximum
     const float m = lanes_max<kWave>(x.m), by = (x.m - m) * c, scale = __builtin_amdgcn_exp2f(by);
@@ -228,10 +245,14 @@ __global__ __launch_bounds__(NT) void logprobs_forward(LpArgs a) {
     const float e = lanes_sum<kWave>(scale * (x.e + da_mul_or_zero(x.s, by)));
     if (lane == 0) stat[0][wave] = m, stat[1][wave] = s, stat[2][wave] = e;
   }
-  const bool mine = kTop && v0 + (int64_t)tid * V < end;
+  const bool mine = kTop && v0 + (int64_t)tid * V < whole;
   if constexpr (kTop) {
     // At least as good as this is one entry of the thread: the last place of that batch.
     uint64_t k = mine ? key_of(most, most_at + (kBatch - 1) * (int64_t)NT * V + V - 1) : 0;
+    if (has_rest) {
+      const uint64_t o = key_of(rest, whole + tid);
+      k = o > k ? o : k;
+    }
     constexpr int kEach = NT / kGroups;  // threads of a group
 #pragma unroll
     for (int off = 1; off < kEach; off <<= 1) {
@@ -262,22 +283,24 @@ __global__ __launch_bounds__(NT) void logprobs_forward(LpArgs a) {
   // At best the thread's largest is the first place of its batch.
   if (mine && key_of(most, most_at) >= bound) winner[atomicAdd(&winners, 1)] = (uint16_t)tid;
   __syncthreads();
+  const auto keep = [&](float f, int64_t at) __attribute__((always_inline)) {
+    const uint64_t k = key_of(f, at);
+    if (k < bound) return;
+    const int place = atomicAdd(&count, 1);  // places do not matter: keys are ranked
+    if (place < kCandidates) found[place] = k;
+  };
+  if (has_rest) keep(rest, whole + tid);
   // Runs of a thread, the same for all (those past the end hold nothing).
-  const int each = (int)((end - v0 + (int64_t)NT * V - 1) / ((int64_t)NT * V)), again = winners * each;
+  const int each = (int)((whole - v0 + (int64_t)NT * V - 1) / ((int64_t)NT * V)), again = winners * each;
 #pragma unroll 2
   for (int i = tid; i < again; i += NT) {
     const int w = i / each;
     const int64_t v = v0 + ((int64_t)winner[w] + (int64_t)(i - w * each) * NT) * V;
+    if (v + V > whole) continue;
     float f[V];
-    unpack16<DT>(load_run<DT>(logits, v, end), f);
+    unpack16<DT>(load_run<DT>(logits, v, whole), f);
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-      if (v + e >= end) continue;
-      const uint64_t k = key_of(f[e], v + e);
-      if (k < bound) continue;
-      const int at = atomicAdd(&count, 1);  // places do not matter: keys are ranked
-      if (at < kCandidates) found[at] = k;
-    }
+    for (int e = 0; e < V; ++e) keep(f[e], v + e);
   }
   __syncthreads();
   int n = count;
@@ -307,14 +330,16 @@ __global__ __launch_bounds__(NT) void logprobs_forward(LpArgs a) {
   uint64_t last = ~0ull;
   for (int at = 0; at < a.top; ++at) {
     uint64_t k = 0;
-    for (int64_t v = v0 + (int64_t)tid * V; v < end; v += (int64_t)NT * V) {
+    const auto larger = [&](float f, int64_t v) __attribute__((always_inline)) {
+      const uint64_t o = key_of(f, v);
+      if (o < last && o > k) k = o;
+    };
+    if (has_rest) larger(rest, whole + tid);
+    for (int64_t v = v0 + (int64_t)tid * V; v < whole; v += (int64_t)NT * V) {
       float f[V];
-      unpack16<DT>(load_run<DT>(logits, v, end), f);
+      unpack16<DT>(load_run<DT>(logits, v, whole), f);
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const uint64_t o = v + e < end ? key_of(f[e], v + e) : 0;
-        if (o < last && o > k) k = o;
-      }
+      for (int e = 0; e < V; ++e) larger(f[e], v + e);
     }
     k = wave_max_key(k);
     __syncthreads();
@@ -405,23 +430,28 @@ __global__ __launch_bounds__(NT) void logprobs_backward(LpArgs a) {
   const float up_lse = live && a.up_lse ? a.up_lse[b * a.ul_b + t * a.ul_t] * a.inv_temperature : 0.f;
   const float lse = live ? a.lse_in[row] : 0.f;
   const float whole = up_lse - up - (a.up_h && live ? up_h * a.entropy_in[row] : 0.f), slope = -up_h;
-  for (int64_t v = v0 + (int64_t)threadIdx.x * V; v < end; v += (int64_t)NT * V * kBatch) {
+  const auto of = [&](float f) __attribute__((always_inline)) {
+    const float d = fmaf(f, a.inv_temperature, -lse), p = __builtin_amdgcn_exp2f(d * kLog2e);
+    return live ? da_mul_or_zero(p, fmaf(d, slope, whole)) : 0.f;
+  };
+  const int64_t runs = end - (end - v0) % V;  // where the whole runs end
+  const int last = (int)(end - runs);
+  if ((int)threadIdx.x < last) {
+    const int64_t at = runs + threadIdx.x;
+    Elem<DT>::store(grad, at, of(live ? Elem<DT>::load(logits, at) : 0.f) + (at == target ? up : 0.f));
+  }
+  for (int64_t v = v0 + (int64_t)threadIdx.x * V; v < runs; v += (int64_t)NT * V * kBatch) {
     u32x4 raw[kBatch];
 #pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-      raw[i] = u32x4{0, 0, 0, 0};
-      if (live) raw[i] = load_run<DT>(logits, v + (int64_t)i * NT * V, end);
-    }
+    for (int i = 0; i < kBatch; ++i) raw[i] = load_run<DT>(logits, v + (int64_t)i * NT * V, live ? runs : 0);
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
       const int64_t at = v + (int64_t)i * NT * V;
+      if (at >= runs) continue;
       float f[V];
       unpack16<DT>(raw[i], f);
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const float d = fmaf(f[e], a.inv_temperature, -lse), p = __builtin_amdgcn_exp2f(d * kLog2e);
-        f[e] = live ? da_mul_or_zero(p, fmaf(d, slope, whole)) : 0.f;
-      }
+      for (int e = 0; e < V; ++e) f[e] = of(f[e]);
       if (target >= at && target < at + V) {
 #pragma unroll
         for (int e = 0; e < V; ++e) f[e] += at + e == target ? up : 0.f;
@@ -432,16 +462,7 @@ __global__ __launch_bounds__(NT) void logprobs_backward(LpArgs a) {
         if constexpr (DT == DA_F32) w[k] = __float_as_uint(f[k]);
         else w[k] = pack2<DT>(f[2 * k], f[2 * k + 1]);
       }
-      if (at + V <= end) {
-        st16_any<ES>(grad + at * ES, w);
-      } else {
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-          if (at + e >= end) continue;
-          if constexpr (ES == 4) *(uint32_t*)(grad + (at + e) * 4) = w[e];
-          else *(uint16_t*)(grad + (at + e) * 2) = (uint16_t)(w[e / 2] >> (16 * (e % 2)));
-        }
-      }
+      st16_any<ES>(grad + at * ES, w);
     }
   }
 }
