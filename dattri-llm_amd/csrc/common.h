@@ -247,6 +247,12 @@ __device__ __forceinline__ void st16_any(void* p, u32x4 v) {
   if constexpr (ES == 4) *(u32x4_at4*)p = v;
   else *(u32x4_at2*)p = v;
 }
+// The same with the non-temporal hint: what is written pushes nothing out of the caches.
+template <int ES>
+__device__ __forceinline__ void st16_any_nt(void* p, u32x4 v) {
+  if constexpr (ES == 4) __builtin_nontemporal_store((u32x4_at4)v, (u32x4_at4*)p);
+  else __builtin_nontemporal_store((u32x4_at2)v, (u32x4_at2*)p);
+}
 
 // ---------------------------------------------------------------------------
 // Buffer loads straight into LDS (gfx950: 16 bytes per lane).

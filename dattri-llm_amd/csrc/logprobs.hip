@@ -30,6 +30,7 @@ constexpr int kMaxTop = 32;
 constexpr int kGroups = 64;       // groups whose maxima bound the alternatives: kMaxTop and more
 constexpr int kCandidates = 2048; // entries that reach the bound, at most: past it the row is searched
 constexpr int kBatch = 4;         // runs of 16 bytes a thread has under way
+constexpr int64_t kLastLevel = 256 << 20;  // bytes of the last-level cache
 constexpr float kLog2e = 1.44269504088896341f;
 constexpr float kLn2 = 0.69314718055994531f;
 constexpr float kFloor = -3.4028234663852886e38f;  // the maximum where there is none or -inf: the lowest value
@@ -411,12 +412,15 @@ __global__ __launch_bounds__(kJoin) void logprobs_join(LpArgs a, int dt) {
 }
 
 // ---------------------------------------------------------------------------
-// Backward: workgroup (row, part), a run of 16 bytes a thread and step.
+// Backward: workgroup (row, part), the last rows first: a forward call just before left them
+// in the last-level cache.  kStream: gradients that do not fit there are written past it, and
+// leave it to the logits (3 x 509 rows of 50257 in fp32, forward and backward: 195 us without,
+// 163 with both).
 // ---------------------------------------------------------------------------
-template <int DT, int NT>
+template <int DT, int NT, bool kStream>
 __global__ __launch_bounds__(NT) void logprobs_backward(LpArgs a) {
   constexpr int ES = Elem<DT>::kBytes, V = Elem<DT>::kVec;
-  const int64_t row = blockIdx.x / a.parts, part = blockIdx.x - row * a.parts;
+  const int64_t id = gridDim.x - 1 - blockIdx.x, row = id / a.parts, part = id - row * a.parts;
   const int64_t b = row / a.tokens, t = row - b * a.tokens;
   const bool live = !a.mask || a.mask[b * a.m_b + t * a.m_t];
   const char* logits = a.logits + (b * a.l_b + t * a.l_t) * ES;
@@ -462,7 +466,8 @@ __global__ __launch_bounds__(NT) void logprobs_backward(LpArgs a) {
         if constexpr (DT == DA_F32) w[k] = __float_as_uint(f[k]);
         else w[k] = pack2<DT>(f[2 * k], f[2 * k + 1]);
       }
-      st16_any<ES>(grad + at * ES, w);
+      if constexpr (kStream) st16_any_nt<ES>(grad + at * ES, w);
+      else st16_any<ES>(grad + at * ES, w);
     }
   }
 }
@@ -610,7 +615,10 @@ int da_token_logprobs_grad(const float* up, int64_t up_bstride, int64_t up_tstri
   const hipStream_t st = (hipStream_t)stream;
   return by_type(dtype, nt, [&](auto dt, auto n) {
     constexpr int NT = decltype(n)::value;
-    logprobs_backward<decltype(dt)::value, NT><<<(unsigned)(a.rows * a.parts), NT, 0, st>>>(a);
+    constexpr int DT = decltype(dt)::value;
+    const unsigned grid = (unsigned)(a.rows * a.parts);
+    if (a.rows * vocab * (int64_t)elem_bytes(dtype) > kLastLevel / 2) logprobs_backward<DT, NT, true><<<grid, NT, 0, st>>>(a);
+    else logprobs_backward<DT, NT, false><<<grid, NT, 0, st>>>(a);
     return check_launch("da_token_logprobs_grad");
   });
 }
