@@ -51,27 +51,46 @@ struct AddNormArgs {
   float eps;
 };
 
-// Entries e0 .. e0 + kVec of a row of d; those past its end are zero and not read.
-template <int DT>
+// Entries e0 .. e0 + kVec of a row of d.  The run that holds a row's last entries is read
+// from where it ends with the row, and brought to its place by settle() when it is used, so
+// that no load has a branch behind it; runs past the end are zero.  kShort: rows of less than
+// a run, entry by entry.
+template <int DT, bool kStream, bool kShort>
 __device__ __forceinline__ u32x4 load_run(const char* row, int e0, int d) {
   constexpr int ES = Elem<DT>::kBytes, V = Elem<DT>::kVec;
-  if (e0 + V <= d) return ld16_any<ES>(row + (int64_t)e0 * ES);
   u32x4 v = {0, 0, 0, 0};
-  if (e0 >= d) return v;
+  if constexpr (kShort) {
 #pragma unroll
-  for (int e = 0; e < V; ++e) {
-    if (e0 + e >= d) continue;
-    if constexpr (ES == 4) v[e] = *(const uint32_t*)(row + (int64_t)(e0 + e) * 4);
-    else v[e / 2] |= (uint32_t)(*(const uint16_t*)(row + (int64_t)(e0 + e) * 2)) << (16 * (e % 2));
+    for (int e = 0; e < V; ++e) {
+      if (e0 + e >= d) continue;
+      if constexpr (ES == 4) v[e] = *(const uint32_t*)(row + (e0 + e) * 4);
+      else v[e / 2] |= (uint32_t)(*(const uint16_t*)(row + (e0 + e) * 2)) << (16 * (e % 2));
+    }
+  } else if (e0 < d) {
+    const char* p = row + (int64_t)min(e0, d - V) * ES;
+    v = kStream ? ld16_any_nt<ES>(p) : ld16_any<ES>(p);
   }
   return v;
 }
 
-template <int DT>
+template <int DT, bool kShort>
+__device__ __forceinline__ u32x4 settle(u32x4 v, int e0, int d) {
+  constexpr int ES = Elem<DT>::kBytes, V = Elem<DT>::kVec;
+  const int skip = (V - d % V) % V;  // entries before the run's first
+  if (kShort || skip == 0) return v;
+  u32x4 w = v;
+  if (skip * ES & 8) w = u32x4{w[2], w[3], 0, 0};
+  if (skip * ES & 4) w = u32x4{w[1], w[2], w[3], 0};
+  if (skip * ES & 2) w = u32x4{w[0] >> 16 | w[1] << 16, w[1] >> 16 | w[2] << 16, w[2] >> 16 | w[3] << 16, w[3] >> 16};
+  return e0 < d && e0 + V > d ? w : v;
+}
+
+template <int DT, bool kStream = false>
 __device__ __forceinline__ void store_run(char* row, int e0, int d, u32x4 v) {
   constexpr int ES = Elem<DT>::kBytes, V = Elem<DT>::kVec;
   if (e0 + V <= d) {
-    st16_any<ES>(row + (int64_t)e0 * ES, v);
+    if constexpr (kStream) st16_any_nt<ES>(row + (int64_t)e0 * ES, v);
+    else st16_any<ES>(row + (int64_t)e0 * ES, v);
     return;
   }
 #pragma unroll
@@ -115,7 +134,7 @@ __device__ __forceinline__ void store_run8(char* row, int e0, int d, const float
 }
 
 // Weights of a lane's runs, in the rows' type or in fp32.
-template <int DT, bool kWide, int S>
+template <int DT, bool kWide, int S, bool kShort>
 struct Weights {
   static constexpr int V = Elem<DT>::kVec, N = kWide && DT != DA_F32 ? 2 : 1;
   u32x4 raw[S][N];
@@ -124,10 +143,11 @@ struct Weights {
     for (int i = 0; i < S; ++i) {
       const int e0 = (first + i * step) * V;
       if constexpr (N == 2) {
-        raw[i][0] = load_run<DA_F32>(w, e0, d);
-        raw[i][1] = load_run<DA_F32>(w, e0 + 4, d);
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+          raw[i][k] = settle<DA_F32, kShort>(load_run<DA_F32, false, kShort>(w, e0 + 4 * k, d), e0 + 4 * k, d);
       } else {
-        raw[i][0] = load_run<DT>(w, e0, d);
+        raw[i][0] = settle<DT, kShort>(load_run<DT, false, kShort>(w, e0, d), e0, d);
       }
     }
   }
@@ -163,14 +183,14 @@ __device__ __forceinline__ float max_f(float a, float b) { return fmaxf(a, b); }
 // ---------------------------------------------------------------------------
 // Forward.  A workgroup is NW waves on one row, or four waves on a row each.
 // ---------------------------------------------------------------------------
-template <int DT, bool kWide, int NW, int S, int kOut>
+template <int DT, bool kWide, int NW, int S, int kOut, bool kStream, bool kShort>
 __global__ __launch_bounds__(NW == 1 ? 256 : NW * kWave) void add_norm_forward(AddNormArgs a) {
   constexpr int ES = Elem<DT>::kBytes, V = Elem<DT>::kVec, kStep = NW * kWave;
   constexpr int kRows = NW == 1 ? 4 : 1;  // rows of a workgroup
   __shared__ float parts[2][NW];
   const int at = NW == 1 ? threadIdx.x % kWave : threadIdx.x;
   int slot = 0;
-  Weights<DT, kWide, S> w;
+  Weights<DT, kWide, S, kShort> w;
   w.load(a.weight, at, kStep, a.d);
   const int64_t stride = (int64_t)gridDim.x * kRows;
   int64_t row = (int64_t)blockIdx.x * kRows + (NW == 1 ? threadIdx.x / kWave : 0);
@@ -184,11 +204,11 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * kWave) void add_norm_forward(A
 #pragma unroll
     for (int i = 0; i < S; ++i) {
       x[i] = r[i] = u32x4{0, 0, 0, 0};
-      if (live) x[i] = load_run<DT>(xr, (at + i * kStep) * V, a.d);
+      if (live) x[i] = load_run<DT, kStream, kShort>(xr, (at + i * kStep) * V, a.d);
     }
     if (a.residual && live)
 #pragma unroll
-      for (int i = 0; i < S; ++i) r[i] = load_run<DT>(rr, (at + i * kStep) * V, a.d);
+      for (int i = 0; i < S; ++i) r[i] = load_run<DT, kStream, kShort>(rr, (at + i * kStep) * V, a.d);
     b += a.step_b;
     t += a.step_t;
     if (t >= a.tokens) t -= a.tokens, ++b;
@@ -201,8 +221,9 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * kWave) void add_norm_forward(A
 #pragma unroll
     for (int i = 0; i < S; ++i) {
       float p[V], q[V];
-      unpack16<DT>(x[i], p);
-      unpack16<DT>(r[i], q);
+      const int e0 = (at + i * kStep) * V;
+      unpack16<DT>(settle<DT, kShort>(x[i], e0, a.d), p);
+      unpack16<DT>(settle<DT, kShort>(r[i], e0, a.d), q);
 #pragma unroll
       for (int e = 0; e < V; ++e) p[e] += q[e];
       h[i] = pack16<DT>(p);
@@ -218,14 +239,14 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * kWave) void add_norm_forward(A
 #pragma unroll
     for (int i = 0; i < S; ++i) {
       const int e0 = (at + i * kStep) * V;
-      if (total) store_run<DT>(total, e0, a.d, h[i]);
+      if (total) store_run<DT, kStream>(total, e0, a.d, h[i]);
       float p[V], f[V];
       unpack16<DT>(h[i], p);
       w.get(i, f);
 #pragma unroll
       for (int e = 0; e < V; ++e) p[e] = now ? p[e] * rstd * f[e] : 0.f;
       if constexpr (kOut == kPlain) {
-        store_run<DT>(a.out + row * a.d * ES, e0, a.d, pack16<DT>(p));
+        store_run<DT, kStream>(a.out + row * a.d * ES, e0, a.d, pack16<DT>(p));
       } else {
         float top = 0.f;
 #pragma unroll
@@ -265,7 +286,7 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * kWave) void add_norm_forward(A
 // ---------------------------------------------------------------------------
 // Backward.  Workgroup (sample, chunk): its tokens' dx, and their sum of g t.
 // ---------------------------------------------------------------------------
-template <int DT, bool kWide, int NW, int S>
+template <int DT, bool kWide, int NW, int S, bool kStream, bool kShort>
 __global__ __launch_bounds__(NW == 1 ? 256 : NW * kWave) void add_norm_backward(AddNormArgs a) {
   constexpr int ES = Elem<DT>::kBytes, V = Elem<DT>::kVec, kStep = NW * kWave;
   constexpr int kRows = NW == 1 ? 4 : 1;
@@ -276,7 +297,7 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * kWave) void add_norm_backward(
   const int64_t b = blockIdx.x / a.chunks, c = blockIdx.x - b * a.chunks;
   const int64_t t1 = min((c + 1) * a.chunk, a.tokens);
   int64_t t = c * a.chunk + (NW == 1 ? wave : 0);
-  Weights<DT, kWide, S> w;
+  Weights<DT, kWide, S, kShort> w;
   w.load(a.weight, at, kStep, a.d);
   const uint8_t* mask = a.mask ? a.mask + b * a.mask_b : nullptr;
   const char* g0 = a.x + b * a.x_b * ES;
@@ -291,9 +312,9 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * kWave) void add_norm_backward(
       const int e0 = (at + i * kStep) * V;
       g[i] = gt[i] = h[i] = u32x4{0, 0, 0, 0};
       if (live) {
-        h[i] = load_run<DT>(h0 + to * a.h_t * ES, e0, a.d);
-        g[i] = load_run<DT>(g0 + to * a.x_t * ES, e0, a.d);
-        if (gt0) gt[i] = load_run<DT>(gt0 + to * a.r_t * ES, e0, a.d);
+        h[i] = load_run<DT, kStream, kShort>(h0 + to * a.h_t * ES, e0, a.d);
+        g[i] = load_run<DT, kStream, kShort>(g0 + to * a.x_t * ES, e0, a.d);
+        if (gt0) gt[i] = load_run<DT, kStream, kShort>(gt0 + to * a.r_t * ES, e0, a.d);
       }
     }
   };
@@ -308,6 +329,10 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * kWave) void add_norm_backward(
     float sq = 0.f, dot = 0.f;
 #pragma unroll
     for (int i = 0; i < S; ++i) {
+      const int e0 = (at + i * kStep) * V;
+      h[i] = settle<DT, kShort>(h[i], e0, a.d);
+      g[i] = settle<DT, kShort>(g[i], e0, a.d);
+      gt[i] = settle<DT, kShort>(gt[i], e0, a.d);
       float hf[V], gf[V], wf[V];
       unpack16<DT>(h[i], hf);
       unpack16<DT>(g[i], gf);
@@ -341,7 +366,7 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * kWave) void add_norm_backward(
     }
     fetch(t + kRows);
 #pragma unroll
-    for (int i = 0; i < S; ++i) store_run<DT>(out, (at + i * kStep) * V, a.d, dx[i]);
+    for (int i = 0; i < S; ++i) store_run<DT, kStream>(out, (at + i * kStep) * V, a.d, dx[i]);
   }
   if (!a.partial) return;
   if constexpr (NW == 1) {  // the four waves, in order
@@ -394,11 +419,16 @@ __global__ __launch_bounds__(kJoinGroups * kJoinWidth) void add_norm_join(const 
 // ---------------------------------------------------------------------------
 struct Plan {
   int waves, runs;  // waves of a row, runs of 16 bytes a lane
+  bool small;       // rows of less than a run
 };
+
+// Rows that together do not fit the last-level cache (256 MB) are read and written past it.
+constexpr int64_t kStreamBytes = 128 << 20;
 
 // As many waves as leave a lane two runs or more where the rows are wide.
 Plan plan(int64_t d, int dtype) {
-  const int64_t n = (d + (dtype == DA_F32 ? 3 : 7)) / (dtype == DA_F32 ? 4 : 8);
+  const int64_t vec = dtype == DA_F32 ? 4 : 8, n = (d + vec - 1) / vec;
+  if (d < vec) return {1, 1, true};
   if (n <= 64) return {1, 1};
   if (n <= 128) return {1, 2};
   if (n <= 256) return {4, 1};
@@ -433,9 +463,11 @@ int check_rows(const char* what, int dtype, int weight_dtype, int64_t batch, int
   return DA_OK;
 }
 
-// f(waves, runs) with both as constants.
+// f(waves, runs, small) with all as constants.
 template <class F>
-int by_plan(const Plan& p, F f) {
+int by_plan(const Plan& p, F g) {
+  const auto f = [&](auto waves, auto runs) { return g(waves, runs, std::false_type{}); };
+  if (p.small) return g(std::integral_constant<int, 1>{}, std::integral_constant<int, 1>{}, std::true_type{});
   if (p.waves == 1) return p.runs == 1 ? f(std::integral_constant<int, 1>{}, std::integral_constant<int, 1>{})
                                        : f(std::integral_constant<int, 1>{}, std::integral_constant<int, 2>{});
   if (p.waves == 16) return f(std::integral_constant<int, 16>{}, std::integral_constant<int, 4>{});
@@ -494,17 +526,22 @@ int da_add_rms_norm(const void* x, const void* residual, const void* weight, int
   const hipStream_t st = (hipStream_t)stream;
   const Plan p = plan(d, dtype);
   return by_types(dtype, weight_dtype, [&](auto dt, auto wide) {
-    return by_plan(p, [&](auto nw, auto s) {
+    return by_plan(p, [&](auto nw, auto s, auto small) {
       constexpr int DT = decltype(dt)::value, NW = decltype(nw)::value, S = decltype(s)::value;
-      constexpr bool kWide = decltype(wide)::value;
+      constexpr bool kWide = decltype(wide)::value, kShort = decltype(small)::value;
       const int64_t groups = NW == 1 ? (a.rows + 3) / 4 : a.rows;
       const unsigned grid = (unsigned)std::min<int64_t>(groups, cus * (NW > 4 ? 2 : 8));
       const int64_t step = (int64_t)grid * (NW == 1 ? 4 : 1);
       a.step_b = step / tokens, a.step_t = step % tokens;
       constexpr int kN = NW == 1 ? 256 : NW * kWave;
-      if (quantize == kPlain) add_norm_forward<DT, kWide, NW, S, kPlain><<<grid, kN, 0, st>>>(a);
-      else if (quantize == kRowScale) add_norm_forward<DT, kWide, NW, S, kRowScale><<<grid, kN, 0, st>>>(a);
-      else add_norm_forward<DT, kWide, NW, S, kRunScale><<<grid, kN, 0, st>>>(a);
+      const auto launch = [&](auto stream) {
+        constexpr bool kStream = decltype(stream)::value;
+        if (quantize == kPlain) add_norm_forward<DT, kWide, NW, S, kPlain, kStream, kShort><<<grid, kN, 0, st>>>(a);
+        else if (quantize == kRowScale) add_norm_forward<DT, kWide, NW, S, kRowScale, kStream, kShort><<<grid, kN, 0, st>>>(a);
+        else add_norm_forward<DT, kWide, NW, S, kRunScale, kStream, kShort><<<grid, kN, 0, st>>>(a);
+      };
+      if (!kShort && a.rows * d * (int64_t)elem_bytes(dtype) > kStreamBytes / 4) launch(std::bool_constant<!kShort>{});
+      else launch(std::false_type{});
       return check_launch("da_add_rms_norm");
     });
   });
@@ -555,10 +592,15 @@ int da_add_rms_norm_grad(const void* g, const void* g_total, const void* total, 
   a.d = (int)d;
   a.eps = eps;
   rc = by_types(dtype, weight_dtype, [&](auto dt, auto wide) {
-    return by_plan(plan(d, dtype), [&](auto nw, auto s) {
+    return by_plan(plan(d, dtype), [&](auto nw, auto s, auto small) {
       constexpr int NW = decltype(nw)::value;
-      add_norm_backward<decltype(dt)::value, decltype(wide)::value, NW, decltype(s)::value>
-          <<<(unsigned)(batch * a.chunks), NW == 1 ? 256 : NW * kWave, 0, st>>>(a);
+      constexpr bool kShort = decltype(small)::value;
+      const auto launch = [&](auto stream) {
+        add_norm_backward<decltype(dt)::value, decltype(wide)::value, NW, decltype(s)::value, decltype(stream)::value,
+                          kShort><<<(unsigned)(batch * a.chunks), NW == 1 ? 256 : NW * kWave, 0, st>>>(a);
+      };
+      if (!kShort && batch * tokens * d * (int64_t)elem_bytes(dtype) > kStreamBytes / 4) launch(std::bool_constant<!kShort>{});
+      else launch(std::false_type{});
       return check_launch("da_add_rms_norm_grad");
     });
   });

@@ -247,7 +247,12 @@ __device__ __forceinline__ void st16_any(void* p, u32x4 v) {
   if constexpr (ES == 4) *(u32x4_at4*)p = v;
   else *(u32x4_at2*)p = v;
 }
-// The same with the non-temporal hint: what is written pushes nothing out of the caches.
+// Both with the non-temporal hint: what passes pushes nothing out of the caches.
+template <int ES>
+__device__ __forceinline__ u32x4 ld16_any_nt(const void* p) {
+  if constexpr (ES == 4) return __builtin_nontemporal_load((const u32x4_at4*)p);
+  else return __builtin_nontemporal_load((const u32x4_at2*)p);
+}
 template <int ES>
 __device__ __forceinline__ void st16_any_nt(void* p, u32x4 v) {
   if constexpr (ES == 4) __builtin_nontemporal_store((u32x4_at4)v, (u32x4_at4*)p);
