@@ -177,6 +177,21 @@ __device__ __forceinline__ float over_row(float v, float (*parts)[NW], int& slot
   }
   return v;
 }
+// Two sums at once.
+template <int NW>
+__device__ __forceinline__ void sums_over_row(float& u, float& v, float2 (*parts)[NW], int& slot) {
+  u = lanes_sum<64>(u);
+  v = lanes_sum<64>(v);
+  if constexpr (NW > 1) {
+    const int wave = threadIdx.x / kWave;
+    if (threadIdx.x % kWave == 0) parts[slot][wave] = float2{u, v};
+    __syncthreads();
+    u = parts[slot][0].x, v = parts[slot][0].y;
+#pragma unroll
+    for (int w = 1; w < NW; ++w) u += parts[slot][w].x, v += parts[slot][w].y;
+    slot ^= 1;
+  }
+}
 __device__ __forceinline__ float add_f(float a, float b) { return a + b; }
 __device__ __forceinline__ float max_f(float a, float b) { return fmaxf(a, b); }
 
@@ -287,10 +302,10 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * kWave) void add_norm_forward(A
 // Backward.  Workgroup (sample, chunk): its tokens' dx, and their sum of g t.
 // ---------------------------------------------------------------------------
 template <int DT, bool kWide, int NW, int S, bool kStream, bool kShort>
-__global__ __launch_bounds__(NW == 1 ? 256 : NW * kWave) void add_norm_backward(AddNormArgs a) {
+__global__ __launch_bounds__(NW == 1 ? 256 : NW * kWave, S <= 2 ? 2 : 1) void add_norm_backward(AddNormArgs a) {
   constexpr int ES = Elem<DT>::kBytes, V = Elem<DT>::kVec, kStep = NW * kWave;
   constexpr int kRows = NW == 1 ? 4 : 1;
-  __shared__ float parts[2][NW];
+  __shared__ float2 parts[2][NW];
   __shared__ float sums[NW == 1 ? 3 * S * V * kWave : 1];
   const int at = NW == 1 ? threadIdx.x % kWave : threadIdx.x, wave = threadIdx.x / kWave;
   int slot = 0;
@@ -343,8 +358,7 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * kWave) void add_norm_backward(
         dot += gf[e] * wf[e] * hf[e];
       }
     }
-    sq = over_row<NW>(sq, parts, slot, add_f);
-    dot = over_row<NW>(dot, parts, slot, add_f);
+    sums_over_row<NW>(sq, dot, parts, slot);
     const float rstd = now ? 1.f / __builtin_sqrtf(sq / (float)a.d + a.eps) : 0.f;
     const float mean = dot * rstd / (float)a.d * rstd;  // mean(h t) r
     char* out = a.out + (b * a.tokens + t) * a.d * ES;
@@ -425,26 +439,30 @@ struct Plan {
 // Rows that together do not fit the last-level cache (256 MB) are read and written past it.
 constexpr int64_t kStreamBytes = 128 << 20;
 
-// As many waves as leave a lane two runs or more where the rows are wide.
-Plan plan(int64_t d, int dtype) {
+// As many waves as leave a lane two runs where the rows are wide enough; one run in the
+// backward pass, whose sums and three operands fill the registers (rows of 4096 bf16: 105 us
+// with eight waves, 109 with four).
+Plan plan(int64_t d, int dtype, bool backward) {
   const int64_t vec = dtype == DA_F32 ? 4 : 8, n = (d + vec - 1) / vec;
   if (d < vec) return {1, 1, true};
   if (n <= 64) return {1, 1};
   if (n <= 128) return {1, 2};
   if (n <= 256) return {4, 1};
-  if (n <= 512) return {4, 2};
+  if (n <= 512) return backward ? Plan{8, 1} : Plan{4, 2};
   if (n <= 1024) return {4, 4};
   if (n <= 2048) return {8, 4};
   return {16, 4};
 }
 
-// Chunks of a sample's tokens: about four workgroups a CU, no chunk under 8 tokens.
+// Chunks of a sample's tokens: four workgroups of four waves a CU, or two larger ones (twice
+// as many: 105 us in place of 101 for 8 x 2048 rows of 4096), no chunk under 8 tokens.
 int chunks_of(int64_t batch, int64_t tokens, int64_t d, int dtype, int64_t* chunk, int64_t* chunks) {
   int64_t cus;
   const int rc = device_cu_count(&cus);
   if (rc) return rc;
-  const int64_t least = plan(d, dtype).waves == 1 ? 32 : 8;
-  const int64_t want = std::max<int64_t>(1, 4 * cus / std::max<int64_t>(batch, 1));
+  const int waves = plan(d, dtype, true).waves;
+  const int64_t least = waves == 1 ? 32 : 8;
+  const int64_t want = std::max<int64_t>(1, (waves < 8 ? 4 : 2) * cus / std::max<int64_t>(batch, 1));
   *chunk = std::max(least, (tokens + want - 1) / want);
   *chunks = std::max<int64_t>(1, (tokens + *chunk - 1) / *chunk);
   return DA_OK;
@@ -471,7 +489,9 @@ int by_plan(const Plan& p, F g) {
   if (p.waves == 1) return p.runs == 1 ? f(std::integral_constant<int, 1>{}, std::integral_constant<int, 1>{})
                                        : f(std::integral_constant<int, 1>{}, std::integral_constant<int, 2>{});
   if (p.waves == 16) return f(std::integral_constant<int, 16>{}, std::integral_constant<int, 4>{});
-  if (p.waves == 8) return f(std::integral_constant<int, 8>{}, std::integral_constant<int, 4>{});
+  if (p.waves == 8)
+    return p.runs == 1 ? f(std::integral_constant<int, 8>{}, std::integral_constant<int, 1>{})
+                       : f(std::integral_constant<int, 8>{}, std::integral_constant<int, 4>{});
   if (p.runs == 1) return f(std::integral_constant<int, 4>{}, std::integral_constant<int, 1>{});
   if (p.runs == 2) return f(std::integral_constant<int, 4>{}, std::integral_constant<int, 2>{});
   return f(std::integral_constant<int, 4>{}, std::integral_constant<int, 4>{});
@@ -524,7 +544,7 @@ int da_add_rms_norm(const void* x, const void* residual, const void* weight, int
   a.runs = quantize == kRunScale ? (int)((d + kRun8 - 1) / kRun8) : 1;
   a.eps = eps;
   const hipStream_t st = (hipStream_t)stream;
-  const Plan p = plan(d, dtype);
+  const Plan p = plan(d, dtype, false);
   return by_types(dtype, weight_dtype, [&](auto dt, auto wide) {
     return by_plan(p, [&](auto nw, auto s, auto small) {
       constexpr int DT = decltype(dt)::value, NW = decltype(nw)::value, S = decltype(s)::value;
@@ -592,7 +612,7 @@ int da_add_rms_norm_grad(const void* g, const void* g_total, const void* total, 
   a.d = (int)d;
   a.eps = eps;
   rc = by_types(dtype, weight_dtype, [&](auto dt, auto wide) {
-    return by_plan(plan(d, dtype), [&](auto nw, auto s, auto small) {
+    return by_plan(plan(d, dtype, true), [&](auto nw, auto s, auto small) {
       constexpr int NW = decltype(nw)::value;
       constexpr bool kShort = decltype(small)::value;
       const auto launch = [&](auto stream) {

@@ -564,7 +564,7 @@ void chunks_of(int64_t groups, int64_t T, int64_t cus, int* chunk, int* chunks) 
 }
 
 // Blocks of one side's entries, and splits of the other's: so many that every CU has two
-// workgroups, none under 256 entries.
+// workgroups, none under 128 entries.
 void share(int64_t mine, int64_t others, int64_t groups, int64_t cus, int* blocks, int* splits, int* each) {
   const int64_t n = std::max<int64_t>(1, (mine + kWaves * kTile - 1) / (kWaves * kTile));
   int64_t want = std::max<int64_t>(1, 2 * cus / std::max<int64_t>(1, groups * n));
