@@ -4,13 +4,13 @@
 //
 //   out = o_1 - lam_h o_2,   o_m = softmax(scale q_m k_m^T) v     (zero for a row without keys)
 //
-// One pass over the keys, a wave to a map: it holds R tiles of 32 rows, with their running
-// maxima and sums.  It forms the transposed scores, k q^T, so that a row is a lane's (two
-// lanes', 16 keys each) and its maximum and sum stay within them; the accumulator's
-// registers then are, rounded, the second operand of o^T = v^T p^T as they stand, where v is
-// read transposed out of LDS.  The accumulators are rescaled only when a maximum grows by
-// more than 2^8: what is summed meanwhile is at most that much larger.  At the end the second
-// map's waves hand their values, divided and weighted, to the first's through LDS.
+// One pass over the keys, a wave to a map and to 32 rows, with their running maxima and
+// sums.  It forms the transposed scores, k q^T, so that a row is a lane's (two lanes', 16
+// keys each) and its maximum and sum stay within them; the accumulator's registers then are,
+// rounded, the second operand of o^T = v^T p^T as they stand, where v is read transposed out
+// of LDS.  The accumulators are rescaled only when a maximum grows by more than 2^8: what is
+// summed meanwhile is at most that much larger.  At the end the second map's waves hand
+// their values, divided and weighted, to the first's through LDS.
 #include <algorithm>
 #include <type_traits>
 
@@ -23,8 +23,8 @@ namespace {
 constexpr int kLeastSplit = 128;  // keys of a split (64: no faster; 256: 111 us in place of 91 for 18 heads of 509 keys in fp32)
 constexpr float kSlack = 8.f;  // log2 of how far exponentials may pass 1 before a rescaling
 
-// NG groups of R tiles of rows, each with a wave for either map.
-template <int DT, int DP, int DVP, int R, int NG>
+// NG tiles of rows, each with a wave for either map.
+template <int DT, int DP, int DVP, int NG>
 struct Smem {
   static constexpr int NT = 2 * NG * kWave;
   static constexpr int kK = Tile<DT, DP, NT>::kBytes, kV = Tile<DT, DVP, NT>::kBytes;
@@ -34,9 +34,9 @@ struct Smem {
 
 // kFine: probabilities as the sum of two 16-bit values.  Where a token's few rows leave the
 // matrix units idle that costs nothing, and the values are rounded once, at the end.
-template <int DT, int DP, int DVP, int R, int NG, bool kFine>
+template <int DT, int DP, int DVP, int NG, bool kFine>
 __global__ __launch_bounds__(2 * NG * kWave, 2) void diff_forward(Args a) {
-  using L = Smem<DT, DP, DVP, R, NG>;
+  using L = Smem<DT, DP, DVP, NG>;
   constexpr int NT = L::NT, ES = Type<DT>::ES, V = Type<DT>::V;
   constexpr int KD = DP / Type<DT>::kStep, NB = DVP / 32, KC = Type<DT>::kChunks;
   extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -50,16 +50,9 @@ __global__ __launch_bounds__(2 * NG * kWave, 2) void diff_forward(Args a) {
   at /= a.splits;
   const int hk = at % a.Hk, b = at / a.Hk;
   const int rows = a.T * a.G;
-  int r[R], t[R], h[R], last[R], most = -1, least = a.S;
-#pragma unroll
-  for (int n = 0; n < R; ++n) {
-    r[n] = ((block * NG + group) * R + n) * kTile + (lane & 31);
-    t[n] = token_of(a, r[n]);
-    h[n] = hk * a.G + (r[n] - t[n] * a.G);
-    last[n] = r[n] < rows ? last_key(a, b, t[n]) : -1;
-    most = max(most, last[n]);
-    least = min(least, last[n]);
-  }
+  const int r = (block * NG + group) * kTile + (lane & 31), t = token_of(a, r), h = hk * a.G + (r - t * a.G);
+  const int last = r < rows ? last_key(a, b, t) : -1;
+  int most = last, least = last;
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) {
     most = max(most, __shfl_xor(most, off, kWave));
@@ -69,26 +62,23 @@ __global__ __launch_bounds__(2 * NG * kWave, 2) void diff_forward(Args a) {
   least = __builtin_amdgcn_readfirstlane(least);
   int end = a.S;
   if (a.causal) {  // rows come in order: the workgroup's last one sees most
-    const int64_t t_last = (min((block + 1) * NG * R * kTile, rows) - 1) / a.G;
+    const int64_t t_last = token_of(a, min((block + 1) * NG * kTile, rows) - 1);
     end = (int)max((int64_t)0, min((int64_t)a.S, t_last + a.q_start + 1));
   }
   int key = split * a.each;
   end = min(end, key + a.each);
 
-  u32x4 q[R][KD];
+  u32x4 q[KD];
 #pragma unroll
-  for (int n = 0; n < R; ++n)
-#pragma unroll
-    for (int kk = 0; kk < KD; ++kk)
-      q[n][kk] = last[n] >= 0
-          ? load_run<DT>(a.q + (b * a.q_b + t[n] * a.q_t + (2 * h[n] + map) * a.q_h) * ES, (2 * kk + half) * V, a.D)
-          : u32x4{0, 0, 0, 0};
+  for (int kk = 0; kk < KD; ++kk)
+    q[kk] = last >= 0 ? load_run<DT>(a.q + (b * a.q_b + t * a.q_t + (2 * h + map) * a.q_h) * ES, (2 * kk + half) * V, a.D)
+                      : u32x4{0, 0, 0, 0};
 
   const Keys<DT, DP, NT> keys(a.k_t, a.D);
   const Keys<DT, DVP, NT> values(a.v_t, a.Dv);
   const char* kp = a.k + (b * a.k_b + 2 * hk * a.k_h) * ES;
   const char* vp = a.v + (b * a.v_b + hk * a.v_h) * ES;
-  auto fetch = [&](int to, int stage, uint32_t live) {
+  const auto fetch = [&](int to, int stage, uint32_t live) __attribute__((always_inline)) {
     const uint32_t l = lds_address(lds) + stage * L::kStage;
     keys.fetch(kp + to * a.k_t * ES, l, live);
     keys.fetch(kp + (to * a.k_t + a.k_h) * ES, l + L::kK, live);
@@ -96,15 +86,10 @@ __global__ __launch_bounds__(2 * NG * kWave, 2) void diff_forward(Args a) {
   };
 
   const float c = a.scale * kLog2e;
-  f32x16 o[R][NB];
-  float top[R], sum[R];
+  f32x16 o[NB];
+  float top = kLowest, sum = 0.f;
 #pragma unroll
-  for (int n = 0; n < R; ++n) {
-    top[n] = kLowest, sum[n] = 0.f;
-#pragma unroll
-    for (int x = 0; x < NB; ++x) o[n][x] = zeros();
-  }
-
+  for (int x = 0; x < NB; ++x) o[x] = zeros();
   const Reader<DT, DP> key_reader(lds + map * L::kK, lane);
   const Reader<DT, DVP> value_reader(lds + 2 * L::kK, lane);
   // The next tile with a live key is on its way while one is multiplied.
@@ -120,56 +105,38 @@ __global__ __launch_bounds__(2 * NG * kWave, 2) void diff_forward(Args a) {
     if (key > most) return;
     const auto lk = key_reader.fresh(key);
     const auto lv = value_reader.fresh(key);
-    f32x16 s[R];
+    f32x16 s = zeros();
 #pragma unroll
-    for (int n = 0; n < R; ++n) s[n] = zeros();
-#pragma unroll
-    for (int kk = 0; kk < KD; ++kk) {
-      const u32x4 x = lk.rows(stage * L::kStage, kk);
-#pragma unroll
-      for (int n = 0; n < R; ++n) Mfma32<DT>::mma(s[n], x, q[n][kk]);
-    }
+    for (int kk = 0; kk < KD; ++kk) Mfma32<DT>::mma(s, lk.rows(stage * L::kStage, kk), q[kk]);
     if (word != ~0u || key + kTile - 1 > least) {
+      const uint32_t seen = seen_of(word, key, last, half);
 #pragma unroll
-      for (int n = 0; n < R; ++n) {
-        const uint32_t seen = seen_of(word, key, last[n], half);
+      for (int i = 0; i < 16; ++i) s[i] = seen & 1u << acc_at(i, 0) ? s[i] : -__builtin_inff();
+    }
+    float x = over_acc(s, [](float u, float v) { return fmaxf(u, v); });
+    x = fmaxf(x, other_half(x)) * c;
+    if (__any(x > top + kSlack)) {  // kLowest + 8 is kLowest
+      const float now = fmaxf(top, x), by = __builtin_amdgcn_exp2f(top - now);
+      top = now;
+      sum *= by;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[n][i] = seen & 1u << acc_at(i, 0) ? s[n][i] : -__builtin_inff();
-      }
+      for (int y = 0; y < NB; ++y)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[y][i] *= by;
     }
 #pragma unroll
-    for (int n = 0; n < R; ++n) {
-      float x = over_acc(s[n], [](float u, float v) { return fmaxf(u, v); });
-      x = fmaxf(x, other_half(x)) * c;
-      if (__any(x > top[n] + kSlack)) {  // kLowest + 8 is kLowest
-        const float now = fmaxf(top[n], x), by = __builtin_amdgcn_exp2f(top[n] - now);
-        top[n] = now;
-        sum[n] *= by;
-#pragma unroll
-        for (int y = 0; y < NB; ++y)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) o[n][y][i] *= by;
-      }
-#pragma unroll
-      for (int i = 0; i < 16; ++i) s[n][i] = __builtin_amdgcn_exp2f(fmaf(s[n][i], c, -top[n]));
-      sum[n] += over_acc(s[n], [](float u, float v) { return u + v; });
-    }
+    for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c, -top));
+    sum += over_acc(s, [](float u, float v) { return u + v; });
 #pragma unroll
     for (int j = 0; j < KC; ++j) {
-      u32x4 p[R], rest[R];
-#pragma unroll
-      for (int n = 0; n < R; ++n) {
-        p[n] = from_acc<DT>(s[n], j);
-        if constexpr (kFine) rest[n] = rest_of<DT>(s[n], j, p[n]);
-      }
+      const u32x4 p = from_acc<DT>(s, j);
+      u32x4 rest;
+      if constexpr (kFine) rest = rest_of<DT>(s, j, p);
 #pragma unroll
       for (int y = 0; y < NB; ++y) {
         const u32x4 x = lv.columns(stage * L::kStage, y, j);
-#pragma unroll
-        for (int n = 0; n < R; ++n) {
-          Mfma32<DT>::mma(o[n][y], x, p[n]);
-          if constexpr (kFine) Mfma32<DT>::mma(o[n][y], x, rest[n]);
-        }
+        Mfma32<DT>::mma(o[y], x, p);
+        if constexpr (kFine) Mfma32<DT>::mma(o[y], x, rest);
       }
     }
   };
@@ -178,54 +145,46 @@ __global__ __launch_bounds__(2 * NG * kWave, 2) void diff_forward(Args a) {
     if (live.word) step(std::integral_constant<int, 1>{});
   }
 
-#pragma unroll
-  for (int n = 0; n < R; ++n) sum[n] += other_half(sum[n]);
+  sum += other_half(sum);
   if (a.splits > 1) {  // this split's sums
+    if (r >= rows) return;
+    float* to = a.part + ((((int64_t)split * a.batch + b) * a.Hk + hk) * rows + r) * 2 * (DVP + 2);
 #pragma unroll
-    for (int n = 0; n < R; ++n) {
-      if (r[n] >= rows) continue;
-      float* to = a.part + ((((int64_t)split * a.batch + b) * a.Hk + hk) * rows + r[n]) * 2 * (DVP + 2);
+    for (int y = 0; y < NB; ++y)
 #pragma unroll
-      for (int y = 0; y < NB; ++y)
-#pragma unroll
-        for (int i = 0; i < 16; i += 4)
-          *(f32x4*)(to + map * DVP + 32 * y + acc_at(i, half)) =
-              f32x4{o[n][y][i], o[n][y][i + 1], o[n][y][i + 2], o[n][y][i + 3]};
-      if (half == 0) to[2 * DVP + 2 * map] = top[n], to[2 * DVP + 2 * map + 1] = sum[n];
-    }
+      for (int i = 0; i < 16; i += 4)
+        *(f32x4*)(to + map * DVP + 32 * y + acc_at(i, half)) = f32x4{o[y][i], o[y][i + 1], o[y][i + 2], o[y][i + 3]};
+    if (half == 0) to[2 * DVP + 2 * map] = top, to[2 * DVP + 2 * map + 1] = sum;
     return;
   }
   f32x4* handed = (f32x4*)(lds + group * (L::kHanded / NG));
+  const bool in = r < rows;
+  const float by = sum > 0.f ? 1.f / sum : 0.f;
+  const int64_t to = (((int64_t)b * a.T + t) * (a.Hk * a.G) + h) * a.Dv * ES;
+  if (a.lse && half == 0 && in)
+    a.lse[(((int64_t)b * a.Hk + hk) * 2 + map) * rows + r] = sum > 0.f ? top + log2f(sum) : __builtin_inff();
+  __syncthreads();  // the tiles have been read
+  if (map) {
+    const float lam = in && by != 0.f ? lam_of(a, h) : 0.f;
 #pragma unroll
-  for (int n = 0; n < R; ++n) {
-    const bool in = r[n] < rows;
-    const float by = sum[n] > 0.f ? 1.f / sum[n] : 0.f;
-    const int64_t to = (((int64_t)b * a.T + t[n]) * (a.Hk * a.G) + h[n]) * a.Dv * ES;
-    if (a.lse && half == 0 && in)
-      a.lse[(((int64_t)b * a.Hk + hk) * 2 + map) * rows + r[n]] = sum[n] > 0.f ? top[n] + log2f(sum[n]) : __builtin_inff();
-    __syncthreads();  // the tiles, and what was handed before, have been read
-    if (map) {
-      const float lam = in && by != 0.f ? lam_of(a, h[n]) : 0.f;
+    for (int y = 0; y < NB; ++y)
 #pragma unroll
-      for (int y = 0; y < NB; ++y)
+      for (int i = 0; i < 16; i += 4) {
+        const f32x4 v = f32x4{o[y][i], o[y][i + 1], o[y][i + 2], o[y][i + 3]} * by;
+        if (a.second && in) store4<DT>(a.second + to, 32 * y + acc_at(i, half), a.Dv, v[0], v[1], v[2], v[3]);
+        handed[(y * 4 + i / 4) * kWave + lane] = v * lam;
+      }
+  }
+  __syncthreads();
+  if (!map && in) {
 #pragma unroll
-        for (int i = 0; i < 16; i += 4) {
-          const f32x4 v = f32x4{o[n][y][i], o[n][y][i + 1], o[n][y][i + 2], o[n][y][i + 3]} * by;
-          if (a.second && in) store4<DT>(a.second + to, 32 * y + acc_at(i, half), a.Dv, v[0], v[1], v[2], v[3]);
-          handed[(y * 4 + i / 4) * kWave + lane] = v * lam;
-        }
-    }
-    __syncthreads();
-    if (!map && in) {
+    for (int y = 0; y < NB; ++y)
 #pragma unroll
-      for (int y = 0; y < NB; ++y)
-#pragma unroll
-        for (int i = 0; i < 16; i += 4) {
-          const f32x4 v = handed[(y * 4 + i / 4) * kWave + lane];
-          store4<DT>(a.out + to, 32 * y + acc_at(i, half), a.Dv, o[n][y][i] * by - v[0], o[n][y][i + 1] * by - v[1],
-                     o[n][y][i + 2] * by - v[2], o[n][y][i + 3] * by - v[3]);
-        }
-    }
+      for (int i = 0; i < 16; i += 4) {
+        const f32x4 v = handed[(y * 4 + i / 4) * kWave + lane];
+        store4<DT>(a.out + to, 32 * y + acc_at(i, half), a.Dv, o[y][i] * by - v[0], o[y][i + 1] * by - v[1],
+                   o[y][i + 2] * by - v[2], o[y][i + 3] * by - v[3]);
+      }
   }
 }
 
@@ -336,26 +295,18 @@ int allow_lds(const void* kernel, int bytes) {
 
 namespace {
 
-// How rows are shared out: R tiles a wave and NG groups a workgroup.
-struct Shape {
-  int r, ng;
-};
-
-// Few rows: a tile a workgroup.  Else two groups; 16-bit maps of up to 64 entries have room
-// for two tiles a wave, which halves what is read from LDS a product.
-int plan(int dtype, int w, int64_t batch, int64_t T, int64_t S, int64_t k_heads, int64_t G, Shape* shape, Args* a) {
+// How rows are shared out: *ng tiles a workgroup, one where there are few.
+int plan(int64_t batch, int64_t T, int64_t S, int64_t k_heads, int64_t G, int* ng, Args* a) {
   int64_t cus;
   const int rc = device_cu_count(&cus);
   if (rc) return rc;
   const int64_t rows = T * G, heads = batch * k_heads;
   const auto blocks_of = [&](int64_t n) { return (rows + n * kTile - 1) / (n * kTile); };
-  *shape = {1, 1};
-  if (dtype != DA_F32 && w < 2 && heads * blocks_of(4) >= 2 * cus) *shape = {2, 2};
-  else if (heads * blocks_of(2) >= 2 * cus) *shape = {1, 2};
-  const int64_t blocks = blocks_of(shape->r * shape->ng), groups = std::max<int64_t>(1, heads * blocks);
+  *ng = heads * blocks_of(2) >= 2 * cus ? 2 : 1;
+  const int64_t blocks = blocks_of(*ng), groups = std::max<int64_t>(1, heads * blocks);
   // Keys are split where the rows leave CUs without work: up to eight workgroups a CU, no
   // split under kLeastSplit keys.
-  int64_t want = shape->ng == 1 ? std::max<int64_t>(1, 8 * cus / groups) : 1;
+  int64_t want = *ng == 1 ? std::max<int64_t>(1, 8 * cus / groups) : 1;
   want = std::max<int64_t>(1, std::min(want, S / kLeastSplit));
   const int64_t each = std::max<int64_t>(kTile, ((S + want - 1) / want + kTile - 1) / kTile * kTile);
   a->blocks = (int)blocks;
@@ -384,9 +335,9 @@ int da_diff_attention_workspace(int dtype, int64_t batch, int64_t q_len, int64_t
   *bytes = 0;
   int rc = check_sizes("da_diff_attention_workspace", dtype, batch, q_len, k_len, heads, k_heads, d, dv, 0);
   if (rc || batch == 0 || q_len == 0) return rc;
-  Shape shape;
+  int ng;
   Args a;
-  rc = plan(dtype, widths(d, dv), batch, q_len, k_len, k_heads, heads / k_heads, &shape, &a);
+  rc = plan(batch, q_len, k_len, k_heads, heads / k_heads, &ng, &a);
   if (rc == DA_OK) *bytes = workspace_of(batch, q_len * (heads / k_heads), k_heads, a.splits, widths(d, dv));
   return rc;
 }
@@ -406,8 +357,8 @@ int da_diff_attention(const da_diff_inputs* in, int dtype, int64_t batch, int64_
   if (rc) return rc;
   a.out = (char*)out, a.second = (char*)second, a.lse = lse;
   const int w = widths(d, dv);
-  Shape shape;
-  rc = plan(dtype, w, batch, q_len, k_len, k_heads, a.G, &shape, &a);
+  int ng;
+  rc = plan(batch, q_len, k_len, k_heads, a.G, &ng, &a);
   if (rc) return rc;
   const int64_t rows = q_len * a.G;
   const size_t need = workspace_of(batch, rows, k_heads, a.splits, w);
@@ -421,22 +372,16 @@ int da_diff_attention(const da_diff_inputs* in, int dtype, int64_t batch, int64_
   const hipStream_t st = (hipStream_t)stream;
   return by_widths(dtype, w, [&](auto dt, auto dp, auto dvp) {
     constexpr int DT = decltype(dt)::value, DP = decltype(dp)::value, DVP = decltype(dvp)::value;
-    const auto launch = [&](auto tiles, auto groups) {
-      constexpr int R = decltype(tiles)::value, NG = decltype(groups)::value;
+    const auto launch = [&](auto groups) {
+      constexpr int NG = decltype(groups)::value;
       constexpr bool kFine = DT != DA_F32 && NG == 1;
-      constexpr int kBytes = Smem<DT, DP, DVP, R, NG>::kBytes;
-      const auto kernel = diff_forward<DT, DP, DVP, R, NG, kFine>;
+      constexpr int kBytes = Smem<DT, DP, DVP, NG>::kBytes;
+      const auto kernel = diff_forward<DT, DP, DVP, NG, kFine>;
       if (const int err = allow_lds((const void*)kernel, kBytes)) return err;
       kernel<<<grid, 2 * NG * kWave, kBytes, st>>>(a);
       return (int)DA_OK;
     };
-    using One = std::integral_constant<int, 1>;
-    using Two = std::integral_constant<int, 2>;
-    int err = DA_OK;
-    if (shape.ng == 1) err = launch(One{}, One{});
-    else if (shape.r == 1) err = launch(One{}, Two{});
-    if constexpr (DT != DA_F32 && DP == 64)
-      if (shape.r == 2) err = launch(Two{}, Two{});
+    const int err = ng == 1 ? launch(std::integral_constant<int, 1>{}) : launch(std::integral_constant<int, 2>{});
     if (err) return err;
     if (a.splits > 1) {
       constexpr int kRows = 256 / (DVP / 4);
