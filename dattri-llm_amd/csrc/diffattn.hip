@@ -8,9 +8,11 @@
 // sums.  It forms the transposed scores, k q^T, so that a row is a lane's (two lanes', 16
 // keys each) and its maximum and sum stay within them; the accumulator's registers then are,
 // rounded, the second operand of o^T = v^T p^T as they stand, where v is read transposed out
-// of LDS.  The accumulators are rescaled only when a maximum grows by more than 2^8: what is
-// summed meanwhile is at most that much larger.  At the end the second map's waves hand
-// their values, divided and weighted, to the first's through LDS.
+// of LDS.  Exponentials are relative to a maximum that is looked for again only when the sum
+// of a lane's sixteen passes 2^10: until then they are at most that much larger than with the
+// last one (the first tile has none, and passes).  The vector unit bounds the loop, so that
+// what a tile need not do is left out.  At the end the second map's waves hand their values,
+// divided and weighted, to the first's through LDS.
 #include <algorithm>
 #include <type_traits>
 
@@ -21,7 +23,7 @@ namespace diff {
 namespace {
 
 constexpr int kLeastSplit = 128;  // keys of a split (64: no faster; 256: 111 us in place of 91 for 18 heads of 509 keys in fp32)
-constexpr float kSlack = 8.f;  // log2 of how far exponentials may pass 1 before a rescaling
+constexpr float kMostSum = 1024.f;  // of sixteen exponentials, before a new maximum
 
 // NG tiles of rows, each with a wave for either map.
 template <int DT, int DP, int DVP, int NG>
@@ -103,19 +105,21 @@ __global__ __launch_bounds__(2 * NG * kWave, 2) void diff_forward(Args a) {
     __syncthreads();
     if (live.word) fetch(live.key, stage ^ 1, live.word);
     if (key > most) return;
-    const auto lk = key_reader.fresh(key);
-    const auto lv = value_reader.fresh(key);
     f32x16 s = zeros();
 #pragma unroll
-    for (int kk = 0; kk < KD; ++kk) Mfma32<DT>::mma(s, lk.rows(stage * L::kStage, kk), q[kk]);
+    for (int kk = 0; kk < KD; ++kk) Mfma32<DT>::mma(s, key_reader.rows(stage * L::kStage, kk), q[kk]);
     if (word != ~0u || key + kTile - 1 > least) {
       const uint32_t seen = seen_of(word, key, last, half);
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[i] = seen & 1u << acc_at(i, 0) ? s[i] : -__builtin_inff();
     }
-    float x = over_acc(s, [](float u, float v) { return fmaxf(u, v); });
-    x = fmaxf(x, other_half(x)) * c;
-    if (__any(x > top + kSlack)) {  // kLowest + 8 is kLowest
+    f32x16 e;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) e[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c, -top));
+    float part = over_acc(e, [](float u, float v) { return u + v; });
+    if (__any(part > kMostSum)) {
+      float x = over_acc(s, [](float u, float v) { return fmaxf(u, v); });
+      x = fmaxf(x, other_half(x)) * c;
       const float now = fmaxf(top, x), by = __builtin_amdgcn_exp2f(top - now);
       top = now;
       sum *= by;
@@ -123,18 +127,19 @@ __global__ __launch_bounds__(2 * NG * kWave, 2) void diff_forward(Args a) {
       for (int y = 0; y < NB; ++y)
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[y][i] *= by;
-    }
 #pragma unroll
-    for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c, -top));
-    sum += over_acc(s, [](float u, float v) { return u + v; });
+      for (int i = 0; i < 16; ++i) e[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c, -top));
+      part = over_acc(e, [](float u, float v) { return u + v; });
+    }
+    sum += part;
 #pragma unroll
     for (int j = 0; j < KC; ++j) {
-      const u32x4 p = from_acc<DT>(s, j);
+      const u32x4 p = from_acc<DT>(e, j);
       u32x4 rest;
-      if constexpr (kFine) rest = rest_of<DT>(s, j, p);
+      if constexpr (kFine) rest = rest_of<DT>(e, j, p);
 #pragma unroll
       for (int y = 0; y < NB; ++y) {
-        const u32x4 x = lv.columns(stage * L::kStage, y, j);
+        const u32x4 x = value_reader.columns(stage * L::kStage, y, j);
         Mfma32<DT>::mma(o[y], x, p);
         if constexpr (kFine) Mfma32<DT>::mma(o[y], x, rest);
       }
