@@ -9,7 +9,7 @@ manager belong to the capture's control plane and are not part of this package.
 from dattri_llm_amd.gradient import ops
 from dattri_llm_amd.gradient.capture import FusedCapture
 from dattri_llm_amd.gradient.gradient import Factorized, Gradient, GradientRecord
-from dattri_llm_amd.gradient.layers import QKNormRope, RelativeBias
+from dattri_llm_amd.gradient.layers import AddRMSNorm, DiffAttention, QKNormRope, RelativeBias
 from dattri_llm_amd.gradient.ops import (
     FisherAccumulator,
     KroneckerAccumulator,
@@ -27,7 +27,9 @@ from dattri_llm_amd.gradient.routing import RowLayout, locate_rows
 from dattri_llm_amd.gradient.store import AsyncGradientWriter, GradientStore
 
 __all__ = [
+    "AddRMSNorm",
     "AsyncGradientWriter",
+    "DiffAttention",
     "Factorized",
     "FisherAccumulator",
     "FusedCapture",

@@ -21,10 +21,13 @@ and runs the capture on ``(input, grad_output)`` on the same stream:
 * unprojected: the raw factors, or the dense ``(B, d_out * (d_in + 1))``
   gradient from the dW kernel.
 
-A :class:`QKNormRope` or :class:`RelativeBias` module is captured by its own
-backward kernel, which gives the per-sample weight gradients: materialized
-layers, ``<name>.q_weight`` and ``<name>.k_weight`` of type ``nn.RMSNorm``, and
-``<name>`` of type ``nn.Embedding``, in fp32.
+The modules of :mod:`dattri_llm_amd.gradient.layers` are captured by their own
+backward kernels, which give the per-sample weight gradients: materialized
+layers in fp32, of type ``nn.RMSNorm`` (``<name>.q_weight`` and
+``<name>.k_weight`` of a :class:`QKNormRope`, ``<name>`` of an
+:class:`AddRMSNorm`, the four vectors ``<name>.lambda_q1`` ... of a
+:class:`DiffAttention`, which scale a map as a norm's weight scales its rows) or
+``nn.Embedding`` (``<name>`` of a :class:`RelativeBias`).
 
 No weight or bias gradient is produced for a captured layer, as with the
 reference's invasive capture: use it for attribution, not for training.  The
@@ -40,7 +43,7 @@ import torch
 from torch import nn
 
 from dattri_llm_amd.gradient.gradient import Factorized, Gradient
-from dattri_llm_amd.gradient.layers import QKNormRope, RelativeBias
+from dattri_llm_amd.gradient.layers import FACTOR_NAMES, AddRMSNorm, DiffAttention, QKNormRope, RelativeBias
 from dattri_llm_amd.gradient.ops import materialize_factors, project_layer, should_materialize
 from dattri_llm_amd.gradient.ops.projection import DattriProjector
 
@@ -138,13 +141,32 @@ class _WeightSlot:
             self.parts.clear()
 
 
+class _FactorSlot:
+    """Takes the per-sample gradient (B, H) of a :class:`DiffAttention`'s factor in one
+    call and hands it on to the slots of the four vectors that the factor was formed
+    from, by their derivatives as they were at the call."""
+
+    def __init__(self, module: DiffAttention, slots: list[_WeightSlot]) -> None:
+        with torch.no_grad():
+            e1, e2 = module.exponentials()
+            rows = (e1 * module.lambda_k1.float(), e1 * module.lambda_q1.float(),
+                    -e2 * module.lambda_k2.float(), -e2 * module.lambda_q2.float())
+        self.parts = list(zip(slots, rows))
+
+    def put(self, per_sample: torch.Tensor) -> None:
+        total = per_sample.sum(1, keepdim=True)  # one factor for all heads
+        for slot, row in self.parts:
+            slot.put(total * row)
+
+
 class FusedCapture:
-    """Capture per-sample gradients of ``nn.Linear``, :class:`QKNormRope` and
-    :class:`RelativeBias` layers inside autograd.
+    """Capture per-sample gradients of ``nn.Linear``, :class:`QKNormRope`,
+    :class:`RelativeBias`, :class:`AddRMSNorm` and :class:`DiffAttention` layers
+    inside autograd.
 
     ``layers``: names of the modules to capture (default: all of these types).
     A captured ``RelativeBias`` has to be called with ``batch``; the gradients of
-    these two are small and kept whole, whatever ``proj_dim`` and
+    all but the linear layers are small and kept whole, whatever ``proj_dim`` and
     ``capture_style`` are.
     ``proj_dim``: LoGRA projection width (``None``: unprojected capture), with
     ``proj_seed`` / ``projector`` as in ``project_factors`` (seed for the
@@ -177,9 +199,13 @@ class FusedCapture:
                 self._add_qk(name, module)
             elif type(module) is RelativeBias:
                 self._add_bias(name, module)
+            elif type(module) is AddRMSNorm:
+                self._add_norm(name, module)
+            elif type(module) is DiffAttention:
+                self._add_diff(name, module)
             elif wanted is not None:
-                raise ValueError(f"layer {name!r} is a {type(module).__name__}, not a plain nn.Linear, QKNormRope or "
-                                 "RelativeBias")
+                raise ValueError(f"layer {name!r} is a {type(module).__name__}, not a plain nn.Linear, QKNormRope, "
+                                 "RelativeBias, AddRMSNorm or DiffAttention")
             seen.add(name)
         if wanted is not None and wanted - seen:
             raise ValueError(f"no such layers: {sorted(wanted - seen)}")
@@ -202,7 +228,7 @@ class FusedCapture:
             slots.append(self.slots[at])
 
         def forward(q, k, positions=None, mask=None):
-            self._check_batch_first(name)
+            self._check_batch_first(name, module)
             return QKNormRope.forward(module, q, k, positions, mask, _slots=tuple(slots))
 
         self._modules.append((module, forward))
@@ -218,9 +244,34 @@ class FusedCapture:
 
         self._modules.append((module, forward))
 
-    def _check_batch_first(self, name: str) -> None:
+    def _add_norm(self, name: str, module: AddRMSNorm) -> None:
+        slot = self.slots[name] = _WeightSlot()
+        self.types[name] = "nn.RMSNorm"
+
+        def forward(x, residual=None, mask=None):
+            self._check_batch_first(name, module)
+            return AddRMSNorm.forward(module, x, residual, mask, _slot=slot)
+
+        self._modules.append((module, forward))
+
+    def _add_diff(self, name: str, module: DiffAttention) -> None:
+        slots = []
+        for part in FACTOR_NAMES:
+            at = f"{name}.{part}" if name else part
+            self.slots[at] = _WeightSlot()
+            self.types[at] = "nn.RMSNorm"
+            slots.append(self.slots[at])
+
+        def forward(q, k, v, mask=None, q_mask=None, *, q_start=None):
+            self._check_batch_first(name, module)
+            slot = _FactorSlot(module, slots) if torch.is_grad_enabled() else None
+            return DiffAttention.forward(module, q, k, v, mask, q_mask, q_start=q_start, _slot=slot)
+
+        self._modules.append((module, forward))
+
+    def _check_batch_first(self, name: str, module: nn.Module) -> None:
         if not self.batch_first:
-            raise ValueError(f"layer {name!r}: QKNormRope is captured batch first only")
+            raise ValueError(f"layer {name!r}: {type(module).__name__} is captured batch first only")
 
     def __enter__(self) -> FusedCapture:
         for m, forward in self._modules:

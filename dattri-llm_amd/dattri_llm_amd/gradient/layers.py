@@ -2,9 +2,10 @@
 :class:`~dattri_llm_amd.gradient.capture.FusedCapture` captures.
 
 A hook on these layers sees no usable pair of input and output gradient (the
-norms' output gradient lies behind the rotation, the bias is shared by the
-batch; the reference's hooks have no counterpart), so they are captured in
-their own backward pass, as per-sample weight gradients.
+norms' output gradient lies behind the rotation, the bias and the factor between
+two maps are shared by the batch; the reference's hooks have no counterpart) or,
+for the norm of the residual stream, would read both once more, so they are
+captured in their own backward pass, as per-sample weight gradients.
 """
 
 from __future__ import annotations
@@ -70,4 +71,52 @@ class RelativeBias(nn.Module):
                                  causal=self.causal, mask=mask, slot=_slot)
 
 
-__all__ = ["QKNormRope", "RelativeBias"]
+class AddRMSNorm(nn.Module):
+    """The residual's addition with the RMS norm that follows it
+    (:func:`ops.add_rms_norm`): ``(out, total)``, or ``out`` alone without a residual.
+
+    Parameter ``weight`` ``(d,)``."""
+
+    def __init__(self, d: int, *, eps: float = 1e-6, device=None, dtype=None) -> None:
+        super().__init__()
+        self.weight = nn.Parameter(torch.ones(d, device=device, dtype=dtype))
+        self.eps = eps
+
+    def forward(self, x, residual=None, mask=None, *, _slot=None):
+        got = ops.add_rms_norm(x, residual, self.weight, eps=self.eps, mask=mask, slot=_slot)
+        return got.out if residual is None else (got.out, got.total)
+
+
+class DiffAttention(nn.Module):
+    """Attention by the difference of two softmax maps (:func:`ops.diff_attention`)
+    with a learned factor, one for all heads:
+
+    ``lam = exp(lambda_q1 . lambda_k1) - exp(lambda_q2 . lambda_k2) + lambda_init``
+
+    of four parameters ``(head_dim,)``, the width of a map."""
+
+    def __init__(self, head_dim: int, *, lambda_init: float = 0.8, causal: bool = False, scale: float | None = None,
+                 device=None, dtype=None) -> None:
+        super().__init__()
+        for name in FACTOR_NAMES:
+            setattr(self, name, nn.Parameter(0.1 * torch.randn(head_dim, device=device, dtype=dtype)))
+        self.lambda_init, self.causal, self.scale = lambda_init, causal, scale
+
+    def exponentials(self):
+        """The two exponentials of the factor, in fp32."""
+        return ((self.lambda_q1.float() * self.lambda_k1.float()).sum().exp(),
+                (self.lambda_q2.float() * self.lambda_k2.float()).sum().exp())
+
+    def factor(self) -> torch.Tensor:
+        """``lam``, in fp32."""
+        e1, e2 = self.exponentials()
+        return e1 - e2 + self.lambda_init
+
+    def forward(self, q, k, v, mask=None, q_mask=None, *, q_start: int | None = None, _slot=None):
+        return ops.diff_attention(q, k, v, self.factor(), scale=self.scale, causal=self.causal, q_start=q_start,
+                                  mask=mask, q_mask=q_mask, slot=_slot)
+
+
+FACTOR_NAMES = ("lambda_q1", "lambda_k1", "lambda_q2", "lambda_k2")
+
+__all__ = ["FACTOR_NAMES", "AddRMSNorm", "DiffAttention", "QKNormRope", "RelativeBias"]

@@ -7,8 +7,8 @@ layer's own input and output, as the reference does for its norm and embedding
 layers (``dattri_llm/gradient/ops/materialize.py:22-48``, ``:96-98``): the
 norms' output gradient is known only behind the rotation, and a bias table is
 looked up once for the whole batch, so that the gradient which reaches it is
-already summed over the samples, as is that of the factor between two maps.  Here the backward pass of each operator
-gives the per-sample gradient itself:
+already summed over the samples, as is that of the factor between two maps.
+Here the backward pass of each operator gives the per-sample gradient itself:
 
 * :func:`qk_norm_rope` / :func:`qk_norm_rope_grad` (``da_qk_norm_rope``);
 * :func:`relative_bias` / :func:`relative_bias_grad` (``da_relative_bias``);

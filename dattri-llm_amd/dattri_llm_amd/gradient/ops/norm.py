@@ -64,10 +64,11 @@ def add_rms_norm(x, residual, weight, *, eps: float = 1e-6, mask=None, quantize:
     ``total * rsqrt(mean(total^2) + eps) * weight``, differentiable.
 
     The norm is that of ``total`` as it is returned, in the rows' dtype.
-    ``residual`` may be None (``total`` is None then); ``weight`` ``(d,)``, in any
-    dtype.  ``mask`` (B, T): a token with a zero gets zero rows, whatever its
-    input holds, and takes no part in any gradient.  Inputs of any strides;
-    outputs are contiguous.  A single new token is ``T = 1``.
+    ``residual`` may be None (``total`` is None then); two dtypes are promoted as an
+    addition promotes them; ``weight`` ``(d,)``, in any dtype.  ``mask`` (B, T): a
+    token with a zero gets zero rows, whatever its input holds, and takes no part
+    in any gradient.  Inputs of any strides; outputs are contiguous.  A single new
+    token is ``T = 1``.
 
     ``quantize``: ``out`` in 8 bits (``torch.float8_e4m3fn``) with fp32
     ``scales``, ``"row"`` ``(B, T)``, or ``"block"`` one for each 128 entries
@@ -78,6 +79,9 @@ def add_rms_norm(x, residual, weight, *, eps: float = 1e-6, mask=None, quantize:
     place of its summed one (``FusedCapture``)."""
     if getattr(forward_ad, "_current_level", 0) >= 0:
         kernels.refuse_tangents("add_rms_norm", x, residual, weight)
+    if residual is not None and residual.dtype != x.dtype:
+        wide = torch.promote_types(x.dtype, residual.dtype)
+        x, residual = x.to(wide), residual.to(wide)
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (
             residual is not None and residual.requires_grad) or (slot is not None)):
         if quantize is not None:

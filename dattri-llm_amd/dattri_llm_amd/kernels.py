@@ -1920,13 +1920,17 @@ def _diff_call(what, q, k, v, lam, mask, q_mask, scale, causal, q_start):
     sizes = _diff_sizes(what, q, k, v, lam)
     b, t, s, h, hk, d, dv = sizes
     code = nat.dtype_code(q.dtype)
+    scale = d ** -0.5 if scale is None else float(scale)
+    if not scale > 0:
+        raise ValueError(f"{what}: the scale must be positive, got {scale}")
+    q_start = s - t if q_start is None else int(q_start)
+    if abs(q_start) >= 1 << 30:
+        raise NotImplementedError(f"{what}: positions below 2^30, got q_start {q_start}")
     mask, mask_ptr, mask_b, mask_k = _token_mask(what, mask, b, s)
     q_mask, qm_ptr, qm_b, qm_t = _token_mask(what, q_mask, b, t)
     dev = nat.same_device(q, k, v, lam, mask, q_mask)
     q, k, v = _head_rows(q), _head_rows(k), _head_rows(v)
     sizes = (b, t, s, h, hk, q.shape[3], v.shape[3])
-    scale = d ** -0.5 if scale is None else float(scale)
-    q_start = s - t if q_start is None else int(q_start)
     words = array.array("q", (
         q.data_ptr(), k.data_ptr(), v.data_ptr(), lam.data_ptr(), nat.DTYPE_CODE[lam.dtype],
         lam.stride(0) if lam.numel() > 1 else 0, *q.stride()[:3], *k.stride()[:3], *v.stride()[:3],
@@ -1996,7 +2000,7 @@ def diff_attention_grad(g: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: to
 # ---------------------------------------------------------------------------
 # Log probabilities of given tokens.
 # ---------------------------------------------------------------------------
-def _token_rows(what: str, logits: torch.Tensor, targets: torch.Tensor, mask):
+def _token_rows(what: str, logits: torch.Tensor, targets: torch.Tensor, mask, temperature: float):
     """(B, T, V) logits, their (B, T) targets and mask; (N, V) rows are one sample."""
     if logits.dim() not in (2, 3) or targets.shape != logits.shape[:-1]:
         raise ValueError(f"{what} expects (B, T, V) or (N, V) logits with a target each, got {tuple(logits.shape)} and "
@@ -2005,6 +2009,8 @@ def _token_rows(what: str, logits: torch.Tensor, targets: torch.Tensor, mask):
         raise ValueError(f"{what}: targets must be int64, got {targets.dtype}")
     if mask is not None and mask.shape != targets.shape:
         raise ValueError(f"{what}: mask must have shape {tuple(targets.shape)}, got {tuple(mask.shape)}")
+    if not temperature > 0:
+        raise ValueError(f"{what}: the temperature must be positive, got {temperature}")
     if logits.dim() == 2:
         logits, targets, mask = logits[None], targets[None], None if mask is None else mask[None]
     return _unit_rows(logits), targets, mask
@@ -2014,7 +2020,7 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, *, mask=None, te
     """``(logprob, entropy, lse, top_logprob, top_index)`` of ``da_token_logprobs``,
     fp32 (int64 indices) in the targets' shape (times ``top``; None without)."""
     what, shape = "token_logprobs", targets.shape
-    logits, targets, mask = _token_rows(what, logits, targets, mask)
+    logits, targets, mask = _token_rows(what, logits, targets, mask, temperature)
     b, t, v = logits.shape
     if isinstance(top, bool) or not isinstance(top, int) or not 0 <= top <= min(32, v):
         raise ValueError(f"{what}: top must be 0 to {min(32, v)}, got {top!r}")
@@ -2052,7 +2058,7 @@ def token_logprobs_grad(up, up_entropy, logits: torch.Tensor, targets: torch.Ten
         if x.shape != shape or x.dtype != torch.float32:
             raise ValueError(f"{what}: lse and entropy must be fp32 of shape {tuple(shape)}, as token_logprobs returns them")
     full = logits.shape
-    logits, targets, mask = _token_rows(what, logits, targets, mask)
+    logits, targets, mask = _token_rows(what, logits, targets, mask, temperature)
     b, t, v = logits.shape
     code = nat.dtype_code(logits.dtype)
     mask, mask_ptr, mask_b, mask_t = _token_mask(what, mask, b, t)
