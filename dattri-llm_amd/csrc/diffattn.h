@@ -41,6 +41,7 @@ struct Args {
   int64_t g_b, g_t, g_h;
   float* delta;   // (batch, Hk, 2, T G): g . o_m
   char* records;  // (batch, Hk, T G): lse and delta of both maps as diff_grad_keys reads them
+  uint8_t* takes_part;  // (batch, Hk, T G): whether the row sees a key
   float* most;    // largest |g| of the call (16-bit floats of five exponent bits)
   char *dq, *dk, *dv;
   float* lam_part;  // (batch, heads, chunks)

@@ -269,7 +269,8 @@ int check_side(const char* what, const char* name, const void* x, int es, int64_
 int fill_args(Args& a, const char* what, int dtype, const da_diff_inputs* in, int64_t batch, int64_t T, int64_t S, int64_t heads,
               int64_t k_heads, int64_t D, int64_t Dv, float scale, int causal, int64_t q_start) {
   if (!valid_dtype((int)in->lam_dtype)) return set_error(DA_ERR_INVALID, "%s: bad dtype %d", what, (int)in->lam_dtype);
-  if (!(scale > 0.f) || !(scale < 1e30f)) return set_error(DA_ERR_INVALID, "%s: the scale must be positive", what);
+  if (!(scale >= 1e-20f) || !(scale <= 1e20f))  // times or over a finite score, and 1e30 times it, stay in range
+    return set_error(DA_ERR_INVALID, "%s: the scale must lie between 1e-20 and 1e20", what);
   const int es = (int)elem_bytes(dtype);
   const int64_t group = heads / k_heads;
   int rc = check_side(what, "q", in->q, es, D, T, 2 * group, in->q_bstride, in->q_tstride, in->q_hstride);

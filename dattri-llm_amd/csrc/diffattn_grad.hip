@@ -78,7 +78,12 @@ __global__ __launch_bounds__(256) void diff_delta(Args a) {
   const int t1 = min((chunk + 1) * a.chunk, a.T);
   float all = 0.f, most = 0.f;
   for (int t = chunk * a.chunk + sub; t < t1; t += kRows) {
-    const bool live = !a.q_mask || a.q_mask[b * a.qm_b + t * a.qm_t];
+    const int64_t of = (int64_t)b * a.Hk + hk;
+    const int r = t * a.G + (h - hk * a.G);
+    const float* lse = a.lse + of * 2 * rows + r;
+    // Of a row that sees no key nothing is read: its gradient may be anything.
+    const float lse0 = lse[0];
+    const bool live = lse0 != __builtin_inff();
     float d0 = 0.f, d1 = 0.f;
     if (live) {
       const char* g = a.g + (b * a.g_b + t * a.g_t + h * a.g_h) * ES;
@@ -99,14 +104,12 @@ __global__ __launch_bounds__(256) void diff_delta(Args a) {
     d0 = lanes_sum<kLanes>(d0);
     d1 = lanes_sum<kLanes>(d1);
     if (l == 0) {
-      const int64_t of = (int64_t)b * a.Hk + hk;
-      const int r = t * a.G + (h - hk * a.G);
       float* to = a.delta + of * 2 * rows + r;
       d0 += lam * d1;  // o_1 = out + lam o_2
       to[0] = d0;
       to[rows] = d1;
-      const float* lse = a.lse + of * 2 * rows + r;
-      put_record<DT>(a.records + (of * rows + r) * Record<DT>::kBytes, a.scale * kLog2e, lse[0],
+      a.takes_part[of * rows + r] = live;
+      put_record<DT>(a.records + (of * rows + r) * Record<DT>::kBytes, a.scale * kLog2e, lse0,
                      lse[rows] - log2f(fabsf(lam)), d0, d1);
     }
     all += d1;
@@ -177,8 +180,13 @@ __global__ __launch_bounds__(kThreads, DT != DA_F32 && DP == 64 ? 2 : 1) void di
   at /= a.splits;
   const int hk = at % a.Hk, b = at / a.Hk;
   const int key0 = (block * kWaves + wave) * kTile, key = key0 + (lane & 31);
-  const bool alive = key < a.S && (!a.mask || a.mask[b * a.m_b + key * a.m_k]);
   const int rows = a.T * a.G, end = min(rows, (split + 1) * a.each);
+  // The rows that see a key are those from this one on.
+  const auto first_row = [&](int to) {
+    const int64_t t = to - a.q_start;
+    return !a.causal || t <= 0 ? 0 : t >= a.T ? rows : (int)t * a.G;
+  };
+  const bool alive = key < a.S && first_row(key) < rows && (!a.mask || a.mask[b * a.m_b + key * a.m_k]);
   u32x4 k[2][KD], v[L::kValues ? 1 : KV];
 #pragma unroll
   for (int kk = 0; kk < KD; ++kk)
@@ -210,11 +218,7 @@ __global__ __launch_bounds__(kThreads, DT != DA_F32 && DP == 64 ? 2 : 1) void di
   constexpr uint32_t kOnes = 0x3f803f80u, kOne = 0x3f80u;
   const uint32_t in_low = half ? 0u : ~0u;
 
-  // The rows that see the lane's key are those from `from` on; the wave's keys, all or some.
-  const auto first_row = [&](int to) {
-    const int64_t t = to - a.q_start;
-    return !a.causal || t <= 0 ? 0 : t >= a.T ? rows : (int)t * a.G;
-  };
+  // Of the wave's keys, some and all.
   const int from_some = first_row(key0), from_all = first_row(key0 + kTile - 1);
   const int first = max(split * a.each, first_row(block * kWaves * kTile) / kTile * kTile);
   const uint32_t q_token = (uint32_t)(a.q_t * ES), q_head = (uint32_t)(2 * a.q_h * ES);
@@ -241,9 +245,10 @@ __global__ __launch_bounds__(kThreads, DT != DA_F32 && DP == 64 ? 2 : 1) void di
   bool any_minus = false;
   for (int i = lane; i < a.G; i += kWave) any_minus |= lam_of(a, hk * a.G + i) < 0.f;
   any_minus = __any(any_minus);
+  const uint8_t* takes_part = a.takes_part + ((int64_t)b * a.Hk + hk) * rows;
   auto row_byte = [&](int r0) {
     const int r = r0 + (lane & 31);
-    return r < end ? (a.q_mask ? a.q_mask[b * a.qm_b + token_of(a, r) * a.qm_t] : 1) : 0;
+    return r < end ? takes_part[r] : 0;
   };
   auto fetch = [&](int r0, int stage, uint32_t live) {
     const int64_t t0 = token_of(a, r0);
@@ -425,7 +430,10 @@ __global__ __launch_bounds__(kThreads, DT != DA_F32 && DVP <= 128 ? 2 : 1) void 
   const int rows = a.T * a.G;
   const int r = (block * kWaves + wave) * kTile + (lane & 31);
   const int t = token_of(a, r), h = hk * a.G + (r - t * a.G);
-  const int last = r < rows ? last_key(a, b, t) : -1;
+  const int64_t base = ((int64_t)b * a.Hk + hk) * 2 * rows + r;
+  int last = r < rows ? last_key(a, b, t) : -1;
+  const float lse0 = last >= 0 ? a.lse[base] : __builtin_inff();
+  if (lse0 == __builtin_inff()) last = -1;  // no key that it could see is live
   int most = last, least = last;
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) {
@@ -453,10 +461,8 @@ __global__ __launch_bounds__(kThreads, DT != DA_F32 && DVP <= 128 ? 2 : 1) void 
   for (int kk = 0; kk < KV; ++kk)
     g[kk] = in ? load_run<DT>(a.g + (b * a.g_b + t * a.g_t + h * a.g_h) * ES, (2 * kk + half) * V, a.Dv)
                : u32x4{0, 0, 0, 0};
-  const int64_t base = ((int64_t)b * a.Hk + hk) * 2 * rows + r;
   // The second map's factor comes with its exponential, the sign with its values' gradient.
   const float lam = in ? lam_of(a, h) : 0.f, sign = lam < 0.f ? 1.f : -1.f;
-  const float lse0 = in ? a.lse[base] : __builtin_inff();
   const float lse1 = in ? a.lse[base + rows] - log2f(fabsf(lam)) : __builtin_inff();
   const float de0 = in ? a.delta[base] : 0.f, de1 = in ? -sign * a.delta[base + rows] : 0.f;
   const float c = a.scale * kLog2e, small = small_scale<DT>(a);
@@ -564,7 +570,7 @@ void chunks_of(int64_t groups, int64_t T, int64_t cus, int* chunk, int* chunks) 
 }
 
 // Blocks of one side's entries, and splits of the other's: so many that every CU has two
-// workgroups, none under 128 entries.
+// workgroups, none under 256 entries.
 void share(int64_t mine, int64_t others, int64_t groups, int64_t cus, int* blocks, int* splits, int* each) {
   const int64_t n = std::max<int64_t>(1, (mine + kWaves * kTile - 1) / (kWaves * kTile));
   int64_t want = std::max<int64_t>(1, 2 * cus / std::max<int64_t>(1, groups * n));
@@ -575,10 +581,10 @@ void share(int64_t mine, int64_t others, int64_t groups, int64_t cus, int* block
 }
 
 // How the two passes are shared out, and the workspace: delta, the parts of dlam, the largest
-// |g|, the records, and the sums of the splits (of one pass after the other).
+// |g|, the records, whether a row takes part, and the sums of the splits (of one pass after the other).
 struct Plan {
   Args keys, rows;  // blocks, splits, each
-  int64_t records_at, parts_at, most_at, sums_at;  // in floats
+  int64_t records_at, parts_at, most_at, takes_part_at, sums_at;  // in floats
   size_t bytes;
 };
 
@@ -593,7 +599,8 @@ int plan(int dtype, int64_t batch, int64_t heads, int64_t k_heads, int64_t T, in
   p->records_at = (batch * heads * T * 2 + 3) / 4 * 4;
   p->parts_at = p->records_at + batch * heads * T * (dtype == DA_BF16 ? Record<DA_BF16>::kBytes : Record<DA_F32>::kBytes) / 4;
   p->most_at = p->parts_at + batch * heads * a->chunks;
-  p->sums_at = (p->most_at + 4) / 4 * 4;
+  p->takes_part_at = p->most_at + 1;
+  p->sums_at = (p->takes_part_at + (batch * heads * T + 3) / 4 + 3) / 4 * 4;
   const int64_t of_keys = p->keys.splits > 1 ? p->keys.splits * batch * S * k_heads * (2 * D + Dv) : 0;
   const int64_t of_rows = p->rows.splits > 1 ? p->rows.splits * batch * T * heads * 2 * D : 0;
   p->bytes = (size_t)(p->sums_at + std::max(of_keys, of_rows)) * sizeof(float);
@@ -665,6 +672,7 @@ int da_diff_attention_grad(const da_diff_inputs* in, const void* g, int64_t g_bs
   a.records = (char*)(a.delta + p.records_at);
   a.lam_part = a.delta + p.parts_at;
   a.most = a.delta + p.most_at;
+  a.takes_part = (uint8_t*)(a.delta + p.takes_part_at);
   a.part = a.delta + p.sums_at;
   a.dq = (char*)dq, a.dk = (char*)dk, a.dv = (char*)dvalue;
   const hipStream_t st = (hipStream_t)stream;

@@ -179,7 +179,8 @@ def test_c_abi_diff_attention_checks():
     for bad in (dict(q=0), dict(k=0), dict(v=0), dict(lam=0)):
         refused(fwd(words(**bad)), nat.DA_ERR_INVALID, "NULL")
     refused(fwd(words(lam_dtype=5)), nat.DA_ERR_INVALID, "dtype")
-    refused(fwd(scale=0.0), nat.DA_ERR_INVALID, "scale")
+    for scale in (0.0, -1.0, 1e-30, 1e30, float("inf"), float("nan")):
+        refused(fwd(scale=scale), nat.DA_ERR_INVALID, "scale")
     refused(fwd(words(q=X + 8)), nat.DA_ERR_INVALID, "16-byte")
     refused(fwd(words(ts=68)), nat.DA_ERR_INVALID, "16-byte")
     refused(fwd(d=60), nat.DA_ERR_INVALID, "16-byte")

@@ -244,6 +244,33 @@ def test_new_tokens_one_at_a_time_equal_the_whole_prompt(device, dt):
         assert bool(((told.logprob - answers.logprob[:, i:i + 1]).abs() < 1e-5).all())
 
 
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16, torch.float16])
+def test_rows_and_keys_that_see_nothing_may_hold_anything(device, dt):
+    """Queries before the first key, queries whose keys are all masked, and keys behind the
+    last query: NaN there, in the gradient that arrives too, reaches nothing else."""
+    torch.manual_seed(7)
+    b, t, s, h, hk, d, dv = 2, 90, 140, 4, 2, 32, 64
+    start = -20  # rows 0 .. 19 see nothing, keys 70 .. 139 are seen by none
+    q, k, v, g = (torch.randn(b, n, m, w, device=device).to(dt)
+                  for n, m, w in ((t, 2 * h, d), (s, 2 * hk, d), (s, hk, dv), (t, h, dv)))
+    lam = torch.full((h,), 0.4, device=device)
+    mask = torch.ones(b, s, dtype=torch.bool, device=device)
+    mask[1, :8] = False  # and in the second sample rows 20 .. 27
+    rows = torch.zeros(b, t, dtype=torch.bool, device=device)
+    rows[:, :20], rows[1, :28] = True, True
+    keys = ~mask
+    keys[:, 70:] = True
+    got = []
+    for fill in (0.0, float("nan")):
+        q[rows], g[rows], k[keys], v[keys] = fill, fill, fill, fill
+        out, state = ops.diff_attention(q, k, v, lam, causal=True, q_start=start, mask=mask, return_state=True)
+        got.append((out, *ops.diff_attention_grad(g, q, k, v, lam, out, state, causal=True, q_start=start, mask=mask)))
+        out, dq, dk, dval, dlam = got[-1]
+        assert not out[rows].any() and not dq[rows].any() and not dk[keys].any() and not dval[keys].any()
+        assert all(bool(x.isfinite().all()) for x in got[-1])
+    assert all(torch.equal(x, y) for x, y in zip(*got))
+
+
 def test_on_another_stream(device):
     model = build(device, 5)
     x, ids, mask = data(device, 3, 40, [40, 3, 25])
