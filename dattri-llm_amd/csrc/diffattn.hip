@@ -37,7 +37,7 @@ struct Smem {
 // kFine: probabilities as the sum of two 16-bit values.  Where a token's few rows leave the
 // matrix units idle that costs nothing, and the values are rounded once, at the end.
 template <int DT, int DP, int DVP, int NG, bool kFine>
-__global__ __launch_bounds__(2 * NG * kWave, 2) void diff_forward(Args a) {
+__global__ __launch_bounds__(2 * NG * kWave, DT == DA_F32 && DVP == 256 ? 1 : 2) void diff_forward(Args a) {
   using L = Smem<DT, DP, DVP, NG>;
   constexpr int NT = L::NT, ES = Type<DT>::ES, V = Type<DT>::V;
   constexpr int KD = DP / Type<DT>::kStep, NB = DVP / 32, KC = Type<DT>::kChunks;

@@ -30,7 +30,7 @@ namespace {
 // a token.
 //
 // Where keys are columns, a row's lse and delta are needed in every lane, by register.  In
-// bf16 they come with the products instead: one more step of contraction over their parts
+// 16 bits they come with the products instead: one more step of contraction over their parts
 // (three bf16 values hold 24 bits) against ones makes the scores' accumulators z - lse / c and
 // g v^T - delta, from two reads of LDS in place of sixteen.  A record then is the parts of
 // [-lse_1 / c | -delta_1 | -lse_2' / c | delta_1 - delta_2], eight entries each; else it is the
@@ -42,7 +42,7 @@ constexpr float kNothing = -1e30f;
 
 template <int DT>
 struct Record {
-  static constexpr bool kParts = DT == DA_BF16;
+  static constexpr bool kParts = DT != DA_F32;
   static constexpr int kBytes = kParts ? 64 : 16;
 };
 
@@ -314,11 +314,11 @@ __global__ __launch_bounds__(kThreads, DT != DA_F32 && DP == 64 ? 2 : 1) void di
       uint32_t low = in_low;
       asm("" : "+v"(low) : "s"(r0));  // two instructions a tile instead of eight registers
       const u32x4 of_low = {kOnes & low, kOne & low, 0, 0}, of_high = {kOnes & ~low, kOne & ~low, 0, 0};
-      Mfma32<DT>::mma(s0, r1, of_low);
-      Mfma32<DT>::mma(s1, r2, of_low);
-      Mfma32<DT>::mma(dp, r1, of_high);
+      Mfma32<DA_BF16>::mma(s0, r1, of_low);
+      Mfma32<DA_BF16>::mma(s1, r2, of_low);
+      Mfma32<DA_BF16>::mma(dp, r1, of_high);
       dp1 = dp;
-      Mfma32<DT>::mma(dp1, r2, of_high);
+      Mfma32<DA_BF16>::mma(dp1, r2, of_high);
     } else {
       dp1 = dp;
 #pragma unroll
@@ -414,7 +414,7 @@ struct RowSmem {
 };
 
 template <int DT, int DP, int DVP>
-__global__ __launch_bounds__(kThreads, DT != DA_F32 && DVP <= 128 ? 2 : 1) void diff_grad_rows(Args a) {
+__global__ __launch_bounds__(kThreads, DT != DA_F32 && DP == 64 ? 2 : 1) void diff_grad_rows(Args a) {
   using L = RowSmem<DT, DP, DVP>;
   constexpr int ES = Type<DT>::ES, V = Type<DT>::V;
   constexpr int KD = DP / Type<DT>::kStep, KV = DVP / Type<DT>::kStep, KC = Type<DT>::kChunks, ND = DP / 32;
@@ -493,16 +493,14 @@ __global__ __launch_bounds__(kThreads, DT != DA_F32 && DVP <= 128 ? 2 : 1) void 
     if (live.word) fetch(live.key, stage ^ 1, live.word);
     if (key > most) return;
     constexpr int skip = stage * L::kStage;
-    const auto lk = key_reader.fresh(key);
-    const auto lv = value_reader.fresh(key);
     f32x16 s0 = zeros(), s1 = zeros(), dp = zeros();
 #pragma unroll
     for (int kk = 0; kk < KD; ++kk) {
-      Mfma32<DT>::mma(s0, lk.rows(skip, kk), q[0][kk]);
-      Mfma32<DT>::mma(s1, lk.rows(skip + L::kK, kk), q[1][kk]);
+      Mfma32<DT>::mma(s0, key_reader.rows(skip, kk), q[0][kk]);
+      Mfma32<DT>::mma(s1, key_reader.rows(skip + L::kK, kk), q[1][kk]);
     }
 #pragma unroll
-    for (int kk = 0; kk < KV; ++kk) Mfma32<DT>::mma(dp, lv.rows(skip, kk), g[kk]);
+    for (int kk = 0; kk < KV; ++kk) Mfma32<DT>::mma(dp, value_reader.rows(skip, kk), g[kk]);
     const bool some = word != ~0u || key + kTile - 1 > least;
     const uint32_t seen = some ? seen_of(word, key, last, half) : ~0u;
 #pragma unroll
@@ -522,8 +520,8 @@ __global__ __launch_bounds__(kThreads, DT != DA_F32 && DVP <= 128 ? 2 : 1) void 
       const u32x4 y0 = from_acc<DT>(s0, j), y1 = from_acc<DT>(s1, j);
 #pragma unroll
       for (int n = 0; n < ND; ++n) {
-        Mfma32<DT>::mma(dq[0][n], lk.columns(skip, n, j), y0);
-        Mfma32<DT>::mma(dq[1][n], lk.columns(skip + L::kK, n, j), y1);
+        Mfma32<DT>::mma(dq[0][n], key_reader.columns(skip, n, j), y0);
+        Mfma32<DT>::mma(dq[1][n], key_reader.columns(skip + L::kK, n, j), y1);
       }
     }
   };
@@ -570,11 +568,13 @@ void chunks_of(int64_t groups, int64_t T, int64_t cus, int* chunk, int* chunks) 
 }
 
 // Blocks of one side's entries, and splits of the other's: so many that every CU has two
-// workgroups, none under 256 entries.
+// workgroups, none under kLeastSplit entries (18 heads of 509 keys in fp32, both passes: 269 us
+// from 256 on, which leaves it whole, 136 from 128, 152 from 64).
+constexpr int kLeastSplit = 128;
 void share(int64_t mine, int64_t others, int64_t groups, int64_t cus, int* blocks, int* splits, int* each) {
   const int64_t n = std::max<int64_t>(1, (mine + kWaves * kTile - 1) / (kWaves * kTile));
   int64_t want = std::max<int64_t>(1, 2 * cus / std::max<int64_t>(1, groups * n));
-  want = std::max<int64_t>(1, std::min(want, others / 256));
+  want = std::max<int64_t>(1, std::min(want, others / kLeastSplit));
   const int64_t e = std::max<int64_t>(kTile, ((others + want - 1) / want + kTile - 1) / kTile * kTile);
   *blocks = (int)n, *each = (int)e;
   *splits = (int)std::max<int64_t>(1, (others + e - 1) / e);
@@ -597,7 +597,7 @@ int plan(int dtype, int64_t batch, int64_t heads, int64_t k_heads, int64_t T, in
   share(S, rows, batch * k_heads, cus, &p->keys.blocks, &p->keys.splits, &p->keys.each);
   share(rows, S, batch * k_heads, cus, &p->rows.blocks, &p->rows.splits, &p->rows.each);
   p->records_at = (batch * heads * T * 2 + 3) / 4 * 4;
-  p->parts_at = p->records_at + batch * heads * T * (dtype == DA_BF16 ? Record<DA_BF16>::kBytes : Record<DA_F32>::kBytes) / 4;
+  p->parts_at = p->records_at + batch * heads * T * (dtype == DA_F32 ? Record<DA_F32>::kBytes : Record<DA_BF16>::kBytes) / 4;
   p->most_at = p->parts_at + batch * heads * a->chunks;
   p->takes_part_at = p->most_at + 1;
   p->sums_at = (p->takes_part_at + (batch * heads * T + 3) / 4 + 3) / 4 * 4;
