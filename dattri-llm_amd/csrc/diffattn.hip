@@ -22,7 +22,8 @@ namespace da {
 namespace diff {
 namespace {
 
-constexpr int kLeastSplit = 128;  // keys of a split (64: no faster; 256: 111 us in place of 91 for 18 heads of 509 keys in fp32)
+// Keys of a split (18 heads of 509 keys in fp32: 65 us with 64, 59 with 128).
+constexpr int kLeastSplit = 128;
 constexpr float kMostSum = 1024.f;  // of sixteen exponentials, before a new maximum
 
 // NG tiles of rows, each with a wave for either map.
@@ -301,18 +302,19 @@ int allow_lds(const void* kernel, int bytes) {
 
 namespace {
 
-// How rows are shared out: *ng tiles a workgroup, one where there are few.
+// How rows are shared out: *ng tiles a workgroup.  Two share the keys they read (18 heads of
+// 509 rows in fp32: 59 us, with one 88; 16 on 4 of 1024, 128 and 256 wide in bf16: 74 and 100).
 int plan(int64_t batch, int64_t T, int64_t S, int64_t k_heads, int64_t G, int* ng, Args* a) {
   int64_t cus;
   const int rc = device_cu_count(&cus);
   if (rc) return rc;
   const int64_t rows = T * G, heads = batch * k_heads;
   const auto blocks_of = [&](int64_t n) { return (rows + n * kTile - 1) / (n * kTile); };
-  *ng = heads * blocks_of(2) >= 2 * cus ? 2 : 1;
+  *ng = rows > kTile ? 2 : 1;
   const int64_t blocks = blocks_of(*ng), groups = std::max<int64_t>(1, heads * blocks);
-  // Keys are split where the rows leave CUs without work: up to eight workgroups a CU, no
-  // split under kLeastSplit keys.
-  int64_t want = *ng == 1 ? std::max<int64_t>(1, 8 * cus / groups) : 1;
+  // Keys are split where the rows leave CUs without work: up to sixteen waves a CU, no split
+  // under kLeastSplit keys.
+  int64_t want = std::max<int64_t>(1, (*ng == 1 ? 8 : 4) * cus / groups);
   want = std::max<int64_t>(1, std::min(want, S / kLeastSplit));
   const int64_t each = std::max<int64_t>(kTile, ((S + want - 1) / want + kTile - 1) / kTile * kTile);
   a->blocks = (int)blocks;
