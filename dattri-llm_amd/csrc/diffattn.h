@@ -172,6 +172,9 @@ struct Rows : Tile<DT, W, NT> {
   }
 };
 
+// A barrier that the tiles under way have to reach first: the compiler does not count their
+// loads, and its own barrier waits for none of them.
+__device__ __forceinline__ void tiles_barrier() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 __device__ __forceinline__ uint32_t lds_address(const char* p) { return (uint32_t)(uintptr_t)(const lds_char*)p; }
 __device__ __forceinline__ u32x4 lds16(uint32_t at) {

@@ -103,7 +103,7 @@ __global__ __launch_bounds__(2 * NG * kWave, DT == DA_F32 && DVP == 256 ? 1 : 2)
     key = live.key;
     const uint32_t word = live.word;
     live.next(a, b, end, lane);
-    __syncthreads();
+    tiles_barrier();
     if (live.word) fetch(live.key, stage ^ 1, live.word);
     if (key > most) return;
     f32x16 s = zeros();

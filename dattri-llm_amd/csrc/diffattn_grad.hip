@@ -289,7 +289,7 @@ __global__ __launch_bounds__(kThreads, DT != DA_F32 && DP == 64 ? 2 : 1) void di
   const auto step = [&](int r0, auto of) __attribute__((always_inline)) {
     constexpr int stage = decltype(of)::value;
     constexpr int skip = stage * L::kStage;
-    __syncthreads();
+    tiles_barrier();
     if (r0 + kTile < end) {
       fetch(r0 + kTile, stage ^ 1, key_word(byte));
       byte = row_byte(r0 + 2 * kTile);
@@ -489,7 +489,7 @@ __global__ __launch_bounds__(kThreads, DT != DA_F32 && DP == 64 ? 2 : 1) void di
     key = live.key;
     const uint32_t word = live.word;
     live.next(a, b, end, lane);
-    __syncthreads();
+    tiles_barrier();
     if (live.word) fetch(live.key, stage ^ 1, live.word);
     if (key > most) return;
     constexpr int skip = stage * L::kStage;

@@ -271,6 +271,23 @@ def test_rows_and_keys_that_see_nothing_may_hold_anything(device, dt):
     assert all(torch.equal(x, y) for x, y in zip(*got))
 
 
+@pytest.mark.parametrize("masked", [False, True])
+def test_a_long_run_of_tiles_gives_the_same_results_every_time(device, masked):
+    """Tiles are read ahead into LDS: with every CU busy they come late, and must be awaited."""
+    torch.manual_seed(8)
+    b, t, h, hk, d, dv = 2, 2048, 32, 8, 64, 128
+    q, k, v, g = (torch.randn(b, t, m, w, device=device).bfloat16() for m, w in ((2 * h, d), (2 * hk, d), (hk, dv), (h, dv)))
+    lam = torch.rand(h, device=device)
+    mask = torch.arange(t, device=device)[None] < torch.tensor([2000, 2048], device=device)[:, None] if masked else None
+    first = None
+    for _ in range(6):
+        out, state = ops.diff_attention(q, k, v, lam, causal=True, mask=mask, return_state=True)
+        got = (out, state.lse, *ops.diff_attention_grad(g, q, k, v, lam, out, state, causal=True, mask=mask))
+        assert all(bool(x.isfinite().all()) for x in got)
+        first = got if first is None else first
+        assert all(torch.equal(x, y) for x, y in zip(got, first))
+
+
 def test_on_another_stream(device):
     model = build(device, 5)
     x, ids, mask = data(device, 3, 40, [40, 3, 25])
