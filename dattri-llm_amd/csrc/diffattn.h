@@ -40,9 +40,11 @@ struct Args {
   const char* g;
   int64_t g_b, g_t, g_h;
   float* delta;   // (batch, Hk, 2, T G): g . o_m
+  int row_splits;
   char* records;  // (batch, Hk, T G): lse and delta of both maps as diff_grad_keys reads them
   uint8_t* takes_part;  // (batch, Hk, T G): whether the row sees a key
-  float* most;    // largest |g| of the call (16-bit floats of five exponent bits)
+  float* off;     // 16 bits: (row splits, batch, Hk, 2, T G): how far delta was off, in parts
+  float* most;    // fp16: largest norms of g's rows and of v's, squared
   char *dq, *dk, *dv;
   float* lam_part;  // (batch, heads, chunks)
   int chunk, chunks;

@@ -7,15 +7,27 @@
 //   dq_m = scale ds_m k_m,   dk_m = scale ds_m^T q_m,   dv = (p_1 - lam p_2)^T g
 //   dlam[sample] = -sum of delta_2
 //
-// Three launches and no atomic sums, so that results do not change from run to run: delta
-// and dlam's parts; dk and dv, a wave holding 32 keys and going over all rows of their
-// heads; dq, a wave holding 32 rows and going over their keys.  The scores are formed
+// Four launches and no atomic sums, so that results do not change from run to run: delta; dq, a
+// wave holding 32 rows and going over their keys; the records of rows and dlam's parts; dk and
+// dv, a wave holding 32 keys and going over all rows of their heads.  The scores are formed
 // twice, the price of sums that are nobody else's.  Where keys are columns, the scores'
 // registers are rows and stand as the operand that is contracted over rows; where rows are
 // columns, they are keys: neither pass moves a score between lanes.
 //
-// 16-bit floats of five exponent bits lose small values of ds: there ds is scaled by the
-// power of two that brings the largest |g| near one, and its products back.
+// What is rounded to 16 bits: ds and the maps' mixture where they are operands, by half a step
+// of each entry, no more than the outputs' own rounding; and out and o_2, from which delta
+// comes, off by as much for a whole row.  dq therefore takes ds as the sum of two 16-bit
+// values (with one, its error was 1.6 times that of its rounding; it costs 79 of 800 us at the
+// size below), and its pass sums ds in fp32: sum ds_m = delta_m - its first value, as the maps
+// sum to one.  The pass of dk and dv and dlam have delta from there.
+//
+// fp16 would lose small values of ds: there ds is scaled by the power of two that brings the
+// bound of the largest to 2^14, and its products back.
+//
+// 4 x 2048 tokens, 32 heads on 8, two 64-wide maps, 128-wide values, causal, bf16: dq 206 and
+// dk, dv 275 GFLOP of products.  Both passes are bound by the vector unit (two exponentials and
+// some twenty instructions an entry of the maps) and the matrix unit nearly in sum: with the
+// registers of two waves a SIMD there is little to put under the other one's work.
 #include <algorithm>
 #include <type_traits>
 
@@ -69,22 +81,19 @@ __device__ __forceinline__ void put_record(char* to, float c, float lse0, float 
 template <int DT>
 __global__ __launch_bounds__(256) void diff_delta(Args a) {
   constexpr int ES = Type<DT>::ES, V = Type<DT>::V, kRows = 256 / kLanes;
-  __shared__ float parts[kRows];
   const int heads = a.Hk * a.G, l = threadIdx.x % kLanes, sub = threadIdx.x / kLanes;
   const int chunk = blockIdx.x % a.chunks;
   const int h = blockIdx.x / a.chunks % heads, b = blockIdx.x / a.chunks / heads;
   const int hk = h / a.G, rows = a.T * a.G;
   const float lam = lam_of(a, h);
   const int t1 = min((chunk + 1) * a.chunk, a.T);
-  float all = 0.f, most = 0.f;
+  float most = 0.f;
   for (int t = chunk * a.chunk + sub; t < t1; t += kRows) {
     const int64_t of = (int64_t)b * a.Hk + hk;
     const int r = t * a.G + (h - hk * a.G);
-    const float* lse = a.lse + of * 2 * rows + r;
     // Of a row that sees no key nothing is read: its gradient may be anything.
-    const float lse0 = lse[0];
-    const bool live = lse0 != __builtin_inff();
-    float d0 = 0.f, d1 = 0.f;
+    const bool live = a.lse[of * 2 * rows + r] != __builtin_inff();
+    float d0 = 0.f, d1 = 0.f, norm = 0.f;
     if (live) {
       const char* g = a.g + (b * a.g_b + t * a.g_t + h * a.g_h) * ES;
       const int64_t at = (((int64_t)b * a.T + t) * heads + h) * a.Dv * ES;
@@ -97,34 +106,74 @@ __global__ __launch_bounds__(256) void diff_delta(Args a) {
         for (int e = 0; e < V; ++e) {
           d0 += x[e] * y[e];
           d1 += x[e] * z[e];
-          if constexpr (DT == DA_F16) most = fmaxf(most, fabsf(x[e]));
+          if constexpr (DT == DA_F16) norm += x[e] * x[e];
         }
       }
     }
     d0 = lanes_sum<kLanes>(d0);
     d1 = lanes_sum<kLanes>(d1);
+    if constexpr (DT == DA_F16) most = fmaxf(most, lanes_sum<kLanes>(norm));
     if (l == 0) {
       float* to = a.delta + of * 2 * rows + r;
-      d0 += lam * d1;  // o_1 = out + lam o_2
-      to[0] = d0;
+      to[0] = d0 + lam * d1;  // o_1 = out + lam o_2
       to[rows] = d1;
       a.takes_part[of * rows + r] = live;
-      put_record<DT>(a.records + (of * rows + r) * Record<DT>::kBytes, a.scale * kLog2e, lse0,
-                     lse[rows] - log2f(fabsf(lam)), d0, d1);
     }
-    all += d1;
   }
   if constexpr (DT == DA_F16) {  // a maximum: the order does not matter
-    most = lanes_max<64>(most);
+    most = lanes_max<64>(most) * fmaxf(1.f, lam * lam);
     if (threadIdx.x % 64 == 0 && most > 0.f) atomicMax((unsigned*)a.most, __float_as_uint(most));
   }
-  if (l == 0) parts[sub] = all;
-  __syncthreads();
-  if (threadIdx.x) return;
-  float v = 0.f;
+}
+
+// The largest norm of the values' rows that a query may see, squared: 16 lanes a row.
+__global__ __launch_bounds__(256) void diff_values_norm(Args a) {
+  constexpr int V = Type<DA_F16>::V, kRows = 256 / kLanes;
+  const int l = threadIdx.x % kLanes;
+  const int64_t all = (int64_t)a.batch * a.S * a.Hk;
+  float most = 0.f;
+  for (int64_t at = (int64_t)blockIdx.x * kRows + threadIdx.x / kLanes; at < all; at += (int64_t)gridDim.x * kRows) {
+    const int hk = (int)(at % a.Hk), key = (int)(at / a.Hk % a.S), b = (int)(at / a.Hk / a.S);
+    float norm = 0.f;
+    if (!(a.causal && key >= a.T + a.q_start) && (!a.mask || a.mask[b * a.m_b + key * a.m_k])) {
+      const char* v = a.v + (b * a.v_b + key * a.v_t + hk * a.v_h) * 2;
+      for (int e0 = l * V; e0 < a.Dv; e0 += kLanes * V) {
+        float x[V];
+        unpack16<DA_F16>(load_run<DA_F16>(v, e0, a.Dv), x);
 #pragma unroll
-  for (int i = 0; i < kRows; ++i) v += parts[i];
-  a.lam_part[blockIdx.x] = -v;
+        for (int e = 0; e < V; ++e) norm += x[e] * x[e];
+      }
+    }
+    most = fmaxf(most, lanes_sum<kLanes>(norm));
+  }
+  most = lanes_max<64>(most);
+  if (threadIdx.x % 64 == 0 && most > 0.f) atomicMax((unsigned*)a.most + 1, __float_as_uint(most));
+}
+
+// After dq: delta as the maps in fp32 have it, the records, and dlam's parts.
+template <int DT>
+__global__ __launch_bounds__(256) void diff_records(Args a) {
+  __shared__ float parts[256 / kWave];
+  const int heads = a.Hk * a.G, chunk = blockIdx.x % a.chunks;
+  const int h = blockIdx.x / a.chunks % heads, b = blockIdx.x / a.chunks / heads;
+  const int hk = h / a.G, rows = a.T * a.G;
+  const float lam = lam_of(a, h), c = a.scale * kLog2e, bits = log2f(fabsf(lam));
+  const int t1 = min((chunk + 1) * a.chunk, a.T);
+  const int64_t of = (int64_t)b * a.Hk + hk, all = (int64_t)a.batch * a.Hk * 2 * rows;
+  float sum = 0.f;
+  for (int t = chunk * a.chunk + threadIdx.x; t < t1; t += 256) {
+    const int r = t * a.G + (h - hk * a.G);
+    const int64_t at = of * 2 * rows + r;
+    float d0 = a.delta[at], d1 = a.delta[at + rows];
+    if constexpr (DT != DA_F32)
+      for (int p = 0; p < a.row_splits; ++p) d0 += a.off[p * all + at], d1 += a.off[p * all + at + rows];
+    put_record<DT>(a.records + (of * rows + r) * Record<DT>::kBytes, c, a.lse[at], a.lse[at + rows] - bits, d0, d1);
+    sum += d1;
+  }
+  sum = lanes_sum<kWave>(sum);
+  if (threadIdx.x % kWave == 0) parts[threadIdx.x / kWave] = sum;
+  __syncthreads();
+  if (threadIdx.x == 0) a.lam_part[blockIdx.x] = -(parts[0] + parts[1] + parts[2] + parts[3]);
 }
 
 __global__ __launch_bounds__(256) void diff_lam_join(const float* parts, float* out, int64_t n, int chunks) {
@@ -135,12 +184,14 @@ __global__ __launch_bounds__(256) void diff_lam_join(const float* parts, float* 
   out[i] = v;
 }
 
-// The power of two that brings the largest |g| to [1, 2): 1 where there is no such.
+// fp16: a power of two under which no |ds| <= 2 max(1, |lam|) |g| |v| passes 2^14, and the
+// largest are near it: the maps' small entries keep their bits.  1 where there is none.
 template <int DT>
 __device__ __forceinline__ float small_scale(const Args& a) {
   if constexpr (DT != DA_F16) return 1.f;
-  const uint32_t e = __float_as_uint(*a.most) >> 23;  // of a float above zero
-  return e == 0 || e == 255 ? 1.f : __uint_as_float((254 - e) << 23);
+  const float bound = __builtin_sqrtf(a.most[0]) * __builtin_sqrtf(a.most[1]);
+  const uint32_t e = __float_as_uint(bound) >> 23;  // bound < 2^(e - 126); of a float from zero on
+  return e < 40 || e > 220 ? 1.f : __uint_as_float((266u - e) << 23);  // 2^(139 - e)
 }
 
 // ---------------------------------------------------------------------------
@@ -477,6 +528,7 @@ __global__ __launch_bounds__(kThreads, DT != DA_F32 && DP == 64 ? 2 : 1) void di
     keys.fetch(kp + (to * a.k_t + a.k_h) * ES, l + L::kK, live);
     values.fetch(vp + to * a.v_t * ES, l + 2 * L::kK, live);
   };
+  float off0 = 0.f, off1 = 0.f;
   f32x16 dq[2][ND];
 #pragma unroll
   for (int n = 0; n < ND; ++n) dq[0][n] = zeros(), dq[1][n] = zeros();
@@ -493,14 +545,16 @@ __global__ __launch_bounds__(kThreads, DT != DA_F32 && DP == 64 ? 2 : 1) void di
     if (live.word) fetch(live.key, stage ^ 1, live.word);
     if (key > most) return;
     constexpr int skip = stage * L::kStage;
+    const auto lk = key_reader.fresh(key);
+    const auto lv = value_reader.fresh(key);
     f32x16 s0 = zeros(), s1 = zeros(), dp = zeros();
 #pragma unroll
     for (int kk = 0; kk < KD; ++kk) {
-      Mfma32<DT>::mma(s0, key_reader.rows(skip, kk), q[0][kk]);
-      Mfma32<DT>::mma(s1, key_reader.rows(skip + L::kK, kk), q[1][kk]);
+      Mfma32<DT>::mma(s0, lk.rows(skip, kk), q[0][kk]);
+      Mfma32<DT>::mma(s1, lk.rows(skip + L::kK, kk), q[1][kk]);
     }
 #pragma unroll
-    for (int kk = 0; kk < KV; ++kk) Mfma32<DT>::mma(dp, value_reader.rows(skip, kk), g[kk]);
+    for (int kk = 0; kk < KV; ++kk) Mfma32<DT>::mma(dp, lv.rows(skip, kk), g[kk]);
     const bool some = word != ~0u || key + kTile - 1 > least;
     const uint32_t seen = some ? seen_of(word, key, last, half) : ~0u;
 #pragma unroll
@@ -514,14 +568,22 @@ __global__ __launch_bounds__(kThreads, DT != DA_F32 && DP == 64 ? 2 : 1) void di
       }
       s0[i] = p0 * (dp[i] - de0);
       s1[i] = p1 * fmaf(dp[i], sign, de1);
+      if constexpr (DT != DA_F32) off0 += s0[i], off1 += s1[i];
     }
 #pragma unroll
     for (int j = 0; j < KC; ++j) {
       const u32x4 y0 = from_acc<DT>(s0, j), y1 = from_acc<DT>(s1, j);
+      u32x4 rest0, rest1;
+      if constexpr (DT != DA_F32) rest0 = rest_of<DT>(s0, j, y0), rest1 = rest_of<DT>(s1, j, y1);
 #pragma unroll
       for (int n = 0; n < ND; ++n) {
-        Mfma32<DT>::mma(dq[0][n], key_reader.columns(skip, n, j), y0);
-        Mfma32<DT>::mma(dq[1][n], key_reader.columns(skip + L::kK, n, j), y1);
+        const u32x4 k0 = lk.columns(skip, n, j), k1 = lk.columns(skip + L::kK, n, j);
+        Mfma32<DT>::mma(dq[0][n], k0, y0);
+        Mfma32<DT>::mma(dq[1][n], k1, y1);
+        if constexpr (DT != DA_F32) {
+          Mfma32<DT>::mma(dq[0][n], k0, rest0);
+          Mfma32<DT>::mma(dq[1][n], k1, rest1);
+        }
       }
     }
   };
@@ -529,7 +591,15 @@ __global__ __launch_bounds__(kThreads, DT != DA_F32 && DP == 64 ? 2 : 1) void di
     step(std::integral_constant<int, 0>{});
     if (live.word) step(std::integral_constant<int, 1>{});
   }
+  off0 += other_half(off0);
+  off1 += other_half(off1);
   if (r >= rows) return;
+  if (DT != DA_F32 && half == 0) {
+    float* to = a.off + (int64_t)split * a.batch * a.Hk * 2 * rows + base;
+    to[0] = off0 / small;
+    // A factor so small that its map's entries vanish tells nothing.
+    to[rows] = fabsf(lam) > 0x1p-60f ? off1 / (sign * fabsf(lam) * small) : 0.f;
+  }
   const float by = a.scale / small;
   const int64_t to = ((int64_t)b * a.T + t) * (a.Hk * a.G) + h;
 #pragma unroll
@@ -584,7 +654,7 @@ void share(int64_t mine, int64_t others, int64_t groups, int64_t cus, int* block
 // |g|, the records, whether a row takes part, and the sums of the splits (of one pass after the other).
 struct Plan {
   Args keys, rows;  // blocks, splits, each
-  int64_t records_at, parts_at, most_at, takes_part_at, sums_at;  // in floats
+  int64_t records_at, parts_at, most_at, off_at, takes_part_at, sums_at;  // in floats
   size_t bytes;
 };
 
@@ -599,7 +669,8 @@ int plan(int dtype, int64_t batch, int64_t heads, int64_t k_heads, int64_t T, in
   p->records_at = (batch * heads * T * 2 + 3) / 4 * 4;
   p->parts_at = p->records_at + batch * heads * T * (dtype == DA_F32 ? Record<DA_F32>::kBytes : Record<DA_BF16>::kBytes) / 4;
   p->most_at = p->parts_at + batch * heads * a->chunks;
-  p->takes_part_at = p->most_at + 1;
+  p->off_at = p->most_at + 2;
+  p->takes_part_at = p->off_at + (dtype == DA_F32 ? 0 : p->rows.splits * batch * heads * T * 2);
   p->sums_at = (p->takes_part_at + (batch * heads * T + 3) / 4 + 3) / 4 * 4;
   const int64_t of_keys = p->keys.splits > 1 ? p->keys.splits * batch * S * k_heads * (2 * D + Dv) : 0;
   const int64_t of_rows = p->rows.splits > 1 ? p->rows.splits * batch * T * heads * 2 * D : 0;
@@ -672,27 +743,21 @@ int da_diff_attention_grad(const da_diff_inputs* in, const void* g, int64_t g_bs
   a.records = (char*)(a.delta + p.records_at);
   a.lam_part = a.delta + p.parts_at;
   a.most = a.delta + p.most_at;
+  a.off = a.delta + p.off_at;
+  a.row_splits = p.rows.splits;
   a.takes_part = (uint8_t*)(a.delta + p.takes_part_at);
   a.part = a.delta + p.sums_at;
   a.dq = (char*)dq, a.dk = (char*)dk, a.dv = (char*)dvalue;
   const hipStream_t st = (hipStream_t)stream;
-  if (dtype == DA_F16 && (rc = zero_f32_2d(a.most, 1, 1, 1, st))) return rc;
+  if (dtype == DA_F16 && (rc = zero_f32_2d(a.most, 1, 2, 2, st))) return rc;
   const unsigned delta_grid = (unsigned)(batch * heads * a.chunks);
   if (dtype == DA_BF16) diff_delta<DA_BF16><<<delta_grid, 256, 0, st>>>(a);
   else if (dtype == DA_F16) diff_delta<DA_F16><<<delta_grid, 256, 0, st>>>(a);
   else diff_delta<DA_F32><<<delta_grid, 256, 0, st>>>(a);
-  diff_lam_join<<<(unsigned)((batch * heads + 255) / 256), 256, 0, st>>>(a.lam_part, dlam, batch * heads, a.chunks);
+  if (dtype == DA_F16 && k_len)
+    diff_values_norm<<<(unsigned)std::min<int64_t>(1024, (pairs * k_len + 15) / 16), 256, 0, st>>>(a);
   rc = by_widths(dtype, widths(d, dv), [&](auto dt, auto dp, auto dvp) {
     constexpr int DT = decltype(dt)::value, DP = decltype(dp)::value, DVP = decltype(dvp)::value;
-    if (k_len) {
-      constexpr int kBytes = KeySmem<DT, DP, DVP>::kBytes;
-      if (const int err = allow_lds((const void*)diff_grad_keys<DT, DP, DVP>, kBytes)) return err;
-      a.blocks = p.keys.blocks, a.splits = p.keys.splits, a.each = p.keys.each;
-      diff_grad_keys<DT, DP, DVP><<<(unsigned)(pairs * a.blocks * a.splits), kThreads, kBytes, st>>>(a);
-      const int64_t n_first = pairs * k_len * 2 * d, n = n_first + pairs * k_len * dv;
-      if (a.splits > 1)
-        if (const int err = join<DT>(a.part, a.splits, n, dk, n_first, dvalue, st)) return err;
-    }
     if (rows) {
       constexpr int kBytes = RowSmem<DT, DP, DVP>::kBytes;
       if (const int err = allow_lds((const void*)diff_grad_rows<DT, DP, DVP>, kBytes)) return err;
@@ -701,6 +766,17 @@ int da_diff_attention_grad(const da_diff_inputs* in, const void* g, int64_t g_bs
       const int64_t n = batch * q_len * heads * 2 * d;
       if (a.splits > 1)
         if (const int err = join<DT>(a.part, a.splits, n, dq, n, nullptr, st)) return err;
+    }
+    diff_records<DT><<<delta_grid, 256, 0, st>>>(a);
+    diff_lam_join<<<(unsigned)((batch * heads + 255) / 256), 256, 0, st>>>(a.lam_part, dlam, batch * heads, a.chunks);
+    if (k_len) {
+      constexpr int kBytes = KeySmem<DT, DP, DVP>::kBytes;
+      if (const int err = allow_lds((const void*)diff_grad_keys<DT, DP, DVP>, kBytes)) return err;
+      a.blocks = p.keys.blocks, a.splits = p.keys.splits, a.each = p.keys.each;
+      diff_grad_keys<DT, DP, DVP><<<(unsigned)(pairs * a.blocks * a.splits), kThreads, kBytes, st>>>(a);
+      const int64_t n_first = pairs * k_len * 2 * d, n = n_first + pairs * k_len * dv;
+      if (a.splits > 1)
+        if (const int err = join<DT>(a.part, a.splits, n, dk, n_first, dvalue, st)) return err;
     }
     return check_launch("da_diff_attention_grad");
   });
