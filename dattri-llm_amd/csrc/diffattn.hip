@@ -10,9 +10,13 @@
 // rounded, the second operand of o^T = v^T p^T as they stand, where v is read transposed out
 // of LDS.  Exponentials are relative to a maximum that is looked for again only when the sum
 // of a lane's sixteen passes 2^10: until then they are at most that much larger than with the
-// last one (the first tile has none, and passes).  The vector unit bounds the loop, so that
-// what a tile need not do is left out.  At the end the second map's waves hand their values,
-// divided and weighted, to the first's through LDS.
+// last one (the first tile has none, and passes; with a new one in every tile that has a larger
+// score 277 us in place of 257 at the first size below).  At the end the second map's waves hand
+// their values, divided and weighted, to the first's through LDS.
+//
+// 4 x 2048 causal tokens in bf16: 32 heads on 8, two 64-wide maps and 128-wide values 257 us
+// (206 GFLOP, 800 TFLOP/s), 16 heads of 128 and 256 261 us (790 TFLOP/s): vector and matrix unit
+// nearly in sum.  16 new tokens of 32 heads on 8 against 8192 positions 94 + 11 us, HBM at 4.8 TB/s.
 #include <algorithm>
 #include <type_traits>
 
@@ -36,7 +40,9 @@ struct Smem {
 };
 
 // kFine: probabilities as the sum of two 16-bit values.  Where a token's few rows leave the
-// matrix units idle that costs nothing, and the values are rounded once, at the end.
+// matrix units idle that costs nothing, and the values are rounded once, at the end (bf16 error
+// 1.7e-3).  Else they are rounded where they are multiplied, by half a step each, no more than
+// the output's own rounding (2.4e-3 together); sums stay in fp32.
 template <int DT, int DP, int DVP, int NG, bool kFine>
 __global__ __launch_bounds__(2 * NG * kWave, DT == DA_F32 && DVP == 256 ? 1 : 2) void diff_forward(Args a) {
   using L = Smem<DT, DP, DVP, NG>;

@@ -107,6 +107,13 @@ CASES = [  # b, t, v, dtype, top, temperature, masked
     (1, 1, 262144, "fp32", 32, 1.0, False),
     (1, 290, 9001, "bf16", 0, 1.0, False),
     (7, 1, 151936, "bf16", 1, 1.0, False),
+    # many short rows
+    (4, 300, 1, "fp32", 1, 1.0, False),
+    (2, 520, 7, "bf16", 5, 1.0, True),
+    (3, 350, 513, "bf16", 20, 1.3, True),
+    (1, 1100, 4097, "fp16", 32, 1.0, False),
+    (4, 256, 8191, "fp32", 32, 0.7, True),
+    (2, 600, 16385, "bf16", 0, 1.0, True),
 ]
 
 
@@ -146,7 +153,7 @@ def test_strides(v, layout):
     check(x, target, mask=mask, top=4)
 
 
-@pytest.mark.parametrize("v,rows", [(50, 4), (3000, 2), (30000, 300), (60000, 3)])
+@pytest.mark.parametrize("v,rows", [(50, 4), (50, 1100), (3000, 2), (3000, 1100), (30000, 300), (60000, 3)])
 @pytest.mark.parametrize("kind", ["equal", "rising", "falling", "two_values", "few_finite", "lowest", "signed_zeros"])
 def test_orders_that_try_the_alternatives(v, rows, kind):
     """Ties in every place, sorted rows (more entries than fit reach the bound), rows of -inf and of a type's lowest value."""
