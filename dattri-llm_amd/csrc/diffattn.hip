@@ -43,6 +43,8 @@ struct Smem {
 // matrix units idle that costs nothing, and the values are rounded once, at the end (bf16 error
 // 1.7e-3).  Else they are rounded where they are multiplied, by half a step each, no more than
 // the output's own rounding (2.4e-3 together); sums stay in fp32.
+// Two waves a SIMD but for the widest maps in fp32, which would spill (8 heads of 2 x 512 tokens
+// 203 us in place of 141) and whose tiles leave LDS for one workgroup anyway.
 template <int DT, int DP, int DVP, int NG, bool kFine>
 __global__ __launch_bounds__(2 * NG * kWave, DT == DA_F32 && DVP == 256 ? 1 : 2) void diff_forward(Args a) {
   using L = Smem<DT, DP, DVP, NG>;
