@@ -28,6 +28,7 @@ namespace {
 
 // Keys of a split (18 heads of 509 keys in fp32: 65 us with 64, 59 with 128).
 constexpr int kLeastSplit = 128;
+constexpr int kFewKeys = 512;
 constexpr float kMostSum = 1024.f;  // of sixteen exponentials, before a new maximum
 
 // NG tiles of rows, each with a wave for either map.
@@ -39,9 +40,10 @@ struct Smem {
   static constexpr int kBytes = 2 * kStage > kHanded ? 2 * kStage : kHanded;
 };
 
-// kFine: probabilities as the sum of two 16-bit values.  Where a token's few rows leave the
-// matrix units idle that costs nothing, and the values are rounded once, at the end (bf16 error
-// 1.7e-3).  Else they are rounded where they are multiplied, by half a step each, no more than
+// kFine: probabilities as the sum of two 16-bit values, so that values are rounded once, at the
+// end (bf16 error 1.7e-3).  Where a token's few rows leave the matrix units idle that costs
+// nothing, and with few keys little (2 x 472 tokens of 15 heads 53 us in place of 51, 16 x 512 of 32
+// on 8 135 and 116; 4 x 2048 would pay two thirds more products).  Else they are rounded where they are multiplied, by half a step each, no more than
 // the output's own rounding (2.4e-3 together); sums stay in fp32.
 // Two waves a SIMD but for the widest maps in fp32, which would spill (8 heads of 2 x 512 tokens
 // 203 us in place of 141) and whose tiles leave LDS for one workgroup anyway.
@@ -388,16 +390,19 @@ int da_diff_attention(const da_diff_inputs* in, int dtype, int64_t batch, int64_
   const hipStream_t st = (hipStream_t)stream;
   return by_widths(dtype, w, [&](auto dt, auto dp, auto dvp) {
     constexpr int DT = decltype(dt)::value, DP = decltype(dp)::value, DVP = decltype(dvp)::value;
-    const auto launch = [&](auto groups) {
+    const auto launch = [&](auto groups, auto fine) {
       constexpr int NG = decltype(groups)::value;
-      constexpr bool kFine = DT != DA_F32 && NG == 1;
+      constexpr bool kFine = DT != DA_F32 && decltype(fine)::value;
       constexpr int kBytes = Smem<DT, DP, DVP, NG>::kBytes;
       const auto kernel = diff_forward<DT, DP, DVP, NG, kFine>;
       if (const int err = allow_lds((const void*)kernel, kBytes)) return err;
       kernel<<<grid, 2 * NG * kWave, kBytes, st>>>(a);
       return (int)DA_OK;
     };
-    const int err = ng == 1 ? launch(std::integral_constant<int, 1>{}) : launch(std::integral_constant<int, 2>{});
+    using One = std::integral_constant<int, 1>;
+    using Two = std::integral_constant<int, 2>;
+    const int err = ng == 1 ? launch(One{}, std::true_type{})
+                    : k_len <= kFewKeys ? launch(Two{}, std::true_type{}) : launch(Two{}, std::false_type{});
     if (err) return err;
     if (a.splits > 1) {
       constexpr int kRows = 256 / (DVP / 4);

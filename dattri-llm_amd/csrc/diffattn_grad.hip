@@ -457,7 +457,11 @@ __global__ __launch_bounds__(kThreads, DT != DA_F32 && DP == 64 ? 2 : 1) void di
 }
 
 // ---------------------------------------------------------------------------
-// dq: four waves of 32 rows over their keys.
+// dq: four waves of 32 rows over their keys.  In 16 bits, where these are few, twice: a first time
+// for the sums that delta comes from.  Of few keys each counts for much, and dq's error was twice
+// its rounding with two of them; of many it is hidden behind theirs.  (64 x 200 tokens of 16 heads
+// on 4: both passes 181 us with one, 240 with two.)  Fewer keys than two splits have: one split
+// knows the whole sum.
 // ---------------------------------------------------------------------------
 template <int DT, int DP, int DVP>
 struct RowSmem {
@@ -468,7 +472,7 @@ struct RowSmem {
 
 // Two waves a SIMD where the operands of 64-wide maps leave room for them (128-wide ones spill:
 // 2 x 2048 tokens of 16 heads, 128 and 128 wide, both passes 670 us with two, 431 with one).
-template <int DT, int DP, int DVP>
+template <int DT, int DP, int DVP, bool kTwice>
 __global__ __launch_bounds__(kThreads, DT != DA_F32 && DP == 64 ? 2 : 1) void diff_grad_rows(Args a) {
   using L = RowSmem<DT, DP, DVP>;
   constexpr int ES = Type<DT>::ES, V = Type<DT>::V;
@@ -519,7 +523,7 @@ __global__ __launch_bounds__(kThreads, DT != DA_F32 && DP == 64 ? 2 : 1) void di
   // The second map's factor comes with its exponential, the sign with its values' gradient.
   const float lam = in ? lam_of(a, h) : 0.f, sign = lam < 0.f ? 1.f : -1.f;
   const float lse1 = in ? a.lse[base + rows] - log2f(fabsf(lam)) : __builtin_inff();
-  const float de0 = in ? a.delta[base] : 0.f, de1 = in ? -sign * a.delta[base + rows] : 0.f;
+  float de0 = in ? a.delta[base] : 0.f, de1 = in ? -sign * a.delta[base + rows] : 0.f;
   const float c = a.scale * kLog2e, small = small_scale<DT>(a);
 
   const Keys<DT, DP, kThreads> keys(a.k_t, a.D);
@@ -536,8 +540,10 @@ __global__ __launch_bounds__(kThreads, DT != DA_F32 && DP == 64 ? 2 : 1) void di
   f32x16 dq[2][ND];
 #pragma unroll
   for (int n = 0; n < ND; ++n) dq[0][n] = zeros(), dq[1][n] = zeros();
+  const int start = key;
   Live live(a, b, key, end, lane);
   if (live.word) fetch(live.key, 0, live.word);
+  bool sums_only = kTwice;
   const Reader<DT, DP> key_reader(lds, lane);
   const Reader<DT, DVP> value_reader(lds + 2 * L::kK, lane);
   const auto step = [&](auto of) __attribute__((always_inline)) {
@@ -574,6 +580,7 @@ __global__ __launch_bounds__(kThreads, DT != DA_F32 && DP == 64 ? 2 : 1) void di
       s1[i] = p1 * fmaf(dp[i], sign, de1);
       if constexpr (DT != DA_F32) off0 += s0[i], off1 += s1[i];
     }
+    if (kTwice && sums_only) return;
 #pragma unroll
     for (int j = 0; j < KC; ++j) {
       const u32x4 y0 = from_acc<DT>(s0, j), y1 = from_acc<DT>(s1, j);
@@ -591,18 +598,30 @@ __global__ __launch_bounds__(kThreads, DT != DA_F32 && DP == 64 ? 2 : 1) void di
       }
     }
   };
-  while (live.word) {
-    step(std::integral_constant<int, 0>{});
-    if (live.word) step(std::integral_constant<int, 1>{});
+  // A factor so small that its map's entries vanish tells nothing of delta.
+  const float to_off0 = 1.f / small, to_off1 = fabsf(lam) > 0x1p-60f ? 1.f / (sign * fabsf(lam) * small) : 0.f;
+  float known0 = 0.f, known1 = 0.f;
+  for (;;) {
+    while (live.word) {
+      step(std::integral_constant<int, 0>{});
+      if (live.word) step(std::integral_constant<int, 1>{});
+    }
+    off0 = known0 + (off0 + other_half(off0)) * to_off0;
+    off1 = known1 + (off1 + other_half(off1)) * to_off1;
+    if (!kTwice || !sums_only) break;
+    sums_only = false;
+    known0 = off0, known1 = off1;
+    de0 += known0, de1 -= sign * known1;
+    off0 = off1 = 0.f;
+    __syncthreads();  // the tiles have been read
+    live = Live(a, b, start, end, lane);
+    if (live.word) fetch(live.key, 0, live.word);
   }
-  off0 += other_half(off0);
-  off1 += other_half(off1);
   if (r >= rows) return;
   if (DT != DA_F32 && half == 0) {
     float* to = a.off + (int64_t)split * a.batch * a.Hk * 2 * rows + base;
-    to[0] = off0 / small;
-    // A factor so small that its map's entries vanish tells nothing.
-    to[rows] = fabsf(lam) > 0x1p-60f ? off1 / (sign * fabsf(lam) * small) : 0.f;
+    to[0] = off0;
+    to[rows] = off1;
   }
   const float by = a.scale / small;
   const int64_t to = ((int64_t)b * a.T + t) * (a.Hk * a.G) + h;
@@ -764,9 +783,11 @@ int da_diff_attention_grad(const da_diff_inputs* in, const void* g, int64_t g_bs
     constexpr int DT = decltype(dt)::value, DP = decltype(dp)::value, DVP = decltype(dvp)::value;
     if (rows) {
       constexpr int kBytes = RowSmem<DT, DP, DVP>::kBytes;
-      if (const int err = allow_lds((const void*)diff_grad_rows<DT, DP, DVP>, kBytes)) return err;
+      const auto kernel = DT != DA_F32 && k_len < 2 * kLeastSplit ? diff_grad_rows<DT, DP, DVP, DT != DA_F32>
+                                                                  : diff_grad_rows<DT, DP, DVP, false>;
+      if (const int err = allow_lds((const void*)kernel, kBytes)) return err;
       a.blocks = p.rows.blocks, a.splits = p.rows.splits, a.each = p.rows.each;
-      diff_grad_rows<DT, DP, DVP><<<(unsigned)(pairs * a.blocks * a.splits), kThreads, kBytes, st>>>(a);
+      kernel<<<(unsigned)(pairs * a.blocks * a.splits), kThreads, kBytes, st>>>(a);
       const int64_t n = batch * q_len * heads * 2 * d;
       if (a.splits > 1)
         if (const int err = join<DT>(a.part, a.splits, n, dq, n, nullptr, st)) return err;
