@@ -2,7 +2,8 @@
 //
 // Head h has two query maps and its key head two key maps:
 //
-//   out = o_1 - lam_h o_2,   o_m = softmax(scale q_m k_m^T) v     (zero for a row without keys)
+//   out = o_1 - lam_h o_2,   o_m = softmax(scale q_m k_m^T) v     (zero for a row without keys,
+//                                                               NaN for one with NaN or infinite scores)
 //
 // One pass over the keys, a wave to a map and to 32 rows, with their running maxima and
 // sums.  It forms the transposed scores, k q^T, so that a row is a lane's (two lanes', 16
@@ -30,6 +31,15 @@ namespace {
 constexpr int kLeastSplit = 128;
 constexpr int kFewKeys = 512;
 constexpr float kMostSum = 1024.f;  // of sixteen exponentials, before a new maximum
+
+// A row that sees keys has a sum of about 1 and more (its maximum's exponential), one that sees
+// none 0.  A split whose live scores are all -inf sums to kOnlyInf: that counts for nothing beside
+// another split's sum, and where it is all there is the row is NaN, as the softmax is.
+constexpr float kOnlyInf = 0x1p-100f;
+__device__ __forceinline__ float settled(float sum) { return sum > 0.f && sum < 0.5f ? __builtin_nanf("") : sum; }
+// Of a settled sum, NaN of NaN.  A row that sees no key is marked by +inf.
+__device__ __forceinline__ float inverse(float sum) { return sum == 0.f ? 0.f : 1.f / sum; }
+__device__ __forceinline__ float lse_of(float top, float sum) { return sum == 0.f ? __builtin_inff() : top + log2f(sum); }
 
 // NG tiles of rows, each with a wave for either map.
 template <int DT, int DP, int DVP, int NG>
@@ -101,6 +111,7 @@ __global__ __launch_bounds__(2 * NG * kWave, DT == DA_F32 && DVP == 256 ? 1 : 2)
   const float c = a.scale * kLog2e;
   f32x16 o[NB];
   float top = kLowest, sum = 0.f;
+  uint32_t saw = 0;  // whether the row has seen a key
 #pragma unroll
   for (int x = 0; x < NB; ++x) o[x] = zeros();
   const Reader<DT, DP> key_reader(lds + map * L::kK, lane);
@@ -121,8 +132,11 @@ __global__ __launch_bounds__(2 * NG * kWave, DT == DA_F32 && DVP == 256 ? 1 : 2)
     for (int kk = 0; kk < KD; ++kk) Mfma32<DT>::mma(s, key_reader.rows(stage * L::kStage, kk), q[kk]);
     if (word != ~0u || key + kTile - 1 > least) {
       const uint32_t seen = seen_of(word, key, last, half);
+      saw |= seen;
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[i] = seen & 1u << acc_at(i, 0) ? s[i] : -__builtin_inff();
+    } else {
+      saw = 1;
     }
     f32x16 e;
 #pragma unroll
@@ -162,6 +176,8 @@ __global__ __launch_bounds__(2 * NG * kWave, DT == DA_F32 && DVP == 256 ? 1 : 2)
   }
 
   sum += other_half(sum);
+  saw |= __float_as_uint(other_half(__uint_as_float(saw)));
+  if (sum == 0.f && saw) sum = kOnlyInf;
   if (a.splits > 1) {  // this split's sums
     if (r >= rows) return;
     float* to = a.part + ((((int64_t)split * a.batch + b) * a.Hk + hk) * rows + r) * 2 * (DVP + 2);
@@ -175,10 +191,11 @@ __global__ __launch_bounds__(2 * NG * kWave, DT == DA_F32 && DVP == 256 ? 1 : 2)
   }
   f32x4* handed = (f32x4*)(lds + group * (L::kHanded / NG));
   const bool in = r < rows;
-  const float by = sum > 0.f ? 1.f / sum : 0.f;
+  sum = settled(sum);
+  const float by = inverse(sum);
   const int64_t to = (((int64_t)b * a.T + t) * (a.Hk * a.G) + h) * a.Dv * ES;
   if (a.lse && half == 0 && in)
-    a.lse[(((int64_t)b * a.Hk + hk) * 2 + map) * rows + r] = sum > 0.f ? top + log2f(sum) : __builtin_inff();
+    a.lse[(((int64_t)b * a.Hk + hk) * 2 + map) * rows + r] = lse_of(top, sum);
   __syncthreads();  // the tiles have been read
   if (map) {
     const float lam = in && by != 0.f ? lam_of(a, h) : 0.f;
@@ -230,7 +247,8 @@ __global__ __launch_bounds__(256) void diff_join(Args a) {
   }
   const int r = (int)(at % rows), hk = (int)(at / rows % a.Hk), b = (int)(at / rows / a.Hk);
   const int t = r / a.G, h = hk * a.G + (r - t * a.G);
-  const float by0 = sum[0] > 0.f ? 1.f / sum[0] : 0.f, by1 = sum[1] > 0.f ? 1.f / sum[1] : 0.f;
+  sum[0] = settled(sum[0]), sum[1] = settled(sum[1]);
+  const float by0 = inverse(sum[0]), by1 = inverse(sum[1]);
   const float by2 = by1 != 0.f ? lam_of(a, h) * by1 : 0.f;
   const int64_t to = ((int64_t)b * a.T + t) * (a.Hk * a.G) + h;
   const f32x4 f = o[0] * by0 - o[1] * by2, g = o[1] * by1;
@@ -238,8 +256,8 @@ __global__ __launch_bounds__(256) void diff_join(Args a) {
   if (a.second) store4<DT>(a.second + to * a.Dv * ES, 4 * l, a.Dv, g[0], g[1], g[2], g[3]);
   if (a.lse && l == 0) {
     float* lse = a.lse + ((int64_t)b * a.Hk + hk) * 2 * rows + r;
-    lse[0] = sum[0] > 0.f ? top[0] + log2f(sum[0]) : __builtin_inff();
-    lse[rows] = sum[1] > 0.f ? top[1] + log2f(sum[1]) : __builtin_inff();
+    lse[0] = lse_of(top[0], sum[0]);
+    lse[rows] = lse_of(top[1], sum[1]);
   }
 }
 

@@ -208,7 +208,8 @@ def diff_attention(q, k, v, lam, *, scale: float | None = None, causal: bool = F
     T`` (the queries are the last positions; one new token against a cache is
     ``T = 1``).  ``mask`` (B, S): a zero hides the key from every query;
     ``q_mask`` (B, T): a zero takes the query out.  Both may hold anything there.
-    A query that sees no key has a zero row and no gradient.
+    A query that sees no key has a zero row and no gradient; one with a NaN or
+    infinite score has NaN in its row, and in the gradients of what it sees.
 
     ``return_state``: ``(out, state)`` for :func:`diff_attention_grad`; not
     differentiable.  ``slot`` takes ``lam``'s per-sample gradient ``(B, H)`` in the

@@ -878,7 +878,8 @@ int da_add_rms_norm_grad(const void* g, const void* g_total, const void* total, 
  * lam (heads) at lam_stride (0 broadcasts).  causal: query i sees the keys up to
  * i + q_start.  mask (batch, k_len) and q_mask (batch, q_len): bytes, 0 marks a key
  * that no query sees, a query that takes no part, whatever they hold; NULL: none.  A
- * query that sees no key has zero rows.  out (batch, q_len, heads, dv), contiguous.
+ * query that sees no key has zero rows, one with a NaN or infinite score NaN, in the
+ * gradients too.  out (batch, q_len, heads, dv), contiguous.
  * d <= 128, dv <= 256, rows whole 16-byte runs at 16-byte aligned addresses (zeros
  * that pad a row change nothing), tokens within 2 GB of each other in a tile of 32.
  *

@@ -1,0 +1,119 @@
+"""Difference attention where it can go wrong: scores that are not finite or very large, fp16
+samples and maps of very different sizes, rows that see few keys, and every CU busy
+(``csrc/diffattn.hip``, ``csrc/diffattn_grad.hip``)."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from conftest import stable_seed
+from dattri_llm_amd.gradient import ops
+
+pytestmark = pytest.mark.gpu
+
+DT = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
+U32 = 2.0**-24
+NAMES = ("out", "dq", "dk", "dv", "dlam")
+
+
+def run(q, k, v, lam, g, **kw):
+    out, state = ops.diff_attention(q, k, v, lam, return_state=True, **kw)
+    return out, *ops.diff_attention_grad(g, q, k, v, lam, out, state, **kw)
+
+
+def exact(q, k, v, lam, g, *, scale=None, seen=None):
+    """The formulas in 64 bits, gradients by automatic differentiation; ``seen`` (b, t, s)."""
+    b, t, h2, d = q.shape
+    s, hk, dv = v.shape[1:]
+    h = h2 // 2
+    lam = lam.double().expand(h) if lam.numel() == 1 else lam.double()
+    q, k, v = (x.double().contiguous().requires_grad_() for x in (q, k, v))
+    lams = lam.expand(b, h).clone().requires_grad_()
+    qs = q.view(b, t, h, 2, d).permute(0, 2, 3, 1, 4).contiguous()
+    ks = k.view(b, s, hk, 2, d).repeat_interleave(h // hk, 2).permute(0, 2, 3, 4, 1).contiguous()
+    x = torch.matmul(qs, ks) * (d ** -0.5 if scale is None else scale)
+    if seen is not None:
+        x = x.masked_fill(~seen[:, None, None], -torch.inf)
+    p = x.softmax(-1)
+    o = torch.matmul(p, v.repeat_interleave(h // hk, 2).transpose(1, 2)[:, :, None].contiguous())
+    out = (o[:, :, 0] - lams[:, :, None, None] * o[:, :, 1]).transpose(1, 2)
+    (out * g.double()).sum().backward()
+    return tuple(y.detach() for y in (out, q.grad, k.grad, v.grad, lams.grad)), p.detach()
+
+
+def normal(gen, *shape, dt=torch.float32, size=1.0):
+    return (size * torch.randn(*shape, generator=gen, device="cuda")).to(dt)
+
+
+def operands(seed, b, t, s, h, hk, d, dv, dt):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    return (normal(gen, b, t, 2 * h, d, dt=dt), normal(gen, b, s, 2 * hk, d, dt=dt), normal(gen, b, s, hk, dv, dt=dt),
+            0.2 + 0.6 * torch.rand(h, generator=gen, device="cuda"), normal(gen, b, t, h, dv, dt=dt, size=0.1))
+
+
+# ---------------------------------------------------------------------------
+# Scores that are not finite
+# ---------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dt,where", [(dt, w) for dt in DT for w in ("q0", "q1", "k0", "k1", "v", "g")
+                                      if dt != "fp16" or w[0] in "qk"])
+@pytest.mark.parametrize("t,s", [(40, 70), (300, 600), (1, 3000)])  # whole, and keys in splits
+@pytest.mark.parametrize("what", [float("nan"), float("inf")])
+def test_what_is_not_finite_reaches_the_gradients(dt, t, s, where, what):
+    """Wherever automatic differentiation of the formula gives NaN there is NaN; the other
+    sample's results do not change by a bit."""
+    q, k, v, lam, g = operands(stable_seed((t, s)), 2, t, s, 4, 2, 32, 48, DT[dt])
+    clean = run(q, k, v, lam, g)
+    if where[0] == "q":
+        q[0, t // 2, 2 + int(where[1]), 5] = what  # head 1
+    elif where[0] == "k":
+        k[0, s // 3, 2 + int(where[1]), 5] = what  # key head 1
+    elif where == "v":
+        v[0, s // 3, 1, 5] = what
+    else:
+        g[0, t // 2, 1, 5] = what
+    got = run(q, k, v, lam, g)
+    want, _ = exact(q, k, v, lam, g)
+    # An infinite g: delta is g . out, +inf or -inf, where automatic differentiation sums p dp of
+    # both signs to NaN; dp - delta, +inf or -inf too, then is NaN for equal signs and infinite for
+    # others.  Everything else has no other order.
+    lost = torch.isnan if (where, what) != ("g", float("inf")) else (lambda x: ~x.isfinite())
+    for name, x, y, z in zip(NAMES, got, want, clean):
+        assert bool(lost(x[y.isnan()]).all()), name
+        assert torch.equal(x[1], z[1]), name
+    assert torch.equal(got[0].isnan(), want[0].isnan())
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("s", [1, 33, 3000])
+def test_rows_whose_scores_are_all_infinite(dt, sign, s):
+    """An overflowed query: scores of +inf alone and of -inf alone give NaN, no zeros; a query
+    that takes no part and a sample whose keys do not stay zero."""
+    q, k, v, lam, g = operands(s, 3, 2, s, 2, 1, 32, 32, DT[dt])
+    k[..., 3] = sign * (1 + k[..., 3].abs())
+    q[:, 0, :, 3] = float("inf")
+    mask = torch.ones(3, s, dtype=torch.bool, device="cuda")
+    q_mask = torch.ones(3, 2, dtype=torch.bool, device="cuda")
+    mask[1], q_mask[2, 0] = False, False
+    out, dq, dk, dv, dlam = run(q, k, v, lam, g, mask=mask, q_mask=q_mask)
+    assert bool(out[0, 0].isnan().all()) and bool(out[:, 1].isfinite().all())
+    assert bool(dq[0, 0].isnan().all()) and bool(dk[0].isnan().any()) and bool(dv[0].isnan().all())
+    assert bool(dlam[0].isnan().all())
+    for x in (out, dq, dk, dv, dlam):
+        assert bool((x[1] == 0).all()) and bool(x[2].isfinite().all())
+    assert bool((out[2, 0] == 0).all()) and bool((dq[2, 0] == 0).all())
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+def test_an_infinite_first_score_of_a_causal_row(dt):
+    """Row 0 sees one key, whose score is -inf; the rows behind it are finite."""
+    q, k, v, lam, g = operands(3, 1, 50, 50, 2, 1, 32, 32, DT[dt])
+    k[0, 0, :, 7] = -1.0
+    q[0, 0, :, 7] = float("inf")
+    out, dq, dk, dv, _ = run(q, k, v, lam, g, causal=True)
+    assert bool(out[0, 0].isnan().all()) and bool(out[0, 1:].isfinite().all())
+    assert bool(dq[0, 0].isnan().all()) and bool(dq[0, 1:].isfinite().all())
+    assert bool(dk[0, 0].isnan().any()) and bool(dv[0, 0].isnan().all())
