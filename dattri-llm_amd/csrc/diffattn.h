@@ -32,7 +32,9 @@ struct Args {
   int g_shift;
   char* out;      // (batch, T, Hk G, Dv)
   char* second;   // like out: the second map's values, for the backward pass; NULL: none
-  float* lse;     // (batch, Hk, 2, T G): log2 of the exponentials' sums; +inf for a row that sees nothing
+  // (2, batch, Hk, 2, T G): log2 of the sums of 2^((score - top) c), +inf for a row that sees
+  // nothing; then top, the largest scores (as products of q and k, not scaled).
+  float* lse;
   int blocks;     // workgroups of one (batch, key head), apart from splits
   int splits, each;  // the other side's entries of a split (a whole number of tiles)
   float* part;    // sums of each split, joined by a second launch
@@ -42,7 +44,7 @@ struct Args {
   float* delta;   // (batch, Hk, 2, T G): g . o_m
   int row_splits;
   char* records;  // (batch, Hk, T G): lse and delta of both maps as diff_grad_keys reads them
-  uint8_t* takes_part;  // (batch, Hk, T G): whether the row sees a key
+  uint8_t* takes_part;  // (batch, Hk, T G): 1 where the row sees a key, 3 where its scores are large besides
   float* off;     // 16 bits: (row splits, batch, Hk, 2, T G): how far delta was off, in parts
   float* most;    // fp16: largest norms of g's rows and of v's, squared
   char *dq, *dk, *dv;
@@ -75,6 +77,10 @@ __device__ __forceinline__ void deal(int n, int blocks, int* group, int* block) 
 __device__ __forceinline__ int token_of(const Args& a, int r) {
   return (int)((uint64_t)(uint32_t)r * a.g_factor >> a.g_shift);
 }
+
+// Largest scores `top` and the rest apart, as a difference of large numbers is formed before it is
+// rounded: of maps that are one key, or a few with equal scores, nothing else would be left.
+__device__ __forceinline__ int64_t tops_at(const Args& a) { return (int64_t)a.batch * a.Hk * 2 * a.T * a.G; }
 
 __device__ __forceinline__ float lam_of(const Args& a, int h) {
   const int64_t at = h * a.lam_stride;

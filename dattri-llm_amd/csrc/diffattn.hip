@@ -9,7 +9,8 @@
 // sums.  It forms the transposed scores, k q^T, so that a row is a lane's (two lanes', 16
 // keys each) and its maximum and sum stay within them; the accumulator's registers then are,
 // rounded, the second operand of o^T = v^T p^T as they stand, where v is read transposed out
-// of LDS.  Exponentials are relative to a maximum that is looked for again only when the sum
+// of LDS.  A difference of scores is formed before it is scaled where they are large (kNear), so
+// that any finite scores have finite exponentials.  These are relative to a maximum that is looked for again only when the sum
 // of a lane's sixteen passes 2^10: until then they are at most that much larger than with the
 // last one (the first tile has none, and passes; with a new one in every tile that has a larger
 // score 277 us in place of 257 at the first size below).  At the end the second map's waves hand
@@ -37,9 +38,22 @@ constexpr float kMostSum = 1024.f;  // of sixteen exponentials, before a new max
 // another split's sum, and where it is all there is the row is NaN, as the softmax is.
 constexpr float kOnlyInf = 0x1p-100f;
 __device__ __forceinline__ float settled(float sum) { return sum > 0.f && sum < 0.5f ? __builtin_nanf("") : sum; }
-// Of a settled sum, NaN of NaN.  A row that sees no key is marked by +inf.
+// Of a settled sum, NaN of NaN.
 __device__ __forceinline__ float inverse(float sum) { return sum == 0.f ? 0.f : 1.f / sum; }
-__device__ __forceinline__ float lse_of(float top, float sum) { return sum == 0.f ? __builtin_inff() : top + log2f(sum); }
+
+// The exponentials are 2^((s - top) c + shift).  shift is what rounding top c leaves of it, so that
+// one fma, s c - round(top c), gives them; where that could be large (it is half a unit of top c's
+// last place), 0, and the difference is formed first.
+constexpr float kNear = 0x1p20f;
+__device__ __forceinline__ bool near(float top, float c) { return fabsf(top * c) < kNear; }
+__device__ __forceinline__ float shift_of(float top, float c) { return near(top, c) ? fmaf(top, c, -(top * c)) : 0.f; }
+
+// What the backward pass needs of a row: the settled sum of 2^((s - top) c), +inf where it sees no
+// key, and top.
+__device__ __forceinline__ void put_lse(const Args& a, int64_t at, float top, float shift, float sum) {
+  a.lse[at] = sum == 0.f ? __builtin_inff() : log2f(sum) - shift;
+  a.lse[tops_at(a) + at] = sum == 0.f ? 0.f : top;
+}
 
 // NG tiles of rows, each with a wave for either map.
 template <int DT, int DP, int DVP, int NG>
@@ -110,7 +124,9 @@ __global__ __launch_bounds__(2 * NG * kWave, DT == DA_F32 && DVP == 256 ? 1 : 2)
 
   const float c = a.scale * kLog2e;
   f32x16 o[NB];
-  float top = kLowest, sum = 0.f;
+  // A lane without a row sees nothing, and does not make the others' scores large.
+  float top = last >= 0 ? kLowest : 0.f, shift = 0.f, sum = 0.f;
+  bool far = true;  // whether a score of the wave is large
   uint32_t saw = 0;  // whether the row has seen a key
 #pragma unroll
   for (int x = 0; x < NB; ++x) o[x] = zeros();
@@ -139,22 +155,31 @@ __global__ __launch_bounds__(2 * NG * kWave, DT == DA_F32 && DVP == 256 ? 1 : 2)
       saw = 1;
     }
     f32x16 e;
+    const auto exponentials = [&]() __attribute__((always_inline)) {
+      if (far) {  // the same in all lanes
 #pragma unroll
-    for (int i = 0; i < 16; ++i) e[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c, -top));
-    float part = over_acc(e, [](float u, float v) { return u + v; });
+        for (int i = 0; i < 16; ++i) e[i] = __builtin_amdgcn_exp2f(fmaf(s[i] - top, c, shift));
+      } else {
+        const float tc = top * c;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) e[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c, -tc));
+      }
+      return over_acc(e, [](float u, float v) { return u + v; });
+    };
+    float part = exponentials();
     if (__any(part > kMostSum)) {
       float x = over_acc(s, [](float u, float v) { return fmaxf(u, v); });
-      x = fmaxf(x, other_half(x)) * c;
-      const float now = fmaxf(top, x), by = __builtin_amdgcn_exp2f(top - now);
-      top = now;
+      x = fmaxf(x, other_half(x));
+      const float now = fmaxf(top, x), shift_now = shift_of(now, c);
+      const float by = __builtin_amdgcn_exp2f(fmaf(top - now, c, shift_now - shift));
+      top = now, shift = shift_now;
+      far = __any(!near(top, c));
       sum *= by;
 #pragma unroll
       for (int y = 0; y < NB; ++y)
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[y][i] *= by;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) e[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c, -top));
-      part = over_acc(e, [](float u, float v) { return u + v; });
+      part = exponentials();
     }
     sum += part;
 #pragma unroll
@@ -194,8 +219,7 @@ __global__ __launch_bounds__(2 * NG * kWave, DT == DA_F32 && DVP == 256 ? 1 : 2)
   sum = settled(sum);
   const float by = inverse(sum);
   const int64_t to = (((int64_t)b * a.T + t) * (a.Hk * a.G) + h) * a.Dv * ES;
-  if (a.lse && half == 0 && in)
-    a.lse[(((int64_t)b * a.Hk + hk) * 2 + map) * rows + r] = lse_of(top, sum);
+  if (a.lse && half == 0 && in) put_lse(a, (((int64_t)b * a.Hk + hk) * 2 + map) * rows + r, top, shift, sum);
   __syncthreads();  // the tiles have been read
   if (map) {
     const float lam = in && by != 0.f ? lam_of(a, h) : 0.f;
@@ -231,6 +255,7 @@ __global__ __launch_bounds__(256) void diff_join(Args a) {
   if (at >= all) return;
   f32x4 o[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}};
   float top[2] = {kLowest, kLowest}, sum[2] = {0.f, 0.f};
+  const float c = a.scale * kLog2e;
 #pragma unroll 4
   for (int p = 0; p < a.splits; ++p) {
     const float* from = a.part + (p * all + at) * 2 * (DVP + 2);
@@ -239,7 +264,8 @@ __global__ __launch_bounds__(256) void diff_join(Args a) {
       const float top2 = from[2 * DVP + 2 * m], sum2 = from[2 * DVP + 2 * m + 1];
       const f32x4 x = *(const f32x4*)(from + m * DVP + 4 * l);
       const float now = fmaxf(top[m], top2);
-      const float f1 = __builtin_amdgcn_exp2f(top[m] - now), f2 = __builtin_amdgcn_exp2f(top2 - now);
+      const float f1 = __builtin_amdgcn_exp2f((top[m] - now) * c);
+      const float f2 = __builtin_amdgcn_exp2f(fmaf(top2 - now, c, -shift_of(top2, c)));
       top[m] = now;
       sum[m] = sum[m] * f1 + sum2 * f2;
       o[m] = o[m] * f1 + x * f2;
@@ -255,9 +281,9 @@ __global__ __launch_bounds__(256) void diff_join(Args a) {
   store4<DT>(a.out + to * a.Dv * ES, 4 * l, a.Dv, f[0], f[1], f[2], f[3]);
   if (a.second) store4<DT>(a.second + to * a.Dv * ES, 4 * l, a.Dv, g[0], g[1], g[2], g[3]);
   if (a.lse && l == 0) {
-    float* lse = a.lse + ((int64_t)b * a.Hk + hk) * 2 * rows + r;
-    lse[0] = lse_of(top[0], sum[0]);
-    lse[rows] = lse_of(top[1], sum[1]);
+    const int64_t to = ((int64_t)b * a.Hk + hk) * 2 * rows + r;
+    put_lse(a, to, top[0], 0.f, sum[0]);
+    put_lse(a, to + rows, top[1], 0.f, sum[1]);
   }
 }
 
@@ -298,7 +324,7 @@ int check_side(const char* what, const char* name, const void* x, int es, int64_
 int fill_args(Args& a, const char* what, int dtype, const da_diff_inputs* in, int64_t batch, int64_t T, int64_t S, int64_t heads,
               int64_t k_heads, int64_t D, int64_t Dv, float scale, int causal, int64_t q_start) {
   if (!valid_dtype((int)in->lam_dtype)) return set_error(DA_ERR_INVALID, "%s: bad dtype %d", what, (int)in->lam_dtype);
-  if (!(scale >= 1e-20f) || !(scale <= 1e20f))  // times or over a finite score, and 1e30 times it, stay in range
+  if (!(scale >= 1e-20f) || !(scale <= 1e20f))  // a logarithm over it stays in range, and 1e30 times it is large
     return set_error(DA_ERR_INVALID, "%s: the scale must lie between 1e-20 and 1e20", what);
   const int es = (int)elem_bytes(dtype);
   const int64_t group = heads / k_heads;

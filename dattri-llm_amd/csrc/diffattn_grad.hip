@@ -1,6 +1,6 @@
 // Attention by the difference of two softmax maps, backward.
 //
-// With p_m the maps (from the scores and the forward call's lse), g the gradient of out:
+// With p_m the maps (from the scores, and the forward call's largest ones and sums), g the gradient of out:
 //
 //   dp = g v^T,   delta_m = g . o_m
 //   ds_1 = p_1 (dp - delta_1),   ds_2 = -lam p_2 (dp - delta_2)
@@ -45,19 +45,27 @@ namespace {
 //
 // Where keys are columns, a row's lse and delta are needed in every lane, by register.  In
 // 16 bits they come with the products instead: one more step of contraction over their parts
-// (three bf16 values hold 24 bits) against ones makes the scores' accumulators z - lse / c and
-// g v^T - delta, from two reads of LDS in place of sixteen.  A record then is the parts of
-// [-lse_1 / c | -delta_1 | -lse_2' / c | delta_1 - delta_2], eight entries each; else it is the
-// four values in fp32.  lse_2' = lse_2 - log2 |lam|: the factor comes with the exponential.
-// A row without keys has an exponential of nothing, by a finite number: no product is NaN.
+// (three bf16 values hold 24 bits) against ones makes the scores' accumulators z - top - lse / c
+// and g v^T - delta, from two reads of LDS in place of sixteen.  A record then is the parts of
+// [-top_1, -lse_1 / c | -delta_1 | -top_2, -lse_2' / c | delta_1 - delta_2], eight entries each;
+// else it is the six values in fp32.  lse_2' = lse_2 - log2 |lam|: the factor comes with the
+// exponential.  A tile with large scores takes top and lse in two steps: the sum of both would
+// be rounded to top's last place.  A row without keys has an exponential of nothing, by a finite
+// number: no product is NaN.
 // ---------------------------------------------------------------------------
 constexpr int kLanes = 16;
 constexpr float kNothing = -1e30f;
+// In 16 bits lse + top c as one number is off by less than 2^-14 up to here, no more than a tenth
+// of a step of the maps.
+constexpr float kNear = 1024.f;
+__device__ __forceinline__ bool near(float top0, float top1, float c) {
+  return fabsf(top0 * c) < kNear && fabsf(top1 * c) < kNear;
+}
 
 template <int DT>
 struct Record {
   static constexpr bool kParts = DT != DA_F32;
-  static constexpr int kBytes = kParts ? 64 : 16;
+  static constexpr int kBytes = kParts ? 64 : 32;
 };
 
 __device__ __forceinline__ u32x4 three_parts(float x) {
@@ -67,16 +75,23 @@ __device__ __forceinline__ u32x4 three_parts(float x) {
   const uint32_t lo = f32_to_bf16_bits(r1 - bf16_bits_to_f32(mid));
   return u32x4{hi | mid << 16, lo, 0, 0};
 }
+__device__ __forceinline__ u32x4 six_parts(float x, float y) {
+  const u32x4 u = three_parts(x), v = three_parts(y);
+  return u32x4{u[0], u[1] | v[0] << 16, v[0] >> 16 | v[1] << 16, 0};
+}
 
 template <int DT>
-__device__ __forceinline__ void put_record(char* to, float c, float lse0, float lse1, float de0, float de1) {
+__device__ __forceinline__ void put_record(char* to, float c, float top0, float top1, float lse0, float lse1, float de0,
+                                           float de1) {
   if constexpr (Record<DT>::kParts) {
-    st16(to, three_parts(lse0 == __builtin_inff() ? kNothing : -lse0 / c));
+    const bool some0 = lse0 != __builtin_inff(), some1 = lse1 != __builtin_inff();
+    st16(to, six_parts(some0 ? -top0 : kNothing, some0 ? -lse0 / c : 0.f));
     st16(to + 16, three_parts(-de0));
-    st16(to + 32, three_parts(lse1 == __builtin_inff() ? kNothing : -lse1 / c));
+    st16(to + 32, six_parts(some1 ? -top1 : kNothing, some1 ? -lse1 / c : 0.f));
     st16(to + 48, three_parts(de0 - de1));
   } else {
-    *(f32x4*)to = f32x4{lse0, lse1, de0, de1};
+    *(f32x4*)to = f32x4{top0, top1, lse0, lse1};
+    *(f32x4*)(to + 16) = f32x4{de0, de1, 0.f, 0.f};
   }
 }
 
@@ -87,7 +102,8 @@ __global__ __launch_bounds__(256) void diff_delta(Args a) {
   const int chunk = blockIdx.x % a.chunks;
   const int h = blockIdx.x / a.chunks % heads, b = blockIdx.x / a.chunks / heads;
   const int hk = h / a.G, rows = a.T * a.G;
-  const float lam = lam_of(a, h);
+  const float lam = lam_of(a, h), c = a.scale * kLog2e;
+  const float* tops = a.lse + tops_at(a);
   const int t1 = min((chunk + 1) * a.chunk, a.T);
   float most = 0.f;
   for (int t = chunk * a.chunk + sub; t < t1; t += kRows) {
@@ -119,7 +135,8 @@ __global__ __launch_bounds__(256) void diff_delta(Args a) {
       float* to = a.delta + of * 2 * rows + r;
       to[0] = d0 + lam * d1;  // o_1 = out + lam o_2
       to[rows] = d1;
-      a.takes_part[of * rows + r] = live;
+      const int64_t at = of * 2 * rows + r;
+      a.takes_part[of * rows + r] = live ? near(tops[at], tops[at + rows], c) ? 1 : 3 : 0;
     }
   }
   if constexpr (DT == DA_F16) {  // a maximum: the order does not matter
@@ -169,7 +186,9 @@ __global__ __launch_bounds__(256) void diff_records(Args a) {
     float d0 = a.delta[at], d1 = a.delta[at + rows];
     if constexpr (DT != DA_F32)
       for (int p = 0; p < a.row_splits; ++p) d0 += a.off[p * all + at], d1 += a.off[p * all + at + rows];
-    put_record<DT>(a.records + (of * rows + r) * Record<DT>::kBytes, c, a.lse[at], a.lse[at + rows] - bits, d0, d1);
+    const float* tops = a.lse + tops_at(a) + at;
+    put_record<DT>(a.records + (of * rows + r) * Record<DT>::kBytes, c, tops[0], tops[rows], a.lse[at],
+                   a.lse[at + rows] - bits, d0, d1);
     sum += d1;
   }
   sum = lanes_sum<kWave>(sum);
@@ -331,8 +350,11 @@ __global__ __launch_bounds__(kThreads, DT != DA_F32 && DP == 64 ? 2 : 1) void di
     }
   };
   int byte = 0;
+  bool far_next = false;  // whether the tile under way has large scores
   if (first < end) {
-    fetch(first, 0, key_word(row_byte(first)));
+    byte = row_byte(first);
+    far_next = __any(byte & 2);
+    fetch(first, 0, key_word(byte));
     byte = row_byte(first + kTile);
   }
   const Reader<DT, DP> q_reader(lds, lane);
@@ -343,7 +365,9 @@ __global__ __launch_bounds__(kThreads, DT != DA_F32 && DP == 64 ? 2 : 1) void di
     constexpr int stage = decltype(of)::value;
     constexpr int skip = stage * L::kStage;
     tiles_barrier();
+    const bool far = far_next;
     if (r0 + kTile < end) {
+      far_next = __any(byte & 2);
       fetch(r0 + kTile, stage ^ 1, key_word(byte));
       byte = row_byte(r0 + 2 * kTile);
     }
@@ -366,7 +390,14 @@ __global__ __launch_bounds__(kThreads, DT != DA_F32 && DP == 64 ? 2 : 1) void di
       const u32x4 r1 = lr.rows(skip, 0), r2 = lr.rows(skip, 1);
       uint32_t low = in_low;
       asm("" : "+v"(low) : "s"(r0));  // two instructions a tile instead of eight registers
-      const u32x4 of_low = {kOnes & low, kOne & low, 0, 0}, of_high = {kOnes & ~low, kOne & ~low, 0, 0};
+      u32x4 of_low = {kOnes & low, kOnes & low, kOnes & low, 0};
+      const u32x4 of_high = {kOnes & ~low, kOne & ~low, 0, 0};
+      if (far) {
+        const u32x4 of_top = {kOnes & low, kOne & low, 0, 0};
+        Mfma32<DA_BF16>::mma(s0, r1, of_top);
+        Mfma32<DA_BF16>::mma(s1, r2, of_top);
+        of_low[0] = 0, of_low[1] = kOne << 16 & low;
+      }
       Mfma32<DA_BF16>::mma(s0, r1, of_low);
       Mfma32<DA_BF16>::mma(s1, r2, of_low);
       Mfma32<DA_BF16>::mma(dp, r1, of_high);
@@ -376,11 +407,12 @@ __global__ __launch_bounds__(kThreads, DT != DA_F32 && DP == 64 ? 2 : 1) void di
       dp1 = dp;
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const f32x4 x = *(const f32x4*)(lds + skip + 2 * L::kQ + L::kG + acc_at(i, half) * 16);
-        s0[i] = fmaf(s0[i], c, -x[0]);
-        s1[i] = fmaf(s1[i], c, -x[1]);
-        dp[i] -= x[2];
-        dp1[i] -= x[3];
+        const f32x4* record = (const f32x4*)(lds + skip + 2 * L::kQ + L::kG + acc_at(i, half) * Rec::kBytes);
+        const f32x4 x = record[0], y = record[1];
+        s0[i] = fmaf(s0[i] - x[0], c, -x[2]);
+        s1[i] = fmaf(s1[i] - x[1], c, -x[3]);
+        dp[i] -= y[0];
+        dp1[i] -= y[1];
       }
     }
 #pragma unroll
@@ -523,8 +555,13 @@ __global__ __launch_bounds__(kThreads, DT != DA_F32 && DP == 64 ? 2 : 1) void di
   // The second map's factor comes with its exponential, the sign with its values' gradient.
   const float lam = in ? lam_of(a, h) : 0.f, sign = lam < 0.f ? 1.f : -1.f;
   const float lse1 = in ? a.lse[base + rows] - log2f(fabsf(lam)) : __builtin_inff();
+  const int64_t tops = tops_at(a) + base;
+  const float top0 = in ? a.lse[tops] : 0.f, top1 = in ? a.lse[tops + rows] : 0.f;
   float de0 = in ? a.delta[base] : 0.f, de1 = in ? -sign * a.delta[base + rows] : 0.f;
   const float c = a.scale * kLog2e, small = small_scale<DT>(a);
+  // Large scores: the difference from the largest first.
+  const bool far = DT == DA_F32 || __any(!near(top0, top1, c));
+  const float whole0 = fmaf(top0, c, lse0), whole1 = fmaf(top1, c, lse1);
 
   const Keys<DT, DP, kThreads> keys(a.k_t, a.D);
   const Keys<DT, DVP, kThreads> values(a.v_t, a.Dv);
@@ -567,10 +604,17 @@ __global__ __launch_bounds__(kThreads, DT != DA_F32 && DP == 64 ? 2 : 1) void di
     for (int kk = 0; kk < KV; ++kk) Mfma32<DT>::mma(dp, lv.rows(skip, kk), g[kk]);
     const bool some = word != ~0u || key + kTile - 1 > least;
     const uint32_t seen = some ? seen_of(word, key, last, half) : ~0u;
+    if (far) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s0[i] = fmaf(s0[i] - top0, c, -lse0), s1[i] = fmaf(s1[i] - top1, c, -lse1);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s0[i] = fmaf(s0[i], c, -whole0), s1[i] = fmaf(s1[i], c, -whole1);
+    }
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      float p0 = __builtin_amdgcn_exp2f(fmaf(s0[i], c, -lse0));
-      float p1 = __builtin_amdgcn_exp2f(fmaf(s1[i], c, -lse1));
+      float p0 = __builtin_amdgcn_exp2f(s0[i]);
+      float p1 = __builtin_amdgcn_exp2f(s1[i]);
       if constexpr (DT == DA_F16) p0 *= small, p1 *= small;
       if (some) {
         p0 = seen & 1u << acc_at(i, 0) ? p0 : 0.f;

@@ -161,7 +161,8 @@ def relative_bias_grad(g, num_buckets: int, *, q_start: int = 0, bidirectional: 
 
 
 class DiffAttentionState(NamedTuple):
-    """What :func:`diff_attention_grad` needs of the forward call beside its output."""
+    """What :func:`diff_attention_grad` needs of the forward call beside its output: the
+    second map's values, and each row's log of its sum and largest score in either map."""
 
     second: torch.Tensor
     lse: torch.Tensor

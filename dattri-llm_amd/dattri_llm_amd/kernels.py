@@ -1950,7 +1950,7 @@ def diff_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lam: torch
     second = lse = None
     if state:
         second = torch.empty((b, t, h, wide), dtype=q.dtype, device=dev)
-        lse = torch.empty((b, hk, 2, t * (h // hk)), dtype=torch.float32, device=dev)
+        lse = torch.empty((2, b, hk, 2, t * (h // hk)), dtype=torch.float32, device=dev)
     nbytes = ctypes.c_size_t(0)
     with _on(dev):
         nat.check(lib.da_diff_attention_workspace(*sizes, ctypes.byref(nbytes)), "diff_attention")
@@ -1977,7 +1977,7 @@ def diff_attention_grad(g: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: to
     for name, x, w in (("g", g, dv), ("out", out, dv), ("second", second, pad_dv)):
         if x.shape != (b, t, h, w) or x.dtype != q.dtype:
             raise ValueError(f"{what}: {name} must be {(b, t, h, w)} {q.dtype}, got {tuple(x.shape)} {x.dtype}")
-    if lse.shape != (b, hk, 2, t * (h // hk)) or lse.dtype != torch.float32:
+    if lse.shape != (2, b, hk, 2, t * (h // hk)) or lse.dtype != torch.float32:
         raise ValueError(f"{what}: the state does not belong to these inputs")
     nat.same_device(q, g, out, second, lse)
     g, out, second, lse = _head_rows(g), prepare_rows(out.contiguous()), second.contiguous(), lse.contiguous()

@@ -883,8 +883,10 @@ int da_add_rms_norm_grad(const void* g, const void* g_total, const void* total, 
  * d <= 128, dv <= 256, rows whole 16-byte runs at 16-byte aligned addresses (zeros
  * that pad a row change nothing), tokens within 2 GB of each other in a tile of 32.
  *
- * second (like out: the second map's values) and lse (batch, 2 heads, q_len values)
- * are what da_diff_attention_grad needs of the forward call; both NULL: not wanted.
+ * second (like out: the second map's values) and lse (2, batch, 2 heads, q_len values:
+ * log2 of the sums of exponentials relative to a row's largest score, +inf for a row that
+ * sees no key, and these scores before scaling) are what da_diff_attention_grad needs of
+ * the forward call; both NULL: not wanted.
  * It writes dq, dk, dv (contiguous) and each sample's gradient of lam (batch, heads)
  * fp32 for the gradient g of out.  All sums run in a fixed order.
  */

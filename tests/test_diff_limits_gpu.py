@@ -117,3 +117,96 @@ def test_an_infinite_first_score_of_a_causal_row(dt):
     assert bool(out[0, 0].isnan().all()) and bool(out[0, 1:].isfinite().all())
     assert bool(dq[0, 0].isnan().all()) and bool(dq[0, 1:].isfinite().all())
     assert bool(dk[0, 0].isnan().any()) and bool(dv[0, 0].isnan().all())
+
+
+# ---------------------------------------------------------------------------
+# Large scores
+# ---------------------------------------------------------------------------
+
+
+def check_maps(q, k, v, lam, g, *, scale, rel, seen=None, grads=NAMES, **kw):
+    """A call whose scores fp32 holds exactly against 64 bits.  ``rel``: how far the maps may be
+    off relatively, for their exponentials' and sums' fp32 roundings; sums over n terms are off
+    by n 2^-24 of their absolute terms besides, 16-bit operands and outputs by half a step."""
+    dt = q.dtype
+    u = 0.0 if dt == torch.float32 else torch.finfo(dt).eps / 2
+    tiny = 2.0**-24 if dt == torch.float16 else 2.0**-126
+    b, t, h2, d = q.shape
+    s, hk, dv = v.shape[1:]
+    h, group = h2 // 2, h2 // 2 // hk
+    c = (s + t * group + d + dv + 64) * U32 + rel
+    want, p = exact(q, k, v, lam, g, scale=scale, seen=seen)
+    got = run(q, k, v, lam, g, scale=scale, **kw)
+    la = lam.double().expand(h)[:, None, None]
+    vs = v.double().abs().repeat_interleave(group, 2).transpose(1, 2).contiguous()  # (b, h, s, dv)
+    gs = g.double().abs().transpose(1, 2).contiguous()
+    a1, a2 = torch.matmul(p[:, :, 0], vs), torch.matmul(p[:, :, 1], vs)
+    off = {"out": (u + c) * (a1 + la * a2).transpose(1, 2)}
+    # delta = g . o_m, from outputs rounded to 16 bits of maps rounded to 16 bits
+    delta = ((3 * u + c) * gs * (a1 + (1 + la) * a2)).sum(-1, keepdim=True)
+    dp = torch.matmul(gs, vs.transpose(-1, -2).contiguous())
+    some = (p.sum(2) > 0).double()
+    # fp16: score gradients are scaled by their largest bound, whose last step is 2^-39 of it
+    least = 2.0**-38 * dp.amax() if dt == torch.float16 else 2.0**-126 * dp.amax()
+    ds_off = [w * p[:, :, m] * (c * dp + delta + (u + c) * (dp + delta / max(u, U32))) + least * some
+              for m, w in ((0, 1.0), (1, la))]
+    qs = q.double().abs().view(b, t, h, 2, d).permute(0, 2, 3, 1, 4)
+    ks = k.double().abs().view(b, s, hk, 2, d).repeat_interleave(group, 2).permute(0, 2, 3, 1, 4)
+    dq = torch.stack([torch.matmul(ds_off[m], ks[:, :, m].contiguous()) for m in (0, 1)], 2) * scale
+    dk = torch.stack([torch.matmul(ds_off[m].transpose(-1, -2).contiguous(), qs[:, :, m].contiguous())
+                      for m in (0, 1)], 2) * scale
+    off["dq"] = dq.permute(0, 3, 1, 2, 4).flatten(2, 3)
+    off["dk"] = dk.unflatten(1, (hk, group)).sum(2).permute(0, 3, 1, 2, 4).flatten(2, 3)
+    both = p[:, :, 0] + la * p[:, :, 1]
+    off["dv"] = torch.matmul(((u + c) * both + tiny * some).transpose(-1, -2).contiguous(), gs)
+    off["dv"] = off["dv"].unflatten(1, (hk, group)).sum(2).transpose(1, 2)
+    off["dlam"] = delta.sum((2, 3))
+    for name, x, y in zip(NAMES, got, want):
+        if name not in grads:
+            continue
+        worst = ((x.double() - y).abs() - off[name] - (0 if name == "dlam" else u) * y.abs() - tiny).max().item()
+        assert worst <= 0, f"{name}: {worst:.3e} past its bound, largest value {y.abs().max().item():.3e}"
+    return got
+
+
+def whole(gen, most, *shape, dt):
+    return torch.randint(-most, most + 1, shape, generator=gen, device="cuda").to(dt)
+
+
+SHAPES = [(60, 200, False), (70, 700, True), (2, 3000, True)]  # few keys, many, in splits
+
+
+def seen_by(b, t, s, causal):
+    seen = torch.ones(b, t, s, dtype=torch.bool, device="cuda")
+    return seen.tril(s - t) if causal else seen
+
+
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("power", [20, 30, 40, 66])
+@pytest.mark.parametrize("t,s,causal", SHAPES)
+def test_any_accepted_scale(dt, power, t, s, causal):
+    """Whole numbers as scores, times up to 2^66: the maps are the largest scores' keys, in equal
+    parts.  log2 of their number and its exponential are off by 2^-20 together."""
+    gen = torch.Generator(device="cuda").manual_seed(stable_seed((t, s)))
+    b, h, hk, d, dv = 2, 4, 2, 32, 48
+    q, k = whole(gen, 1, b, t, 2 * h, d, dt=DT[dt]), whole(gen, 1, b, s, 2 * hk, d, dt=DT[dt])
+    v, g = normal(gen, b, s, hk, dv, dt=DT[dt]), normal(gen, b, t, h, dv, dt=DT[dt], size=0.1)
+    lam = 0.2 + 0.6 * torch.rand(h, generator=gen, device="cuda")
+    names = NAMES if dt != "fp16" else ("out", "dv", "dlam")  # dq and dk pass fp16's range
+    check_maps(q, k, v, lam, g, scale=2.0**power, rel=2.0**-20, seen=seen_by(b, t, s, causal), causal=causal, grads=names)
+
+
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("size,parts", [(64, 8), (1024, 1)])
+@pytest.mark.parametrize("t,s,causal", SHAPES)
+def test_scores_with_a_large_common_part(dt, size, parts, t, s, causal):
+    """Scores of 2^12 and 2^20 with differences of a few: multiples of 2^-6 or 1, exact in fp32.
+    The exponents of what counts are below 2^6, off by 2^-19 with those of the sums."""
+    gen = torch.Generator(device="cuda").manual_seed(stable_seed((size, t)))
+    b, h, hk, d, dv = 2, 4, 2, 32, 48
+    q = whole(gen, parts, b, t, 2 * h, d, dt=DT[dt]) / parts
+    k = whole(gen, parts, b, s, 2 * hk, d, dt=DT[dt]) / parts
+    q[..., -1], k[..., -1] = size, size
+    v, g = normal(gen, b, s, hk, dv, dt=DT[dt]), normal(gen, b, t, h, dv, dt=DT[dt], size=0.1)
+    lam = 0.2 + 0.6 * torch.rand(h, generator=gen, device="cuda")
+    check_maps(q, k, v, lam, g, scale=1.0, rel=2.0**-18, seen=seen_by(b, t, s, causal), causal=causal)
