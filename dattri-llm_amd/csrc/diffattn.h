@@ -46,7 +46,7 @@ struct Args {
   char* records;  // (batch, Hk, T G): lse and delta of both maps as diff_grad_keys reads them
   uint8_t* takes_part;  // (batch, Hk, T G): 1 where the row sees a key, 3 where its scores are large besides
   float* off;     // 16 bits: (row splits, batch, Hk, 2, T G): how far delta was off, in parts
-  float* most;    // fp16: largest norms of g's rows and of v's, squared
+  float* most;    // fp16: (batch, Hk, 2): largest norms of g's rows and of v's, squared
   char *dq, *dk, *dv;
   float* lam_part;  // (batch, heads, chunks)
   int chunk, chunks;

@@ -22,7 +22,8 @@
 // sum to one.  The pass of dk and dv and dlam have delta from there.
 //
 // fp16 would lose small values of ds: there ds is scaled by the power of two that brings the
-// bound of the largest to 2^14, and its products back.
+// bound of the largest to 2^14, and its products back.  Each sample's key heads have a bound of
+// their own: what a sample gets does not depend on the others in its batch.
 //
 // 4 x 2048 tokens, 32 heads on 8, two 64-wide maps, 128-wide values, causal, bf16: delta 35 us,
 // dq 350 us and dk, dv 440 us of 275 GFLOP each (790 and 620 TFLOP/s), records 10 us.  Both large
@@ -95,6 +96,9 @@ __device__ __forceinline__ void put_record(char* to, float c, float top0, float 
   }
 }
 
+// Rows that are not finite have no say in a scale.
+__device__ __forceinline__ float finite(float norm) { return norm < __builtin_inff() ? norm : 0.f; }
+
 template <int DT>
 __global__ __launch_bounds__(256) void diff_delta(Args a) {
   constexpr int ES = Type<DT>::ES, V = Type<DT>::V, kRows = 256 / kLanes;
@@ -130,7 +134,7 @@ __global__ __launch_bounds__(256) void diff_delta(Args a) {
     }
     d0 = lanes_sum<kLanes>(d0);
     d1 = lanes_sum<kLanes>(d1);
-    if constexpr (DT == DA_F16) most = fmaxf(most, lanes_sum<kLanes>(norm));
+    if constexpr (DT == DA_F16) most = fmaxf(most, finite(lanes_sum<kLanes>(norm)));
     if (l == 0) {
       float* to = a.delta + of * 2 * rows + r;
       to[0] = d0 + lam * d1;  // o_1 = out + lam o_2
@@ -141,18 +145,21 @@ __global__ __launch_bounds__(256) void diff_delta(Args a) {
   }
   if constexpr (DT == DA_F16) {  // a maximum: the order does not matter
     most = lanes_max<64>(most) * fmaxf(1.f, lam * lam);
-    if (threadIdx.x % 64 == 0 && most > 0.f) atomicMax((unsigned*)a.most, __float_as_uint(most));
+    if (threadIdx.x % 64 == 0 && most > 0.f)
+      atomicMax((unsigned*)a.most + 2 * ((int64_t)b * a.Hk + hk), __float_as_uint(most));
   }
 }
 
-// The largest norm of the values' rows that a query may see, squared: 16 lanes a row.
-__global__ __launch_bounds__(256) void diff_values_norm(Args a) {
+// The largest norm of the values' rows that a query may see, squared: 16 lanes a row.  Workgroup
+// (b, key head, one of `parts`).
+__global__ __launch_bounds__(256) void diff_values_norm(Args a, int parts) {
   constexpr int V = Type<DA_F16>::V, kRows = 256 / kLanes;
-  const int l = threadIdx.x % kLanes;
-  const int64_t all = (int64_t)a.batch * a.S * a.Hk;
+  const int l = threadIdx.x % kLanes, part = blockIdx.x % parts;
+  const int64_t of = blockIdx.x / parts;
+  const int hk = (int)(of % a.Hk), b = (int)(of / a.Hk);
   float most = 0.f;
-  for (int64_t at = (int64_t)blockIdx.x * kRows + threadIdx.x / kLanes; at < all; at += (int64_t)gridDim.x * kRows) {
-    const int hk = (int)(at % a.Hk), key = (int)(at / a.Hk % a.S), b = (int)(at / a.Hk / a.S);
+  for (int64_t at = (int64_t)part * kRows + threadIdx.x / kLanes; at < a.S; at += (int64_t)parts * kRows) {
+    const int key = (int)at;
     float norm = 0.f;
     if (!(a.causal && key >= a.T + a.q_start) && (!a.mask || a.mask[b * a.m_b + key * a.m_k])) {
       const char* v = a.v + (b * a.v_b + key * a.v_t + hk * a.v_h) * 2;
@@ -163,10 +170,10 @@ __global__ __launch_bounds__(256) void diff_values_norm(Args a) {
         for (int e = 0; e < V; ++e) norm += x[e] * x[e];
       }
     }
-    most = fmaxf(most, lanes_sum<kLanes>(norm));
+    most = fmaxf(most, finite(lanes_sum<kLanes>(norm)));
   }
   most = lanes_max<64>(most);
-  if (threadIdx.x % 64 == 0 && most > 0.f) atomicMax((unsigned*)a.most + 1, __float_as_uint(most));
+  if (threadIdx.x % 64 == 0 && most > 0.f) atomicMax((unsigned*)a.most + 2 * of + 1, __float_as_uint(most));
 }
 
 // After dq: delta as the maps in fp32 have it, the records, and dlam's parts.
@@ -208,9 +215,10 @@ __global__ __launch_bounds__(256) void diff_lam_join(const float* parts, float* 
 // fp16: a power of two under which no |ds| <= 2 max(1, |lam|) |g| |v| passes 2^14, and the
 // largest are near it: the maps' small entries keep their bits.  1 where there is none.
 template <int DT>
-__device__ __forceinline__ float small_scale(const Args& a) {
+__device__ __forceinline__ float small_scale(const Args& a, int b, int hk) {
   if constexpr (DT != DA_F16) return 1.f;
-  const float bound = __builtin_sqrtf(a.most[0]) * __builtin_sqrtf(a.most[1]);
+  const float* most = a.most + 2 * ((int64_t)b * a.Hk + hk);
+  const float bound = __builtin_sqrtf(most[0]) * __builtin_sqrtf(most[1]);
   const uint32_t e = __float_as_uint(bound) >> 23;  // bound < 2^(e - 126); of a float from zero on
   return e < 40 || e > 220 ? 1.f : __uint_as_float((266u - e) << 23);  // 2^(139 - e)
 }
@@ -285,7 +293,7 @@ __global__ __launch_bounds__(kThreads, DT != DA_F32 && DP == 64 ? 2 : 1) void di
   for (int n = 0; n < ND; ++n) dk[0][n] = zeros(), dk[1][n] = zeros();
 #pragma unroll
   for (int n = 0; n < NV; ++n) dv[n] = zeros();
-  const float c = a.scale * kLog2e, small = small_scale<DT>(a);
+  const float c = a.scale * kLog2e, small = small_scale<DT>(a, b, hk);
   // Ones against the parts of one half's records.
   constexpr uint32_t kOnes = 0x3f803f80u, kOne = 0x3f80u;
   const uint32_t in_low = half ? 0u : ~0u;
@@ -558,7 +566,7 @@ __global__ __launch_bounds__(kThreads, DT != DA_F32 && DP == 64 ? 2 : 1) void di
   const int64_t tops = tops_at(a) + base;
   const float top0 = in ? a.lse[tops] : 0.f, top1 = in ? a.lse[tops + rows] : 0.f;
   float de0 = in ? a.delta[base] : 0.f, de1 = in ? -sign * a.delta[base + rows] : 0.f;
-  const float c = a.scale * kLog2e, small = small_scale<DT>(a);
+  const float c = a.scale * kLog2e, small = small_scale<DT>(a, b, hk);
   // Large scores: the difference from the largest first.
   const bool far = DT == DA_F32 || __any(!near(top0, top1, c));
   const float whole0 = fmaf(top0, c, lse0), whole1 = fmaf(top1, c, lse1);
@@ -718,7 +726,7 @@ void share(int64_t mine, int64_t others, int64_t groups, int64_t cus, int* block
 }
 
 // How the two passes are shared out, and the workspace: delta, the parts of dlam, the largest
-// |g|, the records, whether a row takes part, and the sums of the splits (of one pass after the other).
+// |g| and |v|, the records, whether a row takes part, and the sums of the splits (of one pass after the other).
 struct Plan {
   Args keys, rows;  // blocks, splits, each
   int64_t records_at, parts_at, most_at, off_at, takes_part_at, sums_at;  // in floats
@@ -736,7 +744,7 @@ int plan(int dtype, int64_t batch, int64_t heads, int64_t k_heads, int64_t T, in
   p->records_at = (batch * heads * T * 2 + 3) / 4 * 4;
   p->parts_at = p->records_at + batch * heads * T * (dtype == DA_F32 ? Record<DA_F32>::kBytes : Record<DA_BF16>::kBytes) / 4;
   p->most_at = p->parts_at + batch * heads * a->chunks;
-  p->off_at = p->most_at + 2;
+  p->off_at = p->most_at + (dtype == DA_F16 ? 2 * batch * k_heads : 0);
   p->takes_part_at = p->off_at + (dtype == DA_F32 ? 0 : p->rows.splits * batch * heads * T * 2);
   p->sums_at = (p->takes_part_at + (batch * heads * T + 3) / 4 + 3) / 4 * 4;
   const int64_t of_keys = p->keys.splits > 1 ? p->keys.splits * batch * S * k_heads * (2 * D + Dv) : 0;
@@ -816,13 +824,15 @@ int da_diff_attention_grad(const da_diff_inputs* in, const void* g, int64_t g_bs
   a.part = a.delta + p.sums_at;
   a.dq = (char*)dq, a.dk = (char*)dk, a.dv = (char*)dvalue;
   const hipStream_t st = (hipStream_t)stream;
-  if (dtype == DA_F16 && (rc = zero_f32_2d(a.most, 1, 2, 2, st))) return rc;
+  if (dtype == DA_F16 && (rc = zero_f32_2d(a.most, 1, 2 * pairs, 2 * pairs, st))) return rc;
   const unsigned delta_grid = (unsigned)(batch * heads * a.chunks);
   if (dtype == DA_BF16) diff_delta<DA_BF16><<<delta_grid, 256, 0, st>>>(a);
   else if (dtype == DA_F16) diff_delta<DA_F16><<<delta_grid, 256, 0, st>>>(a);
   else diff_delta<DA_F32><<<delta_grid, 256, 0, st>>>(a);
-  if (dtype == DA_F16 && k_len)
-    diff_values_norm<<<(unsigned)std::min<int64_t>(1024, (pairs * k_len + 15) / 16), 256, 0, st>>>(a);
+  if (dtype == DA_F16 && k_len) {  // about 1024 workgroups
+    const int64_t parts = std::max<int64_t>(1, std::min<int64_t>(1024 / pairs, (k_len + 15) / 16));
+    diff_values_norm<<<(unsigned)(pairs * parts), 256, 0, st>>>(a, (int)parts);
+  }
   rc = by_widths(dtype, widths(d, dv), [&](auto dt, auto dp, auto dvp) {
     constexpr int DT = decltype(dt)::value, DP = decltype(dp)::value, DVP = decltype(dvp)::value;
     if (rows) {

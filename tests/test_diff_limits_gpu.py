@@ -210,3 +210,40 @@ def test_scores_with_a_large_common_part(dt, size, parts, t, s, causal):
     v, g = normal(gen, b, s, hk, dv, dt=DT[dt]), normal(gen, b, t, h, dv, dt=DT[dt], size=0.1)
     lam = 0.2 + 0.6 * torch.rand(h, generator=gen, device="cuda")
     check_maps(q, k, v, lam, g, scale=1.0, rel=2.0**-18, seen=seen_by(b, t, s, causal), causal=causal)
+
+
+# ---------------------------------------------------------------------------
+# fp16
+# ---------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("what,which", [*((x, y) for x in ("large", "inf", "nan") for y in "gv"), ("large", "lam")])
+@pytest.mark.parametrize("t,s", [(64, 64), (300, 600), (1, 3000)])
+def test_half_precision_gradients_do_not_depend_on_the_batch(what, which, t, s):
+    """A sample beside one with gradients (values) of 2^20 times its own, or infinite ones, gets
+    what it gets beside zeros; a key head beside another one likewise."""
+    h, hk = 4, 2
+    q, k, v, lam, g = operands(stable_seed((t, s, which)), 3, t, s, h, hk, 64, 64, torch.float16)
+    g, v = g * 2.0**-12, v * 2.0**-6
+    results = []
+    for fill in (0.0, 1.0):
+        q1, k1, v1, g1, lam1 = q.clone(), k.clone(), v.clone(), g.clone(), lam.clone()
+        if which == "lam":  # the heads of key head 0
+            lam1[:2] = 2.0**12 if fill else 0.0
+        else:
+            x = v1 if which == "v" else g1
+            x[0] *= fill * 2.0**20 if which == "g" else fill * 2.0**14
+            x[1, :, 0] *= fill * 2.0**16 if which == "g" else fill * 2.0**14
+            if fill and what != "large":
+                x[0, 0, 0, 3] = float(what)
+                x[1, 0, 0, 3] = float(what)
+        results.append(run(q1, k1, v1, lam1, g1))
+    for name, x, y in zip(NAMES, *results):
+        if which != "lam":
+            assert torch.equal(x[2], y[2]), name
+            # One query's 3000 probabilities of 2^-11.5 times gradients of 2^-15.3: dv of 2^-27 and
+            # dk below that are zeros in fp16, whose last step is 2^-24.
+            assert (t == 1 or bool(x[2].any())) and bool(x[2].isfinite().all())
+        per = x.shape[2 if x.dim() == 4 else 1] // 2  # the second key head's
+        a, b = (z[:, :, per:] if z.dim() == 4 else z[:, per:] for z in (x, y))
+        assert torch.equal(a[1 if which != "lam" else slice(None)], b[1 if which != "lam" else slice(None)]), name
