@@ -22,7 +22,8 @@
 // sum to one.  The pass of dk and dv and dlam have delta from there.
 //
 // fp16 would lose small values of ds: there ds is scaled by the power of two that brings the
-// bound of the largest to 2^14, and its products back.  Each sample's key heads have a bound of
+// bound of the largest to 2^14, and the maps' mixture by one that its factors allow; their products
+// are scaled back.  Each sample's key heads have a bound of
 // their own: what a sample gets does not depend on the others in its batch.
 //
 // 4 x 2048 tokens, 32 heads on 8, two 64-wide maps, 128-wide values, causal, bf16: delta 35 us,
@@ -321,10 +322,19 @@ __global__ __launch_bounds__(kThreads, DT != DA_F32 && DP == 64 ? 2 : 1) void di
       st16(lds + L::kOffsetsAt + (i * kThreads + threadIdx.x) * 16,
            u32x4{at[4 * i], at[4 * i + 1], at[4 * i + 2], at[4 * i + 3]});
   }
-  // Negative factors: their sign is not in the exponential.
+  // Negative factors: their sign is not in the exponential.  fp16: the maps' mixture, at most
+  // 1 + |lam|, times the power of two that brings that bound to 2^15.
   bool any_minus = false;
-  for (int i = lane; i < a.G; i += kWave) any_minus |= lam_of(a, hk * a.G + i) < 0.f;
+  float most_lam = 0.f;
+  for (int i = lane; i < a.G; i += kWave) {
+    const float lam = lam_of(a, hk * a.G + i);
+    any_minus |= lam < 0.f;
+    most_lam = fmaxf(most_lam, fabsf(lam));
+  }
   any_minus = __any(any_minus);
+  float mixture = 1.f;
+  if constexpr (DT == DA_F16)  // 1 + |lam| < 2^(e - 126)
+    mixture = __uint_as_float((268u - (__float_as_uint(1.f + lanes_max<kWave>(most_lam)) >> 23)) << 23);
   const uint8_t* takes_part = a.takes_part + ((int64_t)b * a.Hk + hk) * rows;
   auto row_byte = [&](int r0) {
     const int r = r0 + (lane & 31);
@@ -449,7 +459,7 @@ __global__ __launch_bounds__(kThreads, DT != DA_F32 && DP == 64 ? 2 : 1) void di
       const float p0 = s0[i], p1 = s1[i];
       s0[i] = (DT == DA_F16 ? p0 * small : p0) * dp[i];
       s1[i] = (DT == DA_F16 ? p1 * small : p1) * -dp1[i];
-      dp[i] = p0 - p1;
+      dp[i] = DT == DA_F16 ? (p0 - p1) * mixture : p0 - p1;
     }
 #pragma unroll
     for (int j = 0; j < KC; ++j) {
@@ -468,7 +478,7 @@ __global__ __launch_bounds__(kThreads, DT != DA_F32 && DP == 64 ? 2 : 1) void di
     if (r0 + kTile < end) step(r0 + kTile, std::integral_constant<int, 1>{});
   }
   if (key >= a.S) return;
-  const float by = a.scale / small;
+  const float by = a.scale / small, by_v = 1.f / mixture;
   const int64_t n_keys = (int64_t)a.batch * a.S * a.Hk;
   const int64_t to = ((int64_t)b * a.S + key) * a.Hk + hk;
   // A key that takes no part was a column of its own: whatever it holds is dropped here.
@@ -493,7 +503,7 @@ __global__ __launch_bounds__(kThreads, DT != DA_F32 && DP == 64 ? 2 : 1) void di
 #pragma unroll
     for (int i = 0; i < 16; i += 4)
       put(a.dv, n_keys * 2 * a.D, to, a.Dv, 32 * n + acc_at(i, half),
-          f32x4{dv[n][i], dv[n][i + 1], dv[n][i + 2], dv[n][i + 3]});
+          f32x4{dv[n][i], dv[n][i + 1], dv[n][i + 2], dv[n][i + 3]} * by_v);
 }
 
 // ---------------------------------------------------------------------------

@@ -247,3 +247,35 @@ def test_half_precision_gradients_do_not_depend_on_the_batch(what, which, t, s):
         per = x.shape[2 if x.dim() == 4 else 1] // 2  # the second key head's
         a, b = (z[:, :, per:] if z.dim() == 4 else z[:, per:] for z in (x, y))
         assert torch.equal(a[1 if which != "lam" else slice(None)], b[1 if which != "lam" else slice(None)]), name
+
+
+def test_half_precision_values_gradient_with_many_keys():
+    """Probabilities of 2^-17 lie below fp16's normal range (2^-14).  Rounded to half a step each,
+    where the gradients they weigh have random signs, they leave an error as large as the
+    output's own rounding: sqrt 2 of it together, where steps of 2^-24 leave seven times."""
+    t, s, h, hk, d, dv = 64, 131072, 4, 1, 64, 64
+    q, k, v, lam, g = operands(43, 1, t, s, h, hk, d, dv, torch.float16)
+    q, g = q / 4, g * 640
+    want = exact(q, k, v, lam, g)[0][3]
+    got = run(q, k, v, lam, g)[3].double()
+    rounding = (want.half().double() - want).norm()
+    assert (got - want).norm() < 1.6 * rounding, ((got - want).norm() / rounding).item()
+
+
+@pytest.mark.parametrize("t,s", [(40, 60), (200, 700)])
+def test_half_precision_with_factors_past_its_range(t, s):
+    """|lam| p up to 10^6: the mixture of the maps passes 65504, what it gives does not."""
+    q, k, v, lam, g = operands(47, 1, t, s, 4, 2, 32, 32, torch.float16)
+    q, k = 3 * q, 2 * k  # maps of a few keys
+    lam = torch.tensor([1e6, -1e6, 0.5, 3e5], device="cuda")
+    v, g = v * 2.0**-10, g * 2.0**-10
+    want, p = exact(q, k, v, lam, g)
+    assert (lam.abs()[:, None, None] * p[0, :, 1]).amax() > 65504
+    got = run(q, k, v, lam, g)
+    u, tiny = 2.0**-11, 2.0**-24
+    # Scores of up to 100 of 32 products, in fp32: exponentials off by 2^-24 (40 + 100) at most.
+    both = p[:, :, 0] + lam.abs()[:, None, None] * p[:, :, 1]
+    off = torch.matmul(both.transpose(-1, -2).contiguous(), g.double().abs().transpose(1, 2).contiguous())
+    off = (u + 2.0**-16) * off.unflatten(1, (2, 2)).sum(2).transpose(1, 2)
+    assert bool(((got[3].double() - want[3]).abs() <= off + u * want[3].abs() + tiny).all())
+    assert all(bool(x.isfinite().all()) for x in got)
