@@ -11,8 +11,8 @@
 // rounded, the second operand of o^T = v^T p^T as they stand, where v is read transposed out
 // of LDS.  A difference of scores is formed before it is scaled where they are large (kNear), so
 // that any finite scores have finite exponentials.  These are relative to a maximum that is looked for again only when the sum
-// of a lane's sixteen passes 2^10: until then they are at most that much larger than with the
-// last one (the first tile has none, and passes; with a new one in every tile that has a larger
+// of a lane's sixteen passes 2^10 (fp16: 2^15, the largest being 2^10): until then they are at
+// most that much larger than with the last one (the first tile has none, and passes; with a new one in every tile that has a larger
 // score 277 us in place of 257 at the first size below).  At the end the second map's waves hand
 // their values, divided and weighted, to the first's through LDS.
 //
@@ -31,7 +31,16 @@ namespace {
 // Keys of a split (18 heads of 509 keys in fp32: 65 us with 64, 59 with 128).
 constexpr int kLeastSplit = 128;
 constexpr int kFewKeys = 512;
-constexpr float kMostSum = 1024.f;  // of sixteen exponentials, before a new maximum
+
+// The largest exponential is 2^kUp when it is found, and a lane's sixteen sum to kMostSum before a
+// new maximum is looked for.  As fp16 operands they are lifted so that keys far below the largest
+// keep bits, down to 2^-24: of 2^17 keys 17 below it, which have a tenth of a percent of the row,
+// nothing was left without.
+template <int DT>
+struct Range {
+  static constexpr float kUp = DT == DA_F16 ? 10.f : 0.f;
+  static constexpr float kMostSum = DT == DA_F16 ? 32768.f : 1024.f;
+};
 
 // A row that sees keys has a sum of about 1 and more (its maximum's exponential), one that sees
 // none 0.  A split whose live scores are all -inf sums to kOnlyInf: that counts for nothing beside
@@ -41,12 +50,19 @@ __device__ __forceinline__ float settled(float sum) { return sum > 0.f && sum < 
 // Of a settled sum, NaN of NaN.
 __device__ __forceinline__ float inverse(float sum) { return sum == 0.f ? 0.f : 1.f / sum; }
 
-// The exponentials are 2^((s - top) c + shift).  shift is what rounding top c leaves of it, so that
-// one fma, s c - round(top c), gives them; where that could be large (it is half a unit of top c's
-// last place), 0, and the difference is formed first.
+// The exponentials are 2^((s - top) c + shift).  shift is kUp and what rounding top c - kUp leaves of
+// it, so that one fma, s c - base, gives them; where that could be large (it is half a unit of top
+// c's last place), kUp, and the difference is formed first.
 constexpr float kNear = 0x1p20f;
 __device__ __forceinline__ bool near(float top, float c) { return fabsf(top * c) < kNear; }
-__device__ __forceinline__ float shift_of(float top, float c) { return near(top, c) ? fmaf(top, c, -(top * c)) : 0.f; }
+template <int DT>
+__device__ __forceinline__ float base_of(float top, float c) {
+  return fmaf(top, c, -Range<DT>::kUp);
+}
+template <int DT>
+__device__ __forceinline__ float shift_of(float top, float c) {
+  return near(top, c) ? fmaf(top, c, -base_of<DT>(top, c)) : Range<DT>::kUp;
+}
 
 // What the backward pass needs of a row: the settled sum of 2^((s - top) c), +inf where it sees no
 // key, and top.
@@ -125,7 +141,7 @@ __global__ __launch_bounds__(2 * NG * kWave, DT == DA_F32 && DVP == 256 ? 1 : 2)
   const float c = a.scale * kLog2e;
   f32x16 o[NB];
   // A lane without a row sees nothing, and does not make the others' scores large.
-  float top = last >= 0 ? kLowest : 0.f, shift = 0.f, sum = 0.f;
+  float top = last >= 0 ? kLowest : 0.f, shift = Range<DT>::kUp, sum = 0.f;
   bool far = true;  // whether a score of the wave is large
   uint32_t saw = 0;  // whether the row has seen a key
 #pragma unroll
@@ -160,17 +176,17 @@ __global__ __launch_bounds__(2 * NG * kWave, DT == DA_F32 && DVP == 256 ? 1 : 2)
 #pragma unroll
         for (int i = 0; i < 16; ++i) e[i] = __builtin_amdgcn_exp2f(fmaf(s[i] - top, c, shift));
       } else {
-        const float tc = top * c;
+        const float base = base_of<DT>(top, c);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) e[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c, -tc));
+        for (int i = 0; i < 16; ++i) e[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c, -base));
       }
       return over_acc(e, [](float u, float v) { return u + v; });
     };
     float part = exponentials();
-    if (__any(part > kMostSum)) {
+    if (__any(part > Range<DT>::kMostSum)) {
       float x = over_acc(s, [](float u, float v) { return fmaxf(u, v); });
       x = fmaxf(x, other_half(x));
-      const float now = fmaxf(top, x), shift_now = shift_of(now, c);
+      const float now = fmaxf(top, x), shift_now = shift_of<DT>(now, c);
       const float by = __builtin_amdgcn_exp2f(fmaf(top - now, c, shift_now - shift));
       top = now, shift = shift_now;
       far = __any(!near(top, c));
@@ -265,7 +281,7 @@ __global__ __launch_bounds__(256) void diff_join(Args a) {
       const f32x4 x = *(const f32x4*)(from + m * DVP + 4 * l);
       const float now = fmaxf(top[m], top2);
       const float f1 = __builtin_amdgcn_exp2f((top[m] - now) * c);
-      const float f2 = __builtin_amdgcn_exp2f(fmaf(top2 - now, c, -shift_of(top2, c)));
+      const float f2 = __builtin_amdgcn_exp2f(fmaf(top2 - now, c, -shift_of<DT>(top2, c)));
       top[m] = now;
       sum[m] = sum[m] * f1 + sum2 * f2;
       o[m] = o[m] * f1 + x * f2;

@@ -279,3 +279,27 @@ def test_half_precision_with_factors_past_its_range(t, s):
     off = (u + 2.0**-16) * off.unflatten(1, (2, 2)).sum(2).transpose(1, 2)
     assert bool(((got[3].double() - want[3]).abs() <= off + u * want[3].abs() + tiny).all())
     assert all(bool(x.isfinite().all()) for x in got)
+
+
+@pytest.mark.parametrize("dt,t", [*((dt, t) for dt in DT for t in (1, 70)), ("bf16", 40000), ("fp16", 40000)])
+@pytest.mark.parametrize("below", [14.0, 18.0, 20.0])
+def test_one_large_score_above_many_small_ones(dt, t, below):
+    """131071 keys whose exponentials are e^-14 to e^-20 of the largest: together 11% to 3e-4 of the
+    row.  The largest one's value is 0 and theirs are 1, so that out is their part, to the output's
+    half step, the exponentials' own (16 bits) and the sums' 2^-24 a term (a lane adds s / 32).
+    The most queries leave the keys whole, the others split them."""
+    s = 131072
+    q = torch.zeros(1, t, 2, 16, dtype=DT[dt], device="cuda")
+    k = torch.zeros(1, s, 2, 16, dtype=DT[dt], device="cuda")
+    v = torch.ones(1, s, 1, 16, dtype=DT[dt], device="cuda")
+    q[..., 0], k[:, 777, :, 0], v[:, 777] = 1.0, below, 0.0
+    lam = torch.tensor([0.25], device="cuda")
+    mass = (s - 1) * torch.tensor(-below, dtype=torch.float64).exp().item()
+    want = 0.75 * mass / (1 + mass)
+    got = ops.diff_attention(q, k, v, lam, scale=1.0).double()
+    u = 0.0 if dt == "fp32" else torch.finfo(DT[dt]).eps / 2
+    # fp16 operands below 2^-14 have steps of 2^-24: with the largest at 2^10, half a step is 2^-35 of
+    # it, of each key (at 20 below, where the exponentials are 2^-18.9, that is 2^-6 of them).
+    least = 1.25 * s * 2.0**-35 if dt == "fp16" else 0.0
+    off = want * (u + 1.25 / 0.75 * (u + (s / 32 + 64) * U32)) + least + 2.0**-25
+    assert ((got - want).abs() <= off).all(), got.flatten()[0].item() / want
