@@ -97,14 +97,18 @@ __device__ __forceinline__ float key_value(uint64_t key) {
 __device__ __forceinline__ int64_t key_index(uint64_t key) { return 0xffffffffu - (uint32_t)key; }
 
 // Sums of 2^d and of d 2^d, d = (logit - m) c, relative to the largest logit m.  The
-// difference comes first: logits of a type's lowest value do not overflow.
+// difference comes first: logits of a type's lowest value do not overflow.  Their distance from
+// others does, times c: what a new maximum leaves nothing of is 0, not 0 times it.
+__device__ __forceinline__ float moved(float e, float s, float by, float scale) {
+  return da_mul_or_zero(scale, e + da_mul_or_zero(s, by));
+}
 struct Stats {
   float m, s, e;
   __device__ void join(float m2, float s2, float e2, float c) {
     const float top = fmaxf(m, m2), d1 = (m - top) * c, d2 = (m2 - top) * c;
     const float f1 = __builtin_amdgcn_exp2f(d1), f2 = __builtin_amdgcn_exp2f(d2);
     // s = 0 where nothing was seen: its distance does not count.
-    e = f1 * (e + da_mul_or_zero(s, d1)) + f2 * (e2 + da_mul_or_zero(s2, d2));
+    e = moved(e, s, d1, f1) + moved(e2, s2, d2, f2);
     s = s * f1 + s2 * f2;
     m = top;
   }
@@ -199,7 +203,7 @@ __global__ __launch_bounds__(NT) void logprobs_forward(LpArgs a) {
     if (kTop && top > most) most = top, most_at = v;
     if (__any(top > x.m)) {
       const float m = fmaxf(x.m, top), by = (x.m - m) * c, scale = __builtin_amdgcn_exp2f(by);
-      x.e = scale * (x.e + da_mul_or_zero(x.s, by));
+      x.e = moved(x.e, x.s, by, scale);
       x.s *= scale;
       x.m = m;
     }
@@ -241,14 +245,14 @@ __global__ __launch_bounds__(NT) void logprobs_forward(LpArgs a) {
     add(raw, v);
     const float m = fmaxf(x.m, rest), by = (x.m - m) * c, scale = __builtin_amdgcn_exp2f(by);
     const float d = (rest - m) * c, p = __builtin_amdgcn_exp2f(d);
-    x.e = scale * (x.e + da_mul_or_zero(x.s, by)) + da_mul_or_zero(p, d);
+    x.e = moved(x.e, x.s, by, scale) + da_mul_or_zero(p, d);
     x.s = x.s * scale + p;
     x.m = m;
   }
   {  // the wave's, relative to its maximum
     const float m = lanes_max<kWave>(x.m), by = (x.m - m) * c, scale = __builtin_amdgcn_exp2f(by);
     const float s = lanes_sum<kWave>(x.s * scale);
-    const float e = lanes_sum<kWave>(scale * (x.e + da_mul_or_zero(x.s, by)));
+    const float e = lanes_sum<kWave>(moved(x.e, x.s, by, scale));
     if (lane == 0) stat[0][wave] = m, stat[1][wave] = s, stat[2][wave] = e;
   }
   const bool mine = kTop && v0 + (int64_t)tid * V < whole;
