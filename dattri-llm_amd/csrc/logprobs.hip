@@ -63,6 +63,7 @@ struct LpArgs {
   const float* entropy_in;
   const float* lse_in;
   int64_t u_b, u_t, h_b, h_t, ul_b, ul_t;
+  bool alone;  // whether one workgroup takes the whole of a row with a large lse
   char* grad;
 };
 
@@ -420,9 +421,54 @@ __global__ __launch_bounds__(kJoin) void logprobs_join(LpArgs a, int dt) {
   });
 }
 
+// Over the workgroup's row: its largest logit m, and log sum e^((z - m) / temperature).
+template <int DT, int NT>
+__device__ float2 row_sums(const char* logits, int64_t vocab, float c, float (*stat)[NT / kWave]) {
+  constexpr int V = Elem<DT>::kVec, kWaves = NT / kWave;
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  const int64_t whole = vocab - vocab % V;
+  float m = kFloor, s = 0.f;
+  for (int64_t v = (int64_t)threadIdx.x * V; v < whole; v += (int64_t)NT * V * kBatch) {
+    float f[kBatch][V], top = m;
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      unpack16<DT>(load_run<DT>(logits, v + (int64_t)i * NT * V, whole), f[i]);
+#pragma unroll
+      for (int e = 0; e < V; ++e) top = fmaxf(top, f[i][e]);
+    }
+    s *= __builtin_amdgcn_exp2f((m - top) * c);
+    m = top;
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i)
+#pragma unroll
+      for (int e = 0; e < V; ++e) s += __builtin_amdgcn_exp2f((f[i][e] - m) * c);
+  }
+  if ((int)threadIdx.x < vocab - whole) {
+    const float f = Elem<DT>::load(logits, whole + threadIdx.x), top = fmaxf(m, f);
+    s = s * __builtin_amdgcn_exp2f((m - top) * c) + __builtin_amdgcn_exp2f((f - top) * c);
+    m = top;
+  }
+  float most = lanes_max<kWave>(m);
+  s = lanes_sum<kWave>(s * __builtin_amdgcn_exp2f((m - most) * c));
+  if (lane == 0) stat[0][wave] = most, stat[1][wave] = s;
+  __syncthreads();
+  for (int w = 0; w < kWaves; ++w) most = fmaxf(most, stat[0][w]);
+  s = 0.f;
+  for (int w = 0; w < kWaves; ++w) s += stat[1][w] * __builtin_amdgcn_exp2f((stat[0][w] - most) * c);
+  return float2{most, log2f(s) * kLn2};
+}
+
+// How far from 0 a row's lse may lie for the gradient to take probabilities from it: as an fp32
+// number it is off by 2^-25 of its size and more, and so are all of the row's probabilities,
+// relatively.  2^-20 in fp32; in 16 bits a sixteenth of the gradient's own half step.
+template <int DT>
+constexpr float kFar = DT == DA_F32 ? 32.f : DT == DA_F16 ? 512.f : 4096.f;
+
 // ---------------------------------------------------------------------------
 // Backward: workgroup (row, part), the last rows first: a forward call just before left them
-// in the last-level cache.  kStream: gradients that do not fit there are written past it, and
+// in the last-level cache.  Rows whose lse is large (a common offset, a small temperature) are
+// read twice, for their maximum and sum apart: by one part's workgroup, which then writes the
+// whole row, or with few rows by each.  kStream: gradients that do not fit there are written past it, and
 // leave it to the logits (3 x 509 rows of 50257 in fp32, forward and backward: 195 us without,
 // 163 with both).
 // ---------------------------------------------------------------------------
@@ -434,17 +480,26 @@ __global__ __launch_bounds__(NT) void logprobs_backward(LpArgs a) {
   const bool live = !a.mask || a.mask[b * a.m_b + t * a.m_t];
   const char* logits = a.logits + (b * a.l_b + t * a.l_t) * ES;
   char* grad = a.grad + row * a.vocab * ES;
-  const int64_t v0 = part * a.part, end = min(v0 + a.part, a.vocab);
+  int64_t v0 = part * a.part, end = min(v0 + a.part, a.vocab);
   int64_t target = a.targets[b * a.t_b + t * a.t_t];
   const bool named = live && target >= 0 && target < a.vocab;
   target = named ? target : -1;
   const float up = named && a.up ? a.up[b * a.u_b + t * a.u_t] * a.inv_temperature : 0.f;
   const float up_h = live && a.up_h ? a.up_h[b * a.h_b + t * a.h_t] * a.inv_temperature : 0.f;
   const float up_lse = live && a.up_lse ? a.up_lse[b * a.ul_b + t * a.ul_t] * a.inv_temperature : 0.f;
-  const float lse = live ? a.lse_in[row] : 0.f;
+  float m = 0.f, lse = live ? a.lse_in[row] : 0.f;
+  if (live && !(fabsf(lse) <= kFar<DT>)) {  // the same in all threads
+    __shared__ float stat[2][NT / kWave];
+    if (a.alone) {  // any one part, so that those that stay lie on all dies
+      if (part != ((uint32_t)row * 0x9e3779b1u >> 8) % a.parts) return;
+      v0 = 0, end = a.vocab;
+    }
+    const float2 x = row_sums<DT, NT>(logits, a.vocab, a.inv_temperature * kLog2e, stat);
+    m = x.x, lse = x.y;
+  }
   const float whole = up_lse - up - (a.up_h && live ? up_h * a.entropy_in[row] : 0.f), slope = -up_h;
   const auto of = [&](float f) __attribute__((always_inline)) {
-    const float d = fmaf(f, a.inv_temperature, -lse), p = __builtin_amdgcn_exp2f(d * kLog2e);
+    const float d = fmaf(f - m, a.inv_temperature, -lse), p = __builtin_amdgcn_exp2f(d * kLog2e);
     return live ? da_mul_or_zero(p, fmaf(d, slope, whole)) : 0.f;
   };
   const int64_t runs = end - (end - v0) % V;  // where the whole runs end
@@ -619,6 +674,7 @@ int da_token_logprobs_grad(const float* up, int64_t up_bstride, int64_t up_tstri
   a.part = 2 * (int64_t)kBatch * nt * vec;
   a.parts = (vocab + a.part - 1) / a.part;
   if (a.rows > kMaxBlocks / 4 / a.parts) return set_error(DA_ERR_UNSUPPORTED, "da_token_logprobs_grad: too many rows");
+  a.alone = a.rows * a.parts > 4 * cus;
   a.up = up, a.u_b = up_bstride, a.u_t = up_tstride;
   a.up_h = up_entropy, a.h_b = uh_bstride, a.h_t = uh_tstride;
   a.up_lse = up_lse, a.ul_b = ul_bstride, a.ul_t = ul_tstride;
