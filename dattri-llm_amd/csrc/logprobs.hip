@@ -543,8 +543,9 @@ int check_rows(const char* what, int dtype, int64_t batch, int64_t tokens, int64
   if (!valid_dtype(dtype)) return set_error(DA_ERR_INVALID, "%s: bad dtype %d", what, dtype);
   if (batch < 0 || tokens < 0) return set_error(DA_ERR_INVALID, "%s: negative size", what);
   if (vocab < 1 || vocab > INT32_MAX) return set_error(DA_ERR_UNSUPPORTED, "%s: vocabularies of 1 to 2^31 - 1 tokens", what);
-  if (!(temperature > 0.f) || !(1.f / temperature < 1e30f))
-    return set_error(DA_ERR_INVALID, "%s: the temperature must be positive", what);
+  // Both 1 / temperature and -inf times it have to be what they say.
+  if (!(temperature > 0.f) || !(1.f / temperature < 1e30f) || !(1.f / temperature >= 0x1p-126f))
+    return set_error(DA_ERR_INVALID, "%s: the temperature must lie between 1e-30 and 8e37", what);
   if (tokens && batch > kMaxBlocks / 4 / tokens) return set_error(DA_ERR_UNSUPPORTED, "%s: too many rows", what);
   return DA_OK;
 }

@@ -2009,8 +2009,8 @@ def _token_rows(what: str, logits: torch.Tensor, targets: torch.Tensor, mask, te
         raise ValueError(f"{what}: targets must be int64, got {targets.dtype}")
     if mask is not None and mask.shape != targets.shape:
         raise ValueError(f"{what}: mask must have shape {tuple(targets.shape)}, got {tuple(mask.shape)}")
-    if not temperature > 0:
-        raise ValueError(f"{what}: the temperature must be positive, got {temperature}")
+    if not 1e-30 < temperature < 8e37:
+        raise ValueError(f"{what}: the temperature must lie between 1e-30 and 8e37, got {temperature}")
     if logits.dim() == 2:
         logits, targets, mask = logits[None], targets[None], None if mask is None else mask[None]
     return _unit_rows(logits), targets, mask

@@ -926,7 +926,7 @@ int da_diff_attention_grad(const da_diff_inputs* in, const void* g, int64_t g_bs
  *
  * A target outside the vocabulary (-100, say) names none: logprob 0.  mask: bytes, 0
  * marks a token whose logits are not read and whose outputs are zero (indices -1);
- * NULL: none.  top <= 32; vocab < 2^31.
+ * NULL: none.  top <= 32; vocab < 2^31; temperature 1e-30 to 8e37.
  *
  * The backward call writes the logits' gradient (contiguous) for the gradients up,
  * up_entropy and up_lse (batch, tokens; any strides; NULL: zero) of logprob, entropy
