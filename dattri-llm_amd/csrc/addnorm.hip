@@ -118,6 +118,20 @@ __device__ __forceinline__ u32x4 pack16(const float* f) {
   return v;
 }
 
+// x / scale to the nearest: one step of Markstein's correction of a product with the nearest to
+// 1 / scale.  That product alone is off by up to a unit more, and what lies half way between two
+// 8-bit values goes to the wrong one.  (448 scale is the largest |x|, and scale 2^-109 and more: only
+// quotients next to zero have a remainder that is not exact.)  Zeros keep their sign; with an
+// infinite scale the finite are zero and the infinite NaN.
+struct Quotient {
+  float scale, by;
+  __device__ __forceinline__ explicit Quotient(float s) : scale(s < __builtin_inff() ? s : 1.f), by(1.f / s) {}
+  __device__ __forceinline__ float operator()(float x) const {
+    const float q = x * by;
+    return copysignf(fmaf(fmaf(-q, scale, x), by, q), x);
+  }
+};
+
 // kVec entries of out in 8 bits.
 template <int V>
 __device__ __forceinline__ void store_run8(char* row, int e0, int d, const float* f) {
@@ -278,9 +292,9 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * kWave) void add_norm_forward(A
           constexpr int kLanes = kRun8 / V;  // lanes of a run: consecutive runs of 16 bytes
           top = lanes_max<kLanes>(top);
           const float scale = top < kLeast8 ? 1.f : top / kMost8;
-          const float by = 1.f / scale;
+          const Quotient of(scale);
 #pragma unroll
-          for (int e = 0; e < V; ++e) p[e] *= by;
+          for (int e = 0; e < V; ++e) p[e] = of(p[e]);
           store_run8<V>(a.out + row * a.d, e0, a.d, p);
           if (at % kLanes == 0 && e0 < a.d) a.scales[row * a.runs + e0 / kRun8] = scale;
         }
@@ -289,14 +303,14 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * kWave) void add_norm_forward(A
     if constexpr (kOut == kRowScale) {
       most = over_row<NW>(most, parts, slot, max_f);
       const float scale = most < kLeast8 ? 1.f : most / kMost8;
-      const float by = 1.f / scale;
+      const Quotient of(scale);
 #pragma unroll
       for (int i = 0; i < S; ++i) {
         float p[V], f[V];
         unpack16<DT>(h[i], p);
         w.get(i, f);
 #pragma unroll
-        for (int e = 0; e < V; ++e) p[e] = now ? p[e] * rstd * f[e] * by : 0.f;
+        for (int e = 0; e < V; ++e) p[e] = now ? of(p[e] * rstd * f[e]) : 0.f;
         store_run8<V>(a.out + row * a.d, (at + i * kStep) * V, a.d, p);
       }
       if (at == 0) a.scales[row] = scale;
