@@ -507,22 +507,26 @@ __global__ __launch_bounds__(kThreads, DT != DA_F32 && DP == 64 ? 2 : 1) void di
 }
 
 // ---------------------------------------------------------------------------
-// dq: four waves of 32 rows over their keys.  In 16 bits, where these are few, twice: a first time
-// for the sums that delta comes from.  Of few keys each counts for much, and dq's error was twice
-// its rounding with two of them; of many it is hidden behind theirs.  (64 x 200 tokens of 16 heads
-// on 4: both passes 181 us with one, 240 with two.)  Fewer keys than two splits have: one split
-// knows the whole sum.
+// dq: four waves of 32 rows over their keys.  In 16 bits, where a workgroup's rows see few of them,
+// twice: a first time for the sums that delta comes from.  Of few keys each counts for much: dq's
+// error was twice its rounding, and of a row's only key, whose score has no gradient, all there
+// was.  Of many it is hidden behind theirs.  (64 x 200 tokens of 16 heads on 4: both passes 181 us
+// with one, 240 with two.)  The whole sum is known where all the keys lie in one split.
+constexpr int kFewKeys = 256;
 // ---------------------------------------------------------------------------
 template <int DT, int DP, int DVP>
 struct RowSmem {
   static constexpr int kK = Tile<DT, DP, kThreads>::kBytes, kV = Tile<DT, DVP, kThreads>::kBytes;
   static constexpr int kStage = 2 * kK + kV;
-  static constexpr int kBytes = 2 * kStage;
+  // A lane's largest scores and logarithms apart: few tiles want them, and a spilled register's
+  // load waits for the tiles under way.
+  static constexpr int kFarAt = 2 * kStage;
+  static constexpr int kBytes = kFarAt + kThreads * 16;
 };
 
 // Two waves a SIMD where the operands of 64-wide maps leave room for them (128-wide ones spill:
 // 2 x 2048 tokens of 16 heads, 128 and 128 wide, both passes 670 us with two, 431 with one).
-template <int DT, int DP, int DVP, bool kTwice>
+template <int DT, int DP, int DVP>
 __global__ __launch_bounds__(kThreads, DT != DA_F32 && DP == 64 ? 2 : 1) void diff_grad_rows(Args a) {
   using L = RowSmem<DT, DP, DVP>;
   constexpr int ES = Type<DT>::ES, V = Type<DT>::V;
@@ -557,6 +561,30 @@ __global__ __launch_bounds__(kThreads, DT != DA_F32 && DP == 64 ? 2 : 1) void di
     end = (int)max((int64_t)0, min((int64_t)a.S, t_last + a.q_start + 1));
   }
   int key = split * a.each;
+  // Whether the keys up to `end` are few, and all of them in this split: the same in all waves.
+  bool few = false;
+  if constexpr (DT != DA_F32) {
+    if (a.mask) {
+      int live = 0, here = 0;
+      for (int k = 0; k < end && live <= kFewKeys; k += 4 * kWave) {
+        int byte[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int at = k + i * kWave + lane;
+          byte[i] = at < end ? a.mask[b * a.m_b + at * a.m_k] : 0;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int at = k + i * kWave + lane - key;
+          live += __popcll(__ballot(byte[i] != 0));
+          here += __popcll(__ballot(byte[i] != 0 && at >= 0 && at < a.each));
+        }
+      }
+      few = live <= kFewKeys && here == live;
+    } else {
+      few = end <= kFewKeys && key == 0 && end <= a.each;
+    }
+  }
   end = min(end, key + a.each);
   const bool in = last >= 0;
   u32x4 q[2][KD], g[KV];
@@ -570,16 +598,17 @@ __global__ __launch_bounds__(kThreads, DT != DA_F32 && DP == 64 ? 2 : 1) void di
   for (int kk = 0; kk < KV; ++kk)
     g[kk] = in ? load_run<DT>(a.g + (b * a.g_b + t * a.g_t + h * a.g_h) * ES, (2 * kk + half) * V, a.Dv)
                : u32x4{0, 0, 0, 0};
-  // The second map's factor comes with its exponential, the sign with its values' gradient.
-  const float lam = in ? lam_of(a, h) : 0.f, sign = lam < 0.f ? 1.f : -1.f;
+  // The second map's size of its factor comes with its exponential, the sign at the end.
+  const float lam = in ? lam_of(a, h) : 0.f;
   const float lse1 = in ? a.lse[base + rows] - log2f(fabsf(lam)) : __builtin_inff();
   const int64_t tops = tops_at(a) + base;
   const float top0 = in ? a.lse[tops] : 0.f, top1 = in ? a.lse[tops + rows] : 0.f;
-  float de0 = in ? a.delta[base] : 0.f, de1 = in ? -sign * a.delta[base + rows] : 0.f;
+  float de0 = in ? a.delta[base] : 0.f, de1 = in ? a.delta[base + rows] : 0.f;
   const float c = a.scale * kLog2e, small = small_scale<DT>(a, b, hk);
   // Large scores: the difference from the largest first.
   const bool far = DT == DA_F32 || __any(!near(top0, top1, c));
   const float whole0 = fmaf(top0, c, lse0), whole1 = fmaf(top1, c, lse1);
+  *(f32x4*)(lds + L::kFarAt + threadIdx.x * 16) = f32x4{top0, top1, lse0, lse1};
 
   const Keys<DT, DP, kThreads> keys(a.k_t, a.D);
   const Keys<DT, DVP, kThreads> values(a.v_t, a.Dv);
@@ -598,7 +627,7 @@ __global__ __launch_bounds__(kThreads, DT != DA_F32 && DP == 64 ? 2 : 1) void di
   const int start = key;
   Live live(a, b, key, end, lane);
   if (live.word) fetch(live.key, 0, live.word);
-  bool sums_only = kTwice;
+  bool sums_only = few;
   const Reader<DT, DP> key_reader(lds, lane);
   const Reader<DT, DVP> value_reader(lds + 2 * L::kK, lane);
   const auto step = [&](auto of) __attribute__((always_inline)) {
@@ -623,8 +652,9 @@ __global__ __launch_bounds__(kThreads, DT != DA_F32 && DP == 64 ? 2 : 1) void di
     const bool some = word != ~0u || key + kTile - 1 > least;
     const uint32_t seen = some ? seen_of(word, key, last, half) : ~0u;
     if (far) {
+      const f32x4 x = __builtin_bit_cast(f32x4, lds16(lds_address(lds) + L::kFarAt + threadIdx.x * 16));
 #pragma unroll
-      for (int i = 0; i < 16; ++i) s0[i] = fmaf(s0[i] - top0, c, -lse0), s1[i] = fmaf(s1[i] - top1, c, -lse1);
+      for (int i = 0; i < 16; ++i) s0[i] = fmaf(s0[i] - x[0], c, -x[2]), s1[i] = fmaf(s1[i] - x[1], c, -x[3]);
     } else {
 #pragma unroll
       for (int i = 0; i < 16; ++i) s0[i] = fmaf(s0[i], c, -whole0), s1[i] = fmaf(s1[i], c, -whole1);
@@ -639,41 +669,41 @@ __global__ __launch_bounds__(kThreads, DT != DA_F32 && DP == 64 ? 2 : 1) void di
         p1 = seen & 1u << acc_at(i, 0) ? p1 : 0.f;
       }
       s0[i] = p0 * (dp[i] - de0);
-      s1[i] = p1 * fmaf(dp[i], sign, de1);
+      s1[i] = p1 * (de1 - dp[i]);
       if constexpr (DT != DA_F32) off0 += s0[i], off1 += s1[i];
     }
-    if (kTwice && sums_only) return;
+    if (DT != DA_F32 && sums_only) return;
 #pragma unroll
     for (int j = 0; j < KC; ++j) {
-      const u32x4 y0 = from_acc<DT>(s0, j), y1 = from_acc<DT>(s1, j);
-      u32x4 rest0, rest1;
-      if constexpr (DT != DA_F32) rest0 = rest_of<DT>(s0, j, y0), rest1 = rest_of<DT>(s1, j, y1);
+      // A map after the other: both at once would spill.
+      const auto add = [&](const f32x16& x, int at, f32x16 (&to)[ND]) __attribute__((always_inline)) {
+        const u32x4 y = from_acc<DT>(x, j);
+        u32x4 rest;
+        if constexpr (DT != DA_F32) rest = rest_of<DT>(x, j, y);
 #pragma unroll
-      for (int n = 0; n < ND; ++n) {
-        const u32x4 k0 = lk.columns(skip, n, j), k1 = lk.columns(skip + L::kK, n, j);
-        Mfma32<DT>::mma(dq[0][n], k0, y0);
-        Mfma32<DT>::mma(dq[1][n], k1, y1);
-        if constexpr (DT != DA_F32) {
-          Mfma32<DT>::mma(dq[0][n], k0, rest0);
-          Mfma32<DT>::mma(dq[1][n], k1, rest1);
+        for (int n = 0; n < ND; ++n) {
+          const u32x4 k = lk.columns(at, n, j);
+          Mfma32<DT>::mma(to[n], k, y);
+          if constexpr (DT != DA_F32) Mfma32<DT>::mma(to[n], k, rest);
         }
-      }
+      };
+      add(s0, skip, dq[0]);
+      add(s1, skip + L::kK, dq[1]);
     }
   };
   // A factor so small that its map's entries vanish tells nothing of delta.
-  const float to_off0 = 1.f / small, to_off1 = fabsf(lam) > 0x1p-60f ? 1.f / (sign * fabsf(lam) * small) : 0.f;
-  float known0 = 0.f, known1 = 0.f;
+  const float size = fabsf(lam), to_off0 = 1.f / small, to_off1 = size > 0x1p-60f ? -1.f / (size * small) : 0.f;
   for (;;) {
     while (live.word) {
       step(std::integral_constant<int, 0>{});
       if (live.word) step(std::integral_constant<int, 1>{});
     }
-    off0 = known0 + (off0 + other_half(off0)) * to_off0;
-    off1 = known1 + (off1 + other_half(off1)) * to_off1;
-    if (!kTwice || !sums_only) break;
+    if constexpr (DT == DA_F32) break;
+    off0 = (off0 + other_half(off0)) * to_off0;
+    off1 = (off1 + other_half(off1)) * to_off1;
+    if (!sums_only) break;
     sums_only = false;
-    known0 = off0, known1 = off1;
-    de0 += known0, de1 -= sign * known1;
+    de0 += off0, de1 += off1;
     off0 = off1 = 0.f;
     __syncthreads();  // the tiles have been read
     live = Live(a, b, start, end, lane);
@@ -682,10 +712,11 @@ __global__ __launch_bounds__(kThreads, DT != DA_F32 && DP == 64 ? 2 : 1) void di
   if (r >= rows) return;
   if (DT != DA_F32 && half == 0) {
     float* to = a.off + (int64_t)split * a.batch * a.Hk * 2 * rows + base;
+    if (few && in) off0 += de0 - a.delta[base], off1 += de1 - a.delta[base + rows];
     to[0] = off0;
     to[rows] = off1;
   }
-  const float by = a.scale / small;
+  const float by = a.scale / small, by_map[2] = {by, lam < 0.f ? -by : by};
   const int64_t to = ((int64_t)b * a.T + t) * (a.Hk * a.G) + h;
 #pragma unroll
   for (int m = 0; m < 2; ++m)
@@ -694,7 +725,7 @@ __global__ __launch_bounds__(kThreads, DT != DA_F32 && DP == 64 ? 2 : 1) void di
 #pragma unroll
       for (int i = 0; i < 16; i += 4) {
         const int e = 32 * n + acc_at(i, half);
-        const f32x4 x = f32x4{dq[m][n][i], dq[m][n][i + 1], dq[m][n][i + 2], dq[m][n][i + 3]} * by;
+        const f32x4 x = f32x4{dq[m][n][i], dq[m][n][i + 1], dq[m][n][i + 2], dq[m][n][i + 3]} * by_map[m];
         if (a.splits == 1)
           store4<DT>(a.dq + (2 * to + m) * a.D * ES, e, a.D, x[0], x[1], x[2], x[3]);
         else if (e < a.D)
@@ -847,8 +878,7 @@ int da_diff_attention_grad(const da_diff_inputs* in, const void* g, int64_t g_bs
     constexpr int DT = decltype(dt)::value, DP = decltype(dp)::value, DVP = decltype(dvp)::value;
     if (rows) {
       constexpr int kBytes = RowSmem<DT, DP, DVP>::kBytes;
-      const auto kernel = DT != DA_F32 && k_len < 2 * kLeastSplit ? diff_grad_rows<DT, DP, DVP, DT != DA_F32>
-                                                                  : diff_grad_rows<DT, DP, DVP, false>;
+      const auto kernel = diff_grad_rows<DT, DP, DVP>;
       if (const int err = allow_lds((const void*)kernel, kBytes)) return err;
       a.blocks = p.rows.blocks, a.splits = p.rows.splits, a.each = p.rows.each;
       kernel<<<(unsigned)(pairs * a.blocks * a.splits), kThreads, kBytes, st>>>(a);

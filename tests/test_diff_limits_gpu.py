@@ -303,3 +303,58 @@ def test_one_large_score_above_many_small_ones(dt, t, below):
     least = 1.25 * s * 2.0**-35 if dt == "fp16" else 0.0
     off = want * (u + 1.25 / 0.75 * (u + (s / 32 + 64) * U32)) + least + 2.0**-25
     assert ((got - want).abs() <= off).all(), got.flatten()[0].item() / want
+
+
+# ---------------------------------------------------------------------------
+# Rows that see few keys
+# ---------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp16"])
+@pytest.mark.parametrize("s", [40, 255, 256, 257, 1024])
+@pytest.mark.parametrize("kind", ["causal", "mask", "late", "both"])
+def test_the_only_key_of_a_row_has_no_score_gradient(dt, s, kind):
+    """One key: its probability is 1 whatever the score is.  What is left of its gradient is fp32's,
+    c terms of |g| |v| (dp and delta as sums of 64), and not the rounding of out in 16 bits."""
+    b, t, h, hk, d, dv = 3, s, 4, 2, 64, 64
+    q, k, v, lam, g = operands(stable_seed((s, kind)), b, t, s, h, hk, d, dv, DT[dt])
+    kw, rows, key = {}, slice(0, 1), 0
+    if kind in ("causal", "both"):
+        kw["causal"] = True
+    if kind != "causal":  # one live key in the first sample, all in the second, none in the third
+        key = {"mask": s // 2, "late": s - 1, "both": 0}[kind]
+        mask = torch.zeros(b, s, dtype=torch.bool, device="cuda")
+        mask[0, key] = mask[1] = True
+        kw["mask"] = mask
+        rows = slice(0, t)
+    _, dq, dk, _, dlam = run(q, k, v, lam, g, **kw)
+    size = g[0, rows].double().abs().sum(-1).amax() * v[0, key].double().abs().amax()
+    off = 128 * U32 * size * k[0, key].double().abs().amax() * d ** -0.5
+    tiny = 2.0**-24 if dt == "fp16" else 0.0
+    assert dq[0, rows].double().abs().max() <= off + tiny, (dq[0, rows].double().abs().max() / off).item()
+    if kind != "causal":
+        n = h // hk * t  # rows that add to the key's gradient
+        assert dk[0, key].double().abs().max() <= n * 128 * U32 * size * q[0].double().abs().amax() * d ** -0.5 + tiny
+        want = -(g[0].double() * v[0, key].double().repeat_interleave(h // hk, 0)).sum((0, 2))
+        assert ((dlam[0] - want).abs() <= (t + 128) * U32 * t * size).all()
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp16"])
+@pytest.mark.parametrize("t,s,live", [(255, 255, 255), (300, 300, 40), (90, 1024, 200), (1024, 1024, 256), (2, 3000, 100)])
+@pytest.mark.parametrize("causal", [False, True])
+def test_score_gradients_of_few_keys(dt, t, s, live, causal):
+    """dq from two 16-bit parts of ds and a repaired delta is off by its own rounding and little
+    else: less than 1.15 times it in norm, where an unrepaired delta leaves 1.3 and more."""
+    b, h, hk, d, dv = 2, 4, 2, 64, 64
+    q, k, v, lam, g = operands(stable_seed((t, s)), b, t, s, h, hk, d, dv, DT[dt])
+    mask = torch.arange(s, device="cuda")[None] < torch.tensor([[live], [s]], device="cuda")
+    q_start = live - t if causal else None  # the last row sees what is live
+    seen = mask[:, None].expand(b, t, s)
+    if causal:
+        seen = seen & (torch.arange(s, device="cuda") <= torch.arange(t, device="cuda")[:, None] + q_start)
+    rows = seen[0].any(-1)
+    some = seen | ~seen.any(-1, keepdim=True)  # rows without keys have no maps in 64 bits
+    want = exact(q, k, v, lam, g.masked_fill(~seen.any(-1)[..., None, None], 0), seen=some)[0][1][0, rows]
+    got = run(q, k, v, lam, g, mask=mask, causal=causal, q_start=q_start)[1][0, rows].double()
+    rounding = (want.to(DT[dt]).double() - want).norm()
+    assert (got - want).norm() < 1.15 * rounding, ((got - want).norm() / rounding).item()
