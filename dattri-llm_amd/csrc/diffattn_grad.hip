@@ -107,8 +107,7 @@ __global__ __launch_bounds__(256) void diff_delta(Args a) {
   const int chunk = blockIdx.x % a.chunks;
   const int h = blockIdx.x / a.chunks % heads, b = blockIdx.x / a.chunks / heads;
   const int hk = h / a.G, rows = a.T * a.G;
-  const float lam = lam_of(a, h), c = a.scale * kLog2e;
-  const float* tops = a.lse + tops_at(a);
+  const float lam = lam_of(a, h);
   const int t1 = min((chunk + 1) * a.chunk, a.T);
   float most = 0.f;
   for (int t = chunk * a.chunk + sub; t < t1; t += kRows) {
@@ -140,8 +139,6 @@ __global__ __launch_bounds__(256) void diff_delta(Args a) {
       float* to = a.delta + of * 2 * rows + r;
       to[0] = d0 + lam * d1;  // o_1 = out + lam o_2
       to[rows] = d1;
-      const int64_t at = of * 2 * rows + r;
-      a.takes_part[of * rows + r] = live ? near(tops[at], tops[at + rows], c) ? 1 : 3 : 0;
     }
   }
   if constexpr (DT == DA_F16) {  // a maximum: the order does not matter
@@ -195,8 +192,10 @@ __global__ __launch_bounds__(256) void diff_records(Args a) {
     if constexpr (DT != DA_F32)
       for (int p = 0; p < a.row_splits; ++p) d0 += a.off[p * all + at], d1 += a.off[p * all + at + rows];
     const float* tops = a.lse + tops_at(a) + at;
-    put_record<DT>(a.records + (of * rows + r) * Record<DT>::kBytes, c, tops[0], tops[rows], a.lse[at],
-                   a.lse[at + rows] - bits, d0, d1);
+    const float lse0 = a.lse[at];
+    put_record<DT>(a.records + (of * rows + r) * Record<DT>::kBytes, c, tops[0], tops[rows], lse0, a.lse[at + rows] - bits,
+                   d0, d1);
+    a.takes_part[of * rows + r] = lse0 == __builtin_inff() ? 0 : near(tops[0], tops[rows], c) ? 1 : 3;
     sum += d1;
   }
   sum = lanes_sum<kWave>(sum);
