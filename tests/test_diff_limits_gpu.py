@@ -358,3 +358,59 @@ def test_score_gradients_of_few_keys(dt, t, s, live, causal):
     got = run(q, k, v, lam, g, mask=mask, causal=causal, q_start=q_start)[1][0, rows].double()
     rounding = (want.to(DT[dt]).double() - want).norm()
     assert (got - want).norm() < 1.15 * rounding, ((got - want).norm() / rounding).item()
+
+
+# ---------------------------------------------------------------------------
+# Errors as a whole, and every CU busy
+# ---------------------------------------------------------------------------
+
+
+def error(got, want):
+    """In units of what rounding the exact result to the output's type leaves."""
+    return ((got.double() - want).norm() / (want.to(got.dtype).double() - want).norm()).item()
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp16"])
+@pytest.mark.parametrize("t,s,fine", [(1, 90, True), (1, 5000, True), (5, 700, True), (100, 512, True), (100, 513, False),
+                                      (700, 700, False)])
+def test_outputs_are_rounded_once_where_keys_or_rows_are_few(dt, t, s, fine):
+    """With probabilities in two parts little but the output's rounding is left.  Else theirs comes
+    to it, as large where values have random signs: sqrt 2 of it together, in bf16 (whose steps
+    are as coarse in both)."""
+    q, k, v, lam, g = operands(stable_seed((t, s)), 2, t, s, 4, 2, 64, 64, DT[dt])
+    want = exact(q, k, v, lam, g)[0][0]
+    got = error(ops.diff_attention(q, k, v, lam), want)
+    assert got < (1.1 if fine else 1.6), got
+
+
+@pytest.mark.parametrize("masked", [False, True])
+def test_every_cu_busy_against_64_bits(masked):
+    """4 x 2048 causal tokens, 32 heads on 8: samples' and key heads' results at full load.  Errors in
+    units of the outputs' rounding, as the roundings on the way add up to them: out and dv have
+    that of the maps, dk of the score gradients, dq none but delta's."""
+    b, t, h, hk, d, dv = 4, 2048, 32, 8, 64, 128
+    q, k, v, lam, g = operands(53, b, t, t, h, hk, d, dv, torch.bfloat16)
+    mask = torch.arange(t, device="cuda")[None] < torch.tensor([[2048], [1900], [300], [2047]], device="cuda") if masked else None
+    got = run(q, k, v, lam, g, causal=True, mask=mask, q_mask=mask)
+    group = h // hk
+    for i, j in ((0, 0), (1, 3), (2, 6), (3, 7)):
+        n = t if mask is None else int(mask[i].sum())
+        heads, maps, key_maps = slice(j * group, (j + 1) * group), slice(2 * j * group, 2 * (j + 1) * group), slice(2 * j, 2 * j + 2)
+        one = (q[i:i + 1, :n, maps], k[i:i + 1, :n, key_maps], v[i:i + 1, :n, j:j + 1], lam[heads], g[i:i + 1, :n, heads])
+        want, _ = exact(*one, seen=torch.ones(1, n, n, dtype=torch.bool, device="cuda").tril())
+        mine = (got[0][i:i + 1, :n, heads], got[1][i:i + 1, :n, maps], got[2][i:i + 1, :n, key_maps],
+                got[3][i:i + 1, :n, j:j + 1])
+        for name, x, y, most in zip(NAMES, mine, want, (1.6, 1.4, 1.6, 1.6)):
+            assert error(x, y) < most, (i, j, name, error(x, y))
+        # fp32 sums of 2^18 terms; delta from fp32 score gradients
+        assert bool(((got[4][i, heads] - want[4][0]).abs() <= 1e-4 * want[4].abs().max()).all())
+        for x in got[:4]:
+            assert not bool(x[i, n:].any())
+
+
+def test_a_state_of_other_inputs_is_refused():
+    q, k, v, lam, g = operands(59, 2, 5, 7, 4, 2, 32, 32, torch.float32)
+    out, state = ops.diff_attention(q, k, v, lam, return_state=True)
+    for lse in (state.lse[0], state.lse[:, :1], state.lse.double(), state.lse.transpose(1, 2)[:, :, :1]):
+        with pytest.raises(ValueError, match="state"):
+            ops.diff_attention_grad(g, q, k, v, lam, out, state._replace(lse=lse))
