@@ -4,7 +4,7 @@
 // nothing to a gradient):
 //
 //   total = round(x + residual),   r = (mean(total^2) + eps)^(-1/2)
-//   out_i = total_i r w_i
+//   out_i = total_i w_i r
 //
 // The norm is that of total as it is returned, so that the backward pass, which has
 // only total, differentiates the same function.  In 8 bits (e4m3) out is divided by a
@@ -20,7 +20,9 @@
 // a second launch joins a sample's chunks in order.
 //
 // Everything between the loads and a result is in fp32 and rounded once: total, then out from
-// total as rounded; dx; out in 8 bits from its fp32 value, not from a rounded one.
+// total as rounded; dx; out in 8 bits from its fp32 value, not from a rounded one.  out is (total w)
+// r: a product of two 16-bit values is exact in fp32, which leaves one rounding (8-bit values on the
+// wrong side of a border: an error of 8.0e-4 in place of 8.9e-4 for (total r) w at the size below).
 //
 // HBM bounds both.  8 x 2048 rows of 4096 in bf16: 94 us forward (537 MB, 5.7 TB/s), 74 with
 // out in 8 bits (470 MB, 6.4 TB/s), 101 backward (537 MB, 5.3 TB/s).
@@ -279,7 +281,7 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * kWave) void add_norm_forward(A
       unpack16<DT>(h[i], p);
       w.get(i, f);
 #pragma unroll
-      for (int e = 0; e < V; ++e) p[e] = now ? p[e] * rstd * f[e] : 0.f;
+      for (int e = 0; e < V; ++e) p[e] = now ? p[e] * f[e] * rstd : 0.f;
       if constexpr (kOut == kPlain) {
         store_run<DT, kStream>(a.out + row * a.d * ES, e0, a.d, pack16<DT>(p));
       } else {
@@ -310,7 +312,7 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * kWave) void add_norm_forward(A
         unpack16<DT>(h[i], p);
         w.get(i, f);
 #pragma unroll
-        for (int e = 0; e < V; ++e) p[e] = now ? of(p[e] * rstd * f[e]) : 0.f;
+        for (int e = 0; e < V; ++e) p[e] = now ? of(p[e] * f[e] * rstd) : 0.f;
         store_run8<V>(a.out + row * a.d, (at + i * kStep) * V, a.d, p);
       }
       if (at == 0) a.scales[row] = scale;
