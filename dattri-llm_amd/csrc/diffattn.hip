@@ -10,15 +10,16 @@
 // keys each) and its maximum and sum stay within them; the accumulator's registers then are,
 // rounded, the second operand of o^T = v^T p^T as they stand, where v is read transposed out
 // of LDS.  A difference of scores is formed before it is scaled where they are large (kNear), so
-// that any finite scores have finite exponentials.  These are relative to a maximum that is looked for again only when the sum
-// of a lane's sixteen passes 2^10 (fp16: 2^15, the largest being 2^10): until then they are at
-// most that much larger than with the last one (the first tile has none, and passes; with a new one in every tile that has a larger
-// score 277 us in place of 257 at the first size below).  At the end the second map's waves hand
-// their values, divided and weighted, to the first's through LDS.
+// that any finite scores have finite exponentials.  These are relative to a maximum that is looked
+// for again only when the sum of a lane's sixteen passes 2^10 (fp16: 2^15, the largest being 2^10):
+// until then they are at most that much larger than with the last one (the first tile has none, and
+// passes; with a new one in every tile that has a larger score a twelfth more time at the first size
+// below).  At the end the second map's waves hand their values, divided and weighted, to the first's
+// through LDS.
 //
-// 4 x 2048 causal tokens in bf16: 32 heads on 8, two 64-wide maps and 128-wide values 257 us
-// (206 GFLOP, 800 TFLOP/s), 16 heads of 128 and 256 261 us (790 TFLOP/s): vector and matrix unit
-// nearly in sum.  16 new tokens of 32 heads on 8 against 8192 positions 94 + 11 us, HBM at 4.8 TB/s.
+// 4 x 2048 causal tokens in bf16: 32 heads on 8, two 64-wide maps and 128-wide values 260 us
+// (206 GFLOP, 790 TFLOP/s), 16 heads of 128 and 256 267 us (770 TFLOP/s): vector and matrix unit
+// nearly in sum.  16 new tokens of 32 heads on 8 against 8192 positions 94 + 12 us, HBM at 4.8 TB/s.
 #include <algorithm>
 #include <type_traits>
 
@@ -82,9 +83,11 @@ struct Smem {
 
 // kFine: probabilities as the sum of two 16-bit values, so that values are rounded once, at the
 // end (bf16 error 1.7e-3).  Where a token's few rows leave the matrix units idle that costs
-// nothing, and with few keys little (2 x 472 tokens of 15 heads 53 us in place of 51, 16 x 512 of 32
-// on 8 135 and 116; 4 x 2048 would pay two thirds more products).  Else they are rounded where they are multiplied, by half a step each, no more than
-// the output's own rounding (2.4e-3 together); sums stay in fp32.
+// nothing; else the products with v double.  With up to kFewKeys keys, where each counts for more, that
+// is at most a fifth of the time (32 heads on 8 of 64 and 128: 16 x 256 tokens 49 us and 43 without,
+// 16 x 512 120 and 99), past it more (8 x 768 118 and 93, 8 x 1024 186 and 140, 4 x 2048 332 and 242):
+// there they are rounded where they are multiplied, by half a step each, no more than the output's
+// own rounding (2.4e-3 together).  Sums stay in fp32.
 // Two waves a SIMD but for the widest maps in fp32, which would spill (8 heads of 2 x 512 tokens
 // 203 us in place of 141) and whose tiles leave LDS for one workgroup anyway.
 template <int DT, int DP, int DVP, int NG, bool kFine>

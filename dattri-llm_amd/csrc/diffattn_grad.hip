@@ -1,15 +1,17 @@
 // Attention by the difference of two softmax maps, backward.
 //
-// With p_m the maps (from the scores, and the forward call's largest ones and sums), g the gradient of out:
+// With p_m the maps (from the scores, and the forward call's largest ones and sums), g the
+// gradient of out:
 //
 //   dp = g v^T,   delta_m = g . o_m
 //   ds_1 = p_1 (dp - delta_1),   ds_2 = -lam p_2 (dp - delta_2)
 //   dq_m = scale ds_m k_m,   dk_m = scale ds_m^T q_m,   dv = (p_1 - lam p_2)^T g
 //   dlam[sample] = -sum of delta_2
 //
-// Four launches and no atomic sums, so that results do not change from run to run: delta; dq, a
-// wave holding 32 rows and going over their keys; the records of rows and dlam's parts; dk and
-// dv, a wave holding 32 keys and going over all rows of their heads.  The scores are formed
+// No atomic sums, so that results do not change from run to run, and five launches: delta; dq, a
+// wave holding 32 rows and going over their keys; the records of rows and dlam's parts; these
+// joined; dk and dv, a wave holding 32 keys and going over all rows of their heads.  Either large
+// pass has a join more where it is split, and fp16 two launches for the sizes of g and v.  The scores are formed
 // twice, the price of sums that are nobody else's.  Where keys are columns, the scores'
 // registers are rows and stand as the operand that is contracted over rows; where rows are
 // columns, they are keys: neither pass moves a score between lanes.
@@ -18,16 +20,17 @@
 // of each entry, no more than the outputs' own rounding; and out and o_2, from which delta
 // comes, off by as much for a whole row.  dq therefore takes ds as the sum of two 16-bit
 // values (with one, its error was 1.6 times that of its rounding; it costs 79 of 800 us at the
-// size below), and its pass sums ds in fp32: sum ds_m = delta_m - its first value, as the maps
-// sum to one.  The pass of dk and dv and dlam have delta from there.
+// size below), and its pass sums ds in fp32: the sum of ds_m is how far delta_m was off, as the
+// maps sum to one.  The pass of dk and dv and dlam have delta from there, and so has dq where a
+// row sees few keys (kFewKeys).
 //
 // fp16 would lose small values of ds: there ds is scaled by the power of two that brings the
 // bound of the largest to 2^14, and the maps' mixture by one that its factors allow; their products
-// are scaled back.  Each sample's key heads have a bound of
-// their own: what a sample gets does not depend on the others in its batch.
+// are scaled back.  Each sample's key heads have a bound of their own: what a sample gets does not
+// depend on the others in its batch.
 //
-// 4 x 2048 tokens, 32 heads on 8, two 64-wide maps, 128-wide values, causal, bf16: delta 35 us,
-// dq 350 us and dk, dv 440 us of 275 GFLOP each (790 and 620 TFLOP/s), records 10 us.  Both large
+// 4 x 2048 tokens, 32 heads on 8, two 64-wide maps, 128-wide values, causal, bf16: delta 36 us,
+// dq 355 us and dk, dv 437 us of 275 GFLOP each (770 and 630 TFLOP/s), records 11 us.  Both large
 // passes are bound by the vector unit (two exponentials and some twenty instructions an entry of
 // the maps) and the matrix unit nearly in sum: with the registers of two waves a SIMD there is
 // little to put under the other one's work.  dk and dv wait for the first keys' workgroups besides,

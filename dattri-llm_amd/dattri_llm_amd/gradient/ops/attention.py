@@ -214,8 +214,9 @@ def diff_attention(q, k, v, lam, *, scale: float | None = None, causal: bool = F
 
     ``return_state``: ``(out, state)`` for :func:`diff_attention_grad`; not
     differentiable.  ``slot`` takes ``lam``'s per-sample gradient ``(B, H)`` in the
-    backward pass, in place of its summed one (``FusedCapture``).  In 16 bits that
-    gradient carries the rounding of the maps' values."""
+    backward pass, in place of its summed one (``FusedCapture``).  It is formed from
+    the maps in 32 bits (in 16 bits that of a factor below 2^-60 from the second map's
+    rounded values)."""
     if getattr(forward_ad, "_current_level", 0) >= 0:
         kernels.refuse_tangents("diff_attention", q, k, v, lam)
     cfg = {"scale": scale, "causal": causal, "q_start": q_start}

@@ -6,7 +6,8 @@ over logits whose tokens stay apart.  :func:`token_logprobs` gives them with the
 entropy and the most likely alternatives in one pass over the logits, and is
 differentiable; :func:`token_logprobs_grad` is the same backward pass as a plain
 call, which can be captured into a HIP graph.  Second and forward-mode
-derivatives are refused.  Sums are held in 32 bits.
+derivatives are refused.  Sums are held in 32 bits, of differences from a row's
+largest logit: a common offset or a small temperature costs no accuracy.
 """
 
 from __future__ import annotations
@@ -64,8 +65,9 @@ def token_logprobs(logits, targets, *, mask=None, temperature: float = 1.0, top:
     ``mask`` in the same shape: a token with a zero gets zeros (indices -1),
     whatever its logits hold, and takes no part in any gradient.  ``top``: how
     many of the most likely tokens (at most 32) to return; of equal logits the
-    lower index comes first.  A logit of ``-inf`` has no probability; a row with
-    NaN gives NaN."""
+    lower index comes first.  A logit of ``-inf`` (or of its type's lowest value
+    beside others) has no probability; a row with NaN gives NaN.  ``temperature``
+    lies between 1e-30 and 8e37."""
     if getattr(forward_ad, "_current_level", 0) >= 0:
         kernels.refuse_tangents("token_logprobs", logits)
     if torch.is_grad_enabled() and logits.requires_grad:
