@@ -11,9 +11,9 @@
 // No atomic sums, so that results do not change from run to run, and five launches: delta; dq, a
 // wave holding 32 rows and going over their keys; the records of rows and dlam's parts; these
 // joined; dk and dv, a wave holding 32 keys and going over all rows of their heads.  Either large
-// pass has a join more where it is split, and fp16 two launches for the sizes of g and v.  The scores are formed
-// twice, the price of sums that are nobody else's.  Where keys are columns, the scores'
-// registers are rows and stand as the operand that is contracted over rows; where rows are
+// pass has a join more where it is split, and fp16 two launches for the sizes of g and v.  The
+// scores are formed twice, the price of sums that are nobody else's.  Where keys are columns, the
+// scores' registers are rows and stand as the operand that is contracted over rows; where rows are
 // columns, they are keys: neither pass moves a score between lanes.
 //
 // What is rounded to 16 bits: ds and the maps' mixture where they are operands, by half a step
@@ -45,7 +45,7 @@ namespace diff {
 namespace {
 
 // ---------------------------------------------------------------------------
-// delta, its records, parts of dlam, largest |g|.  Workgroup (b, h, chunk of tokens), 16 lanes
+// delta, its records, parts of dlam, largest |g|: workgroups (b, h, chunk of tokens), 16 lanes
 // a token.
 //
 // Where keys are columns, a row's lse and delta are needed in every lane, by register.  In
@@ -60,8 +60,8 @@ namespace {
 // ---------------------------------------------------------------------------
 constexpr int kLanes = 16;
 constexpr float kNothing = -1e30f;
-// In 16 bits lse + top c as one number is off by less than 2^-14 up to here, no more than a tenth
-// of a step of the maps.
+// In 16 bits lse + top c as one number is off by half a unit of its last place, 2^-15 up to here:
+// no more than a tenth of the half step that the maps are rounded by.
 constexpr float kNear = 1024.f;
 __device__ __forceinline__ bool near(float top0, float top1, float c) {
   return fabsf(top0 * c) < kNear && fabsf(top1 * c) < kNear;
@@ -600,7 +600,7 @@ __global__ __launch_bounds__(kThreads, DT != DA_F32 && DP == 64 ? 2 : 1) void di
   for (int kk = 0; kk < KV; ++kk)
     g[kk] = in ? load_run<DT>(a.g + (b * a.g_b + t * a.g_t + h * a.g_h) * ES, (2 * kk + half) * V, a.Dv)
                : u32x4{0, 0, 0, 0};
-  // The second map's size of its factor comes with its exponential, the sign at the end.
+  // The size of the second map's factor comes with its exponential, the sign at the end.
   const float lam = in ? lam_of(a, h) : 0.f;
   const float lse1 = in ? a.lse[base + rows] - log2f(fabsf(lam)) : __builtin_inff();
   const int64_t tops = tops_at(a) + base;

@@ -21,9 +21,11 @@
 //
 // Logits are read in their type and everything from there on is fp32, differences from the row's
 // maximum; only the gradient is rounded, once.  It takes the row's lse as the forward call returned
-// it, and sums a row again whose lse is large (kFar).  2 x 1024 rows of 128256 in bf16 with five alternatives take 93 us (525 MB,
-// 5.6 TB/s; an exponential and some eight instructions an entry nearly fill the vector unit), 16
-// rows with twenty 10 and 6 us; 4 x 1024 rows forward and backward 539 us (3.15 GB, 5.8 TB/s).
+// it, and sums a row again whose lse is large (kFar).
+//
+// 2 x 1024 rows of 128256 in bf16 with five alternatives take 92 us (525 MB, 5.7 TB/s; an exponential
+// and some eight instructions an entry nearly fill the vector unit), 16 rows with twenty 9 and 6 us;
+// 4 x 1024 rows forward and backward 540 us (3.15 GB, 5.8 TB/s).
 #include <algorithm>
 #include <type_traits>
 
